@@ -239,7 +239,7 @@ def _inputs_logits(c, r):
         start = [sum(count[:i]) for i in range(rows + 1)]
         st.update(bias_start=_i32(start),
                   bias_ids=torch.cat([r.order(vocab)[:n] for n in count]).to(torch.int32),
-                  bias_values=r.uniform(total) * 20 - 10)
+                  bias_values=r.uniform(total, dtype=torch.float64) * 20 - 10)
     if c["masked"]:
         n = max(1, int(c["masked"] * rows))
         # a grammar permits a handful of tokens or most of them
@@ -423,7 +423,7 @@ def _plain_logits(st):
         at = torch.arange(st["bias_ids"].shape[0], device="cuda", dtype=torch.int32)
         row = torch.searchsorted(st["bias_start"], at, right=True) - 1
         bias = torch.zeros(rows, vocab, device="cuda")
-        bias[row, st["bias_ids"].long()] = st["bias_values"]
+        bias[row, st["bias_ids"].long()] = st["bias_values"].float()
         s = s + bias
     allowed = torch.ones_like(x, dtype=torch.bool)
     if st["mask"] is not None:
@@ -521,7 +521,7 @@ def _exact_logits(st):
             - st["frequency"][r] * count
         if st["bias_ids"] is not None:
             lo, hi = st["bias_start"][r:r + 2].tolist()
-            x[r, st["bias_ids"][lo:hi].long()] += st["bias_values"][lo:hi].double()
+            x[r, st["bias_ids"][lo:hi].long()] += st["bias_values"][lo:hi]
         which = -1 if st["mask"] is None else int(st["mask_rows"][r])
         if which >= 0:
             at = torch.arange(x.shape[1], device="cuda")
