@@ -315,7 +315,7 @@ def _own_logits(st):
         st["logits"], history=st["history"], history_len=st["history_len"],
         repetition=st["repetition"], presence=st["presence"], frequency=st["frequency"],
         bias_start=st["bias_start"], bias_ids=st["bias_ids"], bias_values=st["bias_values"],
-        mask=st["mask"], mask_rows=st["mask_rows"])
+        mask=st["mask"], mask_rows=st["mask_rows"], masked=-math.inf)
     return dict(out=out, flags=flags)
 
 
