@@ -200,6 +200,13 @@ int orinfer_attention_prefill(const __half* q, const __half* gate, const int* ch
                               const __half* vscale, __half* out, int qh, int kvh, int head_dim,
                               int num_pages, int context, cudaStream_t stream);
 
+// Single rows whose contexts begin with the same pages (attention_shared.cu).
+int orinfer_attention_shared(const __half* q, const __half* gate, const int* row_req,
+                             const int* row_pos, const int* page_table, int max_pages,
+                             const int8_t* kc, const int8_t* vc, const __half* ks,
+                             const __half* vs, __half* out, int rows, int qh, int kvh,
+                             int head_dim, int num_pages, cudaStream_t stream);
+
 // ---- expert-parallel all-to-alls over peer memory (moe_a2a.cu); cap = owned rows x top_k
 typedef struct OrinferA2aDispatch {
   void* rows[8];               // every rank's receive buffer: int8 [tp][cap][K]
@@ -258,6 +265,36 @@ int orinfer_gdn_gated_norm(const float* o, const __half* z, int z_stride, const 
 int orinfer_sample_topk(const float* logits, int rows, int vocab, long long row_stride,
                         const int* top_k, const double* temperature, const double* top_p,
                         const double* uniform, int* token, int* flag, cudaStream_t stream);
+
+// ---- penalties, biases and masks on logits (logits.cu)
+int orinfer_process_logits(const float* logits, long long row_stride, const int* history,
+                           long long history_stride, int history_cap, const int* history_len,
+                           const double* repetition, const double* presence,
+                           const double* frequency, const int* bias_start, const int* bias_ids,
+                           const double* bias_values, int bias_total, const int* mask,
+                           long long mask_stride, const int* mask_rows, int mask_count,
+                           float masked, float* out, long long out_stride, int* flags, int rows,
+                           int vocab, cudaStream_t stream);
+
+// ---- pages of the cache (pages.cu).  The cache is n tensors [pages, 128, ...]: their addresses,
+// bytes per token, and the units (tensor, first token, tokens) that a page is copied in.
+size_t orinfer_fork_work(int n, int slots);
+size_t orinfer_compact_work(int pages);
+int orinfer_copy_pages(const long long* bases, const int* token_bytes, const int* units,
+                       int n_units, int pages, const int* copies, const int* count, int most,
+                       cudaStream_t stream);
+int orinfer_fork_pages(const long long* bases, const int* token_bytes, const int* units,
+                       int n_units, int pages, const int* table, int* table_out, const int* lens,
+                       int* lens_out, const int* refs, int* refs_out, const int* parents,
+                       const int* children, int n, int slots, int max_pages, int* work,
+                       int* status, cudaStream_t stream);
+int orinfer_free_pages(const int* table, int* table_out, const int* lens, int* lens_out,
+                       const int* refs, int* refs_out, const int* gone, int n, int slots,
+                       int max_pages, int pages, cudaStream_t stream);
+int orinfer_compact_pages(const long long* bases, const int* token_bytes, const int* units,
+                          int n_units, int pages, const int* table, int* table_out,
+                          const int* refs, int* refs_out, int* moved, int slots, int max_pages,
+                          int* work, cudaStream_t stream);
 
 // ---- E8P nearest-codeword encoder: x fp32 [V,8] -> int32 codes [V]
 int orinfer_e8p_encode(const float* x, int* codes, long long vectors, cudaStream_t stream);

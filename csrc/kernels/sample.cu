@@ -1,5 +1,7 @@
 // Device top-k / top-p categorical sampler for rows whose options need no host state
 // (temperature > 0, 1 <= top_k <= 64, no penalties, bias, mask or probability report).
+// Scores of -1e30 and below (what process_logits leaves of tokens that a mask does not permit) are
+// no candidates: a row has at most as many as it has scores above that.
 // One CTA per row:
 //   1. exact radix select (4 passes of 8-bit histograms over order-preserving keys) of the
 //      top_k-th largest logit;
@@ -21,6 +23,7 @@ namespace orinfer {
 constexpr int SAMPLE_THREADS = 1024;
 constexpr int MAX_TOPK = 64;
 constexpr int TIE_CAP = 256;
+constexpr float NO_CANDIDATE = -1e30f;
 
 __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v);
@@ -36,19 +39,20 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_topk_kernel(
   const float* lg = logits + static_cast<long long>(row) * row_stride;
   __shared__ unsigned int hist[256];
   __shared__ uint32_t s_prefix, s_mask;
-  __shared__ int s_need, s_bad;
+  __shared__ int s_need, s_bad, s_candidates;
   __shared__ int n_above, n_tie;
   __shared__ float sl_val[MAX_TOPK];
   __shared__ int sl_id[MAX_TOPK];
   __shared__ int tie_id[TIE_CAP];
   __shared__ float so_val[MAX_TOPK];
   __shared__ int so_id[MAX_TOPK];
-  const int k = min(max(top_k[row], 1), min(MAX_TOPK, vocab));
+  int k = min(max(top_k[row], 1), min(MAX_TOPK, vocab));
   if (tid == 0) {
     s_prefix = 0;
     s_mask = 0;
     s_need = k;
     s_bad = 0;
+    s_candidates = 0;
     n_above = 0;
     n_tie = 0;
   }
@@ -58,15 +62,19 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_topk_kernel(
     if (tid < 256) hist[tid] = 0;
     __syncthreads();
     const uint32_t prefix = s_prefix, mask = s_mask;
+    int candidates = 0;
     for (int i = tid; i < vocab; i += SAMPLE_THREADS) {
       const float v = lg[i];
       if (pass == 3 && !isfinite(v)) s_bad = 1;
+      candidates += v > NO_CANDIDATE;
       const uint32_t key = order_key(v);
       if ((key & mask) == prefix) atomicAdd(&hist[(key >> (8 * pass)) & 255u], 1u);
     }
+    if (pass == 3 && candidates > 0) atomicAdd(&s_candidates, candidates);
     __syncthreads();
+    if (pass == 3) k = min(k, s_candidates);
     if (tid == 0) {
-      int need = s_need, d = 255;
+      int need = pass == 3 ? k : s_need, d = 255;
       for (; d > 0; --d) {
         const int c = static_cast<int>(hist[d]);
         if (c >= need) break;
@@ -97,7 +105,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_topk_kernel(
   }
   __syncthreads();
   const int above = n_above, ties = n_tie;
-  if (s_bad || above + need_ties != k || ties > TIE_CAP) {
+  if (s_bad || k == 0 || above + need_ties != k || ties > TIE_CAP) {
     if (tid == 0) {
       flag[row] = 1;
       token[row] = -1;

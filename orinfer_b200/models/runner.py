@@ -42,6 +42,10 @@ class KVPool:
         return cls(mk(cfg.head_dim, torch.int8), mk(cfg.head_dim, torch.int8),
                    mk(g, torch.float16), mk(g, torch.float16), pages)
 
+    def cache_pages(self) -> F.CachePages:
+        """The pool as ``fork_pages``, ``compact_pages`` and ``copy_pages`` address it."""
+        return F.CachePages([*self.k, *self.v, *self.ks, *self.vs])
+
     @staticmethod
     def bytes_per_page(cfg: ModelConfig, extra_layers: int = 0) -> int:
         n = sum(cfg.is_full_attention(i) for i in range(cfg.layers)) + extra_layers

@@ -7,7 +7,7 @@ The matching fp32 PyTorch statement of each op lives in ``orinfer_b200.ref.ops_r
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -19,6 +19,11 @@ def _cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise native.KernelError("device op called with a CPU tensor")
+
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise native.KernelError(what)
 
 
 def embed_w8(ids: torch.Tensor, table_q: torch.Tensor, table_s: torch.Tensor,
@@ -228,6 +233,195 @@ def attention_prefill(q: torch.Tensor, gate: Optional[torch.Tensor], chunks: tor
     check(rc, "attention_prefill")
     count_launches(1)
     return True
+
+
+class SharedPrefix:
+    """Plan of a batch of single rows whose contexts share prefixes, for :func:`attention_shared`.
+    ``groups``: (first row, rows, keys) each; the page-table rows of a group's rows begin with the
+    same pages as far as their first ``keys`` keys lie on them (whole pages, as ``fork_pages`` and
+    the prefix cache share them).  Groups do not overlap; rows of no group share nothing.
+    ``max_kv_len`` bounds the keys that any row sees while the plan is in use, so that one plan
+    serves the steps of a decode loop."""
+
+    def __init__(self, groups: Sequence[Tuple[int, int, int]], rows: int, *, qh: int, kvh: int,
+                 head_dim: int, max_kv_len: int, device):
+        _need(rows >= 0 and max_kv_len >= 0, "rows and max_kv_len are not negative")
+        _need(head_dim in (64, 128, 256), "heads of 64, 128 or 256 channels")
+        rep = qh // kvh if kvh > 0 and qh % kvh == 0 else 0
+        _need(rep in (1, 2, 4, 8) or (rep == 5 and head_dim == 128),
+              f"{qh} query heads on {kvh} KV heads of {head_dim} channels")
+        taken = [False] * rows
+        for first, n, keys in groups:
+            _need(0 <= first and n >= 0 and first + n <= rows, f"group outside the {rows} rows")
+            _need(0 <= keys <= max_kv_len, f"{keys} shared keys of {max_kv_len}")
+            _need(not any(taken[first:first + n]), "a row is in two groups")
+            taken[first:first + n] = [True] * n
+        self.rows, self.qh, self.kvh, self.head_dim = rows, qh, kvh, head_dim
+        self.groups = [(int(f), int(n), int(k)) for f, n, k in groups if n > 0 and k > 0]
+        self.max_kv_len, self.device = max_kv_len, torch.device(device)
+
+
+def attention_shared(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: torch.Tensor,
+                     row_pos: torch.Tensor, page_table: torch.Tensor, kcache: torch.Tensor,
+                     vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor,
+                     plan: SharedPrefix, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`attention` of a batch whose rows share prefixes (``plan``): a shared key is read once
+    for all rows of its group.  A row sees keys 0..row_pos[r]; one at position -1 sees none and
+    gives zeros."""
+    _cuda(q, gate, row_req, row_pos, page_table, kcache, vcache, kscale, vscale, out)
+    n, qh, d = q.shape
+    _need(n == plan.rows and qh == plan.qh and d == plan.head_dim, "q is not what the plan is for")
+    _need(q.dtype == torch.float16 and q.is_contiguous(), "q: contiguous FP16 [rows, heads, D]")
+    _need(gate is None or (gate.dtype == torch.float16 and gate.is_contiguous()
+                           and gate.numel() == q.numel()), "gate: contiguous FP16, as q")
+    _need(row_req.dtype == torch.int32 and row_pos.dtype == torch.int32
+          and page_table.dtype == torch.int32, "row_req, row_pos, page_table: int32")
+    _need(row_req.numel() >= n and row_pos.numel() >= n and page_table.dim() == 2
+          and page_table.is_contiguous(), "row_req, row_pos: [rows]; page_table: [requests, pages]")
+    pages, cell = kcache.shape[0], (kcache.shape[0], 128, plan.kvh)
+    _need(kcache.shape == (*cell, d) and vcache.shape == (*cell, d)
+          and kcache.dtype == torch.int8 and vcache.dtype == torch.int8
+          and kcache.is_contiguous() and vcache.is_contiguous(),
+          "caches: contiguous int8 [pages, 128, kvh, D]")
+    _need(kscale.shape == (*cell, d // 64) and vscale.shape == (*cell, d // 64)
+          and kscale.dtype == torch.float16 and vscale.dtype == torch.float16
+          and kscale.is_contiguous() and vscale.is_contiguous(),
+          "scales: contiguous FP16 [pages, 128, kvh, D / 64]")
+    if out is None:
+        out = torch.empty(n, qh * d, dtype=torch.float16, device=q.device)
+    else:
+        _need(out.dtype == torch.float16 and out.is_contiguous() and out.numel() == q.numel(),
+              "out: contiguous FP16 [rows, heads * D]")
+    check(native.lib().orinfer_attention_shared(
+        ptr(q), ptr(gate), ptr(row_req), ptr(row_pos), ptr(page_table), page_table.shape[1],
+        ptr(kcache), ptr(vcache), ptr(kscale), ptr(vscale), ptr(out), n, qh, plan.kvh, d, pages,
+        stream()), "attention_shared")
+    count_launches(1)
+    return out
+
+
+# ---------------------------------------------------------------- pages of the cache
+class CachePages:
+    """The tensors of a paged cache (each contiguous [pages, 128, ...], all on one device), as the
+    page operators address them: ``KVPool.cache_pages()`` makes one for a model's cache.  It holds
+    the tensors."""
+
+    UNIT = 16384                                   # bytes that a CTA copies at a time
+
+    def __init__(self, tensors: Sequence[torch.Tensor]):
+        _need(len(tensors) > 0, "a cache has tensors")
+        _cuda(*tensors)
+        self.tensors = list(tensors)
+        self.pages, self.device = tensors[0].shape[0], tensors[0].device
+        sizes, units = [], []
+        for i, t in enumerate(tensors):
+            _need(t.dim() >= 2 and t.shape[0] == self.pages and t.shape[1] == 128
+                  and t.is_contiguous() and t.device == self.device and t.numel() > 0,
+                  "cache tensors: contiguous [pages, 128, ...] on one device")
+            size = t.element_size() * (t.numel() // (self.pages * 128))
+            step = max(16, min(128, self.UNIT // size // 16 * 16))
+            sizes.append(size)
+            units += [(i, at, min(step, 128 - at)) for at in range(0, 128, step)]
+        put = lambda v, dt: torch.tensor(v, dtype=dt, device=self.device)
+        self.bases = put([t.data_ptr() for t in tensors], torch.int64)
+        self.token_bytes, self.units = put(sizes, torch.int32), put(units, torch.int32)
+        self._args = (ptr(self.bases), ptr(self.token_bytes), ptr(self.units), len(units),
+                      self.pages)
+
+
+def _tables(table, lens, refs, out):
+    """The tensors that a page operator writes: ``out``, or new ones like its inputs."""
+    ins = [t for t in (table, lens, refs) if t is not None]
+    _cuda(*ins)
+    for t in ins:
+        _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == ins[0].device,
+              "table, lens, refs: contiguous int32")
+    _need(table.dim() == 2 and table.numel() > 0, "table: [slots, pages of a slot]")
+    _need(lens is None or lens.shape == table.shape[:1], "lens: [slots]")
+    if out is None:
+        return [torch.empty_like(t) for t in ins]
+    _need(len(out) == len(ins), "out: a tensor for each input")
+    for t, o in zip(ins, out):
+        _need(o.shape == t.shape and o.dtype == t.dtype and o.is_contiguous()
+              and o.device == t.device, "out: tensors like the inputs")
+    return list(out)
+
+
+def _slots(*lists):
+    _cuda(*lists)
+    for t in lists:
+        _need(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()
+              and t.shape == lists[0].shape, "lists of slots or pages: int32 [n]")
+    return lists[0].shape[0]
+
+
+def copy_pages(cache: CachePages, source: torch.Tensor, target: torch.Tensor,
+               tokens: Optional[torch.Tensor] = None) -> None:
+    """Copies pages ``source`` to ``target`` in every tensor of the cache, or their first
+    ``tokens`` tokens (int32 [n] each).  No target is a source, and none is named twice."""
+    n = _slots(source, target) if tokens is None else _slots(source, target, tokens)
+    if tokens is None:
+        tokens = torch.full_like(source, 128)
+    copies = torch.stack((source, target, tokens), dim=1)
+    count = torch.full((1,), n, dtype=torch.int32, device=source.device)
+    check(native.lib().orinfer_copy_pages(*cache._args, ptr(copies), ptr(count), n, stream()),
+          "copy_pages")
+    count_launches(1 if n else 0)
+
+
+def fork_pages(cache: CachePages, table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor,
+               parents: torch.Tensor, children: torch.Tensor, *, out=None):
+    """Makes slot ``children[i]``, which is empty, a copy of slot ``parents[i]``: whole pages are
+    shared, and a page that is not full is copied to a free one, the lowest first in the order of
+    the pairs.  ``table`` int32 [slots, pages], ``lens`` tokens per slot, ``refs`` references per
+    page (page 0 is nobody's).  Returns (table, lens, refs, status int32 [1]); ``out`` may be the
+    inputs.  Status 1: not enough free pages, 2: a pair that cannot be (a slot that does not exist,
+    a child that is not empty, named twice or a parent as well, a parent's page that nobody holds);
+    nothing is changed then."""
+    n = _slots(parents, children)
+    t, l, r = _tables(table, lens, refs, out)
+    _need(refs.shape == (cache.pages,), "refs: [pages]")
+    slots, width = table.shape
+    lib = native.lib()
+    work = torch.empty(lib.orinfer_fork_work(n, slots) + 1, dtype=torch.int32, device=table.device)
+    status = work[-1:]
+    check(lib.orinfer_fork_pages(
+        *cache._args, ptr(table), ptr(t), ptr(lens), ptr(l), ptr(refs), ptr(r), ptr(parents),
+        ptr(children), n, slots, width, ptr(work), ptr(status), stream()), "fork_pages")
+    count_launches(3 if n else 2)
+    return t, l, r, status
+
+
+def free_pages(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, slots: torch.Tensor, *,
+               out=None):
+    """Empties ``slots`` (int32 [n]; one named again is emptied once): every page of their rows
+    loses a reference.  Returns (table, lens, refs); ``out`` may be the inputs.  A slot or page that
+    does not exist, or a page that nobody holds, is left alone and reported by the status word."""
+    n = _slots(slots)
+    t, l, r = _tables(table, lens, refs, out)
+    _need(refs.dim() == 1 and refs.numel() > 0, "refs: [pages]")
+    check(native.lib().orinfer_free_pages(
+        ptr(table), ptr(t), ptr(lens), ptr(l), ptr(refs), ptr(r), ptr(slots), n, table.shape[0],
+        table.shape[1], refs.shape[0], stream()), "free_pages")
+    count_launches((t is not table or l is not lens or r is not refs) + (n > 0))
+    return t, l, r
+
+
+def compact_pages(cache: CachePages, table: torch.Tensor, refs: torch.Tensor, *, out=None):
+    """Moves the pages that are held to the front: with L of them, the k-th one above page L goes to
+    the k-th free page of 1..L.  Returns (table, refs, moved): ``moved`` int32 [pages] says where
+    each page has gone.  ``out`` (table, refs) may be the inputs."""
+    t, r = _tables(table, None, refs, out)
+    _need(refs.shape == (cache.pages,), "refs: [pages]")
+    lib = native.lib()
+    moved = torch.empty_like(refs)
+    work = torch.empty(lib.orinfer_compact_work(cache.pages), dtype=torch.int32,
+                       device=table.device)
+    check(lib.orinfer_compact_pages(
+        *cache._args, ptr(table), ptr(t), ptr(refs), ptr(r), ptr(moved), table.shape[0],
+        table.shape[1], ptr(work), stream()), "compact_pages")
+    count_launches(3 if cache.pages > 1 else 2)
+    return t, r, moved
 
 
 def argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -454,3 +648,78 @@ def sample_topk(logits: torch.Tensor, top_k: torch.Tensor, temperature: torch.Te
                                            ptr(flag), stream()), "sample_topk")
     count_launches(1)
     return tok, flag
+
+
+MASKED = -1e30      # a score that is never drawn: the arg-max and the sampler want finite ones
+
+
+def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
+                   history_len: Optional[torch.Tensor] = None,
+                   repetition: Optional[torch.Tensor] = None,
+                   presence: Optional[torch.Tensor] = None,
+                   frequency: Optional[torch.Tensor] = None,
+                   bias_start: Optional[torch.Tensor] = None,
+                   bias_ids: Optional[torch.Tensor] = None,
+                   bias_values: Optional[torch.Tensor] = None,
+                   mask: Optional[torch.Tensor] = None, mask_rows: Optional[torch.Tensor] = None,
+                   masked: float = MASKED, out: Optional[torch.Tensor] = None,
+                   flags: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Penalties, biases and grammar masks on ``logits`` fp32 [rows, vocab], by the host law's
+    arithmetic (64 bits), rounded once to FP32.
+
+    ``history`` int32 [rows, n] holds ``history_len[r]`` tokens of row r (ids outside the vocabulary
+    do not count); ``repetition``, ``presence``, ``frequency`` are fp64 [rows] (1, 0, 0 without
+    them).  Row r's biases are ``bias_values`` (fp64) of tokens ``bias_ids`` at bias_start[r] ..
+    bias_start[r + 1], the last one of a token counting.  ``mask`` int32 [m, (vocab + 31) / 32]: a
+    set bit permits its token; row r is bound by mask ``mask_rows[r]``, by none below 0, by mask r
+    without ``mask_rows``.  Tokens that are not permitted get ``masked``.  Returns (out, flags int32
+    [rows]): 1 where nothing is permitted, 2 where a logit or a permitted token's score is not
+    finite or the mask does not exist (the host law refuses those rows), else 0.  ``out`` may be ``logits``."""
+    _cuda(logits, history, history_len, repetition, presence, frequency, bias_start, bias_ids,
+          bias_values, mask, mask_rows, out, flags)
+    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.stride(1) == 1
+          and logits.shape[1] > 0, "logits: fp32 [rows, vocab], rows in one piece")
+    rows, vocab = logits.shape
+    hist_stride = cap = bias_total = mask_stride = masks = 0
+    if history is not None:
+        _need(history.dtype == torch.int32 and history.dim() == 2 and history.shape[0] == rows
+              and (history.shape[1] < 2 or history.stride(1) == 1), "history: int32 [rows, n]")
+        _need(history_len is not None and history_len.dtype == torch.int32
+              and history_len.shape == (rows,) and history_len.is_contiguous(),
+              "history_len: int32 [rows]")
+        hist_stride, cap = history.stride(0), history.shape[1]
+    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        _need(t is None or (t.dtype == torch.float64 and t.shape == (rows,) and t.is_contiguous()
+                            and history is not None), f"{name}: fp64 [rows], with a history")
+    if bias_start is not None:
+        _need(bias_start.dtype == torch.int32 and bias_start.shape == (rows + 1,)
+              and bias_start.is_contiguous(), "bias_start: int32 [rows + 1]")
+        _need(bias_ids is not None and bias_values is not None and bias_ids.dtype == torch.int32
+              and bias_values.dtype == torch.float64 and bias_ids.dim() == 1
+              and bias_ids.shape == bias_values.shape and bias_ids.is_contiguous()
+              and bias_values.is_contiguous(), "bias_ids: int32, bias_values: fp64, [entries]")
+        bias_total = bias_ids.shape[0]
+    if mask is not None:
+        _need(mask.dtype == torch.int32 and mask.dim() == 2 and mask.stride(1) == 1
+              and mask.shape[1] >= (vocab + 31) // 32, "mask: int32 [m, (vocab + 31) / 32]")
+        _need(mask.shape[0] >= rows if mask_rows is None else
+              (mask_rows.dtype == torch.int32 and mask_rows.shape == (rows,)
+               and mask_rows.is_contiguous()), "mask_rows: int32 [rows], or a mask per row")
+        mask_stride, masks = mask.stride(0), mask.shape[0]
+    if out is None:
+        out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
+    else:
+        _need(out.shape == logits.shape and out.dtype == torch.float32 and out.stride(1) == 1,
+              "out: fp32 [rows, vocab]")
+    if flags is None:
+        flags = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    else:
+        _need(flags.shape == (rows,) and flags.dtype == torch.int32 and flags.is_contiguous(),
+              "flags: int32 [rows]")
+    check(native.lib().orinfer_process_logits(
+        ptr(logits), logits.stride(0), ptr(history), hist_stride, cap, ptr(history_len),
+        ptr(repetition), ptr(presence), ptr(frequency), ptr(bias_start), ptr(bias_ids),
+        ptr(bias_values), bias_total, ptr(mask), mask_stride, ptr(mask_rows), masks, masked,
+        ptr(out), out.stride(0), ptr(flags), rows, vocab, stream()), "process_logits")
+    count_launches(1 if rows else 0)
+    return out, flags
