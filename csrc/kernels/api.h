@@ -201,11 +201,14 @@ int orinfer_attention_prefill(const __half* q, const __half* gate, const int* ch
                               int num_pages, int context, cudaStream_t stream);
 
 // Single rows whose contexts begin with the same pages (attention_shared.cu).
+int orinfer_shared_step(int head_dim);
 int orinfer_attention_shared(const __half* q, const __half* gate, const int* row_req,
-                             const int* row_pos, const int* page_table, int max_pages,
+                             const int* row_pos, const int* page_table, int slots, int max_pages,
                              const int8_t* kc, const int8_t* vc, const __half* ks,
                              const __half* vs, __half* out, int rows, int qh, int kvh,
-                             int head_dim, int num_pages, cudaStream_t stream);
+                             int head_dim, int num_pages, const int* items, int n_items,
+                             const int* rows_info, float* parts, int n_parts, int splits,
+                             float* scratch, int context, cudaStream_t stream);
 
 // ---- expert-parallel all-to-alls over peer memory (moe_a2a.cu); cap = owned rows x top_k
 typedef struct OrinferA2aDispatch {

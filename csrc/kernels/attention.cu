@@ -7,6 +7,7 @@
 // configurations of causal_attention_int8 and merge_attention_int8
 // (kernels/cuda/model/attention_rows.py:61-276,280-400).
 #include "api.h"
+#include "attention_shared.h"
 #include "common.cuh"
 #include "tma.h"
 
@@ -115,13 +116,56 @@ __device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
 
+// A head's shared parts join its own keys' sums `o` of channel lane + 32 i, `m` and `l`; a warp
+// together.  Eight parts at a time: each is a load of its own to wait for.
+template <int D>
+__device__ __forceinline__ void attn_join(const SharedParts& parts, int row, int head, int qh,
+                                          float& m, float& l, float (&o)[D / 32]) {
+  const int lane = threadIdx.x & 31;
+  const int4 info = parts.rows[row];
+  const float2* ml = parts.ml + static_cast<size_t>(info.y) * qh + head;
+  const float* po = parts.o + (static_cast<size_t>(info.y) * qh + head) * D + lane;
+  float top = m;
+  for (int i = lane; i < info.z; i += 32) top = fmaxf(top, ml[static_cast<size_t>(i) * qh].x);
+  top = warp_max(top);
+  const float own = m == -INFINITY ? 0.f : exp2f(m - top);
+  l *= own;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) o[k] *= own;
+  m = top;
+  for (int i0 = 0; i0 < info.z; i0 += 32) {
+    const float2 p = i0 + lane < info.z ? ml[static_cast<size_t>(i0 + lane) * qh]
+                                        : make_float2(-INFINITY, 0.f);
+    const float f = p.x == -INFINITY ? 0.f : exp2f(p.x - m);
+    l += warp_sum(p.y * f);
+    const int n = min(32, info.z - i0);
+    for (int i = 0; i < n; i += 8) {
+      float v[8][D / 32];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k)
+          v[j][k] = i + j < n ? po[static_cast<size_t>(i0 + i + j) * qh * D + 32 * k] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, (i + j) & 31);
+        if (i + j < n) {
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) o[k] = fmaf(v[j][k], fj, o[k]);
+        }
+      }
+    }
+  }
+}
+
 // The four warps' results (R rows of heads each, and the maxima and sums of their weights) become
 // the row's output or, where the keys are split, a record for the merge.
-template <int D, int R>
+template <int D, int R, bool SHARED = false>
 __device__ __forceinline__ void attn_finish(const float (*s_o)[R][D], const float (*s_m)[R],
                                             const float (*s_l)[R], bool apart, bool idle, int rep,
                                             int row, int h, int qh, int split, int splits,
-                                            const __half* gate, __half* out, float* scratch) {
+                                            const __half* gate, __half* out, float* scratch,
+                                            const SharedParts& parts = SharedParts()) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __syncthreads();
   if (idle) return;
@@ -136,6 +180,20 @@ __device__ __forceinline__ void attn_finish(const float (*s_o)[R][D], const floa
         f[w] = s_m[w][r] == -INFINITY ? 0.f : exp2f(s_m[w][r] - m);
         l = fmaf(s_l[w][r], f[w], l);
       }
+    }
+    if (SHARED && splits == 1) {
+      float o[D / 32];
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        o[k] = 0.f;
+#pragma unroll
+        for (int w = 0; w < ATTN_WARPS; ++w) o[k] = fmaf(s_o[w][r][lane + 32 * k], f[w], o[k]);
+      }
+      attn_join<D>(parts, row, h * rep + r, qh, m, l, o);
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k)
+        attn_store(l > 0.f ? o[k] / l : 0.f, gate, out, head * D + lane + 32 * k);
+      continue;
     }
     float* rec = scratch + (head * splits + split) * (D + 2);
     if (splits > 1 && lane == 0) {
@@ -165,13 +223,13 @@ __device__ __forceinline__ void attn_finish(const float (*s_o)[R][D], const floa
 // 120 keys 87 -> 62; 32 / 8, 128 rows of 64 keys 13.2 -> 12.3, but 64 rows (no second wave) 9.0 ->
 // 9.9; fewer than four KV heads leave warps idle (16 / 2 of 256, 512 rows of 60 keys 28 -> 30).
 // Longer rows of such a launch pay up to 3 % for the form (8 / 8 of 64, 128 rows of 640 keys).
-template <int D, bool WIDE, bool APART>
+template <int D, bool WIDE, bool APART, bool SHARED = false>
 __global__ void __launch_bounds__(
     ATTN_WARPS * 32, D == 64 && !APART ? 3 : AttnTile<D>::MIN_CTAS) attn_rows_kernel(
     const __half* q, const __half* gate, const int* row_req, const int* row_pos,
     const int* page_table, int max_pages, const int8_t* kc, const int8_t* vc, const __half* ks,
     const __half* vs, __half* __restrict__ out, int qh, int kvh, int splits,
-    float* __restrict__ scratch, int rep, int apart_keys) {
+    float* __restrict__ scratch, int rep, int apart_keys, const SharedParts parts) {
   constexpr int G = AttnTile<D>::G, KB = AttnTile<D>::KB;
   constexpr int NT = KB / 8, UT = KB / 16;         // 8-key score tiles, 16-key value tiles
   grid_wait();
@@ -184,8 +242,9 @@ __global__ void __launch_bounds__(
   if (apart && (blockIdx.y & (ATTN_WARPS - 1)) != 0) return;
   const int h = apart ? min(static_cast<int>(blockIdx.y) + warp, kvh - 1) : blockIdx.y;
   const bool idle = apart && static_cast<int>(blockIdx.y) + warp >= kvh;
-  const int per = (kv_len + splits - 1) / splits;
-  const int k_lo = split * per, k_hi = min(kv_len, k_lo + per);
+  const int first = SHARED ? min(parts.rows[row].x, max(kv_len, 0)) : 0;
+  const int per = (kv_len - first + splits - 1) / splits;
+  const int k_lo = first + split * per, k_hi = min(kv_len, k_lo + per);
   const int* pages = page_table + static_cast<size_t>(row_req[row]) * max_pages;
   const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
 
@@ -432,7 +491,8 @@ __global__ void __launch_bounds__(
       s_l[warp][g] = l_run;
     }
   }
-  attn_finish<D, 8>(s_o, s_m, s_l, apart, idle, rep, row, h, qh, split, splits, gate, out, scratch);
+  attn_finish<D, 8, SHARED>(s_o, s_m, s_l, apart, idle, rep, row, h, qh, split, splits, gate, out,
+                            scratch, parts);
 }
 
 // ---------------------------------------------------------------- digit form
@@ -529,13 +589,13 @@ __device__ __forceinline__ void load_pair(float (&v)[2 * G], const float* p) {
   }
 }
 
-template <int D, bool APART>
+template <int D, bool APART, bool SHARED = false>
 __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_digits_kernel(
     const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
     const __half* q, const __half* gate, const int* row_req, const int* row_pos,
     const int* page_table, int max_pages, const __half* ks, const __half* vs,
     __half* __restrict__ out, int qh, int kvh, int splits, float* __restrict__ scratch, int rep,
-    int apart_keys, int* status) {
+    int apart_keys, int* status, const SharedParts parts) {
   using T = DigitTile<D>;
   constexpr int G = T::G, KB = T::KB, KSTEPS = T::KSTEPS;
   grid_wait();
@@ -548,8 +608,9 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
   if (apart && (blockIdx.y & (ATTN_WARPS - 1)) != 0) return;
   const int h = apart ? min(static_cast<int>(blockIdx.y) + warp, kvh - 1) : blockIdx.y;
   const bool idle = apart && static_cast<int>(blockIdx.y) + warp >= kvh;
-  const int per = (kv_len + splits - 1) / splits;
-  const int k_lo = split * per, k_hi = min(kv_len, k_lo + per);
+  const int first = SHARED ? min(parts.rows[row].x, max(kv_len, 0)) : 0;
+  const int per = (kv_len - first + splits - 1) / splits;
+  const int k_lo = first + split * per, k_hi = min(kv_len, k_lo + per);
   const int* pages = page_table + static_cast<size_t>(row_req[row]) * max_pages;
 
   extern __shared__ unsigned char digits_smem[];
@@ -966,7 +1027,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
     s_m[warp][head] = m_ref;
     s_l[warp][head] = l_run;
   }
-  attn_finish<D, 4>(s_o, s_m, s_l, apart, idle, rep, row, h, qh, split, splits, gate, out, scratch);
+  attn_finish<D, 4, SHARED>(s_o, s_m, s_l, apart, idle, rep, row, h, qh, split, splits, gate, out,
+                            scratch, parts);
 }
 
 // One CTA per row and head.  The records' maxima and sums are read by a lane each and handed round,
@@ -974,9 +1036,10 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
 // a record per step of the loop, and attn_finish computing every factor anew for each channel, one
 // row of 2000 keys and 32 / 8 heads of 128 took 10.7 us (now 8.3), 16 / 2 heads of 256 (32 records)
 // 15.1 (10.0), 64 rows of 640 keys unsplit 26.8 (22.9).
-template <int D>
+template <int D, bool SHARED>
 __global__ void attn_merge_kernel(
-    const float* scratch, const __half* gate, __half* __restrict__ out, int qh, int splits) {
+    const float* scratch, const __half* gate, __half* __restrict__ out, int qh, int splits,
+    const SharedParts parts) {
   grid_wait();
   grid_release();
   const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31;
@@ -984,8 +1047,25 @@ __global__ void attn_merge_kernel(
   float m = -INFINITY;
   for (int s = lane; s < splits; s += 32) m = fmaxf(m, rec[s * (D + 2)]);
   m = warp_max(m);
+  // the shared parts' records follow the row's own
+  const int4 info = SHARED ? parts.rows[row] : make_int4(0, 0, 0, 0);
+  const float2* ml = parts.ml + static_cast<size_t>(info.y) * qh + head;
+  const float* po = parts.o + (static_cast<size_t>(info.y) * qh + head) * D;
+  if (SHARED) {
+    for (int s = lane; s < info.z; s += 32) m = fmaxf(m, ml[static_cast<size_t>(s) * qh].x);
+    m = warp_max(m);
+  }
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
     float l = 0.f, o = 0.f;
+    if (SHARED) {
+#pragma unroll 4
+      for (int s = 0; s < info.z; ++s) {
+        const float2 p = ml[static_cast<size_t>(s) * qh];
+        const float f = p.x == -INFINITY ? 0.f : exp2f(p.x - m);
+        l = fmaf(p.y, f, l);
+        o = fmaf(po[static_cast<size_t>(s) * qh * D + d], f, o);
+      }
+    }
     for (int s0 = 0; s0 < splits; s0 += 32) {
       const int n = min(32, splits - s0);
       const float* own = rec + (s0 + min(lane, n - 1)) * (D + 2);
@@ -1060,15 +1140,16 @@ static bool kv_map(CUtensorMap* map, const int8_t* cache, int kvh) {
          CUDA_SUCCESS;
 }
 
-template <int D>
+template <int D, bool SHARED = false>
 static int launch_attn(const __half* q, const __half* gate, const int* row_req, const int* row_pos,
                        const int* page_table, int max_pages, const int8_t* kc, const int8_t* vc,
                        const __half* ks, const __half* vs, __half* out, int rows, int qh, int kvh,
-                       int rep, int splits, float* scratch, int context, cudaStream_t stream) {
+                       int rep, int splits, float* scratch, int context, cudaStream_t stream,
+                       const SharedParts& parts = SharedParts()) {
   dim3 grid(rows, kvh, splits);
   const bool wide = ((reinterpret_cast<uintptr_t>(q) & 15) | (reinterpret_cast<uintptr_t>(ks) & 7) |
                      (reinterpret_cast<uintptr_t>(vs) & 7)) == 0;
-  const long long ctas = splits > 1 || kvh < ATTN_WARPS ? 0 : static_cast<long long>(rows) * kvh;
+  const long long ctas = SHARED || splits > 1 || kvh < ATTN_WARPS ? 0 : static_cast<long long>(rows) * kvh;
   const long long waves = ctas / (148 * AttnTile<D>::MIN_CTAS);
   const int apart_keys = AttnTile<D>::KB * static_cast<int>(waves < 4 ? waves : 4);
   const bool apart = apart_keys > 0;
@@ -1085,27 +1166,45 @@ static int launch_attn(const __half* q, const __half* gate, const int* row_req, 
   if (attn_digits(D, rep, pages, splits, wide, kc, vc) && kv_map<D>(&tk, kc, kvh) &&
       kv_map<D>(&tv, vc, kvh)) {
     constexpr int D_ = D == 256 ? 128 : D;         // (256 channels: never)
-    auto kernel = apart ? attn_digits_kernel<D_, true> : attn_digits_kernel<D_, false>;
+    auto kernel = !SHARED && apart ? attn_digits_kernel<D_, !SHARED, SHARED>
+                                   : attn_digits_kernel<D_, false, SHARED>;
     static const int slot[2] = {runtime_new_slot(), runtime_new_slot()};
     constexpr int SMEM = DigitTile<D_>::SMEM;
     if (const int e = runtime_allow_smem(slot[apart], kernel, SMEM)) return e;
     start(kernel, SMEM, tk, tv, q, gate, row_req, row_pos, page_table, max_pages, ks, vs, out, qh,
-          kvh, splits, scratch, rep, apart_keys, runtime_status_ptr());
+          kvh, splits, scratch, rep, apart_keys, runtime_status_ptr(), parts);
   } else {
     auto kernel =
-        wide ? (apart ? attn_rows_kernel<D, true, true> : attn_rows_kernel<D, true, false>)
-             : (apart ? attn_rows_kernel<D, false, true> : attn_rows_kernel<D, false, false>);
+        wide ? (apart ? attn_rows_kernel<D, true, !SHARED, SHARED>
+                      : attn_rows_kernel<D, true, false, SHARED>)
+             : (apart ? attn_rows_kernel<D, false, !SHARED, SHARED>
+                      : attn_rows_kernel<D, false, false, SHARED>);
     static const int slot[4] = {runtime_new_slot(), runtime_new_slot(), runtime_new_slot(),
                                 runtime_new_slot()};
     constexpr int SMEM = AttnTile<D>::SMEM;
     if (const int e = runtime_allow_smem(slot[2 * apart + wide], kernel, SMEM)) return e;
     start(kernel, SMEM, q, gate, row_req, row_pos, page_table, max_pages, kc, vc, ks, vs, out, qh,
-          kvh, splits, scratch, rep, apart_keys);
+          kvh, splits, scratch, rep, apart_keys, parts);
   }
   if (splits > 1)
-    launch_early(attn_merge_kernel<D>, dim3(rows, qh), D < 128 ? 64 : 128, 0, stream, scratch, gate,
-                 out, qh, splits);
+    launch_early(attn_merge_kernel<D, SHARED>, dim3(rows, qh), D < 128 ? 64 : 128, 0, stream,
+                 scratch, gate, out, qh, splits, parts);
   return static_cast<int>(cudaGetLastError());
+}
+
+int attention_own_keys(const __half* q, const __half* gate, const int* row_req, const int* row_pos,
+                       const int* page_table, int max_pages, const int8_t* kc, const int8_t* vc,
+                       const __half* ks, const __half* vs, __half* out, int rows, int qh, int kvh,
+                       int head_dim, int splits, float* scratch, int context,
+                       const SharedParts& parts, cudaStream_t stream) {
+#define CASE(DD)                                                                                  \
+  if (head_dim == DD)                                                                             \
+    return launch_attn<DD, true>(q, gate, row_req, row_pos, page_table, max_pages, kc, vc, ks, vs, \
+                                 out, rows, qh, kvh, qh / kvh, splits, scratch, context, stream,  \
+                                 parts);
+  CASE(64) CASE(128) CASE(256)
+#undef CASE
+  return -1;
 }
 
 }  // namespace orinfer

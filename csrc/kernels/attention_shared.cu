@@ -1,78 +1,558 @@
 // Attention of single rows whose contexts begin with the same pages (samples of one prompt,
 // requests under one system prompt), over the paged INT8 cache.
 //
-// One CTA per (row, query head); its warps take the keys in turn, a lane holding the same channels
-// of the query, of every key and of the output.  Online softmax in FP32, joined in shared memory.
+// The shared keys of a group of rows are read once: the group's rows times the `rep` query heads of
+// a KV head are the M axis of one product with the prefix, on tcgen05 tensor cores with TMEM
+// accumulators.  A CTA takes one or two tiles of 128 such rows and a range of the keys, and leaves
+// each row's part of the softmax (reference, sum of weights, sum of weighted values) for the row
+// kernels of attention.cu, which add the row's own keys and join the parts.
+//
+//   S_g = Q K_g^T   a sum of its own per group of 64 channels, K as the exact FP16 integers that the
+//                   cache holds;  score = sum_g S_g x key scale_g in FP32;
+//   O_g = P_g V_g   P_g = weight x value scale_g rounded to FP16, V as exact integers.
+// So a row's result carries one rounding of FP16 per weight (2.9e-4 against 64 bits with the
+// output's own 2.07e-4); keys and values rounded after their scales, as prefill attention has them,
+// would add one each and another 40 %.  P_g is taken under a power of two per group that follows the
+// value scales, so that it stays among FP16's normal numbers.
+//
+// Two contexts of four softmax warps (a thread per row) take turns with the tensor core: two tiles
+// that share every step's keys, or, where a group has one tile left, one tile whose steps they take
+// in turn, each with a softmax of its own.
 #include "api.h"
+#include "attention_shared.h"
 #include "common.cuh"
 
 namespace orinfer {
 namespace sp {
 
-constexpr int WARPS = 4;
+constexpr int TILE = 128;                        // rows of a tile: positions x query heads
+// Fourteen warps: with at most four on a scheduler each thread has 128 registers.
+constexpr int SOFTMAX_WARPS = 8, DQ_WARPS = 4;
+constexpr int MMA_WARP = SOFTMAX_WARPS + DQ_WARPS, SCALE_WARP = MMA_WARP + 1;
+constexpr int THREADS = (SCALE_WARP + 1) * 32;
+constexpr float LAG = 8.f;                       // of the weights' reference, binades
 
 template <int D>
-__global__ void __launch_bounds__(WARPS * 32) rows_kernel(
-    const __half* q, const __half* gate, const int* row_req, const int* row_pos,
-    const int* page_table, int max_pages, const int8_t* kc, const int8_t* vc, const __half* ks,
-    const __half* vs, __half* __restrict__ out, int qh, int kvh, int num_pages, int* status) {
-  constexpr int PER = D / 32, G = D / 64;            // channels of a lane, scale groups
+struct Shape {
+  static constexpr int G = D / 64;               // scale groups of a key
+  static constexpr int DV = D > 128 ? 128 : D;   // value channels of a CTA
+  static constexpr int GV = DV / 64, PARTS = D / DV;
+  static constexpr int KT = D > 128 ? 32 : 64;   // keys of a step: at most 128 score columns
+  static constexpr int NB = D > 128 ? 3 : 4;     // buffers of keys and values
+  static constexpr int PF = 2;                   // steps whose bytes are in flight to registers
+  static constexpr int QSUB = TILE * 128, KSUB = KT * 128;     // bytes of 64 channels of a tile
+  static constexpr int K_BYTES = G * KSUB, V_BYTES = GV * KSUB;
+  static constexpr int Q_OFF = 0;                // two tiles
+  static constexpr int KV_OFF = 2 * G * QSUB;
+  static constexpr int SCALE_OFF = KV_OFF + NB * (K_BYTES + V_BYTES);
+  static constexpr int SCALES = KT * (G + GV) * 4 + 16;        // key and value scales, units
+  static constexpr int BAR_OFF = SCALE_OFF + NB * SCALES;
+  static constexpr int TOTAL = BAR_OFF + 256 + 1024;
+  static_assert(TOTAL <= 227 * 1024, "exceeds the shared memory of one CTA");
+  static_assert(SCALES % 16 == 0, "scales are read sixteen bytes at a time");
+};
+
+// Rows and keys of a CTA (as many as the plan has), per KV head.
+struct Item {
+  int row, rows;                                 // the first row, and how many (at most two tiles)
+  int step_lo, step_hi;                          // its steps of KT keys
+  int shared;                                    // keys that the group shares
+  int part;                                      // its part of a row's parts
+  int pair;                                      // two tiles
+  int unused;
+};
+
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t tmem_d, uint64_t adesc,
+                                       uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a,
+                                       uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 pair_at(uint32_t a, uint32_t b) {
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+
+// Eight INT8 values -> eight FP16 values, exactly: 0x64xx is 1024 + xx, and 1152 is subtracted.
+__device__ __forceinline__ uint4 integers(uint32_t w0, uint32_t w1) {
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+  const uint32_t x0 = w0 ^ 0x80808080u, x1 = w1 ^ 0x80808080u;
+  uint32_t h[4] = {__byte_perm(x0, 0x64646464u, 0x4140), __byte_perm(x0, 0x64646464u, 0x4342),
+                   __byte_perm(x1, 0x64646464u, 0x4140), __byte_perm(x1, 0x64646464u, 0x4342)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h[i]), bias);
+    h[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
+    const __half* q, const int* row_req, const int* row_pos, const int* page_table, int slots,
+    int max_pages, const int8_t* kc, const int8_t* vc, const __half* ks, const __half* vs,
+    const Item* items, const int4* info, float* __restrict__ part_o, float2* __restrict__ part_ml,
+    int qh, int kvh, int rep, int num_pages, int* status) {
+  using L = Shape<D>;
+  constexpr int G = L::G, GV = L::GV, KT = L::KT, NB = L::NB;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* kv_full = bars;              // [NB] keys, values and scales of a step are there
+  uint64_t* kv_free = bars + NB;         // [NB] the last product that reads them is through
+  uint64_t* s_full = bars + 2 * NB;      // [2] scores of a context
+  uint64_t* p_ready = s_full + 2;        // [2] its weights (an arrival per warp)
+  uint64_t* o_done = s_full + 4;         // [2] its last product is through
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 6);
+
+  const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
   grid_wait();
-  grid_release();
-  const int row = blockIdx.x, head = blockIdx.y, h = head / (qh / kvh);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = min(row_pos[row] + 1, max_pages * 128);
-  const int* pages = page_table + static_cast<size_t>(row_req[row]) * max_pages;
-  const size_t at = (static_cast<size_t>(row) * qh + head) * D + lane * PER;
-  float qv[PER], acc[PER], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    qv[i] = __half2float(q[at + i]) * rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
-    acc[i] = 0.f;
-  }
-  for (int key = warp; key < n; key += WARPS) {
-    const int page = pages[key >> 7];
-    if (page < 0 || page >= num_pages) {
-      if (lane == 0) report_status(status, STATUS_BAD_INDEX, 0x50);
-      continue;
+  const Item it = items[blockIdx.x];
+  const int h = blockIdx.y / L::PARTS, vpart = blockIdx.y % L::PARTS;
+  const int P = TILE / rep, tiles = it.pair ? 2 : 1;
+  const int steps = it.step_hi - it.step_lo;
+  // turns of the contexts: both at every step, or one step each in turn
+  const int turns = it.pair ? 2 * steps : steps;
+  const int req = row_req[it.row];
+  const bool known = req >= 0 && req < slots;
+  const int* pages = page_table + static_cast<size_t>(known ? req : 0) * max_pages;
+
+  if (tid == 0) {
+    for (int b = 0; b < NB; ++b) {
+      mbar_init(&kv_full[b], DQ_WARPS + 1);
+      mbar_init(&kv_free[b], 1);
     }
-    const size_t slot = (static_cast<size_t>(page) * 128 + (key & 127)) * kvh + h;
-    const int group = lane * PER / 64;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s = fmaf(qv[i], kc[slot * D + lane * PER + i], s);
-    s = warp_sum(s * __half2float(ks[slot * G + group]));
-    const float m_new = fmaxf(m, s), f = m == -INFINITY ? 0.f : exp2f(m - m_new);
-    const float p = exp2f(s - m_new), scale = p * __half2float(vs[slot * G + group]);
-    l = fmaf(l, f, p);
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      acc[i] = fmaf(acc[i], f, scale * vc[slot * D + lane * PER + i]);
-    m = m_new;
+    for (int c = 0; c < 2; ++c) {
+      mbar_init(&s_full[c], 1);
+      mbar_init(&p_ready[c], 4);
+      mbar_init(&o_done[c], 1);
+    }
+    mbar_fence_init();
   }
-  __shared__ float s_o[WARPS][D], s_m[WARPS], s_l[WARPS];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) s_o[warp][lane * PER + i] = acc[i];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
+  if (warp == MMA_WARP) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
   }
+  // ---- the query rows, 16 bytes at a time, zeros where a tile has none
+  {
+    const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+    constexpr int CPR = D / 8;                   // 16-byte pieces of a row
+    for (int i = tid; i < tiles * TILE * CPR; i += THREADS) {
+      const int m = i / CPR, c = i % CPR, t = m / TILE, r = m % TILE;
+      const int row = t * P + r / rep;
+      __align__(16) __half v[8];
+      *reinterpret_cast<uint4*>(v) = make_uint4(0, 0, 0, 0);
+      if (r < P * rep && row < it.rows) {
+        const __half* from = q + (static_cast<size_t>(it.row + row) * qh + h * rep + r % rep) * D +
+                             c * 8;
+        if (wide) {
+          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(from);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = from[k];
+        }
+      }
+      *reinterpret_cast<uint4*>(smem + L::Q_OFF + (t * G + c / 8) * L::QSUB + swz128(r, c % 8)) =
+          *reinterpret_cast<const uint4*>(v);
+    }
+  }
+  fence_proxy_async();
+  tc_fence_before();
   __syncthreads();
-  float m_all = -INFINITY, l_all = 0.f;
-  for (int w = 0; w < WARPS; ++w) m_all = fmaxf(m_all, s_m[w]);
-  for (int d = threadIdx.x; d < D; d += WARPS * 32) {
-    float o = 0.f;
-    l_all = 0.f;
-    for (int w = 0; w < WARPS; ++w) {
-      const float f = s_m[w] == -INFINITY ? 0.f : exp2f(s_m[w] - m_all);
-      o = fmaf(s_o[w][d], f, o);
-      l_all = fmaf(s_l[w], f, l_all);
+  tc_fence_after();
+  const uint32_t tmem = warp_same(*tmem_slot);
+  grid_release();
+  const uint32_t tmem_o = tmem + 256;            // O of context c at + 128 c; S at 128 c
+
+  if (warp == MMA_WARP) {
+    // ---------------- products, issued by the whole warp (see elect_one)
+    constexpr uint32_t idesc_s = umma_idesc(1, 0, 0, 0, 0, TILE, KT);
+    constexpr uint32_t idesc_o = umma_idesc(1, 0, 0, 0, 1, TILE, 64);
+    const uint32_t leader = elect_one();
+    const uint64_t qd = umma_desc(smem_u32(smem + L::Q_OFF), 16, 1024);
+    const uint64_t kd = umma_desc(smem_u32(smem + L::KV_OFF), 16, 1024);
+    const uint64_t vd = umma_desc(smem_u32(smem + L::KV_OFF + L::K_BYTES), L::KSUB, 1024);
+    const int last = warp_same(turns), pair = warp_same(it.pair);
+    bool ok = true;
+    auto step_of = [&](int t) { return pair ? t >> 1 : t; };
+    auto issue_qk = [&](int t) {
+      const int c = t & 1, s = step_of(t), b = s % NB;
+      if (ok)
+        ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[b], (s / NB) & 1, status, STATUS_MMA_WAIT,
+                                               0x400 | (s & 0xff)));
+      tc_fence_after();
+      if (!ok) return;
+      const uint64_t qt = qd + (pair ? c * G * L::QSUB / 16 : 0);
+      const uint64_t kb = kd + static_cast<uint64_t>(b) * ((L::K_BYTES + L::V_BYTES) / 16);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_ss(leader, tmem + 128 * c + g * KT, qt + (g * L::QSUB + k * 32) / 16,
+                 kb + (g * L::KSUB + k * 32) / 16, idesc_s, k != 0 ? 1u : 0u);
+      tc_commit_by(leader, &s_full[c]);
+    };
+    if (last > 0) issue_qk(0);
+    if (last > 1) issue_qk(1);
+    for (int t = 0; t < last && ok; ++t) {
+      const int c = t & 1, i = t >> 1, b = step_of(t) % NB;
+      ok = __all_sync(0xffffffffu, mbar_wait(&p_ready[c], i & 1, status, STATUS_MMA_WAIT,
+                                             0x500 | (i & 0xff)));
+      tc_fence_after();
+      if (!ok) break;
+      const uint64_t vb = vd + static_cast<uint64_t>(b) * ((L::K_BYTES + L::V_BYTES) / 16);
+#pragma unroll
+      for (int g = 0; g < GV; ++g)
+#pragma unroll
+        for (int k = 0; k < KT / 16; ++k)
+          mma_ts(leader, tmem_o + 128 * c + g * 64, tmem + 128 * c + g * KT + k * 8,
+                 vb + (g * L::KSUB + k * 2048) / 16, idesc_o, (i | k) != 0 ? 1u : 0u);
+      if (!pair || c == 1) tc_commit_by(leader, &kv_free[b]);
+      if (t + 2 >= last) tc_commit_by(leader, &o_done[c]);
+      if (t + 2 < last) issue_qk(t + 2);
     }
-    const size_t to = (static_cast<size_t>(row) * qh + head) * D + d;
-    float v = l_all > 0.f ? o / l_all : 0.f;
-    if (gate) v *= sigmoid_f32(__half2float(gate[to]));
-    out[to] = __float2half_rn(v);
+    __syncwarp();
+  } else if (warp == SCALE_WARP) {
+    // ---------------- scales: times log2 e / sqrt(D) for keys, times the group's unit for values.
+    // All of a lane's are of one group.
+    constexpr int KS = KT * G / 32, VS = KT * GV / 32;
+    const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
+    float unit[GV];
+#pragma unroll
+    for (int g = 0; g < GV; ++g) unit[g] = __uint_as_float((127 + 29) << 23);
+    bool ok = true;
+    __half kraw[KS], vraw[VS];
+    auto load = [&](int s) {
+      const int key0 = (it.step_lo + s) * KT;
+      int page = pages[key0 >> 7];
+      if (!known || page < 0 || page >= num_pages) {
+        if (lane == 0) report_status(status, STATUS_BAD_INDEX, 0x50);
+        page = 0;
+      }
+      const size_t slot = static_cast<size_t>(page) * 128 + (key0 & 127);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int x = lane + 32 * i;
+        kraw[i] = ks[((slot + x / G) * kvh + h) * G + x % G];
+      }
+#pragma unroll
+      for (int i = 0; i < VS; ++i) {
+        const int x = lane + 32 * i;
+        vraw[i] = vs[((slot + x / GV) * kvh + h) * G + vpart * GV + x % GV];
+      }
+    };
+    if (steps > 0) load(0);
+    for (int s = 0; s < steps; ++s) {
+      const int b = s % NB, live = it.shared - (it.step_lo + s) * KT;
+      if (s >= NB)
+        ok = ok && mbar_wait(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, 0x600);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      float* sk = reinterpret_cast<float*>(smem + L::SCALE_OFF + b * L::SCALES);
+      float* sv = sk + KT * G;
+      float* su = sv + KT * GV;
+      // slots behind the shared keys may never have been written: they get no scale
+      uint32_t big = 0;                          // FP16 magnitudes are ordered as their bits
+#pragma unroll
+      for (int i = 0; i < VS; ++i) {
+        const uint32_t bits = __half_as_ushort(vraw[i]) & 0x7fffu;
+        if ((lane + 32 * i) / GV < live && bits < 0x7c00u) big = max(big, bits);
+      }
+#pragma unroll
+      for (int g = 0; g < GV; ++g) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, lane % GV == g ? big : 0u);
+        const float v = __half2float(__ushort_as_half(static_cast<unsigned short>(top)));
+        // v x unit in [16, 32) when chosen, below 128 as long as it is kept
+        if (v * unit[g] >= 128.f)
+          unit[g] = __uint_as_float((127 + 5 + 126 - (__float_as_uint(v) >> 23)) << 23);
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int x = lane + 32 * i, key = x / G, g = x % G;
+        sk[((key >> 1) * G + g) * 2 + (key & 1)] =
+            key < live ? __half2float(kraw[i]) * qscale : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < VS; ++i) {
+        const int x = lane + 32 * i, key = x / GV, g = x % GV;
+        sv[((key >> 1) * GV + g) * 2 + (key & 1)] =
+            key < live ? __half2float(vraw[i]) * unit[GV == 1 ? 0 : g] : 0.f;
+      }
+      if (lane < GV) su[lane] = unit[GV == 1 ? 0 : lane];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kv_full[b]);
+      if (s + 1 < steps) load(s + 1);
+    }
+  } else if (warp >= SOFTMAX_WARPS) {
+    // ---------------- keys and values: INT8 from global memory (PF steps ahead, in registers) to
+    // FP16 integers in swizzled tiles
+    constexpr int DQ = DQ_WARPS * 32;
+    constexpr int KI = KT * D / 16 / DQ, VI = KT * L::DV / 16 / DQ;
+    const int u = tid - SOFTMAX_WARPS * 32;
+    uint4 kraw[L::PF][KI], vraw[L::PF][VI];
+    bool ok = true;
+    auto load = [&](int s, uint4(&kr)[KI], uint4(&vr)[VI]) {
+      const int key0 = (it.step_lo + s) * KT;
+      int page = pages[key0 >> 7];
+      if (!known || page < 0 || page >= num_pages) page = 0;           // (reported by the scale warp)
+      const size_t slot = static_cast<size_t>(page) * 128 + (key0 & 127);
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const int x = u + i * DQ, key = x / (D / 16), c = x % (D / 16);
+        kr[i] = *reinterpret_cast<const uint4*>(kc + ((slot + key) * kvh + h) * D + c * 16);
+      }
+#pragma unroll
+      for (int i = 0; i < VI; ++i) {
+        const int x = u + i * DQ, key = x / (L::DV / 16), c = x % (L::DV / 16);
+        vr[i] = *reinterpret_cast<const uint4*>(vc + ((slot + key) * kvh + h) * D +
+                                                vpart * L::DV + c * 16);
+      }
+    };
+    auto place = [&](unsigned char* to, const uint4& raw, int key, int c) {
+      unsigned char* dst = to + (c / 4) * L::KSUB;
+      *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2)) = integers(raw.x, raw.y);
+      *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + 1)) = integers(raw.z, raw.w);
+    };
+#pragma unroll
+    for (int f = 0; f < L::PF; ++f)
+      if (f < steps) load(f, kraw[f], vraw[f]);
+    for (int s0 = 0; s0 < steps && ok; s0 += L::PF) {
+#pragma unroll
+      for (int f = 0; f < L::PF; ++f) {
+        const int s = s0 + f, b = s % NB;
+        if (s >= steps || !ok) break;
+        if (s >= NB)
+          ok = mbar_wait(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, s & 0xff);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        unsigned char* buf = smem + L::KV_OFF + b * (L::K_BYTES + L::V_BYTES);
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+          const int x = u + i * DQ;
+          place(buf, kraw[f][i], x / (D / 16), x % (D / 16));
+        }
+#pragma unroll
+        for (int i = 0; i < VI; ++i) {
+          const int x = u + i * DQ;
+          place(buf + L::K_BYTES, vraw[f][i], x / (L::DV / 16), x % (L::DV / 16));
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[b]);
+        if (s + L::PF < steps) load(s + L::PF, kraw[f], vraw[f]);
+      }
+    }
+  } else {
+    // ---------------- softmax: a thread per row
+    const int c = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
+    const int t = it.pair ? c : 0, local = t * P + r / rep;
+    const bool valid = r < P * rep && local < it.rows && known;
+    const int row = it.row + (valid ? local : 0);
+    const int sees = valid ? min(it.shared, row_pos[row] + 1) : 0;      // of the shared keys
+    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t tmem_s = tmem + 128 * c + lane_addr, tmem_oc = tmem_o + 128 * c + lane_addr;
+    float m_ref = -INFINITY, l_run = 0.f, unit[GV];
+    bool ok = true;
+    int mine = 0;                                                       // turns taken
+    for (int turn = c; turn < turns; turn += 2, ++mine) {
+      const int s = it.pair ? turn >> 1 : turn, b = s % NB;
+      // (the scales are the scale warp's plain stores: seen by whoever waits for them)
+      ok = __all_sync(0xffffffffu,
+                      mbar_wait(&s_full[c], mine & 1, status, STATUS_EPILOGUE_WAIT, s & 0xff) &&
+                          mbar_wait(&kv_full[b], (s / NB) & 1, status, STATUS_EPILOGUE_WAIT, 0x100));
+      if (!ok) break;
+      tc_fence_after();
+      const float* sk = reinterpret_cast<const float*>(smem + L::SCALE_OFF + b * L::SCALES);
+      const float* sv = sk + KT * G;
+      const float* su = sv + KT * GV;
+      const int vis = sees - (it.step_lo + s) * KT;
+      const bool whole = __all_sync(0xffffffffu, vis >= KT);
+      // ---- scores
+      float x[KT];
+#pragma unroll
+      for (int k0 = 0; k0 < KT; k0 += 16) {
+        uint32_t raw[G][16];
+#pragma unroll
+        for (int g = 0; g < G; ++g) tmem_ld_x16(tmem_s + g * KT + k0, raw[g]);
+        tc_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+          float2 v;
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const float2 w = *reinterpret_cast<const float2*>(sk + ((k0 + k) / 2 * G + g) * 2);
+            const float2 a = pair_at(raw[g][k], raw[g][k + 1]);
+            v = g == 0 ? mul2(a, w) : fma2(a, w, v);
+          }
+          x[k0 + k] = v.x;
+          x[k0 + k + 1] = v.y;
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+          if (k >= vis) x[k] = -INFINITY;
+      }
+      // ---- the reference follows the maximum when that is more than LAG above it
+      float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+      for (int k = 4; k < KT; ++k) top[k & 3] = fmaxf(top[k & 3], x[k]);
+      const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      const bool moves = m_tile > m_ref + LAG;                          // (from -inf: any score)
+      const float m_new = moves ? m_tile : m_ref;
+      float corr = moves ? ex2(m_ref - m_new) : 1.f;
+      l_run *= corr;
+      m_ref = m_new;
+      bool rescale = moves;
+      float fix[GV];
+#pragma unroll
+      for (int g = 0; g < GV; ++g) {
+        const float now = su[g];
+        fix[g] = corr;
+        if (mine > 0 && now != unit[g]) {        // powers of two
+          fix[g] *= now * __uint_as_float((254u << 23) - __float_as_uint(unit[g]));
+          rescale = true;
+        }
+        unit[g] = now;
+      }
+      if (mine > 0 && __any_sync(0xffffffffu, rescale)) {
+        // the product before this one is through: the scores came behind it
+#pragma unroll
+        for (int g = 0; g < GV; ++g)
+#pragma unroll 1
+          for (int d0 = 0; d0 < 64; d0 += 16) {
+            uint32_t o[16];
+            tmem_ld_x16(tmem_oc + g * 64 + d0, o);
+            tc_wait_ld();
+            uint32_t lo[8], hi[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              lo[i] = __float_as_uint(__uint_as_float(o[i]) * fix[g]);
+              hi[i] = __float_as_uint(__uint_as_float(o[8 + i]) * fix[g]);
+            }
+            tmem_st_x8(tmem_oc + g * 64 + d0, lo);
+            tmem_st_x8(tmem_oc + g * 64 + d0 + 8, hi);
+          }
+      }
+      // ---- weights
+      const float2 neg = make_float2(m_ref == -INFINITY ? 0.f : -m_ref,
+                                     m_ref == -INFINITY ? 0.f : -m_ref);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int k0 = 0; k0 < KT; k0 += 16) {
+        uint32_t packed[GV][8];
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+          float2 p = add2(make_float2(x[k0 + k], x[k0 + k + 1]), neg);
+          p.x = ex2(p.x);
+          p.y = ex2(p.y);
+          sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], p);
+#pragma unroll
+          for (int g = 0; g < GV; ++g) {
+            const float2 w = *reinterpret_cast<const float2*>(sv + ((k0 + k) / 2 * GV + g) * 2);
+            const float2 v = mul2(p, w);
+            const __half2 hv = __floats2half2_rn(v.x, v.y);
+            packed[g][k / 2] = *reinterpret_cast<const uint32_t*>(&hv);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < GV; ++g) tmem_st_x8(tmem_s + g * KT + k0 / 2, packed[g]);
+      }
+      sum[0] = add2(sum[0], sum[1]);
+      l_run += sum[0].x + sum[0].y;
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[c]);
+    }
+    // ---- this part of the rows' softmax
+    if (ok && mine > 0) {
+      ok = mbar_wait(&o_done[c], 0, status, STATUS_EPILOGUE_WAIT, 0x200);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    const bool some = ok && mine > 0;
+    const size_t at =
+        (static_cast<size_t>(valid ? info[row].y + (it.pair ? it.part : 2 * it.part + c) : 0)) * qh +
+        h * rep + r % rep;
+    float* to = part_o + at * D + vpart * L::DV;
+#pragma unroll
+    for (int g = 0; g < GV; ++g) {
+      const float back = some ? __uint_as_float((254u << 23) - __float_as_uint(unit[g])) : 0.f;
+#pragma unroll 1
+      for (int d0 = 0; d0 < 64; d0 += 16) {
+        uint32_t o[16];
+        if (some) {
+          tmem_ld_x16(tmem_oc + g * 64 + d0, o);
+          tc_wait_ld();
+        }
+        if (valid) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (some)
+              v = make_float4(__uint_as_float(o[i]) * back, __uint_as_float(o[i + 1]) * back,
+                              __uint_as_float(o[i + 2]) * back, __uint_as_float(o[i + 3]) * back);
+            *reinterpret_cast<float4*>(to + g * 64 + d0 + i) = v;
+          }
+        }
+      }
+    }
+    if (valid && vpart == 0) part_ml[at] = make_float2(some ? m_ref : -INFINITY, some ? l_run : 0.f);
   }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
+}
+
+template <int D>
+static int launch_prefix(const __half* q, const int* row_req, const int* row_pos,
+                         const int* page_table, int slots, int max_pages, const int8_t* kc,
+                         const int8_t* vc, const __half* ks, const __half* vs, const Item* items,
+                         int n_items, const SharedParts& parts, int qh, int kvh, int num_pages,
+                         cudaStream_t stream) {
+  using L = Shape<D>;
+  static const int slot = runtime_new_slot();
+  if (const int e = runtime_allow_smem(slot, prefix_kernel<D>, L::TOTAL)) return e;
+  launch_early(prefix_kernel<D>, dim3(n_items, kvh * L::PARTS), THREADS, L::TOTAL, stream, q,
+               row_req, row_pos, page_table, slots, max_pages, kc, vc, ks, vs, items, parts.rows,
+               const_cast<float*>(parts.o), const_cast<float2*>(parts.ml), qh, kvh, qh / kvh,
+               num_pages, runtime_status_ptr());
+  return static_cast<int>(cudaGetLastError());
 }
 
 }  // namespace sp
@@ -80,22 +560,43 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(
 
 using namespace orinfer;
 
+// Keys of a step, and rows of a tile: what a plan's items are counted in.
+extern "C" int orinfer_shared_step(int head_dim) { return head_dim > 128 ? 32 : 64; }
+
+// items: int32 [n_items, 8], see Item; rows_info: int32 [rows, 4] = (shared keys, first part, parts,
+// 0); parts: FP32 [all parts, query heads, D] and behind it [all parts, query heads, 2]; scratch: for
+// splits > 1, orinfer_attention_scratch_bytes.
 extern "C" int orinfer_attention_shared(
     const __half* q, const __half* gate, const int* row_req, const int* row_pos,
-    const int* page_table, int max_pages, const int8_t* kc, const int8_t* vc, const __half* ks,
-    const __half* vs, __half* out, int rows, int qh, int kvh, int head_dim, int num_pages,
-    cudaStream_t stream) {
+    const int* page_table, int slots, int max_pages, const int8_t* kc, const int8_t* vc,
+    const __half* ks, const __half* vs, __half* out, int rows, int qh, int kvh, int head_dim,
+    int num_pages, const int* items, int n_items, const int* rows_info, float* parts, int n_parts,
+    int splits, float* scratch, int context, cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (kvh <= 0 || qh % kvh || max_pages <= 0 || num_pages <= 0) return -1;
+  if (kvh <= 0 || qh % kvh || max_pages <= 0 || num_pages <= 0 || slots <= 0) return -1;
+  if (n_items < 0 || n_parts < 0 || (n_items > 0 && (!items || !parts)) || !rows_info) return -1;
+  if (splits < 1 || (splits > 1 && !scratch)) return -1;
+  if (((reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc) |
+        reinterpret_cast<uintptr_t>(parts)) & 15) != 0)
+    return -1;
   const int rep = qh / kvh;
   if (rep != 1 && rep != 2 && rep != 4 && rep != 8 && !(rep == 5 && head_dim == 128)) return -1;
   if (runtime_ensure_init() != cudaSuccess) return -2;
-#define CASE(D)                                                                                 \
-  if (head_dim == D)                                                                            \
-    launch_early(sp::rows_kernel<D>, dim3(rows, qh), sp::WARPS * 32, 0, stream, q, gate,        \
-                 row_req, row_pos, page_table, max_pages, kc, vc, ks, vs, out, qh, kvh, num_pages, \
-                 runtime_status_ptr());
-  CASE(64) else CASE(128) else CASE(256) else return -1;
+  SharedParts shared;
+  shared.rows = reinterpret_cast<const int4*>(rows_info);
+  shared.o = parts;
+  shared.ml = reinterpret_cast<const float2*>(parts + static_cast<size_t>(n_parts) * qh * head_dim);
+  const sp::Item* list = reinterpret_cast<const sp::Item*>(items);
+  if (n_items > 0) {
+    int e = -1;
+#define CASE(D)                                                                                  \
+  if (head_dim == D)                                                                             \
+    e = sp::launch_prefix<D>(q, row_req, row_pos, page_table, slots, max_pages, kc, vc, ks, vs,  \
+                             list, n_items, shared, qh, kvh, num_pages, stream);
+    CASE(64) CASE(128) CASE(256)
 #undef CASE
-  return static_cast<int>(cudaGetLastError());
+    if (e != 0) return e;
+  }
+  return attention_own_keys(q, gate, row_req, row_pos, page_table, max_pages, kc, vc, ks, vs, out,
+                            rows, qh, kvh, head_dim, splits, scratch, context, shared, stream);
 }

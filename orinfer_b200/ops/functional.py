@@ -241,7 +241,7 @@ class SharedPrefix:
     same pages as far as their first ``keys`` keys lie on them (whole pages, as ``fork_pages`` and
     the prefix cache share them).  Groups do not overlap; rows of no group share nothing.
     ``max_kv_len`` bounds the keys that any row sees while the plan is in use, so that one plan
-    serves the steps of a decode loop."""
+    serves the steps of a decode loop.  It holds the call's workspace: one stream at a time."""
 
     def __init__(self, groups: Sequence[Tuple[int, int, int]], rows: int, *, qh: int, kvh: int,
                  head_dim: int, max_kv_len: int, device):
@@ -257,8 +257,77 @@ class SharedPrefix:
             _need(not any(taken[first:first + n]), "a row is in two groups")
             taken[first:first + n] = [True] * n
         self.rows, self.qh, self.kvh, self.head_dim = rows, qh, kvh, head_dim
-        self.groups = [(int(f), int(n), int(k)) for f, n, k in groups if n > 0 and k > 0]
-        self.max_kv_len, self.device = max_kv_len, torch.device(device)
+        self.device = torch.device(device)
+        groups = [(int(f), int(n), int(k)) for f, n, k in groups if n > 0 and k > 0]
+        self.longest = max((k for _, _, k in groups), default=0)
+        items, info, self.parts = self._split(groups)
+        put = lambda v: torch.tensor(v, dtype=torch.int32, device=self.device)
+        self.items = put(items) if items else None
+        self.info = put(info if info else [[0] * 4])
+        f32 = lambda n: torch.empty(n, dtype=torch.float32, device=self.device) if n else None
+        self.part_buffer = f32(self.parts * qh * (head_dim + 2))
+        # the own keys, by the row kernels
+        self.own_keys = max_kv_len - min((i[0] for i in info), default=0)
+        self.splits = attention_splits(max(1, self.own_keys), max(1, rows), kvh)
+        self.scratch = f32(rows * qh * self.splits * (head_dim + 2)) if self.splits > 1 else None
+        self._args = (ptr(self.items), len(items), ptr(self.info), ptr(self.part_buffer),
+                      self.parts, self.splits, ptr(self.scratch), max(1, self.own_keys))
+
+    # Microseconds of a step of keys for two tiles and for one, of a CTA besides its steps, and of a
+    # megabyte of parts to be written and read.
+    PAIR_US, SINGLE_US, CTA_US, PART_US = 1.1, 0.6, 4.0, 0.4
+
+    def _split(self, groups):
+        """Which CTAs take which rows and keys: (items, (shared keys, first part, parts, 0) of every
+        row, parts in all).  A unit is one or two tiles of rows; the units' keys are cut so that the
+        CTAs fill their waves and the longest of them ends soonest."""
+        step = native.lib().orinfer_shared_step(self.head_dim)
+        rep = self.qh // self.kvh
+        per = 128 // rep                               # rows of a tile
+        units, info = [], [[0, 0, 0, 0] for _ in range(self.rows)]
+        for first, n, keys in groups:
+            at = first
+            while at < first + n:
+                left = first + n - at
+                pair = left > per
+                took = min(left, 2 * per if pair else per)
+                units.append((at, took, (keys + step - 1) // step, keys, pair))
+                at += took
+        if not units:
+            return [], info, 0
+        columns = self.kvh * max(1, self.head_dim // 128)
+        cost = [s * (self.PAIR_US if pair else self.SINGLE_US) for _, _, s, _, pair in units]
+        bytes_of = self.qh * self.head_dim * 4e-6      # a part of a row, in megabytes
+
+        def cut(limit):
+            """Parts of every unit where no CTA's steps take longer than ``limit``."""
+            return [min(u[2], max(1, -(-c // limit))) for c, u in zip(cost, units)]
+
+        best = None
+        for waves in range(-(-len(units) * columns // 148), -(-len(units) * columns // 148) + 3):
+            room = max(len(units), waves * 148 // columns)
+            lo, hi = 0.0, max(cost)
+            for _ in range(30):
+                mid = (lo + hi) / 2
+                lo, hi = (lo, mid) if mid > 0 and sum(cut(mid)) <= room else (mid, hi)
+            for limit in {hi, hi * 1.25, hi * 1.6, hi * 2.2, hi * 4, max(cost)}:
+                parts = [int(x) for x in cut(limit)]
+                mb = sum(p * u[1] * (1 if u[4] else 2) for p, u in zip(parts, units)) * bytes_of
+                longest = max(c / p for c, p in zip(cost, parts))
+                took = -(-sum(parts) * columns // 148)
+                us = took * (longest + self.CTA_US) + mb * self.PART_US
+                if best is None or us < best[0]:
+                    best = us, parts
+        items, total = [], 0
+        for (at, n, steps, keys, pair), parts in zip(units, best[1]):
+            records = parts if pair else 2 * parts     # one tile leaves one for each context
+            for i in range(n):
+                info[at + i] = [keys, total + i * records, records, 0]
+            total += n * records
+            items += [[at, n, steps * p // parts, steps * (p + 1) // parts, keys, p, int(pair), 0]
+                      for p in range(parts)]
+        items.sort(key=lambda x: (x[2] - x[3]) * (1 + x[6]))       # the longest first
+        return items, info, total
 
 
 def attention_shared(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: torch.Tensor,
@@ -292,11 +361,13 @@ def attention_shared(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: tor
     else:
         _need(out.dtype == torch.float16 and out.is_contiguous() and out.numel() == q.numel(),
               "out: contiguous FP16 [rows, heads * D]")
+    _need(plan.longest <= page_table.shape[1] * 128, "more shared keys than the table has pages")
+    _need(q.device == plan.info.device, "the plan is for another device")
     check(native.lib().orinfer_attention_shared(
-        ptr(q), ptr(gate), ptr(row_req), ptr(row_pos), ptr(page_table), page_table.shape[1],
-        ptr(kcache), ptr(vcache), ptr(kscale), ptr(vscale), ptr(out), n, qh, plan.kvh, d, pages,
-        stream()), "attention_shared")
-    count_launches(1)
+        ptr(q), ptr(gate), ptr(row_req), ptr(row_pos), ptr(page_table), page_table.shape[0],
+        page_table.shape[1], ptr(kcache), ptr(vcache), ptr(kscale), ptr(vscale), ptr(out), n, qh,
+        plan.kvh, d, pages, *plan._args, stream()), "attention_shared")
+    count_launches((plan.items is not None) + (2 if plan.splits > 1 else 1))
     return out
 
 

@@ -84,7 +84,9 @@ def _load() -> ctypes.CDLL:
         "orinfer_gdn_gated_norm": ([P, P, I, P, c_float, I, I, I, I, P, P], I),
         "orinfer_attention_prefill_parts": ([I, I], I),
         "orinfer_attention_prefill": ([P, P, P, I, I, I, P, I, P, P, P, P, P, I, I, I, I, I, P], I),
-        "orinfer_attention_shared": ([P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, P], I),
+        "orinfer_shared_step": ([I], I),
+        "orinfer_attention_shared": ([P, P, P, P, P, I, I, P, P, P, P, P, I, I, I, I, I, P, I, P, P,
+                                      I, I, P, I, P], I),
         "orinfer_process_logits": ([P, c_longlong, P, c_longlong, I, P, P, P, P, P, P, P, I, P,
                                     c_longlong, P, I, c_float, P, c_longlong, P, I, I, P], I),
         "orinfer_fork_work": ([I, I], c_size_t),
