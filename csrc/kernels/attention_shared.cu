@@ -15,9 +15,9 @@
 // would add one each and another 40 %.  P_g is taken under a power of two per group that follows the
 // value scales, so that it stays among FP16's normal numbers.
 //
-// Two contexts of four softmax warps (a thread per row) take turns with the tensor core: two tiles
-// that share every step's keys, or, where a group has one tile left, one tile whose steps they take
-// in turn, each with a softmax of its own.
+// Two contexts of eight softmax warps (two threads per row, each with half of a step's keys) take
+// turns with the tensor core: two tiles that share every step's keys, or, where a group has one tile
+// left, one tile whose steps they take in turn, each with a softmax of its own.
 #include "api.h"
 #include "attention_shared.h"
 #include "common.cuh"
@@ -26,8 +26,7 @@ namespace orinfer {
 namespace sp {
 
 constexpr int TILE = 128;                        // rows of a tile: positions x query heads
-// Fourteen warps: with at most four on a scheduler each thread has 128 registers.
-constexpr int SOFTMAX_WARPS = 8, DQ_WARPS = 4;
+constexpr int SOFTMAX_WARPS = 16, DQ_WARPS = 4;
 constexpr int MMA_WARP = SOFTMAX_WARPS + DQ_WARPS, SCALE_WARP = MMA_WARP + 1;
 constexpr int THREADS = (SCALE_WARP + 1) * 32;
 constexpr float LAG = 8.f;                       // of the weights' reference, binades
@@ -39,15 +38,17 @@ struct Shape {
   static constexpr int GV = DV / 64, PARTS = D / DV;
   static constexpr int KT = D > 128 ? 32 : 64;   // keys of a step: at most 128 score columns
   static constexpr int NB = D > 128 ? 3 : 4;     // buffers of keys and values
-  static constexpr int PF = 2;                   // steps whose bytes are in flight to registers
   static constexpr int QSUB = TILE * 128, KSUB = KT * 128;     // bytes of 64 channels of a tile
   static constexpr int K_BYTES = G * KSUB, V_BYTES = GV * KSUB;
   static constexpr int Q_OFF = 0;                // two tiles
   static constexpr int KV_OFF = 2 * G * QSUB;
   static constexpr int SCALE_OFF = KV_OFF + NB * (K_BYTES + V_BYTES);
   static constexpr int SCALES = KT * (G + GV) * 4 + 16;        // key and value scales, units
-  static constexpr int BAR_OFF = SCALE_OFF + NB * SCALES;
+  static constexpr int MAX_OFF = SCALE_OFF + NB * SCALES;      // [2 contexts][2 turns][2 halves][128]
+  static constexpr int BAR_OFF = MAX_OFF + 8 * TILE * 4;
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;
+  static constexpr int OUT_WARP = 4096;          // of a warp's results on their way out (in the ring)
+  static_assert(SOFTMAX_WARPS * OUT_WARP <= NB * (K_BYTES + V_BYTES), "results fit the ring");
   static_assert(TOTAL <= 227 * 1024, "exceeds the shared memory of one CTA");
   static_assert(SCALES % 16 == 0, "scales are read sixteen bytes at a time");
 };
@@ -92,12 +93,72 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+// Sixteen TMEM lanes as the fragments of a warp's matrix product: per eight columns lane (g = lane /
+// 4, t = lane % 4) holds columns 2t and 2t + 1 of rows g and g + 8.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {       // 32 columns
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[8]) {        // 16 columns
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[8]) {  // 16 columns
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
       : "memory");
 }
+// The same rows and columns as pairs of FP16 values, half as many columns: per four columns lane (g,
+// t) holds column t of rows g and g + 8.
+__device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t (&r)[8]) { // 16 columns
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t (&r)[4]) { // 8 columns
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+// mbar_wait for warps that wait long: suspended for up to 20 us at a time, so that sixteen of them do
+// not take the issue slots of those that work.
+__device__ __forceinline__ bool wait_long(uint64_t* bar, uint32_t parity, int* status, int code,
+                                          int detail) {
+  long long start = 0, limit = 0;
+  for (uint32_t spins = 1;; ++spins) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
+        : "memory");
+    if (done) return true;
+    if ((spins & 255u) == 0) {
+      if (limit == 0) {
+        limit = wait_limit(status);
+        start = clock64();
+      } else if (clock64() - start > limit) {
+        report_status(status, code, detail);
+        return false;
+      }
+    }
+  }
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -128,7 +189,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     const Item* items, const int4* info, float* __restrict__ part_o, float2* __restrict__ part_ml,
     int qh, int kvh, int rep, int num_pages, int* status) {
   using L = Shape<D>;
-  constexpr int G = L::G, GV = L::GV, KT = L::KT, NB = L::NB;
+  constexpr int G = L::G, GV = L::GV, KT = L::KT, KH = KT / 2, NB = L::NB;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
@@ -137,7 +198,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
   uint64_t* s_full = bars + 2 * NB;      // [2] scores of a context
   uint64_t* p_ready = s_full + 2;        // [2] its weights (an arrival per warp)
   uint64_t* o_done = s_full + 4;         // [2] its last product is through
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 6);
+  uint64_t* q_full = s_full + 6;         // the query rows are there (an arrival per softmax warp)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 7);
 
   const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
   grid_wait();
@@ -158,39 +220,16 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     }
     for (int c = 0; c < 2; ++c) {
       mbar_init(&s_full[c], 1);
-      mbar_init(&p_ready[c], 4);
+      mbar_init(&p_ready[c], SOFTMAX_WARPS / 2);
       mbar_init(&o_done[c], 1);
     }
+    mbar_init(q_full, SOFTMAX_WARPS);
     mbar_fence_init();
   }
   if (warp == MMA_WARP) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  // ---- the query rows, 16 bytes at a time, zeros where a tile has none
-  {
-    const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-    constexpr int CPR = D / 8;                   // 16-byte pieces of a row
-    for (int i = tid; i < tiles * TILE * CPR; i += THREADS) {
-      const int m = i / CPR, c = i % CPR, t = m / TILE, r = m % TILE;
-      const int row = t * P + r / rep;
-      __align__(16) __half v[8];
-      *reinterpret_cast<uint4*>(v) = make_uint4(0, 0, 0, 0);
-      if (r < P * rep && row < it.rows) {
-        const __half* from = q + (static_cast<size_t>(it.row + row) * qh + h * rep + r % rep) * D +
-                             c * 8;
-        if (wide) {
-          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(from);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = from[k];
-        }
-      }
-      *reinterpret_cast<uint4*>(smem + L::Q_OFF + (t * G + c / 8) * L::QSUB + swz128(r, c % 8)) =
-          *reinterpret_cast<const uint4*>(v);
-    }
-  }
-  fence_proxy_async();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -207,12 +246,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     const uint64_t kd = umma_desc(smem_u32(smem + L::KV_OFF), 16, 1024);
     const uint64_t vd = umma_desc(smem_u32(smem + L::KV_OFF + L::K_BYTES), L::KSUB, 1024);
     const int last = warp_same(turns), pair = warp_same(it.pair);
-    bool ok = true;
+    bool ok = __all_sync(0xffffffffu, wait_long(q_full, 0, status, STATUS_MMA_WAIT, 0x300));
     auto step_of = [&](int t) { return pair ? t >> 1 : t; };
     auto issue_qk = [&](int t) {
       const int c = t & 1, s = step_of(t), b = s % NB;
       if (ok)
-        ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[b], (s / NB) & 1, status, STATUS_MMA_WAIT,
+        ok = __all_sync(0xffffffffu, wait_long(&kv_full[b], (s / NB) & 1, status, STATUS_MMA_WAIT,
                                                0x400 | (s & 0xff)));
       tc_fence_after();
       if (!ok) return;
@@ -230,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     if (last > 1) issue_qk(1);
     for (int t = 0; t < last && ok; ++t) {
       const int c = t & 1, i = t >> 1, b = step_of(t) % NB;
-      ok = __all_sync(0xffffffffu, mbar_wait(&p_ready[c], i & 1, status, STATUS_MMA_WAIT,
+      ok = __all_sync(0xffffffffu, wait_long(&p_ready[c], i & 1, status, STATUS_MMA_WAIT,
                                              0x500 | (i & 0xff)));
       tc_fence_after();
       if (!ok) break;
@@ -239,7 +278,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       for (int g = 0; g < GV; ++g)
 #pragma unroll
         for (int k = 0; k < KT / 16; ++k)
-          mma_ts(leader, tmem_o + 128 * c + g * 64, tmem + 128 * c + g * KT + k * 8,
+          mma_ts(leader, tmem_o + 128 * c + g * 64,
+                 tmem + 128 * c + g * KT + k / (KH / 16) * KH + k % (KH / 16) * 8,
                  vb + (g * L::KSUB + k * 2048) / 16, idesc_o, (i | k) != 0 ? 1u : 0u);
       if (!pair || c == 1) tc_commit_by(leader, &kv_free[b]);
       if (t + 2 >= last) tc_commit_by(leader, &o_done[c]);
@@ -279,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     for (int s = 0; s < steps; ++s) {
       const int b = s % NB, live = it.shared - (it.step_lo + s) * KT;
       if (s >= NB)
-        ok = ok && mbar_wait(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, 0x600);
+        ok = ok && wait_long(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, 0x600);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       float* sk = reinterpret_cast<float*>(smem + L::SCALE_OFF + b * L::SCALES);
@@ -318,221 +358,355 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       if (s + 1 < steps) load(s + 1);
     }
   } else if (warp >= SOFTMAX_WARPS) {
-    // ---------------- keys and values: INT8 from global memory (PF steps ahead, in registers) to
-    // FP16 integers in swizzled tiles
+    // ---------------- keys and values: INT8 from global memory (a step ahead, in registers) to FP16
+    // integers in swizzled tiles
     constexpr int DQ = DQ_WARPS * 32;
     constexpr int KI = KT * D / 16 / DQ, VI = KT * L::DV / 16 / DQ;
     const int u = tid - SOFTMAX_WARPS * 32;
-    uint4 kraw[L::PF][KI], vraw[L::PF][VI];
-    bool ok = true;
-    auto load = [&](int s, uint4(&kr)[KI], uint4(&vr)[VI]) {
+    uint4 kraw[KI], vraw[VI];
+    auto load = [&](int s) {
       const int key0 = (it.step_lo + s) * KT;
       int page = pages[key0 >> 7];
-      if (!known || page < 0 || page >= num_pages) page = 0;           // (reported by the scale warp)
+      if (!known || page < 0 || page >= num_pages) page = 0;           // (the scale warp reports it)
       const size_t slot = static_cast<size_t>(page) * 128 + (key0 & 127);
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
         const int x = u + i * DQ, key = x / (D / 16), c = x % (D / 16);
-        kr[i] = *reinterpret_cast<const uint4*>(kc + ((slot + key) * kvh + h) * D + c * 16);
+        kraw[i] = *reinterpret_cast<const uint4*>(kc + ((slot + key) * kvh + h) * D + c * 16);
       }
 #pragma unroll
       for (int i = 0; i < VI; ++i) {
         const int x = u + i * DQ, key = x / (L::DV / 16), c = x % (L::DV / 16);
-        vr[i] = *reinterpret_cast<const uint4*>(vc + ((slot + key) * kvh + h) * D +
-                                                vpart * L::DV + c * 16);
+        vraw[i] = *reinterpret_cast<const uint4*>(vc + ((slot + key) * kvh + h) * D +
+                                                  vpart * L::DV + c * 16);
       }
     };
     auto place = [&](unsigned char* to, const uint4& raw, int key, int c) {
+      // lanes of every other group of channels store their second half first: eight lanes that
+      // store together then meet on no bank
       unsigned char* dst = to + (c / 4) * L::KSUB;
-      *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2)) = integers(raw.x, raw.y);
-      *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + 1)) = integers(raw.z, raw.w);
+      const bool swap = c & 4;
+      const uint4 lo = integers(swap ? raw.z : raw.x, swap ? raw.w : raw.y);
+      const uint4 hi = integers(swap ? raw.x : raw.z, swap ? raw.y : raw.w);
+      *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + swap)) = lo;
+      *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + !swap)) = hi;
     };
+    bool ok = true;
+    if (steps > 0) load(0);
+    for (int s = 0; s < steps; ++s) {
+      const int b = s % NB;
+      if (s >= NB)
+        ok = wait_long(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, s & 0xff);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      unsigned char* buf = smem + L::KV_OFF + b * (L::K_BYTES + L::V_BYTES);
 #pragma unroll
-    for (int f = 0; f < L::PF; ++f)
-      if (f < steps) load(f, kraw[f], vraw[f]);
-    for (int s0 = 0; s0 < steps && ok; s0 += L::PF) {
-#pragma unroll
-      for (int f = 0; f < L::PF; ++f) {
-        const int s = s0 + f, b = s % NB;
-        if (s >= steps || !ok) break;
-        if (s >= NB)
-          ok = mbar_wait(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, s & 0xff);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        unsigned char* buf = smem + L::KV_OFF + b * (L::K_BYTES + L::V_BYTES);
-#pragma unroll
-        for (int i = 0; i < KI; ++i) {
-          const int x = u + i * DQ;
-          place(buf, kraw[f][i], x / (D / 16), x % (D / 16));
-        }
-#pragma unroll
-        for (int i = 0; i < VI; ++i) {
-          const int x = u + i * DQ;
-          place(buf + L::K_BYTES, vraw[f][i], x / (L::DV / 16), x % (L::DV / 16));
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[b]);
-        if (s + L::PF < steps) load(s + L::PF, kraw[f], vraw[f]);
+      for (int i = 0; i < KI; ++i) {
+        const int x = u + i * DQ;
+        place(buf, kraw[i], x / (D / 16), x % (D / 16));
       }
+#pragma unroll
+      for (int i = 0; i < VI; ++i) {
+        const int x = u + i * DQ;
+        place(buf + L::K_BYTES, vraw[i], x / (L::DV / 16), x % (L::DV / 16));
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kv_full[b]);
+      if (s + 1 < steps) load(s + 1);
     }
   } else {
-    // ---------------- softmax: a thread per row
-    const int c = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
-    const int t = it.pair ? c : 0, local = t * P + r / rep;
-    const bool valid = r < P * rep && local < it.rows && known;
-    const int row = it.row + (valid ? local : 0);
-    const int sees = valid ? min(it.shared, row_pos[row] + 1) : 0;      // of the shared keys
+    // ---------------- softmax: two threads per row, each with half of a step's keys and, of what is
+    // done to O, half of the channels
+    const int c = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, r = quad * 32 + lane;
+    constexpr int CH = L::DV / 2;                // channels of a half, all of one group
+    const int gh = GV == 2 ? half : 0;           // that group
+    // ---- the query rows, 16 bytes at a time, zeros where a tile has none
+    {
+      const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+      constexpr int CPR = D / 8, BATCH = 8;      // 16-byte pieces of a row; loads in flight
+      for (int i0 = tid; i0 < tiles * TILE * CPR; i0 += BATCH * SOFTMAX_WARPS * 32) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int i = i0 + k * SOFTMAX_WARPS * 32, m = i / CPR, t = m / TILE, qr = m % TILE;
+          const int row = t * P + qr / rep;
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (t < tiles && qr < P * rep && row < it.rows) {
+            const __half* from =
+                q + (static_cast<size_t>(it.row + row) * qh + h * rep + qr % rep) * D + i % CPR * 8;
+            if (wide) {
+              v[k] = *reinterpret_cast<const uint4*>(from);
+            } else {
+              const unsigned short* f = reinterpret_cast<const unsigned short*>(from);
+              v[k] = make_uint4(f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16,
+                                f[6] | f[7] << 16);
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int i = i0 + k * SOFTMAX_WARPS * 32, m = i / CPR, t = m / TILE, qr = m % TILE;
+          if (t < tiles)
+            *reinterpret_cast<uint4*>(smem + L::Q_OFF + (t * G + i % CPR / 8) * L::QSUB +
+                                      swz128(qr, i % CPR % 8)) = v[k];
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    const int t = it.pair ? c : 0;
+    // TMEM hands scores out as fragments: a thread holds columns 2 qt and 2 qt + 1 of every eight, of
+    // rows qg + 8 i, so that each scale that it loads serves four rows.  (A row per thread loads
+    // all scales for itself: 64 rows behind 16384 keys, 32 / 4 heads of 128, 46 us with four rows
+    // of a warp's lanes each against 27.)
+    const int qg = lane >> 2, qt = lane & 3;
+    constexpr int PAIRS = KH / 8;                // pairs of keys of a thread
+    auto row_of = [&](int tr) {                  // of row `tr` of the tile, or none
+      return tr < P * rep && t * P + tr / rep < it.rows && known ? it.row + t * P + tr / rep : -1;
+    };
+    int sees[4];                                 // shared keys that its rows see
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row_of(quad * 32 + qg + 8 * i);
+      sees[i] = (row < 0 ? 0 : min(it.shared, row_pos[row] + 1)) - half * KH - 2 * qt;
+    }
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t tmem_s = tmem + 128 * c + lane_addr, tmem_oc = tmem_o + 128 * c + lane_addr;
-    float m_ref = -INFINITY, l_run = 0.f, unit[GV];
+    const uint32_t tmem_s = tmem + 128 * c + half * KH + lane_addr;
+    const uint32_t tmem_oc = tmem_o + 128 * c + half * CH + lane_addr;
+    constexpr uint32_t LANES16 = 16u << 16;
+    // maxima of the two halves, double buffered: a slot is rewritten two exchanges later
+    float* row_max = reinterpret_cast<float*>(smem + L::MAX_OFF) + c * 4 * TILE + quad * 32;
+    auto meet = [&]() {                          // the two warps of these rows
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + c * 4 + quad) : "memory");
+    };
+    auto mine_of = [&](const float(&v)[4]) {     // row qg + 8 qt's
+      return qt < 2 ? (qt == 0 ? v[0] : v[1]) : (qt == 2 ? v[2] : v[3]);
+    };
+    // where this lane's row goes at the end (on the way out a row per lane)
+    const int row = row_of(r);
+    const int part = row < 0 ? -1 : info[row].y + (it.pair ? it.part : 2 * it.part + c);
+    float m_ref[4], l_run[4], unit = 1.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m_ref[i] = -INFINITY;
+      l_run[i] = 0.f;
+    }
     bool ok = true;
-    int mine = 0;                                                       // turns taken
+    int mine = 0;                                // turns taken
     for (int turn = c; turn < turns; turn += 2, ++mine) {
       const int s = it.pair ? turn >> 1 : turn, b = s % NB;
       // (the scales are the scale warp's plain stores: seen by whoever waits for them)
-      ok = __all_sync(0xffffffffu,
-                      mbar_wait(&s_full[c], mine & 1, status, STATUS_EPILOGUE_WAIT, s & 0xff) &&
-                          mbar_wait(&kv_full[b], (s / NB) & 1, status, STATUS_EPILOGUE_WAIT, 0x100));
-      if (!ok) break;
+      ok = ok && wait_long(&s_full[c], mine & 1, status, STATUS_EPILOGUE_WAIT, s & 0xff) &&
+           wait_long(&kv_full[b], (s / NB) & 1, status, STATUS_EPILOGUE_WAIT, 0x100);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {                                 // a warp that gave up still meets its partner
+        meet();
+        continue;
+      }
       tc_fence_after();
+      // scales by pairs of keys and groups: those of this thread's pair `j`
       const float* sk = reinterpret_cast<const float*>(smem + L::SCALE_OFF + b * L::SCALES);
       const float* sv = sk + KT * G;
       const float* su = sv + KT * GV;
-      const int vis = sees - (it.step_lo + s) * KT;
-      const bool whole = __all_sync(0xffffffffu, vis >= KT);
+      const int key0 = (it.step_lo + s) * KT;
+      bool whole = true;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) whole = whole && sees[i] - key0 >= KH;
+      whole = __all_sync(0xffffffffu, whole);
       // ---- scores
-      float x[KT];
+      float2 x[4][PAIRS];
 #pragma unroll
-      for (int k0 = 0; k0 < KT; k0 += 16) {
-        uint32_t raw[G][16];
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t raw[G][KH / 2];
 #pragma unroll
-        for (int g = 0; g < G; ++g) tmem_ld_x16(tmem_s + g * KT + k0, raw[g]);
+        for (int g = 0; g < G; ++g) tmem_ld_frag(tmem_s + hf * LANES16 + g * KT, raw[g]);
         tc_wait_ld();
 #pragma unroll
-        for (int k = 0; k < 16; k += 2) {
-          float2 v;
+        for (int j = 0; j < PAIRS; ++j) {
+          const float2* w =
+              reinterpret_cast<const float2*>(sk) + (half * (KH / 2) + 4 * j + qt) * G;
+          float2 wg[G];
+          if (G == 1) {
+            wg[0] = w[0];
+          } else {
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            const float2 w = *reinterpret_cast<const float2*>(sk + ((k0 + k) / 2 * G + g) * 2);
-            const float2 a = pair_at(raw[g][k], raw[g][k + 1]);
-            v = g == 0 ? mul2(a, w) : fma2(a, w, v);
+            for (int g = 0; g < G; g += 2) {
+              const float4 v = *reinterpret_cast<const float4*>(w + g);
+              wg[g] = make_float2(v.x, v.y);
+              wg[(g + 1) % G] = make_float2(v.z, v.w);
+            }
           }
-          x[k0 + k] = v.x;
-          x[k0 + k + 1] = v.y;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float2 v;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const float2 a = pair_at(raw[g][4 * j + 2 * i], raw[g][4 * j + 2 * i + 1]);
+              v = g == 0 ? mul2(a, wg[0]) : fma2(a, wg[g], v);
+            }
+            x[2 * hf + i][j] = v;
+          }
         }
       }
       if (!whole) {
 #pragma unroll
-        for (int k = 0; k < KT; ++k)
-          if (k >= vis) x[k] = -INFINITY;
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < PAIRS; ++j) {
+            if (8 * j >= sees[i] - key0) x[i][j].x = -INFINITY;
+            if (8 * j + 1 >= sees[i] - key0) x[i][j].y = -INFINITY;
+          }
       }
       // ---- the reference follows the maximum when that is more than LAG above it
-      float top[4] = {x[0], x[1], x[2], x[3]};
+      float top[4];
 #pragma unroll
-      for (int k = 4; k < KT; ++k) top[k & 3] = fmaxf(top[k & 3], x[k]);
-      const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      const bool moves = m_tile > m_ref + LAG;                          // (from -inf: any score)
-      const float m_new = moves ? m_tile : m_ref;
-      float corr = moves ? ex2(m_ref - m_new) : 1.f;
-      l_run *= corr;
-      m_ref = m_new;
-      bool rescale = moves;
-      float fix[GV];
+      for (int i = 0; i < 4; ++i) {
+        top[i] = fmaxf(x[i][0].x, x[i][0].y);
 #pragma unroll
-      for (int g = 0; g < GV; ++g) {
-        const float now = su[g];
-        fix[g] = corr;
-        if (mine > 0 && now != unit[g]) {        // powers of two
-          fix[g] *= now * __uint_as_float((254u << 23) - __float_as_uint(unit[g]));
-          rescale = true;
-        }
-        unit[g] = now;
+        for (int j = 1; j < PAIRS; ++j) top[i] = fmaxf(top[i], fmaxf(x[i][j].x, x[i][j].y));
       }
-      if (mine > 0 && __any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+      float* slot = row_max + (mine & 1) * 2 * TILE;
+      slot[half * TILE + qg + 8 * qt] = mine_of(top);
+      meet();
+      const float now = su[gh];                  // units are powers of two
+      const float same = mine > 0 && now != unit
+                             ? now * __uint_as_float((254u << 23) - __float_as_uint(unit))
+                             : 1.f;
+      bool moves = same != 1.f;
+      float fix[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float m_tile = fmaxf(top[i], slot[(1 - half) * TILE + qg + 8 * i]);
+        fix[i] = same;
+        if (m_tile > m_ref[i] + LAG) {           // (from -inf: any score)
+          const float corr = ex2(m_ref[i] - m_tile);
+          l_run[i] *= corr;
+          fix[i] *= corr;
+          m_ref[i] = m_tile;
+          moves = true;
+        }
+      }
+      unit = now;
+      if (mine > 0 && __any_sync(0xffffffffu, moves)) {
         // the product before this one is through: the scores came behind it
-#pragma unroll
-        for (int g = 0; g < GV; ++g)
 #pragma unroll 1
-          for (int d0 = 0; d0 < 64; d0 += 16) {
-            uint32_t o[16];
-            tmem_ld_x16(tmem_oc + g * 64 + d0, o);
+        for (int hf = 0; hf < 2; ++hf) {
+          const float f0 = hf == 0 ? fix[0] : fix[2], f1 = hf == 0 ? fix[1] : fix[3];
+#pragma unroll 1
+          for (int d0 = 0; d0 < CH; d0 += 16) {
+            uint32_t o[8];
+            tmem_ld_frag(tmem_oc + hf * LANES16 + d0, o);
             tc_wait_ld();
-            uint32_t lo[8], hi[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              lo[i] = __float_as_uint(__uint_as_float(o[i]) * fix[g]);
-              hi[i] = __float_as_uint(__uint_as_float(o[8 + i]) * fix[g]);
-            }
-            tmem_st_x8(tmem_oc + g * 64 + d0, lo);
-            tmem_st_x8(tmem_oc + g * 64 + d0 + 8, hi);
+            for (int i = 0; i < 8; ++i)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * (i & 2 ? f1 : f0));
+            tmem_st_frag(tmem_oc + hf * LANES16 + d0, o);
           }
+        }
       }
       // ---- weights
-      const float2 neg = make_float2(m_ref == -INFINITY ? 0.f : -m_ref,
-                                     m_ref == -INFINITY ? 0.f : -m_ref);
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      float2 w[PAIRS][GV];
 #pragma unroll
-      for (int k0 = 0; k0 < KT; k0 += 16) {
-        uint32_t packed[GV][8];
+      for (int j = 0; j < PAIRS; ++j) {
+        const float2* from =
+            reinterpret_cast<const float2*>(sv) + (half * (KH / 2) + 4 * j + qt) * GV;
+        if (GV == 1) {
+          w[j][0] = from[0];
+        } else {
+          const float4 v = *reinterpret_cast<const float4*>(from);
+          w[j][0] = make_float2(v.x, v.y);
+          w[j][GV - 1] = make_float2(v.z, v.w);
+        }
+      }
 #pragma unroll
-        for (int k = 0; k < 16; k += 2) {
-          float2 p = add2(make_float2(x[k0 + k], x[k0 + k + 1]), neg);
-          p.x = ex2(p.x);
-          p.y = ex2(p.y);
-          sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], p);
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t packed[GV][KH / 4];
 #pragma unroll
-          for (int g = 0; g < GV; ++g) {
-            const float2 w = *reinterpret_cast<const float2*>(sv + ((k0 + k) / 2 * GV + g) * 2);
-            const float2 v = mul2(p, w);
-            const __half2 hv = __floats2half2_rn(v.x, v.y);
-            packed[g][k / 2] = *reinterpret_cast<const uint32_t*>(&hv);
+        for (int i = 0; i < 2; ++i) {
+          const float n = m_ref[2 * hf + i] == -INFINITY ? 0.f : -m_ref[2 * hf + i];
+          const float2 neg = make_float2(n, n);
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < PAIRS; ++j) {
+            float2 p = add2(x[2 * hf + i][j], neg);
+            p.x = ex2(p.x);
+            p.y = ex2(p.y);
+            sum = add2(sum, p);
+#pragma unroll
+            for (int g = 0; g < GV; ++g) {
+              const float2 v = mul2(p, w[j][g]);
+              const __half2 hv = __floats2half2_rn(v.x, v.y);
+              packed[g][2 * j + i] = *reinterpret_cast<const uint32_t*>(&hv);
+            }
           }
+          l_run[2 * hf + i] += sum.x + sum.y;
         }
 #pragma unroll
-        for (int g = 0; g < GV; ++g) tmem_st_x8(tmem_s + g * KT + k0 / 2, packed[g]);
+        for (int g = 0; g < GV; ++g)
+          tmem_st_pairs(tmem_s + hf * LANES16 + g * KT, packed[g]);
       }
-      sum[0] = add2(sum[0], sum[1]);
-      l_run += sum[0].x + sum[0].y;
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[c]);
     }
-    // ---- this part of the rows' softmax
-    if (ok && mine > 0) {
-      ok = mbar_wait(&o_done[c], 0, status, STATUS_EPILOGUE_WAIT, 0x200);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after();
-    }
+    // ---- this part of the rows' softmax.  The ring is free when both contexts' products are through:
+    // a warp puts 32 rows of 32 channels there and writes whole lines.
+    for (int k = 0; k < 2; ++k)
+      if (k < turns) ok = ok && wait_long(&o_done[k], 0, status, STATUS_EPILOGUE_WAIT, 0x200);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
     const bool some = ok && mine > 0;
-    const size_t at =
-        (static_cast<size_t>(valid ? info[row].y + (it.pair ? it.part : 2 * it.part + c) : 0)) * qh +
-        h * rep + r % rep;
-    float* to = part_o + at * D + vpart * L::DV;
 #pragma unroll
-    for (int g = 0; g < GV; ++g) {
-      const float back = some ? __uint_as_float((254u << 23) - __float_as_uint(unit[g])) : 0.f;
+    for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], o);
+    row_max[half * TILE + qg + 8 * qt] = mine_of(l_run);          // (the turns' maxima are read)
+    if (half == 0) row_max[2 * TILE + qg + 8 * qt] = mine_of(m_ref);
+    const size_t at = static_cast<size_t>(part) * qh + h * rep + r % rep;
+    const float back = __uint_as_float((254u << 23) - __float_as_uint(unit));
+    unsigned char* out = smem + L::KV_OFF + warp * L::OUT_WARP;
+    meet();
+    if (half == 0 && vpart == 0 && part >= 0)
+      part_ml[at] = some ? make_float2(row_max[2 * TILE + lane], row_max[lane] + row_max[TILE + lane])
+                         : make_float2(-INFINITY, 0.f);
 #pragma unroll 1
-      for (int d0 = 0; d0 < 64; d0 += 16) {
+    for (int d0 = 0; d0 < CH; d0 += 32) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 16) {
         uint32_t o[16];
         if (some) {
-          tmem_ld_x16(tmem_oc + g * 64 + d0, o);
+          tmem_ld_x16(tmem_oc + d0 + e, o);
           tc_wait_ld();
         }
-        if (valid) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (some)
-              v = make_float4(__uint_as_float(o[i]) * back, __uint_as_float(o[i + 1]) * back,
-                              __uint_as_float(o[i + 2]) * back, __uint_as_float(o[i + 3]) * back);
-            *reinterpret_cast<float4*>(to + g * 64 + d0 + i) = v;
-          }
+        for (int i = 0; i < 16; i += 4) {
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (some)
+            v = make_float4(__uint_as_float(o[i]) * back, __uint_as_float(o[i + 1]) * back,
+                            __uint_as_float(o[i + 2]) * back, __uint_as_float(o[i + 3]) * back);
+          *reinterpret_cast<float4*>(out + swz128(lane, (e + i) / 4)) = v;
         }
       }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int from = i * 4 + lane / 8;
+        const size_t to = __shfl_sync(0xffffffffu, static_cast<unsigned long long>(at), from);
+        if (__shfl_sync(0xffffffffu, part, from) >= 0)
+          *reinterpret_cast<float4*>(part_o + to * D + vpart * L::DV + half * CH + d0 +
+                                     lane % 8 * 4) =
+              *reinterpret_cast<const float4*>(out + swz128(from, lane % 8));
+      }
+      __syncwarp();
     }
-    if (valid && vpart == 0) part_ml[at] = make_float2(some ? m_ref : -INFINITY, some ? l_run : 0.f);
   }
   tc_fence_before();
   __syncthreads();

@@ -7,8 +7,18 @@
 //   s -= frequency * c;  s += bias;  a token that the row's mask does not permit gets `masked`.
 // Only tokens that occur or have a bias need any of it; the others are copied.
 //
-// One CTA per row walks the vocabulary in tiles and counts the history's tokens of a tile in shared
-// memory.
+// It is a pass over memory, 8 bytes a token.  A cluster of eight CTAs takes a row.  Each CTA streams an
+// eighth of the vocabulary, copying what is permitted, four tokens to a load.  Of the tokens that occur
+// or have a bias it looks after those that leave its rank modulo eight: it reads the whole history
+// (from L2), counts its own in a table in shared memory and lists them, and when the row has been
+// streamed it computes their scores, which whole warps then do, whichever tokens are frequent.
+//
+// 256 rows of 151936 tokens: 56 us without penalties and masks (a copy takes 49), 68 with a mask per
+// row, 114 with histories of 8000 tokens; one row 4.2, 4.9 and 10.0.  What a history costs is a chain
+// in 32 warps of an SM: four rounds of 1600 cycles of counting, a cluster barrier, 2500 of scores.
+// Tried: scores as a branch of the streaming loop (a slice's few tokens one by one: 256 rows 210),
+// slices of neighbouring tokens counted by atomics in each other's shared memory (155, and 200 where
+// most of the history falls to one slice), the CTA that met a token first looking after it (158).
 #include "api.h"
 #include "common.cuh"
 
@@ -16,7 +26,12 @@ namespace orinfer {
 namespace lp {
 
 constexpr int THREADS = 512;
-constexpr int TILE = 4096;                         // tokens whose counts are held at a time
+constexpr int CTAS = 8;                            // per row
+constexpr int TABLE = 24576;                       // tokens that a CTA looks after at a time, at most
+constexpr int LIST = 4096;                         // of which so many are listed
+constexpr int BIASES = 64 * THREADS;               // of a row, at most
+constexpr int BATCH = 5;                           // loads of a thread in flight
+constexpr int SHORT = 32767;                       // tokens of a history whose counts take 16 bits
 
 struct Args {
   const float* logits;
@@ -39,12 +54,79 @@ struct Args {
   int rows, vocab, bias_total;
 };
 
-__global__ void __launch_bounds__(THREADS) process_logits_kernel(const Args a) {
-  __shared__ int count[TILE], entry[TILE];         // occurrences; the last bias entry, plus one
-  __shared__ int s_bad, s_any;
-  const int row = blockIdx.x, tid = threadIdx.x;
+// A word per token: its occurrences, and in the top bit whether it has a bias, whose thread then writes
+// it.  Words of 16 bits, for histories that cannot count further, leave the L1 cache, through which the
+// logits come, the room to have them in flight (256 rows of 151936 without a history, of 49 us for a
+// copy: 59 with it, 69 without).
+template <class W>
+struct Words {
+  static constexpr unsigned BIASED = 1u << (8 * sizeof(W) - 1);
+  W* at;
+  __device__ __forceinline__ unsigned operator[](unsigned i) const { return at[i]; }
+  __device__ __forceinline__ void set(unsigned i, unsigned v) { at[i] = static_cast<W>(v); }
+  // adds one, and returns what was there
+  __device__ __forceinline__ unsigned count(unsigned i) {
+    if (sizeof(W) == 4) return atomicAdd(reinterpret_cast<unsigned*>(at) + i, 1u);
+    const unsigned shift = (i & 1) * 16;
+    return atomicAdd(reinterpret_cast<unsigned*>(at) + i / 2, 1u << shift) >> shift & 0xffffu;
+  }
+  __device__ __forceinline__ void raise(unsigned i, unsigned v) {
+    unsigned* word = reinterpret_cast<unsigned*>(at) + (sizeof(W) == 4 ? i : i / 2);
+    const unsigned shift = sizeof(W) == 4 ? 0 : (i & 1) * 16, all = sizeof(W) == 4 ? ~0u : 0xffffu;
+    unsigned old = *word;
+    while ((old >> shift & all) < v) {
+      const unsigned was = atomicCAS(word, old, (old & ~(all << shift)) | v << shift);
+      if (was == old) break;
+      old = was;
+    }
+  }
+};
+
+// Tokens that a CTA looks after at a time, and its dynamic shared memory: their words, the mask's words
+// of its slice and one more, the list.
+__host__ __device__ inline int table_words(int vocab) {
+  const int own = (vocab + CTAS - 1) / CTAS;
+  return ((own < TABLE ? own : TABLE) + 7) / 8 * 8;
+}
+__host__ __device__ inline int slice_of(int vocab) {
+  return (vocab + 32 * CTAS - 1) / (32 * CTAS) * 32;
+}
+constexpr int MASK_WORDS = 1024;                   // of a slice, held in shared memory
+
+template <class W>
+__global__ void __launch_bounds__(THREADS, 2) process_logits_kernel(const Args a) {
+  extern __shared__ __align__(16) unsigned char space[];
+  __shared__ unsigned s_mask[MASK_WORDS + 1];
+  __shared__ unsigned short list[LIST];
+  __shared__ int s_flags[CTAS];
+  __shared__ int s_listed, s_bad;
+  grid_wait();
+  grid_release();
+  const int row = blockIdx.x / CTAS, rank = blockIdx.x % CTAS, tid = threadIdx.x;
+  const int words = table_words(a.vocab);
+  Words<W> table{reinterpret_cast<W*>(space)};
+  constexpr unsigned BIASED = Words<W>::BIASED;
   const float* x = a.logits + row * a.row_stride;
   float* out = a.out + row * a.out_stride;
+  // ---- the slice that is streamed: four tokens at a time behind the first 16-byte boundary, where
+  // both rows have theirs together
+  const int slice = slice_of(a.vocab);
+  const int lo = rank * slice, n = max(0, min(slice, a.vocab - lo));
+  const bool vectors =
+      ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  const int first =
+      vectors ? static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) / 4 & 3) : 0;
+  const int groups = vectors ? max(0, n - first) / 4 : 0;
+  const float4* x4 = reinterpret_cast<const float4*>(x + lo + first);
+  float4* out4 = reinterpret_cast<float4*>(out + lo + first);
+  float4 v[BATCH];
+  auto load = [&](int g0) {
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (g0 + k * THREADS < groups) v[k] = x4[g0 + k * THREADS];
+  };
+  load(tid);                                       // on their way while the table is made
+
   const double rep = a.repetition ? a.repetition[row] : 1.0;
   const double pres = a.presence ? a.presence[row] : 0.0;
   const double freq = a.frequency ? a.frequency[row] : 0.0;
@@ -52,53 +134,177 @@ __global__ void __launch_bounds__(THREADS) process_logits_kernel(const Args a) {
   const int seen = counted ? min(max(a.history_len[row], 0), a.history_cap) : 0;
   const int* history = a.history + row * a.history_stride;
   const int b_lo = a.bias_start ? max(a.bias_start[row], 0) : 0;
-  const int b_hi = a.bias_start ? min(a.bias_start[row + 1], a.bias_total) : 0;
+  const int entries = a.bias_start ? min(a.bias_start[row + 1], a.bias_total) - b_lo : 0;
   const int which = a.mask ? (a.mask_rows ? a.mask_rows[row] : row) : -1;
-  const unsigned int* mask =
+  const unsigned* mask =
       which >= 0 && which < a.mask_count ? a.mask + which * a.mask_stride : nullptr;
-  if (tid == 0) s_bad = s_any = 0;
-  bool bad = which >= a.mask_count, any = false;   // (a mask that does not exist)
-  for (int lo = 0; lo < a.vocab; lo += TILE) {
-    const int n = min(TILE, a.vocab - lo);
-    __syncthreads();
-    for (int i = tid; i < n; i += THREADS) count[i] = entry[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < seen; i += THREADS) {
-      const unsigned id = static_cast<unsigned>(history[i]) - lo;
-      if (id < static_cast<unsigned>(n)) atomicAdd(&count[id], 1);
+  // (a mask that does not exist, more biases than the winners' bits)
+  const bool odd = (which >= 0 && !mask) || entries > BIASES;
+  const bool biased = entries > 0 && !odd, special = seen > 0 || biased;
+  if (tid == 0) s_bad = odd;
+  // the slice's permissions (from global memory where they are too many)
+  const bool held = slice <= 32 * MASK_WORDS;
+  unsigned any = mask ? 0u : 1u;
+  if (mask)
+    for (int w = tid; w < (n + 31) / 32; w += THREADS) {
+      const unsigned bits = mask[lo / 32 + w];
+      if (held) s_mask[w] = bits;
+      any |= n - 32 * w < 32 ? bits & ((1u << (n - 32 * w)) - 1u) : bits;
     }
-    for (int i = b_lo + tid; i < b_hi; i += THREADS) {
-      const unsigned id = static_cast<unsigned>(a.bias_ids[i]) - lo;
-      if (id < static_cast<unsigned>(n)) atomicMax(&entry[id], i - b_lo + 1);
+
+  // ---- the words of tokens rank + 8 (done .. done + words): occurrences, and which have a bias
+  unsigned long long wins = 0;                     // this thread's bias entries that count
+  auto own_at = [&](int token, int done) {         // a token's word, or something past the table
+    const unsigned id = token;
+    return id < static_cast<unsigned>(a.vocab) && id % CTAS == static_cast<unsigned>(rank)
+               ? id / CTAS - done
+               : 0xffffffffu;
+  };
+  const bool wide = (reinterpret_cast<uintptr_t>(history) & 15) == 0;
+  auto tokens_at = [&](int i) {                    // four of the history
+    int4 t = make_int4(-1, -1, -1, -1);
+    if (wide && i + 3 < seen) {
+      t = *reinterpret_cast<const int4*>(history + i);
+    } else {
+      if (i < seen) t.x = history[i];
+      if (i + 1 < seen) t.y = history[i + 1];
+      if (i + 2 < seen) t.z = history[i + 2];
+      if (i + 3 < seen) t.w = history[i + 3];
     }
+    return t;
+  };
+  auto make_table = [&](int done) {
+    int4 next = tokens_at(4 * tid), after = tokens_at(4 * (THREADS + tid));
+    if (tid == 0) s_listed = 0;
+    for (int q = tid; q < words * static_cast<int>(sizeof(W)) / 16; q += THREADS)
+      reinterpret_cast<uint4*>(space)[q] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
-    for (int i = tid; i < n; i += THREADS) {
-      const int id = lo + i;
-      const bool permitted = !mask || (mask[id >> 5] >> (id & 31) & 1u);
-      float v = x[id];
-      bad = bad || !isfinite(v);
-      any = any || permitted;
-      if (!permitted) {
-        v = a.masked;
-      } else if (count[i] || entry[i]) {
-        const int c = count[i];
-        double s = v;
-        if (c > 0) {
-          s = s < 0.0 ? s * rep : s / rep;
-          s -= pres;
+    const unsigned most = words;
+    if (biased) {                                  // the last entry of a token is the one that counts
+      wins = 0;
+      auto entry_at = [&](int i) { return own_at(a.bias_ids[b_lo + i], done); };
+      for (int i = tid; i < entries; i += THREADS)
+        if (entry_at(i) < most) table.raise(entry_at(i), i + 1u);
+      __syncthreads();
+      for (int i = tid, k = 0; i < entries; i += THREADS, ++k)
+        if (entry_at(i) < most && table[entry_at(i)] == i + 1u) wins |= 1ull << k;
+      __syncthreads();
+      for (int i = tid, k = 0; i < entries; i += THREADS, ++k)
+        if (wins >> k & 1) table.set(entry_at(i), BIASED);
+      __syncthreads();
+    }
+    // tokens met for the first time are listed
+    for (int i = 4 * tid; i < seen; i += 4 * THREADS) {
+      const int4 t = next;
+      next = after;
+      after = tokens_at(i + 8 * THREADS);
+      const unsigned at[4] = {own_at(t.x, done), own_at(t.y, done), own_at(t.z, done),
+                              own_at(t.w, done)};
+      unsigned old[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) old[e] = at[e] < most ? table.count(at[e]) : 1u;
+      const unsigned fresh = (old[0] == 0 ? 1u : 0u) | (old[1] == 0 ? 2u : 0u) |
+                             (old[2] == 0 ? 4u : 0u) | (old[3] == 0 ? 8u : 0u);
+      if (fresh == 0) continue;
+      int to = atomicAdd(&s_listed, __popc(fresh));
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (fresh >> e & 1u) {
+          if (to < LIST) list[to] = static_cast<unsigned short>(at[e]);
+          ++to;
         }
-        s -= freq * c;
-        if (entry[i]) s += a.bias_values[b_lo + entry[i] - 1];
-        v = static_cast<float>(s);
-        bad = bad || !isfinite(v);
+    }
+    __syncthreads();
+  };
+  if (special)
+    make_table(0);
+  else if (mask)
+    __syncthreads();
+
+  // ---- the slice
+  float nothing = 0.f;                             // 0, or NaN once a logit was not finite
+  for (int g0 = tid; g0 < groups; g0 += BATCH * THREADS) {
+    if (g0 > tid) load(g0);
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int g = g0 + k * THREADS;
+      if (g >= groups) break;
+      float4 y = v[k];
+      nothing = fmaf(y.x, 0.f, fmaf(y.y, 0.f, fmaf(y.z, 0.f, fmaf(y.w, 0.f, nothing))));
+      if (mask) {
+        const int i = first + 4 * g, at = i & 31;
+        const unsigned* m = held ? s_mask + (i >> 5) : mask + (lo + i >> 5);
+        unsigned allowed = m[0] >> at;
+        if (at > 28) allowed |= m[1] << (32 - at);                       // (of tokens of the group)
+        if (!(allowed & 1u)) y.x = a.masked;
+        if (!(allowed & 2u)) y.y = a.masked;
+        if (!(allowed & 4u)) y.z = a.masked;
+        if (!(allowed & 8u)) y.w = a.masked;
       }
-      out[id] = v;
+      out4[g] = y;
     }
   }
-  if (bad) s_bad = 1;
-  if (any) s_any = 1;
+  auto permitted = [&](int id) { return !mask || (mask[id >> 5] >> (id & 31) & 1u); };
+  for (int j = tid; j < n - 4 * groups; j += THREADS) {          // ahead of the groups and behind them
+    const int id = lo + (j < min(first, n) ? j : j + 4 * groups);
+    const float f = x[id];
+    nothing = fmaf(f, 0.f, nothing);
+    out[id] = permitted(id) ? f : a.masked;
+  }
+
+  // ---- scores of tokens that occur or have a bias, in 64 bits.  What is permitted has been copied, so
+  // that its logit is still there where out is the logits.
+  auto write_score = [&](int id, unsigned word, const double* bias) {
+    if (!permitted(id)) return;
+    const int count = word & (BIASED - 1u);
+    double s = x[id];
+    if (count > 0) {
+      s = s < 0.0 ? s * rep : s / rep;
+      s -= pres;
+    }
+    s -= freq * count;
+    if (bias) s += *bias;
+    const float f = static_cast<float>(s);
+    out[id] = f;
+    if (!isfinite(f)) s_bad = 1;
+  };
+  if (special) {
+    __syncthreads();
+    cluster_sync_all();                            // the row has been streamed
+    for (int done = 0;; done += words) {
+      auto look_after = [&](unsigned i) {
+        write_score((done + static_cast<int>(i)) * CTAS + rank, table[i], nullptr);
+      };
+      if (s_listed <= LIST) {
+        for (int i = tid; i < s_listed; i += THREADS) look_after(list[i]);
+      } else {                                     // the list has no room: all that occur
+        for (int i = tid; i < words; i += THREADS)
+          if (table[i] != 0 && !(table[i] & BIASED)) look_after(i);
+      }
+      for (int i = tid, k = 0; i < entries && biased; i += THREADS, ++k)
+        if (wins >> k & 1) {
+          const int id = a.bias_ids[b_lo + i];
+          write_score(id, table[own_at(id, done)], a.bias_values + b_lo + i);
+        }
+      if ((done + words) * CTAS >= a.vocab) break;
+      __syncthreads();
+      make_table(done + words);
+    }
+  }
+  // ---- flags, in the first CTA
+  const bool bad = __syncthreads_or(!(nothing == 0.f));
+  const bool some = __syncthreads_or(any);
+  if (tid == 0)
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(smem_u32(&s_flags[rank]), 0)),
+                 "r"((bad || s_bad ? 2 : 0) | (some ? 1 : 0))
+                 : "memory");
   __syncthreads();
-  if (tid == 0) a.flags[row] = s_bad ? 2 : s_any ? 0 : 1;
+  cluster_sync_all();
+  if (rank == 0 && tid == 0) {
+    int all = 0;
+    for (int c = 0; c < CTAS; ++c) all |= *reinterpret_cast<volatile int*>(&s_flags[c]);
+    a.flags[row] = all & 2 ? 2 : all & 1 ? 0 : 1;
+  }
 }
 
 }  // namespace lp
@@ -111,7 +317,8 @@ using namespace orinfer;
 // 0).  Biases of row r are entries bias_start[r] .. bias_start[r + 1] of bias_total; the last one of
 // a token counts.  mask: rows of (vocab + 31) / 32 words, bit set = permitted; row r uses row
 // mask_rows[r] (none below 0), or row r where mask_rows is null.  flags[r]: 0, 1 where nothing is
-// permitted, 2 where a logit or a permitted token's score is not finite or the mask does not exist.
+// permitted, 2 where a logit or a permitted token's score is not finite, the mask does not exist or
+// the row has more than 32768 biases.
 extern "C" int orinfer_process_logits(
     const float* logits, long long row_stride, const int* history, long long history_stride,
     int history_cap, const int* history_len, const double* repetition, const double* presence,
@@ -120,14 +327,32 @@ extern "C" int orinfer_process_logits(
     float masked, float* out, long long out_stride, int* flags, int rows, int vocab,
     cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (vocab <= 0 || row_stride < vocab || out_stride < vocab || !logits || !out || !flags) return -1;
-  if (history && (!history_len || history_cap < 0)) return -1;
+  if (rows > (1 << 27) || vocab <= 0 || row_stride < vocab || out_stride < vocab || !logits || !out || !flags) return -1;
+  if (history && (!history_len || history_cap < 0 || history_cap > 1 << 29)) return -1;
   if (bias_start && (bias_total < 0 || (bias_total > 0 && (!bias_ids || !bias_values)))) return -1;
   if (mask && (mask_stride < (vocab + 31) / 32 || mask_count < (mask_rows ? 0 : rows))) return -1;
   const lp::Args a = {logits, row_stride, history, history_stride, history_len, history_cap,
                       repetition, presence, frequency, bias_start, bias_ids, bias_values,
                       reinterpret_cast<const unsigned int*>(mask), mask_stride, mask_rows,
                       mask_count, masked, out, out_stride, flags, rows, vocab, bias_total};
-  lp::process_logits_kernel<<<rows, lp::THREADS, 0, stream>>>(a);
-  return static_cast<int>(cudaGetLastError());
+  const bool narrow = !history || history_cap <= lp::SHORT;
+  auto kernel = narrow ? lp::process_logits_kernel<uint16_t> : lp::process_logits_kernel<uint32_t>;
+  static const int slot[2] = {runtime_new_slot(), runtime_new_slot()};
+  if (const int e = runtime_allow_smem(slot[narrow], kernel, 4 * lp::TABLE)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * lp::CTAS);
+  cfg.blockDim = dim3(lp::THREADS);
+  cfg.dynamicSmemBytes = (narrow ? 2 : 4) * static_cast<size_t>(lp::table_words(vocab));
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;       // see launch_early
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = lp::CTAS;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = rows <= EARLY_CTAS / lp::CTAS ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }

@@ -745,7 +745,8 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     set bit permits its token; row r is bound by mask ``mask_rows[r]``, by none below 0, by mask r
     without ``mask_rows``.  Tokens that are not permitted get ``masked``.  Returns (out, flags int32
     [rows]): 1 where nothing is permitted, 2 where a logit or a permitted token's score is not
-    finite or the mask does not exist (the host law refuses those rows), else 0.  ``out`` may be ``logits``."""
+    finite (the host law refuses those rows), the mask does not exist or the row has more than 32768
+    biases, else 0.  ``out`` may be ``logits``."""
     _cuda(logits, history, history_len, repetition, presence, frequency, bias_start, bias_ids,
           bias_values, mask, mask_rows, out, flags)
     _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.stride(1) == 1

@@ -154,6 +154,31 @@ def test_rows_that_the_host_law_refuses(dev):
     assert int(flags[0]) == 2
 
 
+@pytest.mark.parametrize("hist,step", [(32767, 8), (60000, 1), (40000, 8)])
+def test_long_histories_of_many_tokens(dev, hist, step):
+    """Counts of 16 bits and more, and tokens that all fall to one CTA or fill every list."""
+    logits, kw, permitted = case(2, 151936, hist, 20, seed=hist)
+    g = torch.Generator().manual_seed(step)
+    kw["history"] = torch.randint(0, 151936 // step, (2, hist), generator=g, dtype=torch.int32) * step
+    check(dev, logits, kw, permitted)
+
+
+def test_many_biases_on_a_large_vocabulary(dev):
+    """As many entries as a row may have, most tokens named more than once, on more tokens than the
+    tables of a cluster hold; one entry more is refused."""
+    vocab, n = 300001, 32768
+    g = torch.Generator().manual_seed(3)
+    logits, kw, permitted = case(2, vocab, 500, 0, masks=False)
+    kw.update(bias_start=torch.tensor([0, n, n + 9], dtype=torch.int32),
+              bias_ids=torch.randint(0, vocab // 20, (n + 9,), generator=g, dtype=torch.int32) * 19,
+              bias_values=torch.rand(n + 9, generator=g, dtype=torch.float64))
+    check(dev, logits, kw, permitted)
+    from orinfer_b200.ops import functional as F
+    kw["bias_start"] = torch.tensor([0, n + 1, n + 9], dtype=torch.int32)
+    _, flags = F.process_logits(logits.to(dev), **{k: v.to(dev) for k, v in kw.items()})
+    assert flags.tolist() == [2, 0]
+
+
 def test_the_sampler_and_the_argmax_take_masked_scores(dev):
     """One permitted token is drawn by both, whatever the others' logits are."""
     from orinfer_b200.ops import functional as F
