@@ -44,10 +44,6 @@ __device__ __forceinline__ int block_rank(bool flag, int* warp_sums, int& total)
 
 // ---------------------------------------------------------------- fork
 // work: head; copies [n][3]; pairs in the order of their new pages [n]; pair of a child slot [slots]
-__host__ __device__ inline size_t fork_work(int n, int slots) {
-  return WORK_HEAD + 4 * static_cast<size_t>(n) + slots;
-}
-
 __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(
     const int* table, const int* lens, const int* refs, int* refs_out, const int* parents,
     const int* children, int n, int slots, int max_pages, int pages, int* work, int* status_out) {
@@ -63,16 +59,17 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(
   for (int s = tid; s < slots; s += PLAN_THREADS) child_of[s] = -1;
   __syncthreads();
   // ---- the pairs: slots that exist, a child that is empty and named once, pages that are held
-  for (int i = tid; i < n; i += PLAN_THREADS) {
-    const int p = parents[i], c = children[i];
+  for (int i = tid / 32; i < n; i += PLAN_THREADS / 32) {        // a warp per pair
+    const int p = parents[i], c = children[i], lane = tid & 31;
     bool wrong = p < 0 || p >= slots || c < 0 || c >= slots || p == c;
-    if (!wrong) wrong = lens[c] != 0 || lens[p] < 0 || lens[p] > max_pages * PAGE;
-    if (!wrong) wrong = atomicCAS(&child_of[c], -1, i) != -1;
     if (!wrong) {
+      const int len = lens[p];
+      wrong = lens[c] != 0 || len < 0 || len > max_pages * PAGE;
+      if (!wrong && lane == 0) wrong = atomicCAS(&child_of[c], -1, i) != -1;
       const int* row = table + static_cast<size_t>(p) * max_pages;
-      for (int j = 0; j < (lens[p] + PAGE - 1) / PAGE; ++j) {
+      for (int j = lane; !wrong && j < (len + PAGE - 1) / PAGE; j += 32) {
         const int page = row[j];
-        wrong = wrong || page <= 0 || page >= pages || refs[page] <= 0;
+        wrong = page <= 0 || page >= pages || refs[page] <= 0;
       }
     }
     if (wrong) s_wrong = 1;
@@ -123,54 +120,32 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(
   }
 }
 
-// The table's rows, lens and the references of shared pages; CTA per slot.
-__global__ void __launch_bounds__(128) fork_rows_kernel(
-    const int* table, int* table_out, const int* lens, int* lens_out, int* refs_out,
-    const int* parents, int n, int slots, int max_pages, const int* work) {
-  grid_wait();
-  grid_release();
-  const int* copies = work + WORK_HEAD;
-  const int s = blockIdx.x, pair = work[0] == 0 ? (copies + 4 * n)[s] : -1;
-  const int from = pair < 0 ? s : parents[pair];
-  const int len = lens[from], full = len / PAGE;
-  const int* row = table + static_cast<size_t>(from) * max_pages;
-  int* row_out = table_out + static_cast<size_t>(s) * max_pages;
-  if (pair < 0) {
-    if (table_out != table)
-      for (int j = threadIdx.x; j < max_pages; j += blockDim.x) row_out[j] = row[j];
-  } else {
-    for (int j = threadIdx.x; j < max_pages; j += blockDim.x) {
-      int page = 0;
-      if (j < full) {
-        page = row[j];
-        atomicAdd(&refs_out[page], 1);
-      } else if (j == full && len % PAGE) {
-        page = copies[3 * pair + 1];
-      }
-      row_out[j] = page;
-    }
-  }
-  if (threadIdx.x == 0 && (pair >= 0 || lens_out != lens)) lens_out[s] = len;
-}
-
 // ---------------------------------------------------------------- copies
+// Four loads of a thread ahead of their stores (one at a time, 128 pages of 9.7 MB moved at 5.7 TB/s).
 template <class T>
 __device__ __forceinline__ void copy_as(const unsigned char* from, unsigned char* to, int bytes) {
+  constexpr int BATCH = 4;
   const int n = bytes / static_cast<int>(sizeof(T));
-  for (int i = threadIdx.x; i < n; i += COPY_THREADS)
-    reinterpret_cast<T*>(to)[i] = reinterpret_cast<const T*>(from)[i];
+  const T* src = reinterpret_cast<const T*>(from);
+  T* dst = reinterpret_cast<T*>(to);
+  for (int i0 = threadIdx.x; i0 < n; i0 += BATCH * COPY_THREADS) {
+    T v[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (i0 + k * COPY_THREADS < n) v[k] = __ldcs(src + i0 + k * COPY_THREADS);
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (i0 + k * COPY_THREADS < n) __stcs(dst + i0 + k * COPY_THREADS, v[k]);
+  }
   for (int i = n * static_cast<int>(sizeof(T)) + threadIdx.x; i < bytes; i += COPY_THREADS)
     to[i] = from[i];
 }
 
-// copies [*count][3]: source page, target page, tokens from the page's first on
-__global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const Cache cache,
-                                                                  const int* copies,
-                                                                  const int* count, int* status) {
-  grid_wait();
-  grid_release();
+// copies [*count][3]: source page, target page, tokens from the page's first on; by CTA `cta` of `ctas`
+__device__ __forceinline__ void copy_units(const Cache& cache, const int* copies, const int* count,
+                                           int cta, int ctas, int* status) {
   const long long total = static_cast<long long>(*count) * cache.n_units;
-  for (long long w = blockIdx.x; w < total; w += gridDim.x) {
+  for (long long w = cta; w < total; w += ctas) {
     const int* c = copies + w / cache.n_units * 3;
     const int* u = cache.units + w % cache.n_units * 3;
     const int from = c[0], to = c[1], tokens = min(c[2] - u[1], u[2]);
@@ -194,49 +169,123 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const Cache ca
   }
 }
 
-// ---------------------------------------------------------------- free
-__global__ void __launch_bounds__(256) copy_ints_kernel(const int* a, int* a_out, long long na,
-                                                        const int* b, int* b_out, long long nb,
-                                                        const int* c, int* c_out, long long nc) {
+__global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const Cache cache,
+                                                                  const int* copies,
+                                                                  const int* count, int* status) {
   grid_wait();
   grid_release();
-  const long long at = blockIdx.x * 256LL + threadIdx.x, step = gridDim.x * 256LL;
-  if (a != a_out)
-    for (long long i = at; i < na; i += step) a_out[i] = a[i];
-  if (b != b_out)
-    for (long long i = at; i < nb; i += step) b_out[i] = b[i];
-  if (c != c_out)
-    for (long long i = at; i < nc; i += step) c_out[i] = c[i];
+  copy_units(cache, copies, count, blockIdx.x, gridDim.x, status);
 }
 
-// CTA per listed slot; a slot that is named again is left to the first
-__global__ void __launch_bounds__(128) free_kernel(int* table, int* lens, int* refs,
-                                                   const int* gone, int slots, int max_pages,
-                                                   int pages, int* status) {
+// The table's rows, lens and the references of shared pages, a CTA per slot; the CTAs behind them copy.
+__global__ void __launch_bounds__(COPY_THREADS) fork_apply_kernel(
+    const int* table, int* table_out, const int* lens, int* lens_out, int* refs_out,
+    const int* parents, int n, int slots, int max_pages, const int* work, const Cache cache,
+    int* status) {
   grid_wait();
   grid_release();
-  const int s = gone[blockIdx.x];
-  bool again = false;
-  for (int i = threadIdx.x; i < static_cast<int>(blockIdx.x); i += blockDim.x)
-    again = again || gone[i] == s;
-  if (__syncthreads_or(again)) return;
-  if (s < 0 || s >= slots) {
-    if (threadIdx.x == 0) report_status(status, STATUS_BAD_INDEX, 0x41);
+  const int* copies = work + WORK_HEAD;
+  if (static_cast<int>(blockIdx.x) >= slots) {
+    copy_units(cache, copies, work + 1, blockIdx.x - slots, gridDim.x - slots, status);
     return;
   }
-  int* row = table + static_cast<size_t>(s) * max_pages;
-  for (int j = threadIdx.x; j < max_pages; j += blockDim.x) {
-    const int page = row[j];
-    row[j] = 0;
-    if (page == 0) continue;
-    if (page < 0 || page >= pages) {
-      report_status(status, STATUS_BAD_INDEX, 0x42);
-    } else if (atomicSub(&refs[page], 1) <= 0) {       // released more often than held
-      atomicAdd(&refs[page], 1);
-      report_status(status, STATUS_BAD_INDEX, 0x43);
+  const int s = blockIdx.x, pair = work[0] == 0 ? (copies + 4 * n)[s] : -1;
+  const int from = pair < 0 ? s : parents[pair];
+  const int len = lens[from], full = len / PAGE;
+  const int* row = table + static_cast<size_t>(from) * max_pages;
+  int* row_out = table_out + static_cast<size_t>(s) * max_pages;
+  if (pair < 0) {
+    if (table_out != table)
+      for (int j = threadIdx.x; j < max_pages; j += blockDim.x) row_out[j] = row[j];
+  } else {
+    for (int j = threadIdx.x; j < max_pages; j += blockDim.x) {
+      int page = 0;
+      if (j < full) {
+        page = row[j];
+        atomicAdd(&refs_out[page], 1);
+      } else if (j == full && len % PAGE) {
+        page = copies[3 * pair + 1];
+      }
+      row_out[j] = page;
     }
   }
-  if (threadIdx.x == 0) lens[s] = 0;
+  if (threadIdx.x == 0 && (pair >= 0 || lens_out != lens)) lens_out[s] = len;
+}
+
+// ---------------------------------------------------------------- free
+// CTAs [0, slots): the rows; the CTAs behind them: the references of RANGE pages each, less what the
+// listed slots hold of them.  `parts`: 1 rows, 2 references, both where no row is read and written.
+constexpr int RANGE = 2048;
+constexpr int ROWS = 1, REFS = 2;
+constexpr int FREE_THREADS = 512;
+constexpr int FREE_MOST = 1 << 17;                 // slots and entries whose bits fit beside the counts
+
+__global__ void __launch_bounds__(FREE_THREADS) free_kernel(const int* table, int* table_out, const int* lens,
+                                                   int* lens_out, const int* refs, int* refs_out,
+                                                   const int* gone, int n, int slots, int max_pages,
+                                                   int pages, int parts, int* status) {
+  extern __shared__ int marks[];                   // a bit per slot: listed, and not yet claimed
+  int* claims = marks + (slots + 31) / 32;         // a bit per entry: it is its slot's first
+  __shared__ int held[RANGE];
+  grid_wait();
+  grid_release();
+  const int row_ctas = parts & ROWS ? slots : 0;
+  if (static_cast<int>(blockIdx.x) < row_ctas) {
+    const int s = blockIdx.x;
+    bool listed = false;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) listed = listed || gone[i] == s;
+    listed = __syncthreads_or(listed);
+    if (!listed && table == table_out && lens == lens_out) return;
+    const size_t row = static_cast<size_t>(s) * max_pages;
+    for (int j = threadIdx.x; j < max_pages; j += blockDim.x)
+      table_out[row + j] = listed ? 0 : table[row + j];
+    if (threadIdx.x == 0) lens_out[s] = listed ? 0 : lens[s];
+    return;
+  }
+  const int first = (blockIdx.x - row_ctas) * RANGE;
+  const bool reports = first == 0;
+  for (int i = threadIdx.x; i < (slots + 31) / 32 + (n + 31) / 32; i += FREE_THREADS) marks[i] = 0;
+  for (int i = threadIdx.x; i < RANGE; i += FREE_THREADS) held[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += FREE_THREADS) {
+    const int s = gone[i];
+    if (s >= 0 && s < slots)
+      atomicOr(&marks[s >> 5], 1 << (s & 31));
+    else if (reports)
+      report_status(status, STATUS_BAD_INDEX, 0x41);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += FREE_THREADS) {
+    const int s = gone[i];
+    if (s >= 0 && s < slots && atomicAnd(&marks[s >> 5], ~(1 << (s & 31))) >> (s & 31) & 1)
+      atomicOr(&claims[i >> 5], 1 << (i & 31));
+  }
+  __syncthreads();
+  const unsigned cells = static_cast<unsigned>(n) * max_pages;
+  for (unsigned c0 = threadIdx.x; c0 < cells; c0 += 4 * FREE_THREADS) {
+    int page[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const unsigned c = c0 + k * FREE_THREADS, i = c / max_pages;
+      page[k] = c < cells && claims[i >> 5] >> (i & 31) & 1
+                    ? table[static_cast<size_t>(gone[i]) * max_pages + (c - i * max_pages)]
+                    : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (page[k] < 0 || page[k] >= pages) {
+        if (reports) report_status(status, STATUS_BAD_INDEX, 0x42);
+      } else if (page[k] > 0 && page[k] >= first && page[k] < first + RANGE) {
+        atomicAdd(&held[page[k] - first], 1);
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < RANGE && first + i < pages; i += FREE_THREADS) {
+    const int left = refs[first + i] - held[i];
+    if (held[i] > 0 && left < 0) report_status(status, STATUS_BAD_INDEX, 0x43);   // held less often
+    if (held[i] > 0 || refs_out != refs) refs_out[first + i] = held[i] > 0 ? max(left, 0) : left;
+  }
 }
 
 // ---------------------------------------------------------------- compact
@@ -290,11 +339,19 @@ __global__ void __launch_bounds__(PLAN_THREADS) compact_plan_kernel(const int* r
   }
 }
 
-__global__ void __launch_bounds__(256) remap_kernel(const int* table, int* table_out, long long n,
-                                                    const int* moved, int pages, int* status) {
+// CTAs [0, remap_ctas) write the table, those behind them copy.
+__global__ void __launch_bounds__(COPY_THREADS) compact_apply_kernel(
+    const int* table, int* table_out, long long n, const int* moved, int pages, int remap_ctas,
+    const int* work, const Cache cache, int* status) {
   grid_wait();
   grid_release();
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
+  if (static_cast<int>(blockIdx.x) >= remap_ctas) {
+    copy_units(cache, work + WORK_HEAD, work + 1, blockIdx.x - remap_ctas, gridDim.x - remap_ctas,
+               status);
+    return;
+  }
+  const long long step = static_cast<long long>(remap_ctas) * COPY_THREADS;
+  for (long long i = static_cast<long long>(blockIdx.x) * COPY_THREADS + threadIdx.x; i < n; i += step) {
     const int page = table[i];
     const bool known = page >= 0 && page < pages;
     if (!known) report_status(status, STATUS_BAD_INDEX, 0x44);
@@ -302,31 +359,21 @@ __global__ void __launch_bounds__(256) remap_kernel(const int* table, int* table
   }
 }
 
-static void launch_copies(const Cache& cache, const int* copies, const int* count, int most,
-                          cudaStream_t stream) {
+// CTAs that copy at most `most` pages
+static int copy_ctas(const Cache& cache, int most) {
   const long long units = static_cast<long long>(most) * cache.n_units;
-  const int grid = static_cast<int>(units < 8 * 148 ? units : 8 * 148);
-  if (grid > 0)
-    launch_early(copy_pages_kernel, dim3(grid), COPY_THREADS, 0, stream, cache, copies, count,
-                 runtime_status_ptr());
+  return static_cast<int>(units < 8 * 148 ? units : 8 * 148);
 }
 
 static int grid_of(long long n) {
-  const long long g = (n + 255) / 256;
-  return static_cast<int>(g < 1 ? 1 : g < 592 ? g : 592);
+  const long long g = (n + COPY_THREADS - 1) / COPY_THREADS;
+  return static_cast<int>(g < 592 ? g : 592);
 }
 
 }  // namespace pg
 }  // namespace orinfer
 
 using namespace orinfer;
-
-extern "C" size_t orinfer_fork_work(int n, int slots) {
-  return n < 0 || slots < 0 ? 0 : pg::fork_work(n, slots);
-}
-extern "C" size_t orinfer_compact_work(int pages) {
-  return pages < 0 ? 0 : pg::WORK_HEAD + 3 * (static_cast<size_t>(pages) / 2 + 1);
-}
 
 // copies: int32 [*count, 3] on the device, at most `most` of them
 extern "C" int orinfer_copy_pages(const long long* bases, const int* token_bytes, const int* units,
@@ -335,13 +382,14 @@ extern "C" int orinfer_copy_pages(const long long* bases, const int* token_bytes
   if (most <= 0 || n_units <= 0) return most < 0 || n_units < 0 ? -1 : 0;
   if (!bases || !token_bytes || !units || !copies || !count || pages <= 0) return -1;
   if (runtime_ensure_init() != cudaSuccess) return -2;
-  pg::launch_copies(pg::Cache{bases, token_bytes, units, n_units, pages}, copies, count, most,
-                    stream);
+  const pg::Cache cache = {bases, token_bytes, units, n_units, pages};
+  launch_early(pg::copy_pages_kernel, dim3(pg::copy_ctas(cache, most)), pg::COPY_THREADS, 0, stream,
+               cache, copies, count, runtime_status_ptr());
   return static_cast<int>(cudaGetLastError());
 }
 
 // status: 0, 1 (not enough free pages) or 2 (a pair that cannot be); then nothing is changed.
-// work: int32 [orinfer_fork_work(n, slots)].
+// work: int32 [4 + 4 n + slots].
 extern "C" int orinfer_fork_pages(const long long* bases, const int* token_bytes, const int* units,
                                   int n_units, int pages, const int* table, int* table_out,
                                   const int* lens, int* lens_out, const int* refs, int* refs_out,
@@ -352,10 +400,10 @@ extern "C" int orinfer_fork_pages(const long long* bases, const int* token_bytes
   if (runtime_ensure_init() != cudaSuccess) return -2;
   launch_early(pg::fork_plan_kernel, dim3(1), pg::PLAN_THREADS, 0, stream, table, lens, refs,
                refs_out, parents, children, n, slots, max_pages, pages, work, status);
-  launch_early(pg::fork_rows_kernel, dim3(slots), 128, 0, stream, table, table_out, lens, lens_out,
-               refs_out, parents, n, slots, max_pages, work);
-  pg::launch_copies(pg::Cache{bases, token_bytes, units, n_units, pages}, work + pg::WORK_HEAD,
-                    work + 1, n, stream);
+  const pg::Cache cache = {bases, token_bytes, units, n_units, pages};
+  launch_early(pg::fork_apply_kernel, dim3(slots + pg::copy_ctas(cache, n)), pg::COPY_THREADS, 0,
+               stream, table, table_out, lens, lens_out, refs_out, parents, n, slots, max_pages, work,
+               cache, runtime_status_ptr());
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -364,18 +412,27 @@ extern "C" int orinfer_free_pages(const int* table, int* table_out, const int* l
                                   int max_pages, int pages, cudaStream_t stream) {
   if (n < 0 || slots <= 0 || max_pages <= 0 || pages <= 0) return -1;
   if (runtime_ensure_init() != cudaSuccess) return -2;
-  const long long cells = static_cast<long long>(slots) * max_pages;
-  if (table != table_out || lens != lens_out || refs != refs_out)
-    launch_early(pg::copy_ints_kernel, dim3(pg::grid_of(cells)), 256, 0, stream, table, table_out,
-                 cells, lens, lens_out, static_cast<long long>(slots), refs, refs_out,
-                 static_cast<long long>(pages));
-  if (n > 0)
-    launch_early(pg::free_kernel, dim3(n), 128, 0, stream, table_out, lens_out, refs_out, gone,
-                 slots, max_pages, pages, runtime_status_ptr());
+  if (slots > pg::FREE_MOST || n > pg::FREE_MOST) return -1;
+  if (static_cast<long long>(n) * max_pages >= 1LL << 31) return -1;
+  const size_t smem = ((slots + 31) / 32 + (n + 31) / 32) * sizeof(int);
+  const int ranges = (pages + pg::RANGE - 1) / pg::RANGE;
+  // in place the references come first: the rows that they are counted from are emptied
+  const bool apart = table == table_out || lens == lens_out;
+  auto start = [&](int parts) {
+    const int ctas = (parts & pg::ROWS ? slots : 0) + (parts & pg::REFS ? ranges : 0);
+    launch_early(pg::free_kernel, dim3(ctas), pg::FREE_THREADS, smem, stream, table, table_out, lens, lens_out,
+                 refs, refs_out, gone, n, slots, max_pages, pages, parts, runtime_status_ptr());
+  };
+  if (apart) {
+    start(pg::REFS);
+    start(pg::ROWS);
+  } else {
+    start(pg::REFS | pg::ROWS);
+  }
   return static_cast<int>(cudaGetLastError());
 }
 
-// moved: int32 [pages], where each page has gone.  work: int32 [orinfer_compact_work(pages)].
+// moved: int32 [pages], where each page has gone.  work: int32 [4 + 3 (pages / 2 + 1)].
 extern "C" int orinfer_compact_pages(const long long* bases, const int* token_bytes,
                                      const int* units, int n_units, int pages, const int* table,
                                      int* table_out, const int* refs, int* refs_out, int* moved,
@@ -385,10 +442,10 @@ extern "C" int orinfer_compact_pages(const long long* bases, const int* token_by
   const long long cells = static_cast<long long>(slots) * max_pages;
   launch_early(pg::compact_plan_kernel, dim3(1), pg::PLAN_THREADS, 0, stream, refs, refs_out, moved,
                pages, work);
-  if (cells > 0)
-    launch_early(pg::remap_kernel, dim3(pg::grid_of(cells)), 256, 0, stream, table, table_out,
-                 cells, moved, pages, runtime_status_ptr());
-  pg::launch_copies(pg::Cache{bases, token_bytes, units, n_units, pages}, work + pg::WORK_HEAD,
-                    work + 1, pages / 2, stream);
+  const pg::Cache cache = {bases, token_bytes, units, n_units, pages};
+  const int remap = pg::grid_of(cells), ctas = remap + pg::copy_ctas(cache, pages / 2);
+  if (ctas > 0)
+    launch_early(pg::compact_apply_kernel, dim3(ctas), pg::COPY_THREADS, 0, stream, table, table_out,
+                 cells, moved, pages, remap, work, cache, runtime_status_ptr());
   return static_cast<int>(cudaGetLastError());
 }

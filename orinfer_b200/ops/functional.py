@@ -454,12 +454,12 @@ def fork_pages(cache: CachePages, table: torch.Tensor, lens: torch.Tensor, refs:
     _need(refs.shape == (cache.pages,), "refs: [pages]")
     slots, width = table.shape
     lib = native.lib()
-    work = torch.empty(lib.orinfer_fork_work(n, slots) + 1, dtype=torch.int32, device=table.device)
-    status = work[-1:]
+    work = torch.empty(4 + 4 * n + slots, dtype=torch.int32, device=table.device)
+    status = torch.empty(1, dtype=torch.int32, device=table.device)
     check(lib.orinfer_fork_pages(
         *cache._args, ptr(table), ptr(t), ptr(lens), ptr(l), ptr(refs), ptr(r), ptr(parents),
         ptr(children), n, slots, width, ptr(work), ptr(status), stream()), "fork_pages")
-    count_launches(3 if n else 2)
+    count_launches(2)
     return t, l, r, status
 
 
@@ -474,7 +474,7 @@ def free_pages(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, slot
     check(native.lib().orinfer_free_pages(
         ptr(table), ptr(t), ptr(lens), ptr(l), ptr(refs), ptr(r), ptr(slots), n, table.shape[0],
         table.shape[1], refs.shape[0], stream()), "free_pages")
-    count_launches((t is not table or l is not lens or r is not refs) + (n > 0))
+    count_launches(2 if t is table or l is lens else 1)
     return t, l, r
 
 
@@ -486,12 +486,11 @@ def compact_pages(cache: CachePages, table: torch.Tensor, refs: torch.Tensor, *,
     _need(refs.shape == (cache.pages,), "refs: [pages]")
     lib = native.lib()
     moved = torch.empty_like(refs)
-    work = torch.empty(lib.orinfer_compact_work(cache.pages), dtype=torch.int32,
-                       device=table.device)
+    work = torch.empty(4 + 3 * (cache.pages // 2 + 1), dtype=torch.int32, device=table.device)
     check(lib.orinfer_compact_pages(
         *cache._args, ptr(table), ptr(t), ptr(refs), ptr(r), ptr(moved), table.shape[0],
         table.shape[1], ptr(work), stream()), "compact_pages")
-    count_launches(3 if cache.pages > 1 else 2)
+    count_launches(2)
     return t, r, moved
 
 

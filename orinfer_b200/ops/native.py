@@ -89,8 +89,6 @@ def _load() -> ctypes.CDLL:
                                       I, I, P, I, P], I),
         "orinfer_process_logits": ([P, c_longlong, P, c_longlong, I, P, P, P, P, P, P, P, I, P,
                                     c_longlong, P, I, c_float, P, c_longlong, P, I, I, P], I),
-        "orinfer_fork_work": ([I, I], c_size_t),
-        "orinfer_compact_work": ([I], c_size_t),
         "orinfer_copy_pages": ([P, P, P, I, I, P, P, I, P], I),
         "orinfer_fork_pages": ([P, P, P, I, I, P, P, P, P, P, P, P, P, I, I, I, P, P, P], I),
         "orinfer_free_pages": ([P, P, P, P, P, P, P, I, I, I, I, P], I),
@@ -134,7 +132,8 @@ def ptr(t: Optional[torch.Tensor]):
 
 
 def stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream's handle, without an object around it (3.2 us of a call's 20)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def check(code: int, what: str) -> None:
