@@ -3,9 +3,9 @@
 //
 // The shared keys of a group of rows are read once: the group's rows times the `rep` query heads of
 // a KV head are the M axis of one product with the prefix, on tcgen05 tensor cores with TMEM
-// accumulators.  A CTA takes one or two tiles of 128 such rows and a range of the keys, and leaves
-// each row's part of the softmax (reference, sum of weights, sum of weighted values) for the row
-// kernels of attention.cu, which add the row's own keys and join the parts.
+// accumulators.  A CTA takes a tile of 128 such rows and a range of the keys, and leaves each row's
+// part of the softmax (reference, sum of weights, sum of weighted values) for the row kernels of
+// attention.cu, which add the row's own keys and join the parts.
 //
 //   S_g = Q K_g^T   a sum of its own per group of 64 channels, K as the exact FP16 integers that the
 //                   cache holds;  score = sum_g S_g x key scale_g in FP32;
@@ -15,9 +15,9 @@
 // would add one each and another 40 %.  P_g is taken under a power of two per group that follows the
 // value scales, so that it stays among FP16's normal numbers.
 //
-// Two contexts of eight softmax warps (two threads per row, each with half of a step's keys) take
-// turns with the tensor core: two tiles that share every step's keys, or, where a group has one tile
-// left, one tile whose steps they take in turn, each with a softmax of its own.
+// Scores of three steps have a place in TMEM, so that the products run ahead of the eight softmax warps
+// (sixteen rows each), which go from step to step without a wait.  The weights replace the scores that
+// they are made of.
 #include "api.h"
 #include "attention_shared.h"
 #include "common.cuh"
@@ -26,7 +26,7 @@ namespace orinfer {
 namespace sp {
 
 constexpr int TILE = 128;                        // rows of a tile: positions x query heads
-constexpr int SOFTMAX_WARPS = 16, DQ_WARPS = 4;
+constexpr int SOFTMAX_WARPS = 8, DQ_WARPS = 8;
 constexpr int MMA_WARP = SOFTMAX_WARPS + DQ_WARPS, SCALE_WARP = MMA_WARP + 1;
 constexpr int THREADS = (SCALE_WARP + 1) * 32;
 constexpr float LAG = 8.f;                       // of the weights' reference, binades
@@ -37,30 +37,30 @@ struct Shape {
   static constexpr int DV = D > 128 ? 128 : D;   // value channels of a CTA
   static constexpr int GV = DV / 64, PARTS = D / DV;
   static constexpr int KT = D > 128 ? 32 : 64;   // keys of a step: at most 128 score columns
-  static constexpr int NB = D > 128 ? 3 : 4;     // buffers of keys and values
+  static constexpr int NB = 5, PF = 2;           // buffers of keys and values; steps in registers
   static constexpr int QSUB = TILE * 128, KSUB = KT * 128;     // bytes of 64 channels of a tile
   static constexpr int K_BYTES = G * KSUB, V_BYTES = GV * KSUB;
-  static constexpr int Q_OFF = 0;                // two tiles
-  static constexpr int KV_OFF = 2 * G * QSUB;
+  static constexpr int Q_OFF = 0;
+  static constexpr int KV_OFF = G * QSUB;
   static constexpr int SCALE_OFF = KV_OFF + NB * (K_BYTES + V_BYTES);
   static constexpr int SCALES = KT * (G + GV) * 4 + 16;        // key and value scales, units
-  static constexpr int MAX_OFF = SCALE_OFF + NB * SCALES;      // [2 contexts][2 turns][2 halves][128]
-  static constexpr int BAR_OFF = MAX_OFF + 8 * TILE * 4;
+  static constexpr int STAT_OFF = SCALE_OFF + NB * SCALES;     // [sum, reference][128]
+  static constexpr int BAR_OFF = STAT_OFF + 2 * TILE * 4;
+  static constexpr int CC = D > 128 ? 16 : 32;   // score columns of a group that are read at a time
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;
-  static constexpr int OUT_WARP = 4096;          // of a warp's results on their way out (in the ring)
-  static_assert(SOFTMAX_WARPS * OUT_WARP <= NB * (K_BYTES + V_BYTES), "results fit the ring");
+  static constexpr int SUB = DV / 2;             // channels that a warp writes, of 32 rows: in the ring
+  static_assert(SOFTMAX_WARPS * 32 * SUB * 4 <= NB * (K_BYTES + V_BYTES), "results fit the ring");
   static_assert(TOTAL <= 227 * 1024, "exceeds the shared memory of one CTA");
   static_assert(SCALES % 16 == 0, "scales are read sixteen bytes at a time");
 };
 
 // Rows and keys of a CTA (as many as the plan has), per KV head.
 struct Item {
-  int row, rows;                                 // the first row, and how many (at most two tiles)
+  int row, rows;                                 // the first row of the tile, and how many
   int step_lo, step_hi;                          // its steps of KT keys
   int shared;                                    // keys that the group shares
   int part;                                      // its part of a row's parts
-  int pair;                                      // two tiles
-  int unused;
+  int unused[2];
 };
 
 __device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t tmem_d, uint64_t adesc,
@@ -189,26 +189,24 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     const Item* items, const int4* info, float* __restrict__ part_o, float2* __restrict__ part_ml,
     int qh, int kvh, int rep, int num_pages, int* status) {
   using L = Shape<D>;
-  constexpr int G = L::G, GV = L::GV, KT = L::KT, KH = KT / 2, NB = L::NB;
+  constexpr int G = L::G, GV = L::GV, KT = L::KT, NB = L::NB, CC = L::CC;
+  constexpr int NS = 3;                  // steps whose scores have a place
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
   uint64_t* kv_full = bars;              // [NB] keys, values and scales of a step are there
   uint64_t* kv_free = bars + NB;         // [NB] the last product that reads them is through
-  uint64_t* s_full = bars + 2 * NB;      // [2] scores of a context
-  uint64_t* p_ready = s_full + 2;        // [2] its weights (an arrival per warp)
-  uint64_t* o_done = s_full + 4;         // [2] its last product is through
-  uint64_t* q_full = s_full + 6;         // the query rows are there (an arrival per softmax warp)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 7);
+  uint64_t* s_full = bars + 2 * NB;      // [NS] scores of a step
+  uint64_t* p_ready = s_full + NS;       // [NS] its weights (an arrival per softmax warp)
+  uint64_t* o_done = p_ready + NS;       // [NS] the product with them is through
+  uint64_t* q_full = o_done + NS;         // the query rows are there (an arrival per softmax warp)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
 
   const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
   grid_wait();
   const Item it = items[blockIdx.x];
   const int h = blockIdx.y / L::PARTS, vpart = blockIdx.y % L::PARTS;
-  const int P = TILE / rep, tiles = it.pair ? 2 : 1;
   const int steps = it.step_hi - it.step_lo;
-  // turns of the contexts: both at every step, or one step each in turn
-  const int turns = it.pair ? 2 * steps : steps;
   const int req = row_req[it.row];
   const bool known = req >= 0 && req < slots;
   const int* pages = page_table + static_cast<size_t>(known ? req : 0) * max_pages;
@@ -218,10 +216,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       mbar_init(&kv_full[b], DQ_WARPS + 1);
       mbar_init(&kv_free[b], 1);
     }
-    for (int c = 0; c < 2; ++c) {
-      mbar_init(&s_full[c], 1);
-      mbar_init(&p_ready[c], SOFTMAX_WARPS / 2);
-      mbar_init(&o_done[c], 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], SOFTMAX_WARPS);
+      mbar_init(&o_done[i], 1);
     }
     mbar_init(q_full, SOFTMAX_WARPS);
     mbar_fence_init();
@@ -235,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
   tc_fence_after();
   const uint32_t tmem = warp_same(*tmem_slot);
   grid_release();
-  const uint32_t tmem_o = tmem + 256;            // O of context c at + 128 c; S at 128 c
+  const uint32_t tmem_o = tmem + 128 * NS;       // scores at 128 (step modulo NS)
 
   if (warp == MMA_WARP) {
     // ---------------- products, issued by the whole warp (see elect_one)
@@ -245,32 +243,35 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     const uint64_t qd = umma_desc(smem_u32(smem + L::Q_OFF), 16, 1024);
     const uint64_t kd = umma_desc(smem_u32(smem + L::KV_OFF), 16, 1024);
     const uint64_t vd = umma_desc(smem_u32(smem + L::KV_OFF + L::K_BYTES), L::KSUB, 1024);
-    const int last = warp_same(turns), pair = warp_same(it.pair);
+    const int last = warp_same(steps);
     bool ok = __all_sync(0xffffffffu, wait_long(q_full, 0, status, STATUS_MMA_WAIT, 0x300));
-    auto step_of = [&](int t) { return pair ? t >> 1 : t; };
-    auto issue_qk = [&](int t) {
-      const int c = t & 1, s = step_of(t), b = s % NB;
-      if (ok)
-        ok = __all_sync(0xffffffffu, wait_long(&kv_full[b], (s / NB) & 1, status, STATUS_MMA_WAIT,
-                                               0x400 | (s & 0xff)));
+    auto wait_kv = [&](int s) {
+      if (ok && s < last)
+        ok = __all_sync(0xffffffffu, wait_long(&kv_full[s % NB], (s / NB) & 1, status,
+                                               STATUS_MMA_WAIT, 0x400 | (s & 0xff)));
+    };
+    auto issue_qk = [&](int s) {
       tc_fence_after();
       if (!ok) return;
-      const uint64_t qt = qd + (pair ? c * G * L::QSUB / 16 : 0);
-      const uint64_t kb = kd + static_cast<uint64_t>(b) * ((L::K_BYTES + L::V_BYTES) / 16);
+      const uint64_t kb = kd + static_cast<uint64_t>(s % NB) * ((L::K_BYTES + L::V_BYTES) / 16);
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          mma_ss(leader, tmem + 128 * c + g * KT, qt + (g * L::QSUB + k * 32) / 16,
+          mma_ss(leader, tmem + 128 * (s % NS) + g * KT, qd + (g * L::QSUB + k * 32) / 16,
                  kb + (g * L::KSUB + k * 32) / 16, idesc_s, k != 0 ? 1u : 0u);
-      tc_commit_by(leader, &s_full[c]);
+      tc_commit_by(leader, &s_full[s % NS]);
     };
-    if (last > 0) issue_qk(0);
-    if (last > 1) issue_qk(1);
-    for (int t = 0; t < last && ok; ++t) {
-      const int c = t & 1, i = t >> 1, b = step_of(t) % NB;
-      ok = __all_sync(0xffffffffu, wait_long(&p_ready[c], i & 1, status, STATUS_MMA_WAIT,
-                                             0x500 | (i & 0xff)));
+    for (int s = 0; s < NS && s < last; ++s) {
+      wait_kv(s);
+      issue_qk(s);
+    }
+    for (int s = 0; s < last && ok; ++s) {
+      const int b = s % NB;
+      wait_kv(s + NS);                           // (ahead of the weights, which come later)
+      if (!ok) break;
+      ok = __all_sync(0xffffffffu, wait_long(&p_ready[s % NS], (s / NS) & 1, status,
+                                             STATUS_MMA_WAIT, 0x500 | (s & 0xff)));
       tc_fence_after();
       if (!ok) break;
       const uint64_t vb = vd + static_cast<uint64_t>(b) * ((L::K_BYTES + L::V_BYTES) / 16);
@@ -278,12 +279,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       for (int g = 0; g < GV; ++g)
 #pragma unroll
         for (int k = 0; k < KT / 16; ++k)
-          mma_ts(leader, tmem_o + 128 * c + g * 64,
-                 tmem + 128 * c + g * KT + k / (KH / 16) * KH + k % (KH / 16) * 8,
-                 vb + (g * L::KSUB + k * 2048) / 16, idesc_o, (i | k) != 0 ? 1u : 0u);
-      if (!pair || c == 1) tc_commit_by(leader, &kv_free[b]);
-      if (t + 2 >= last) tc_commit_by(leader, &o_done[c]);
-      if (t + 2 < last) issue_qk(t + 2);
+          mma_ts(leader, tmem_o + g * 64,
+                 tmem + 128 * (s % NS) + g * KT + k * 8, vb + (g * L::KSUB + k * 2048) / 16, idesc_o, (s | k) != 0 ? 1u : 0u);
+      tc_commit_by(leader, &kv_free[b]);
+      tc_commit_by(leader, &o_done[s % NS]);
+      if (s + NS < last) issue_qk(s + NS);       // (in the place of the weights just used)
     }
     __syncwarp();
   } else if (warp == SCALE_WARP) {
@@ -358,13 +358,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       if (s + 1 < steps) load(s + 1);
     }
   } else if (warp >= SOFTMAX_WARPS) {
-    // ---------------- keys and values: INT8 from global memory (a step ahead, in registers) to FP16
-    // integers in swizzled tiles
+    // ---------------- keys and values: INT8 from global memory (PF steps ahead, in registers) to
+    // FP16 integers in swizzled tiles
     constexpr int DQ = DQ_WARPS * 32;
     constexpr int KI = KT * D / 16 / DQ, VI = KT * L::DV / 16 / DQ;
     const int u = tid - SOFTMAX_WARPS * 32;
-    uint4 kraw[KI], vraw[VI];
-    auto load = [&](int s) {
+    uint4 kraw[L::PF][KI], vraw[L::PF][VI];
+    auto load = [&](int s, uint4(&kr)[KI], uint4(&vr)[VI]) {
       const int key0 = (it.step_lo + s) * KT;
       int page = pages[key0 >> 7];
       if (!known || page < 0 || page >= num_pages) page = 0;           // (the scale warp reports it)
@@ -372,13 +372,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
         const int x = u + i * DQ, key = x / (D / 16), c = x % (D / 16);
-        kraw[i] = *reinterpret_cast<const uint4*>(kc + ((slot + key) * kvh + h) * D + c * 16);
+        kr[i] = *reinterpret_cast<const uint4*>(kc + ((slot + key) * kvh + h) * D + c * 16);
       }
 #pragma unroll
       for (int i = 0; i < VI; ++i) {
         const int x = u + i * DQ, key = x / (L::DV / 16), c = x % (L::DV / 16);
-        vraw[i] = *reinterpret_cast<const uint4*>(vc + ((slot + key) * kvh + h) * D +
-                                                  vpart * L::DV + c * 16);
+        vr[i] = *reinterpret_cast<const uint4*>(vc + ((slot + key) * kvh + h) * D +
+                                                vpart * L::DV + c * 16);
       }
     };
     auto place = [&](unsigned char* to, const uint4& raw, int key, int c) {
@@ -392,47 +392,49 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + !swap)) = hi;
     };
     bool ok = true;
-    if (steps > 0) load(0);
-    for (int s = 0; s < steps; ++s) {
-      const int b = s % NB;
-      if (s >= NB)
-        ok = wait_long(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, s & 0xff);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      unsigned char* buf = smem + L::KV_OFF + b * (L::K_BYTES + L::V_BYTES);
 #pragma unroll
-      for (int i = 0; i < KI; ++i) {
-        const int x = u + i * DQ;
-        place(buf, kraw[i], x / (D / 16), x % (D / 16));
-      }
+    for (int f = 0; f < L::PF; ++f)
+      if (f < steps) load(f, kraw[f], vraw[f]);
+    for (int s0 = 0; s0 < steps && ok; s0 += L::PF) {
 #pragma unroll
-      for (int i = 0; i < VI; ++i) {
-        const int x = u + i * DQ;
-        place(buf + L::K_BYTES, vraw[i], x / (L::DV / 16), x % (L::DV / 16));
+      for (int f = 0; f < L::PF; ++f) {
+        const int s = s0 + f, b = s % NB;
+        if (s >= steps) break;
+        if (s >= NB)
+          ok = ok && wait_long(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, s & 0xff);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        unsigned char* buf = smem + L::KV_OFF + b * (L::K_BYTES + L::V_BYTES);
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+          const int x = u + i * DQ;
+          place(buf, kraw[f][i], x / (D / 16), x % (D / 16));
+        }
+#pragma unroll
+        for (int i = 0; i < VI; ++i) {
+          const int x = u + i * DQ;
+          place(buf + L::K_BYTES, vraw[f][i], x / (L::DV / 16), x % (L::DV / 16));
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[b]);
+        if (s + L::PF < steps) load(s + L::PF, kraw[f], vraw[f]);
       }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&kv_full[b]);
-      if (s + 1 < steps) load(s + 1);
     }
   } else {
-    // ---------------- softmax: two threads per row, each with half of a step's keys and, of what is
-    // done to O, half of the channels
-    const int c = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, r = quad * 32 + lane;
-    constexpr int CH = L::DV / 2;                // channels of a half, all of one group
-    const int gh = GV == 2 ? half : 0;           // that group
+    // ---------------- softmax: sixteen rows per warp
+    const int quad = warp & 3, half = warp >> 2;
     // ---- the query rows, 16 bytes at a time, zeros where a tile has none
     {
       const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-      constexpr int CPR = D / 8, BATCH = 8;      // 16-byte pieces of a row; loads in flight
-      for (int i0 = tid; i0 < tiles * TILE * CPR; i0 += BATCH * SOFTMAX_WARPS * 32) {
+      constexpr int CPR = D / 8, BATCH = D / 32; // 16-byte pieces of a row; loads in flight
+      for (int i0 = tid; i0 < TILE * CPR; i0 += BATCH * SOFTMAX_WARPS * 32) {
         uint4 v[BATCH];
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
-          const int i = i0 + k * SOFTMAX_WARPS * 32, m = i / CPR, t = m / TILE, qr = m % TILE;
-          const int row = t * P + qr / rep;
+          const int i = i0 + k * SOFTMAX_WARPS * 32, qr = i / CPR, row = qr / rep;
           v[k] = make_uint4(0, 0, 0, 0);
-          if (t < tiles && qr < P * rep && row < it.rows) {
+          if (qr < TILE / rep * rep && row < it.rows) {
             const __half* from =
                 q + (static_cast<size_t>(it.row + row) * qh + h * rep + qr % rep) * D + i % CPR * 8;
             if (wide) {
@@ -446,9 +448,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
         }
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
-          const int i = i0 + k * SOFTMAX_WARPS * 32, m = i / CPR, t = m / TILE, qr = m % TILE;
-          if (t < tiles)
-            *reinterpret_cast<uint4*>(smem + L::Q_OFF + (t * G + i % CPR / 8) * L::QSUB +
+          const int i = i0 + k * SOFTMAX_WARPS * 32, qr = i / CPR;
+          if (qr < TILE)
+            *reinterpret_cast<uint4*>(smem + L::Q_OFF + i % CPR / 8 * L::QSUB +
                                       swz128(qr, i % CPR % 8)) = v[k];
         }
       }
@@ -456,77 +458,51 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
-    const int t = it.pair ? c : 0;
     // TMEM hands scores out as fragments: a thread holds columns 2 qt and 2 qt + 1 of every eight, of
-    // rows qg + 8 i, so that each scale that it loads serves four rows.  (A row per thread loads
-    // all scales for itself: 64 rows behind 16384 keys, 32 / 4 heads of 128, 46 us with four rows
-    // of a warp's lanes each against 27.)
+    // rows qg and qg + 8, so that each scale that it loads serves two rows.
     const int qg = lane >> 2, qt = lane & 3;
-    constexpr int PAIRS = KH / 8;                // pairs of keys of a thread
+    const int row0 = quad * 32 + half * 16;      // of the tile
     auto row_of = [&](int tr) {                  // of row `tr` of the tile, or none
-      return tr < P * rep && t * P + tr / rep < it.rows && known ? it.row + t * P + tr / rep : -1;
+      return tr < TILE / rep * rep && tr / rep < it.rows && known ? it.row + tr / rep : -1;
     };
-    int sees[4];                                 // shared keys that its rows see
+    int sees[2];                                 // shared keys that its rows see
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = row_of(quad * 32 + qg + 8 * i);
-      sees[i] = (row < 0 ? 0 : min(it.shared, row_pos[row] + 1)) - half * KH - 2 * qt;
+    for (int i = 0; i < 2; ++i) {
+      const int row = row_of(row0 + qg + 8 * i);
+      sees[i] = row < 0 ? 0 : min(it.shared, row_pos[row] + 1);
     }
-    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t tmem_s = tmem + 128 * c + half * KH + lane_addr;
-    const uint32_t tmem_oc = tmem_o + 128 * c + half * CH + lane_addr;
-    constexpr uint32_t LANES16 = 16u << 16;
-    // maxima of the two halves, double buffered: a slot is rewritten two exchanges later
-    float* row_max = reinterpret_cast<float*>(smem + L::MAX_OFF) + c * 4 * TILE + quad * 32;
-    auto meet = [&]() {                          // the two warps of these rows
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + c * 4 + quad) : "memory");
-    };
-    auto mine_of = [&](const float(&v)[4]) {     // row qg + 8 qt's
-      return qt < 2 ? (qt == 0 ? v[0] : v[1]) : (qt == 2 ? v[2] : v[3]);
-    };
-    // where this lane's row goes at the end (on the way out a row per lane)
-    const int row = row_of(r);
-    const int part = row < 0 ? -1 : info[row].y + (it.pair ? it.part : 2 * it.part + c);
-    float m_ref[4], l_run[4], unit = 1.f;
+    const int all_see = __reduce_min_sync(0xffffffffu, min(sees[0], sees[1]));
+    const uint32_t lane_addr = static_cast<uint32_t>(row0) << 16;
+    constexpr int PAIRS = KT / 8, CP = CC / 8;   // pairs of keys of a thread, of a step and at a time
+    float m_ref[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, unit[GV];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      m_ref[i] = -INFINITY;
-      l_run[i] = 0.f;
-    }
+    for (int g = 0; g < GV; ++g) unit[g] = 1.f;
     bool ok = true;
-    int mine = 0;                                // turns taken
-    for (int turn = c; turn < turns; turn += 2, ++mine) {
-      const int s = it.pair ? turn >> 1 : turn, b = s % NB;
+    for (int s = 0; s < steps; ++s) {
+      const int b = s % NB;
       // (the scales are the scale warp's plain stores: seen by whoever waits for them)
-      ok = ok && wait_long(&s_full[c], mine & 1, status, STATUS_EPILOGUE_WAIT, s & 0xff) &&
+      ok = wait_long(&s_full[s % NS], (s / NS) & 1, status, STATUS_EPILOGUE_WAIT, s & 0xff) &&
            wait_long(&kv_full[b], (s / NB) & 1, status, STATUS_EPILOGUE_WAIT, 0x100);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) {                                 // a warp that gave up still meets its partner
-        meet();
-        continue;
-      }
+      if (!ok) break;
       tc_fence_after();
+      const uint32_t tmem_s = tmem + 128 * (s % NS) + lane_addr;
       // scales by pairs of keys and groups: those of this thread's pair `j`
       const float* sk = reinterpret_cast<const float*>(smem + L::SCALE_OFF + b * L::SCALES);
       const float* sv = sk + KT * G;
       const float* su = sv + KT * GV;
       const int key0 = (it.step_lo + s) * KT;
-      bool whole = true;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) whole = whole && sees[i] - key0 >= KH;
-      whole = __all_sync(0xffffffffu, whole);
       // ---- scores
-      float2 x[4][PAIRS];
+      float2 x[2][PAIRS];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t raw[G][KH / 2];
+      for (int k0 = 0; k0 < KT; k0 += CC) {
+        uint32_t raw[G][CC / 2];
 #pragma unroll
-        for (int g = 0; g < G; ++g) tmem_ld_frag(tmem_s + hf * LANES16 + g * KT, raw[g]);
+        for (int g = 0; g < G; ++g) tmem_ld_frag(tmem_s + g * KT + k0, raw[g]);
         tc_wait_ld();
 #pragma unroll
-        for (int j = 0; j < PAIRS; ++j) {
-          const float2* w =
-              reinterpret_cast<const float2*>(sk) + (half * (KH / 2) + 4 * j + qt) * G;
+        for (int j = 0; j < CP; ++j) {
+          const float2* w = reinterpret_cast<const float2*>(sk) + (k0 / 2 + 4 * j + qt) * G;
           float2 wg[G];
           if (G == 1) {
             wg[0] = w[0];
@@ -546,166 +522,170 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
               const float2 a = pair_at(raw[g][4 * j + 2 * i], raw[g][4 * j + 2 * i + 1]);
               v = g == 0 ? mul2(a, wg[0]) : fma2(a, wg[g], v);
             }
-            x[2 * hf + i][j] = v;
+            x[i][k0 / 8 + j] = v;
           }
         }
       }
-      if (!whole) {
+      if (all_see < key0 + KT) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < PAIRS; ++j) {
-            if (8 * j >= sees[i] - key0) x[i][j].x = -INFINITY;
-            if (8 * j + 1 >= sees[i] - key0) x[i][j].y = -INFINITY;
+            const int key = key0 + 8 * j + 2 * qt;
+            if (key >= sees[i]) x[i][j].x = -INFINITY;
+            if (key + 1 >= sees[i]) x[i][j].y = -INFINITY;
           }
       }
       // ---- the reference follows the maximum when that is more than LAG above it
-      float top[4];
+      float top[2][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        top[i] = fmaxf(x[i][0].x, x[i][0].y);
+      for (int i = 0; i < 2; ++i) {
+        top[i][0] = fmaxf(x[i][0].x, x[i][0].y);
+        top[i][1] = fmaxf(x[i][1].x, x[i][1].y);
 #pragma unroll
-        for (int j = 1; j < PAIRS; ++j) top[i] = fmaxf(top[i], fmaxf(x[i][j].x, x[i][j].y));
+        for (int j = 2; j < PAIRS; ++j)
+          top[i][j & 1] = fmaxf(top[i][j & 1], fmaxf(x[i][j].x, x[i][j].y));
+        top[i][0] = fmaxf(top[i][0], top[i][1]);
       }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-      float* slot = row_max + (mine & 1) * 2 * TILE;
-      slot[half * TILE + qg + 8 * qt] = mine_of(top);
-      meet();
-      const float now = su[gh];                  // units are powers of two
-      const float same = mine > 0 && now != unit
-                             ? now * __uint_as_float((254u << 23) - __float_as_uint(unit))
-                             : 1.f;
-      bool moves = same != 1.f;
-      float fix[4];
+        for (int i = 0; i < 2; ++i)
+          top[i][0] = fmaxf(top[i][0], __shfl_xor_sync(0xffffffffu, top[i][0], o));
+      bool moves = false;
+      float corr[2], same[GV];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float m_tile = fmaxf(top[i], slot[(1 - half) * TILE + qg + 8 * i]);
-        fix[i] = same;
-        if (m_tile > m_ref[i] + LAG) {           // (from -inf: any score)
-          const float corr = ex2(m_ref[i] - m_tile);
-          l_run[i] *= corr;
-          fix[i] *= corr;
-          m_ref[i] = m_tile;
+      for (int i = 0; i < 2; ++i) {
+        corr[i] = 1.f;
+        if (top[i][0] > m_ref[i] + LAG) {        // (from -inf: any score)
+          corr[i] = ex2(m_ref[i] - top[i][0]);
+          l_run[i] *= corr[i];
+          m_ref[i] = top[i][0];
           moves = true;
         }
       }
-      unit = now;
-      if (mine > 0 && __any_sync(0xffffffffu, moves)) {
-        // the product before this one is through: the scores came behind it
+#pragma unroll
+      for (int g = 0; g < GV; ++g) {             // units are powers of two
+        const float now = su[g];
+        same[g] = now * __uint_as_float((254u << 23) - __float_as_uint(unit[g]));
+        moves = moves || now != unit[g];
+        unit[g] = now;
+      }
+      if (__any_sync(0xffffffffu, moves) && s > 0) {
+        // O has to stand still: the product before this one is through (the one before on its barrier
+        // is, since scores that came behind that have been read)
+        ok = __all_sync(0xffffffffu, wait_long(&o_done[(s - 1) % NS], ((s - 1) / NS) & 1, status,
+                                               STATUS_EPILOGUE_WAIT, 0x180));
+        tc_fence_after();
+        const uint32_t tmem_oc = tmem_o + lane_addr;
+#pragma unroll
+        for (int g = 0; g < GV; ++g)
 #pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {
-          const float f0 = hf == 0 ? fix[0] : fix[2], f1 = hf == 0 ? fix[1] : fix[3];
-#pragma unroll 1
-          for (int d0 = 0; d0 < CH; d0 += 16) {
+          for (int d0 = 0; d0 < 64; d0 += 16) {
             uint32_t o[8];
-            tmem_ld_frag(tmem_oc + hf * LANES16 + d0, o);
+            tmem_ld_frag(tmem_oc + g * 64 + d0, o);
             tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              o[i] = __float_as_uint(__uint_as_float(o[i]) * (i & 2 ? f1 : f0));
-            tmem_st_frag(tmem_oc + hf * LANES16 + d0, o);
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * (corr[i >> 1 & 1] * same[g]));
+            tmem_st_frag(tmem_oc + g * 64 + d0, o);
           }
-        }
       }
       // ---- weights
-      float2 w[PAIRS][GV];
+      float2 neg[2], sum[2];
 #pragma unroll
-      for (int j = 0; j < PAIRS; ++j) {
-        const float2* from =
-            reinterpret_cast<const float2*>(sv) + (half * (KH / 2) + 4 * j + qt) * GV;
-        if (GV == 1) {
-          w[j][0] = from[0];
-        } else {
-          const float4 v = *reinterpret_cast<const float4*>(from);
-          w[j][0] = make_float2(v.x, v.y);
-          w[j][GV - 1] = make_float2(v.z, v.w);
-        }
+      for (int i = 0; i < 2; ++i) {
+        const float n = m_ref[i] == -INFINITY ? 0.f : -m_ref[i];
+        neg[i] = make_float2(n, n);
+        sum[i] = make_float2(0.f, 0.f);
       }
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t packed[GV][KH / 4];
+      for (int k0 = 0; k0 < KT; k0 += CC) {
+        uint32_t packed[GV][CC / 4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float n = m_ref[2 * hf + i] == -INFINITY ? 0.f : -m_ref[2 * hf + i];
-          const float2 neg = make_float2(n, n);
-          float2 sum = make_float2(0.f, 0.f);
+        for (int j = 0; j < CP; ++j) {
+          const float2* from = reinterpret_cast<const float2*>(sv) + (k0 / 2 + 4 * j + qt) * GV;
+          float2 w[GV];
+          if (GV == 1) {
+            w[0] = from[0];
+          } else {
+            const float4 v = *reinterpret_cast<const float4*>(from);
+            w[0] = make_float2(v.x, v.y);
+            w[GV - 1] = make_float2(v.z, v.w);
+          }
 #pragma unroll
-          for (int j = 0; j < PAIRS; ++j) {
-            float2 p = add2(x[2 * hf + i][j], neg);
+          for (int i = 0; i < 2; ++i) {
+            float2 p = add2(x[i][k0 / 8 + j], neg[i]);
             p.x = ex2(p.x);
             p.y = ex2(p.y);
-            sum = add2(sum, p);
+            sum[i] = add2(sum[i], p);
 #pragma unroll
             for (int g = 0; g < GV; ++g) {
-              const float2 v = mul2(p, w[j][g]);
+              const float2 v = mul2(p, w[g]);
               const __half2 hv = __floats2half2_rn(v.x, v.y);
               packed[g][2 * j + i] = *reinterpret_cast<const uint32_t*>(&hv);
             }
           }
-          l_run[2 * hf + i] += sum.x + sum.y;
         }
 #pragma unroll
-        for (int g = 0; g < GV; ++g)
-          tmem_st_pairs(tmem_s + hf * LANES16 + g * KT, packed[g]);
+        for (int g = 0; g < GV; ++g) tmem_st_pairs(tmem_s + g * KT + k0 / 2, packed[g]);
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) l_run[i] += sum[i].x + sum[i].y;
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[c]);
+      if (lane == 0) mbar_arrive(&p_ready[s % NS]);
     }
-    // ---- this part of the rows' softmax.  The ring is free when both contexts' products are through:
-    // a warp puts 32 rows of 32 channels there and writes whole lines.
-    for (int k = 0; k < 2; ++k)
-      if (k < turns) ok = ok && wait_long(&o_done[k], 0, status, STATUS_EPILOGUE_WAIT, 0x200);
+    // ---- this part of the rows' softmax, from here on a row per lane.  The ring is free when the last
+    // product is through: a warp puts 32 rows of half of the channels there and writes whole lines.
+    const int r = quad * 32 + lane, row = row_of(r);
+    const int part = row < 0 ? -1 : info[row].y + it.part;
+    ok = ok && wait_long(&o_done[(steps - 1) % NS], ((steps - 1) / NS) & 1, status,
+                         STATUS_EPILOGUE_WAIT, 0x200);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
-    const bool some = ok && mine > 0;
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], o);
-    row_max[half * TILE + qg + 8 * qt] = mine_of(l_run);          // (the turns' maxima are read)
-    if (half == 0) row_max[2 * TILE + qg + 8 * qt] = mine_of(m_ref);
+      for (int i = 0; i < 2; ++i) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], o);
+    float* stat = reinterpret_cast<float*>(smem + L::STAT_OFF);
+    if (qt < 2) {
+      stat[row0 + qg + 8 * qt] = qt == 0 ? l_run[0] : l_run[1];
+      stat[TILE + row0 + qg + 8 * qt] = qt == 0 ? m_ref[0] : m_ref[1];
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_WARPS * 32) : "memory");
     const size_t at = static_cast<size_t>(part) * qh + h * rep + r % rep;
-    const float back = __uint_as_float((254u << 23) - __float_as_uint(unit));
-    unsigned char* out = smem + L::KV_OFF + warp * L::OUT_WARP;
-    meet();
     if (half == 0 && vpart == 0 && part >= 0)
-      part_ml[at] = some ? make_float2(row_max[2 * TILE + lane], row_max[lane] + row_max[TILE + lane])
-                         : make_float2(-INFINITY, 0.f);
-#pragma unroll 1
-    for (int d0 = 0; d0 < CH; d0 += 32) {
+      part_ml[at] = ok ? make_float2(stat[TILE + r], stat[r]) : make_float2(-INFINITY, 0.f);
+    constexpr int SUB = L::SUB;
+    const int d_lo = half * SUB;                 // this warp's channels, all of one group
+    const float last_unit = GV == 2 && half == 1 ? unit[GV - 1] : unit[0];
+    const float back = ok ? __uint_as_float((254u << 23) - __float_as_uint(last_unit)) : 0.f;
+    unsigned char* slab = smem + L::KV_OFF + warp * (32 * SUB * 4);
+    auto cell = [](int row, int chunk) {
+      return row * (SUB * 4) + (chunk ^ (row & (SUB / 4 - 1))) * 16;
+    };
 #pragma unroll
-      for (int e = 0; e < 32; e += 16) {
-        uint32_t o[16];
-        if (some) {
-          tmem_ld_x16(tmem_oc + d0 + e, o);
-          tc_wait_ld();
-        }
+    for (int d0 = 0; d0 < SUB; d0 += 16) {
+      uint32_t o[16];
+      tmem_ld_x16(tmem_o + d_lo + d0 + (static_cast<uint32_t>(quad * 32) << 16), o);
+      tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (some)
-            v = make_float4(__uint_as_float(o[i]) * back, __uint_as_float(o[i + 1]) * back,
-                            __uint_as_float(o[i + 2]) * back, __uint_as_float(o[i + 3]) * back);
-          *reinterpret_cast<float4*>(out + swz128(lane, (e + i) / 4)) = v;
-        }
-      }
-      __syncwarp();
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(slab + cell(lane, (d0 + i) / 4)) =
+            make_float4(__uint_as_float(o[i]) * back, __uint_as_float(o[i + 1]) * back,
+                        __uint_as_float(o[i + 2]) * back, __uint_as_float(o[i + 3]) * back);
+    }
+    __syncwarp();
+    constexpr int CHUNKS = SUB / 4, ROWS = 32 / CHUNKS;          // rows that a warp writes at a time
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int from = i * 4 + lane / 8;
-        const size_t to = __shfl_sync(0xffffffffu, static_cast<unsigned long long>(at), from);
-        if (__shfl_sync(0xffffffffu, part, from) >= 0)
-          *reinterpret_cast<float4*>(part_o + to * D + vpart * L::DV + half * CH + d0 +
-                                     lane % 8 * 4) =
-              *reinterpret_cast<const float4*>(out + swz128(from, lane % 8));
-      }
-      __syncwarp();
+    for (int i = 0; i < 32 / ROWS; ++i) {
+      const int from = i * ROWS + lane / CHUNKS;
+      const size_t to = __shfl_sync(0xffffffffu, static_cast<unsigned long long>(at), from);
+      if (__shfl_sync(0xffffffffu, part, from) >= 0)
+        *reinterpret_cast<float4*>(part_o + to * D + vpart * L::DV + d_lo + lane % CHUNKS * 4) =
+            *reinterpret_cast<const float4*>(slab + cell(from, lane % CHUNKS));
     }
   }
   tc_fence_before();

@@ -273,60 +273,52 @@ class SharedPrefix:
         self._args = (ptr(self.items), len(items), ptr(self.info), ptr(self.part_buffer),
                       self.parts, self.splits, ptr(self.scratch), max(1, self.own_keys))
 
-    # Microseconds of a step of keys for two tiles and for one, of a CTA besides its steps, and of a
-    # megabyte of parts to be written and read.
-    PAIR_US, SINGLE_US, CTA_US, PART_US = 1.1, 0.6, 4.0, 0.4
+    # Microseconds of a step of keys, of a CTA besides its steps, and of a megabyte of parts to be
+    # written and read.
+    STEP_US, CTA_US, PART_US = 0.65, 4.0, 0.4
 
     def _split(self, groups):
         """Which CTAs take which rows and keys: (items, (shared keys, first part, parts, 0) of every
-        row, parts in all).  A unit is one or two tiles of rows; the units' keys are cut so that the
-        CTAs fill their waves and the longest of them ends soonest."""
+        row, parts in all).  A unit is a tile of rows; the units' keys are cut so that the CTAs fill
+        their waves and the longest of them ends soonest."""
         step = native.lib().orinfer_shared_step(self.head_dim)
-        rep = self.qh // self.kvh
-        per = 128 // rep                               # rows of a tile
+        per = 128 // (self.qh // self.kvh)             # rows of a tile
         units, info = [], [[0, 0, 0, 0] for _ in range(self.rows)]
         for first, n, keys in groups:
-            at = first
-            while at < first + n:
-                left = first + n - at
-                pair = left > per
-                took = min(left, 2 * per if pair else per)
-                units.append((at, took, (keys + step - 1) // step, keys, pair))
-                at += took
+            units += [(at, min(per, first + n - at), -(-keys // step), keys)
+                      for at in range(first, first + n, per)]
         if not units:
             return [], info, 0
         columns = self.kvh * max(1, self.head_dim // 128)
-        cost = [s * (self.PAIR_US if pair else self.SINGLE_US) for _, _, s, _, pair in units]
         bytes_of = self.qh * self.head_dim * 4e-6      # a part of a row, in megabytes
 
         def cut(limit):
-            """Parts of every unit where no CTA's steps take longer than ``limit``."""
-            return [min(u[2], max(1, -(-c // limit))) for c, u in zip(cost, units)]
+            """Parts of every unit where no CTA takes more than ``limit`` steps."""
+            return [-(-u[2] // limit) for u in units]
 
         best = None
-        for waves in range(-(-len(units) * columns // 148), -(-len(units) * columns // 148) + 3):
-            room = max(len(units), waves * 148 // columns)
-            lo, hi = 0.0, max(cost)
-            for _ in range(30):
-                mid = (lo + hi) / 2
-                lo, hi = (lo, mid) if mid > 0 and sum(cut(mid)) <= room else (mid, hi)
-            for limit in {hi, hi * 1.25, hi * 1.6, hi * 2.2, hi * 4, max(cost)}:
-                parts = [int(x) for x in cut(limit)]
-                mb = sum(p * u[1] * (1 if u[4] else 2) for p, u in zip(parts, units)) * bytes_of
-                longest = max(c / p for c, p in zip(cost, parts))
+        waves = -(-len(units) * columns // 148)
+        for room in ((waves + i) * 148 // columns for i in range(3)):
+            lo, hi = 1, max(u[2] for u in units)       # the fewest steps that fit the waves
+            while lo < hi:
+                mid = (lo + hi) // 2
+                lo, hi = (lo, mid) if sum(cut(mid)) <= room else (mid + 1, hi)
+            for limit in {lo, lo * 5 // 4 + 1, lo * 8 // 5 + 1, 2 * lo + 1, 4 * lo + 1}:
+                parts = cut(limit)
+                mb = sum(p * u[1] for p, u in zip(parts, units)) * bytes_of
+                longest = max(-(-u[2] // p) for p, u in zip(parts, units))
                 took = -(-sum(parts) * columns // 148)
-                us = took * (longest + self.CTA_US) + mb * self.PART_US
+                us = took * (longest * self.STEP_US + self.CTA_US) + mb * self.PART_US
                 if best is None or us < best[0]:
                     best = us, parts
         items, total = [], 0
-        for (at, n, steps, keys, pair), parts in zip(units, best[1]):
-            records = parts if pair else 2 * parts     # one tile leaves one for each context
+        for (at, n, steps, keys), parts in zip(units, best[1]):
             for i in range(n):
-                info[at + i] = [keys, total + i * records, records, 0]
-            total += n * records
-            items += [[at, n, steps * p // parts, steps * (p + 1) // parts, keys, p, int(pair), 0]
+                info[at + i] = [keys, total + i * parts, parts, 0]
+            total += n * parts
+            items += [[at, n, steps * p // parts, steps * (p + 1) // parts, keys, p, 0, 0]
                       for p in range(parts)]
-        items.sort(key=lambda x: (x[2] - x[3]) * (1 + x[6]))       # the longest first
+        items.sort(key=lambda x: x[2] - x[3])          # the longest first
         return items, info, total
 
 
