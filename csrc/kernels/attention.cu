@@ -167,6 +167,10 @@ __device__ __forceinline__ void attn_finish(const float (*s_o)[R][D], const floa
                                             const __half* gate, __half* out, float* scratch,
                                             const SharedParts& parts = SharedParts()) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // The kernel in front makes the shared parts and nothing that came before; it let this one start
+  // when all its CTAs had waited for what lies before it, so that only here there is something to
+  // wait for.
+  if (SHARED && parts.pending) grid_wait();
   __syncthreads();
   if (idle) return;
   for (int r = apart ? 0 : warp; r < rep; r += apart ? 1 : ATTN_WARPS) {   // a head per warp
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(
     float* __restrict__ scratch, int rep, int apart_keys, const SharedParts parts) {
   constexpr int G = AttnTile<D>::G, KB = AttnTile<D>::KB;
   constexpr int NT = KB / 8, UT = KB / 16;         // 8-key score tiles, 16-key value tiles
-  grid_wait();
+  if (!SHARED || !parts.pending) grid_wait();      // (SHARED: see attn_finish)
   grid_release();
   const int row = blockIdx.x, split = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -598,7 +602,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
     int apart_keys, int* status, const SharedParts parts) {
   using T = DigitTile<D>;
   constexpr int G = T::G, KB = T::KB, KSTEPS = T::KSTEPS;
-  grid_wait();
+  if (!SHARED || !parts.pending) grid_wait();      // (SHARED: see attn_finish)
   grid_release();
   const int row = blockIdx.x, split = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -1156,7 +1160,9 @@ static int launch_attn(const __half* q, const __half* gate, const int* row_req, 
   if (runtime_ensure_init() != cudaSuccess) return -2;
   const bool early = attn_starts_early(D, static_cast<long long>(rows) * kvh * splits);
   auto start = [&](auto kernel, size_t smem, auto... args) {
-    if (early)
+    if (SHARED && parts.pending)
+      launch_overlapped(kernel, grid, ATTN_WARPS * 32, smem, stream, args...);
+    else if (early)
       launch_early(kernel, grid, ATTN_WARPS * 32, smem, stream, args...);
     else
       kernel<<<grid, ATTN_WARPS * 32, smem, stream>>>(args...);

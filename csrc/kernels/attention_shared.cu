@@ -132,33 +132,6 @@ __device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t (&r
                "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
                : "memory");
 }
-// mbar_wait for warps that wait long: suspended for up to 20 us at a time, so that sixteen of them do
-// not take the issue slots of those that work.
-__device__ __forceinline__ bool wait_long(uint64_t* bar, uint32_t parity, int* status, int code,
-                                          int detail) {
-  long long start = 0, limit = 0;
-  for (uint32_t spins = 1;; ++spins) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
-        : "memory");
-    if (done) return true;
-    if ((spins & 255u) == 0) {
-      if (limit == 0) {
-        limit = wait_limit(status);
-        start = clock64();
-      } else if (clock64() - start > limit) {
-        report_status(status, code, detail);
-        return false;
-      }
-    }
-  }
-}
-
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -244,10 +217,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     const uint64_t kd = umma_desc(smem_u32(smem + L::KV_OFF), 16, 1024);
     const uint64_t vd = umma_desc(smem_u32(smem + L::KV_OFF + L::K_BYTES), L::KSUB, 1024);
     const int last = warp_same(steps);
-    bool ok = __all_sync(0xffffffffu, wait_long(q_full, 0, status, STATUS_MMA_WAIT, 0x300));
+    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, status, STATUS_MMA_WAIT, 0x300));
     auto wait_kv = [&](int s) {
       if (ok && s < last)
-        ok = __all_sync(0xffffffffu, wait_long(&kv_full[s % NB], (s / NB) & 1, status,
+        ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[s % NB], (s / NB) & 1, status,
                                                STATUS_MMA_WAIT, 0x400 | (s & 0xff)));
     };
     auto issue_qk = [&](int s) {
@@ -270,7 +243,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       const int b = s % NB;
       wait_kv(s + NS);                           // (ahead of the weights, which come later)
       if (!ok) break;
-      ok = __all_sync(0xffffffffu, wait_long(&p_ready[s % NS], (s / NS) & 1, status,
+      ok = __all_sync(0xffffffffu, mbar_wait(&p_ready[s % NS], (s / NS) & 1, status,
                                              STATUS_MMA_WAIT, 0x500 | (s & 0xff)));
       tc_fence_after();
       if (!ok) break;
@@ -319,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     for (int s = 0; s < steps; ++s) {
       const int b = s % NB, live = it.shared - (it.step_lo + s) * KT;
       if (s >= NB)
-        ok = ok && wait_long(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, 0x600);
+        ok = ok && mbar_wait(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, 0x600);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       float* sk = reinterpret_cast<float*>(smem + L::SCALE_OFF + b * L::SCALES);
@@ -401,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
         const int s = s0 + f, b = s % NB;
         if (s >= steps) break;
         if (s >= NB)
-          ok = ok && wait_long(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, s & 0xff);
+          ok = ok && mbar_wait(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, s & 0xff);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         unsigned char* buf = smem + L::KV_OFF + b * (L::K_BYTES + L::V_BYTES);
@@ -481,8 +454,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     for (int s = 0; s < steps; ++s) {
       const int b = s % NB;
       // (the scales are the scale warp's plain stores: seen by whoever waits for them)
-      ok = wait_long(&s_full[s % NS], (s / NS) & 1, status, STATUS_EPILOGUE_WAIT, s & 0xff) &&
-           wait_long(&kv_full[b], (s / NB) & 1, status, STATUS_EPILOGUE_WAIT, 0x100);
+      ok = mbar_wait(&s_full[s % NS], (s / NS) & 1, status, STATUS_EPILOGUE_WAIT, s & 0xff) &&
+           mbar_wait(&kv_full[b], (s / NB) & 1, status, STATUS_EPILOGUE_WAIT, 0x100);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -574,7 +547,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       if (__any_sync(0xffffffffu, moves) && s > 0) {
         // O has to stand still: the product before this one is through (the one before on its barrier
         // is, since scores that came behind that have been read)
-        ok = __all_sync(0xffffffffu, wait_long(&o_done[(s - 1) % NS], ((s - 1) / NS) & 1, status,
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(s - 1) % NS], ((s - 1) / NS) & 1, status,
                                                STATUS_EPILOGUE_WAIT, 0x180));
         tc_fence_after();
         const uint32_t tmem_oc = tmem_o + lane_addr;
@@ -641,7 +614,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     // product is through: a warp puts 32 rows of half of the channels there and writes whole lines.
     const int r = quad * 32 + lane, row = row_of(r);
     const int part = row < 0 ? -1 : info[row].y + it.part;
-    ok = ok && wait_long(&o_done[(steps - 1) % NS], ((steps - 1) / NS) & 1, status,
+    ok = ok && mbar_wait(&o_done[(steps - 1) % NS], ((steps - 1) / NS) & 1, status,
                          STATUS_EPILOGUE_WAIT, 0x200);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
@@ -737,6 +710,7 @@ extern "C" int orinfer_attention_shared(
   if (rep != 1 && rep != 2 && rep != 4 && rep != 8 && !(rep == 5 && head_dim == 128)) return -1;
   if (runtime_ensure_init() != cudaSuccess) return -2;
   SharedParts shared;
+  shared.pending = n_items > 0;
   shared.rows = reinterpret_cast<const int4*>(rows_info);
   shared.o = parts;
   shared.ml = reinterpret_cast<const float2*>(parts + static_cast<size_t>(n_parts) * qh * head_dim);

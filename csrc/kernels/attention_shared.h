@@ -9,6 +9,7 @@
 namespace orinfer {
 
 struct SharedParts {
+  int pending = 0;                 // the kernel in front makes the parts: they are waited for, no more
   const int4* rows = nullptr;      // per row: shared keys, first part, parts, -
   const float* o = nullptr;        // [parts][query heads][D]: sums of weighted values
   const float2* ml = nullptr;      // [parts][query heads]: the weights' reference and their sum

@@ -601,8 +601,8 @@ int runtime_new_slot();
 // recurrence).
 constexpr long long EARLY_CTAS = 4 * 148;
 template <class... P, class... A>
-void launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                  A&&... args) {
+void launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
+                       cudaStream_t stream, A&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -612,9 +612,22 @@ void launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cuda
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  const long long ctas = static_cast<long long>(grid.x) * grid.y * grid.z;
-  cfg.numAttrs = ctas <= EARLY_CTAS ? 1 : 0;
+  cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);   // failures: cudaGetLastError
+}
+template <class... P, class... A>
+void launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                  A&&... args) {
+  if (static_cast<long long>(grid.x) * grid.y * grid.z <= EARLY_CTAS) {
+    launch_overlapped(kernel, grid, block, smem, stream, args...);
+    return;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
 // ---------------------------------------------------------------- math
