@@ -116,38 +116,39 @@ __device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
 
-// A head's shared parts join its own keys' sums `o` of channel lane + 32 i, `m` and `l`; a warp
-// together.  Eight parts at a time: each is a load of its own to wait for.
+// A head's shared parts (info: the row's entry) join its own keys' sums `o` of channel lane + 32 i, `m`
+// and `l`; a warp together.  Sums are asked for ahead of the references that weigh them, sixteen parts
+// at a time: each is a load of its own to wait for.
 template <int D>
-__device__ __forceinline__ void attn_join(const SharedParts& parts, int row, int head, int qh,
+__device__ __forceinline__ void attn_join(const SharedParts& parts, const int4& info, int head, int qh,
                                           float& m, float& l, float (&o)[D / 32]) {
+  constexpr int AHEAD = D > 128 ? 8 : 16;
   const int lane = threadIdx.x & 31;
-  const int4 info = parts.rows[row];
   const float2* ml = parts.ml + static_cast<size_t>(info.y) * qh + head;
   const float* po = parts.o + (static_cast<size_t>(info.y) * qh + head) * D + lane;
-  float top = m;
-  for (int i = lane; i < info.z; i += 32) top = fmaxf(top, ml[static_cast<size_t>(i) * qh].x);
-  top = warp_max(top);
-  const float own = m == -INFINITY ? 0.f : exp2f(m - top);
-  l *= own;
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) o[k] *= own;
-  m = top;
   for (int i0 = 0; i0 < info.z; i0 += 32) {
-    const float2 p = i0 + lane < info.z ? ml[static_cast<size_t>(i0 + lane) * qh]
-                                        : make_float2(-INFINITY, 0.f);
-    const float f = p.x == -INFINITY ? 0.f : exp2f(p.x - m);
-    l += warp_sum(p.y * f);
     const int n = min(32, info.z - i0);
-    for (int i = 0; i < n; i += 8) {
-      float v[8][D / 32];
+    float v[AHEAD][D / 32];
+    auto ask = [&](int i) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
         for (int k = 0; k < D / 32; ++k)
           v[j][k] = i + j < n ? po[static_cast<size_t>(i0 + i + j) * qh * D + 32 * k] : 0.f;
+    };
+    ask(0);
+    const float2 p = lane < n ? ml[static_cast<size_t>(i0 + lane) * qh] : make_float2(-INFINITY, 0.f);
+    const float top = fmaxf(m, warp_max(p.x));
+    const float own = m == -INFINITY ? 0.f : exp2f(m - top);
+    const float f = p.x == -INFINITY ? 0.f : exp2f(p.x - top);
+    m = top;
+    l = fmaf(l, own, warp_sum(p.y * f));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+    for (int k = 0; k < D / 32; ++k) o[k] *= own;
+    for (int i = 0; i < n; i += AHEAD) {
+      if (i > 0) ask(i);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
         const float fj = __shfl_sync(0xffffffffu, f, (i + j) & 31);
         if (i + j < n) {
 #pragma unroll
@@ -170,6 +171,7 @@ __device__ __forceinline__ void attn_finish(const float (*s_o)[R][D], const floa
   // The kernel in front makes the shared parts and nothing that came before; it let this one start
   // when all its CTAs had waited for what lies before it, so that only here there is something to
   // wait for.
+  const int4 info = SHARED ? parts.rows[row] : make_int4(0, 0, 0, 0);
   if (SHARED && parts.pending) grid_wait();
   __syncthreads();
   if (idle) return;
@@ -193,7 +195,7 @@ __device__ __forceinline__ void attn_finish(const float (*s_o)[R][D], const floa
 #pragma unroll
         for (int w = 0; w < ATTN_WARPS; ++w) o[k] = fmaf(s_o[w][r][lane + 32 * k], f[w], o[k]);
       }
-      attn_join<D>(parts, row, h * rep + r, qh, m, l, o);
+      attn_join<D>(parts, info, h * rep + r, qh, m, l, o);
 #pragma unroll
       for (int k = 0; k < D / 32; ++k)
         attn_store(l > 0.f ? o[k] / l : 0.f, gate, out, head * D + lane + 32 * k);
@@ -1051,25 +1053,8 @@ __global__ void attn_merge_kernel(
   float m = -INFINITY;
   for (int s = lane; s < splits; s += 32) m = fmaxf(m, rec[s * (D + 2)]);
   m = warp_max(m);
-  // the shared parts' records follow the row's own
-  const int4 info = SHARED ? parts.rows[row] : make_int4(0, 0, 0, 0);
-  const float2* ml = parts.ml + static_cast<size_t>(info.y) * qh + head;
-  const float* po = parts.o + (static_cast<size_t>(info.y) * qh + head) * D;
-  if (SHARED) {
-    for (int s = lane; s < info.z; s += 32) m = fmaxf(m, ml[static_cast<size_t>(s) * qh].x);
-    m = warp_max(m);
-  }
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
     float l = 0.f, o = 0.f;
-    if (SHARED) {
-#pragma unroll 4
-      for (int s = 0; s < info.z; ++s) {
-        const float2 p = ml[static_cast<size_t>(s) * qh];
-        const float f = p.x == -INFINITY ? 0.f : exp2f(p.x - m);
-        l = fmaf(p.y, f, l);
-        o = fmaf(po[static_cast<size_t>(s) * qh * D + d], f, o);
-      }
-    }
     for (int s0 = 0; s0 < splits; s0 += 32) {
       const int n = min(32, splits - s0);
       const float* own = rec + (s0 + min(lane, n - 1)) * (D + 2);
@@ -1087,6 +1072,38 @@ __global__ void attn_merge_kernel(
           if (b + i < n) {
             l = fmaf(l_s, fs, l);
             o = fmaf(v[i], fs, o);
+          }
+        }
+      }
+    }
+    if (SHARED) {                                // a warp's 32 channels of the shared parts
+      const int4 info = parts.rows[row];
+      const float2* ml = parts.ml + static_cast<size_t>(info.y) * qh + head;
+      const float* po = parts.o + (static_cast<size_t>(info.y) * qh + head) * D + d;
+      float top = m;
+      for (int s0 = 0; s0 < info.z; s0 += 32) {
+        const int n = min(32, info.z - s0);
+        float v[16];
+        auto ask = [&](int s) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            v[i] = s + i < n ? po[static_cast<size_t>(s0 + s + i) * qh * D] : 0.f;
+        };
+        ask(0);
+        const float2 p =
+            lane < n ? ml[static_cast<size_t>(s0 + lane) * qh] : make_float2(-INFINITY, 0.f);
+        const float now = fmaxf(top, warp_max(p.x));
+        const float was = top == -INFINITY ? 0.f : exp2f(top - now);
+        const float f = p.x == -INFINITY ? 0.f : exp2f(p.x - now);
+        top = now;
+        l = fmaf(l, was, warp_sum(p.y * f));
+        o *= was;
+        for (int s = 0; s < n; s += 16) {
+          if (s > 0) ask(s);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float fs = __shfl_sync(0xffffffffu, f, (s + i) & 31);
+            if (s + i < n) o = fmaf(v[i], fs, o);
           }
         }
       }

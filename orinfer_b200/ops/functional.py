@@ -241,10 +241,12 @@ class SharedPrefix:
     same pages as far as their first ``keys`` keys lie on them (whole pages, as ``fork_pages`` and
     the prefix cache share them).  Groups do not overlap; rows of no group share nothing.
     ``max_kv_len`` bounds the keys that any row sees while the plan is in use, so that one plan
-    serves the steps of a decode loop.  It holds the call's workspace: one stream at a time."""
+    serves the steps of a decode loop.  It holds the call's workspace: one stream at a time.  A batch
+    whose shared keys are cheaper read again by every row is left to the row kernels, unless
+    ``force``."""
 
     def __init__(self, groups: Sequence[Tuple[int, int, int]], rows: int, *, qh: int, kvh: int,
-                 head_dim: int, max_kv_len: int, device):
+                 head_dim: int, max_kv_len: int, device, force: bool = False):
         _need(rows >= 0 and max_kv_len >= 0, "rows and max_kv_len are not negative")
         _need(head_dim in (64, 128, 256), "heads of 64, 128 or 256 channels")
         rep = qh // kvh if kvh > 0 and qh % kvh == 0 else 0
@@ -260,24 +262,30 @@ class SharedPrefix:
         self.device = torch.device(device)
         groups = [(int(f), int(n), int(k)) for f, n, k in groups if n > 0 and k > 0]
         self.longest = max((k for _, _, k in groups), default=0)
-        items, info, self.parts = self._split(groups)
+        items, info, self.parts = self._split(groups, force)
         put = lambda v: torch.tensor(v, dtype=torch.int32, device=self.device)
         self.items = put(items) if items else None
         self.info = put(info if info else [[0] * 4])
         f32 = lambda n: torch.empty(n, dtype=torch.float32, device=self.device) if n else None
         self.part_buffer = f32(self.parts * qh * (head_dim + 2))
-        # the own keys, by the row kernels
-        self.own_keys = max_kv_len - min((i[0] for i in info), default=0)
-        self.splits = attention_splits(max(1, self.own_keys), max(1, rows), kvh)
+        # The own keys, by the row kernels: as many as the middle row may have.  Beside a prefix they
+        # are split only where they are long: a merge is a launch of its own.
+        shared = sorted(i[0] for i in info)
+        self.own_keys = max(1, max_kv_len - (shared[len(shared) // 2] if items else 0))
+        self.splits = attention_splits(self.own_keys, max(1, rows), kvh)
+        if items:
+            self.splits = max(1, min(self.splits, self.own_keys // 512))
         self.scratch = f32(rows * qh * self.splits * (head_dim + 2)) if self.splits > 1 else None
         self._args = (ptr(self.items), len(items), ptr(self.info), ptr(self.part_buffer),
-                      self.parts, self.splits, ptr(self.scratch), max(1, self.own_keys))
+                      self.parts, self.splits, ptr(self.scratch), self.own_keys)
 
-    # Microseconds of a step of keys, of a CTA besides its steps, and of a megabyte of parts to be
-    # written and read.
-    STEP_US, CTA_US, PART_US = 0.65, 4.0, 0.4
+    # Microseconds of a step of keys, of a CTA besides its steps, of a megabyte of parts to be written
+    # and read, and of a megabyte of keys and values that the row kernels would read again.  32 / 8
+    # heads of 128, 200 own keys, with the prefix shared and without: 2 rows behind 2048 keys 17 and
+    # 11 us, 16 rows 20 and 18, 32 rows 17 and 27, 64 rows 22 and 56, 64 behind 8192 34 and 185.
+    STEP_US, CTA_US, PART_US, AGAIN_US = 0.9, 5.0, 0.4, 0.16
 
-    def _split(self, groups):
+    def _split(self, groups, force):
         """Which CTAs take which rows and keys: (items, (shared keys, first part, parts, 0) of every
         row, parts in all).  A unit is a tile of rows; the units' keys are cut so that the CTAs fill
         their waves and the longest of them ends soonest."""
@@ -311,6 +319,10 @@ class SharedPrefix:
                 us = took * (longest * self.STEP_US + self.CTA_US) + mb * self.PART_US
                 if best is None or us < best[0]:
                     best = us, parts
+        again = sum((n - 1) * keys for _, n, keys in groups) * \
+            self.kvh * (2 * self.head_dim + 4 * (self.head_dim // 64)) * 1e-6
+        if not force and again * self.AGAIN_US < best[0]:          # cheaper read again than shared
+            return [], info, 0
         items, total = [], 0
         for (at, n, steps, keys), parts in zip(units, best[1]):
             for i in range(n):
@@ -329,36 +341,38 @@ def attention_shared(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: tor
     """:func:`attention` of a batch whose rows share prefixes (``plan``): a shared key is read once
     for all rows of its group.  A row sees keys 0..row_pos[r]; one at position -1 sees none and
     gives zeros."""
-    _cuda(q, gate, row_req, row_pos, page_table, kcache, vcache, kscale, vscale, out)
-    n, qh, d = q.shape
-    _need(n == plan.rows and qh == plan.qh and d == plan.head_dim, "q is not what the plan is for")
-    _need(q.dtype == torch.float16 and q.is_contiguous(), "q: contiguous FP16 [rows, heads, D]")
-    _need(gate is None or (gate.dtype == torch.float16 and gate.is_contiguous()
-                           and gate.numel() == q.numel()), "gate: contiguous FP16, as q")
-    _need(row_req.dtype == torch.int32 and row_pos.dtype == torch.int32
-          and page_table.dtype == torch.int32, "row_req, row_pos, page_table: int32")
-    _need(row_req.numel() >= n and row_pos.numel() >= n and page_table.dim() == 2
-          and page_table.is_contiguous(), "row_req, row_pos: [rows]; page_table: [requests, pages]")
-    pages, cell = kcache.shape[0], (kcache.shape[0], 128, plan.kvh)
-    _need(kcache.shape == (*cell, d) and vcache.shape == (*cell, d)
-          and kcache.dtype == torch.int8 and vcache.dtype == torch.int8
-          and kcache.is_contiguous() and vcache.is_contiguous(),
-          "caches: contiguous int8 [pages, 128, kvh, D]")
-    _need(kscale.shape == (*cell, d // 64) and vscale.shape == (*cell, d // 64)
-          and kscale.dtype == torch.float16 and vscale.dtype == torch.float16
-          and kscale.is_contiguous() and vscale.is_contiguous(),
-          "scales: contiguous FP16 [pages, 128, kvh, D / 64]")
+    n, d, kvh, i32, f16 = plan.rows, plan.head_dim, plan.kvh, torch.int32, torch.float16
+    _need(q.shape == (n, plan.qh, d) and q.dtype == f16 and q.is_contiguous(),
+          "q: contiguous FP16 [rows, heads, D], as the plan has them")
+    _need(row_req.dtype == i32 and row_pos.dtype == i32 and page_table.dtype == i32
+          and row_req.numel() >= n and row_pos.numel() >= n and row_req.is_contiguous()
+          and row_pos.is_contiguous() and page_table.dim() == 2 and page_table.is_contiguous(),
+          "row_req, row_pos: int32 [rows]; page_table: int32 [requests, pages]")
+    slots, width = page_table.shape
+    pages = kcache.shape[0]
+    for t in (kcache, vcache):
+        _need(t.shape == (pages, 128, kvh, d) and t.dtype == torch.int8 and t.is_contiguous(),
+              "caches: contiguous int8 [pages, 128, kvh, D]")
+    for t in (kscale, vscale):
+        _need(t.shape == (pages, 128, kvh, d // 64) and t.dtype == f16 and t.is_contiguous(),
+              "scales: contiguous FP16 [pages, 128, kvh, D / 64]")
+    if gate is not None:
+        _need(gate.dtype == f16 and gate.is_contiguous() and gate.numel() == n * plan.qh * d,
+              "gate: contiguous FP16, as q")
     if out is None:
-        out = torch.empty(n, qh * d, dtype=torch.float16, device=q.device)
+        out = torch.empty(n, plan.qh * d, dtype=f16, device=q.device)
     else:
-        _need(out.dtype == torch.float16 and out.is_contiguous() and out.numel() == q.numel(),
+        _need(out.dtype == f16 and out.is_contiguous() and out.numel() == n * plan.qh * d,
               "out: contiguous FP16 [rows, heads * D]")
-    _need(plan.longest <= page_table.shape[1] * 128, "more shared keys than the table has pages")
-    _need(q.device == plan.info.device, "the plan is for another device")
+    where = plan.info.device
+    _need(where.type == "cuda", "the plan is not for a GPU")
+    for t in (q, gate, row_req, row_pos, page_table, kcache, vcache, kscale, vscale, out):
+        _need(t is None or t.device == where, "every tensor on the plan's GPU")
+    _need(plan.longest <= width * 128, "more shared keys than the table has pages")
     check(native.lib().orinfer_attention_shared(
-        ptr(q), ptr(gate), ptr(row_req), ptr(row_pos), ptr(page_table), page_table.shape[0],
-        page_table.shape[1], ptr(kcache), ptr(vcache), ptr(kscale), ptr(vscale), ptr(out), n, qh,
-        plan.kvh, d, pages, *plan._args, stream()), "attention_shared")
+        ptr(q), ptr(gate), ptr(row_req), ptr(row_pos), ptr(page_table), slots, width, ptr(kcache),
+        ptr(vcache), ptr(kscale), ptr(vscale), ptr(out), n, plan.qh, kvh, d, pages, *plan._args,
+        stream()), "attention_shared")
     count_launches((plan.items is not None) + (2 if plan.splits > 1 else 1))
     return out
 

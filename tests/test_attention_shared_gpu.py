@@ -90,7 +90,8 @@ def check(dev, spec, args, max_kv_len=None, plan=None, out=None):
     if plan is None:
         plan = F.SharedPrefix(spec, q.shape[0], qh=q.shape[1], kvh=args[5].shape[2],
                               head_dim=q.shape[2],
-                              max_kv_len=max_kv_len or int(pos.max()) + 1, device=dev)
+                              max_kv_len=max_kv_len or int(pos.max()) + 1, device=dev,
+                              force=True)
     out = F.attention_shared(*args, plan, out=out)
     ref, size, reach = R.attention_rows(*args)
     off = (out.double().view_as(ref) - ref).abs()
@@ -203,7 +204,8 @@ def test_a_long_cache_with_offsets_past_32_bits(dev):
     q = torch.randn(3, 32, d, generator=g).half().to(dev)
     args = (q, None, i32([0, 1, 2]), i32([299, 256, 383]), table.to(dev), kc, vc, ks, ks)
     check(dev, [(0, 3, 256)], args)
-    plan = F.SharedPrefix([], 3, qh=32, kvh=kvh, head_dim=d, max_kv_len=512, device=dev)
+    plan = F.SharedPrefix([], 3, qh=32, kvh=kvh, head_dim=d, max_kv_len=512, device=dev,
+                          force=True)
     check(dev, [], args, plan=plan)
 
 
@@ -212,7 +214,8 @@ def test_one_plan_serves_the_steps_of_a_loop(dev):
     plan that knows them; the same call twice gives the same bits."""
     from orinfer_b200.ops import functional as F
     spec, args = batch(dev, [(384, [400, 450, 520])], 8, 2, 128, seed=11)
-    plan = F.SharedPrefix(spec, 3, qh=8, kvh=2, head_dim=128, max_kv_len=4096, device=dev)
+    plan = F.SharedPrefix(spec, 3, qh=8, kvh=2, head_dim=128, max_kv_len=4096, device=dev,
+                          force=True)
     first, _ = check(dev, spec, args, plan=plan)
     first = first.clone()
     out = torch.empty_like(first)
@@ -220,10 +223,33 @@ def test_one_plan_serves_the_steps_of_a_loop(dev):
     assert again is out and torch.equal(first, again)
 
 
+@pytest.mark.parametrize("rows,shared,items", [(2, 384, False), (8, 1024, False), (128, 1024, True),
+                                               (40, 5120, True)])
+def test_what_is_cheaper_read_again_is_not_shared(dev, rows, shared, items):
+    from orinfer_b200.ops import functional as F
+    spec, args = batch(dev, [(shared, [shared + 1 + 7 * r % 90 for r in range(rows)])], 32, 8, 128,
+                       seed=rows)
+    plan = F.SharedPrefix(spec, rows, qh=32, kvh=8, head_dim=128, max_kv_len=shared + 90, device=dev)
+    assert (plan.items is not None) == items
+    check(dev, spec, args, plan=plan)
+
+
+def test_own_keys_in_parts(dev):
+    """Own keys that are long enough to be split, behind a prefix and without one, gated and not."""
+    for qh, kvh, d in ((8, 2, 128), (4, 2, 64), (8, 1, 256)):
+        spec, args = batch(dev, [(256, [2500, 300, 256])], qh, kvh, d, loners=(1700, 40, 0), seed=d,
+                           gated=d == 256)
+        from orinfer_b200.ops import functional as F
+        plan = F.SharedPrefix(spec, 6, qh=qh, kvh=kvh, head_dim=d, max_kv_len=2600, device=dev,
+                              force=True)
+        assert plan.splits > 1
+        check(dev, spec, args, plan=plan)
+
+
 def test_on_another_stream_and_in_a_graph(dev):
     from orinfer_b200.ops import functional as F
     spec, args = batch(dev, [(640, [700, 641, 900, 780]), (256, [300, 257])], 32, 8, 128, seed=13)
-    plan = F.SharedPrefix(spec, 6, qh=32, kvh=8, head_dim=128, max_kv_len=900, device=dev)
+    plan = F.SharedPrefix(spec, 6, qh=32, kvh=8, head_dim=128, max_kv_len=900, device=dev, force=True)
     want = F.attention_shared(*args, plan).clone()
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
