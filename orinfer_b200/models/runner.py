@@ -145,6 +145,9 @@ class Packet:
     # Host-side bound on the keys that the prefill chunks reach (0: ``max_kv_len``, which also
     # counts the decode rows); their attention launch is chosen by it.
     max_chunk_kv: int = 0
+    # Single rows whose contexts begin with the same pages (samples of one prompt): the plan of
+    # their attention, for exactly the packet's rows.  None = every row reads all of its keys.
+    shared: Optional[F.SharedPrefix] = None
 
     def ensure_segments(self) -> None:
         if self.segments is not None:
@@ -221,6 +224,14 @@ class ModelRunner:
                      gate_out=ws.gate, rows=rows)
         gated = cfg.gated_attention and lw.qkv.n == cfg.q_dim + 2 * cfg.kv_dim
         gate = ws.gate if gated else None
+        if p.shared is not None:
+            if p.chunks is not None or p.attend_pos is not None:
+                raise ValueError("a packet with shared prefixes has single rows only")
+            F.attention_shared(ws.q[:rows], None if gate is None else gate[:rows], p.row_req,
+                               p.row_pos, p.page_table, self.kv.k[kv_slot], self.kv.v[kv_slot],
+                               self.kv.ks[kv_slot], self.kv.vs[kv_slot], p.shared,
+                               out=ws.attn[:rows])
+            return
         row_rows = rows
         if p.chunks is not None and p.attend_pos is None and cfg.head_dim in (64, 128, 256):
             done = F.attention_prefill(ws.q, gate, p.chunks, p.max_q_len, p.page_table,
