@@ -116,6 +116,14 @@ __device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
 
+// A row kernel beside the kernel of the prefix is started once all of that kernel's CTAs have waited for
+// what lies before them: queries, positions and keys are complete and in L2 by then.  It does not wait
+// for them itself, so that it drops here what its SM may still hold of older contents.
+__device__ __forceinline__ void attn_start_beside() {
+  __threadfence();
+  asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
 // A head's shared parts (info: the row's entry) join its own keys' sums `o` of channel lane + 32 i, `m`
 // and `l`; a warp together.  Sums are asked for ahead of the references that weigh them, sixteen parts
 // at a time: each is a load of its own to wait for.
@@ -238,7 +246,10 @@ __global__ void __launch_bounds__(
     float* __restrict__ scratch, int rep, int apart_keys, const SharedParts parts) {
   constexpr int G = AttnTile<D>::G, KB = AttnTile<D>::KB;
   constexpr int NT = KB / 8, UT = KB / 16;         // 8-key score tiles, 16-key value tiles
-  if (!SHARED || !parts.pending) grid_wait();      // (SHARED: see attn_finish)
+  if (SHARED && parts.pending)
+    attn_start_beside();                           // (it waits in attn_finish)
+  else
+    grid_wait();
   grid_release();
   const int row = blockIdx.x, split = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -604,7 +615,10 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
     int apart_keys, int* status, const SharedParts parts) {
   using T = DigitTile<D>;
   constexpr int G = T::G, KB = T::KB, KSTEPS = T::KSTEPS;
-  if (!SHARED || !parts.pending) grid_wait();      // (SHARED: see attn_finish)
+  if (SHARED && parts.pending)
+    attn_start_beside();                           // (it waits in attn_finish)
+  else
+    grid_wait();
   grid_release();
   const int row = blockIdx.x, split = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;

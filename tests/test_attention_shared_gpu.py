@@ -267,6 +267,51 @@ def test_on_another_stream_and_in_a_graph(dev):
         assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("rows,shared,qh,kvh,d", [(24, 1024, 8, 2, 128), (70, 512, 4, 2, 64),
+                                                  (9, 640, 16, 2, 256)])
+def test_steps_that_follow_each_other_without_a_wait(dev, rows, shared, qh, kvh, d):
+    """A decode loop writes the queries of each step over those of the last and its keys behind
+    theirs.  In one graph the row kernels run beside the prefix's kernel, and the next step's beside
+    them; with a wait after every call they cannot.  The results have the same bits."""
+    from orinfer_b200.ops import functional as F
+    steps, g = 24, torch.Generator().manual_seed(rows)
+    width = (shared + 128) // 128
+    spec, args = batch(dev, [(shared, [shared + 1] * rows)], qh, kvh, d, seed=rows)
+    _, _, row_req, _, table, kc, vc, ks, vs = args
+    assert table.shape[1] >= width
+    qkv = torch.randn(steps, rows, (qh + 2 * kvh) * d, generator=g).half().to(dev)
+    pos = (torch.arange(steps, dtype=torch.int32)[:, None] + shared
+           + torch.zeros(rows, dtype=torch.int32)).to(dev)
+    plan = F.SharedPrefix(spec, rows, qh=qh, kvh=kvh, head_dim=d, max_kv_len=shared + steps,
+                          device=dev, force=True)
+    q = torch.empty(rows, qh, d, dtype=torch.float16, device=dev)
+    cos, sin = (torch.empty(rows, d // 2, dtype=torch.float32, device=dev) for _ in range(2))
+    caches = [t.clone() for t in (kc, vc, ks, vs)]
+
+    def loop(out, wait):
+        for t, first in zip((kc, vc, ks, vs), caches):
+            t.copy_(first)
+        for s in range(steps):
+            F.rope_table(pos[s], d, 1e6, cos, sin, rows=rows)
+            F.qk_rope_kv(qkv[s], None, None, cos, sin, row_req, pos[s], table, kc, vc, ks, vs, qh=qh,
+                         kvh=kvh, head_dim=d, gated=False, eps=1e-6, zero_centered=False, q_out=q,
+                         gate_out=None, rows=rows)
+            wait()
+            F.attention_shared(q, None, row_req, pos[s], table, kc, vc, ks, vs, plan, out=out[s])
+            wait()
+
+    want, got = (torch.empty(steps, rows, qh * d, dtype=torch.float16, device=dev) for _ in range(2))
+    loop(want, torch.cuda.synchronize)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loop(got, lambda: None)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        assert torch.equal(got, want)
+    assert float(want.float().abs().max()) > 0 and not torch.equal(want[0], want[1])
+
+
 def test_refusals(dev):
     from orinfer_b200.ops import functional as F
     from orinfer_b200.ops.native import KernelError
