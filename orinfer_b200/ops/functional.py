@@ -381,7 +381,7 @@ def attention_shared(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: tor
 class CachePages:
     """The tensors of a paged cache (each contiguous [pages, 128, ...], all on one device), as the
     page operators address them: ``KVPool.cache_pages()`` makes one for a model's cache.  It holds
-    the tensors."""
+    the tensors, and the calls' workspace: one stream at a time."""
 
     UNIT = 16384                                   # bytes that a CTA copies at a time
 
@@ -404,32 +404,42 @@ class CachePages:
         self.token_bytes, self.units = put(sizes, torch.int32), put(units, torch.int32)
         self._args = (ptr(self.bases), ptr(self.token_bytes), ptr(self.units), len(units),
                       self.pages)
+        self._words = [torch.empty(4 + 3 * (self.pages // 2 + 1), dtype=torch.int32,
+                                   device=self.device)]
+
+    def _work(self, words: int) -> int:
+        """Address of as many words.  Smaller buffers stay too: a captured graph may hold them."""
+        if self._words[-1].numel() < words:
+            self._words.append(torch.empty(2 * words, dtype=torch.int32, device=self.device))
+        return self._words[-1].data_ptr()
 
 
-def _tables(table, lens, refs, out):
-    """The tensors that a page operator writes: ``out``, or new ones like its inputs."""
-    ins = [t for t in (table, lens, refs) if t is not None]
-    _cuda(*ins)
+def _tables(ins, out):
+    """The tensors that a page operator writes: ``out``, or new ones like its inputs (the table
+    first)."""
+    table, i32 = ins[0], torch.int32
+    where = table.device
     for t in ins:
-        _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == ins[0].device,
-              "table, lens, refs: contiguous int32")
-    _need(table.dim() == 2 and table.numel() > 0, "table: [slots, pages of a slot]")
-    _need(lens is None or lens.shape == table.shape[:1], "lens: [slots]")
+        if t.dtype != i32 or not t.is_contiguous() or not t.is_cuda or t.device != where:
+            raise native.KernelError("table, lens, refs: contiguous int32, on one GPU")
+    if table.dim() != 2 or table.numel() == 0:
+        raise native.KernelError("table: [slots, pages of a slot]")
     if out is None:
         return [torch.empty_like(t) for t in ins]
     _need(len(out) == len(ins), "out: a tensor for each input")
     for t, o in zip(ins, out):
-        _need(o.shape == t.shape and o.dtype == t.dtype and o.is_contiguous()
-              and o.device == t.device, "out: tensors like the inputs")
-    return list(out)
+        _need(o.shape == t.shape and o.dtype == i32 and o.is_contiguous() and o.device == where,
+              "out: tensors like the inputs")
+    return out
 
 
 def _slots(*lists):
-    _cuda(*lists)
+    n = lists[0].numel()
     for t in lists:
-        _need(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()
-              and t.shape == lists[0].shape, "lists of slots or pages: int32 [n]")
-    return lists[0].shape[0]
+        if (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous()
+                or not t.is_cuda):
+            raise native.KernelError("lists of slots or pages: int32 [n], on a GPU")
+    return n
 
 
 def copy_pages(cache: CachePages, source: torch.Tensor, target: torch.Tensor,
@@ -456,15 +466,15 @@ def fork_pages(cache: CachePages, table: torch.Tensor, lens: torch.Tensor, refs:
     a child that is not empty, named twice or a parent as well, a parent's page that nobody holds);
     nothing is changed then."""
     n = _slots(parents, children)
-    t, l, r = _tables(table, lens, refs, out)
-    _need(refs.shape == (cache.pages,), "refs: [pages]")
+    t, l, r = _tables((table, lens, refs), out)
     slots, width = table.shape
-    lib = native.lib()
-    work = torch.empty(4 + 4 * n + slots, dtype=torch.int32, device=table.device)
-    status = torch.empty(1, dtype=torch.int32, device=table.device)
-    check(lib.orinfer_fork_pages(
-        *cache._args, ptr(table), ptr(t), ptr(lens), ptr(l), ptr(refs), ptr(r), ptr(parents),
-        ptr(children), n, slots, width, ptr(work), ptr(status), stream()), "fork_pages")
+    if lens.dim() != 1 or lens.numel() != slots or refs.dim() != 1 or refs.numel() != cache.pages:
+        raise native.KernelError("lens: [slots], refs: [pages]")
+    status = torch.empty(1, dtype=torch.int32, device=cache.device)
+    check(native.lib().orinfer_fork_pages(
+        *cache._args, table.data_ptr(), t.data_ptr(), lens.data_ptr(), l.data_ptr(),
+        refs.data_ptr(), r.data_ptr(), parents.data_ptr(), children.data_ptr(), n, slots, width,
+        cache._work(4 + 4 * n + slots), status.data_ptr(), stream()), "fork_pages")
     count_launches(2)
     return t, l, r, status
 
@@ -475,11 +485,14 @@ def free_pages(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, slot
     loses a reference.  Returns (table, lens, refs); ``out`` may be the inputs.  A slot or page that
     does not exist, or a page that nobody holds, is left alone and reported by the status word."""
     n = _slots(slots)
-    t, l, r = _tables(table, lens, refs, out)
-    _need(refs.dim() == 1 and refs.numel() > 0, "refs: [pages]")
+    t, l, r = _tables((table, lens, refs), out)
+    total, width = table.shape
+    pages = refs.numel()
+    if lens.dim() != 1 or lens.numel() != total or refs.dim() != 1 or pages == 0:
+        raise native.KernelError("lens: [slots], refs: [pages]")
     check(native.lib().orinfer_free_pages(
-        ptr(table), ptr(t), ptr(lens), ptr(l), ptr(refs), ptr(r), ptr(slots), n, table.shape[0],
-        table.shape[1], refs.shape[0], stream()), "free_pages")
+        table.data_ptr(), t.data_ptr(), lens.data_ptr(), l.data_ptr(), refs.data_ptr(),
+        r.data_ptr(), slots.data_ptr(), n, total, width, pages, stream()), "free_pages")
     count_launches(2 if t is table or l is lens else 1)
     return t, l, r
 
@@ -488,14 +501,15 @@ def compact_pages(cache: CachePages, table: torch.Tensor, refs: torch.Tensor, *,
     """Moves the pages that are held to the front: with L of them, the k-th one above page L goes to
     the k-th free page of 1..L.  Returns (table, refs, moved): ``moved`` int32 [pages] says where
     each page has gone.  ``out`` (table, refs) may be the inputs."""
-    t, r = _tables(table, None, refs, out)
-    _need(refs.shape == (cache.pages,), "refs: [pages]")
-    lib = native.lib()
+    t, r = _tables((table, refs), out)
+    if refs.dim() != 1 or refs.numel() != cache.pages:
+        raise native.KernelError("refs: [pages]")
+    slots, width = table.shape
     moved = torch.empty_like(refs)
-    work = torch.empty(4 + 3 * (cache.pages // 2 + 1), dtype=torch.int32, device=table.device)
-    check(lib.orinfer_compact_pages(
-        *cache._args, ptr(table), ptr(t), ptr(refs), ptr(r), ptr(moved), table.shape[0],
-        table.shape[1], ptr(work), stream()), "compact_pages")
+    check(native.lib().orinfer_compact_pages(
+        *cache._args, table.data_ptr(), t.data_ptr(), refs.data_ptr(), r.data_ptr(),
+        moved.data_ptr(), slots, width, cache._work(4 + 3 * (cache.pages // 2 + 1)), stream()),
+        "compact_pages")
     count_launches(2)
     return t, r, moved
 
@@ -752,47 +766,50 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     [rows]): 1 where nothing is permitted, 2 where a logit or a permitted token's score is not
     finite (the host law refuses those rows), the mask does not exist or the row has more than 32768
     biases, else 0.  ``out`` may be ``logits``."""
-    _cuda(logits, history, history_len, repetition, presence, frequency, bias_start, bias_ids,
-          bias_values, mask, mask_rows, out, flags)
-    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.stride(1) == 1
-          and logits.shape[1] > 0, "logits: fp32 [rows, vocab], rows in one piece")
+    i32, f64 = torch.int32, torch.float64
+    for t in (logits, history, history_len, repetition, presence, frequency, bias_start, bias_ids,
+              bias_values, mask, mask_rows, out, flags):
+        if t is not None and not t.is_cuda:
+            raise native.KernelError("device op called with a CPU tensor")
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise native.KernelError("logits: fp32 [rows, vocab], rows in one piece")
     rows, vocab = logits.shape
+    _need(vocab > 0, "logits: fp32 [rows, vocab], rows in one piece")
     hist_stride = cap = bias_total = mask_stride = masks = 0
+
+    def of_rows(t, dtype, n=rows):
+        return t is not None and t.dtype == dtype and t.shape == (n,) and t.is_contiguous()
+
     if history is not None:
-        _need(history.dtype == torch.int32 and history.dim() == 2 and history.shape[0] == rows
-              and (history.shape[1] < 2 or history.stride(1) == 1), "history: int32 [rows, n]")
-        _need(history_len is not None and history_len.dtype == torch.int32
-              and history_len.shape == (rows,) and history_len.is_contiguous(),
-              "history_len: int32 [rows]")
-        hist_stride, cap = history.stride(0), history.shape[1]
-    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        _need(t is None or (t.dtype == torch.float64 and t.shape == (rows,) and t.is_contiguous()
-                            and history is not None), f"{name}: fp64 [rows], with a history")
+        if history.dtype != i32 or history.dim() != 2:
+            raise native.KernelError("history: int32 [rows, n]")
+        (of, cap), (hist_stride, step) = history.shape, history.stride()
+        if of != rows or (cap > 1 and step != 1) or not of_rows(history_len, i32):
+            raise native.KernelError("history: int32 [rows, n], history_len: int32 [rows]")
+    for t in (repetition, presence, frequency):
+        if t is not None and (history is None or not of_rows(t, f64)):
+            raise native.KernelError("repetition, presence, frequency: fp64 [rows], with a history")
     if bias_start is not None:
-        _need(bias_start.dtype == torch.int32 and bias_start.shape == (rows + 1,)
-              and bias_start.is_contiguous(), "bias_start: int32 [rows + 1]")
-        _need(bias_ids is not None and bias_values is not None and bias_ids.dtype == torch.int32
-              and bias_values.dtype == torch.float64 and bias_ids.dim() == 1
-              and bias_ids.shape == bias_values.shape and bias_ids.is_contiguous()
-              and bias_values.is_contiguous(), "bias_ids: int32, bias_values: fp64, [entries]")
-        bias_total = bias_ids.shape[0]
+        _need(of_rows(bias_start, i32, rows + 1), "bias_start: int32 [rows + 1]")
+        _need(bias_ids is not None and bias_values is not None, "bias_ids and bias_values")
+        bias_total = bias_ids.numel()
+        _need(of_rows(bias_ids, i32, bias_total) and of_rows(bias_values, f64, bias_total),
+              "bias_ids: int32, bias_values: fp64, [entries]")
     if mask is not None:
-        _need(mask.dtype == torch.int32 and mask.dim() == 2 and mask.stride(1) == 1
+        _need(mask.dtype == i32 and mask.dim() == 2 and mask.stride(1) == 1
               and mask.shape[1] >= (vocab + 31) // 32, "mask: int32 [m, (vocab + 31) / 32]")
-        _need(mask.shape[0] >= rows if mask_rows is None else
-              (mask_rows.dtype == torch.int32 and mask_rows.shape == (rows,)
-               and mask_rows.is_contiguous()), "mask_rows: int32 [rows], or a mask per row")
         mask_stride, masks = mask.stride(0), mask.shape[0]
+        _need(masks >= rows if mask_rows is None else of_rows(mask_rows, i32),
+              "mask_rows: int32 [rows], or a mask per row")
     if out is None:
         out = torch.empty(rows, vocab, dtype=torch.float32, device=logits.device)
     else:
         _need(out.shape == logits.shape and out.dtype == torch.float32 and out.stride(1) == 1,
               "out: fp32 [rows, vocab]")
     if flags is None:
-        flags = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        flags = torch.empty(rows, dtype=i32, device=logits.device)
     else:
-        _need(flags.shape == (rows,) and flags.dtype == torch.int32 and flags.is_contiguous(),
-              "flags: int32 [rows]")
+        _need(of_rows(flags, i32), "flags: int32 [rows]")
     check(native.lib().orinfer_process_logits(
         ptr(logits), logits.stride(0), ptr(history), hist_stride, cap, ptr(history_len),
         ptr(repetition), ptr(presence), ptr(frequency), ptr(bias_start), ptr(bias_ids),
