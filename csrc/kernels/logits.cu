@@ -25,12 +25,12 @@
 namespace orinfer {
 namespace lp {
 
-constexpr int THREADS = 512;
 constexpr int CTAS = 8;                            // per row
 constexpr int TABLE = 24576;                       // tokens that a CTA looks after at a time, at most
 constexpr int LIST = 4096;                         // of which so many are listed
-constexpr int BIASES = 64 * THREADS;               // of a row, at most
+constexpr int BIASES = 32768;                      // of a row, at most
 constexpr int BATCH = 5;                           // loads of a thread in flight
+constexpr int SEG = 2048;                          // tokens of a history that a CTA sorts at a time
 constexpr int SHORT = 32767;                       // tokens of a history whose counts take 16 bits
 
 struct Args {
@@ -93,15 +93,40 @@ __host__ __device__ inline int slice_of(int vocab) {
 }
 constexpr int MASK_WORDS = 1024;                   // of a slice, held in shared memory
 
-template <class W>
-__global__ void __launch_bounds__(THREADS, 2) process_logits_kernel(const Args a) {
+// All CTAs of the cluster have started where one of them is past the wait.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// What the CTA `rank` of the cluster has at the place of `p`.
+__device__ __forceinline__ int cluster_load(const int* p, int rank) {
+  int v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_u32(smem_u32(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned cluster_load(const unsigned short* p, int rank) {
+  unsigned short v;
+  asm volatile("ld.shared::cluster.u16 %0, [%1];" : "=h"(v) : "r"(mapa_u32(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+template <class W, int THREADS, int RESIDENT>
+__global__ void __launch_bounds__(THREADS, RESIDENT) process_logits_kernel(const Args a) {
+  constexpr int WINS = (BIASES / THREADS + 64) / 64;       // words of a bit per bias entry of a thread
   extern __shared__ __align__(16) unsigned char space[];
   __shared__ unsigned s_mask[MASK_WORDS + 1];
   __shared__ unsigned short list[LIST];
+  __shared__ unsigned short sorted[SEG];           // what this CTA sorted, by the CTA that looks after it
+  __shared__ int s_count[CTAS], s_start[CTAS + 1]; // tokens for each of them, and where they begin
+  __shared__ int s_at[CTAS], s_sum[CTAS + 1];      // what the CTAs sorted for this one
   __shared__ int s_flags[CTAS];
-  __shared__ int s_listed, s_bad;
+  __shared__ int s_listed;
   grid_wait();
   grid_release();
+  cluster_arrive();                                // see cluster_wait
   const int row = blockIdx.x / CTAS, rank = blockIdx.x % CTAS, tid = threadIdx.x;
   const int words = table_words(a.vocab);
   Words<W> table{reinterpret_cast<W*>(space)};
@@ -141,7 +166,6 @@ __global__ void __launch_bounds__(THREADS, 2) process_logits_kernel(const Args a
   // (a mask that does not exist, more biases than the winners' bits)
   const bool odd = (which >= 0 && !mask) || entries > BIASES;
   const bool biased = entries > 0 && !odd, special = seen > 0 || biased;
-  if (tid == 0) s_bad = odd;
   // the slice's permissions (from global memory where they are too many)
   const bool held = slice <= 32 * MASK_WORDS;
   unsigned any = mask ? 0u : 1u;
@@ -153,7 +177,8 @@ __global__ void __launch_bounds__(THREADS, 2) process_logits_kernel(const Args a
     }
 
   // ---- the words of tokens rank + 8 (done .. done + words): occurrences, and which have a bias
-  unsigned long long wins = 0;                     // this thread's bias entries that count
+  unsigned long long wins[WINS] = {};              // this thread's bias entries that count
+  auto won = [&](int k) { return (WINS > 1 && k > 63 ? wins[WINS - 1] : wins[0]) >> (k & 63) & 1; };
   auto own_at = [&](int token, int done) {         // a token's word, or something past the table
     const unsigned id = token;
     return id < static_cast<unsigned>(a.vocab) && id % CTAS == static_cast<unsigned>(rank)
@@ -173,49 +198,126 @@ __global__ void __launch_bounds__(THREADS, 2) process_logits_kernel(const Args a
     }
     return t;
   };
+  const bool sorts = seen > 4 * THREADS;           // (else each CTA looks through all of them)
+  constexpr int TAKES = (SEG / 4 + THREADS - 1) / THREADS;
   auto make_table = [&](int done) {
-    int4 next = tokens_at(4 * tid), after = tokens_at(4 * (THREADS + tid));
+    int4 next[TAKES];
+    int part = 0;
+    auto ask = [&](int from) {                     // this CTA's part of the tokens from there on
+      part = min(SEG, ((seen - from + CTAS - 1) / CTAS + 3) / 4 * 4);
+#pragma unroll
+      for (int k = 0; k < TAKES; ++k) {
+        const int i = 4 * (tid + k * THREADS);
+        next[k] = i < part ? tokens_at(from + rank * part + i) : make_int4(-1, -1, -1, -1);
+      }
+    };
+    if (sorts)
+      ask(0);
+    else
+      next[0] = tokens_at(4 * tid);
     if (tid == 0) s_listed = 0;
     for (int q = tid; q < words * static_cast<int>(sizeof(W)) / 16; q += THREADS)
       reinterpret_cast<uint4*>(space)[q] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     const unsigned most = words;
     if (biased) {                                  // the last entry of a token is the one that counts
-      wins = 0;
+#pragma unroll
+      for (int w = 0; w < WINS; ++w) wins[w] = 0;
       auto entry_at = [&](int i) { return own_at(a.bias_ids[b_lo + i], done); };
       for (int i = tid; i < entries; i += THREADS)
         if (entry_at(i) < most) table.raise(entry_at(i), i + 1u);
       __syncthreads();
       for (int i = tid, k = 0; i < entries; i += THREADS, ++k)
-        if (entry_at(i) < most && table[entry_at(i)] == i + 1u) wins |= 1ull << k;
-      __syncthreads();
-      for (int i = tid, k = 0; i < entries; i += THREADS, ++k)
-        if (wins >> k & 1) table.set(entry_at(i), BIASED);
+        if (entry_at(i) < most && table[entry_at(i)] == i + 1u) {
+          (k > 63 ? wins[WINS - 1] : wins[0]) |= 1ull << (k & 63);
+          table.set(entry_at(i), BIASED);          // (no other entry of the token has this number)
+        }
       __syncthreads();
     }
-    // tokens met for the first time are listed
-    for (int i = 4 * tid; i < seen; i += 4 * THREADS) {
-      const int4 t = next;
-      next = after;
-      after = tokens_at(i + 8 * THREADS);
-      const unsigned at[4] = {own_at(t.x, done), own_at(t.y, done), own_at(t.z, done),
-                              own_at(t.w, done)};
-      unsigned old[4];
+    auto count = [&](unsigned at) {                // tokens met for the first time are listed
+      if (at >= most || table.count(at) != 0) return;
+      const int to = atomicAdd(&s_listed, 1);
+      if (to < LIST) list[to] = static_cast<unsigned short>(at);
+    };
+    if (!sorts) {
+      count(own_at(next[0].x, done));
+      count(own_at(next[0].y, done));
+      count(own_at(next[0].z, done));
+      count(own_at(next[0].w, done));
+    }
+    for (int from = 0; sorts && from < seen; from += CTAS * SEG) {
+      if (from > 0) ask(from);
+      if (tid < CTAS) s_count[tid] = 0;
+      __syncthreads();
+      unsigned own[4 * TAKES];                     // the token's word, and behind it its place
+      auto place = [&](int e, int token) {
+        const unsigned id = token, at = id / CTAS - done;
+        own[e] = 0xffffffffu;
+        if (id < static_cast<unsigned>(a.vocab) && at < most)
+          own[e] = at | static_cast<unsigned>(atomicAdd(&s_count[id % CTAS], 1)) << 16;
+      };
 #pragma unroll
-      for (int e = 0; e < 4; ++e) old[e] = at[e] < most ? table.count(at[e]) : 1u;
-      const unsigned fresh = (old[0] == 0 ? 1u : 0u) | (old[1] == 0 ? 2u : 0u) |
-                             (old[2] == 0 ? 4u : 0u) | (old[3] == 0 ? 8u : 0u);
-      if (fresh == 0) continue;
-      int to = atomicAdd(&s_listed, __popc(fresh));
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (fresh >> e & 1u) {
-          if (to < LIST) list[to] = static_cast<unsigned short>(at[e]);
-          ++to;
+      for (int k = 0; k < TAKES; ++k) {
+        place(4 * k, next[k].x);
+        place(4 * k + 1, next[k].y);
+        place(4 * k + 2, next[k].z);
+        place(4 * k + 3, next[k].w);
+      }
+      __syncthreads();
+      if (tid < 32) {                              // (a warp: lane c has CTA c's)
+        const int mine = tid < CTAS ? s_count[tid] : 0;
+        int sum = mine;
+        for (int d = 1; d < CTAS; d *= 2) {
+          const int below = __shfl_up_sync(0xffffffffu, sum, d);
+          if (tid >= d) sum += below;
         }
+        if (tid < CTAS) s_start[tid + 1] = sum;
+        if (tid == 0) s_start[0] = 0;
+      }
+      __syncthreads();
+      auto sort = [&](int e, int token) {
+        if (own[e] != 0xffffffffu)
+          sorted[s_start[static_cast<unsigned>(token) % CTAS] + (own[e] >> 16)] =
+              static_cast<unsigned short>(own[e]);
+      };
+#pragma unroll
+      for (int k = 0; k < TAKES; ++k) {
+        sort(4 * k, next[k].x);
+        sort(4 * k + 1, next[k].y);
+        sort(4 * k + 2, next[k].z);
+        sort(4 * k + 3, next[k].w);
+      }
+      __syncthreads();
+      cluster_sync_all();
+      if (tid < 32) {
+        const int at = tid < CTAS ? cluster_load(&s_start[rank], tid) : 0;
+        int sum = tid < CTAS ? cluster_load(&s_start[rank + 1], tid) - at : 0;
+        for (int d = 1; d < CTAS; d *= 2) {
+          const int below = __shfl_up_sync(0xffffffffu, sum, d);
+          if (tid >= d) sum += below;
+        }
+        if (tid < CTAS) {
+          s_at[tid] = at;
+          s_sum[tid + 1] = sum;
+        }
+        if (tid == 0) s_sum[0] = 0;
+      }
+      __syncthreads();
+      for (int i = tid; i < s_sum[CTAS]; i += THREADS) {
+        int c = 0;
+#pragma unroll
+        for (int k = 1; k < CTAS; ++k) c += i >= s_sum[k];
+        count(cluster_load(&sorted[s_at[c] + i - s_sum[c]], c));
+      }
+      if (done > 0 || from + CTAS * SEG < seen) {  // (else the row's barrier is still to come)
+        __syncthreads();
+        cluster_sync_all();                        // what was sorted has been read
+      }
     }
     __syncthreads();
   };
+  __syncwarp();
+  cluster_wait();
   if (special)
     make_table(0);
   else if (mask)
@@ -266,11 +368,24 @@ __global__ void __launch_bounds__(THREADS, 2) process_logits_kernel(const Args a
     if (bias) s += *bias;
     const float f = static_cast<float>(s);
     out[id] = f;
-    if (!isfinite(f)) s_bad = 1;
+    if (!isfinite(f)) atomicMax(a.flags + row, 2);
   };
+  const bool bad = __syncthreads_or(odd || !(nothing == 0.f));
+  const bool some = __syncthreads_or(any);
+  if (tid == 0) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(smem_u32(&s_flags[rank]), 0)),
+                 "r"((bad ? 2 : 0) | (some ? 1 : 0))
+                 : "memory");
+    if (rank == 0) a.flags[row] = 0;
+  }
+  __syncthreads();
+  cluster_sync_all();                              // the row has been streamed
+  if (rank == 0 && tid == 0) {
+    int all = 0;
+    for (int c = 0; c < CTAS; ++c) all |= *reinterpret_cast<volatile int*>(&s_flags[c]);
+    if (all != 1) atomicMax(a.flags + row, all & 2 ? 2 : 1);
+  }
   if (special) {
-    __syncthreads();
-    cluster_sync_all();                            // the row has been streamed
     for (int done = 0;; done += words) {
       auto look_after = [&](unsigned i) {
         write_score((done + static_cast<int>(i)) * CTAS + rank, table[i], nullptr);
@@ -282,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, 2) process_logits_kernel(const Args a
           if (table[i] != 0 && !(table[i] & BIASED)) look_after(i);
       }
       for (int i = tid, k = 0; i < entries && biased; i += THREADS, ++k)
-        if (wins >> k & 1) {
+        if (won(k)) {
           const int id = a.bias_ids[b_lo + i];
           write_score(id, table[own_at(id, done)], a.bias_values + b_lo + i);
         }
@@ -290,20 +405,6 @@ __global__ void __launch_bounds__(THREADS, 2) process_logits_kernel(const Args a
       __syncthreads();
       make_table(done + words);
     }
-  }
-  // ---- flags, in the first CTA
-  const bool bad = __syncthreads_or(!(nothing == 0.f));
-  const bool some = __syncthreads_or(any);
-  if (tid == 0)
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(smem_u32(&s_flags[rank]), 0)),
-                 "r"((bad || s_bad ? 2 : 0) | (some ? 1 : 0))
-                 : "memory");
-  __syncthreads();
-  cluster_sync_all();
-  if (rank == 0 && tid == 0) {
-    int all = 0;
-    for (int c = 0; c < CTAS; ++c) all |= *reinterpret_cast<volatile int*>(&s_flags[c]);
-    a.flags[row] = all & 2 ? 2 : all & 1 ? 0 : 1;
   }
 }
 
@@ -336,12 +437,17 @@ extern "C" int orinfer_process_logits(
                       reinterpret_cast<const unsigned int*>(mask), mask_stride, mask_rows,
                       mask_count, masked, out, out_stride, flags, rows, vocab, bias_total};
   const bool narrow = !history || history_cap <= lp::SHORT;
-  auto kernel = narrow ? lp::process_logits_kernel<uint16_t> : lp::process_logits_kernel<uint32_t>;
-  static const int slot[2] = {runtime_new_slot(), runtime_new_slot()};
-  if (const int e = runtime_allow_smem(slot[narrow], kernel, 4 * lp::TABLE)) return e;
+  const bool few = rows * static_cast<long long>(lp::CTAS) <= 2 * 148;
+  auto kernel = few ? (narrow ? lp::process_logits_kernel<uint16_t, 512, 2>
+                              : lp::process_logits_kernel<uint32_t, 512, 2>)
+                    : (narrow ? lp::process_logits_kernel<uint16_t, 320, 3>
+                              : lp::process_logits_kernel<uint32_t, 320, 3>);
+  static const int slot[4] = {runtime_new_slot(), runtime_new_slot(), runtime_new_slot(),
+                              runtime_new_slot()};
+  if (const int e = runtime_allow_smem(slot[2 * few + narrow], kernel, 4 * lp::TABLE)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * lp::CTAS);
-  cfg.blockDim = dim3(lp::THREADS);
+  cfg.blockDim = dim3(few ? 512 : 320);
   cfg.dynamicSmemBytes = (narrow ? 2 : 4) * static_cast<size_t>(lp::table_words(vocab));
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
