@@ -9,16 +9,22 @@
 //
 // It is a pass over memory, 8 bytes a token.  A cluster of eight CTAs takes a row.  Each CTA streams an
 // eighth of the vocabulary, copying what is permitted, four tokens to a load.  Of the tokens that occur
-// or have a bias it looks after those that leave its rank modulo eight: it reads the whole history
-// (from L2), counts its own in a table in shared memory and lists them, and when the row has been
-// streamed it computes their scores, which whole warps then do, whichever tokens are frequent.
+// or have a bias it looks after those that leave its rank modulo eight: it counts them in a table in
+// shared memory and lists them, and when the row has been streamed it computes their scores, which
+// whole warps then do, whichever tokens are frequent.  Of a long history each CTA sorts an eighth by
+// the CTA that looks after a token, and fetches its own tokens from all eight.  The barriers between
+// these steps are in halves, with the streaming or the counting between them, and all that a row needs
+// besides its logits is asked for at the start: under load each round trip is 2500 cycles.
 //
-// 256 rows of 151936 tokens: 56 us without penalties and masks (a copy takes 49), 68 with a mask per
-// row, 114 with histories of 8000 tokens; one row 4.2, 4.9 and 10.0.  What a history costs is a chain
-// in 32 warps of an SM: four rounds of 1600 cycles of counting, a cluster barrier, 2500 of scores.
+// 256 rows of 151936 tokens: 56 us without penalties and masks (a copy takes 49), 58 with a mask for
+// half of the rows, 64 with histories of 250 tokens, 83 with 8000, 88 with 150 biases too; 64 rows 29,
+// 16 rows 14.5, one row with 900 tokens 6.5.  What bounds it is memory first, then the chain of a CTA
+// (a third of its time streams), of which three share an SM.
 // Tried: scores as a branch of the streaming loop (a slice's few tokens one by one: 256 rows 210),
 // slices of neighbouring tokens counted by atomics in each other's shared memory (155, and 200 where
-// most of the history falls to one slice), the CTA that met a token first looking after it (158).
+// most of the history falls to one slice), the CTA that met a token first looking after it (158), each
+// CTA reading the whole history (118), that by half of its warps while the others stream (121), whole
+// barriers between the steps (97).
 #include "api.h"
 #include "common.cuh"
 
@@ -93,12 +99,13 @@ __host__ __device__ inline int slice_of(int vocab) {
 }
 constexpr int MASK_WORDS = 1024;                   // of a slice, held in shared memory
 
-// All CTAs of the cluster have started where one of them is past the wait.
+// The cluster's barrier in two halves, whole warps each: what a thread wrote before it arrived, the
+// others see past the wait.
 __device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() {
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // What the CTA `rank` of the cluster has at the place of `p`.
@@ -116,6 +123,9 @@ __device__ __forceinline__ unsigned cluster_load(const unsigned short* p, int ra
 template <class W, int THREADS, int RESIDENT>
 __global__ void __launch_bounds__(THREADS, RESIDENT) process_logits_kernel(const Args a) {
   constexpr int WINS = (BIASES / THREADS + 64) / 64;       // words of a bit per bias entry of a thread
+  constexpr int TAKES = (SEG / 4 + THREADS - 1) / THREADS; // fours of tokens that a thread sorts
+  constexpr int HOLDS = (MASK_WORDS + THREADS - 1) / THREADS;
+  constexpr unsigned BIASED = Words<W>::BIASED;
   extern __shared__ __align__(16) unsigned char space[];
   __shared__ unsigned s_mask[MASK_WORDS + 1];
   __shared__ unsigned short list[LIST];
@@ -126,11 +136,11 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) process_logits_kernel(const
   __shared__ int s_listed;
   grid_wait();
   grid_release();
-  cluster_arrive();                                // see cluster_wait
+  cluster_arrive();                                // 1: all CTAs have started
   const int row = blockIdx.x / CTAS, rank = blockIdx.x % CTAS, tid = threadIdx.x;
   const int words = table_words(a.vocab);
+  const unsigned most = words;
   Words<W> table{reinterpret_cast<W*>(space)};
-  constexpr unsigned BIASED = Words<W>::BIASED;
   const float* x = a.logits + row * a.row_stride;
   float* out = a.out + row * a.out_stride;
   // ---- the slice that is streamed: four tokens at a time behind the first 16-byte boundary, where
@@ -155,36 +165,27 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) process_logits_kernel(const
   const double rep = a.repetition ? a.repetition[row] : 1.0;
   const double pres = a.presence ? a.presence[row] : 0.0;
   const double freq = a.frequency ? a.frequency[row] : 0.0;
-  const bool counted = a.history && (rep != 1.0 || pres != 0.0 || freq != 0.0);
-  const int seen = counted ? min(max(a.history_len[row], 0), a.history_cap) : 0;
+  const int len = a.history ? min(max(a.history_len[row], 0), a.history_cap) : 0;
   const int* history = a.history + row * a.history_stride;
   const int b_lo = a.bias_start ? max(a.bias_start[row], 0) : 0;
   const int entries = a.bias_start ? min(a.bias_start[row + 1], a.bias_total) - b_lo : 0;
   const int which = a.mask ? (a.mask_rows ? a.mask_rows[row] : row) : -1;
+  const int seen = rep != 1.0 || pres != 0.0 || freq != 0.0 ? len : 0;
   const unsigned* mask =
       which >= 0 && which < a.mask_count ? a.mask + which * a.mask_stride : nullptr;
   // (a mask that does not exist, more biases than the winners' bits)
   const bool odd = (which >= 0 && !mask) || entries > BIASES;
   const bool biased = entries > 0 && !odd, special = seen > 0 || biased;
-  // the slice's permissions (from global memory where they are too many)
-  const bool held = slice <= 32 * MASK_WORDS;
-  unsigned any = mask ? 0u : 1u;
-  if (mask)
-    for (int w = tid; w < (n + 31) / 32; w += THREADS) {
-      const unsigned bits = mask[lo / 32 + w];
-      if (held) s_mask[w] = bits;
-      any |= n - 32 * w < 32 ? bits & ((1u << (n - 32 * w)) - 1u) : bits;
-    }
+  const bool sorts = seen > 4 * THREADS;           // (else each CTA looks through all of them)
 
-  // ---- the words of tokens rank + 8 (done .. done + words): occurrences, and which have a bias
-  unsigned long long wins[WINS] = {};              // this thread's bias entries that count
-  auto won = [&](int k) { return (WINS > 1 && k > 63 ? wins[WINS - 1] : wins[0]) >> (k & 63) & 1; };
-  auto own_at = [&](int token, int done) {         // a token's word, or something past the table
-    const unsigned id = token;
-    return id < static_cast<unsigned>(a.vocab) && id % CTAS == static_cast<unsigned>(rank)
-               ? id / CTAS - done
-               : 0xffffffffu;
-  };
+  // What a row needs besides its logits is asked for at once, and used as it comes: the slice's
+  // permissions (from global memory later where they are too many), tokens, the first bias.
+  const bool held = slice <= 32 * MASK_WORDS;
+  const int mask_words = mask ? (n + 31) / 32 : 0;
+  unsigned bits[HOLDS];
+#pragma unroll
+  for (int k = 0; k < HOLDS; ++k)
+    bits[k] = held && tid + k * THREADS < mask_words ? mask[lo / 32 + tid + k * THREADS] : 0u;
   const bool wide = (reinterpret_cast<uintptr_t>(history) & 15) == 0;
   auto tokens_at = [&](int i) {                    // four of the history
     int4 t = make_int4(-1, -1, -1, -1);
@@ -198,130 +199,155 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) process_logits_kernel(const
     }
     return t;
   };
-  const bool sorts = seen > 4 * THREADS;           // (else each CTA looks through all of them)
-  constexpr int TAKES = (SEG / 4 + THREADS - 1) / THREADS;
-  auto make_table = [&](int done) {
-    int4 next[TAKES];
-    int part = 0;
-    auto ask = [&](int from) {                     // this CTA's part of the tokens from there on
-      part = min(SEG, ((seen - from + CTAS - 1) / CTAS + 3) / 4 * 4);
+  int4 next[TAKES];
+  auto ask = [&](int from) {                       // this CTA's part of the tokens from there on
+    const int part =
+        sorts ? min(SEG, ((seen - from + CTAS - 1) / CTAS + 3) / 4 * 4) : 4 * THREADS;
 #pragma unroll
-      for (int k = 0; k < TAKES; ++k) {
-        const int i = 4 * (tid + k * THREADS);
-        next[k] = i < part ? tokens_at(from + rank * part + i) : make_int4(-1, -1, -1, -1);
-      }
-    };
-    if (sorts)
-      ask(0);
-    else
-      next[0] = tokens_at(4 * tid);
+    for (int k = 0; k < TAKES; ++k) {
+      const int i = 4 * (tid + k * THREADS);
+      next[k] = i < part ? tokens_at((sorts ? from + rank * part : 0) + i)
+                         : make_int4(-1, -1, -1, -1);
+    }
+  };
+  ask(0);
+  const int bias_id = biased && tid < entries ? a.bias_ids[b_lo + tid] : -1;
+
+  // ---- the words of tokens rank + 8 (done .. done + words): occurrences, and which have a bias
+  unsigned long long wins[WINS] = {};              // this thread's bias entries that count
+  auto won = [&](int k) { return (WINS > 1 && k > 63 ? wins[WINS - 1] : wins[0]) >> (k & 63) & 1; };
+  auto own_at = [&](int token, int done) {         // a token's word, or something past the table
+    const unsigned id = token;
+    return id < static_cast<unsigned>(a.vocab) && id % CTAS == static_cast<unsigned>(rank)
+               ? id / CTAS - done
+               : 0xffffffffu;
+  };
+  auto make_table = [&](int done) {                // without the history
     if (tid == 0) s_listed = 0;
     for (int q = tid; q < words * static_cast<int>(sizeof(W)) / 16; q += THREADS)
       reinterpret_cast<uint4*>(space)[q] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
-    const unsigned most = words;
-    if (biased) {                                  // the last entry of a token is the one that counts
+    if (!biased) return;                           // the last entry of a token is the one that counts
 #pragma unroll
-      for (int w = 0; w < WINS; ++w) wins[w] = 0;
-      auto entry_at = [&](int i) { return own_at(a.bias_ids[b_lo + i], done); };
-      for (int i = tid; i < entries; i += THREADS)
-        if (entry_at(i) < most) table.raise(entry_at(i), i + 1u);
-      __syncthreads();
-      for (int i = tid, k = 0; i < entries; i += THREADS, ++k)
-        if (entry_at(i) < most && table[entry_at(i)] == i + 1u) {
-          (k > 63 ? wins[WINS - 1] : wins[0]) |= 1ull << (k & 63);
-          table.set(entry_at(i), BIASED);          // (no other entry of the token has this number)
-        }
-      __syncthreads();
-    }
-    auto count = [&](unsigned at) {                // tokens met for the first time are listed
-      if (at >= most || table.count(at) != 0) return;
-      const int to = atomicAdd(&s_listed, 1);
-      if (to < LIST) list[to] = static_cast<unsigned short>(at);
-    };
-    if (!sorts) {
-      count(own_at(next[0].x, done));
-      count(own_at(next[0].y, done));
-      count(own_at(next[0].z, done));
-      count(own_at(next[0].w, done));
-    }
-    for (int from = 0; sorts && from < seen; from += CTAS * SEG) {
-      if (from > 0) ask(from);
-      if (tid < CTAS) s_count[tid] = 0;
-      __syncthreads();
-      unsigned own[4 * TAKES];                     // the token's word, and behind it its place
-      auto place = [&](int e, int token) {
-        const unsigned id = token, at = id / CTAS - done;
-        own[e] = 0xffffffffu;
-        if (id < static_cast<unsigned>(a.vocab) && at < most)
-          own[e] = at | static_cast<unsigned>(atomicAdd(&s_count[id % CTAS], 1)) << 16;
-      };
-#pragma unroll
-      for (int k = 0; k < TAKES; ++k) {
-        place(4 * k, next[k].x);
-        place(4 * k + 1, next[k].y);
-        place(4 * k + 2, next[k].z);
-        place(4 * k + 3, next[k].w);
+    for (int w = 0; w < WINS; ++w) wins[w] = 0;
+    auto entry_at = [&](int i) { return own_at(i == tid ? bias_id : a.bias_ids[b_lo + i], done); };
+    for (int i = tid; i < entries; i += THREADS)
+      if (entry_at(i) < most) table.raise(entry_at(i), i + 1u);
+    __syncthreads();
+    for (int i = tid, k = 0; i < entries; i += THREADS, ++k)
+      if (entry_at(i) < most && table[entry_at(i)] == i + 1u) {
+        (k > 63 ? wins[WINS - 1] : wins[0]) |= 1ull << (k & 63);
+        table.set(entry_at(i), BIASED);            // (no other entry of the token has this number)
       }
-      __syncthreads();
-      if (tid < 32) {                              // (a warp: lane c has CTA c's)
-        const int mine = tid < CTAS ? s_count[tid] : 0;
-        int sum = mine;
-        for (int d = 1; d < CTAS; d *= 2) {
-          const int below = __shfl_up_sync(0xffffffffu, sum, d);
-          if (tid >= d) sum += below;
-        }
-        if (tid < CTAS) s_start[tid + 1] = sum;
-        if (tid == 0) s_start[0] = 0;
-      }
-      __syncthreads();
-      auto sort = [&](int e, int token) {
-        if (own[e] != 0xffffffffu)
-          sorted[s_start[static_cast<unsigned>(token) % CTAS] + (own[e] >> 16)] =
-              static_cast<unsigned short>(own[e]);
-      };
-#pragma unroll
-      for (int k = 0; k < TAKES; ++k) {
-        sort(4 * k, next[k].x);
-        sort(4 * k + 1, next[k].y);
-        sort(4 * k + 2, next[k].z);
-        sort(4 * k + 3, next[k].w);
-      }
-      __syncthreads();
-      cluster_sync_all();
-      if (tid < 32) {
-        const int at = tid < CTAS ? cluster_load(&s_start[rank], tid) : 0;
-        int sum = tid < CTAS ? cluster_load(&s_start[rank + 1], tid) - at : 0;
-        for (int d = 1; d < CTAS; d *= 2) {
-          const int below = __shfl_up_sync(0xffffffffu, sum, d);
-          if (tid >= d) sum += below;
-        }
-        if (tid < CTAS) {
-          s_at[tid] = at;
-          s_sum[tid + 1] = sum;
-        }
-        if (tid == 0) s_sum[0] = 0;
-      }
-      __syncthreads();
-      for (int i = tid; i < s_sum[CTAS]; i += THREADS) {
-        int c = 0;
-#pragma unroll
-        for (int k = 1; k < CTAS; ++k) c += i >= s_sum[k];
-        count(cluster_load(&sorted[s_at[c] + i - s_sum[c]], c));
-      }
-      if (done > 0 || from + CTAS * SEG < seen) {  // (else the row's barrier is still to come)
-        __syncthreads();
-        cluster_sync_all();                        // what was sorted has been read
-      }
-    }
     __syncthreads();
   };
-  __syncwarp();
-  cluster_wait();
-  if (special)
-    make_table(0);
-  else if (mask)
+  auto count = [&](unsigned at) {                  // tokens met for the first time are listed
+    if (at >= most || table.count(at) != 0) return;
+    const int to = atomicAdd(&s_listed, 1);
+    if (to < LIST) list[to] = static_cast<unsigned short>(at);
+  };
+  auto look_through = [&](int done) {
+    count(own_at(next[0].x, done));
+    count(own_at(next[0].y, done));
+    count(own_at(next[0].z, done));
+    count(own_at(next[0].w, done));
+  };
+  auto sort = [&](int done) {
+    if (tid < CTAS) s_count[tid] = 0;
     __syncthreads();
+    unsigned own[4 * TAKES];                       // the token's word, and above it its place
+    auto place = [&](int e, int token) {
+      const unsigned id = token, at = id / CTAS - done;
+      own[e] = 0xffffffffu;
+      if (id < static_cast<unsigned>(a.vocab) && at < most)
+        own[e] = at | static_cast<unsigned>(atomicAdd(&s_count[id % CTAS], 1)) << 16;
+    };
+#pragma unroll
+    for (int k = 0; k < TAKES; ++k) {
+      place(4 * k, next[k].x);
+      place(4 * k + 1, next[k].y);
+      place(4 * k + 2, next[k].z);
+      place(4 * k + 3, next[k].w);
+    }
+    __syncthreads();
+    if (tid < 32) {                                // (a warp: lane c has CTA c's)
+      int sum = tid < CTAS ? s_count[tid] : 0;
+      for (int d = 1; d < CTAS; d *= 2) {
+        const int below = __shfl_up_sync(0xffffffffu, sum, d);
+        if (tid >= d) sum += below;
+      }
+      if (tid < CTAS) s_start[tid + 1] = sum;
+      if (tid == 0) s_start[0] = 0;
+    }
+    __syncthreads();
+    auto put = [&](int e, int token) {
+      if (own[e] != 0xffffffffu)
+        sorted[s_start[static_cast<unsigned>(token) % CTAS] + (own[e] >> 16)] =
+            static_cast<unsigned short>(own[e]);
+    };
+#pragma unroll
+    for (int k = 0; k < TAKES; ++k) {
+      put(4 * k, next[k].x);
+      put(4 * k + 1, next[k].y);
+      put(4 * k + 2, next[k].z);
+      put(4 * k + 3, next[k].w);
+    }
+  };
+  auto gather = [&] {                              // counts what the CTAs have sorted for this one
+    if (tid < 32) {
+      const int at = tid < CTAS ? cluster_load(&s_start[rank], tid) : 0;
+      int sum = tid < CTAS ? cluster_load(&s_start[rank + 1], tid) - at : 0;
+      for (int d = 1; d < CTAS; d *= 2) {
+        const int below = __shfl_up_sync(0xffffffffu, sum, d);
+        if (tid >= d) sum += below;
+      }
+      if (tid < CTAS) {
+        s_at[tid] = at;
+        s_sum[tid + 1] = sum;
+      }
+      if (tid == 0) s_sum[0] = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < s_sum[CTAS]; i += THREADS) {
+      int c = 0;
+#pragma unroll
+      for (int k = 1; k < CTAS; ++k) c += i >= s_sum[k];
+      count(cluster_load(&sorted[s_at[c] + i - s_sum[c]], c));
+    }
+  };
+  auto sort_and_gather = [&](int from, int done) { // with all CTAs past the last of them
+    for (; from < seen; from += CTAS * SEG) {
+      __syncthreads();
+      cluster_sync_all();
+      ask(from);
+      sort(done);
+      __syncthreads();
+      cluster_sync_all();
+      gather();
+    }
+  };
+  if (special) {
+    make_table(0);
+    if (sorts)
+      sort(0);
+    else
+      look_through(0);
+  }
+  unsigned any = mask ? 0u : 1u;
+  for (int w = tid, k = 0; w < mask_words; w += THREADS, ++k) {
+    unsigned word = 0;
+#pragma unroll
+    for (int i = 0; i < HOLDS; ++i)
+      if (i == k) word = bits[i];
+    if (held)
+      s_mask[w] = word;
+    else
+      word = mask[lo / 32 + w];
+    any |= n - 32 * w < 32 ? word & ((1u << (n - 32 * w)) - 1u) : word;
+  }
+  __syncthreads();
+  cluster_wait();                                  // 1
+  if (sorts) cluster_arrive();                     // 2: the first tokens have been sorted
 
   // ---- the slice
   float nothing = 0.f;                             // 0, or NaN once a logit was not finite
@@ -346,30 +372,15 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) process_logits_kernel(const
       out4[g] = y;
     }
   }
-  auto permitted = [&](int id) { return !mask || (mask[id >> 5] >> (id & 31) & 1u); };
+  auto mask_at = [&](int id) { return mask ? mask[id >> 5] >> (id & 31) & 1u : 1u; };
   for (int j = tid; j < n - 4 * groups; j += THREADS) {          // ahead of the groups and behind them
     const int id = lo + (j < min(first, n) ? j : j + 4 * groups);
     const float f = x[id];
     nothing = fmaf(f, 0.f, nothing);
-    out[id] = permitted(id) ? f : a.masked;
+    out[id] = mask_at(id) ? f : a.masked;
   }
-
-  // ---- scores of tokens that occur or have a bias, in 64 bits.  What is permitted has been copied, so
-  // that its logit is still there where out is the logits.
-  auto write_score = [&](int id, unsigned word, const double* bias) {
-    if (!permitted(id)) return;
-    const int count = word & (BIASED - 1u);
-    double s = x[id];
-    if (count > 0) {
-      s = s < 0.0 ? s * rep : s / rep;
-      s -= pres;
-    }
-    s -= freq * count;
-    if (bias) s += *bias;
-    const float f = static_cast<float>(s);
-    out[id] = f;
-    if (!isfinite(f)) atomicMax(a.flags + row, 2);
-  };
+  __syncwarp();
+  if (sorts) cluster_wait();                       // 2
   const bool bad = __syncthreads_or(odd || !(nothing == 0.f));
   const bool some = __syncthreads_or(any);
   if (tid == 0) {
@@ -379,32 +390,80 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) process_logits_kernel(const
     if (rank == 0) a.flags[row] = 0;
   }
   __syncthreads();
-  cluster_sync_all();                              // the row has been streamed
+  cluster_arrive();                                // 3: the row has been streamed
+  if (sorts) gather();
+  __syncthreads();
+  cluster_wait();                                  // 3
   if (rank == 0 && tid == 0) {
     int all = 0;
     for (int c = 0; c < CTAS; ++c) all |= *reinterpret_cast<volatile int*>(&s_flags[c]);
     if (all != 1) atomicMax(a.flags + row, all & 2 ? 2 : 1);
   }
-  if (special) {
-    for (int done = 0;; done += words) {
-      auto look_after = [&](unsigned i) {
-        write_score((done + static_cast<int>(i)) * CTAS + rank, table[i], nullptr);
-      };
-      if (s_listed <= LIST) {
-        for (int i = tid; i < s_listed; i += THREADS) look_after(list[i]);
-      } else {                                     // the list has no room: all that occur
-        for (int i = tid; i < words; i += THREADS)
-          if (table[i] != 0 && !(table[i] & BIASED)) look_after(i);
-      }
-      for (int i = tid, k = 0; i < entries && biased; i += THREADS, ++k)
-        if (won(k)) {
-          const int id = a.bias_ids[b_lo + i];
-          write_score(id, table[own_at(id, done)], a.bias_values + b_lo + i);
-        }
-      if ((done + words) * CTAS >= a.vocab) break;
-      __syncthreads();
-      make_table(done + words);
+  if (!special) return;
+
+  // ---- scores of tokens that occur or have a bias, in 64 bits.  What is permitted has been copied, so
+  // that its logit is still there where out is the logits.
+  auto write_score = [&](int id, unsigned word, unsigned permitted, float logit, double bias) {
+    if (!permitted) return;
+    const int times = word & (BIASED - 1u);
+    double s = logit;
+    if (times > 0) {
+      s = s < 0.0 ? s * rep : s / rep;
+      s -= pres;
     }
+    s -= freq * times;
+    if (word & BIASED) s += bias;
+    const float f = static_cast<float>(s);
+    out[id] = f;
+    if (!isfinite(f)) atomicMax(a.flags + row, 2);
+  };
+  if (sorts) {
+    sort_and_gather(CTAS * SEG, 0);
+    __syncthreads();
+    cluster_arrive();                              // 4: what was sorted has been read
+  }
+  for (int done = 0;; done += words) {
+    // the first bias is on its way beside the first of the list
+    const bool leads = biased && won(0);
+    const unsigned lead_may = leads ? mask_at(bias_id) : 0u;
+    const float lead_logit = leads ? x[bias_id] : 0.f;
+    const double lead_bias = leads ? a.bias_values[b_lo + tid] : 0.0;
+    auto look_after = [&](unsigned i) {
+      const int id = (done + static_cast<int>(i)) * CTAS + rank;
+      const unsigned may = mask_at(id);
+      write_score(id, table[i], may, x[id], 0.0);
+    };
+    if (s_listed <= LIST) {
+      for (int i = tid; i < s_listed; i += THREADS) look_after(list[i]);
+    } else {                                       // the list has no room: all that occur
+      for (int i = tid; i < words; i += THREADS)
+        if (table[i] != 0 && !(table[i] & BIASED)) look_after(i);
+    }
+    if (leads)
+      write_score(bias_id, table[own_at(bias_id, done)], lead_may, lead_logit, lead_bias);
+    for (int i = tid + THREADS, k = 1; i < entries && biased; i += THREADS, ++k)
+      if (won(k)) {
+        const int id = a.bias_ids[b_lo + i];
+        const unsigned may = mask_at(id);
+        const float logit = x[id];
+        write_score(id, table[own_at(id, done)], may, logit, a.bias_values[b_lo + i]);
+      }
+    __syncwarp();
+    if (sorts && done == 0) cluster_wait();        // 4
+    if ((done + words) * CTAS >= a.vocab) {
+      if (sorts && done > 0) {
+        __syncthreads();
+        cluster_sync_all();
+      }
+      return;
+    }
+    __syncthreads();
+    make_table(done + words);
+    if (sorts)
+      sort_and_gather(0, done + words);
+    else
+      look_through(done + words);
+    __syncthreads();
   }
 }
 
@@ -437,6 +496,8 @@ extern "C" int orinfer_process_logits(
                       reinterpret_cast<const unsigned int*>(mask), mask_stride, mask_rows,
                       mask_count, masked, out, out_stride, flags, rows, vocab, bias_total};
   const bool narrow = !history || history_cap <= lp::SHORT;
+  // Threads of a CTA, and with them CTAs of an SM: 512 and two where one such wave takes all rows (32
+  // rows 17 us, with 320 threads 20), else 320 and three (256 rows 88 us, with 512 threads 98).
   const bool few = rows * static_cast<long long>(lp::CTAS) <= 2 * 148;
   auto kernel = few ? (narrow ? lp::process_logits_kernel<uint16_t, 512, 2>
                               : lp::process_logits_kernel<uint32_t, 512, 2>)
