@@ -269,12 +269,16 @@ class SharedPrefix:
         f32 = lambda n: torch.empty(n, dtype=torch.float32, device=self.device) if n else None
         self.part_buffer = f32(self.parts * qh * (head_dim + 2))
         # The own keys, by the row kernels: as many as the middle row may have.  Beside a prefix they
-        # are split only where they are long: a merge is a launch of its own.
+        # are split only where they are long, else where they are not short: a merge is a launch of
+        # its own (32 / 8 heads of 128, 384 keys: two rows 6.0 us in one part and 5.5 in six, eight
+        # rows 6.1 and 7.4, and the launch takes the host 2.3).
         shared = sorted(i[0] for i in info)
         self.own_keys = max(1, max_kv_len - (shared[len(shared) // 2] if items else 0))
         self.splits = attention_splits(self.own_keys, max(1, rows), kvh)
         if items:
             self.splits = max(1, min(self.splits, self.own_keys // 512))
+        elif self.own_keys <= 384 and head_dim <= 128:
+            self.splits = 1
         self.scratch = f32(rows * qh * self.splits * (head_dim + 2)) if self.splits > 1 else None
         self._args = (ptr(self.items), len(items), ptr(self.info), ptr(self.part_buffer),
                       self.parts, self.splits, ptr(self.scratch), self.own_keys)
