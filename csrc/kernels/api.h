@@ -281,7 +281,7 @@ int orinfer_process_logits(const float* logits, long long row_stride, const int*
 
 // ---- pages of the cache (pages.cu).  The cache is n tensors [pages, 128, ...]: their addresses,
 // bytes per token, and the units (tensor, first token, tokens) that a page is copied in.  work: int32
-// [4 + 4 n + slots] for n forks, [4 + 3 (pages / 2 + 1)] for a compaction.
+// [4 + 6 n + 2 slots] for n forks, [4 + 3 (pages / 2 + 1)] for a compaction.
 int orinfer_copy_pages(const long long* bases, const int* token_bytes, const int* units,
                        int n_units, int pages, const int* copies, const int* count, int most,
                        cudaStream_t stream);

@@ -8,6 +8,11 @@
 // The bookkeeping is one CTA's work (a few scans over the pages).  It leaves a list of (source
 // page, target page, tokens), and a second kernel moves those bytes of all tensors and writes the
 // table.  Outputs may be the inputs themselves.
+//
+// A copy is bound by memory: 8 requests of up to 1500 tokens, eight branches each, in 36 layers of 8 KV
+// heads of 128 take 73 us (340 MB written, an eighth of it read, at 5.9 TB/s behind 8 us of
+// bookkeeping), 64 of 256 pages moved within the cache 206 (1.24 GB at 6.1).  Small calls are launches:
+// a fork of one request into four 6.4, a compaction of a few pages 4.2, a freed slot 2.4.
 #include "api.h"
 #include "common.cuh"
 
@@ -43,31 +48,36 @@ __device__ __forceinline__ int block_rank(bool flag, int* warp_sums, int& total)
 }
 
 // ---------------------------------------------------------------- fork
-// work: head; copies [n][3]; pairs in the order of their new pages [n]; pair of a child slot [slots]
+// work: head; copies [n][3]; pairs in the order of their new pages [n]; pair of a child slot [slots];
+// a pair of a parent slot [slots]; from there the next one of the same parent [n]; these first pairs [n]
 __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(
     const int* table, const int* lens, const int* refs, int* refs_out, const int* parents,
-    const int* children, int n, int slots, int max_pages, int pages, int* work, int* status_out) {
+    const int* children, int n, int slots, int max_pages, int pages, int apart, int* work,
+    int* status_out) {
   __shared__ int sums[PLAN_THREADS / 32];
-  __shared__ int s_wrong;
+  __shared__ int s_wrong, s_firsts;
   int* copies = work + WORK_HEAD;
   int* owner = copies + 3 * n;
   int* child_of = owner + n;
+  int* pair_of = child_of + slots;
+  int* chain = pair_of + slots;
+  int* firsts = chain + n;
   const int tid = threadIdx.x;
   grid_wait();
   grid_release();
-  if (tid == 0) s_wrong = 0;
-  for (int s = tid; s < slots; s += PLAN_THREADS) child_of[s] = -1;
+  if (tid == 0) s_wrong = s_firsts = 0;
+  for (int s = tid; s < slots; s += PLAN_THREADS) child_of[s] = pair_of[s] = -1;
   __syncthreads();
   // ---- the pairs: slots that exist, a child that is empty and named once, pages that are held
-  for (int i = tid / 32; i < n; i += PLAN_THREADS / 32) {        // a warp per pair
-    const int p = parents[i], c = children[i], lane = tid & 31;
+  for (int i = tid / 16; i < n; i += PLAN_THREADS / 16) {        // sixteen lanes per pair
+    const int p = parents[i], c = children[i], lane = tid & 15;
     bool wrong = p < 0 || p >= slots || c < 0 || c >= slots || p == c;
     if (!wrong) {
       const int len = lens[p];
       wrong = lens[c] != 0 || len < 0 || len > max_pages * PAGE;
       if (!wrong && lane == 0) wrong = atomicCAS(&child_of[c], -1, i) != -1;
       const int* row = table + static_cast<size_t>(p) * max_pages;
-      for (int j = lane; !wrong && j < (len + PAGE - 1) / PAGE; j += 32) {
+      for (int j = lane; !wrong && j < (len + PAGE - 1) / PAGE; j += 16) {
         const int page = row[j];
         wrong = page <= 0 || page >= pages || refs[page] <= 0;
       }
@@ -93,7 +103,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(
       copies[3 * i] = tail ? table[static_cast<size_t>(p) * max_pages + lens[p] / PAGE] : 0;
       copies[3 * i + 1] = 0;
       copies[3 * i + 2] = tail;
-      if (tail) owner[rank] = i;
+      if (tail) {
+        owner[rank] = i;
+        if (!apart) chain[i] = atomicExch(&pair_of[p], i);
+      }
     }
     need += total;
   }
@@ -109,63 +122,84 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(
     if (p > 0 && held <= 0 && rank < need) copies[3 * owner[rank] + 1] = p;
     found += total;
   }
-  __syncthreads();
   if (status == 0 && found < need) status = 1;
+  if (status == 0 && !apart)
+    for (int i = tid; i < n; i += PLAN_THREADS)
+      if (copies[3 * i + 2] > 0 && pair_of[parents[i]] == i)
+        firsts[atomicAdd(&s_firsts, 1)] = i;
+  __syncthreads();
   if (status == 0)
     for (int r = tid; r < need; r += PLAN_THREADS) refs_out[copies[3 * owner[r] + 1]] = 1;
   if (tid == 0) {
     work[0] = status;
-    work[1] = status == 0 ? n : 0;
+    work[1] = status != 0 ? 0 : apart ? n : s_firsts;
     *status_out = status;
   }
 }
 
 // ---------------------------------------------------------------- copies
 // Four loads of a thread ahead of their stores (one at a time, 128 pages of 9.7 MB moved at 5.7 TB/s).
-template <class T>
-__device__ __forceinline__ void copy_as(const unsigned char* from, unsigned char* to, int bytes) {
+// `next` names the targets in turn: what several children get is read once.
+template <class T, class Next>
+__device__ __forceinline__ void copy_as(const unsigned char* from, int bytes, Next next) {
   constexpr int BATCH = 4;
   const int n = bytes / static_cast<int>(sizeof(T));
   const T* src = reinterpret_cast<const T*>(from);
-  T* dst = reinterpret_cast<T*>(to);
   for (int i0 = threadIdx.x; i0 < n; i0 += BATCH * COPY_THREADS) {
     T v[BATCH];
 #pragma unroll
     for (int k = 0; k < BATCH; ++k)
       if (i0 + k * COPY_THREADS < n) v[k] = __ldcs(src + i0 + k * COPY_THREADS);
+    int at = -1;
+    while (unsigned char* to = next(at)) {
+      T* dst = reinterpret_cast<T*>(to);
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k)
-      if (i0 + k * COPY_THREADS < n) __stcs(dst + i0 + k * COPY_THREADS, v[k]);
+      for (int k = 0; k < BATCH; ++k)
+        if (i0 + k * COPY_THREADS < n) __stcs(dst + i0 + k * COPY_THREADS, v[k]);
+    }
   }
-  for (int i = n * static_cast<int>(sizeof(T)) + threadIdx.x; i < bytes; i += COPY_THREADS)
-    to[i] = from[i];
+  const int rest = n * static_cast<int>(sizeof(T));
+  if (rest + static_cast<int>(threadIdx.x) < bytes) {
+    int at = -1;
+    while (unsigned char* to = next(at)) to[rest + threadIdx.x] = from[rest + threadIdx.x];
+  }
 }
 
-// copies [*count][3]: source page, target page, tokens from the page's first on; by CTA `cta` of `ctas`
+// copies [][3]: source page, target page, tokens from the page's first on; *count of them, or where
+// there are `firsts` as many of those, each with the copies of the same source that `chain` leads to.
+// By CTA `cta` of `ctas`.
 __device__ __forceinline__ void copy_units(const Cache& cache, const int* copies, const int* count,
-                                           int cta, int ctas, int* status) {
+                                           int cta, int ctas, int* status,
+                                           const int* firsts = nullptr, const int* chain = nullptr) {
   const long long total = static_cast<long long>(*count) * cache.n_units;
   for (long long w = cta; w < total; w += ctas) {
-    const int* c = copies + w / cache.n_units * 3;
+    const long long item = w / cache.n_units;
+    const long long first = firsts ? firsts[item] : item;
+    const int* c = copies + 3 * first;
     const int* u = cache.units + w % cache.n_units * 3;
-    const int from = c[0], to = c[1], tokens = min(c[2] - u[1], u[2]);
+    const int from = c[0], tokens = min(c[2] - u[1], u[2]);
     if (tokens <= 0) continue;
-    if (from < 0 || from >= cache.pages || to < 0 || to >= cache.pages || c[2] > PAGE) {
+    if (from < 0 || from >= cache.pages || c[1] < 0 || c[1] >= cache.pages || c[2] > PAGE) {
       if (threadIdx.x == 0) report_status(status, STATUS_BAD_INDEX, 0x40);
       continue;
     }
     const long long per = cache.token_bytes[u[0]];
     unsigned char* base = reinterpret_cast<unsigned char*>(cache.bases[u[0]]) + u[1] * per;
     const unsigned char* src = base + from * PAGE * per;
-    unsigned char* dst = base + to * PAGE * per;
     const int bytes = tokens * static_cast<int>(per);
-    const uintptr_t off = reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst);
+    // (pages are multiples of 128 bytes: all targets are aligned as the source is)
+    auto next = [&](int& at) -> unsigned char* {
+      at = at < 0 ? static_cast<int>(first) : chain ? chain[at] : -1;
+      if (at < 0) return nullptr;
+      return base + static_cast<long long>(copies[3 * static_cast<long long>(at) + 1]) * PAGE * per;
+    };
+    const uintptr_t off = reinterpret_cast<uintptr_t>(src);
     if ((off & 15) == 0)
-      copy_as<uint4>(src, dst, bytes);
+      copy_as<uint4>(src, bytes, next);
     else if ((off & 3) == 0)
-      copy_as<uint32_t>(src, dst, bytes);
+      copy_as<uint32_t>(src, bytes, next);
     else
-      copy_as<unsigned char>(src, dst, bytes);
+      copy_as<unsigned char>(src, bytes, next);
   }
 }
 
@@ -180,13 +214,15 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const Cache ca
 // The table's rows, lens and the references of shared pages, a CTA per slot; the CTAs behind them copy.
 __global__ void __launch_bounds__(COPY_THREADS) fork_apply_kernel(
     const int* table, int* table_out, const int* lens, int* lens_out, int* refs_out,
-    const int* parents, int n, int slots, int max_pages, const int* work, const Cache cache,
-    int* status) {
+    const int* parents, int n, int slots, int max_pages, int apart, const int* work,
+    const Cache cache, int* status) {
   grid_wait();
   grid_release();
   const int* copies = work + WORK_HEAD;
   if (static_cast<int>(blockIdx.x) >= slots) {
-    copy_units(cache, copies, work + 1, blockIdx.x - slots, gridDim.x - slots, status);
+    const int* chain = copies + 4 * n + 2 * slots;
+    copy_units(cache, copies, work + 1, blockIdx.x - slots, gridDim.x - slots, status,
+               apart ? nullptr : chain + n, apart ? nullptr : chain);
     return;
   }
   const int s = blockIdx.x, pair = work[0] == 0 ? (copies + 4 * n)[s] : -1;
@@ -359,10 +395,12 @@ __global__ void __launch_bounds__(COPY_THREADS) compact_apply_kernel(
   }
 }
 
-// CTAs that copy at most `most` pages
+// CTAs that copy at most `most` pages: four times as many as there is room for, so that one that ends
+// early makes room for the next (8 per SM: 8 parents with eight children each 80 us, 64 pages moved 228;
+// 32: 73 and 206; 64: 73 and 204, and a CTA without work costs its start).
 static int copy_ctas(const Cache& cache, int most) {
   const long long units = static_cast<long long>(most) * cache.n_units;
-  return static_cast<int>(units < 8 * 148 ? units : 8 * 148);
+  return static_cast<int>(units < 32 * 148 ? units : 32 * 148);
 }
 
 static int grid_of(long long n) {
@@ -389,7 +427,7 @@ extern "C" int orinfer_copy_pages(const long long* bases, const int* token_bytes
 }
 
 // status: 0, 1 (not enough free pages) or 2 (a pair that cannot be); then nothing is changed.
-// work: int32 [4 + 4 n + slots].
+// work: int32 [4 + 6 n + 2 slots].
 extern "C" int orinfer_fork_pages(const long long* bases, const int* token_bytes, const int* units,
                                   int n_units, int pages, const int* table, int* table_out,
                                   const int* lens, int* lens_out, const int* refs, int* refs_out,
@@ -398,12 +436,15 @@ extern "C" int orinfer_fork_pages(const long long* bases, const int* token_bytes
   if (n < 0 || slots <= 0 || max_pages <= 0 || pages <= 0 || n_units < 0) return -1;
   if (max_pages > (1 << 24) || !work || !status) return -1;
   if (runtime_ensure_init() != cudaSuccess) return -2;
-  launch_early(pg::fork_plan_kernel, dim3(1), pg::PLAN_THREADS, 0, stream, table, lens, refs,
-               refs_out, parents, children, n, slots, max_pages, pages, work, status);
+  // Children of one parent get its page from one read (8 parents with eight each 110 -> 79 us), but by
+  // CTAs of their own where all fit at once (a fork into four 7.3 -> 6.4).
   const pg::Cache cache = {bases, token_bytes, units, n_units, pages};
+  const int apart = static_cast<long long>(n) * n_units <= 8 * 148;
+  launch_early(pg::fork_plan_kernel, dim3(1), pg::PLAN_THREADS, 0, stream, table, lens, refs,
+               refs_out, parents, children, n, slots, max_pages, pages, apart, work, status);
   launch_early(pg::fork_apply_kernel, dim3(slots + pg::copy_ctas(cache, n)), pg::COPY_THREADS, 0,
-               stream, table, table_out, lens, lens_out, refs_out, parents, n, slots, max_pages, work,
-               cache, runtime_status_ptr());
+               stream, table, table_out, lens, lens_out, refs_out, parents, n, slots, max_pages, apart,
+               work, cache, runtime_status_ptr());
   return static_cast<int>(cudaGetLastError());
 }
 

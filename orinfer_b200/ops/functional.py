@@ -478,7 +478,7 @@ def fork_pages(cache: CachePages, table: torch.Tensor, lens: torch.Tensor, refs:
     check(native.lib().orinfer_fork_pages(
         *cache._args, table.data_ptr(), t.data_ptr(), lens.data_ptr(), l.data_ptr(),
         refs.data_ptr(), r.data_ptr(), parents.data_ptr(), children.data_ptr(), n, slots, width,
-        cache._work(4 + 4 * n + slots), status.data_ptr(), stream()), "fork_pages")
+        cache._work(4 + 6 * n + 2 * slots), status.data_ptr(), stream()), "fork_pages")
     count_launches(2)
     return t, l, r, status
 

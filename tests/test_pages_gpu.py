@@ -111,6 +111,27 @@ def test_fork_of_many_slots_and_pages(dev):
         assert torch.equal(a.cpu(), b)
 
 
+@pytest.mark.parametrize("by", [0, 4, 1])
+@pytest.mark.parametrize("lens", [[333, 70], [128, 1, 511], [257]])
+def test_children_that_get_their_parents_page_from_one_read(dev, by, lens):
+    """More pairs and tensors than have CTAs of their own: a parent's page is read for all of its
+    children, whose pages are each of their own."""
+    from orinfer_b200.ops import functional as F
+    table, length, refs, cache, used, free = state(len(lens), slots=50, pages=60, width=5, lens=lens,
+                                                   kvh=8, d=128)
+    n = 40
+    gpu = [_unaligned(t.to(dev), by) for t in cache]
+    handle = F.CachePages(gpu)
+    assert n * len(handle.units) > 8 * 148
+    args = (i32([used[i * i % len(lens)] for i in range(n)]), i32(free[:n]))
+    tables = _to(dev, table, length, refs)
+    got = F.fork_pages(handle, *tables, *_to(dev, *args), out=tables)
+    want = R.fork_pages(cache, table, length, refs, *args)
+    assert int(got[3]) == want[3] == 0
+    for a, b in zip([*got[:3], *gpu], [*want[:3], *cache]):
+        assert torch.equal(a.cpu(), b)
+
+
 def test_forks_that_cannot_be_change_nothing(dev):
     from orinfer_b200.ops import functional as F
     table, length, refs, cache, used, free = state(3, slots=12, pages=12, width=4,
