@@ -17,16 +17,18 @@
 //
 // Scores of three steps have a place in TMEM, so that the products run ahead of the eight softmax warps
 // (sixteen rows each), which go from step to step without a wait.  The weights replace the scores that
-// they are made of.
+// they are made of.  Two teams of dequantising warps take a step each in turn.
 //
-// 64 rows of 32 query heads behind 16384 keys of 4 KV heads of 128: 40 us, 430 TFLOP/s, with the rows'
-// own keys and the join 47 (each row reading all keys 237).  What bounds it is a step of 64 keys, 1750
-// cycles: 1460 of a softmax warp's (two and as many dequantising warps share a scheduler, which issues
-// in 52 % of its cycles) and 290 of its waits; the tensor pipe is at work for 23 %, DRAM for 5 %.
+// 64 rows of 32 query heads behind 16384 keys of 4 KV heads of 128: 34 us, 510 TFLOP/s, with the rows'
+// own keys and the join 46 (each row reading all keys 237); 5 us of the 34 are the start and the end.
+// What bounds it is a step of 64 keys, 1800 cycles, in which nothing is at work for long: a scheduler
+// issues in half of its cycles, the tensor pipe works for a quarter, exponentials for a quarter, DRAM
+// for 5 %.  Without the softmax's arithmetic a step takes 1650 cycles, without the dequantisation 1450,
+// with neither 1000: each is a chain in few warps, and they wait for one another.
 // Tried: two tiles to a CTA, sixteen softmax warps that exchange maxima and sums, raw tiles by bulk
 // copies ahead of the dequantisation (each slower by 5 to 20 %); scores read from TMEM ahead of the
-// exponentials of the step before (50 to 53 us); no maxima, the weights' sum saying when the
-// reference has to move (48: fewer instructions in the same time).
+// exponentials of the step before (50 to 53 us); all dequantising warps on each step (47), four teams
+// (47); a second warp for the scales (46).
 #include "api.h"
 #include "attention_shared.h"
 #include "common.cuh"
@@ -35,10 +37,10 @@ namespace orinfer {
 namespace sp {
 
 constexpr int TILE = 128;                        // rows of a tile: positions x query heads
-constexpr int SOFTMAX_WARPS = 8, DQ_WARPS = 8;
+constexpr int SOFTMAX_WARPS = 8, DQ_WARPS = 8, DQ_TEAMS = 2;
 constexpr int MMA_WARP = SOFTMAX_WARPS + DQ_WARPS, SCALE_WARP = MMA_WARP + 1;
 constexpr int THREADS = (SCALE_WARP + 1) * 32;
-constexpr float LAG = 8.f;                       // of the weights' reference, binades
+constexpr float CAP = 256.f;                     // of a thread's weights of a step, in all
 
 template <int D>
 struct Shape {
@@ -46,7 +48,7 @@ struct Shape {
   static constexpr int DV = D > 128 ? 128 : D;   // value channels of a CTA
   static constexpr int GV = DV / 64, PARTS = D / DV;
   static constexpr int KT = D > 128 ? 32 : 64;   // keys of a step: at most 128 score columns
-  static constexpr int NB = 5, PF = 2;           // buffers of keys and values; steps in registers
+  static constexpr int NB = 5;                   // buffers of keys and values
   static constexpr int QSUB = TILE * 128, KSUB = KT * 128;     // bytes of 64 channels of a tile
   static constexpr int K_BYTES = G * KSUB, V_BYTES = GV * KSUB;
   static constexpr int Q_OFF = 0;
@@ -55,7 +57,8 @@ struct Shape {
   static constexpr int SCALES = KT * (G + GV) * 4 + 16;        // key and value scales, units
   static constexpr int STAT_OFF = SCALE_OFF + NB * SCALES;     // [sum, reference][128]
   static constexpr int BAR_OFF = STAT_OFF + 2 * TILE * 4;
-  static constexpr int CC = D > 128 ? 16 : 32;   // score columns of a group that are read at a time
+  static constexpr int CC = KT;                  // score columns of a group that are read at a time
+  static constexpr int CS = D > 128 ? 16 : 32;   // and that are replaced by weights at a time
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;
   static constexpr int SUB = DV / 2;             // channels that a warp writes, of 32 rows: in the ring
   static_assert(SOFTMAX_WARPS * 32 * SUB * 4 <= NB * (K_BYTES + V_BYTES), "results fit the ring");
@@ -111,6 +114,19 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) 
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[32]) {       // 64 columns
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
 }
@@ -171,7 +187,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     const Item* items, const int4* info, float* __restrict__ part_o, float2* __restrict__ part_ml,
     int qh, int kvh, int rep, int num_pages, int* status) {
   using L = Shape<D>;
-  constexpr int G = L::G, GV = L::GV, KT = L::KT, NB = L::NB, CC = L::CC;
+  constexpr int G = L::G, GV = L::GV, KT = L::KT, NB = L::NB, CC = L::CC, CS = L::CS;
   constexpr int NS = 3;                  // steps whose scores have a place
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -192,10 +208,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
   const int req = row_req[it.row];
   const bool known = req >= 0 && req < slots;
   const int* pages = page_table + static_cast<size_t>(known ? req : 0) * max_pages;
+  // A warp's page ids, a lane each, 32 at a time: one that is fetched when it is needed holds up what
+  // is asked for by it.
+  const int page_lo = it.step_lo * KT >> 7, page_hi = it.step_hi * KT - 1 >> 7;
+  auto pages_from = [&](int i) { return page_lo + i + lane <= page_hi ? pages[page_lo + i + lane] : 0; };
 
   if (tid == 0) {
     for (int b = 0; b < NB; ++b) {
-      mbar_init(&kv_full[b], DQ_WARPS + 1);
+      mbar_init(&kv_full[b], DQ_WARPS / DQ_TEAMS + 1);
       mbar_init(&kv_free[b], 1);
     }
     for (int i = 0; i < NS; ++i) {
@@ -278,9 +298,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     for (int g = 0; g < GV; ++g) unit[g] = __uint_as_float((127 + 29) << 23);
     bool ok = true;
     __half kraw[KS], vraw[VS];
+    int ids = pages_from(0), ids_at = 0;
     auto load = [&](int s) {
-      const int key0 = (it.step_lo + s) * KT;
-      int page = pages[key0 >> 7];
+      const int key0 = (it.step_lo + s) * KT, at = (key0 >> 7) - page_lo;
+      if (at >= ids_at + 32) ids = pages_from(ids_at += 32);
+      int page = __shfl_sync(0xffffffffu, ids, at - ids_at);
       if (!known || page < 0 || page >= num_pages) {
         if (lane == 0) report_status(status, STATUS_BAD_INDEX, 0x50);
         page = 0;
@@ -340,15 +362,17 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       if (s + 1 < steps) load(s + 1);
     }
   } else if (warp >= SOFTMAX_WARPS) {
-    // ---------------- keys and values: INT8 from global memory (PF steps ahead, in registers) to
-    // FP16 integers in swizzled tiles
-    constexpr int DQ = DQ_WARPS * 32;
+    // ---------------- keys and values: INT8 from global memory (a step of the team's ahead, in
+    // registers) to FP16 integers in swizzled tiles
+    constexpr int DQ = DQ_WARPS / DQ_TEAMS * 32;
     constexpr int KI = KT * D / 16 / DQ, VI = KT * L::DV / 16 / DQ;
-    const int u = tid - SOFTMAX_WARPS * 32;
-    uint4 kraw[L::PF][KI], vraw[L::PF][VI];
+    const int u = (tid - SOFTMAX_WARPS * 32) % DQ, team = warp_same((tid - SOFTMAX_WARPS * 32) / DQ);
+    uint4 kraw[KI], vraw[VI];
+    int ids = pages_from(0), ids_at = 0;
     auto load = [&](int s, uint4(&kr)[KI], uint4(&vr)[VI]) {
-      const int key0 = (it.step_lo + s) * KT;
-      int page = pages[key0 >> 7];
+      const int key0 = (it.step_lo + s) * KT, at = (key0 >> 7) - page_lo;
+      if (at >= ids_at + 32) ids = pages_from(ids_at += 32);
+      int page = __shfl_sync(0xffffffffu, ids, at - ids_at);
       if (!known || page < 0 || page >= num_pages) page = 0;           // (the scale warp reports it)
       const size_t slot = static_cast<size_t>(page) * 128 + (key0 & 127);
 #pragma unroll
@@ -374,34 +398,28 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + !swap)) = hi;
     };
     bool ok = true;
+    if (team < steps) load(team, kraw, vraw);
+    for (int s = team; s < steps; s += DQ_TEAMS) {
+      const int b = s % NB;
+      if (s >= NB)
+        ok = ok && mbar_wait(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, s & 0xff);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      unsigned char* buf = smem + L::KV_OFF + b * (L::K_BYTES + L::V_BYTES);
 #pragma unroll
-    for (int f = 0; f < L::PF; ++f)
-      if (f < steps) load(f, kraw[f], vraw[f]);
-    for (int s0 = 0; s0 < steps && ok; s0 += L::PF) {
-#pragma unroll
-      for (int f = 0; f < L::PF; ++f) {
-        const int s = s0 + f, b = s % NB;
-        if (s >= steps) break;
-        if (s >= NB)
-          ok = ok && mbar_wait(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, s & 0xff);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        unsigned char* buf = smem + L::KV_OFF + b * (L::K_BYTES + L::V_BYTES);
-#pragma unroll
-        for (int i = 0; i < KI; ++i) {
-          const int x = u + i * DQ;
-          place(buf, kraw[f][i], x / (D / 16), x % (D / 16));
-        }
-#pragma unroll
-        for (int i = 0; i < VI; ++i) {
-          const int x = u + i * DQ;
-          place(buf + L::K_BYTES, vraw[f][i], x / (L::DV / 16), x % (L::DV / 16));
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[b]);
-        if (s + L::PF < steps) load(s + L::PF, kraw[f], vraw[f]);
+      for (int i = 0; i < KI; ++i) {
+        const int x = u + i * DQ;
+        place(buf, kraw[i], x / (D / 16), x % (D / 16));
       }
+#pragma unroll
+      for (int i = 0; i < VI; ++i) {
+        const int x = u + i * DQ;
+        place(buf + L::K_BYTES, vraw[i], x / (L::DV / 16), x % (L::DV / 16));
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kv_full[b]);
+      if (s + DQ_TEAMS < steps) load(s + DQ_TEAMS, kraw, vraw);
     }
   } else {
     // ---------------- softmax: sixteen rows per warp
@@ -455,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     }
     const int all_see = __reduce_min_sync(0xffffffffu, min(sees[0], sees[1]));
     const uint32_t lane_addr = static_cast<uint32_t>(row0) << 16;
-    constexpr int PAIRS = KT / 8, CP = CC / 8;   // pairs of keys of a thread, of a step and at a time
+    constexpr int CP = CC / 8;                   // pairs of keys of a thread, at a time
     float m_ref[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, unit[GV];
 #pragma unroll
     for (int g = 0; g < GV; ++g) unit[g] = 1.f;
@@ -474,78 +492,56 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       const float* sv = sk + KT * G;
       const float* su = sv + KT * GV;
       const int key0 = (it.step_lo + s) * KT;
-      // ---- scores
-      float2 x[2][PAIRS];
+      // `f(k0, x)`: scores less `less`, of CC keys from k0 on, pair by pair of this thread's two rows
+      auto scores = [&](const float2(&less)[2], auto f) {
 #pragma unroll
-      for (int k0 = 0; k0 < KT; k0 += CC) {
-        uint32_t raw[G][CC / 2];
+        for (int k0 = 0; k0 < KT; k0 += CC) {
+          uint32_t raw[G][CC / 2];
 #pragma unroll
-        for (int g = 0; g < G; ++g) tmem_ld_frag(tmem_s + g * KT + k0, raw[g]);
-        tc_wait_ld();
+          for (int g = 0; g < G; ++g) tmem_ld_frag(tmem_s + g * KT + k0, raw[g]);
+          tc_wait_ld();
+          float2 x[2][CP];
 #pragma unroll
-        for (int j = 0; j < CP; ++j) {
-          const float2* w = reinterpret_cast<const float2*>(sk) + (k0 / 2 + 4 * j + qt) * G;
-          float2 wg[G];
-          if (G == 1) {
-            wg[0] = w[0];
-          } else {
+          for (int j = 0; j < CP; ++j) {
+            const float2* w = reinterpret_cast<const float2*>(sk) + (k0 / 2 + 4 * j + qt) * G;
+            float2 wg[G];
+            if (G == 1) {
+              wg[0] = w[0];
+            } else {
 #pragma unroll
-            for (int g = 0; g < G; g += 2) {
-              const float4 v = *reinterpret_cast<const float4*>(w + g);
-              wg[g] = make_float2(v.x, v.y);
-              wg[(g + 1) % G] = make_float2(v.z, v.w);
+              for (int g = 0; g < G; g += 2) {
+                const float4 v = *reinterpret_cast<const float4*>(w + g);
+                wg[g] = make_float2(v.x, v.y);
+                wg[(g + 1) % G] = make_float2(v.z, v.w);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              x[i][j] = less[i];
+#pragma unroll
+              for (int g = 0; g < G; ++g)
+                x[i][j] = fma2(pair_at(raw[g][4 * j + 2 * i], raw[g][4 * j + 2 * i + 1]), wg[g],
+                               x[i][j]);
             }
           }
+          if (all_see < key0 + KT) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float2 v;
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              const float2 a = pair_at(raw[g][4 * j + 2 * i], raw[g][4 * j + 2 * i + 1]);
-              v = g == 0 ? mul2(a, wg[0]) : fma2(a, wg[g], v);
-            }
-            x[i][k0 / 8 + j] = v;
+              for (int j = 0; j < CP; ++j) {
+                const int key = key0 + k0 + 8 * j + 2 * qt;
+                if (key >= sees[i]) x[i][j].x = -INFINITY;
+                if (key + 1 >= sees[i]) x[i][j].y = -INFINITY;
+              }
           }
+          f(k0, x);
         }
-      }
-      if (all_see < key0 + KT) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < PAIRS; ++j) {
-            const int key = key0 + 8 * j + 2 * qt;
-            if (key >= sees[i]) x[i][j].x = -INFINITY;
-            if (key + 1 >= sees[i]) x[i][j].y = -INFINITY;
-          }
-      }
-      // ---- the reference follows the maximum when that is more than LAG above it
-      float top[2][2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[i][0] = fmaxf(x[i][0].x, x[i][0].y);
-        top[i][1] = fmaxf(x[i][1].x, x[i][1].y);
-#pragma unroll
-        for (int j = 2; j < PAIRS; ++j)
-          top[i][j & 1] = fmaxf(top[i][j & 1], fmaxf(x[i][j].x, x[i][j].y));
-        top[i][0] = fmaxf(top[i][0], top[i][1]);
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          top[i][0] = fmaxf(top[i][0], __shfl_xor_sync(0xffffffffu, top[i][0], o));
-      bool moves = false;
-      float corr[2], same[GV];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        corr[i] = 1.f;
-        if (top[i][0] > m_ref[i] + LAG) {        // (from -inf: any score)
-          corr[i] = ex2(m_ref[i] - top[i][0]);
-          l_run[i] *= corr[i];
-          m_ref[i] = top[i][0];
-          moves = true;
-        }
-      }
+      };
+      // ---- weights, under a reference that is the maximum of some step: their sum, which is wanted
+      // anyway, says whether they stay small (CAP times a value scale's 128 is within FP16).  Only
+      // steps where it does not take maxima, move the reference and make their weights once more.
+      bool moves = s == 0;
+      float same[GV];
 #pragma unroll
       for (int g = 0; g < GV; ++g) {             // units are powers of two
         const float now = su[g];
@@ -553,65 +549,101 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
         moves = moves || now != unit[g];
         unit[g] = now;
       }
-      if (__any_sync(0xffffffffu, moves) && s > 0) {
-        // O has to stand still: the product before this one is through (the one before on its barrier
-        // is, since scores that came behind that have been read)
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(s - 1) % NS], ((s - 1) / NS) & 1, status,
-                                               STATUS_EPILOGUE_WAIT, 0x180));
-        tc_fence_after();
-        const uint32_t tmem_oc = tmem_o + lane_addr;
+      float2 sum[2];
+      uint32_t packed[GV][KT / 4];
+      for (;;) {
+        if (moves) {
+          float top[2] = {-INFINITY, -INFINITY}, corr[2];
+          const float2 none[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          scores(none, [&](int, const float2(&x)[2][CP]) {
 #pragma unroll
-        for (int g = 0; g < GV; ++g)
-#pragma unroll 1
-          for (int d0 = 0; d0 < 64; d0 += 16) {
-            uint32_t o[8];
-            tmem_ld_frag(tmem_oc + g * 64 + d0, o);
-            tc_wait_ld();
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              o[i] = __float_as_uint(__uint_as_float(o[i]) * (corr[i >> 1 & 1] * same[g]));
-            tmem_st_frag(tmem_oc + g * 64 + d0, o);
-          }
-      }
-      // ---- weights
-      float2 neg[2], sum[2];
+              for (int j = 0; j < CP; ++j) top[i] = fmaxf(top[i], fmaxf(x[i][j].x, x[i][j].y));
+          });
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float n = m_ref[i] == -INFINITY ? 0.f : -m_ref[i];
-        neg[i] = make_float2(n, n);
-        sum[i] = make_float2(0.f, 0.f);
-      }
+          for (int o = 1; o < 4; o <<= 1)
 #pragma unroll
-      for (int k0 = 0; k0 < KT; k0 += CC) {
-        uint32_t packed[GV][CC / 4];
-#pragma unroll
-        for (int j = 0; j < CP; ++j) {
-          const float2* from = reinterpret_cast<const float2*>(sv) + (k0 / 2 + 4 * j + qt) * GV;
-          float2 w[GV];
-          if (GV == 1) {
-            w[0] = from[0];
-          } else {
-            const float4 v = *reinterpret_cast<const float4*>(from);
-            w[0] = make_float2(v.x, v.y);
-            w[GV - 1] = make_float2(v.z, v.w);
-          }
+            for (int i = 0; i < 2; ++i)
+              top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float2 p = add2(x[i][k0 / 8 + j], neg[i]);
-            p.x = ex2(p.x);
-            p.y = ex2(p.y);
-            sum[i] = add2(sum[i], p);
-#pragma unroll
-            for (int g = 0; g < GV; ++g) {
-              const float2 v = mul2(p, w[g]);
-              const __half2 hv = __floats2half2_rn(v.x, v.y);
-              packed[g][2 * j + i] = *reinterpret_cast<const uint32_t*>(&hv);
+            corr[i] = 1.f;
+            if (top[i] > m_ref[i]) {             // (from -inf: any score)
+              corr[i] = ex2(m_ref[i] - top[i]);
+              l_run[i] *= corr[i];
+              m_ref[i] = top[i];
             }
           }
-        }
+          if (s > 0) {
+            // O has to stand still: the product before this one is through (the one before on its
+            // barrier is, since scores that came behind that have been read)
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(s - 1) % NS], ((s - 1) / NS) & 1, status,
+                                                   STATUS_EPILOGUE_WAIT, 0x180));
+            tc_fence_after();
+            const uint32_t tmem_oc = tmem_o + lane_addr;
 #pragma unroll
-        for (int g = 0; g < GV; ++g) tmem_st_pairs(tmem_s + g * KT + k0 / 2, packed[g]);
+            for (int g = 0; g < GV; ++g)
+#pragma unroll 1
+              for (int d0 = 0; d0 < 64; d0 += 16) {
+                uint32_t o[8];
+                tmem_ld_frag(tmem_oc + g * 64 + d0, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  o[i] = __float_as_uint(__uint_as_float(o[i]) * (corr[i >> 1 & 1] * same[g]));
+                tmem_st_frag(tmem_oc + g * 64 + d0, o);
+              }
+          }
+        }
+        float2 neg[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float n = m_ref[i] == -INFINITY ? 0.f : -m_ref[i];
+          neg[i] = make_float2(n, n);
+          sum[i] = make_float2(0.f, 0.f);
+        }
+        scores(neg, [&](int k0, const float2(&x)[2][CP]) {
+#pragma unroll
+          for (int j = 0; j < CP; ++j) {
+            const float2* from = reinterpret_cast<const float2*>(sv) + (k0 / 2 + 4 * j + qt) * GV;
+            float2 w[GV];
+            if (GV == 1) {
+              w[0] = from[0];
+            } else {
+              const float4 v = *reinterpret_cast<const float4*>(from);
+              w[0] = make_float2(v.x, v.y);
+              w[GV - 1] = make_float2(v.z, v.w);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 p = make_float2(ex2(x[i][j].x), ex2(x[i][j].y));
+              sum[i] = add2(sum[i], p);
+#pragma unroll
+              for (int g = 0; g < GV; ++g) {
+                const float2 v = mul2(p, w[g]);
+                const __half2 hv = __floats2half2_rn(v.x, v.y);
+                packed[g][2 * j + i] = *reinterpret_cast<const uint32_t*>(&hv);
+              }
+            }
+          }
+        });
+        if (moves) break;
+        // (a sum that is not a number comes from scores that are none: it is not asked about again)
+        moves = __any_sync(0xffffffffu, sum[0].x + sum[0].y > CAP || sum[1].x + sum[1].y > CAP);
+        if (!moves) break;
+#pragma unroll
+        for (int g = 0; g < GV; ++g) same[g] = 1.f;
       }
+#pragma unroll
+      for (int c = 0; c < KT / CS; ++c)
+#pragma unroll
+        for (int g = 0; g < GV; ++g) {
+          uint32_t part[CS / 4];
+#pragma unroll
+          for (int k = 0; k < CS / 4; ++k) part[k] = packed[g][c * (CS / 4) + k];
+          tmem_st_pairs(tmem_s + g * KT + c * (CS / 2), part);
+        }
 #pragma unroll
       for (int i = 0; i < 2; ++i) l_run[i] += sum[i].x + sum[i].y;
       tc_wait_st();

@@ -163,6 +163,19 @@ def test_serving_geometries(dev, qh, kvh, d, rows, groups, shared):
     assert float((out.double() - ref).norm() / ref.norm()) < 2 * 2.0 ** -11 / 3 ** 0.5 * 1.1
 
 
+@pytest.mark.parametrize("qh,kvh,d", [(64, 8, 128), (32, 8, 256)])
+def test_more_pages_to_a_cta_than_a_warp_has_lanes(dev, qh, kvh, d):
+    from orinfer_b200.ops import functional as F
+    rows = 128 // (qh // kvh) * (148 // (kvh * max(1, d // 128))) + 1
+    spec, args = batch(dev, [(128 * 136 + 40, [128 * 136 + 41 + r % 60 for r in range(rows)])], qh, kvh,
+                       d, seed=d)
+    plan = F.SharedPrefix(spec, rows, qh=qh, kvh=kvh, head_dim=d, max_kv_len=128 * 138, device=dev,
+                          force=True)
+    keys = (plan.items[:, 3] - plan.items[:, 2]) * (32 if d > 128 else 64)
+    assert int(keys.max()) > 32 * 128
+    check(dev, spec, args, plan=plan)
+
+
 def test_scores_that_leap_and_scales_over_many_binades(dev):
     spec, args = batch(dev, [(1024, [1024 + n for n in range(1, 40, 3)]), (512, [700, 701])], 8, 2,
                        128, seed=9, score=6.0, fill=False)
