@@ -163,6 +163,29 @@ def test_long_histories_of_many_tokens(dev, hist, step):
     check(dev, logits, kw, permitted)
 
 
+@pytest.mark.parametrize("rows,vocab,hist,biases", [
+    (3, 5000, 2048, 9), (3, 5000, 2049, 9), (38, 5000, 1280, 9), (38, 4000, 1283, 9),
+    (2, 3000, 16384, 5), (2, 3000, 16385, 5), (39, 2000, 17001, 5), (3, 500001, 20001, 40),
+    (38, 200003, 2500, 10)])
+def test_histories_that_the_ctas_of_a_row_sort(dev, rows, vocab, hist, biases):
+    """As long as each CTA looks through, one token more, as long as is sorted at a time and more,
+    for few rows and many, on vocabularies of one table and of several; at any alignment."""
+    logits, kw, permitted = case(rows, vocab, hist, biases)
+    kw["history_len"][-1] = hist - 1
+    check(dev, logits, kw, permitted)
+
+
+def test_many_biases_of_a_row_among_many(dev):
+    n, rows, vocab = 32768, 38, 30000
+    g = torch.Generator().manual_seed(4)
+    logits, kw, permitted = case(rows, vocab, 40, 0, masks=False)
+    start = torch.full((rows + 1,), n, dtype=torch.int32)
+    start[0] = 0
+    kw.update(bias_start=start, bias_values=torch.rand(n, generator=g, dtype=torch.float64),
+              bias_ids=torch.randint(0, vocab, (n,), generator=g, dtype=torch.int32))
+    check(dev, logits, kw, permitted)
+
+
 def test_many_biases_on_a_large_vocabulary(dev):
     """As many entries as a row may have, most tokens named more than once, on more tokens than the
     tables of a cluster hold; one entry more is refused."""
