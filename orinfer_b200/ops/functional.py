@@ -269,14 +269,18 @@ class SharedPrefix:
         f32 = lambda n: torch.empty(n, dtype=torch.float32, device=self.device) if n else None
         self.part_buffer = f32(self.parts * qh * (head_dim + 2))
         # The own keys, by the row kernels: as many as the middle row may have.  Beside a prefix they
-        # are split only where they are long, else where they are not short: a merge is a launch of
-        # its own (32 / 8 heads of 128, 384 keys: two rows 6.0 us in one part and 5.5 in six, eight
-        # rows 6.1 and 7.4, and the launch takes the host 2.3).
+        # are split where they are long, and where a CTA has eight heads to join and there are few of
+        # them (the merge's have one; 16 / 2 heads of 256, 37 rows of 150 keys 34.4 us in one part,
+        # 30.7 in three, 100 rows 54 and 60; 32 / 8 of 128, 40 rows of 250 keys 29.1 and 37.0).  Without
+        # a prefix they are split where they are not short: a merge is a launch of its own (32 / 8
+        # heads of 128, 384 keys: two rows 6.0 us in one part and 5.5 in six, eight rows 6.1 and 7.4,
+        # and the launch takes the host 2.3).
         shared = sorted(i[0] for i in info)
         self.own_keys = max(1, max_kv_len - (shared[len(shared) // 2] if items else 0))
         self.splits = attention_splits(self.own_keys, max(1, rows), kvh)
         if items:
-            self.splits = max(1, min(self.splits, self.own_keys // 512))
+            few = min(3, self.own_keys // 48, 2 * 148 // (rows * kvh)) if rep == 8 else 1
+            self.splits = max(1, few, min(self.splits, self.own_keys // 512))
         elif self.own_keys <= 384 and head_dim <= 128:
             self.splits = 1
         self.scratch = f32(rows * qh * self.splits * (head_dim + 2)) if self.splits > 1 else None
