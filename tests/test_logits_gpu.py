@@ -166,7 +166,7 @@ def test_long_histories_of_many_tokens(dev, hist, step):
 @pytest.mark.parametrize("rows,vocab,hist,biases", [
     (3, 5000, 2048, 9), (3, 5000, 2049, 9), (38, 5000, 1280, 9), (38, 4000, 1283, 9),
     (2, 3000, 16384, 5), (2, 3000, 16385, 5), (39, 2000, 17001, 5), (3, 500001, 20001, 40),
-    (38, 200003, 2500, 10)])
+    (38, 200003, 2500, 10), (38, 3001, 33001, 5)])
 def test_histories_that_the_ctas_of_a_row_sort(dev, rows, vocab, hist, biases):
     """As long as each CTA looks through, one token more, as long as is sorted at a time and more,
     for few rows and many, on vocabularies of one table and of several; at any alignment."""
