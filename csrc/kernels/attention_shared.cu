@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
               for (int g = 0; g < GV; ++g) {
                 const float2 v = mul2(p, w[g]);
                 const __half2 hv = __floats2half2_rn(v.x, v.y);
-                packed[g][2 * j + i] = *reinterpret_cast<const uint32_t*>(&hv);
+                packed[g][k0 / 4 + 2 * j + i] = *reinterpret_cast<const uint32_t*>(&hv);
               }
             }
           }
