@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     const __half* q, const int* row_req, const int* row_pos, const int* page_table, int slots,
     int max_pages, const int8_t* kc, const int8_t* vc, const __half* ks, const __half* vs,
     const Item* items, const int4* info, float* __restrict__ part_o, float2* __restrict__ part_ml,
-    int qh, int kvh, int rep, int num_pages, int* status) {
+    int* ready, int qh, int kvh, int rep, int num_pages, int* status) {
   using L = Shape<D>;
   constexpr int G = L::G, GV = L::GV, KT = L::KT, NB = L::NB, CC = L::CC, CS = L::CS;
   constexpr int NS = 3;                  // steps whose scores have a place
@@ -202,6 +202,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
 
   const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
   grid_wait();
+  // The row kernel runs beside this one (attn_start_beside): it is let go by grid_release, and by this
+  // word it sees what lies before the wait.  So the wait comes first, in every CTA, and both behind it.
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(ready), "r"(1) : "memory");
   const Item it = items[blockIdx.x];
   const int h = blockIdx.y / L::PARTS, vpart = blockIdx.y % L::PARTS;
   const int steps = it.step_hi - it.step_lo;
@@ -718,8 +722,8 @@ static int launch_prefix(const __half* q, const int* row_req, const int* row_pos
   if (const int e = runtime_allow_smem(slot, prefix_kernel<D>, L::TOTAL)) return e;
   launch_early(prefix_kernel<D>, dim3(n_items, kvh * L::PARTS), THREADS, L::TOTAL, stream, q,
                row_req, row_pos, page_table, slots, max_pages, kc, vc, ks, vs, items, parts.rows,
-               const_cast<float*>(parts.o), const_cast<float2*>(parts.ml), qh, kvh, qh / kvh,
-               num_pages, runtime_status_ptr());
+               const_cast<float*>(parts.o), const_cast<float2*>(parts.ml), parts.ready, qh, kvh,
+               qh / kvh, num_pages, runtime_status_ptr());
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -732,8 +736,8 @@ using namespace orinfer;
 extern "C" int orinfer_shared_step(int head_dim) { return head_dim > 128 ? 32 : 64; }
 
 // items: int32 [n_items, 8], see Item; rows_info: int32 [rows, 4] = (shared keys, first part, parts,
-// 0); parts: FP32 [all parts, query heads, D] and behind it [all parts, query heads, 2]; scratch: for
-// splits > 1, orinfer_attention_scratch_bytes.
+// 0); parts: FP32 [all parts, query heads, D], behind it [all parts, query heads, 2] and a word that is 0
+// before the first call; scratch: for splits > 1, orinfer_attention_scratch_bytes.
 extern "C" int orinfer_attention_shared(
     const __half* q, const __half* gate, const int* row_req, const int* row_pos,
     const int* page_table, int slots, int max_pages, const int8_t* kc, const int8_t* vc,
@@ -754,7 +758,9 @@ extern "C" int orinfer_attention_shared(
   shared.pending = n_items > 0;
   shared.rows = reinterpret_cast<const int4*>(rows_info);
   shared.o = parts;
-  shared.ml = reinterpret_cast<const float2*>(parts + static_cast<size_t>(n_parts) * qh * head_dim);
+  const size_t cells = static_cast<size_t>(n_parts) * qh;
+  shared.ml = reinterpret_cast<const float2*>(parts + cells * head_dim);
+  shared.ready = reinterpret_cast<int*>(parts + cells * (head_dim + 2));
   const sp::Item* list = reinterpret_cast<const sp::Item*>(items);
   if (n_items > 0) {
     int e = -1;

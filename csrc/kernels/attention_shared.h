@@ -9,10 +9,11 @@
 namespace orinfer {
 
 struct SharedParts {
-  int pending = 0;                 // the kernel in front makes the parts: they are waited for, no more
+  int pending = 0;                 // the kernel in front makes the parts; the row kernel runs beside it
   const int4* rows = nullptr;      // per row: shared keys, first part, parts, -
   const float* o = nullptr;        // [parts][query heads][D]: sums of weighted values
   const float2* ml = nullptr;      // [parts][query heads]: the weights' reference and their sum
+  int* ready = nullptr;            // 1 where the kernel in front has waited for what lies before it
 };
 
 // Attention of single rows over the keys behind row.x, joined with the parts; see orinfer_attention.

@@ -140,7 +140,8 @@ __device__ __forceinline__ void hand_back(uint64_t* bar, uint32_t seen) {
 // goes for weights too, which a program may copy between two launches.  (It cost nothing: every
 // call measured took the same time within 1 %.)  grid_release lets the next kernel become resident
 // in turn; kernels that allocate tensor memory call it after that, so that a successor cannot take
-// what they need.
+// what they need.  One exception reads before it waits, attention's row kernels beside the kernel of
+// a shared prefix: that kernel releases a word behind its own wait, which they acquire.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

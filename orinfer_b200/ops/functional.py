@@ -267,7 +267,9 @@ class SharedPrefix:
         self.items = put(items) if items else None
         self.info = put(info if info else [[0] * 4])
         f32 = lambda n: torch.empty(n, dtype=torch.float32, device=self.device) if n else None
-        self.part_buffer = f32(self.parts * qh * (head_dim + 2))
+        # (behind the parts the word by which the kernels of a call hand on what lies before them)
+        self.part_buffer = (torch.zeros(self.parts * qh * (head_dim + 2) + 1, dtype=torch.float32,
+                                        device=self.device) if items else None)
         # The own keys, by the row kernels: as many as the middle row may have.  Beside a prefix they
         # are split where they are long, and where a CTA has eight heads to join and there are few of
         # them (the merge's have one; 16 / 2 heads of 256, 37 rows of 150 keys 34.4 us in one part,
