@@ -9,29 +9,33 @@
 //
 //   S_g = Q K_g^T   a sum of its own per group of 64 channels, K as the exact FP16 integers that the
 //                   cache holds;  score = sum_g S_g x key scale_g in FP32;
-//   O_g = P_g V_g   P_g = weight x value scale_g rounded to FP16, V as exact integers.
-// So a row's result carries one rounding of FP16 per weight (2.9e-4 against 64 bits with the
-// output's own 2.07e-4); keys and values rounded after their scales, as prefill attention has them,
-// would add one each and another 40 %.  P_g is taken under a power of two per group that follows the
-// value scales, so that it stays among FP16's normal numbers.
+//   O_g = P_g V_g   P_g = weight x value scale_g as the sum of two BF16 numbers, V as the exact BF16
+//                   integers that the cache holds.
+// So a weight is off by 2^-18 of it at most, whatever the other keys' weights and value scales are: BF16
+// has FP32's range.  (One FP16 number under a unit that follows the value scales left 2.9e-4 against 64
+// bits where the output's own rounding is 2.07e-4, and lost the bits of keys beside one with a large
+// scale and no weight.)
 //
 // Scores of three steps have a place in TMEM, so that the products run ahead of the eight softmax warps
 // (sixteen rows each), which go from step to step without a wait.  The weights replace the scores that
 // they are made of.  Two teams of dequantising warps take a step each in turn.
 //
-// 64 rows of 32 query heads behind 16384 keys of 4 KV heads of 128: 34 us, 510 TFLOP/s, with the rows'
-// own keys and the join 46 (each row reading all keys 237); 5 us of the 34 are the start and the end.
-// What bounds it is a step of 64 keys, 1800 cycles, in which nothing is at work for long: a scheduler
-// issues in half of its cycles, the tensor pipe works for a quarter, exponentials for a quarter, DRAM
-// for 5 %.  Without the softmax's arithmetic a step takes 1650 cycles, without the dequantisation 1450,
-// with neither 1000: each is a chain in few warps, and they wait for one another.
-// Tried: two tiles to a CTA, sixteen softmax warps that exchange maxima and sums, raw tiles by bulk
-// copies ahead of the dequantisation (each slower by 5 to 20 %); scores read from TMEM ahead of the
-// exponentials of the step before (50 to 53 us); all dequantising warps on each step (47), four teams
-// (47); a second warp for the scales (46).
+// 64 rows of 32 query heads behind 16384 keys of 4 KV heads of 128: 40 us, with the rows' own keys and the
+// join 49.5 (each row reading all keys 237); 5 us are the start and the end.  With one FP16 number to a
+// weight it is 35.5 and 45.9: a weight's second half is four instructions for two of them, of which two
+// are conversions at half a scheduler's rate, next to the exponentials at a quarter (with the weights
+// made behind all exponentials of a step 51.6, with shifts and masks for the remainders 50).
+// What bounds it is a step of 64 keys, 2300 cycles, in which nothing is at work for long: each role is a
+// chain in few warps, and they wait for one another.
+// Tried with one FP16 number to a weight (46 us): two tiles to a CTA, sixteen softmax warps that exchange
+// maxima and sums, raw tiles by bulk copies ahead of the dequantisation (each slower by 5 to 20 %);
+// scores read from TMEM ahead of the exponentials of the step before (50 to 53); all dequantising warps
+// on each step (47), four teams (47); a second warp for the scales (46).
 #include "api.h"
 #include "attention_shared.h"
 #include "common.cuh"
+
+#include <cuda_bf16.h>
 
 namespace orinfer {
 namespace sp {
@@ -40,7 +44,7 @@ constexpr int TILE = 128;                        // rows of a tile: positions x 
 constexpr int SOFTMAX_WARPS = 8, DQ_WARPS = 8, DQ_TEAMS = 2;
 constexpr int MMA_WARP = SOFTMAX_WARPS + DQ_WARPS, SCALE_WARP = MMA_WARP + 1;
 constexpr int THREADS = (SCALE_WARP + 1) * 32;
-constexpr float CAP = 256.f;                     // of a thread's weights of a step, in all
+constexpr float LEAD = 60.f;                     // of a score above the reference, in binades
 
 template <int D>
 struct Shape {
@@ -54,16 +58,16 @@ struct Shape {
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = G * QSUB;
   static constexpr int SCALE_OFF = KV_OFF + NB * (K_BYTES + V_BYTES);
-  static constexpr int SCALES = KT * (G + GV) * 4 + 16;        // key and value scales, units
+  static constexpr int SCALES = KT * (G + GV) * 4;             // key and value scales
   static constexpr int STAT_OFF = SCALE_OFF + NB * SCALES;     // [sum, reference][128]
   static constexpr int BAR_OFF = STAT_OFF + 2 * TILE * 4;
-  static constexpr int CC = KT;                  // score columns of a group that are read at a time
-  static constexpr int CS = D > 128 ? 16 : 32;   // and that are replaced by weights at a time
+  static constexpr int CS = 16;                  // keys whose weights are stored at a time
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;
   static constexpr int SUB = DV / 2;             // channels that a warp writes, of 32 rows: in the ring
   static_assert(SOFTMAX_WARPS * 32 * SUB * 4 <= NB * (K_BYTES + V_BYTES), "results fit the ring");
   static_assert(TOTAL <= 227 * 1024, "exceeds the shared memory of one CTA");
   static_assert(SCALES % 16 == 0, "scales are read sixteen bytes at a time");
+  static_assert(GV <= G, "both halves of the weights, 16 bits each, fit the places of their scores");
 };
 
 // Rows and keys of a CTA (as many as the plan has), per KV head.
@@ -162,12 +166,47 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 __device__ __forceinline__ float2 pair_at(uint32_t a, uint32_t b) {
   return make_float2(__uint_as_float(a), __uint_as_float(b));
 }
+// Two values as BF16 numbers and as BF16 numbers for what those leave: off by 2^-18 of them at most.
+__device__ __forceinline__ void split_bf16(const float2& v, uint32_t& big, uint32_t& rest) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
+  big = *reinterpret_cast<const uint32_t*>(&b);
+  float2 left;                                   // (an FP32 number less a half of a word: one instruction)
+  asm("{\n\t.reg .b16 l, h, m;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "mov.b16 m, 0xbf80;\n\t"
+      "fma.rn.f32.bf16 %0, l, m, %3;\n\t"
+      "fma.rn.f32.bf16 %1, h, m, %4;\n\t}"
+      : "=f"(left.x), "=f"(left.y)
+      : "r"(big), "f"(v.x), "f"(v.y));
+  const __nv_bfloat162 r = __floats2bfloat162_rn(left.x, left.y);
+  rest = *reinterpret_cast<const uint32_t*>(&r);
+}
 
+// Eight INT8 values -> eight BF16 values, exactly: 0x43xx is 128 + xx for seven bits, from which 128 is
+// subtracted, or 256 where the eighth is set.
+__device__ __forceinline__ uint4 integers_bf16(uint32_t w0, uint32_t w1) {
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = i < 2 ? w0 : w1, at = i % 2 ? 0x4342u : 0x4140u;
+    const uint32_t low = __byte_perm(w & 0x7f7f7f7fu, 0x43434343u, at);
+    const uint32_t off = __byte_perm(w & 0x80808080u, 0x43434343u, at);
+    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&low),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&off));
+    h[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(h[0], h[1], h[2], h[3]);
+}
 // Eight INT8 values -> eight FP16 values, exactly: 0x64xx is 1024 + xx, and 1152 is subtracted.
-__device__ __forceinline__ uint4 integers(uint32_t w0, uint32_t w1) {
+__device__ __forceinline__ uint4 integers_fp16(uint32_t w0, uint32_t w1) {
   const __half2 bias = __half2half2(__ushort_as_half(0x6480));
   const uint32_t x0 = w0 ^ 0x80808080u, x1 = w1 ^ 0x80808080u;
   uint32_t h[4] = {__byte_perm(x0, 0x64646464u, 0x4140), __byte_perm(x0, 0x64646464u, 0x4342),
@@ -187,7 +226,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     const Item* items, const int4* info, float* __restrict__ part_o, float2* __restrict__ part_ml,
     int* ready, int qh, int kvh, int rep, int num_pages, int* status) {
   using L = Shape<D>;
-  constexpr int G = L::G, GV = L::GV, KT = L::KT, NB = L::NB, CC = L::CC, CS = L::CS;
+  constexpr int G = L::G, GV = L::GV, KT = L::KT, NB = L::NB, CS = L::CS;
   constexpr int NS = 3;                  // steps whose scores have a place
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -244,7 +283,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
   if (warp == MMA_WARP) {
     // ---------------- products, issued by the whole warp (see elect_one)
     constexpr uint32_t idesc_s = umma_idesc(1, 0, 0, 0, 0, TILE, KT);
-    constexpr uint32_t idesc_o = umma_idesc(1, 0, 0, 0, 1, TILE, 64);
+    constexpr uint32_t idesc_o = umma_idesc(1, 1, 1, 0, 1, TILE, 64);
     const uint32_t leader = elect_one();
     const uint64_t qd = umma_desc(smem_u32(smem + L::Q_OFF), 16, 1024);
     const uint64_t kd = umma_desc(smem_u32(smem + L::KV_OFF), 16, 1024);
@@ -285,21 +324,20 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       for (int g = 0; g < GV; ++g)
 #pragma unroll
         for (int k = 0; k < KT / 16; ++k)
-          mma_ts(leader, tmem_o + g * 64,
-                 tmem + 128 * (s % NS) + g * KT + k * 8, vb + (g * L::KSUB + k * 2048) / 16, idesc_o, (s | k) != 0 ? 1u : 0u);
+#pragma unroll
+          for (int part = 0; part < 2; ++part)   // of the weights
+            mma_ts(leader, tmem_o + g * 64,
+                   tmem + 128 * (s % NS) + g * KT + part * (KT / 2) + k * 8,
+                   vb + (g * L::KSUB + k * 2048) / 16, idesc_o, (s | k | part) != 0 ? 1u : 0u);
       tc_commit_by(leader, &kv_free[b]);
       tc_commit_by(leader, &o_done[s % NS]);
       if (s + NS < last) issue_qk(s + NS);       // (in the place of the weights just used)
     }
     __syncwarp();
   } else if (warp == SCALE_WARP) {
-    // ---------------- scales: times log2 e / sqrt(D) for keys, times the group's unit for values.
-    // All of a lane's are of one group.
+    // ---------------- scales, of keys times log2 e / sqrt(D)
     constexpr int KS = KT * G / 32, VS = KT * GV / 32;
     const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
-    float unit[GV];
-#pragma unroll
-    for (int g = 0; g < GV; ++g) unit[g] = __uint_as_float((127 + 29) << 23);
     bool ok = true;
     __half kraw[KS], vraw[VS];
     int ids = pages_from(0), ids_at = 0;
@@ -332,22 +370,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       if (!ok) break;
       float* sk = reinterpret_cast<float*>(smem + L::SCALE_OFF + b * L::SCALES);
       float* sv = sk + KT * G;
-      float* su = sv + KT * GV;
       // slots behind the shared keys may never have been written: they get no scale
-      uint32_t big = 0;                          // FP16 magnitudes are ordered as their bits
-#pragma unroll
-      for (int i = 0; i < VS; ++i) {
-        const uint32_t bits = __half_as_ushort(vraw[i]) & 0x7fffu;
-        if ((lane + 32 * i) / GV < live && bits < 0x7c00u) big = max(big, bits);
-      }
-#pragma unroll
-      for (int g = 0; g < GV; ++g) {
-        const uint32_t top = __reduce_max_sync(0xffffffffu, lane % GV == g ? big : 0u);
-        const float v = __half2float(__ushort_as_half(static_cast<unsigned short>(top)));
-        // v x unit in [16, 32) when chosen, below 128 as long as it is kept
-        if (v * unit[g] >= 128.f)
-          unit[g] = __uint_as_float((127 + 5 + 126 - (__float_as_uint(v) >> 23)) << 23);
-      }
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         const int x = lane + 32 * i, key = x / G, g = x % G;
@@ -357,10 +380,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
 #pragma unroll
       for (int i = 0; i < VS; ++i) {
         const int x = lane + 32 * i, key = x / GV, g = x % GV;
-        sv[((key >> 1) * GV + g) * 2 + (key & 1)] =
-            key < live ? __half2float(vraw[i]) * unit[GV == 1 ? 0 : g] : 0.f;
+        sv[((key >> 1) * GV + g) * 2 + (key & 1)] = key < live ? __half2float(vraw[i]) : 0.f;
       }
-      if (lane < GV) su[lane] = unit[GV == 1 ? 0 : lane];
       __syncwarp();
       if (lane == 0) mbar_arrive(&kv_full[b]);
       if (s + 1 < steps) load(s + 1);
@@ -391,7 +412,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
                                                 vpart * L::DV + c * 16);
       }
     };
-    auto place = [&](unsigned char* to, const uint4& raw, int key, int c) {
+    auto place = [&](unsigned char* to, const uint4& raw, int key, int c, auto integers) {
       // lanes of every other group of channels store their second half first: eight lanes that
       // store together then meet on no bank
       unsigned char* dst = to + (c / 4) * L::KSUB;
@@ -413,12 +434,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
         const int x = u + i * DQ;
-        place(buf, kraw[i], x / (D / 16), x % (D / 16));
+        place(buf, kraw[i], x / (D / 16), x % (D / 16), integers_fp16);
       }
 #pragma unroll
       for (int i = 0; i < VI; ++i) {
         const int x = u + i * DQ;
-        place(buf + L::K_BYTES, vraw[i], x / (L::DV / 16), x % (L::DV / 16));
+        place(buf + L::K_BYTES, vraw[i], x / (L::DV / 16), x % (L::DV / 16), integers_bf16);
       }
       fence_proxy_async();
       __syncwarp();
@@ -477,10 +498,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     }
     const int all_see = __reduce_min_sync(0xffffffffu, min(sees[0], sees[1]));
     const uint32_t lane_addr = static_cast<uint32_t>(row0) << 16;
-    constexpr int CP = CC / 8;                   // pairs of keys of a thread, at a time
-    float m_ref[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, unit[GV];
-#pragma unroll
-    for (int g = 0; g < GV; ++g) unit[g] = 1.f;
+    float m_ref[2] = {0.f, 0.f}, l_run[2] = {0.f, 0.f};
     bool ok = true;
     for (int s = 0; s < steps; ++s) {
       const int b = s % NB;
@@ -494,160 +512,129 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       // scales by pairs of keys and groups: those of this thread's pair `j`
       const float* sk = reinterpret_cast<const float*>(smem + L::SCALE_OFF + b * L::SCALES);
       const float* sv = sk + KT * G;
-      const float* su = sv + KT * GV;
       const int key0 = (it.step_lo + s) * KT;
-      // `f(k0, x)`: scores less `less`, of CC keys from k0 on, pair by pair of this thread's two rows
-      auto scores = [&](const float2(&less)[2], auto f) {
+      // ---- scores less the reference, pair by pair of this thread's two rows
+      float2 x[2][KT / 8];
+      {
+        uint32_t raw[G][KT / 2];
 #pragma unroll
-        for (int k0 = 0; k0 < KT; k0 += CC) {
-          uint32_t raw[G][CC / 2];
+        for (int g = 0; g < G; ++g) tmem_ld_frag(tmem_s + g * KT, raw[g]);
+        tc_wait_ld();
 #pragma unroll
-          for (int g = 0; g < G; ++g) tmem_ld_frag(tmem_s + g * KT + k0, raw[g]);
-          tc_wait_ld();
-          float2 x[2][CP];
+        for (int j = 0; j < KT / 8; ++j) {
+          const float2* w = reinterpret_cast<const float2*>(sk) + (4 * j + qt) * G;
+          float2 wg[G];
+          if (G == 1) {
+            wg[0] = w[0];
+          } else {
 #pragma unroll
-          for (int j = 0; j < CP; ++j) {
-            const float2* w = reinterpret_cast<const float2*>(sk) + (k0 / 2 + 4 * j + qt) * G;
-            float2 wg[G];
-            if (G == 1) {
-              wg[0] = w[0];
-            } else {
-#pragma unroll
-              for (int g = 0; g < G; g += 2) {
-                const float4 v = *reinterpret_cast<const float4*>(w + g);
-                wg[g] = make_float2(v.x, v.y);
-                wg[(g + 1) % G] = make_float2(v.z, v.w);
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              x[i][j] = less[i];
-#pragma unroll
-              for (int g = 0; g < G; ++g)
-                x[i][j] = fma2(pair_at(raw[g][4 * j + 2 * i], raw[g][4 * j + 2 * i + 1]), wg[g],
-                               x[i][j]);
+            for (int g = 0; g < G; g += 2) {
+              const float4 v = *reinterpret_cast<const float4*>(w + g);
+              wg[g] = make_float2(v.x, v.y);
+              wg[(g + 1) % G] = make_float2(v.z, v.w);
             }
           }
-          if (all_see < key0 + KT) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int j = 0; j < CP; ++j) {
-                const int key = key0 + k0 + 8 * j + 2 * qt;
-                if (key >= sees[i]) x[i][j].x = -INFINITY;
-                if (key + 1 >= sees[i]) x[i][j].y = -INFINITY;
-              }
-          }
-          f(k0, x);
-        }
-      };
-      // ---- weights, under a reference that is the maximum of some step: their sum, which is wanted
-      // anyway, says whether they stay small (CAP times a value scale's 128 is within FP16).  Only
-      // steps where it does not take maxima, move the reference and make their weights once more.
-      bool moves = s == 0;
-      float same[GV];
-#pragma unroll
-      for (int g = 0; g < GV; ++g) {             // units are powers of two
-        const float now = su[g];
-        same[g] = now * __uint_as_float((254u << 23) - __float_as_uint(unit[g]));
-        moves = moves || now != unit[g];
-        unit[g] = now;
-      }
-      float2 sum[2];
-      uint32_t packed[GV][KT / 4];
-      for (;;) {
-        if (moves) {
-          float top[2] = {-INFINITY, -INFINITY}, corr[2];
-          const float2 none[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          scores(none, [&](int, const float2(&x)[2][CP]) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int j = 0; j < CP; ++j) top[i] = fmaxf(top[i], fmaxf(x[i][j].x, x[i][j].y));
-          });
-#pragma unroll
-          for (int o = 1; o < 4; o <<= 1)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            corr[i] = 1.f;
-            if (top[i] > m_ref[i]) {             // (from -inf: any score)
-              corr[i] = ex2(m_ref[i] - top[i]);
-              l_run[i] *= corr[i];
-              m_ref[i] = top[i];
-            }
-          }
-          if (s > 0) {
-            // O has to stand still: the product before this one is through (the one before on its
-            // barrier is, since scores that came behind that have been read)
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(s - 1) % NS], ((s - 1) / NS) & 1, status,
-                                                   STATUS_EPILOGUE_WAIT, 0x180));
-            tc_fence_after();
-            const uint32_t tmem_oc = tmem_o + lane_addr;
+            x[i][j] = make_float2(-m_ref[i], -m_ref[i]);
 #pragma unroll
-            for (int g = 0; g < GV; ++g)
-#pragma unroll 1
-              for (int d0 = 0; d0 < 64; d0 += 16) {
-                uint32_t o[8];
-                tmem_ld_frag(tmem_oc + g * 64 + d0, o);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  o[i] = __float_as_uint(__uint_as_float(o[i]) * (corr[i >> 1 & 1] * same[g]));
-                tmem_st_frag(tmem_oc + g * 64 + d0, o);
-              }
+            for (int g = 0; g < G; ++g)
+              x[i][j] = fma2(pair_at(raw[g][4 * j + 2 * i], raw[g][4 * j + 2 * i + 1]), wg[g],
+                             x[i][j]);
           }
         }
-        float2 neg[2];
+      }
+      if (all_see < key0 + KT) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j) {
+            const int key = key0 + 8 * j + 2 * qt;
+            if (key >= sees[i]) x[i][j].x = -INFINITY;
+            if (key + 1 >= sees[i]) x[i][j].y = -INFINITY;
+          }
+      }
+      // ---- the reference is the maximum of some step, and moves where a score is LEAD above it: weights,
+      // their products with value scales and integers and a prefix's sums of them stay in FP32's range
+      float top[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(x[i][0].x, x[i][0].y);
+#pragma unroll
+        for (int j = 1; j < KT / 8; ++j) top[i] = max3(top[i], x[i][j].x, x[i][j].y);
+      }
+      if (__any_sync(0xffffffffu, s == 0 || fmaxf(top[0], top[1]) > LEAD)) {
+        float corr[2];
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float n = m_ref[i] == -INFINITY ? 0.f : -m_ref[i];
-          neg[i] = make_float2(n, n);
-          sum[i] = make_float2(0.f, 0.f);
+          // (a row that sees none of these keys stays; at first there is nothing to be lost)
+          const float by = top[i] == -INFINITY ? 0.f : s == 0 ? top[i] : fmaxf(top[i], 0.f);
+          corr[i] = s == 0 ? 0.f : ex2(-by);
+          l_run[i] *= corr[i];
+          m_ref[i] += by;
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j) x[i][j] = add2(x[i][j], make_float2(-by, -by));
         }
-        scores(neg, [&](int k0, const float2(&x)[2][CP]) {
+        if (s > 0) {
+          // O has to stand still: the product before this one is through (the one before on its
+          // barrier is, since scores that came behind that have been read)
+          ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(s - 1) % NS], ((s - 1) / NS) & 1, status,
+                                                 STATUS_EPILOGUE_WAIT, 0x180));
+          tc_fence_after();
+          const uint32_t tmem_oc = tmem_o + lane_addr;
 #pragma unroll
-          for (int j = 0; j < CP; ++j) {
-            const float2* from = reinterpret_cast<const float2*>(sv) + (k0 / 2 + 4 * j + qt) * GV;
-            float2 w[GV];
-            if (GV == 1) {
-              w[0] = from[0];
-            } else {
-              const float4 v = *reinterpret_cast<const float4*>(from);
-              w[0] = make_float2(v.x, v.y);
-              w[GV - 1] = make_float2(v.z, v.w);
+          for (int g = 0; g < GV; ++g)
+#pragma unroll 1
+            for (int d0 = 0; d0 < 64; d0 += 16) {
+              uint32_t o[8];
+              tmem_ld_frag(tmem_oc + g * 64 + d0, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                o[i] = __float_as_uint(__uint_as_float(o[i]) * corr[i >> 1 & 1]);
+              tmem_st_frag(tmem_oc + g * 64 + d0, o);
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float2 p = make_float2(ex2(x[i][j].x), ex2(x[i][j].y));
-              sum[i] = add2(sum[i], p);
-#pragma unroll
-              for (int g = 0; g < GV; ++g) {
-                const float2 v = mul2(p, w[g]);
-                const __half2 hv = __floats2half2_rn(v.x, v.y);
-                packed[g][k0 / 4 + 2 * j + i] = *reinterpret_cast<const uint32_t*>(&hv);
-              }
-            }
-          }
-        });
-        if (moves) break;
-        // (a sum that is not a number comes from scores that are none: it is not asked about again)
-        moves = __any_sync(0xffffffffu, sum[0].x + sum[0].y > CAP || sum[1].x + sum[1].y > CAP);
-        if (!moves) break;
-#pragma unroll
-        for (int g = 0; g < GV; ++g) same[g] = 1.f;
+        }
       }
+      // ---- weights, times the value scales: each as a BF16 number and another for what that leaves, in
+      // the place of the scores
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < KT / CS; ++c)
+      for (int c = 0; c < KT / CS; ++c) {
+        uint32_t big[GV][CS / 4], rest[GV][CS / 4];
+#pragma unroll
+        for (int j = 0; j < CS / 8; ++j) {
+          const float2* from =
+              reinterpret_cast<const float2*>(sv) + (c * (CS / 2) + 4 * j + qt) * GV;
+          float2 w[GV];
+          if (GV == 1) {
+            w[0] = from[0];
+          } else {
+            const float4 v = *reinterpret_cast<const float4*>(from);
+            w[0] = make_float2(v.x, v.y);
+            w[GV - 1] = make_float2(v.z, v.w);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 at = x[i][c * (CS / 8) + j];
+            const float2 p = make_float2(ex2(at.x), ex2(at.y));
+            sum[i] = add2(sum[i], p);
+#pragma unroll
+            for (int g = 0; g < GV; ++g)
+              split_bf16(mul2(p, w[g]), big[g][2 * j + i], rest[g][2 * j + i]);
+          }
+        }
 #pragma unroll
         for (int g = 0; g < GV; ++g) {
-          uint32_t part[CS / 4];
-#pragma unroll
-          for (int k = 0; k < CS / 4; ++k) part[k] = packed[g][c * (CS / 4) + k];
-          tmem_st_pairs(tmem_s + g * KT + c * (CS / 2), part);
+          tmem_st_pairs(tmem_s + g * KT + c * (CS / 2), big[g]);
+          tmem_st_pairs(tmem_s + g * KT + KT / 2 + c * (CS / 2), rest[g]);
         }
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) l_run[i] += sum[i].x + sum[i].y;
       tc_wait_st();
@@ -675,11 +662,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_WARPS * 32) : "memory");
     const size_t at = static_cast<size_t>(part) * qh + h * rep + r % rep;
     if (half == 0 && vpart == 0 && part >= 0)
-      part_ml[at] = ok ? make_float2(stat[TILE + r], stat[r]) : make_float2(-INFINITY, 0.f);
+      part_ml[at] = ok && stat[r] != 0.f ? make_float2(stat[TILE + r], stat[r])
+                                         : make_float2(-INFINITY, 0.f);
     constexpr int SUB = L::SUB;
     const int d_lo = half * SUB;                 // this warp's channels, all of one group
-    const float last_unit = GV == 2 && half == 1 ? unit[GV - 1] : unit[0];
-    const float back = ok ? __uint_as_float((254u << 23) - __float_as_uint(last_unit)) : 0.f;
     unsigned char* slab = smem + L::KV_OFF + warp * (32 * SUB * 4);
     auto cell = [](int row, int chunk) {
       return row * (SUB * 4) + (chunk ^ (row & (SUB / 4 - 1))) * 16;
@@ -692,8 +678,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
         *reinterpret_cast<float4*>(slab + cell(lane, (d0 + i) / 4)) =
-            make_float4(__uint_as_float(o[i]) * back, __uint_as_float(o[i + 1]) * back,
-                        __uint_as_float(o[i + 2]) * back, __uint_as_float(o[i + 3]) * back);
+            ok ? make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
+                             __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]))
+               : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncwarp();
     constexpr int CHUNKS = SUB / 4, ROWS = 32 / CHUNKS;          // rows that a warp writes at a time

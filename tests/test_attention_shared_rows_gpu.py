@@ -63,3 +63,84 @@ def test_the_row_kernels_see_what_came_before_the_prefix(dev, rows, shared, own,
         got.zero_()
         graph.replay()
         assert bool((got == want).all()) and int(word) == 0
+
+
+def near(ref, size, reach):
+    """What arithmetic in FP32 leaves, and the output's rounding, 2^-11 of it at most.  A weight of two
+    BF16 numbers is off by 2^-9 of 2^-9 of it; a score, a sum of up to 256 products of the queries with
+    integers and FP16 scales, by 2^-19 of its terms' magnitudes (2^-23 for each of its up to sixteen
+    additions of sixteen products, which may be cut off); the sums over up to 1200 keys, by 2^-23 for
+    each of 75 additions of sixteen.  FP16 ends at 2^-25."""
+    return 2.0 ** -11 * ref.abs() + size * (2.0 ** -18 + 2.0 ** -19 * reach + 75 * 2.0 ** -23) + 2.0 ** -24
+
+
+def assert_near(args, out, reach=None):
+    ref, size, all_reach = R.attention_rows(*args)
+    reach = all_reach if reach is None else reach
+    off = ((out.double().view_as(ref) - ref).abs() / near(ref, size, reach)).max()
+    assert float(off) <= 1, float(off)
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(2, 2, 64), (8, 2, 64), (8, 2, 128), (10, 2, 128), (8, 1, 128),
+                                      (8, 1, 256), (4, 2, 256)])
+@pytest.mark.parametrize("score", [1.0, 4.0])
+def test_weights_have_the_bits_that_decode_attention_has(dev, qh, kvh, d, score):
+    """Few heavy keys, whose roundings do not cancel, and many light ones; nothing but the output is
+    rounded to FP16."""
+    from orinfer_b200.ops import functional as F
+    spec, args = batch(dev, [(1024, [1024 + n for n in (0, 1, 40, 130)]), (3, [3, 3, 2, 1]),
+                             (64, [64, 70, 65]), (130, [130, 131])], qh, kvh, d, seed=3, score=score,
+                       gated=d == 256)
+    plan = plan_of(args, spec, dev)
+    assert plan.items is not None
+    assert_near(args, F.attention_shared(*args, plan))
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(4, 2, 64), (8, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("key", [0, 70, 500, 1023])
+@pytest.mark.parametrize("binades", [10, 18, 26])
+def test_a_large_value_scale_without_weight_costs_nothing(dev, qh, kvh, d, key, binades):
+    """One key whose values are 2^binades times the others' and whose weight is e^-50 or less."""
+    from orinfer_b200.ops import functional as F
+    spec, args = batch(dev, [(1024, [1024 + n for n in (0, 3, 200)])], qh, kvh, d, seed=binades,
+                       scales=(2.0 ** -12, 2.0 ** -11), fill=False)
+    q, gate, req, pos, table, kc, vc, ks, vs = args
+    q.abs_().add_(0.25)
+    page, at = int(table[int(req[0]), key // 128]), key % 128
+    kc[page, at], ks[page, at], vs[page, at] = 0, 0.06, 2.0 ** (binades - 12)
+    _, _, reach = R.attention_rows(*args)            # (of the keys that have a weight)
+    kc[page, at] = -127
+    assert_near(args, F.attention_shared(*args, plan_of(args, spec, dev)), reach)
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(4, 2, 64), (8, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("key", [0, 1000])
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -24])
+def test_a_key_that_takes_the_weight_and_has_no_value(dev, qh, kvh, d, key, scale):
+    """What the other keys give is small beside it in weight, and all that there is in value."""
+    from orinfer_b200.ops import functional as F
+    spec, args = batch(dev, [(1024, [1024 + n for n in (0, 3, 200)])], qh, kvh, d, seed=key,
+                       scales=(0.01, 0.02), score=0.5, fill=False)
+    q, gate, req, pos, table, kc, vc, ks, vs = args
+    q.abs_().add_(0.25)
+    vs.mul_(1000.0)
+    page, at = int(table[int(req[0]), key // 128]), key % 128
+    kc[page, at], ks[page, at], vs[page, at] = 127, 0.02, scale
+    assert_near(args, F.attention_shared(*args, plan_of(args, spec, dev)))
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(4, 2, 64), (8, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("way", ["up", "down", "steps"])
+def test_references_that_have_to_move_far(dev, qh, kvh, d, way):
+    """Scores over several hundred binades, that climb, fall, or leap every 160 keys."""
+    from orinfer_b200.ops import functional as F
+    spec, args = batch(dev, [(1024, [1024 + n for n in (0, 3, 200)])], qh, kvh, d, seed=len(way),
+                       score=0.5, fill=False)
+    q, gate, req, pos, table, kc, vc, ks, vs = args
+    q.abs_().add_(0.25)
+    kc.copy_(kc.abs().clamp(min=100))
+    at = torch.arange(1024)
+    ramp = {"up": at, "down": 1023 - at, "steps": at // 160 * 170}[way].to(dev) * 2e-4
+    pages = table[req[0].long(), :8].long()
+    ks[pages] = ramp.view(8, 128, 1, 1).half().expand_as(ks[pages])
+    assert_near(args, F.attention_shared(*args, plan_of(args, spec, dev)))
