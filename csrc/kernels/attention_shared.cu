@@ -247,14 +247,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(ready), "r"(1) : "memory");
   const Item it = items[blockIdx.x];
   const int h = blockIdx.y / L::PARTS, vpart = blockIdx.y % L::PARTS;
-  const int steps = it.step_hi - it.step_lo;
-  const int req = row_req[it.row];
-  const bool known = req >= 0 && req < slots;
-  const int* pages = page_table + static_cast<size_t>(known ? req : 0) * max_pages;
-  // A warp's page ids, a lane each, 32 at a time: one that is fetched when it is needed holds up what
-  // is asked for by it.
-  const int page_lo = it.step_lo * KT >> 7, page_hi = it.step_hi * KT - 1 >> 7;
-  auto pages_from = [&](int i) { return page_lo + i + lane <= page_hi ? pages[page_lo + i + lane] : 0; };
+  int request_of_lane[TILE / 32], pos_of_lane[TILE / 32];      // of the tile's rows
+#pragma unroll
+  for (int i = 0; i < TILE / 32; ++i) {
+    const bool there = lane + 32 * i < it.rows;
+    request_of_lane[i] = there ? row_req[it.row + lane + 32 * i] : -1;
+    pos_of_lane[i] = there ? row_pos[it.row + lane + 32 * i] : -1;
+  }
 
   if (tid == 0) {
     for (int b = 0; b < NB; ++b) {
@@ -279,6 +278,26 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
   const uint32_t tmem = warp_same(*tmem_slot);
   grid_release();
   const uint32_t tmem_o = tmem + 128 * NS;       // scores at 128 (step modulo NS)
+
+  // The pages are read from the table row of one that sees the most of the tile's rows, and no further than
+  // that: the others may end before, and their table rows may be empty from there on.
+  int req = 0, last_pos = -1;
+#pragma unroll
+  for (int i = 0; i < TILE / 32; ++i)
+    if (request_of_lane[i] >= 0 && request_of_lane[i] < slots && pos_of_lane[i] > last_pos) {
+      req = request_of_lane[i];
+      last_pos = pos_of_lane[i];
+    }
+  const int top_pos = __reduce_max_sync(0xffffffffu, last_pos);
+  req = __shfl_sync(0xffffffffu, req, __ffs(__ballot_sync(0xffffffffu, last_pos == top_pos)) - 1);
+  const int seen = min(it.shared, top_pos + 1);  // shared keys that some row sees
+  const int step_hi = min(it.step_hi, (seen + KT - 1) / KT);
+  const int steps = max(step_hi - it.step_lo, 0);
+  const int* pages = page_table + static_cast<size_t>(req) * max_pages;
+  // A warp's page ids, a lane each, 32 at a time: one that is fetched when it is needed holds up what
+  // is asked for by it.
+  const int page_lo = it.step_lo * KT >> 7, page_hi = step_hi * KT - 1 >> 7;
+  auto pages_from = [&](int i) { return page_lo + i + lane <= page_hi ? pages[page_lo + i + lane] : 0; };
 
   if (warp == MMA_WARP) {
     // ---------------- products, issued by the whole warp (see elect_one)
@@ -345,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       const int key0 = (it.step_lo + s) * KT, at = (key0 >> 7) - page_lo;
       if (at >= ids_at + 32) ids = pages_from(ids_at += 32);
       int page = __shfl_sync(0xffffffffu, ids, at - ids_at);
-      if (!known || page < 0 || page >= num_pages) {
+      if (page < 0 || page >= num_pages) {
         if (lane == 0) report_status(status, STATUS_BAD_INDEX, 0x50);
         page = 0;
       }
@@ -363,14 +382,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     };
     if (steps > 0) load(0);
     for (int s = 0; s < steps; ++s) {
-      const int b = s % NB, live = it.shared - (it.step_lo + s) * KT;
+      const int b = s % NB, live = seen - (it.step_lo + s) * KT;
       if (s >= NB)
         ok = ok && mbar_wait(&kv_free[b], (s / NB - 1) & 1, status, STATUS_DECODE_WAIT, 0x600);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       float* sk = reinterpret_cast<float*>(smem + L::SCALE_OFF + b * L::SCALES);
       float* sv = sk + KT * G;
-      // slots behind the shared keys may never have been written: they get no scale
+      // slots behind the keys that are seen may never have been written: they get no scale
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         const int x = lane + 32 * i, key = x / G, g = x % G;
@@ -398,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       const int key0 = (it.step_lo + s) * KT, at = (key0 >> 7) - page_lo;
       if (at >= ids_at + 32) ids = pages_from(ids_at += 32);
       int page = __shfl_sync(0xffffffffu, ids, at - ids_at);
-      if (!known || page < 0 || page >= num_pages) page = 0;           // (the scale warp reports it)
+      if (page < 0 || page >= num_pages) page = 0;           // (the scale warp reports it)
       const size_t slot = static_cast<size_t>(page) * 128 + (key0 & 127);
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
@@ -488,13 +507,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     const int qg = lane >> 2, qt = lane & 3;
     const int row0 = quad * 32 + half * 16;      // of the tile
     auto row_of = [&](int tr) {                  // of row `tr` of the tile, or none
-      return tr < TILE / rep * rep && tr / rep < it.rows && known ? it.row + tr / rep : -1;
+      return tr < TILE / rep * rep && tr / rep < it.rows ? it.row + tr / rep : -1;
     };
     int sees[2];                                 // shared keys that its rows see
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = row_of(row0 + qg + 8 * i);
-      sees[i] = row < 0 ? 0 : min(it.shared, row_pos[row] + 1);
+      sees[i] = row < 0 ? 0 : min(seen, row_pos[row] + 1);
     }
     const int all_see = __reduce_min_sync(0xffffffffu, min(sees[0], sees[1]));
     const uint32_t lane_addr = static_cast<uint32_t>(row0) << 16;
@@ -642,11 +661,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[s % NS]);
     }
-    // ---- this part of the rows' softmax, from here on a row per lane.  The ring is free when the last
-    // product is through: a warp puts 32 rows of half of the channels there and writes whole lines.
+    // ---- this part of the rows' softmax, from here on a row per lane: none where no row sees any of these
+    // keys.  The ring is free when the last product is through: a warp puts 32 rows of half of the
+    // channels there and writes whole lines.
     const int r = quad * 32 + lane, row = row_of(r);
     const int part = row < 0 ? -1 : info[row].y + it.part;
-    ok = ok && mbar_wait(&o_done[(steps - 1) % NS], ((steps - 1) / NS) & 1, status,
+    ok = ok && steps > 0 && mbar_wait(&o_done[(steps - 1) % NS], ((steps - 1) / NS) & 1, status,
                          STATUS_EPILOGUE_WAIT, 0x200);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();

@@ -350,7 +350,7 @@ def attention_shared(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: tor
                      plan: SharedPrefix, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`attention` of a batch whose rows share prefixes (``plan``): a shared key is read once
     for all rows of its group.  A row sees keys 0..row_pos[r]; one at position -1 sees none and
-    gives zeros."""
+    gives zeros (a request that has ended may leave its row so while the plan stays)."""
     n, d, kvh, i32, f16 = plan.rows, plan.head_dim, plan.kvh, torch.int32, torch.float16
     _need(q.shape == (n, plan.qh, d) and q.dtype == f16 and q.is_contiguous(),
           "q: contiguous FP16 [rows, heads, D], as the plan has them")

@@ -144,3 +144,47 @@ def test_references_that_have_to_move_far(dev, qh, kvh, d, way):
     pages = table[req[0].long(), :8].long()
     ks[pages] = ramp.view(8, 128, 1, 1).half().expand_as(ks[pages])
     assert_near(args, F.attention_shared(*args, plan_of(args, spec, dev)))
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(4, 2, 64), (8, 2, 128), (8, 1, 128), (8, 1, 256)])
+@pytest.mark.parametrize("nobody", [0, -1, 1 << 20])
+def test_rows_that_have_ended_anywhere_in_a_group(dev, qh, kvh, d, nobody):
+    """Rows at position -1, whose table rows have been given back or whose requests do not exist, at the
+    start of every tile of 128 / rep rows, between the others, and as whole tiles and groups; the plan
+    stays.  The others see their prefix, those give zeros."""
+    from orinfer_b200.ops import functional as F
+    per = 128 // (qh // kvh)
+    rows = 3 * per + 2
+    spec, args = batch(dev, [(640, [641 + r % 90 for r in range(rows)]), (256, [300, 280])], qh, kvh, d,
+                       seed=d, gated=d == 256)
+    q, gate, req, pos, table, *cache = args
+    ended = [0, 1, 5, per, 3 * per, 3 * per + 1, rows, rows + 1] + list(range(2 * per, 3 * per))
+    for r in ended:
+        table[int(req[r])] = 0
+    pos[ended] = -1
+    if nobody:
+        req[ended] = nobody
+    plan = plan_of((q, gate, req, pos, table, *cache), spec, dev, max_kv_len=731)
+    assert plan.items is not None
+    plan.part_buffer[:-1] = float("nan")             # what nobody writes is not read
+    out = F.attention_shared(q, gate, req, pos, table, *cache, plan)
+    assert bool((out[ended] == 0).all())
+    safe = req.clone()
+    safe[ended] = 0
+    assert_near((q, gate, safe, pos, table, *cache), out)
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(4, 2, 64), (8, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("first", [1, 63, 64, 100, 129, 500])
+def test_a_first_row_that_ends_inside_the_prefix(dev, qh, kvh, d, first):
+    """Its table row has nothing that can be read behind its last page, and the rows behind it see all.
+    Where nobody sees the rest of a prefix, nothing of it is read."""
+    from orinfer_b200.ops import functional as F
+    groups = [(1024, [first, 1024, 1030, 900]), (1024, [first, max(1, first // 2)])]
+    spec, args = batch(dev, groups, qh, kvh, d, seed=first)
+    req, pos, table = args[2], args[3], args[4]
+    for r in (0, 4, 5):
+        table[int(req[r]), (int(pos[r]) + 128) // 128:] = -7
+    plan = plan_of(args, spec, dev)
+    plan.part_buffer[:-1] = float("nan")
+    assert_near(args, F.attention_shared(*args, plan))
