@@ -35,6 +35,7 @@
 #include "attention_shared.h"
 #include "common.cuh"
 
+#include <climits>
 #include <cuda_bf16.h>
 
 namespace orinfer {
@@ -60,7 +61,8 @@ struct Shape {
   static constexpr int SCALE_OFF = KV_OFF + NB * (K_BYTES + V_BYTES);
   static constexpr int SCALES = KT * (G + GV) * 4;             // key and value scales
   static constexpr int STAT_OFF = SCALE_OFF + NB * SCALES;     // [sum, reference][128]
-  static constexpr int BAR_OFF = STAT_OFF + 2 * TILE * 4;
+  static constexpr int ODD_OFF = STAT_OFF + 2 * TILE * 4;      // [GV] first key whose value scale is no number
+  static constexpr int BAR_OFF = ODD_OFF + 16;
   static constexpr int CS = 16;                  // keys whose weights are stored at a time
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;
   static constexpr int SUB = DV / 2;             // channels that a warp writes, of 32 rows: in the ring
@@ -255,7 +257,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
     pos_of_lane[i] = there ? row_pos[it.row + lane + 32 * i] : -1;
   }
 
+  int* odd = reinterpret_cast<int*>(smem + L::ODD_OFF);
   if (tid == 0) {
+    for (int g = 0; g < GV; ++g) odd[g] = INT_MAX;
     for (int b = 0; b < NB; ++b) {
       mbar_init(&kv_full[b], DQ_WARPS / DQ_TEAMS + 1);
       mbar_init(&kv_free[b], 1);
@@ -389,7 +393,17 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
       if (!ok) break;
       float* sk = reinterpret_cast<float*>(smem + L::SCALE_OFF + b * L::SCALES);
       float* sv = sk + KT * G;
-      // slots behind the keys that are seen may never have been written: they get no scale
+      // Slots behind the keys that are seen may never have been written: they get no scale.  Nor do values
+      // whose scale is no number, or rows that do not see them would get 0 times it: those that do are
+      // given theirs at the end.
+#pragma unroll
+      for (int i = 0; i < VS; ++i) {
+        const int x = lane + 32 * i, key = x / GV;
+        if ((__half_as_ushort(vraw[i]) & 0x7c00u) == 0x7c00u) {
+          if (key < live) atomicMin(&odd[x % GV], (it.step_lo + s) * KT + key);
+          vraw[i] = __ushort_as_half(0);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         const int x = lane + 32 * i, key = x / G, g = x % G;
@@ -686,6 +700,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
                                          : make_float2(-INFINITY, 0.f);
     constexpr int SUB = L::SUB;
     const int d_lo = half * SUB;                 // this warp's channels, all of one group
+    const int first_odd = odd[GV == 2 ? half : 0];
+    const bool spoilt = first_odd != INT_MAX && row >= 0 && first_odd <= row_pos[row];
+    auto value = [&](uint32_t v) {
+      return !ok ? 0.f : spoilt ? __int_as_float(0x7fc00000) : __uint_as_float(v);
+    };
     unsigned char* slab = smem + L::KV_OFF + warp * (32 * SUB * 4);
     auto cell = [](int row, int chunk) {
       return row * (SUB * 4) + (chunk ^ (row & (SUB / 4 - 1))) * 16;
@@ -698,9 +717,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_kernel(
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
         *reinterpret_cast<float4*>(slab + cell(lane, (d0 + i) / 4)) =
-            ok ? make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
-                             __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]))
-               : make_float4(0.f, 0.f, 0.f, 0.f);
+            make_float4(value(o[i]), value(o[i + 1]), value(o[i + 2]), value(o[i + 3]));
     }
     __syncwarp();
     constexpr int CHUNKS = SUB / 4, ROWS = 32 / CHUNKS;          // rows that a warp writes at a time

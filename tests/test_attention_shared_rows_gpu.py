@@ -188,3 +188,25 @@ def test_a_first_row_that_ends_inside_the_prefix(dev, qh, kvh, d, first):
     plan = plan_of(args, spec, dev)
     plan.part_buffer[:-1] = float("nan")
     assert_near(args, F.attention_shared(*args, plan))
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(4, 2, 64), (8, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("key", [1, 40, 64, 200, 1023])
+@pytest.mark.parametrize("what", [float("inf"), float("nan")])
+def test_a_key_that_a_row_does_not_see_may_be_no_number(dev, qh, kvh, d, key, what):
+    """Shared keys that some rows of the group see and others end ahead of."""
+    from orinfer_b200.ops import functional as F
+    spec, args = batch(dev, [(1024, [key, 1030, max(1, key - 1), max(1, key // 2), 1024])], qh, kvh, d,
+                       seed=key)
+    req, table, ks, vs = args[2], args[4], args[7], args[8]
+    page = int(table[int(req[1]), key // 128])
+    clean = [t.clone() for t in (ks, vs)]
+    vs[page, key % 128] = what
+    plan = plan_of(args, spec, dev)
+    assert not bool(F.attention_shared(*args, plan)[1].isfinite().any())
+    ks[page, key % 128] = what
+    out = F.attention_shared(*args, plan)
+    ref, size, reach = R.attention_rows(*args[:7], *clean)
+    for r in (0, 2, 3):
+        off = (out[r].double() - ref[r]).abs() / near(ref[r], size[r], reach[r])
+        assert float(off.max()) <= 1 and bool(out[r].isfinite().all())
