@@ -198,10 +198,9 @@ class _Run:
                 first = r
         self.plan = None
         if groups:
-            longest = max(self.prompt_len[i] for i in live) + self.max_new
             self.plan = F.SharedPrefix(groups, len(live), qh=cfg.q_heads, kvh=cfg.kv_heads,
-                                       head_dim=cfg.head_dim, max_kv_len=longest,
-                                       device=pool.device, force=self.force)
+                                       head_dim=cfg.head_dim, device=pool.device, force=self.force,
+                                       max_kv_len=[self.prompt_len[i] + self.max_new for i in live])
         biases = [sorted(self.options[i].logit_bias.items()) for i in live]
         self.extra = {}
         if any(biases):

@@ -7,7 +7,7 @@ The matching fp32 PyTorch statement of each op lives in ``orinfer_b200.ref.ops_r
 
 from __future__ import annotations
 
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -241,12 +241,18 @@ class SharedPrefix:
     same pages as far as their first ``keys`` keys lie on them (whole pages, as ``fork_pages`` and
     the prefix cache share them).  Groups do not overlap; rows of no group share nothing.
     ``max_kv_len`` bounds the keys that any row sees while the plan is in use, so that one plan
-    serves the steps of a decode loop.  It holds the call's workspace: one stream at a time.  A batch
+    serves the steps of a decode loop; rows of unlike lengths are served better by a list with a bound
+    for each.  It holds the call's workspace: one stream at a time.  A batch
     whose shared keys are cheaper read again by every row is left to the row kernels, unless
     ``force``."""
 
     def __init__(self, groups: Sequence[Tuple[int, int, int]], rows: int, *, qh: int, kvh: int,
-                 head_dim: int, max_kv_len: int, device, force: bool = False):
+                 head_dim: int, max_kv_len: Union[int, Sequence[int]], device, force: bool = False):
+        bounds = None
+        if isinstance(max_kv_len, (list, tuple)):
+            bounds = [int(n) for n in max_kv_len]
+            _need(len(bounds) == rows and min(bounds, default=0) >= 0, "max_kv_len: one for each row")
+            max_kv_len = max(bounds, default=0)
         _need(rows >= 0 and max_kv_len >= 0, "rows and max_kv_len are not negative")
         _need(head_dim in (64, 128, 256), "heads of 64, 128 or 256 channels")
         rep = qh // kvh if kvh > 0 and qh % kvh == 0 else 0
@@ -270,24 +276,47 @@ class SharedPrefix:
         # (behind the parts the word by which the kernels of a call hand on what lies before them)
         self.part_buffer = (torch.zeros(self.parts * qh * (head_dim + 2) + 1, dtype=torch.float32,
                                         device=self.device) if items else None)
-        # The own keys, by the row kernels: as many as the middle row may have.  Beside a prefix they
-        # are split where they are long, and where a CTA has eight heads to join and there are few of
-        # them (the merge's have one; 16 / 2 heads of 256, 37 rows of 150 keys 34.4 us in one part,
-        # 30.7 in three, 100 rows 54 and 60; 32 / 8 of 128, 40 rows of 250 keys 29.1 and 37.0).  Without
-        # a prefix they are split where they are not short: a merge is a launch of its own (32 / 8
-        # heads of 128, 384 keys: two rows 6.0 us in one part and 5.5 in six, eight rows 6.1 and 7.4,
-        # and the launch takes the host 2.3).
-        shared = sorted(i[0] for i in info)
-        self.own_keys = max(1, max_kv_len - (shared[len(shared) // 2] if items else 0))
-        self.splits = attention_splits(self.own_keys, max(1, rows), kvh)
-        if items:
-            few = min(3, self.own_keys // 48, 2 * 148 // (rows * kvh)) if rep == 8 else 1
-            self.splits = max(1, few, min(self.splits, self.own_keys // 512))
-        elif self.own_keys <= 384 and head_dim <= 128:
-            self.splits = 1
+        self.own_keys, self.splits = self._own_parts([i[0] for i in info[:rows]], bounds, max_kv_len)
         self.scratch = f32(rows * qh * self.splits * (head_dim + 2)) if self.splits > 1 else None
         self._args = (ptr(self.items), len(items), ptr(self.info), ptr(self.part_buffer),
                       self.parts, self.splits, ptr(self.scratch), self.own_keys)
+
+    # The row kernels cut every row's own keys into as many parts.  Microseconds of 128 channels of a key
+    # in a part, of a CTA, of a record of 128 channels for the merge and of its launch; and what a wave
+    # behind the first counts beside a prefix, whose CTAs end one by one.  Over 720 batches of five
+    # geometries (1 to 128 rows of 16 to 5000 own keys, with and without a prefix, and with one long row
+    # among short ones) the number that this chooses takes 2 % more than the best of ten on average, 45 %
+    # at worst (4 rows of 1000 behind 8192).  32 / 8 heads of 128: one row of 16500 keys beside eight of
+    # 100 behind 16384 takes 174 us in one part and 61 in sixteen; without a prefix 64 rows of 1000 keys 38
+    # in one part and 56 in six, 16 rows of 2000 (three parts are a wave) 21 in three and 26 in four.
+    KEY_US, OWN_CTA_US, RECORD_US, MERGE_US, WAVE = 0.0135, 0.0056, 0.0015, 2.2, 0.4
+
+    def _own_parts(self, shared, bounds, max_kv_len):
+        """(own keys of the row that has the most, as far as that is known, parts of every row's)."""
+        rows, wide = max(1, self.rows), self.head_dim / 128
+        if bounds is not None:
+            own = [max(0, n - s) for n, s in zip(bounds, shared)]
+        else:
+            # One number for all: a row behind a shorter prefix, or none, may have as many keys (a long
+            # request) or be no longer than those behind the longest (or padding).  Taken between the two,
+            # a long row among short ones takes 16 % more than with the best number of parts (without the
+            # allowance 92 %), rows that all are short 13 % (with the whole of it 25 %).
+            near = max(1, max_kv_len - max(shared, default=0))
+            own = [near ** 0.4 * (max_kv_len - s) ** 0.6 for s in shared]
+        longest = max(1, round(max(own, default=1)))
+        if not self.parts:
+            from ..tuning import tables
+            if tables.attention_lookup(longest, rows, self.kvh) is not None:
+                return longest, attention_splits(longest, rows, self.kvh)
+        more = sum(own) / rows * (self.WAVE if self.parts else 1)
+        wave = 148 * (2 if self.head_dim > 128 else 3 if self.head_dim > 64 else 4)
+
+        def us(n):
+            waves = -(-rows * self.kvh * n // wave)
+            each = self.kvh * self.OWN_CTA_US + (n > 1) * self.qh * self.RECORD_US * wide
+            return ((longest + (waves - 1) * more) / n * self.KEY_US * wide + n * rows * each
+                    + (n > 1) * self.MERGE_US)
+        return longest, min(range(1, min(32, max(1, longest // 16)) + 1), key=us)
 
     # Microseconds of a step of keys, of a CTA besides its steps, of a megabyte of parts to be written
     # and read, and of a megabyte of keys and values that the row kernels would read again.  32 / 8

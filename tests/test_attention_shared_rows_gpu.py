@@ -210,3 +210,21 @@ def test_a_key_that_a_row_does_not_see_may_be_no_number(dev, qh, kvh, d, key, wh
     for r in (0, 2, 3):
         off = (out[r].double() - ref[r]).abs() / near(ref[r], size[r], reach[r])
         assert float(off.max()) <= 1 and bool(out[r].isfinite().all())
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(16, 8, 64), (32, 8, 128), (32, 4, 128), (16, 2, 256)])
+@pytest.mark.parametrize("listed", [True, False])
+def test_a_long_row_beside_short_ones(dev, qh, kvh, d, listed):
+    """In no group, and behind a shorter prefix; most parts of the short rows are empty then."""
+    from orinfer_b200.ops import functional as F
+    lens = [1024 + n for n in (1, 30, 60, 0, 90, 9)]
+    spec, args = batch(dev, [(1024, lens), (128, [4000, 140])], qh, kvh, d, seed=d, loners=(4100, 3, 0),
+                       gated=d == 256)
+    bounds = [n + 64 for n in lens] + [4064, 204, 4164, 64, 0]
+    plan = plan_of(args, spec, dev, max_kv_len=bounds if listed else 4164)
+    assert plan.splits > 1
+    out = F.attention_shared(*args, plan)
+    ref, size, reach = R.attention_rows(*args)
+    # (the sums of 4100 keys, 2^-23 for each of 257 additions of sixteen)
+    off = (out.double().view_as(ref) - ref).abs() / (near(ref, size, reach) + size * 182 * 2.0 ** -23)
+    assert float(off.max()) <= 1 and bool((out[-1] == 0).all())
