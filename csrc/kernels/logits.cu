@@ -401,18 +401,17 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) process_logits_kernel(const
   }
   if (!special) return;
 
-  // ---- scores of tokens that occur or have a bias, in 64 bits.  What is permitted has been copied, so
-  // that its logit is still there where out is the logits.
+  // ---- scores of tokens that occur or have a bias, in 64 bits and each operation rounded by itself, as
+  // on the host: a product that goes into a difference unrounded (which the compiler would do) leaves
+  // 1e-17 where the host has 0, and breaks a tie.  What is permitted has been copied, so that its logit
+  // is still there where out is the logits.
   auto write_score = [&](int id, unsigned word, unsigned permitted, float logit, double bias) {
     if (!permitted) return;
     const int times = word & (BIASED - 1u);
     double s = logit;
-    if (times > 0) {
-      s = s < 0.0 ? s * rep : s / rep;
-      s -= pres;
-    }
-    s -= freq * times;
-    if (word & BIASED) s += bias;
+    if (times > 0) s = __dsub_rn(s < 0.0 ? __dmul_rn(s, rep) : s / rep, pres);
+    s = __dsub_rn(s, __dmul_rn(freq, times));
+    if (word & BIASED) s = __dadd_rn(s, bias);
     const float f = static_cast<float>(s);
     out[id] = f;
     if (!isfinite(f)) atomicMax(a.flags + row, 2);
