@@ -1,7 +1,8 @@
 // Device top-k / top-p categorical sampler for rows whose options need no host state
 // (temperature > 0, 1 <= top_k <= 64, no penalties, bias, mask or probability report).
 // Scores of -1e30 and below (what process_logits leaves of tokens that a mask does not permit) are
-// no candidates: a row has at most as many as it has scores above that.
+// no candidates where a row has any above: it has at most as many then as it has of those.  (The others'
+// weights are 0 beside them, but they would be ties at the threshold, more than the shortlist holds.)
 // One CTA per row:
 //   1. exact radix select (4 passes of 8-bit histograms over order-preserving keys) of the
 //      top_k-th largest logit;
@@ -66,13 +67,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_topk_kernel(
     for (int i = tid; i < vocab; i += SAMPLE_THREADS) {
       const float v = lg[i];
       if (pass == 3 && !isfinite(v)) s_bad = 1;
-      candidates += v > NO_CANDIDATE;
+      if (pass == 3) candidates += v > NO_CANDIDATE;
       const uint32_t key = order_key(v);
       if ((key & mask) == prefix) atomicAdd(&hist[(key >> (8 * pass)) & 255u], 1u);
     }
     if (pass == 3 && candidates > 0) atomicAdd(&s_candidates, candidates);
     __syncthreads();
-    if (pass == 3) k = min(k, s_candidates);
+    if (pass == 3 && s_candidates > 0) k = min(k, s_candidates);
     if (tid == 0) {
       int need = pass == 3 ? k : s_need, d = 255;
       for (; d > 0; --d) {
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_topk_kernel(
   }
   __syncthreads();
   const int above = n_above, ties = n_tie;
-  if (s_bad || k == 0 || above + need_ties != k || ties > TIE_CAP) {
+  if (s_bad || above + need_ties != k || ties > TIE_CAP) {
     if (tid == 0) {
       flag[row] = 1;
       token[row] = -1;
