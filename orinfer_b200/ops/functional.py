@@ -453,14 +453,13 @@ class CachePages:
         return self._words[-1].data_ptr()
 
 
-def _tables(ins, out):
-    """The tensors that a page operator writes: ``out``, or new ones like its inputs (the table
-    first)."""
+def _tables(ins, out, where):
+    """The tensors that a page operator writes, all on GPU ``where``: ``out``, or new ones like its
+    inputs (the table first)."""
     table, i32 = ins[0], torch.int32
-    where = table.device
     for t in ins:
-        if t.dtype != i32 or not t.is_contiguous() or not t.is_cuda or t.device != where:
-            raise native.KernelError("table, lens, refs: contiguous int32, on one GPU")
+        if t.dtype != i32 or not t.is_contiguous() or t.device != where or not t.is_cuda:
+            raise native.KernelError("table, lens, refs: contiguous int32, on one GPU, the cache's")
     if table.dim() != 2 or table.numel() == 0:
         raise native.KernelError("table: [slots, pages of a slot]")
     if out is None:
@@ -468,16 +467,16 @@ def _tables(ins, out):
     _need(len(out) == len(ins), "out: a tensor for each input")
     for t, o in zip(ins, out):
         _need(o.shape == t.shape and o.dtype == i32 and o.is_contiguous() and o.device == where,
-              "out: tensors like the inputs")
+              "out: tensors like the inputs, on their GPU")
     return out
 
 
-def _slots(*lists):
+def _slots(*lists, where):
     n = lists[0].numel()
     for t in lists:
         if (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous()
-                or not t.is_cuda):
-            raise native.KernelError("lists of slots or pages: int32 [n], on a GPU")
+                or not t.is_cuda or t.device != where):
+            raise native.KernelError("lists of slots or pages: int32 [n], on the others' GPU")
     return n
 
 
@@ -485,7 +484,8 @@ def copy_pages(cache: CachePages, source: torch.Tensor, target: torch.Tensor,
                tokens: Optional[torch.Tensor] = None) -> None:
     """Copies pages ``source`` to ``target`` in every tensor of the cache, or their first
     ``tokens`` tokens (int32 [n] each).  No target is a source, and none is named twice."""
-    n = _slots(source, target) if tokens is None else _slots(source, target, tokens)
+    lists = (source, target) if tokens is None else (source, target, tokens)
+    n = _slots(*lists, where=cache.device)
     if tokens is None:
         tokens = torch.full_like(source, 128)
     copies = torch.stack((source, target, tokens), dim=1)
@@ -504,8 +504,8 @@ def fork_pages(cache: CachePages, table: torch.Tensor, lens: torch.Tensor, refs:
     inputs.  Status 1: not enough free pages, 2: a pair that cannot be (a slot that does not exist,
     a child that is not empty, named twice or a parent as well, a parent's page that nobody holds);
     nothing is changed then."""
-    n = _slots(parents, children)
-    t, l, r = _tables((table, lens, refs), out)
+    n = _slots(parents, children, where=cache.device)
+    t, l, r = _tables((table, lens, refs), out, cache.device)
     slots, width = table.shape
     if lens.dim() != 1 or lens.numel() != slots or refs.dim() != 1 or refs.numel() != cache.pages:
         raise native.KernelError("lens: [slots], refs: [pages]")
@@ -523,8 +523,8 @@ def free_pages(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, slot
     """Empties ``slots`` (int32 [n]; one named again is emptied once): every page of their rows
     loses a reference.  Returns (table, lens, refs); ``out`` may be the inputs.  A slot or page that
     does not exist, or a page that nobody holds, is left alone and reported by the status word."""
-    n = _slots(slots)
-    t, l, r = _tables((table, lens, refs), out)
+    n = _slots(slots, where=table.device)
+    t, l, r = _tables((table, lens, refs), out, table.device)
     total, width = table.shape
     pages = refs.numel()
     if lens.dim() != 1 or lens.numel() != total or refs.dim() != 1 or pages == 0:
@@ -540,7 +540,7 @@ def compact_pages(cache: CachePages, table: torch.Tensor, refs: torch.Tensor, *,
     """Moves the pages that are held to the front: with L of them, the k-th one above page L goes to
     the k-th free page of 1..L.  Returns (table, refs, moved): ``moved`` int32 [pages] says where
     each page has gone.  ``out`` (table, refs) may be the inputs."""
-    t, r = _tables((table, refs), out)
+    t, r = _tables((table, refs), out, cache.device)
     if refs.dim() != 1 or refs.numel() != cache.pages:
         raise native.KernelError("refs: [pages]")
     slots, width = table.shape
@@ -806,10 +806,12 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     finite (the host law refuses those rows), the mask does not exist or the row has more than 32768
     biases, else 0.  ``out`` may be ``logits``."""
     i32, f64 = torch.int32, torch.float64
-    for t in (logits, history, history_len, repetition, presence, frequency, bias_start, bias_ids,
+    _cuda(logits)
+    where = logits.device
+    for t in (history, history_len, repetition, presence, frequency, bias_start, bias_ids,
               bias_values, mask, mask_rows, out, flags):
-        if t is not None and not t.is_cuda:
-            raise native.KernelError("device op called with a CPU tensor")
+        if t is not None and t.device != where:
+            raise native.KernelError("every tensor on the GPU of the logits")
     if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
         raise native.KernelError("logits: fp32 [rows, vocab], rows in one piece")
     rows, vocab = logits.shape
