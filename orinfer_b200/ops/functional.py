@@ -318,11 +318,16 @@ class SharedPrefix:
                     + (n > 1) * self.MERGE_US)
         return longest, min(range(1, min(32, max(1, longest // 16)) + 1), key=us)
 
-    # Microseconds of a step of keys, of a CTA besides its steps, of a megabyte of parts to be written
-    # and read, and of a megabyte of keys and values that the row kernels would read again.  32 / 8
-    # heads of 128, 200 own keys, with the prefix shared and without: 2 rows behind 2048 keys 17 and
-    # 11 us, 16 rows 20 and 18, 32 rows 17 and 27, 64 rows 22 and 56, 64 behind 8192 34 and 185.
-    STEP_US, CTA_US, PART_US, AGAIN_US = 0.9, 5.0, 0.4, 0.16
+    # Microseconds of a step of keys (64, or 32 with 256 channels), of a CTA besides its steps, of a megabyte
+    # of parts to be written and read, and of a megabyte of keys and values that the row kernels would
+    # read again.  Over 1440 batches of eight geometries (2 to 128 rows in one group or four behind 128 to
+    # 16384 keys) what this chooses takes 0.5 % more than the better on average, 23 % at worst.  Up to 300
+    # own keys, with the prefix shared and without, 32 / 8 heads of 128: 2 rows behind 2048 keys 11.5 and
+    # 10.2 us, 8 rows 17.3 and 14.4, 32 rows 19.5 and 30.6, 64 rows 25.1 and 53.2, 64 behind 8192 38.4 and
+    # 142; 16 / 8 of 64: 16 rows behind 2048 13.8 and 12.6, 64 behind 8192 19.8 and 84; 16 / 2 of 256: 16
+    # rows 23.9 and 17.8, 64 behind 8192 48.8 and 125.
+    STEP_US = {64: 0.62, 128: 0.94, 256: 0.81}
+    CTA_US, PART_US, AGAIN_US = 4.9, 0.2, 0.167
 
     def _split(self, groups, force):
         """Which CTAs take which rows and keys: (items, (shared keys, first part, parts, 0) of every
@@ -355,7 +360,7 @@ class SharedPrefix:
                 mb = sum(p * u[1] for p, u in zip(parts, units)) * bytes_of
                 longest = max(-(-u[2] // p) for p, u in zip(parts, units))
                 took = -(-sum(parts) * columns // 148)
-                us = took * (longest * self.STEP_US + self.CTA_US) + mb * self.PART_US
+                us = took * (longest * self.STEP_US[self.head_dim] + self.CTA_US) + mb * self.PART_US
                 if best is None or us < best[0]:
                     best = us, parts
         again = sum((n - 1) * keys for _, n, keys in groups) * \
