@@ -122,8 +122,8 @@ __device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
 // came before: queries, positions, keys.  A thread that does not find it set waits for the kernel in
 // front itself.  When that has ended and the parts are joined, the word is cleared (attn_parts_are_there):
 // CTAs that start later wait, for nothing.  The next call's kernel in front, which waits for this one,
-// sets it again.  (125 rows under five prompts 46.6 us, with a wait at the start 50.7; 64 rows behind
-// 16384 keys 45.9 and 48.4, 37 gated rows 31.1 and 32.0.)
+// sets it again.  (125 rows under five prompts 48.5 us, with a wait at the start 52.9; 64 rows behind
+// 16384 keys 50.2 and 52.8, 37 gated rows 32.1 and 33.6.)
 __device__ __forceinline__ void attn_start_beside(const SharedParts& parts) {
   int ready;
   asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(ready) : "l"(parts.ready) : "memory");

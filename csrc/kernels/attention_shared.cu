@@ -20,13 +20,16 @@
 // (sixteen rows each), which go from step to step without a wait.  The weights replace the scores that
 // they are made of.  Two teams of dequantising warps take a step each in turn.
 //
-// 64 rows of 32 query heads behind 16384 keys of 4 KV heads of 128: 40 us, with the rows' own keys and the
-// join 49.5 (each row reading all keys 237); 5 us are the start and the end.  With one FP16 number to a
-// weight it is 35.5 and 45.9: a weight's second half is four instructions for two of them, of which two
-// are conversions at half a scheduler's rate, next to the exponentials at a quarter (with the weights
-// made behind all exponentials of a step 51.6, with shifts and masks for the remainders 50).
-// What bounds it is a step of 64 keys, 2300 cycles, in which nothing is at work for long: each role is a
-// chain in few warps, and they wait for one another.
+// 64 rows of 32 query heads behind 16384 keys of 4 KV heads of 128: 38.7 us, 445 TFLOP/s, with the rows' own
+// keys and the join 50.2 (each row reading all keys 237); 6.6 us of the 38.7 are the start and the end.
+// What bounds it is a step of 64 keys, 2170 cycles, in which nothing is at work for long: a scheduler
+// issues in 57 % of its cycles, the tensor pipe works for a third, conversions and logic for 42 %,
+// exponentials for 22 %, DRAM for 5 %.  Without the weights (exponentials, halves, stores) a step takes
+// 1560 cycles, without the dequantisation 1870, with neither 1230: each is a chain in few warps, and they
+// wait for one another.  The weights' second halves cost 3.6 us (without their arithmetic 46.6): two
+// conversions and two differences for each two weights.  (With those made behind all exponentials of a
+// step, the range looked after by the weights' sum, 51.6; with the first halves cut off, not rounded,
+// 0.6 less and two bits worse.)
 // Tried with one FP16 number to a weight (46 us): two tiles to a CTA, sixteen softmax warps that exchange
 // maxima and sums, raw tiles by bulk copies ahead of the dequantisation (each slower by 5 to 20 %);
 // scores read from TMEM ahead of the exponentials of the step before (50 to 53); all dequantising warps
