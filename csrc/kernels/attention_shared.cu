@@ -153,14 +153,8 @@ __device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&r)
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
       : "memory");
 }
-// The same rows and columns as pairs of FP16 values, half as many columns: per four columns lane (g,
+// The same rows and columns as pairs of BF16 values, half as many columns: per four columns lane (g,
 // t) holds column t of rows g and g + 8.
-__device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t (&r)[8]) { // 16 columns
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st_pairs(uint32_t taddr, const uint32_t (&r)[4]) { // 8 columns
   asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr),
                "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
