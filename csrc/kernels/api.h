@@ -188,6 +188,19 @@ int orinfer_attention(const __half* q, const __half* gate, const int* row_req, c
                       __half* out, int rows, int qh, int kvh, int head_dim, int splits,
                       float* scratch, int context, cudaStream_t stream);
 
+// The same, and sums[request][KV head][key] = weights[...] + the weight that every key got from the
+// call's rows (FP32, strides in elements, `capacity` keys of a request; sums may be weights).  keys: what
+// any row sees at most, which the scores' place is made for; scratch: 16-byte aligned.
+size_t orinfer_attention_weighed_scratch_bytes(int rows, int qh, int head_dim, int splits, int keys);
+int orinfer_attention_weighed(const __half* q, const __half* gate, const int* row_req,
+                              const int* row_pos, const int* page_table, int max_pages,
+                              const int8_t* kc, const int8_t* vc, const __half* ks,
+                              const __half* vs, __half* out, const float* weights,
+                              long long slot_stride, long long head_stride, float* sums,
+                              long long sums_slot_stride, long long sums_head_stride, int capacity,
+                              int rows, int qh, int kvh, int head_dim, int splits, int keys,
+                              float* scratch, int context, cudaStream_t stream);
+
 // Parts that the keys of a prefill tile are cut into (heads of 256 channels).
 int orinfer_attention_prefill_parts(int ctas, int max_pages);
 // Prefill chunks on tensor cores.  chunks: device int32 [n_chunks, 4] =
@@ -209,6 +222,16 @@ int orinfer_attention_shared(const __half* q, const __half* gate, const int* row
                              int head_dim, int num_pages, const int* items, int n_items,
                              const int* rows_info, float* parts, int n_parts, int splits,
                              float* scratch, int context, cudaStream_t stream);
+
+// Eviction from the cache (evict.cu).  bases: device int64 [4][layers], the addresses of the keys, values
+// (16-byte aligned) and their scales; weights, sums: FP32 [layers][slots][KV heads][capacity]; work: as
+// many words as the first says.  Outputs may be the inputs.
+size_t orinfer_evict_work_words(int slots, int n, int max_pages, int keep);
+int orinfer_evict_keys(const long long* bases, int layers, int kvh, int head_dim, int pages,
+                       const int* table, int* table_out, const int* lens, int* lens_out,
+                       const int* refs, int* refs_out, const int* list, int n, int slots,
+                       int max_pages, int keep, int first, int recent, const float* weights,
+                       float* sums, int capacity, int* work, int* status_out, cudaStream_t stream);
 
 // ---- expert-parallel all-to-alls over peer memory (moe_a2a.cu); cap = owned rows x top_k
 typedef struct OrinferA2aDispatch {

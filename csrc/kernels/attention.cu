@@ -88,6 +88,15 @@ struct RowScales {
 // scale shuffles, a permute and a subtraction per pair of INT8 values, the head and remainder, two
 // maxima per block) with under three warps per scheduler, which wait for fixed latencies and for
 // each other; for loads they wait a third of that (0.3 to 0.6 warps per issue).
+// What a call that also weighs the keys (attention_weighed) gets out of the row kernels: every score,
+// times log2 e, and every part's reference and sum of weights.  (Nothing else of a kernel changes, so
+// that its outputs have the bits of `attention`.)
+struct Weighed {
+  float* scores = nullptr;         // [rows][query heads][keys]
+  float2* ml = nullptr;            // [rows][query heads][splits]
+  int keys = 0;                    // a multiple of 4; what a row sees beyond is not written
+};
+
 template <int D>
 struct AttnTile {
   static constexpr int G = D / 64;                 // scale groups per row
@@ -186,7 +195,8 @@ __device__ __forceinline__ void attn_finish(const float (*s_o)[R][D], const floa
                                             const float (*s_l)[R], bool apart, bool idle, int rep,
                                             int row, int h, int qh, int split, int splits,
                                             const __half* gate, __half* out, float* scratch,
-                                            const SharedParts& parts = SharedParts()) {
+                                            const SharedParts& parts = SharedParts(),
+                                            float2* ml = nullptr) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 info = SHARED ? parts.rows[row] : make_int4(0, 0, 0, 0);
   if (SHARED && parts.pending) attn_parts_are_there(parts);
@@ -204,6 +214,7 @@ __device__ __forceinline__ void attn_finish(const float (*s_o)[R][D], const floa
         l = fmaf(s_l[w][r], f[w], l);
       }
     }
+    if (ml && lane == 0) ml[head * splits + split] = make_float2(m, l);
     if (SHARED && splits == 1) {
       float o[D / 32];
 #pragma unroll
@@ -246,13 +257,14 @@ __device__ __forceinline__ void attn_finish(const float (*s_o)[R][D], const floa
 // 120 keys 87 -> 62; 32 / 8, 128 rows of 64 keys 13.2 -> 12.3, but 64 rows (no second wave) 9.0 ->
 // 9.9; fewer than four KV heads leave warps idle (16 / 2 of 256, 512 rows of 60 keys 28 -> 30).
 // Longer rows of such a launch pay up to 3 % for the form (8 / 8 of 64, 128 rows of 640 keys).
-template <int D, bool WIDE, bool APART, bool SHARED = false>
+template <int D, bool WIDE, bool APART, bool SHARED = false, bool WEIGH = false>
 __global__ void __launch_bounds__(
     ATTN_WARPS * 32, D == 64 && !APART ? 3 : AttnTile<D>::MIN_CTAS) attn_rows_kernel(
     const __half* q, const __half* gate, const int* row_req, const int* row_pos,
     const int* page_table, int max_pages, const int8_t* kc, const int8_t* vc, const __half* ks,
     const __half* vs, __half* __restrict__ out, int qh, int kvh, int splits,
-    float* __restrict__ scratch, int rep, int apart_keys, const SharedParts parts) {
+    float* __restrict__ scratch, int rep, int apart_keys, const SharedParts parts,
+    const Weighed weighed) {
   constexpr int G = AttnTile<D>::G, KB = AttnTile<D>::KB;
   constexpr int NT = KB / 8, UT = KB / 16;         // 8-key score tiles, 16-key value tiles
   if (SHARED && parts.pending)
@@ -411,6 +423,19 @@ __global__ void __launch_bounds__(
           }
         }
     }
+    if (WEIGH && g < rep) {
+      float* to = weighed.scores + (static_cast<size_t>(row) * qh + h * rep + g) * weighed.keys;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int key = key0 + i * 8 + 2 * t;
+        if (key >= k_lo && key + 1 < min(k_hi, weighed.keys)) {
+          *reinterpret_cast<float2*>(to + key) = make_float2(s[i][0], s[i][1]);
+        } else {
+          if (key >= k_lo && key < min(k_hi, weighed.keys)) to[key] = s[i][0];
+          if (key + 1 >= k_lo && key + 1 < min(k_hi, weighed.keys)) to[key + 1] = s[i][1];
+        }
+      }
+    }
     // ---- softmax state
     float mb = s[0][0], vmax = 0.f;
 #pragma unroll
@@ -518,7 +543,7 @@ __global__ void __launch_bounds__(
     }
   }
   attn_finish<D, 8, SHARED>(s_o, s_m, s_l, apart, idle, rep, row, h, qh, split, splits, gate, out,
-                            scratch, parts);
+                            scratch, parts, WEIGH ? weighed.ml : nullptr);
 }
 
 // ---------------------------------------------------------------- digit form
@@ -615,13 +640,13 @@ __device__ __forceinline__ void load_pair(float (&v)[2 * G], const float* p) {
   }
 }
 
-template <int D, bool APART, bool SHARED = false>
+template <int D, bool APART, bool SHARED = false, bool WEIGH = false>
 __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_digits_kernel(
     const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
     const __half* q, const __half* gate, const int* row_req, const int* row_pos,
     const int* page_table, int max_pages, const __half* ks, const __half* vs,
     __half* __restrict__ out, int qh, int kvh, int splits, float* __restrict__ scratch, int rep,
-    int apart_keys, int* status, const SharedParts parts) {
+    int apart_keys, int* status, const SharedParts parts, const Weighed weighed) {
   using T = DigitTile<D>;
   constexpr int G = T::G, KB = T::KB, KSTEPS = T::KSTEPS;
   if (SHARED && parts.pending)
@@ -891,6 +916,21 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
           if (key < k_lo || key >= k_hi) s[m][x] = -INFINITY;
         }
     }
+    if (WEIGH && head < rep) {                     // (the halves of a warp have the same sums)
+      float* to = weighed.scores + (static_cast<size_t>(row) * qh + h * rep + head) * weighed.keys;
+      const int end = min(k_hi, weighed.keys);
+#pragma unroll
+      for (int x = 0; x < 4; x += 2) {
+        const int key = key0 + 16 * upper + T::key_of(t, x);      // an even key and the next one
+        const float2 two = upper ? make_float2(s[1][x], s[1][x + 1]) : make_float2(s[0][x], s[0][x + 1]);
+        if (key >= k_lo && key + 1 < end) {
+          *reinterpret_cast<float2*>(to + key) = two;
+        } else {
+          if (key >= k_lo && key < end) to[key] = two.x;
+          if (key + 1 >= k_lo && key + 1 < end) to[key + 1] = two.y;
+        }
+      }
+    }
     // ---- softmax state
     float mb = s[0][0];
 #pragma unroll
@@ -1057,7 +1097,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
     s_l[warp][head] = l_run;
   }
   attn_finish<D, 4, SHARED>(s_o, s_m, s_l, apart, idle, rep, row, h, qh, split, splits, gate, out,
-                            scratch, parts);
+                            scratch, parts, WEIGH ? weighed.ml : nullptr);
 }
 
 // One CTA per row and head.  The records' maxima and sums are read by a lane each and handed round,
@@ -1135,6 +1175,75 @@ __global__ void attn_merge_kernel(
   }
 }
 
+// ---------------------------------------------------------------- weights of the keys
+// sums[request][KV head][key] = weights[...] + the weights 2^(score - reference) / sum that the key got
+// from the row's query heads of that KV head, in the order of the heads; rows of one request (a
+// verification's) in the order of the rows, by the CTA of the first of them.  So no order of arrival
+// shows in the sums, and a row's output does not wait for them.
+//
+// A CTA takes WEIGH_KEYS keys of a row and KV head.  Scores are written once by the row kernels and read
+// once here, 4 rep bytes a key beside the 2 D and more of its key and value, mostly within L2.
+constexpr int WEIGH_THREADS = 256, WEIGH_KEYS = 4 * WEIGH_THREADS;
+__global__ void __launch_bounds__(WEIGH_THREADS) attn_weigh_kernel(
+    const Weighed weighed, const int* row_req, const int* row_pos, const float* weights,
+    long long slot_stride, long long head_stride, float* sums, long long sums_slot_stride,
+    long long sums_head_stride, int capacity, int rows, int qh, int rep, int splits, int* status) {
+  __shared__ unsigned s_same[WEIGH_THREADS / 32];
+  __shared__ float2 s_f[8];                        // a head's reference and 1 / sum
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  grid_wait();
+  grid_release();
+  const int row = blockIdx.x, h = blockIdx.y, key = blockIdx.z * WEIGH_KEYS + 4 * tid;
+  if (row_pos[row] < 0) return;
+  const int req = row_req[row];
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  int seen = 0;                                    // keys that some row of the request sees
+  for (int r0 = 0; r0 < rows; r0 += WEIGH_THREADS) {
+    const int mine = r0 + tid;
+    const bool same = mine < rows && row_req[mine] == req && row_pos[mine] >= 0;
+    const unsigned votes = __ballot_sync(0xffffffffu, same);
+    if (__syncthreads_or(same && mine < row)) return;             // an earlier row's CTA has it
+    if (lane == 0) s_same[warp] = votes;
+    __syncthreads();
+    for (int w = 0; w < WEIGH_THREADS / 32; ++w) {
+      for (unsigned left = s_same[w]; left != 0; left &= left - 1) {
+        const int r = r0 + 32 * w + __ffs(left) - 1;
+        const int n = min(min(row_pos[r] + 1, weighed.keys), capacity);
+        seen = max(seen, n);
+        if (static_cast<int>(blockIdx.z) * WEIGH_KEYS >= n) continue;
+        const size_t head0 = static_cast<size_t>(r) * qh + h * rep;
+        __syncthreads();                           // (the factors of the row before are used)
+        if (warp < rep) {
+          const float2* ml = weighed.ml + (head0 + warp) * splits;
+          const float2 own = lane < splits ? ml[lane] : make_float2(-INFINITY, 0.f);
+          const float m = warp_max(own.x);
+          const float l = warp_sum(own.x == -INFINITY ? 0.f : own.y * exp2f(own.x - m));
+          if (lane == 0) s_f[warp] = make_float2(m, l > 0.f ? 1.f / l : l == 0.f ? 0.f : l);
+        }
+        __syncthreads();
+        if (key >= n) continue;
+        for (int i = 0; i < rep; ++i) {
+          const float2 f = s_f[i];
+          const float* from = weighed.scores + (head0 + i) * weighed.keys + key;
+          const float4 v = *reinterpret_cast<const float4*>(from);
+          const float s[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (key + k < n) acc[k] = fmaf(exp2f(s[k] - f.x), f.y, acc[k]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (tid == 0 && blockIdx.z == 0 && row_pos[row] >= min(weighed.keys, capacity))
+    report_status(status, STATUS_BAD_INDEX, 0x60);
+  const float* from = weights + req * slot_stride + h * head_stride;
+  float* to = sums + req * sums_slot_stride + h * sums_head_stride;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (key + k < seen) to[key + k] = from[key + k] + acc[k];
+}
+
 // Whether a launch of the row kernel may start early.  Of 64 and 128 channels three and more CTAs
 // fit an SM, and a grid of more than one and little more than two per SM then gathers where the
 // kernel in front ends first, while other SMs get one CTA or none: 32 / 8 heads of 128, contexts of
@@ -1184,12 +1293,13 @@ static bool kv_map(CUtensorMap* map, const int8_t* cache, int kvh) {
          CUDA_SUCCESS;
 }
 
-template <int D, bool SHARED = false>
+template <int D, bool SHARED = false, bool WEIGH = false>
 static int launch_attn(const __half* q, const __half* gate, const int* row_req, const int* row_pos,
                        const int* page_table, int max_pages, const int8_t* kc, const int8_t* vc,
                        const __half* ks, const __half* vs, __half* out, int rows, int qh, int kvh,
                        int rep, int splits, float* scratch, int context, cudaStream_t stream,
-                       const SharedParts& parts = SharedParts()) {
+                       const SharedParts& parts = SharedParts(),
+                       const Weighed& weighed = Weighed()) {
   dim3 grid(rows, kvh, splits);
   const bool wide = ((reinterpret_cast<uintptr_t>(q) & 15) | (reinterpret_cast<uintptr_t>(ks) & 7) |
                      (reinterpret_cast<uintptr_t>(vs) & 7)) == 0;
@@ -1212,25 +1322,25 @@ static int launch_attn(const __half* q, const __half* gate, const int* row_req, 
   if (attn_digits(D, rep, pages, splits, wide, kc, vc) && kv_map<D>(&tk, kc, kvh) &&
       kv_map<D>(&tv, vc, kvh)) {
     constexpr int D_ = D == 256 ? 128 : D;         // (256 channels: never)
-    auto kernel = !SHARED && apart ? attn_digits_kernel<D_, !SHARED, SHARED>
-                                   : attn_digits_kernel<D_, false, SHARED>;
+    auto kernel = !SHARED && apart ? attn_digits_kernel<D_, !SHARED, SHARED, WEIGH>
+                                   : attn_digits_kernel<D_, false, SHARED, WEIGH>;
     static const int slot[2] = {runtime_new_slot(), runtime_new_slot()};
     constexpr int SMEM = DigitTile<D_>::SMEM;
     if (const int e = runtime_allow_smem(slot[apart], kernel, SMEM)) return e;
     start(kernel, SMEM, tk, tv, q, gate, row_req, row_pos, page_table, max_pages, ks, vs, out, qh,
-          kvh, splits, scratch, rep, apart_keys, runtime_status_ptr(), parts);
+          kvh, splits, scratch, rep, apart_keys, runtime_status_ptr(), parts, weighed);
   } else {
     auto kernel =
-        wide ? (apart ? attn_rows_kernel<D, true, !SHARED, SHARED>
-                      : attn_rows_kernel<D, true, false, SHARED>)
-             : (apart ? attn_rows_kernel<D, false, !SHARED, SHARED>
-                      : attn_rows_kernel<D, false, false, SHARED>);
+        wide ? (apart ? attn_rows_kernel<D, true, !SHARED, SHARED, WEIGH>
+                      : attn_rows_kernel<D, true, false, SHARED, WEIGH>)
+             : (apart ? attn_rows_kernel<D, false, !SHARED, SHARED, WEIGH>
+                      : attn_rows_kernel<D, false, false, SHARED, WEIGH>);
     static const int slot[4] = {runtime_new_slot(), runtime_new_slot(), runtime_new_slot(),
                                 runtime_new_slot()};
     constexpr int SMEM = AttnTile<D>::SMEM;
     if (const int e = runtime_allow_smem(slot[2 * apart + wide], kernel, SMEM)) return e;
     start(kernel, SMEM, q, gate, row_req, row_pos, page_table, max_pages, kc, vc, ks, vs, out, qh,
-          kvh, splits, scratch, rep, apart_keys, parts);
+          kvh, splits, scratch, rep, apart_keys, parts, weighed);
   }
   if (splits > 1)
     launch_early(attn_merge_kernel<D, SHARED>, dim3(rows, qh), D < 128 ? 64 : 128, 0, stream,
@@ -1292,4 +1402,50 @@ extern "C" int orinfer_attention(const __half* q, const __half* gate, const int*
   CASE(64) CASE(128) CASE(256)
 #undef CASE
   return -1;
+}
+
+// Floats of scores and parts of such a call (keys: what any row sees at most), behind them
+// orinfer_attention_scratch_bytes for splits > 1.
+static size_t weighed_floats(int rows, int qh, int splits, int keys) {
+  return static_cast<size_t>(rows) * qh * (keys + 2 * splits);
+}
+extern "C" size_t orinfer_attention_weighed_scratch_bytes(int rows, int qh, int head_dim, int splits,
+                                                          int keys) {
+  return weighed_floats(rows, qh, splits, (keys + 3) / 4 * 4) * sizeof(float) +
+         orinfer_attention_scratch_bytes(rows, qh, head_dim, splits);
+}
+
+extern "C" int orinfer_attention_weighed(
+    const __half* q, const __half* gate, const int* row_req, const int* row_pos,
+    const int* page_table, int max_pages, const int8_t* kc, const int8_t* vc, const __half* ks,
+    const __half* vs, __half* out, const float* weights, long long slot_stride,
+    long long head_stride, float* sums, long long sums_slot_stride, long long sums_head_stride,
+    int capacity, int rows, int qh, int kvh, int head_dim, int splits, int keys, float* scratch,
+    int context, cudaStream_t stream) {
+  if (rows <= 0) return 0;
+  if (splits < 1 || splits > 32 || keys < 1 || scratch == nullptr || kvh <= 0 || qh % kvh) return -1;
+  if (weights == nullptr || sums == nullptr || capacity < 0) return -1;
+  if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return -1;
+  const int rep = qh / kvh;
+  if (rep != 1 && rep != 2 && rep != 4 && rep != 8 && !(rep == 5 && head_dim == 128)) return -1;
+  Weighed w;
+  w.keys = (keys + 3) / 4 * 4;
+  const size_t heads = static_cast<size_t>(rows) * qh;
+  w.scores = scratch;
+  w.ml = reinterpret_cast<float2*>(scratch + heads * w.keys);
+  float* parts = scratch + weighed_floats(rows, qh, splits, w.keys);
+  int e = -1;
+#define CASE(DD)                                                                                  \
+  if (head_dim == DD)                                                                             \
+    e = launch_attn<DD, false, true>(q, gate, row_req, row_pos, page_table, max_pages, kc, vc, ks, \
+                                     vs, out, rows, qh, kvh, rep, splits, parts, context, stream, \
+                                     SharedParts(), w);
+  CASE(64) CASE(128) CASE(256)
+#undef CASE
+  if (e != 0) return e;
+  const dim3 grid(rows, kvh, (w.keys + WEIGH_KEYS - 1) / WEIGH_KEYS);
+  launch_early(attn_weigh_kernel, grid, WEIGH_THREADS, 0, stream, w, row_req, row_pos, weights,
+               slot_stride, head_stride, sums, sums_slot_stride, sums_head_stride, capacity, rows,
+               qh, rep, splits, runtime_status_ptr());
+  return static_cast<int>(cudaGetLastError());
 }

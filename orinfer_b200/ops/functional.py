@@ -208,6 +208,94 @@ def attention(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: torch.Tens
     return out
 
 
+def _current(where):
+    """Kernels go to a stream of the GPU that is current, with its status word and workspaces."""
+    if where.index != torch._C._cuda_getDevice():
+        raise native.KernelError(f"tensors on {where}, which is not the current device")
+
+
+def _weight_sums(weights, weights_out, lead, kvh, where):
+    """(capacity, strides of weights, the sums that are written and their strides)."""
+    out = weights if weights_out is None else weights_out
+    for t in (weights, out):
+        if (t.dtype != torch.float32 or t.dim() != 3 or t.shape[1] != kvh or t.device != where
+                or t.stride(2) != 1 or t.shape != weights.shape):
+            raise native.KernelError("weights: fp32 [slots, KV heads, keys] on the cache's GPU, keys in "
+                                     "one piece, weights_out like them")
+    _need(weights.shape[0] >= lead, "weights: a slot for each row of the page table")
+    return weights.shape[2], out
+
+
+def _cached(where, page_table, *tensors):
+    """Checks a cache's tensors [pages, 128, KV heads, channels or groups]; returns (pages, KV heads,
+    channels)."""
+    codes = [t for t in tensors if t.dtype == torch.int8]
+    scales = [t for t in tensors if t.dtype == torch.float16]
+    pages, tokens, kvh, d = codes[0].shape if codes and codes[0].dim() == 4 else (0, 0, 0, 0)
+    _need(tokens == 128 and d in (64, 128, 256) and len(codes) == len(scales) == len(tensors) // 2
+          and all(t.shape == (pages, 128, kvh, d) for t in codes)
+          and all(t.shape == (pages, 128, kvh, d // 64) for t in scales),
+          "a cache: int8 [pages, 128, KV heads, 64, 128 or 256] and fp16 scales, one per 64 channels")
+    for t in (page_table, *tensors):
+        if not t.is_contiguous() or t.device != where:
+            raise native.KernelError("page table and cache: contiguous, on the queries' GPU")
+    _need(page_table.dtype == torch.int32 and page_table.dim() == 2, "page_table: int32 [slots, pages]")
+    return pages, kvh, d
+
+
+def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: torch.Tensor,
+                      row_pos: torch.Tensor, page_table: torch.Tensor, kcache: torch.Tensor,
+                      vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor,
+                      weights: torch.Tensor, *, splits: int = 1,
+                      scratch: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                      rows: Optional[int] = None, max_kv_len: Optional[int] = None,
+                      weights_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`attention` (the same output, bit for bit) which also adds up what weight it gives:
+    ``weights`` fp32 [slots, KV heads, keys], slots as in the page table, gets for every key that a row
+    sees the softmax weights of the row's query heads of that KV head.  Rows of one request are added
+    in their order; what no row sees stays.  With ``weights_out`` the sums of seen keys go there
+    instead, so that a step may be taken back.  Rows see at most ``max_kv_len`` keys (by default as
+    many as the page table has), which the call's ``scratch`` is made for; keys beyond that, or beyond
+    what ``weights`` holds, get none and set the status word."""
+    _cuda(q, gate, row_req, row_pos, weights)
+    where = q.device
+    _need(q.dim() == 3 and q.dtype == torch.float16 and q.is_contiguous(), "q: fp16 [rows, heads, D]")
+    n, qh, d = q.shape
+    _, kvh, dim = _cached(where, page_table, kcache, vcache, kscale, vscale)
+    _need(d == dim and qh % kvh == 0, f"{qh} query heads of {d} on {kvh} KV heads of {dim} channels")
+    if gate is not None:
+        _need(gate.dtype == torch.float16 and gate.numel() == q.numel() and gate.is_contiguous()
+              and gate.device == where, "gate: fp16, as many as q has")
+    live = n if rows is None else rows
+    _need(0 <= live <= n, f"{live} rows of {n}")
+    for t in (row_req, row_pos):
+        _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] >= live and t.is_contiguous()
+              and t.device == where, "row_req, row_pos: int32, one for each row, on the queries' GPU")
+    capacity, sums = _weight_sums(weights, weights_out, page_table.shape[0], kvh, where)
+    _current(where)
+    width = page_table.shape[1] * 128
+    keys = width if max_kv_len is None else max(1, min(int(max_kv_len), width))
+    _need(1 <= splits <= 32 and keys > 0, "1 to 32 splits of some keys")
+    if out is None:
+        out = torch.empty(n, qh * d, dtype=torch.float16, device=where)
+    else:
+        _need(out.dtype == torch.float16 and out.is_contiguous() and out.numel() >= live * qh * d
+              and out.device == where, "out: fp16 [rows, heads * D]")
+    need = native.lib().orinfer_attention_weighed_scratch_bytes(live, qh, d, splits, keys)
+    if scratch is None:
+        scratch = torch.empty(need // 4, dtype=torch.float32, device=where)
+    else:
+        _need(scratch.numel() * scratch.element_size() >= need and scratch.is_contiguous()
+              and scratch.device == where, f"scratch: {need} bytes")
+    check(native.lib().orinfer_attention_weighed(
+        ptr(q), ptr(gate), ptr(row_req), ptr(row_pos), ptr(page_table), page_table.shape[1],
+        ptr(kcache), ptr(vcache), ptr(kscale), ptr(vscale), ptr(out), ptr(weights),
+        weights.stride(0), weights.stride(1), ptr(sums), sums.stride(0), sums.stride(1), capacity,
+        live, qh, kvh, d, splits, keys, ptr(scratch), max_kv_len or 0, stream()), "attention_weighed")
+    count_launches((3 if splits > 1 else 2) if live else 0)
+    return out
+
+
 def attention_prefill(q: torch.Tensor, gate: Optional[torch.Tensor], chunks: torch.Tensor,
                       max_q_len: int, page_table: torch.Tensor, kcache: torch.Tensor,
                       vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor, *,
@@ -556,6 +644,71 @@ def compact_pages(cache: CachePages, table: torch.Tensor, refs: torch.Tensor, *,
         "compact_pages")
     count_launches(2)
     return t, r, moved
+
+
+class KeyCache:
+    """The layers' paged caches as :func:`evict_keys` addresses them: ``k`` and ``v`` int8 [pages, 128, KV
+    heads, D] and their FP16 scales [pages, 128, KV heads, D / 64], a tensor for each layer.  It keeps
+    the tensors."""
+
+    def __init__(self, k: Sequence[torch.Tensor], v: Sequence[torch.Tensor],
+                 ks: Sequence[torch.Tensor], vs: Sequence[torch.Tensor]):
+        _need(len(k) > 0 and len(k) == len(v) == len(ks) == len(vs), "k, v, ks, vs of every layer")
+        self.tensors = [*k, *v, *ks, *vs]
+        _cuda(*self.tensors)
+        self.device, self.layers = k[0].device, len(k)
+        any_table = torch.empty(0, 0, dtype=torch.int32, device=self.device)
+        for layer in zip(k, v, ks, vs):
+            got = _cached(self.device, any_table, *layer)
+            _need(layer[0].dtype == layer[1].dtype == torch.int8 and got == (*k[0].shape[:1], *k[0].shape[2:])
+                  and layer[0].data_ptr() % 16 == layer[1].data_ptr() % 16 == 0,
+                  "layers alike, keys and values on 16-byte boundaries")
+        self.pages, _, self.kvh, self.head_dim = k[0].shape
+        self.bases = torch.tensor([t.data_ptr() for t in self.tensors], dtype=torch.int64,
+                                  device=self.device)
+
+
+def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor,
+               weights: torch.Tensor, slots: torch.Tensor, keep: int, *, first: int = 0,
+               recent: int = 0, out=None, weights_out: Optional[torch.Tensor] = None):
+    """Cuts every slot of ``slots`` (int32 [n]) that has more than ``keep`` tokens down to ``keep``: in
+    each layer and KV head the ``first`` and the last ``recent`` keys stay, and of those between the
+    ones with the largest ``weights`` (fp32 [layers, slots, KV heads, keys], equal ones the earlier
+    first, what is no number last), all in their order.  They move to free pages, the lowest first in the
+    order of the slots; the pages of the slots' rows lose a reference, so the free pages have to hold
+    the kept keys beside them.  ``table`` int32 [slots, pages], ``lens`` tokens per slot, ``refs``
+    references per page (page 0 is nobody's).
+
+    Returns (table, lens, refs, status int32 [1]); ``out`` may be the inputs.  The slots' rows of
+    ``weights`` move along, with zeros behind, in place or to ``weights_out``; those of slots that are
+    not cut stay (``weights_out`` gets a copy), and a slot that is named again is cut once.  Status 1: not
+    enough free pages, 2: a slot that does not exist, a length that its row does not hold or a page
+    that nobody holds; nothing is changed then."""
+    n = _slots(slots, where=cache.device)
+    t, l, r = _tables((table, lens, refs), out, cache.device)
+    total, width = table.shape
+    if lens.dim() != 1 or lens.numel() != total or refs.dim() != 1 or refs.numel() != cache.pages:
+        raise native.KernelError("lens: [slots], refs: [pages]")
+    sums = weights if weights_out is None else weights_out
+    for w in (weights, sums):
+        if (w.dtype != torch.float32 or w.shape[:3] != (cache.layers, total, cache.kvh) or w.dim() != 4
+                or not w.is_contiguous() or w.device != cache.device or w.shape != weights.shape):
+            raise native.KernelError("weights: contiguous fp32 [layers, slots, KV heads, keys] on the "
+                                     "cache's GPU, weights_out like them")
+    _need(weights.shape[3] >= width * 128, "weights: a place for each key of a table row")
+    _need(1 <= keep <= width * 128 and first >= 0 and recent >= 0 and first + recent <= keep,
+          f"{keep} keys of {width * 128} with {first} first and {recent} last ones")
+    _current(cache.device)
+    status = torch.empty(1, dtype=torch.int32, device=cache.device)
+    work = torch.empty(native.lib().orinfer_evict_work_words(total, n, width, keep),
+                       dtype=torch.int32, device=cache.device)
+    check(native.lib().orinfer_evict_keys(
+        cache.bases.data_ptr(), cache.layers, cache.kvh, cache.head_dim, cache.pages,
+        table.data_ptr(), t.data_ptr(), lens.data_ptr(), l.data_ptr(), refs.data_ptr(), r.data_ptr(),
+        slots.data_ptr(), n, total, width, keep, first, recent, weights.data_ptr(), sums.data_ptr(),
+        weights.shape[3], work.data_ptr(), status.data_ptr(), stream()), "evict_keys")
+    count_launches(2 if n or t is not table else 1)
+    return t, l, r, status
 
 
 def argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None,

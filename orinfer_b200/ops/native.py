@@ -55,6 +55,9 @@ def _load() -> ctypes.CDLL:
         "orinfer_qgemm": ([I, P, P, P, P, P, I, I, I, I, I, P], I),
         "orinfer_attention_scratch_bytes": ([I, I, I, I], c_size_t),
         "orinfer_attention": ([P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, P, I, P], I),
+        "orinfer_attention_weighed_scratch_bytes": ([I, I, I, I, I], c_size_t),
+        "orinfer_attention_weighed": ([P, P, P, P, P, I, P, P, P, P, P, P, c_longlong, c_longlong, P,
+                                       c_longlong, c_longlong, I, I, I, I, I, I, I, P, I, P], I),
         "orinfer_e8p_encode": ([P, P, c_longlong, P], I),
         "orinfer_router_topk": ([P, P, I, I, I, I, I, I, P, P, P, P], I),
         "orinfer_attention_starts_early": ([I, I, I, I], I),
@@ -92,6 +95,9 @@ def _load() -> ctypes.CDLL:
         "orinfer_copy_pages": ([P, P, P, I, I, P, P, I, P], I),
         "orinfer_fork_pages": ([P, P, P, I, I, P, P, P, P, P, P, P, P, I, I, I, P, P, P], I),
         "orinfer_free_pages": ([P, P, P, P, P, P, P, I, I, I, I, P], I),
+        "orinfer_evict_work_words": ([I, I, I, I], c_size_t),
+        "orinfer_evict_keys": ([P, I, I, I, I, P, P, P, P, P, P, P, I, I, I, I, I, I, P, P, I, P, P,
+                                P], I),
         "orinfer_compact_pages": ([P, P, P, I, I, P, P, P, P, P, I, I, P, P], I),
     }
     for name, (args, res) in sig.items():
