@@ -213,6 +213,18 @@ int orinfer_attention_prefill(const __half* q, const __half* gate, const int* ch
                               const __half* vscale, __half* out, int qh, int kvh, int head_dim,
                               int num_pages, int context, cudaStream_t stream);
 
+// The weight that the rows of such chunks give to every key (weigh.cu): sums[slot][KV head][key] =
+// weights[...] + it, FP32, strides in elements; sums may be weights.  limit: keys of a request at most; a
+// chunk beyond it, or of more than max_q_len rows, is left out and reported.  Queries, keys and work on
+// 16-byte boundaries.
+size_t orinfer_prefill_weights_work_bytes(int n_chunks, int max_q_len, int kvh, int rep, int limit);
+int orinfer_prefill_weights(const __half* q, const int* chunks, int n_chunks, int max_q_len,
+                            int total_rows, const int* page_table, int slots, int max_pages,
+                            const int8_t* kc, const __half* ks, int num_pages, const float* weights,
+                            long long slot_stride, long long head_stride, float* sums,
+                            long long sums_slot_stride, long long sums_head_stride, int limit, int qh,
+                            int kvh, int head_dim, float* work, cudaStream_t stream);
+
 // Single rows whose contexts begin with the same pages (attention_shared.cu).
 int orinfer_shared_step(int head_dim);
 int orinfer_attention_shared(const __half* q, const __half* gate, const int* row_req,

@@ -1,0 +1,1001 @@
+// The attention weight that the rows of prefill chunks give to every key of the paged INT8 cache:
+//   sums[slot][KV head][j] += sum over the chunk's rows i that see j, and the query heads h of the KV head,
+//                             of exp(q_ih . k_j / sqrt D - lse_ih).
+// A row's lse is known only behind all of its keys, and the sums run over rows, so the scores are
+// made twice, by two kernels on tcgen05 tensor cores, neither of which writes any:
+//   stats_kernel  S = Q K^T, a row per TMEM lane: maxima and sums of weights, one lse for each row;
+//   sums_kernel   S^T = K Q^T, a key per lane: a thread adds the weights of its key, no lane to lane sums.
+// The third adds what the parts of a key's sum have, in their order, to the sums so far.
+//
+// A query tile is 128 rows: P = 128 / rep positions of one request times the `rep` query heads that
+// share a KV head.  K is the exact FP16 integers that the cache holds; products of each group of 64
+// channels have an accumulator of their own and meet, times the key's group scales, in FP32, so
+// that a score is as exact as FP32 products give it.
+//
+// Work is counted in units, 128 rows by 128 keys (64 in stats_kernel with heads of 256 channels), in the
+// order (chunk, KV head, tile, step): row tiles walk their keys, key tiles the row tiles that see them.
+// Every CTA takes as many units, wherever a tile begins or ends, and leaves a part of each tile that it
+// had at place (tile + CTA) of a list, which is nobody else's; the tile's first and last CTA are noted.
+#include <cuda.h>
+
+#include "api.h"
+#include "common.cuh"
+#include "tma.h"
+
+namespace orinfer {
+namespace kw {
+
+constexpr int TILE = 128;                        // rows of a tile: positions x query heads; keys of a tile
+constexpr int MAX_CHUNKS = 512;
+constexpr int EP_WARPS = 8, DQ_WARPS = 4;        // softmax or sums; INT8 to FP16
+constexpr int MMA_WARP = EP_WARPS + DQ_WARPS, AUX_WARP = MMA_WARP + 1, TMA_WARP = AUX_WARP + 1;
+constexpr int THREADS = (TMA_WARP + 1) * 32;
+constexpr int CTAS = 148;
+constexpr int NS = 4;                            // places of scales, or of rows' lse
+constexpr float LEAD = 60.f;                     // of a score above the reference, in binades
+
+struct Chunk {            // of one request
+  int row_start;          // first packed row
+  int q_len;              // rows in the chunk
+  int pos0;               // absolute position of the first row
+  int slot;               // row of the page table
+};
+
+// What bounds a chunk, and how rows are packed.
+struct Geometry {
+  const Chunk* chunks;
+  const int* page_table;
+  int n_chunks, total_rows, slots, max_pages, num_pages;
+  int longest, limit;                            // rows of a chunk, keys of a request at most
+  int qh, kvh, rep, per;                         // per: positions of a row tile
+  __device__ Chunk at(int c) const {             // without rows where it is out of bounds
+    Chunk ch = chunks[c];
+    if (ch.q_len <= 0 || ch.q_len > longest || ch.q_len > limit || ch.row_start < 0 ||
+        ch.row_start > total_rows - ch.q_len || ch.pos0 < 0 || ch.pos0 > limit - ch.q_len ||
+        ch.slot < 0 || ch.slot >= slots)
+      ch.q_len = 0;
+    return ch;
+  }
+};
+
+// Tiles of a chunk and steps of a tile.  KT keys to a step of a row tile; 0: key tiles, a step is a row
+// tile, the last ones of the chunk.
+template <int KT>
+struct Order {
+  __device__ static int row_tiles(const Geometry& g, const Chunk& ch) {
+    return (ch.q_len + g.per - 1) / g.per;
+  }
+  __device__ static int tiles(const Geometry& g, const Chunk& ch) {
+    if (ch.q_len <= 0) return 0;
+    return KT ? row_tiles(g, ch) : (ch.pos0 + ch.q_len + TILE - 1) / TILE;
+  }
+  __device__ static int steps(const Geometry& g, const Chunk& ch, int tile) {
+    if (KT) return (ch.pos0 + min((tile + 1) * g.per, ch.q_len) + (KT ? KT : 1) - 1) / (KT ? KT : 1);
+    return row_tiles(g, ch) - max(tile * TILE - ch.pos0, 0) / g.per;
+  }
+};
+
+// Per chunk: units and tiles of a KV head.  Filled by the CTA together.
+struct Plan {
+  int units[MAX_CHUNKS], tiles[MAX_CHUNKS];
+};
+template <int KT>
+__device__ __forceinline__ void make_plan(Plan& plan, const Geometry& g, int* status) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int c = warp; c < g.n_chunks; c += THREADS / 32) {
+    const Chunk ch = g.at(c);
+    if (ch.q_len == 0 && blockIdx.x == 0 && lane == 0 && g.chunks[c].q_len != 0)
+      report_status(status, STATUS_BAD_INDEX, 0x70);
+    const int tiles = Order<KT>::tiles(g, ch);
+    int sum = 0;
+    for (int t = lane; t < tiles; t += 32) sum += Order<KT>::steps(g, ch, t);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) {
+      plan.units[c] = sum;
+      plan.tiles[c] = tiles;
+    }
+  }
+}
+
+// A CTA's walk over its units, tile by tile.  All warps have one, a warp together.
+template <int KT>
+struct Walk {
+  const Geometry& g;
+  const Plan& plan;
+  Chunk ch;
+  int c, h, tile, step, steps, left, index;      // index: of the tile, among all chunks' and heads'
+  __device__ Walk(const Geometry& geo, const Plan& p) : g(geo), plan(p) {
+    const int lane = threadIdx.x & 31;
+    int total = 0;
+    for (int i = lane; i < g.n_chunks; i += 32) total += plan.units[i];
+    total = __reduce_add_sync(0xffffffffu, total) * g.kvh;
+    const int share = (total + gridDim.x - 1) / gridDim.x;
+    int at = blockIdx.x * share;
+    left = max(min(total - at, share), 0);
+    if (left == 0) return;
+    index = 0;
+    for (c = 0;; ++c) {
+      const int here = plan.units[c] * g.kvh;
+      if (at < here) break;
+      at -= here;
+      index += plan.tiles[c] * g.kvh;
+    }
+    h = at / plan.units[c];
+    at -= h * plan.units[c];
+    index += h * plan.tiles[c];
+    ch = g.at(c);
+    for (int t0 = 0;; t0 += 32) {                // the tile in which it lies, 32 at a time
+      const int n = t0 + lane < plan.tiles[c] ? Order<KT>::steps(g, ch, t0 + lane) : 0;
+      int before = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+      }
+      const unsigned later = __ballot_sync(0xffffffffu, before > at);
+      if (later != 0) {
+        const int who = __ffs(later) - 1;
+        tile = t0 + who;
+        steps = __shfl_sync(0xffffffffu, n, who);
+        step = at - __shfl_sync(0xffffffffu, before, who) + steps;
+        break;
+      }
+      at -= __shfl_sync(0xffffffffu, before, 31);
+    }
+    index += tile;
+  }
+  __device__ int here() const { return min(steps - step, left); }        // units of this tile
+  __device__ void next_tile() {
+    left -= here();
+    if (left == 0) return;
+    step = 0;
+    ++index;
+    if (++tile == plan.tiles[c]) {
+      tile = 0;
+      if (++h == g.kvh) {
+        h = 0;
+        do ++c; while (plan.units[c] == 0);
+        ch = g.at(c);
+      }
+    }
+    steps = Order<KT>::steps(g, ch, tile);
+  }
+};
+// The same unit by unit, for roles that go ahead of the others.
+template <int KT>
+struct Units {
+  Walk<KT> w;
+  int i;                                         // of the tile's
+  __device__ Units(const Geometry& g, const Plan& p) : w(g, p), i(0) {}
+  __device__ bool more() const { return w.left > 0; }
+  __device__ int step() const { return w.step + i; }
+  __device__ void next() {
+    if (++i < w.here()) return;
+    i = 0;
+    w.next_tile();
+  }
+};
+
+template <int D>
+struct Shape {
+  static constexpr int G = D / 64;               // scale groups of a key
+  static constexpr int QSUB = TILE * 128;        // bytes of 64 channels of a query tile
+  static constexpr int Q_BYTES = G * QSUB;
+  // ---- stats_kernel
+  static constexpr int KT = D > 128 ? 64 : 128;  // keys of a step: at most 256 score columns
+  static constexpr int KSUB = KT * 128, K_BYTES = G * KSUB;
+  static constexpr int NQ = 2, NK = D > 128 ? 2 : 3;           // buffers of queries and of keys
+  static constexpr int A_K = NQ * Q_BYTES;
+  static constexpr int A_SCALE = A_K + NK * K_BYTES;
+  static constexpr int SCALES = KT * G * 4;
+  static constexpr int A_BAR = A_SCALE + NS * SCALES;
+  static constexpr int A_TOTAL = A_BAR + 256 + 1024;
+  // ---- sums_kernel
+  static constexpr int N = D > 128 ? 64 : 128;   // rows of a product: at most 256 score columns
+  static constexpr int PER = TILE / N;           // products of a unit and group
+  static constexpr int BQ = D > 128 ? 2 : 3, BK = D > 128 ? 1 : 2;
+  static constexpr int TSUB = TILE * 128, T_BYTES = G * TSUB;  // a tile of 128 keys
+  static constexpr int B_Q = BK * T_BYTES;
+  static constexpr int B_LSE = B_Q + BQ * Q_BYTES;
+  static constexpr int B_BAR = B_LSE + NS * TILE * 4;
+  static constexpr int B_TOTAL = B_BAR + 256 + 1024;
+  static_assert(A_TOTAL + sizeof(Plan) <= 227 * 1024 && B_TOTAL + sizeof(Plan) <= 227 * 1024,
+                "exceeds the shared memory of one CTA");
+};
+
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t tmem_d, uint64_t adesc,
+                                       uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+// Sixteen TMEM lanes, 32 columns, as fragments: per eight columns lane (g = lane / 4, t = lane % 4) holds
+// columns 2t and 2t + 1 of rows g and g + 8.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {   // a row per lane
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 pair_at(uint32_t a, uint32_t b) {
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+// Eight INT8 values -> eight FP16 values, exactly: 0x64xx is 1024 + xx, and 1152 is subtracted.
+__device__ __forceinline__ uint4 integers_fp16(uint32_t w0, uint32_t w1) {
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+  const uint32_t x0 = w0 ^ 0x80808080u, x1 = w1 ^ 0x80808080u;
+  uint32_t h[4] = {__byte_perm(x0, 0x64646464u, 0x4140), __byte_perm(x0, 0x64646464u, 0x4342),
+                   __byte_perm(x1, 0x64646464u, 0x4140), __byte_perm(x1, 0x64646464u, 0x4342)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h[i]), bias);
+    h[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(h[0], h[1], h[2], h[3]);
+}
+// Sixteen channels (unit c of a key's D / 16) into swizzled tiles of 64 channels, `sub` bytes each.
+// Lanes of every other group of channels store their second half first: eight lanes that store
+// together then meet on no bank.
+__device__ __forceinline__ void place(unsigned char* to, int sub, const uint4& raw, int key, int c) {
+  unsigned char* dst = to + (c / 4) * sub;
+  const bool swap = c & 4;
+  const uint4 lo = integers_fp16(swap ? raw.z : raw.x, swap ? raw.w : raw.y);
+  const uint4 hi = integers_fp16(swap ? raw.x : raw.z, swap ? raw.y : raw.w);
+  *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + swap)) = lo;
+  *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + !swap)) = hi;
+}
+
+// Page of a request's `key`; one that does not exist is reported, and page 0 is read instead.
+__device__ __forceinline__ int page_of(const Geometry& g, int slot, int key, int* status) {
+  const int page = g.page_table[static_cast<size_t>(slot) * g.max_pages + (key >> 7)];
+  if (page >= 0 && page < g.num_pages) return page;
+  report_status(status, STATUS_BAD_INDEX, 0x71);
+  return 0;
+}
+
+// The rows of the query tiles that no copy writes hold zeros: their scores are 0, not what was there.
+__device__ __forceinline__ void clear_tails(unsigned char* q, int tiles, int rows) {
+  const int tail = (TILE - rows) * 8;            // 16-byte units of 64 channels
+  for (int i = threadIdx.x; i < tiles * tail; i += THREADS)
+    *reinterpret_cast<uint4*>(q + i / tail * (TILE * 128) + rows * 128 + i % tail * 16) =
+        make_uint4(0, 0, 0, 0);
+  fence_proxy_async();
+}
+
+// lse: [row tiles + CTAs][128], log2 of a part's sum of weights; span: a row tile's first and last CTA.
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) stats_kernel(
+    const __grid_constant__ CUtensorMap tmap_q, const Geometry g, const int8_t* kc, const __half* ks,
+    float* lse, int* span, int* status) {
+  using L = Shape<D>;
+  constexpr int G = L::G, KT = L::KT, NQ = L::NQ, NK = L::NK;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ Plan plan;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::A_BAR);
+  uint64_t* q_full = bars;                       // [NQ] a tile's queries
+  uint64_t* q_free = q_full + NQ;                // [NQ] its last product is through
+  uint64_t* k_full = q_free + NQ;                // [NK] a unit's keys
+  uint64_t* k_free = k_full + NK;                // [NK] its product is through
+  uint64_t* s_full = k_free + NK;                // [2] its scores
+  uint64_t* s_free = s_full + 2;                 // [2] they have been read (an arrival per softmax warp)
+  uint64_t* c_full = s_free + 2;                 // [NS] its scales
+  uint64_t* c_free = c_full + NS;                // [NS] they have been used (the same)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_free + NS);
+  const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
+  if (tid == 0) {
+    for (int b = 0; b < NQ; ++b) {
+      mbar_init(&q_full[b], 1);
+      mbar_init(&q_free[b], 1);
+    }
+    for (int b = 0; b < NK; ++b) {
+      mbar_init(&k_full[b], DQ_WARPS);
+      mbar_init(&k_free[b], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&s_full[b], 1);
+      mbar_init(&s_free[b], EP_WARPS);
+    }
+    for (int b = 0; b < NS; ++b) {
+      mbar_init(&c_full[b], 1);
+      mbar_init(&c_free[b], EP_WARPS);
+    }
+    mbar_fence_init();
+    prefetch_tmap(&tmap_q);
+  }
+  if (g.per * g.rep < TILE) clear_tails(smem, NQ * G, g.per * g.rep);
+  grid_wait();
+  make_plan<KT>(plan, g, status);
+  if (warp == MMA_WARP) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = warp_same(*tmem_slot);
+  grid_release();
+  bool ok = true;
+
+  if (warp == TMA_WARP) {
+    Walk<KT> w(g, plan);
+    if (lane == 0) {
+      int n = 0;
+      for (; w.left > 0; w.next_tile(), ++n) {
+        const int b = n % NQ;
+        if (n >= NQ && !mbar_wait(&q_free[b], (n / NQ - 1) & 1, status, STATUS_TMA_WAIT, 0x10)) break;
+        mbar_expect_tx(&q_full[b], static_cast<uint32_t>(G) * 64 * 2 * g.rep * g.per);
+        for (int s = 0; s < G; ++s)
+          tma_load_3d(smem + b * L::Q_BYTES + s * L::QSUB, &tmap_q, &q_full[b], s * 64, w.h * g.rep,
+                      w.ch.row_start + w.tile * g.per);
+      }
+      for (int i = max(n - NQ, 0); i < n; ++i)     // our copies have landed before exit
+        mbar_wait(&q_full[i % NQ], (i / NQ) & 1, status, STATUS_TMA_WAIT, 0x11);
+    }
+  } else if (warp == MMA_WARP) {
+    constexpr uint32_t idesc = umma_idesc(1, 0, 0, 0, 0, TILE, KT);
+    const uint32_t leader = elect_one();
+    const uint64_t qd = umma_desc(smem_u32(smem), 16, 1024);
+    const uint64_t kd = umma_desc(smem_u32(smem + L::A_K), 16, 1024);
+    int n = 0, i = 0;
+    for (Walk<KT> w(g, plan); w.left > 0 && ok; w.next_tile(), ++n) {
+      const int last = i + w.here();
+      ok = warp_all(mbar_wait(&q_full[n % NQ], (n / NQ) & 1, status, STATUS_MMA_WAIT, 0x12));
+      const uint64_t qb = qd + static_cast<uint64_t>(n % NQ) * (L::Q_BYTES / 16);
+      for (; i < last && ok; ++i) {
+        const int b = i % NK, s = i & 1;
+        ok = warp_all(mbar_wait(&k_full[b], (i / NK) & 1, status, STATUS_MMA_WAIT, 0x13) &&
+                      (i < 2 || mbar_wait(&s_free[s], (i / 2 - 1) & 1, status, STATUS_MMA_WAIT, 0x14)));
+        tc_fence_after();
+        if (!ok) break;
+        const uint64_t kb = kd + static_cast<uint64_t>(b) * (L::K_BYTES / 16);
+#pragma unroll
+        for (int c = 0; c < G; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_ss(leader, tmem + 256 * s + c * KT, qb + (c * L::QSUB + k * 32) / 16,
+                   kb + (c * L::KSUB + k * 32) / 16, idesc, k != 0 ? 1u : 0u);
+        tc_commit_by(leader, &k_free[b]);
+        tc_commit_by(leader, &s_full[s]);
+      }
+      if (ok) tc_commit_by(leader, &q_free[n % NQ]);
+    }
+    __syncwarp();
+  } else if (warp == AUX_WARP) {
+    // ---------------- scales times log2 e / sqrt D, pairs of keys by groups
+    constexpr int KS = KT * G / 32;
+    const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
+    __half raw[KS];
+    Units<KT> load(g, plan);
+    auto fetch = [&] {
+      const size_t slot = static_cast<size_t>(page_of(g, load.w.ch.slot, load.step() * KT, status)) * 128 +
+                          (load.step() * KT & 127);
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const int x = lane + 32 * j;
+        raw[j] = ks[((slot + x / G) * g.kvh + load.w.h) * G + x % G];
+      }
+    };
+    if (load.more()) fetch();
+    for (int i = 0; load.more(); ++i) {
+      const int b = i % NS;
+      if (i >= NS) ok = mbar_wait(&c_free[b], (i / NS - 1) & 1, status, STATUS_DECODE_WAIT, 0x15);
+      ok = warp_all(ok);
+      if (!ok) break;
+      float* sk = reinterpret_cast<float*>(smem + L::A_SCALE + b * L::SCALES);
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const int x = lane + 32 * j, key = x / G, c = x % G;
+        sk[((key >> 1) * G + c) * 2 + (key & 1)] = __half2float(raw[j]) * qscale;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c_full[b]);
+      load.next();
+      if (load.more()) fetch();
+    }
+  } else if (warp >= EP_WARPS) {
+    // ---------------- keys: INT8 from global memory, a unit ahead in registers, to FP16 integers
+    constexpr int DQ = DQ_WARPS * 32, KI = KT * D / 16 / DQ;
+    const int u = tid - EP_WARPS * 32;
+    uint4 raw[KI];
+    Units<KT> load(g, plan);
+    auto fetch = [&] {
+      const size_t slot = static_cast<size_t>(page_of(g, load.w.ch.slot, load.step() * KT, status)) * 128 +
+                          (load.step() * KT & 127);
+#pragma unroll
+      for (int j = 0; j < KI; ++j) {
+        const int x = u + j * DQ, key = x / (D / 16), c = x % (D / 16);
+        raw[j] = *reinterpret_cast<const uint4*>(kc + ((slot + key) * g.kvh + load.w.h) * D + c * 16);
+      }
+    };
+    if (load.more()) fetch();
+    for (int i = 0; load.more(); ++i) {
+      const int b = i % NK;
+      if (i >= NK) ok = mbar_wait(&k_free[b], (i / NK - 1) & 1, status, STATUS_DECODE_WAIT, 0x16);
+      ok = warp_all(ok);
+      if (!ok) break;
+      unsigned char* buf = smem + L::A_K + b * L::K_BYTES;
+#pragma unroll
+      for (int j = 0; j < KI; ++j) {
+        const int x = u + j * DQ;
+        place(buf, L::KSUB, raw[j], x / (D / 16), x % (D / 16));
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[b]);
+      load.next();
+      if (load.more()) fetch();
+    }
+  } else {
+    // ---------------- sixteen rows per warp; a thread holds columns 2 qt and 2 qt + 1 of every eight, of
+    // rows qg and qg + 8
+    const int qg = lane >> 2, qt = lane & 3, row0 = (warp & 3) * 32 + (warp >> 2) * 16;
+    const uint32_t lane_addr = static_cast<uint32_t>(row0) << 16;
+    int i = 0;
+    for (Walk<KT> w(g, plan); w.left > 0 && ok; w.next_tile()) {
+      int sees[2];                               // keys that its rows see
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int p = w.tile * g.per + (row0 + qg + 8 * r) / g.rep;
+        sees[r] = (row0 + qg + 8 * r) < g.per * g.rep && p < w.ch.q_len ? w.ch.pos0 + p + 1 : 0;
+      }
+      const int all_see = __reduce_min_sync(0xffffffffu, min(sees[0], sees[1]));
+      float m_ref[2] = {0.f, 0.f};
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      const int n = w.here();
+      for (int j0 = 0; j0 < n; ++j0, ++i) {
+        const int sb = i & 1, cb = i % NS, key0 = (w.step + j0) * KT;
+        ok = mbar_wait(&s_full[sb], (i / 2) & 1, status, STATUS_EPILOGUE_WAIT, 0x17) &&
+             mbar_wait(&c_full[cb], (i / NS) & 1, status, STATUS_EPILOGUE_WAIT, 0x18);
+        ok = warp_all(ok);
+        if (!ok) break;
+        tc_fence_after();
+        const float* sk = reinterpret_cast<const float*>(smem + L::A_SCALE + cb * L::SCALES);
+#pragma unroll
+        for (int c0 = 0; c0 < KT; c0 += 32) {
+          uint32_t raw[G][16];
+#pragma unroll
+          for (int c = 0; c < G; ++c) tmem_ld_frag(tmem + 256 * sb + c * KT + c0 + lane_addr, raw[c]);
+          tc_wait_ld();
+          if (c0 + 32 == KT) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[sb]);
+          }
+          float2 x[2][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2* s = reinterpret_cast<const float2*>(sk) + (c0 / 2 + 4 * j + qt) * G;
+            float2 f[G];
+            if (G == 1) {
+              f[0] = s[0];
+            } else {
+#pragma unroll
+              for (int c = 0; c < G; c += 2) {
+                const float4 v = *reinterpret_cast<const float4*>(s + c);
+                f[c] = make_float2(v.x, v.y);
+                f[(c + 1) % G] = make_float2(v.z, v.w);
+              }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              x[r][j] = make_float2(-m_ref[r], -m_ref[r]);
+#pragma unroll
+              for (int c = 0; c < G; ++c)
+                x[r][j] = fma2(pair_at(raw[c][4 * j + 2 * r], raw[c][4 * j + 2 * r + 1]), f[c], x[r][j]);
+            }
+          }
+          if (all_see < key0 + c0 + 32) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int key = key0 + c0 + 8 * j + 2 * qt;
+                if (key >= sees[r]) x[r][j].x = -INFINITY;
+                if (key + 1 >= sees[r]) x[r][j].y = -INFINITY;
+              }
+          }
+          // The reference is the maximum of the first columns, and moves where a score is LEAD above it.
+          // (A row that sees none of the first sees none behind them.)
+          float top[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            top[r] = fmaxf(x[r][0].x, x[r][0].y);
+#pragma unroll
+            for (int j = 1; j < 4; ++j) top[r] = fmaxf(top[r], fmaxf(x[r][j].x, x[r][j].y));
+          }
+          const bool start = j0 == 0 && c0 == 0;
+          if (__any_sync(0xffffffffu, start || fmaxf(top[0], top[1]) > LEAD)) {
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], o));
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float by = top[r] == -INFINITY ? 0.f : start ? top[r] : fmaxf(top[r], 0.f);
+              const float f = start ? 0.f : ex2(-by);
+              sum[r] = mul2(sum[r], make_float2(f, f));
+              m_ref[r] += by;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[r][j] = add2(x[r][j], make_float2(-by, -by));
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float2 part = make_float2(0.f, 0.f);   // of these columns: short chains of sums
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              part = add2(part, make_float2(ex2(x[r][j].x), ex2(x[r][j].y)));
+            sum[r] = add2(sum[r], part);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c_free[cb]);
+      }
+      if (!ok) break;
+      const int place = w.index + blockIdx.x;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float l = sum[r].x + sum[r].y;
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (qt == 0)
+          lse[static_cast<size_t>(place) * TILE + row0 + qg + 8 * r] = m_ref[r] + log2f(l);
+      }
+      if (tid == 0) {
+        if (w.step == 0) span[2 * w.index] = blockIdx.x;
+        if (w.step + n == w.steps) span[2 * w.index + 1] = blockIdx.x;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
+}
+
+// parts: [key tiles + CTAs][2][128], sums over the lower and the upper rows of its units; span_out: a key
+// tile's first and last CTA.
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) sums_kernel(
+    const __grid_constant__ CUtensorMap tmap_q, const Geometry g, const int8_t* kc, const __half* ks,
+    const float* lse, const int* span, float* parts, int* span_out, int* status) {
+  using L = Shape<D>;
+  constexpr int G = L::G, N = L::N, PER = L::PER, BQ = L::BQ, BK = L::BK;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ Plan plan;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::B_BAR);
+  uint64_t* k_full = bars;                       // [BK] a tile's keys
+  uint64_t* k_free = k_full + BK;                // [BK] its last product is through
+  uint64_t* q_full = k_free + BK;                // [BQ] a unit's queries
+  uint64_t* q_free = q_full + BQ;                // [BQ] its products are through
+  uint64_t* s_full = q_free + BQ;                // [2] scores of a product
+  uint64_t* s_free = s_full + 2;                 // [2] they have been read (an arrival per warp)
+  uint64_t* l_full = s_free + 2;                 // [NS] a unit's lse
+  uint64_t* l_free = l_full + NS;                // [NS] they have been used (an arrival per warp)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(l_free + NS);
+  const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
+  if (tid == 0) {
+    for (int b = 0; b < BK; ++b) {
+      mbar_init(&k_full[b], DQ_WARPS);
+      mbar_init(&k_free[b], 1);
+    }
+    for (int b = 0; b < BQ; ++b) {
+      mbar_init(&q_full[b], 1);
+      mbar_init(&q_free[b], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&s_full[b], 1);
+      mbar_init(&s_free[b], EP_WARPS);
+    }
+    for (int b = 0; b < NS; ++b) {
+      mbar_init(&l_full[b], 1);
+      mbar_init(&l_free[b], EP_WARPS);
+    }
+    mbar_fence_init();
+    prefetch_tmap(&tmap_q);
+  }
+  if (g.per * g.rep < TILE) clear_tails(smem + L::B_Q, BQ * G, g.per * g.rep);
+  grid_wait();
+  make_plan<0>(plan, g, status);
+  if (warp == MMA_WARP) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = warp_same(*tmem_slot);
+  grid_release();
+  bool ok = true;
+  // row tile of a unit: the tile's steps are the last ones of the chunk
+  auto row_tile = [&](const Walk<0>& w, int step) {
+    return Order<0>::row_tiles(g, w.ch) - w.steps + step;
+  };
+
+  if (warp == TMA_WARP) {
+    Units<0> u(g, plan);
+    if (lane == 0) {
+      int n = 0;
+      for (; u.more(); u.next(), ++n) {
+        const int b = n % BQ;
+        if (n >= BQ && !mbar_wait(&q_free[b], (n / BQ - 1) & 1, status, STATUS_TMA_WAIT, 0x20)) break;
+        mbar_expect_tx(&q_full[b], static_cast<uint32_t>(G) * 64 * 2 * g.rep * g.per);
+        for (int s = 0; s < G; ++s)
+          tma_load_3d(smem + L::B_Q + b * L::Q_BYTES + s * L::QSUB, &tmap_q, &q_full[b], s * 64,
+                      u.w.h * g.rep, u.w.ch.row_start + row_tile(u.w, u.step()) * g.per);
+      }
+      for (int i = max(n - BQ, 0); i < n; ++i)     // our copies have landed before exit
+        mbar_wait(&q_full[i % BQ], (i / BQ) & 1, status, STATUS_TMA_WAIT, 0x21);
+    }
+  } else if (warp == MMA_WARP) {
+    constexpr uint32_t idesc = umma_idesc(1, 0, 0, 0, 0, TILE, N);
+    const uint32_t leader = elect_one();
+    const uint64_t kd = umma_desc(smem_u32(smem), 16, 1024);
+    const uint64_t qd = umma_desc(smem_u32(smem + L::B_Q), 16, 1024);
+    int n = 0, i = 0, x = 0;                       // tiles, units, products
+    for (Walk<0> w(g, plan); w.left > 0 && ok; w.next_tile(), ++n) {
+      const int last = i + w.here();
+      ok = warp_all(mbar_wait(&k_full[n % BK], (n / BK) & 1, status, STATUS_MMA_WAIT, 0x22));
+      const uint64_t kb = kd + static_cast<uint64_t>(n % BK) * (L::T_BYTES / 16);
+      for (; i < last && ok; ++i) {
+        const int b = i % BQ;
+        ok = warp_all(mbar_wait(&q_full[b], (i / BQ) & 1, status, STATUS_MMA_WAIT, 0x23));
+        for (int part = 0; part < PER && ok; ++part, ++x) {
+          const int s = x & 1;
+          if (x >= 2) ok = mbar_wait(&s_free[s], (x / 2 - 1) & 1, status, STATUS_MMA_WAIT, 0x24);
+          ok = warp_all(ok);
+          tc_fence_after();
+          if (!ok) break;
+          const uint64_t qb = qd + static_cast<uint64_t>(b) * (L::Q_BYTES / 16) + part * (N * 128 / 16);
+#pragma unroll
+          for (int c = 0; c < G; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_ss(leader, tmem + 256 * s + c * N, kb + (c * L::TSUB + k * 32) / 16,
+                     qb + (c * L::QSUB + k * 32) / 16, idesc, k != 0 ? 1u : 0u);
+          tc_commit_by(leader, &s_full[s]);
+        }
+        if (ok) tc_commit_by(leader, &q_free[b]);
+      }
+      if (ok) tc_commit_by(leader, &k_free[n % BK]);
+    }
+    __syncwarp();
+  } else if (warp == AUX_WARP) {
+    // ---------------- the rows' lse, of the parts that a tile's CTAs have left; four rows a lane.  A row
+    // that is none gets one that leaves no weight.
+    int base_c = 0, base = 0;                      // row tiles of the chunks before
+    int n = 0;
+    for (Units<0> u(g, plan); u.more(); u.next(), ++n) {
+      const int b = n % NS, rt = row_tile(u.w, u.step());
+      for (; base_c < u.w.c; ++base_c) {
+        const Chunk ch = g.at(base_c);
+        if (ch.q_len > 0) base += Order<0>::row_tiles(g, ch) * g.kvh;
+      }
+      const int index = base + u.w.h * Order<0>::row_tiles(g, u.w.ch) + rt;
+      const int lo = span[2 * index], hi = span[2 * index + 1];
+      auto part = [&](int x) {
+        return *reinterpret_cast<const float4*>(lse + static_cast<size_t>(index + x) * TILE + 4 * lane);
+      };
+      float4 v = part(lo);
+      if (hi > lo) {
+        float4 m = v, l = make_float4(1.f, 1.f, 1.f, 1.f);
+        auto join = [](float& m, float& l, float x) {
+          const float top = fmaxf(m, x);
+          l = (m == -INFINITY ? 0.f : l * exp2f(m - top)) + (x == -INFINITY ? 0.f : exp2f(x - top));
+          m = top;
+        };
+        for (int x = lo + 1; x <= hi; ++x) {
+          const float4 p = part(x);
+          join(m.x, l.x, p.x);
+          join(m.y, l.y, p.y);
+          join(m.z, l.z, p.z);
+          join(m.w, l.w, p.w);
+        }
+        v = make_float4(m.x + log2f(l.x), m.y + log2f(l.y), m.z + log2f(l.z), m.w + log2f(l.w));
+      }
+      const int rows = min(g.per, u.w.ch.q_len - rt * g.per) * g.rep;
+      v.x = 4 * lane < rows ? -v.x : -INFINITY;
+      v.y = 4 * lane + 1 < rows ? -v.y : -INFINITY;
+      v.z = 4 * lane + 2 < rows ? -v.z : -INFINITY;
+      v.w = 4 * lane + 3 < rows ? -v.w : -INFINITY;
+      if (n >= NS) ok = mbar_wait(&l_free[b], (n / NS - 1) & 1, status, STATUS_DECODE_WAIT, 0x25);
+      ok = warp_all(ok);
+      if (!ok) break;
+      *reinterpret_cast<float4*>(smem + L::B_LSE + b * TILE * 4 + lane * 16) = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&l_full[b]);
+    }
+  } else if (warp >= EP_WARPS) {
+    // ---------------- keys: a tile, INT8 to FP16 integers
+    constexpr int DQ = DQ_WARPS * 32, KI = TILE * D / 16 / DQ, AHEAD = KI < 8 ? KI : 8;
+    const int t = tid - EP_WARPS * 32;
+    int n = 0;
+    for (Walk<0> w(g, plan); w.left > 0; w.next_tile(), ++n) {
+      const int b = n % BK;
+      const size_t slot = static_cast<size_t>(page_of(g, w.ch.slot, w.tile * TILE, status)) * 128;
+      unsigned char* buf = smem + b * L::T_BYTES;
+#pragma unroll
+      for (int j0 = 0; j0 < KI; j0 += AHEAD) {
+        uint4 raw[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+          const int x = t + (j0 + j) * DQ, key = x / (D / 16), c = x % (D / 16);
+          raw[j] = *reinterpret_cast<const uint4*>(kc + ((slot + key) * g.kvh + w.h) * D + c * 16);
+        }
+        if (j0 == 0 && n >= BK)
+          ok = mbar_wait(&k_free[b], (n / BK - 1) & 1, status, STATUS_DECODE_WAIT, 0x26);
+        ok = warp_all(ok);
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+          const int x = t + (j0 + j) * DQ;
+          place(buf, L::TSUB, raw[j], x / (D / 16), x % (D / 16));
+        }
+      }
+      if (!ok) break;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[b]);
+    }
+  } else {
+    // ---------------- sums: a key per lane, half of a product's rows per warp
+    const int quad = warp & 3, half = warp >> 2, key_at = quad * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+    const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
+    constexpr int CB = G > 2 ? 16 : 32;            // columns read at a time
+    auto scales_of = [&](const Walk<0>& w, float (&f)[G]) {
+      const size_t slot =
+          static_cast<size_t>(page_of(g, w.ch.slot, w.tile * TILE, status)) * 128 + key_at;
+#pragma unroll
+      for (int c = 0; c < G; ++c) f[c] = __half2float(ks[(slot * g.kvh + w.h) * G + c]) * qscale;
+    };
+    Walk<0> w(g, plan), ahead(g, plan);            // the scales are asked for a tile ahead
+    float f_next[G];
+    if (ahead.left > 0) {
+      scales_of(ahead, f_next);
+      ahead.next_tile();
+    }
+    int i = 0, x = 0;
+    for (; w.left > 0 && ok; w.next_tile()) {
+      float f[G];
+#pragma unroll
+      for (int c = 0; c < G; ++c) f[c] = f_next[c];
+      if (ahead.left > 0) {
+        scales_of(ahead, f_next);
+        ahead.next_tile();
+      }
+      const int key = w.tile * TILE + key_at, n = w.here();
+      float2 total = make_float2(0.f, 0.f);
+      for (int j0 = 0; j0 < n && ok; ++j0, ++i) {
+        const int lb = i % NS, rt = row_tile(w, w.step + j0);
+        // columns whose rows see the key: those from `see` up to `rows`
+        const int see = (key - w.ch.pos0 - rt * g.per) * g.rep;
+        const int rows = min(g.per, w.ch.q_len - rt * g.per) * g.rep;
+        const bool edge = w.tile * TILE + TILE - 1 > w.ch.pos0 + rt * g.per || rows < g.per * g.rep;
+        const float* neg = reinterpret_cast<const float*>(smem + L::B_LSE + lb * TILE * 4);
+#pragma unroll
+        for (int part = 0; part < PER; ++part, ++x) {
+          const int sb = x & 1;
+          ok = mbar_wait(&s_full[sb], (x / 2) & 1, status, STATUS_EPILOGUE_WAIT, 0x27) &&
+               (part > 0 || mbar_wait(&l_full[lb], (i / NS) & 1, status, STATUS_EPILOGUE_WAIT, 0x28));
+          ok = warp_all(ok);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c0 = 0; c0 < N / 2; c0 += CB) {
+            const int col0 = half * (N / 2) + c0;
+            uint32_t raw[G][CB];
+#pragma unroll
+            for (int c = 0; c < G; ++c) {
+              const uint32_t from = tmem + 256 * sb + c * N + col0 + lane_addr;
+              if constexpr (CB == 32)
+                tmem_ld_32x32(from, raw[c]);
+              else
+                tmem_ld_x16(from, raw[c]);
+            }
+            tc_wait_ld();
+            if (c0 + CB == N / 2) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s_free[sb]);
+            }
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < CB; j += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(neg + part * N + col0 + j);
+              float2 y[2] = {make_float2(v.x, v.y), make_float2(v.z, v.w)};
+#pragma unroll
+              for (int p = 0; p < 2; ++p) {
+#pragma unroll
+                for (int c = 0; c < G; ++c)
+                  y[p] = fma2(pair_at(raw[c][j + 2 * p], raw[c][j + 2 * p + 1]), make_float2(f[c], f[c]),
+                              y[p]);
+                y[p] = make_float2(ex2(y[p].x), ex2(y[p].y));
+                if (edge) {
+                  const int col = part * N + col0 + j + 2 * p;
+                  if (col < see || col >= rows) y[p].x = 0.f;
+                  if (col + 1 < see || col + 1 >= rows) y[p].y = 0.f;
+                }
+                sum = add2(sum, y[p]);
+              }
+            }
+            total = add2(total, sum);
+          }
+        }
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(&l_free[lb]);
+      }
+      if (!ok) break;
+      parts[(static_cast<size_t>(w.index + blockIdx.x) * 2 + half) * TILE + key_at] = total.x + total.y;
+      if (tid == 0) {
+        if (w.step == 0) span_out[2 * w.index] = blockIdx.x;
+        if (w.step + n == w.steps) span_out[2 * w.index + 1] = blockIdx.x;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
+}
+
+// A CTA per key tile, KV head and chunk: chunks of one request are added in their order by the first's.
+__global__ void __launch_bounds__(TILE) add_kernel(
+    const Geometry g, const float* parts, const int* span, const float* weights, long long slot_stride,
+    long long head_stride, float* sums, long long sums_slot_stride, long long sums_head_stride) {
+  grid_wait();
+  grid_release();
+  const int c = blockIdx.z, h = blockIdx.y, tile = blockIdx.x, tid = threadIdx.x;
+  const Chunk ch = g.at(c);
+  if (ch.q_len <= 0) return;
+  float total = 0.f;
+  int base = 0, seen = 0;                          // key tiles of the chunks before; keys that are seen
+  for (int d = 0; d < g.n_chunks; ++d) {
+    const Chunk other = g.at(d);
+    const int tiles = Order<0>::tiles(g, other);
+    if (other.q_len > 0 && other.slot == ch.slot) {
+      if (d < c) return;
+      if (tile < tiles) {
+        const int index = base + h * tiles + tile;
+        const int lo = span[2 * index], hi = span[2 * index + 1];
+        float sum = 0.f;
+        for (int x = lo; x <= hi; ++x)
+          for (int half = 0; half < 2; ++half)
+            sum += parts[(static_cast<size_t>(index + x) * 2 + half) * TILE + tid];
+        total += sum;
+        seen = max(seen, other.pos0 + other.q_len);
+      }
+    }
+    base += tiles * g.kvh;
+  }
+  const int key = tile * TILE + tid;
+  if (key < seen)
+    sums[ch.slot * sums_slot_stride + h * sums_head_stride + key] =
+        weights[ch.slot * slot_stride + h * head_stride + key] + total;
+}
+
+// Tiles that a call may have at most, of rows and of keys, and its units.
+struct Bounds {
+  long long row_tiles, key_tiles, units;
+};
+static Bounds bounds(int n_chunks, int max_q_len, int kvh, int rep, int limit) {
+  const long long per = TILE / rep;
+  const long long rows = (max_q_len + per - 1) / per * n_chunks * kvh;
+  const long long keys = (limit + TILE - 1LL) / TILE;
+  return {rows, keys * n_chunks * kvh, rows * keys * 2};
+}
+
+static int ctas_for(long long units) { return units < CTAS ? static_cast<int>(units) : CTAS; }
+
+template <int D>
+static int launch(const __half* q, const Geometry& g, const int8_t* kc, const __half* ks,
+                  const float* weights, long long slot_stride, long long head_stride, float* sums,
+                  long long sums_slot_stride, long long sums_head_stride, float* work,
+                  cudaStream_t stream) {
+  using L = Shape<D>;
+  PFN_encodeTiled enc = runtime_tma_encoder();
+  if (!enc) return -3;
+  CUtensorMap tq;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(g.qh),
+                        static_cast<cuuint64_t>(g.total_rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(g.qh) * D * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(g.rep), static_cast<cuuint32_t>(g.per)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  if (enc(&tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(q), dims, strides, box, estr,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return -3;
+  static const int slot[2] = {runtime_new_slot(), runtime_new_slot()};
+  if (const int e = runtime_allow_smem(slot[0], stats_kernel<D>, L::A_TOTAL)) return e;
+  if (const int e = runtime_allow_smem(slot[1], sums_kernel<D>, L::B_TOTAL)) return e;
+  const Bounds b = bounds(g.n_chunks, g.longest, g.kvh, g.rep, g.limit);
+  float* lse = work;
+  float* parts = lse + (b.row_tiles + CTAS) * TILE;
+  int* row_span = reinterpret_cast<int*>(parts + (b.key_tiles + CTAS) * 2 * TILE);
+  int* key_span = row_span + 2 * b.row_tiles;
+  const int ctas = ctas_for(b.units);
+  launch_early(stats_kernel<D>, dim3(ctas), THREADS, L::A_TOTAL, stream, tq, g, kc, ks, lse, row_span,
+               runtime_status_ptr());
+  launch_early(sums_kernel<D>, dim3(ctas), THREADS, L::B_TOTAL, stream, tq, g, kc, ks,
+               static_cast<const float*>(lse), static_cast<const int*>(row_span), parts, key_span,
+               runtime_status_ptr());
+  launch_early(add_kernel, dim3((g.limit + TILE - 1) / TILE, g.kvh, g.n_chunks), TILE, 0, stream, g,
+               static_cast<const float*>(parts), static_cast<const int*>(key_span), weights, slot_stride,
+               head_stride, sums, sums_slot_stride, sums_head_stride);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace kw
+}  // namespace orinfer
+
+using namespace orinfer;
+
+extern "C" size_t orinfer_prefill_weights_work_bytes(int n_chunks, int max_q_len, int kvh, int rep,
+                                                     int limit) {
+  if (n_chunks <= 0 || rep <= 0) return 0;
+  const kw::Bounds b = kw::bounds(n_chunks, max_q_len, kvh, rep, limit);
+  return ((b.row_tiles + kw::CTAS) * kw::TILE + (b.key_tiles + kw::CTAS) * 2 * kw::TILE) * sizeof(float) +
+         2 * (b.row_tiles + b.key_tiles) * sizeof(int);
+}
+
+extern "C" int orinfer_prefill_weights(const __half* q, const int* chunks, int n_chunks, int max_q_len,
+                                       int total_rows, const int* page_table, int slots, int max_pages,
+                                       const int8_t* kc, const __half* ks, int num_pages,
+                                       const float* weights, long long slot_stride, long long head_stride,
+                                       float* sums, long long sums_slot_stride,
+                                       long long sums_head_stride, int limit, int qh, int kvh,
+                                       int head_dim, float* work, cudaStream_t stream) {
+  if (n_chunks <= 0 || max_q_len <= 0 || total_rows <= 0 || limit <= 0) return 0;
+  if (n_chunks > kw::MAX_CHUNKS || kvh <= 0 || qh % kvh || qh / kvh > 16 || !work) return -1;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kc) |
+        reinterpret_cast<uintptr_t>(work)) & 15) != 0)
+    return -1;
+  if (limit > max_pages * 128LL) return -1;
+  const kw::Bounds b = kw::bounds(n_chunks, max_q_len, kvh, qh / kvh, limit);
+  if (b.units > 0x3fffffffLL || b.key_tiles > 0x3fffffffLL) return -1;
+  if (runtime_ensure_init() != cudaSuccess) return -2;
+  kw::Geometry g;
+  g.chunks = reinterpret_cast<const kw::Chunk*>(chunks);
+  g.page_table = page_table;
+  g.n_chunks = n_chunks;
+  g.total_rows = total_rows;
+  g.slots = slots;
+  g.max_pages = max_pages;
+  g.num_pages = num_pages;
+  g.longest = max_q_len;
+  g.limit = limit;
+  g.qh = qh;
+  g.kvh = kvh;
+  g.rep = qh / kvh;
+  g.per = kw::TILE / g.rep;
+#define CASE(D)                                                                                     \
+  if (head_dim == D)                                                                                \
+    return kw::launch<D>(q, g, kc, ks, weights, slot_stride, head_stride, sums,          \
+                         sums_slot_stride, sums_head_stride, work, stream);
+  CASE(64) CASE(128) CASE(256)
+#undef CASE
+  return -1;
+}

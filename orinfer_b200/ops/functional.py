@@ -323,6 +323,50 @@ def attention_prefill(q: torch.Tensor, gate: Optional[torch.Tensor], chunks: tor
     return True
 
 
+def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
+                    page_table: torch.Tensor, kcache: torch.Tensor, kscale: torch.Tensor,
+                    weights: torch.Tensor, *, total_rows: Optional[int] = None,
+                    max_kv_len: Optional[int] = None,
+                    weights_out: Optional[torch.Tensor] = None) -> None:
+    """The attention weight that the rows of prefill chunks give to the keys, beside
+    :func:`attention_prefill` of the same chunks or on its own (the last rows of a prompt, say): a
+    chunk's entry names the rows that count.  ``weights`` fp32 [slots, KV heads, keys], slots as in
+    the page table, gets for every key that a row sees the softmax weights of the query heads of that
+    KV head, summed over the rows; chunks of one request are added in their order.  With
+    ``weights_out`` the sums of seen keys go there instead.  A chunk that reaches beyond
+    ``max_kv_len`` keys (by default as many as the page table and ``weights`` have), of more than
+    ``max_q_len`` rows or of rows that are not there is left out and sets the status word."""
+    _cuda(q, chunks, weights)
+    where = q.device
+    _need(q.dim() == 3 and q.dtype == torch.float16 and q.is_contiguous(), "q: fp16 [rows, heads, D]")
+    n, qh, d = q.shape
+    pages, kvh, dim = _cached(where, page_table, kcache, kscale)
+    _need(d == dim and qh % kvh == 0 and qh // kvh <= 16,
+          f"{qh} query heads of {d} on {kvh} KV heads of {dim} channels")
+    _need(q.data_ptr() % 16 == kcache.data_ptr() % 16 == 0, "q and kcache on 16-byte boundaries")
+    _need(chunks.dtype == torch.int32 and chunks.dim() == 2 and chunks.shape[1] == 4
+          and chunks.is_contiguous() and chunks.device == where, "chunks: int32 [C, 4], on the queries' GPU")
+    _need(chunks.shape[0] <= 512, "at most 512 chunks")
+    live = n if total_rows is None else total_rows
+    _need(0 <= live <= n and max_q_len >= 0, f"{live} rows of {n}, chunks of {max_q_len}")
+    capacity, sums = _weight_sums(weights, weights_out, page_table.shape[0], kvh, where)
+    _current(where)
+    limit = min(page_table.shape[1] * 128, capacity)
+    if max_kv_len is not None:
+        limit = min(limit, max_kv_len)
+    max_q_len = min(max_q_len, live)
+    if chunks.shape[0] == 0 or max_q_len == 0 or limit <= 0:
+        return
+    work = torch.empty(native.lib().orinfer_prefill_weights_work_bytes(
+        chunks.shape[0], max_q_len, kvh, qh // kvh, limit) // 4, dtype=torch.float32, device=where)
+    check(native.lib().orinfer_prefill_weights(
+        ptr(q), ptr(chunks), chunks.shape[0], max_q_len, live, ptr(page_table), page_table.shape[0],
+        page_table.shape[1], ptr(kcache), ptr(kscale), pages, ptr(weights), weights.stride(0),
+        weights.stride(1), ptr(sums), sums.stride(0), sums.stride(1), limit, qh, kvh, d, ptr(work),
+        stream()), "prefill_weights")
+    count_launches(3)
+
+
 class SharedPrefix:
     """Plan of a batch of single rows whose contexts share prefixes, for :func:`attention_shared`.
     ``groups``: (first row, rows, keys) each; the page-table rows of a group's rows begin with the

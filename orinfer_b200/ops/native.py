@@ -87,6 +87,9 @@ def _load() -> ctypes.CDLL:
         "orinfer_gdn_gated_norm": ([P, P, I, P, c_float, I, I, I, I, P, P], I),
         "orinfer_attention_prefill_parts": ([I, I], I),
         "orinfer_attention_prefill": ([P, P, P, I, I, I, P, I, P, P, P, P, P, I, I, I, I, I, P], I),
+        "orinfer_prefill_weights_work_bytes": ([I, I, I, I, I], c_size_t),
+        "orinfer_prefill_weights": ([P, P, I, I, I, P, I, I, P, P, I, P, c_longlong, c_longlong, P,
+                                     c_longlong, c_longlong, I, I, I, I, P, P], I),
         "orinfer_shared_step": ([I], I),
         "orinfer_attention_shared": ([P, P, P, P, P, I, I, P, P, P, P, P, I, I, I, I, I, P, I, P, P,
                                       I, I, P, I, P], I),
