@@ -27,12 +27,15 @@ namespace kw {
 
 constexpr int TILE = 128;                        // rows of a tile: positions x query heads; keys of a tile
 constexpr int MAX_CHUNKS = 512;
-constexpr int EP_WARPS = 8, DQ_WARPS = 4;        // softmax or sums; INT8 to FP16
-constexpr int MMA_WARP = EP_WARPS + DQ_WARPS, AUX_WARP = MMA_WARP + 1, TMA_WARP = AUX_WARP + 1;
-constexpr int THREADS = (TMA_WARP + 1) * 32;
+constexpr int EP_WARPS = 16;                     // softmax or sums
+constexpr int DQ_WARPS = 4, TEAMS = 2;           // INT8 to FP16: a team's warps, which take turns
+constexpr int AUX_WARPS = 2;                     // scales or rows' lse, in turn
+constexpr int AUX_WARP = EP_WARPS + TEAMS * DQ_WARPS, MMA_WARP = AUX_WARP + AUX_WARPS;
+constexpr int TMA_WARP = MMA_WARP + 1, THREADS = (TMA_WARP + 1) * 32;
 constexpr int CTAS = 148;
 constexpr int NS = 4;                            // places of scales, or of rows' lse
-constexpr float LEAD = 60.f;                     // of a score above the reference, in binades
+constexpr int ROW_PARTS = 2, KEY_PARTS = 4;      // warps that share a row's keys, or a key's rows
+constexpr float LEAD = 1.1529215046068470e18f;   // 2^60: weights under a reference that has to move
 
 struct Chunk {            // of one request
   int row_start;          // first packed row
@@ -40,6 +43,12 @@ struct Chunk {            // of one request
   int pos0;               // absolute position of the first row
   int slot;               // row of the page table
 };
+
+// First and last CTA of a tile.  (Where a kernel gave up waiting they are anything, and its status is set.)
+__device__ __forceinline__ int2 span_of(const int* span, int index) {
+  const int lo = span[2 * index], hi = span[2 * index + 1];
+  return make_int2(max(0, min(lo, CTAS - 1)), max(0, min(hi, CTAS - 1)));
+}
 
 // What bounds a chunk, and how rows are packed.
 struct Geometry {
@@ -174,6 +183,9 @@ struct Units {
     i = 0;
     w.next_tile();
   }
+  __device__ void skip(int n) {
+    for (; n > 0 && more(); --n) next();
+  }
 };
 
 template <int D>
@@ -189,7 +201,7 @@ struct Shape {
   static constexpr int A_SCALE = A_K + NK * K_BYTES;
   static constexpr int SCALES = KT * G * 4;
   static constexpr int A_BAR = A_SCALE + NS * SCALES;
-  static constexpr int A_TOTAL = A_BAR + 256 + 1024;
+  static constexpr int A_TOTAL = A_BAR + 512 + 1024;
   // ---- sums_kernel
   static constexpr int N = D > 128 ? 64 : 128;   // rows of a product: at most 256 score columns
   static constexpr int PER = TILE / N;           // products of a unit and group
@@ -197,8 +209,9 @@ struct Shape {
   static constexpr int TSUB = TILE * 128, T_BYTES = G * TSUB;  // a tile of 128 keys
   static constexpr int B_Q = BK * T_BYTES;
   static constexpr int B_LSE = B_Q + BQ * Q_BYTES;
-  static constexpr int B_BAR = B_LSE + NS * TILE * 4;
-  static constexpr int B_TOTAL = B_BAR + 256 + 1024;
+  static constexpr int B_SCALE = B_LSE + NS * TILE * 4;        // [NS][G][128]
+  static constexpr int B_BAR = B_SCALE + NS * G * TILE * 4;
+  static constexpr int B_TOTAL = B_BAR + 512 + 1024;
   static_assert(A_TOTAL + sizeof(Plan) <= 227 * 1024 && B_TOTAL + sizeof(Plan) <= 227 * 1024,
                 "exceeds the shared memory of one CTA");
 };
@@ -213,9 +226,9 @@ __device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t tmem_d, uint64_
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
-// Sixteen TMEM lanes, 32 columns, as fragments: per eight columns lane (g = lane / 4, t = lane % 4) holds
-// columns 2t and 2t + 1 of rows g and g + 8.
-__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
+// Sixteen TMEM lanes as fragments: per eight columns lane (g = lane / 4, t = lane % 4) holds columns 2t
+// and 2t + 1 of rows g and g + 8.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {       // 32 columns
   asm volatile(
       "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -225,13 +238,30 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) 
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {   // a row per lane
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[8]) {        // 16 columns
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+// 32 lanes, a row each
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[16]) {       // 16 columns
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&r)[8]) {        // 8 columns
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
       : "r"(taddr)
       : "memory");
 }
@@ -268,13 +298,26 @@ __device__ __forceinline__ void place(unsigned char* to, int sub, const uint4& r
   *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + !swap)) = hi;
 }
 
-// Page of a request's `key`; one that does not exist is reported, and page 0 is read instead.
-__device__ __forceinline__ int page_of(const Geometry& g, int slot, int key, int* status) {
-  const int page = g.page_table[static_cast<size_t>(slot) * g.max_pages + (key >> 7)];
+// A page that does not exist is reported, and page 0 is read instead.  (By the one who uses the number, a
+// step after it was asked for.)
+__device__ __forceinline__ int page_or_0(const Geometry& g, int page, int* status) {
   if (page >= 0 && page < g.num_pages) return page;
   report_status(status, STATUS_BAD_INDEX, 0x71);
   return 0;
 }
+// Where a role that goes ahead reads its next keys: their page, asked for a turn before, the first key's
+// place on it and the head.
+struct Ahead {
+  int page = 0, at = 0, h = 0;
+  __device__ void ask(const Geometry& g, const Chunk& ch, int key, int head) {
+    page = g.page_table[static_cast<size_t>(ch.slot) * g.max_pages + (key >> 7)];
+    at = key & 127;
+    h = head;
+  }
+  __device__ size_t cell(const Geometry& g, int* status) const {         // of the first key and its head
+    return (static_cast<size_t>(page_or_0(g, page, status)) * 128 + at) * g.kvh + h;
+  }
+};
 
 // The rows of the query tiles that no copy writes hold zeros: their scores are 0, not what was there.
 __device__ __forceinline__ void clear_tails(unsigned char* q, int tiles, int rows) {
@@ -285,7 +328,7 @@ __device__ __forceinline__ void clear_tails(unsigned char* q, int tiles, int row
   fence_proxy_async();
 }
 
-// lse: [row tiles + CTAs][128], log2 of a part's sum of weights; span: a row tile's first and last CTA.
+// lse: [row tiles + CTAs][2][128], log2 of a part's sum of weights; span: a row tile's first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     const __grid_constant__ CUtensorMap tmap_q, const Geometry g, const int8_t* kc, const __half* ks,
@@ -384,23 +427,31 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       if (ok) tc_commit_by(leader, &q_free[n % NQ]);
     }
     __syncwarp();
-  } else if (warp == AUX_WARP) {
+  } else if (warp >= AUX_WARP) {
     // ---------------- scales times log2 e / sqrt D, pairs of keys by groups
     constexpr int KS = KT * G / 32;
     const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
     __half raw[KS];
-    Units<KT> load(g, plan);
-    auto fetch = [&] {
-      const size_t slot = static_cast<size_t>(page_of(g, load.w.ch.slot, load.step() * KT, status)) * 128 +
-                          (load.step() * KT & 127);
+    Ahead next;
+    Units<KT> u(g, plan);
+    auto ask = [&] {
+      if (u.more()) next.ask(g, u.w.ch, u.step() * KT, u.w.h);
+    };
+    auto fetch = [&] {                             // what `next` names, and the page behind it
+      const size_t cell = next.cell(g, status);
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
         const int x = lane + 32 * j;
-        raw[j] = ks[((slot + x / G) * g.kvh + load.w.h) * G + x % G];
+        raw[j] = ks[(cell + static_cast<size_t>(x / G) * g.kvh) * G + x % G];
       }
+      u.skip(AUX_WARPS);
+      ask();
     };
-    if (load.more()) fetch();
-    for (int i = 0; load.more(); ++i) {
+    const int mine = warp - AUX_WARP, units = max(u.w.left, 0);
+    u.skip(mine);
+    ask();
+    if (mine < units) fetch();
+    for (int i = mine; i < units; i += AUX_WARPS) {
       const int b = i % NS;
       if (i >= NS) ok = mbar_wait(&c_free[b], (i / NS - 1) & 1, status, STATUS_DECODE_WAIT, 0x15);
       ok = warp_all(ok);
@@ -413,26 +464,34 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&c_full[b]);
-      load.next();
-      if (load.more()) fetch();
+      if (i + AUX_WARPS < units) fetch();
     }
   } else if (warp >= EP_WARPS) {
-    // ---------------- keys: INT8 from global memory, a unit ahead in registers, to FP16 integers
+    // ---------------- keys: INT8 from global memory, a unit of the team's ahead in registers, to FP16
+    // integers
     constexpr int DQ = DQ_WARPS * 32, KI = KT * D / 16 / DQ;
-    const int u = tid - EP_WARPS * 32;
+    const int t = (tid - EP_WARPS * 32) % DQ, team = warp_same((tid - EP_WARPS * 32) / DQ);
     uint4 raw[KI];
-    Units<KT> load(g, plan);
+    Ahead next;
+    Units<KT> u(g, plan);
+    auto ask = [&] {
+      if (u.more()) next.ask(g, u.w.ch, u.step() * KT, u.w.h);
+    };
     auto fetch = [&] {
-      const size_t slot = static_cast<size_t>(page_of(g, load.w.ch.slot, load.step() * KT, status)) * 128 +
-                          (load.step() * KT & 127);
+      const size_t cell = next.cell(g, status);
 #pragma unroll
       for (int j = 0; j < KI; ++j) {
-        const int x = u + j * DQ, key = x / (D / 16), c = x % (D / 16);
-        raw[j] = *reinterpret_cast<const uint4*>(kc + ((slot + key) * g.kvh + load.w.h) * D + c * 16);
+        const int x = t + j * DQ, key = x / (D / 16), c = x % (D / 16);
+        raw[j] = *reinterpret_cast<const uint4*>(kc + (cell + static_cast<size_t>(key) * g.kvh) * D + c * 16);
       }
+      u.skip(TEAMS);
+      ask();
     };
-    if (load.more()) fetch();
-    for (int i = 0; load.more(); ++i) {
+    const int units = max(u.w.left, 0);
+    u.skip(team);
+    ask();
+    if (team < units) fetch();
+    for (int i = team; i < units; i += TEAMS) {
       const int b = i % NK;
       if (i >= NK) ok = mbar_wait(&k_free[b], (i / NK - 1) & 1, status, STATUS_DECODE_WAIT, 0x16);
       ok = warp_all(ok);
@@ -440,19 +499,20 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       unsigned char* buf = smem + L::A_K + b * L::K_BYTES;
 #pragma unroll
       for (int j = 0; j < KI; ++j) {
-        const int x = u + j * DQ;
+        const int x = t + j * DQ;
         place(buf, L::KSUB, raw[j], x / (D / 16), x % (D / 16));
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[b]);
-      load.next();
-      if (load.more()) fetch();
+      if (i + TEAMS < units) fetch();
     }
   } else {
-    // ---------------- sixteen rows per warp; a thread holds columns 2 qt and 2 qt + 1 of every eight, of
-    // rows qg and qg + 8
-    const int qg = lane >> 2, qt = lane & 3, row0 = (warp & 3) * 32 + (warp >> 2) * 16;
+    // ---------------- sixteen rows by half of the step's keys per warp; a thread holds columns 2 qt and 2
+    // qt + 1 of every eight, of rows qg and qg + 8
+    const int qg = lane >> 2, qt = lane & 3, row0 = (warp & 3) * 32 + (warp >> 2 & 1) * 16;
+    constexpr int COLS = KT / ROW_PARTS, CH = G > 2 ? 16 : 32;   // of a warp, and at a time
+    const int part = warp >> 3;
     const uint32_t lane_addr = static_cast<uint32_t>(row0) << 16;
     int i = 0;
     for (Walk<KT> w(g, plan); w.left > 0 && ok; w.next_tile()) {
@@ -467,28 +527,30 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       const int n = w.here();
       for (int j0 = 0; j0 < n; ++j0, ++i) {
-        const int sb = i & 1, cb = i % NS, key0 = (w.step + j0) * KT;
+        const int sb = i & 1, cb = i % NS, key0 = (w.step + j0) * KT + part * COLS;
         ok = mbar_wait(&s_full[sb], (i / 2) & 1, status, STATUS_EPILOGUE_WAIT, 0x17) &&
              mbar_wait(&c_full[cb], (i / NS) & 1, status, STATUS_EPILOGUE_WAIT, 0x18);
         ok = warp_all(ok);
         if (!ok) break;
         tc_fence_after();
-        const float* sk = reinterpret_cast<const float*>(smem + L::A_SCALE + cb * L::SCALES);
+        const float2* sk = reinterpret_cast<const float2*>(smem + L::A_SCALE + cb * L::SCALES) +
+                           (part * COLS / 2 + qt) * G;
 #pragma unroll
-        for (int c0 = 0; c0 < KT; c0 += 32) {
-          uint32_t raw[G][16];
+        for (int c0 = 0; c0 < COLS; c0 += CH) {
+          uint32_t raw[G][CH / 2];
 #pragma unroll
-          for (int c = 0; c < G; ++c) tmem_ld_frag(tmem + 256 * sb + c * KT + c0 + lane_addr, raw[c]);
+          for (int c = 0; c < G; ++c)
+            tmem_ld_frag(tmem + 256 * sb + c * KT + part * COLS + c0 + lane_addr, raw[c]);
           tc_wait_ld();
-          if (c0 + 32 == KT) {
+          if (c0 + CH == COLS) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[sb]);
           }
-          float2 x[2][4];
+          float2 x[2][CH / 8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2* s = reinterpret_cast<const float2*>(sk) + (c0 / 2 + 4 * j + qt) * G;
+          for (int j = 0; j < CH / 8; ++j) {
+            const float2* s = sk + (c0 / 2 + 4 * j) * G;
             float2 f[G];
             if (G == 1) {
               f[0] = s[0];
@@ -508,62 +570,58 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
                 x[r][j] = fma2(pair_at(raw[c][4 * j + 2 * r], raw[c][4 * j + 2 * r + 1]), f[c], x[r][j]);
             }
           }
-          if (all_see < key0 + c0 + 32) {
+          if (all_see < key0 + c0 + CH) {
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
+              for (int j = 0; j < CH / 8; ++j) {
                 const int key = key0 + c0 + 8 * j + 2 * qt;
                 if (key >= sees[r]) x[r][j].x = -INFINITY;
                 if (key + 1 >= sees[r]) x[r][j].y = -INFINITY;
               }
           }
-          // The reference is the maximum of the first columns, and moves where a score is LEAD above it.
-          // (A row that sees none of the first sees none behind them.)
-          float top[2];
+          auto weights = [&](int r) {              // of these columns: short chains of sums
+            float2 v = make_float2(ex2(x[r][0].x), ex2(x[r][0].y));
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            top[r] = fmaxf(x[r][0].x, x[r][0].y);
-#pragma unroll
-            for (int j = 1; j < 4; ++j) top[r] = fmaxf(top[r], fmaxf(x[r][j].x, x[r][j].y));
-          }
+            for (int j = 1; j < CH / 8; ++j) v = add2(v, make_float2(ex2(x[r][j].x), ex2(x[r][j].y)));
+            return v;
+          };
+          float2 more[2] = {weights(0), weights(1)};
+          // The reference is the maximum of the first columns, and moves where weights are far above 1:
+          // no maximum is taken but then.  (A row that sees none of the first sees none behind them.)
           const bool start = j0 == 0 && c0 == 0;
-          if (__any_sync(0xffffffffu, start || fmaxf(top[0], top[1]) > LEAD)) {
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], o));
+          const float far = fmaxf(more[0].x + more[0].y, more[1].x + more[1].y);
+          if (__any_sync(0xffffffffu, start || far > LEAD)) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const float by = top[r] == -INFINITY ? 0.f : start ? top[r] : fmaxf(top[r], 0.f);
+              float top = fmaxf(x[r][0].x, x[r][0].y);
+#pragma unroll
+              for (int j = 1; j < CH / 8; ++j) top = fmaxf(top, fmaxf(x[r][j].x, x[r][j].y));
+#pragma unroll
+              for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+              const float by = top == -INFINITY ? 0.f : start ? top : fmaxf(top, 0.f);
               const float f = start ? 0.f : ex2(-by);
               sum[r] = mul2(sum[r], make_float2(f, f));
               m_ref[r] += by;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) x[r][j] = add2(x[r][j], make_float2(-by, -by));
+              for (int j = 0; j < CH / 8; ++j) x[r][j] = add2(x[r][j], make_float2(-by, -by));
+              more[r] = weights(r);
             }
           }
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float2 part = make_float2(0.f, 0.f);   // of these columns: short chains of sums
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              part = add2(part, make_float2(ex2(x[r][j].x), ex2(x[r][j].y)));
-            sum[r] = add2(sum[r], part);
-          }
+          for (int r = 0; r < 2; ++r) sum[r] = add2(sum[r], more[r]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&c_free[cb]);
       }
       if (!ok) break;
-      const int place = w.index + blockIdx.x;
+      const size_t place = static_cast<size_t>(w.index + blockIdx.x) * ROW_PARTS + part;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float l = sum[r].x + sum[r].y;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (qt == 0)
-          lse[static_cast<size_t>(place) * TILE + row0 + qg + 8 * r] = m_ref[r] + log2f(l);
+        if (qt == 0) lse[place * TILE + row0 + qg + 8 * r] = m_ref[r] + log2f(l);
       }
       if (tid == 0) {
         if (w.step == 0) span[2 * w.index] = blockIdx.x;
@@ -576,7 +634,7 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-// parts: [key tiles + CTAs][2][128], sums over the lower and the upper rows of its units; span_out: a key
+// parts: [key tiles + CTAs][4][128], sums over a quarter of the rows of its units each; span_out: a key
 // tile's first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
@@ -596,11 +654,13 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
   uint64_t* s_free = s_full + 2;                 // [2] they have been read (an arrival per warp)
   uint64_t* l_full = s_free + 2;                 // [NS] a unit's lse
   uint64_t* l_free = l_full + NS;                // [NS] they have been used (an arrival per warp)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(l_free + NS);
+  uint64_t* c_full = l_free + NS;                // [NS] a tile's scales
+  uint64_t* c_free = c_full + NS;                // [NS] they have been read (an arrival per warp)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_free + NS);
   const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
   if (tid == 0) {
     for (int b = 0; b < BK; ++b) {
-      mbar_init(&k_full[b], DQ_WARPS);
+      mbar_init(&k_full[b], TEAMS * DQ_WARPS / BK);
       mbar_init(&k_free[b], 1);
     }
     for (int b = 0; b < BQ; ++b) {
@@ -614,6 +674,8 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     for (int b = 0; b < NS; ++b) {
       mbar_init(&l_full[b], 1);
       mbar_init(&l_free[b], EP_WARPS);
+      mbar_init(&c_full[b], TEAMS * DQ_WARPS / BK);
+      mbar_init(&c_free[b], EP_WARPS);
     }
     mbar_fence_init();
     prefetch_tmap(&tmap_q);
@@ -684,44 +746,64 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       if (ok) tc_commit_by(leader, &k_free[n % BK]);
     }
     __syncwarp();
-  } else if (warp == AUX_WARP) {
+  } else if (warp >= AUX_WARP) {
     // ---------------- the rows' lse, of the parts that a tile's CTAs have left; four rows a lane.  A row
-    // that is none gets one that leaves no weight.
+    // that is none gets one that leaves no weight.  A unit's CTAs are asked for a turn before.
     int base_c = 0, base = 0;                      // row tiles of the chunks before
-    int n = 0;
-    for (Units<0> u(g, plan); u.more(); u.next(), ++n) {
-      const int b = n % NS, rt = row_tile(u.w, u.step());
+    Units<0> u(g, plan);
+    int index = 0, rows = 0, first = 0, last = 0;
+    auto ask = [&] {
+      if (!u.more()) return;
       for (; base_c < u.w.c; ++base_c) {
         const Chunk ch = g.at(base_c);
         if (ch.q_len > 0) base += Order<0>::row_tiles(g, ch) * g.kvh;
       }
-      const int index = base + u.w.h * Order<0>::row_tiles(g, u.w.ch) + rt;
-      const int lo = span[2 * index], hi = span[2 * index + 1];
-      auto part = [&](int x) {
-        return *reinterpret_cast<const float4*>(lse + static_cast<size_t>(index + x) * TILE + 4 * lane);
+      const int rt = row_tile(u.w, u.step());
+      index = base + u.w.h * Order<0>::row_tiles(g, u.w.ch) + rt;
+      rows = min(g.per, u.w.ch.q_len - rt * g.per) * g.rep;
+      first = span[2 * index];
+      last = span[2 * index + 1];
+    };
+    const int mine = warp - AUX_WARP, units = max(u.w.left, 0);
+    u.skip(mine);
+    ask();
+    for (int n = mine; n < units; n += AUX_WARPS) {
+      const int b = n % NS, live = rows;         // (see span_of)
+      const int lo = max(0, min(first, CTAS - 1)), hi = max(lo, min(last, CTAS - 1));
+      auto part = [&, at = index](int x) {
+        return *reinterpret_cast<const float4*>(lse + (static_cast<size_t>(at + lo) * ROW_PARTS + x) * TILE +
+                                                4 * lane);
       };
-      float4 v = part(lo);
-      if (hi > lo) {
-        float4 m = v, l = make_float4(1.f, 1.f, 1.f, 1.f);
-        auto join = [](float& m, float& l, float x) {
-          const float top = fmaxf(m, x);
-          l = (m == -INFINITY ? 0.f : l * exp2f(m - top)) + (x == -INFINITY ? 0.f : exp2f(x - top));
-          m = top;
-        };
-        for (int x = lo + 1; x <= hi; ++x) {
-          const float4 p = part(x);
-          join(m.x, l.x, p.x);
-          join(m.y, l.y, p.y);
-          join(m.z, l.z, p.z);
-          join(m.w, l.w, p.w);
+      float4 m = part(0), l = make_float4(1.f, 1.f, 1.f, 1.f);
+      auto join = [](float& m, float& l, float x) {
+        const float top = fmaxf(m, x);
+        l = (m == -INFINITY ? 0.f : l * exp2f(m - top)) + (x == -INFINITY ? 0.f : exp2f(x - top));
+        m = top;
+      };
+      constexpr int BATCH = 3;
+      for (int x = 1; x < (hi - lo + 1) * ROW_PARTS; x += BATCH) {
+        float4 p[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+          p[k] = x + k < (hi - lo + 1) * ROW_PARTS
+                     ? part(x + k) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (x == 1) {
+          u.skip(AUX_WARPS);
+          ask();
         }
-        v = make_float4(m.x + log2f(l.x), m.y + log2f(l.y), m.z + log2f(l.z), m.w + log2f(l.w));
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          join(m.x, l.x, p[k].x);
+          join(m.y, l.y, p[k].y);
+          join(m.z, l.z, p[k].z);
+          join(m.w, l.w, p[k].w);
+        }
       }
-      const int rows = min(g.per, u.w.ch.q_len - rt * g.per) * g.rep;
-      v.x = 4 * lane < rows ? -v.x : -INFINITY;
-      v.y = 4 * lane + 1 < rows ? -v.y : -INFINITY;
-      v.z = 4 * lane + 2 < rows ? -v.z : -INFINITY;
-      v.w = 4 * lane + 3 < rows ? -v.w : -INFINITY;
+      float4 v;
+      v.x = 4 * lane < live ? -m.x - log2f(l.x) : -INFINITY;
+      v.y = 4 * lane + 1 < live ? -m.y - log2f(l.y) : -INFINITY;
+      v.z = 4 * lane + 2 < live ? -m.z - log2f(l.z) : -INFINITY;
+      v.w = 4 * lane + 3 < live ? -m.w - log2f(l.w) : -INFINITY;
       if (n >= NS) ok = mbar_wait(&l_free[b], (n / NS - 1) & 1, status, STATUS_DECODE_WAIT, 0x25);
       ok = warp_all(ok);
       if (!ok) break;
@@ -730,67 +812,88 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       if (lane == 0) mbar_arrive(&l_full[b]);
     }
   } else if (warp >= EP_WARPS) {
-    // ---------------- keys: a tile, INT8 to FP16 integers
-    constexpr int DQ = DQ_WARPS * 32, KI = TILE * D / 16 / DQ, AHEAD = KI < 8 ? KI : 8;
-    const int t = tid - EP_WARPS * 32;
-    int n = 0;
-    for (Walk<0> w(g, plan); w.left > 0; w.next_tile(), ++n) {
-      const int b = n % BK;
-      const size_t slot = static_cast<size_t>(page_of(g, w.ch.slot, w.tile * TILE, status)) * 128;
+    // ---------------- keys: a tile, INT8 to FP16 integers, and their scales; the team's next tile in
+    // registers
+    // (a team per buffer: one that waits for a buffer two turns behind cannot tell the turns apart)
+    constexpr int DQ = TEAMS * DQ_WARPS * 32 / BK, KI = TILE * D / 16 / DQ;
+    static_assert(BK <= TEAMS, "a team per buffer");
+    const int t = (tid - EP_WARPS * 32) % DQ, team = warp_same((tid - EP_WARPS * 32) / DQ);
+    const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
+    uint4 raw[KI];
+    __half scale[G];
+    Ahead next;
+    Walk<0> w(g, plan);
+    auto ask = [&] {
+      if (w.left > 0) next.ask(g, w.ch, w.tile * TILE, w.h);
+    };
+    auto skip = [&](int n) {
+      for (; n > 0 && w.left > 0; --n) w.next_tile();
+    };
+    bool more;
+    auto fetch = [&] {                             // what `next` names, and the page behind it
+      more = w.left > 0;
+      if (!more) return;
+      const size_t cell = next.cell(g, status);
+#pragma unroll
+      for (int j = 0; j < KI; ++j) {
+        const int x = t + j * DQ, key = x / (D / 16), c = x % (D / 16);
+        raw[j] = *reinterpret_cast<const uint4*>(kc + (cell + static_cast<size_t>(key) * g.kvh) * D + c * 16);
+      }
+#pragma unroll
+      for (int c = 0; c < G; ++c) scale[c] = ks[(cell + static_cast<size_t>(t & (TILE - 1)) * g.kvh) * G + c];
+      skip(BK);
+      ask();
+    };
+    skip(team);
+    ask();
+    fetch();
+    for (int n = team; more; n += BK) {
+      const int b = n % BK, cb = n % NS;
+      if (n >= BK) ok = mbar_wait(&k_free[b], (n / BK - 1) & 1, status, STATUS_DECODE_WAIT, 0x26);
+      ok = warp_all(ok);
+      if (!ok) break;
       unsigned char* buf = smem + b * L::T_BYTES;
 #pragma unroll
-      for (int j0 = 0; j0 < KI; j0 += AHEAD) {
-        uint4 raw[AHEAD];
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-          const int x = t + (j0 + j) * DQ, key = x / (D / 16), c = x % (D / 16);
-          raw[j] = *reinterpret_cast<const uint4*>(kc + ((slot + key) * g.kvh + w.h) * D + c * 16);
-        }
-        if (j0 == 0 && n >= BK)
-          ok = mbar_wait(&k_free[b], (n / BK - 1) & 1, status, STATUS_DECODE_WAIT, 0x26);
-        ok = warp_all(ok);
-        if (!ok) break;
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-          const int x = t + (j0 + j) * DQ;
-          place(buf, L::TSUB, raw[j], x / (D / 16), x % (D / 16));
-        }
+      for (int j = 0; j < KI; ++j) {
+        const int x = t + j * DQ;
+        place(buf, L::TSUB, raw[j], x / (D / 16), x % (D / 16));
       }
-      if (!ok) break;
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[b]);
+      if (n >= NS) ok = mbar_wait(&c_free[cb], (n / NS - 1) & 1, status, STATUS_DECODE_WAIT, 0x29);
+      ok = warp_all(ok);
+      if (!ok) break;
+      float* sc = reinterpret_cast<float*>(smem + L::B_SCALE + cb * G * TILE * 4);
+#pragma unroll
+      for (int c = 0; c < G; ++c)
+        if (t < TILE) sc[c * TILE + t] = __half2float(scale[c]) * qscale;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c_full[cb]);
+      fetch();
     }
   } else {
-    // ---------------- sums: a key per lane, half of a product's rows per warp
-    const int quad = warp & 3, half = warp >> 2, key_at = quad * 32 + lane;
+    // ---------------- sums: a key per lane, a quarter of a product's rows per warp
+    const int quad = warp & 3, part = warp >> 2, key_at = quad * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
-    const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
-    constexpr int CB = G > 2 ? 16 : 32;            // columns read at a time
-    auto scales_of = [&](const Walk<0>& w, float (&f)[G]) {
-      const size_t slot =
-          static_cast<size_t>(page_of(g, w.ch.slot, w.tile * TILE, status)) * 128 + key_at;
+    constexpr int COLS = N / KEY_PARTS, CB = G > 2 ? 8 : 16;     // of a warp, and at a time
+    int i = 0, x = 0, n = 0;                       // units, products, tiles
+    for (Walk<0> w(g, plan); w.left > 0 && ok; w.next_tile(), ++n) {
+      const int cb = n % NS, here = w.here();
+      ok = mbar_wait(&c_full[cb], (n / NS) & 1, status, STATUS_EPILOGUE_WAIT, 0x2a);
+      ok = warp_all(ok);
+      if (!ok) break;
+      float2 f[G];
 #pragma unroll
-      for (int c = 0; c < G; ++c) f[c] = __half2float(ks[(slot * g.kvh + w.h) * G + c]) * qscale;
-    };
-    Walk<0> w(g, plan), ahead(g, plan);            // the scales are asked for a tile ahead
-    float f_next[G];
-    if (ahead.left > 0) {
-      scales_of(ahead, f_next);
-      ahead.next_tile();
-    }
-    int i = 0, x = 0;
-    for (; w.left > 0 && ok; w.next_tile()) {
-      float f[G];
-#pragma unroll
-      for (int c = 0; c < G; ++c) f[c] = f_next[c];
-      if (ahead.left > 0) {
-        scales_of(ahead, f_next);
-        ahead.next_tile();
+      for (int c = 0; c < G; ++c) {
+        const float v = *reinterpret_cast<const float*>(smem + L::B_SCALE + ((cb * G + c) * TILE + key_at) * 4);
+        f[c] = make_float2(v, v);
       }
-      const int key = w.tile * TILE + key_at, n = w.here();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c_free[cb]);
+      const int key = w.tile * TILE + key_at;
       float2 total = make_float2(0.f, 0.f);
-      for (int j0 = 0; j0 < n && ok; ++j0, ++i) {
+      for (int j0 = 0; j0 < here && ok; ++j0, ++i) {
         const int lb = i % NS, rt = row_tile(w, w.step + j0);
         // columns whose rows see the key: those from `see` up to `rows`
         const int see = (key - w.ch.pos0 - rt * g.per) * g.rep;
@@ -798,27 +901,21 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
         const bool edge = w.tile * TILE + TILE - 1 > w.ch.pos0 + rt * g.per || rows < g.per * g.rep;
         const float* neg = reinterpret_cast<const float*>(smem + L::B_LSE + lb * TILE * 4);
 #pragma unroll
-        for (int part = 0; part < PER; ++part, ++x) {
+        for (int p0 = 0; p0 < PER; ++p0, ++x) {
           const int sb = x & 1;
           ok = mbar_wait(&s_full[sb], (x / 2) & 1, status, STATUS_EPILOGUE_WAIT, 0x27) &&
-               (part > 0 || mbar_wait(&l_full[lb], (i / NS) & 1, status, STATUS_EPILOGUE_WAIT, 0x28));
+               (p0 > 0 || mbar_wait(&l_full[lb], (i / NS) & 1, status, STATUS_EPILOGUE_WAIT, 0x28));
           ok = warp_all(ok);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int c0 = 0; c0 < N / 2; c0 += CB) {
-            const int col0 = half * (N / 2) + c0;
+          for (int c0 = 0; c0 < COLS; c0 += CB) {
+            const int col0 = part * COLS + c0;
             uint32_t raw[G][CB];
 #pragma unroll
-            for (int c = 0; c < G; ++c) {
-              const uint32_t from = tmem + 256 * sb + c * N + col0 + lane_addr;
-              if constexpr (CB == 32)
-                tmem_ld_32x32(from, raw[c]);
-              else
-                tmem_ld_x16(from, raw[c]);
-            }
+            for (int c = 0; c < G; ++c) tmem_ld_rows(tmem + 256 * sb + c * N + col0 + lane_addr, raw[c]);
             tc_wait_ld();
-            if (c0 + CB == N / 2) {
+            if (c0 + CB == COLS) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&s_free[sb]);
@@ -826,17 +923,16 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < CB; j += 4) {
-              const float4 v = *reinterpret_cast<const float4*>(neg + part * N + col0 + j);
+              const float4 v = *reinterpret_cast<const float4*>(neg + p0 * N + col0 + j);
               float2 y[2] = {make_float2(v.x, v.y), make_float2(v.z, v.w)};
 #pragma unroll
               for (int p = 0; p < 2; ++p) {
 #pragma unroll
                 for (int c = 0; c < G; ++c)
-                  y[p] = fma2(pair_at(raw[c][j + 2 * p], raw[c][j + 2 * p + 1]), make_float2(f[c], f[c]),
-                              y[p]);
+                  y[p] = fma2(pair_at(raw[c][j + 2 * p], raw[c][j + 2 * p + 1]), f[c], y[p]);
                 y[p] = make_float2(ex2(y[p].x), ex2(y[p].y));
                 if (edge) {
-                  const int col = part * N + col0 + j + 2 * p;
+                  const int col = p0 * N + col0 + j + 2 * p;
                   if (col < see || col >= rows) y[p].x = 0.f;
                   if (col + 1 < see || col + 1 >= rows) y[p].y = 0.f;
                 }
@@ -850,10 +946,11 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
         if (ok && lane == 0) mbar_arrive(&l_free[lb]);
       }
       if (!ok) break;
-      parts[(static_cast<size_t>(w.index + blockIdx.x) * 2 + half) * TILE + key_at] = total.x + total.y;
+      parts[(static_cast<size_t>(w.index + blockIdx.x) * KEY_PARTS + part) * TILE + key_at] =
+          total.x + total.y;
       if (tid == 0) {
         if (w.step == 0) span_out[2 * w.index] = blockIdx.x;
-        if (w.step + n == w.steps) span_out[2 * w.index + 1] = blockIdx.x;
+        if (w.step + here == w.steps) span_out[2 * w.index + 1] = blockIdx.x;
       }
     }
   }
@@ -880,11 +977,11 @@ __global__ void __launch_bounds__(TILE) add_kernel(
       if (d < c) return;
       if (tile < tiles) {
         const int index = base + h * tiles + tile;
-        const int lo = span[2 * index], hi = span[2 * index + 1];
+        const int2 of = span_of(span, index);
         float sum = 0.f;
-        for (int x = lo; x <= hi; ++x)
-          for (int half = 0; half < 2; ++half)
-            sum += parts[(static_cast<size_t>(index + x) * 2 + half) * TILE + tid];
+        for (int x = of.x; x <= of.y; ++x)
+          for (int part = 0; part < KEY_PARTS; ++part)
+            sum += parts[(static_cast<size_t>(index + x) * KEY_PARTS + part) * TILE + tid];
         total += sum;
         seen = max(seen, other.pos0 + other.q_len);
       }
@@ -933,8 +1030,8 @@ static int launch(const __half* q, const Geometry& g, const int8_t* kc, const __
   if (const int e = runtime_allow_smem(slot[1], sums_kernel<D>, L::B_TOTAL)) return e;
   const Bounds b = bounds(g.n_chunks, g.longest, g.kvh, g.rep, g.limit);
   float* lse = work;
-  float* parts = lse + (b.row_tiles + CTAS) * TILE;
-  int* row_span = reinterpret_cast<int*>(parts + (b.key_tiles + CTAS) * 2 * TILE);
+  float* parts = lse + (b.row_tiles + CTAS) * ROW_PARTS * TILE;
+  int* row_span = reinterpret_cast<int*>(parts + (b.key_tiles + CTAS) * KEY_PARTS * TILE);
   int* key_span = row_span + 2 * b.row_tiles;
   const int ctas = ctas_for(b.units);
   launch_early(stats_kernel<D>, dim3(ctas), THREADS, L::A_TOTAL, stream, tq, g, kc, ks, lse, row_span,
@@ -957,7 +1054,8 @@ extern "C" size_t orinfer_prefill_weights_work_bytes(int n_chunks, int max_q_len
                                                      int limit) {
   if (n_chunks <= 0 || rep <= 0) return 0;
   const kw::Bounds b = kw::bounds(n_chunks, max_q_len, kvh, rep, limit);
-  return ((b.row_tiles + kw::CTAS) * kw::TILE + (b.key_tiles + kw::CTAS) * 2 * kw::TILE) * sizeof(float) +
+  return ((b.row_tiles + kw::CTAS) * kw::ROW_PARTS + (b.key_tiles + kw::CTAS) * kw::KEY_PARTS) *
+             kw::TILE * sizeof(float) +
          2 * (b.row_tiles + b.key_tiles) * sizeof(int);
 }
 
