@@ -27,10 +27,10 @@ namespace kw {
 
 constexpr int TILE = 128;                        // rows of a tile: positions x query heads; keys of a tile
 constexpr int MAX_CHUNKS = 512;
-constexpr int EP_WARPS = 16;                     // softmax or sums
-constexpr int DQ_WARPS = 4, TEAMS = 2;           // INT8 to FP16: a team's warps, which take turns
+constexpr int EP_WARPS = 16, EP_GROUP = 8;       // softmax or sums: two groups, a product each in turn
+constexpr int DQ_WARPS = 8;                      // INT8 to FP16
 constexpr int AUX_WARPS = 2;                     // scales or rows' lse, in turn
-constexpr int AUX_WARP = EP_WARPS + TEAMS * DQ_WARPS, MMA_WARP = AUX_WARP + AUX_WARPS;
+constexpr int AUX_WARP = EP_WARPS + DQ_WARPS, MMA_WARP = AUX_WARP + AUX_WARPS;
 constexpr int TMA_WARP = MMA_WARP + 1, THREADS = (TMA_WARP + 1) * 32;
 constexpr int CTAS = 148;
 constexpr int NS = 4;                            // places of scales, or of rows' lse
@@ -191,39 +191,86 @@ struct Units {
 template <int D>
 struct Shape {
   static constexpr int G = D / 64;               // scale groups of a key
-  static constexpr int QSUB = TILE * 128;        // bytes of 64 channels of a query tile
+  static constexpr int QSUB = TILE * 128;        // bytes of 64 channels of a tile of 128 rows or keys
   static constexpr int Q_BYTES = G * QSUB;
+  static constexpr int N = 64;                   // columns of a product
+  static constexpr int SLOT = G * N;             // and of TMEM, a group of channels after the other
+  static constexpr int SLOTS = D > 128 ? 2 : 4;  // products that have a place
+  static constexpr int RK = D > 128 ? 64 : 128;  // keys that are copied at a time
+  static constexpr int R_BYTES = RK * D;
   // ---- stats_kernel
-  static constexpr int KT = D > 128 ? 64 : 128;  // keys of a step: at most 256 score columns
-  static constexpr int KSUB = KT * 128, K_BYTES = G * KSUB;
-  static constexpr int NQ = 2, NK = D > 128 ? 2 : 3;           // buffers of queries and of keys
+  static constexpr int KT = RK;                  // keys of a step
+  static constexpr int KSUB = KT * 128, K_BYTES = G * KSUB, PER_A = KT / N;
+  static constexpr int NQ = D > 128 ? 1 : 2, NK = 3, NR = 3;   // buffers of queries, keys, raw keys
   static constexpr int A_K = NQ * Q_BYTES;
-  static constexpr int A_SCALE = A_K + NK * K_BYTES;
+  static constexpr int A_R = A_K + NK * K_BYTES;
+  static constexpr int A_SCALE = A_R + NR * R_BYTES;
   static constexpr int SCALES = KT * G * 4;
   static constexpr int A_BAR = A_SCALE + NS * SCALES;
   static constexpr int A_TOTAL = A_BAR + 512 + 1024;
   // ---- sums_kernel
-  static constexpr int N = D > 128 ? 64 : 128;   // rows of a product: at most 256 score columns
-  static constexpr int PER = TILE / N;           // products of a unit and group
-  static constexpr int BQ = D > 128 ? 2 : 3, BK = D > 128 ? 1 : 2;
+  static constexpr int PER_B = TILE / N;         // products of a unit
+  static constexpr int BQ = D > 128 ? 2 : 3, BK = D > 128 ? 1 : 2, BR = D > 128 ? 1 : 2;
   static constexpr int TSUB = TILE * 128, T_BYTES = G * TSUB;  // a tile of 128 keys
   static constexpr int B_Q = BK * T_BYTES;
-  static constexpr int B_LSE = B_Q + BQ * Q_BYTES;
-  static constexpr int B_SCALE = B_LSE + NS * TILE * 4;        // [NS][G][128]
-  static constexpr int B_BAR = B_SCALE + NS * G * TILE * 4;
+  static constexpr int B_R = B_Q + BQ * Q_BYTES;
+  static constexpr int B_LSE = B_R + BR * R_BYTES;
+  static constexpr int B_SCALE = B_LSE + NS * TILE * 4;        // [NC][G][128]
+  static constexpr int NC = 2;
+  static constexpr int B_BAR = B_SCALE + NC * G * TILE * 4;
   static constexpr int B_TOTAL = B_BAR + 512 + 1024;
   static_assert(A_TOTAL + sizeof(Plan) <= 227 * 1024 && B_TOTAL + sizeof(Plan) <= 227 * 1024,
                 "exceeds the shared memory of one CTA");
+  static_assert(SLOT * SLOTS <= 512, "exceeds tensor memory");
 };
 
-__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t tmem_d, uint64_t adesc,
-                                       uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+constexpr int TMA_WAIT = STATUS_TMA_WAIT, MMA_WAIT = STATUS_MMA_WAIT;
+constexpr int EPILOGUE_WAIT = STATUS_EPILOGUE_WAIT, DECODE_WAIT = STATUS_DECODE_WAIT;
+
+// The bounded wait of common.cuh for warps that wait most of the time: each try may sleep for as long as
+// the second number says, in nanoseconds, and takes no issue slots meanwhile.  (Twenty-eight warps that
+// poll took half of them.)
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* status, int code,
+                                          int detail) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long limit = wait_limit(status), start = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (clock64() - start > limit) {
+      report_status(status, code, detail);
+      return false;
+    }
+  }
+  return true;
+}
+
+// Descriptors by their lower words, which are where an operand starts; the upper one is the same for all
+// tiles here (K-major rows of 128 bytes, swizzled, groups of eight 1024 bytes apart).
+constexpr uint32_t DESC_HIGH = 1024 >> 4 | 1u << 14 | static_cast<uint32_t>(UMMA_SWIZZLE_128B) << 29;
+__device__ __forceinline__ uint32_t desc_low(const void* tile) {
+  return (smem_u32(tile) & 0x3ffff) >> 4 | 1u << 16;
+}
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t tmem_d, uint32_t a_low, uint32_t b_low,
+                                       uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
+      ".reg .b64 a, b;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      "mov.b64 a, {%1, %6};\n\t"
+      "mov.b64 b, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(leader), "r"(DESC_HIGH)
       : "memory");
 }
 // Sixteen TMEM lanes as fragments: per eight columns lane (g = lane / 4, t = lane % 4) holds columns 2t
@@ -298,15 +345,19 @@ __device__ __forceinline__ void place(unsigned char* to, int sub, const uint4& r
   *reinterpret_cast<uint4*>(dst + swz128(key, (c % 4) * 2 + !swap)) = hi;
 }
 
-// A page that does not exist is reported, and page 0 is read instead.  (By the one who uses the number, a
-// step after it was asked for.)
-__device__ __forceinline__ int page_or_0(const Geometry& g, int page, int* status) {
-  if (page >= 0 && page < g.num_pages) return page;
-  report_status(status, STATUS_BAD_INDEX, 0x71);
-  return 0;
+// Keys as they were copied, rows of D bytes, to FP16 integers in swizzled tiles, from key `at` on.  By
+// THREADS_ threads.
+template <int D, int PER, int THREADS_>
+__device__ __forceinline__ void convert(const unsigned char* from, unsigned char* to, int sub, int t, int at) {
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int x = t + j * THREADS_;
+    place(to, sub, *reinterpret_cast<const uint4*>(from + x * 16), at + x / (D / 16), x % (D / 16));
+  }
 }
+
 // Where a role that goes ahead reads its next keys: their page, asked for a turn before, the first key's
-// place on it and the head.
+// place on it and the head.  A page that does not exist is reported, and page 0 is read instead.
 struct Ahead {
   int page = 0, at = 0, h = 0;
   __device__ void ask(const Geometry& g, const Chunk& ch, int key, int head) {
@@ -314,8 +365,10 @@ struct Ahead {
     at = key & 127;
     h = head;
   }
-  __device__ size_t cell(const Geometry& g, int* status) const {         // of the first key and its head
-    return (static_cast<size_t>(page_or_0(g, page, status)) * 128 + at) * g.kvh + h;
+  __device__ int row(const Geometry& g, int* status) const {             // of the cache
+    const bool there = page >= 0 && page < g.num_pages;
+    if (!there) report_status(status, STATUS_BAD_INDEX, 0x71);
+    return (there ? page * 128 : 0) + at;
   }
 };
 
@@ -331,21 +384,24 @@ __device__ __forceinline__ void clear_tails(unsigned char* q, int tiles, int row
 // lse: [row tiles + CTAs][2][128], log2 of a part's sum of weights; span: a row tile's first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
-    const __grid_constant__ CUtensorMap tmap_q, const Geometry g, const int8_t* kc, const __half* ks,
-    float* lse, int* span, int* status) {
+    const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+    const Geometry g, const __half* ks, float* lse, int* span, int* status) {
   using L = Shape<D>;
-  constexpr int G = L::G, KT = L::KT, NQ = L::NQ, NK = L::NK;
+  constexpr int G = L::G, KT = L::KT, N = L::N, PER = L::PER_A, NQ = L::NQ, NK = L::NK, NR = L::NR;
+  constexpr int SLOTS = L::SLOTS;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ Plan plan;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::A_BAR);
   uint64_t* q_full = bars;                       // [NQ] a tile's queries
   uint64_t* q_free = q_full + NQ;                // [NQ] its last product is through
-  uint64_t* k_full = q_free + NQ;                // [NK] a unit's keys
-  uint64_t* k_free = k_full + NK;                // [NK] its product is through
-  uint64_t* s_full = k_free + NK;                // [2] its scores
-  uint64_t* s_free = s_full + 2;                 // [2] they have been read (an arrival per softmax warp)
-  uint64_t* c_full = s_free + 2;                 // [NS] its scales
+  uint64_t* r_full = q_free + NQ;                // [NR] a unit's keys as the cache has them
+  uint64_t* r_free = r_full + NR;                // [NR] they have been read
+  uint64_t* k_full = r_free + NR;                // [NK] and as FP16 integers
+  uint64_t* k_free = k_full + NK;                // [NK] its products are through
+  uint64_t* s_full = k_free + NK;                // [SLOTS] scores of a product
+  uint64_t* s_free = s_full + SLOTS;             // [SLOTS] they have been read (an arrival per warp)
+  uint64_t* c_full = s_free + SLOTS;             // [NS] a unit's scales
   uint64_t* c_free = c_full + NS;                // [NS] they have been used (the same)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_free + NS);
   const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
@@ -354,20 +410,25 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       mbar_init(&q_full[b], 1);
       mbar_init(&q_free[b], 1);
     }
+    for (int b = 0; b < NR; ++b) {
+      mbar_init(&r_full[b], 1);
+      mbar_init(&r_free[b], DQ_WARPS);
+    }
     for (int b = 0; b < NK; ++b) {
       mbar_init(&k_full[b], DQ_WARPS);
       mbar_init(&k_free[b], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < SLOTS; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&s_free[b], EP_WARPS);
+      mbar_init(&s_free[b], EP_GROUP);
     }
     for (int b = 0; b < NS; ++b) {
       mbar_init(&c_full[b], 1);
-      mbar_init(&c_free[b], EP_WARPS);
+      mbar_init(&c_free[b], EP_GROUP * PER);
     }
     mbar_fence_init();
     prefetch_tmap(&tmap_q);
+    prefetch_tmap(&tmap_k);
   }
   if (g.per * g.rep < TILE) clear_tails(smem, NQ * G, g.per * g.rep);
   grid_wait();
@@ -384,45 +445,65 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
   bool ok = true;
 
   if (warp == TMA_WARP) {
-    Walk<KT> w(g, plan);
+    Units<KT> u(g, plan);
     if (lane == 0) {
-      int n = 0;
-      for (; w.left > 0; w.next_tile(), ++n) {
-        const int b = n % NQ;
-        if (n >= NQ && !mbar_wait(&q_free[b], (n / NQ - 1) & 1, status, STATUS_TMA_WAIT, 0x10)) break;
-        mbar_expect_tx(&q_full[b], static_cast<uint32_t>(G) * 64 * 2 * g.rep * g.per);
-        for (int s = 0; s < G; ++s)
-          tma_load_3d(smem + b * L::Q_BYTES + s * L::QSUB, &tmap_q, &q_full[b], s * 64, w.h * g.rep,
-                      w.ch.row_start + w.tile * g.per);
+      int n = 0, i = 0;                            // tiles, units
+      Ahead next;
+      if (u.more()) next.ask(g, u.w.ch, u.step() * KT, u.w.h);
+      bool fresh = true;
+      while (u.more()) {
+        if (fresh) {
+          const int b = n % NQ;
+          if (n >= NQ && !mbar_wait(&q_free[b], (n / NQ - 1) & 1, status, TMA_WAIT, 0x10)) break;
+          mbar_expect_tx(&q_full[b], static_cast<uint32_t>(G) * 64 * 2 * g.rep * g.per);
+          for (int s = 0; s < G; ++s)
+            tma_load_3d(smem + b * L::Q_BYTES + s * L::QSUB, &tmap_q, &q_full[b], s * 64, u.w.h * g.rep,
+                        u.w.ch.row_start + u.w.tile * g.per);
+          ++n;
+        }
+        const int b = i % NR, h = next.h, row = next.row(g, status), tile = u.w.index;
+        u.next();
+        if (u.more()) next.ask(g, u.w.ch, u.step() * KT, u.w.h);
+        fresh = u.w.index != tile;
+        if (i >= NR && !mbar_wait(&r_free[b], (i / NR - 1) & 1, status, TMA_WAIT, 0x11)) break;
+        mbar_expect_tx(&r_full[b], L::R_BYTES);
+        tma_load_3d(smem + L::A_R + b * L::R_BYTES, &tmap_k, &r_full[b], 0, h, row);
+        ++i;
       }
-      for (int i = max(n - NQ, 0); i < n; ++i)     // our copies have landed before exit
-        mbar_wait(&q_full[i % NQ], (i / NQ) & 1, status, STATUS_TMA_WAIT, 0x11);
+      for (int j = max(n - NQ, 0); j < n; ++j)     // our copies have landed before exit
+        mbar_wait(&q_full[j % NQ], (j / NQ) & 1, status, TMA_WAIT, 0x12);
+      for (int j = max(i - NR, 0); j < i; ++j)
+        mbar_wait(&r_full[j % NR], (j / NR) & 1, status, TMA_WAIT, 0x13);
     }
   } else if (warp == MMA_WARP) {
-    constexpr uint32_t idesc = umma_idesc(1, 0, 0, 0, 0, TILE, KT);
+    constexpr uint32_t idesc = umma_idesc(1, 0, 0, 0, 0, TILE, N);
     const uint32_t leader = elect_one();
-    const uint64_t qd = umma_desc(smem_u32(smem), 16, 1024);
-    const uint64_t kd = umma_desc(smem_u32(smem + L::A_K), 16, 1024);
-    int n = 0, i = 0;
-    for (Walk<KT> w(g, plan); w.left > 0 && ok; w.next_tile(), ++n) {
-      const int last = i + w.here();
-      ok = warp_all(mbar_wait(&q_full[n % NQ], (n / NQ) & 1, status, STATUS_MMA_WAIT, 0x12));
-      const uint64_t qb = qd + static_cast<uint64_t>(n % NQ) * (L::Q_BYTES / 16);
+    const uint32_t qd = desc_low(smem);
+    const uint32_t kd = desc_low(smem + L::A_K);
+    int n = 0, i = 0, x = 0;                       // tiles, units, products
+    for (Walk<KT> w(g, plan); warp_same(w.left) > 0 && ok; w.next_tile(), ++n) {
+      const int last = i + warp_same(w.here());
+      ok = warp_all(mbar_wait(&q_full[n % NQ], (n / NQ) & 1, status, MMA_WAIT, 0x14));
+      const uint32_t qb = qd + (n % NQ) * (L::Q_BYTES / 16);
       for (; i < last && ok; ++i) {
-        const int b = i % NK, s = i & 1;
-        ok = warp_all(mbar_wait(&k_full[b], (i / NK) & 1, status, STATUS_MMA_WAIT, 0x13) &&
-                      (i < 2 || mbar_wait(&s_free[s], (i / 2 - 1) & 1, status, STATUS_MMA_WAIT, 0x14)));
-        tc_fence_after();
-        if (!ok) break;
-        const uint64_t kb = kd + static_cast<uint64_t>(b) * (L::K_BYTES / 16);
+        const int b = i % NK;
+        ok = warp_all(mbar_wait(&k_full[b], (i / NK) & 1, status, MMA_WAIT, 0x15));
+        for (int p = 0; p < PER && ok; ++p, ++x) {
+          const int s = x % SLOTS;
+          if (x >= SLOTS) ok = mbar_wait(&s_free[s], (x / SLOTS - 1) & 1, status, MMA_WAIT, 0x16);
+          ok = warp_all(ok);
+          tc_fence_after();
+          if (!ok) break;
+          const uint32_t kb = kd + (b) * (L::K_BYTES / 16) + p * (N * 128 / 16);
 #pragma unroll
-        for (int c = 0; c < G; ++c)
+          for (int c = 0; c < G; ++c)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ss(leader, tmem + 256 * s + c * KT, qb + (c * L::QSUB + k * 32) / 16,
-                   kb + (c * L::KSUB + k * 32) / 16, idesc, k != 0 ? 1u : 0u);
-        tc_commit_by(leader, &k_free[b]);
-        tc_commit_by(leader, &s_full[s]);
+            for (int k = 0; k < 4; ++k)
+              mma_ss(leader, tmem + L::SLOT * s + c * N, qb + (c * L::QSUB + k * 32) / 16,
+                     kb + (c * L::KSUB + k * 32) / 16, idesc, k != 0 ? 1u : 0u);
+          tc_commit_by(leader, &s_full[s]);
+        }
+        if (ok) tc_commit_by(leader, &k_free[b]);
       }
       if (ok) tc_commit_by(leader, &q_free[n % NQ]);
     }
@@ -438,7 +519,7 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       if (u.more()) next.ask(g, u.w.ch, u.step() * KT, u.w.h);
     };
     auto fetch = [&] {                             // what `next` names, and the page behind it
-      const size_t cell = next.cell(g, status);
+      const size_t cell = static_cast<size_t>(next.row(g, status)) * g.kvh + next.h;
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
         const int x = lane + 32 * j;
@@ -453,7 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     if (mine < units) fetch();
     for (int i = mine; i < units; i += AUX_WARPS) {
       const int b = i % NS;
-      if (i >= NS) ok = mbar_wait(&c_free[b], (i / NS - 1) & 1, status, STATUS_DECODE_WAIT, 0x15);
+      if (i >= NS) ok = mbar_wait(&c_free[b], (i / NS - 1) & 1, status, DECODE_WAIT, 0x17);
       ok = warp_all(ok);
       if (!ok) break;
       float* sk = reinterpret_cast<float*>(smem + L::A_SCALE + b * L::SCALES);
@@ -467,53 +548,30 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       if (i + AUX_WARPS < units) fetch();
     }
   } else if (warp >= EP_WARPS) {
-    // ---------------- keys: INT8 from global memory, a unit of the team's ahead in registers, to FP16
-    // integers
-    constexpr int DQ = DQ_WARPS * 32, KI = KT * D / 16 / DQ;
-    const int t = (tid - EP_WARPS * 32) % DQ, team = warp_same((tid - EP_WARPS * 32) / DQ);
-    uint4 raw[KI];
-    Ahead next;
-    Units<KT> u(g, plan);
-    auto ask = [&] {
-      if (u.more()) next.ask(g, u.w.ch, u.step() * KT, u.w.h);
-    };
-    auto fetch = [&] {
-      const size_t cell = next.cell(g, status);
-#pragma unroll
-      for (int j = 0; j < KI; ++j) {
-        const int x = t + j * DQ, key = x / (D / 16), c = x % (D / 16);
-        raw[j] = *reinterpret_cast<const uint4*>(kc + (cell + static_cast<size_t>(key) * g.kvh) * D + c * 16);
-      }
-      u.skip(TEAMS);
-      ask();
-    };
-    const int units = max(u.w.left, 0);
-    u.skip(team);
-    ask();
-    if (team < units) fetch();
-    for (int i = team; i < units; i += TEAMS) {
-      const int b = i % NK;
-      if (i >= NK) ok = mbar_wait(&k_free[b], (i / NK - 1) & 1, status, STATUS_DECODE_WAIT, 0x16);
+    // ---------------- keys: INT8 to FP16 integers
+    constexpr int DQ = DQ_WARPS * 32, KI = L::R_BYTES / 16 / DQ;
+    const int t = tid - EP_WARPS * 32, units = max(Walk<KT>(g, plan).left, 0);
+    for (int i = 0; i < units; ++i) {
+      const int b = i % NK, r = i % NR;
+      ok = mbar_wait(&r_full[r], (i / NR) & 1, status, DECODE_WAIT, 0x18) &&
+           (i < NK || mbar_wait(&k_free[b], (i / NK - 1) & 1, status, DECODE_WAIT, 0x19));
       ok = warp_all(ok);
       if (!ok) break;
-      unsigned char* buf = smem + L::A_K + b * L::K_BYTES;
-#pragma unroll
-      for (int j = 0; j < KI; ++j) {
-        const int x = t + j * DQ;
-        place(buf, L::KSUB, raw[j], x / (D / 16), x % (D / 16));
-      }
+      convert<D, KI, DQ>(smem + L::A_R + r * L::R_BYTES, smem + L::A_K + b * L::K_BYTES, L::KSUB, t, 0);
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[b]);
-      if (i + TEAMS < units) fetch();
+      if (lane == 0) {
+        mbar_arrive(&k_full[b]);
+        mbar_arrive(&r_free[r]);
+      }
     }
   } else {
-    // ---------------- sixteen rows by half of the step's keys per warp; a thread holds columns 2 qt and 2
-    // qt + 1 of every eight, of rows qg and qg + 8
+    // ---------------- sixteen rows per warp, every other product; a thread holds columns 2 qt and 2 qt + 1
+    // of every eight, of rows qg and qg + 8, and has a reference of its own for each
     const int qg = lane >> 2, qt = lane & 3, row0 = (warp & 3) * 32 + (warp >> 2 & 1) * 16;
-    constexpr int COLS = KT / ROW_PARTS, CH = G > 2 ? 16 : 32;   // of a warp, and at a time
-    const int part = warp >> 3;
-    const uint32_t lane_addr = static_cast<uint32_t>(row0) << 16;
+    constexpr int CH = G > 2 ? 16 : 32;          // columns at a time
+    const int group = warp >> 3;
+    const uint32_t scores = tmem + (static_cast<uint32_t>(row0) << 16);
     int i = 0;
     for (Walk<KT> w(g, plan); w.left > 0 && ok; w.next_tile()) {
       int sees[2];                               // keys that its rows see
@@ -526,31 +584,34 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       float m_ref[2] = {0.f, 0.f};
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       const int n = w.here();
-      for (int j0 = 0; j0 < n; ++j0, ++i) {
-        const int sb = i & 1, cb = i % NS, key0 = (w.step + j0) * KT + part * COLS;
-        ok = mbar_wait(&s_full[sb], (i / 2) & 1, status, STATUS_EPILOGUE_WAIT, 0x17) &&
-             mbar_wait(&c_full[cb], (i / NS) & 1, status, STATUS_EPILOGUE_WAIT, 0x18);
+      bool start = true;
+      // every unit where it has two products, else every other one
+      for (int j0 = PER > 1 || (i & 1) == group ? 0 : 1; j0 < n; j0 += PER > 1 ? 1 : 2) {
+        const int u = i + j0, cb = u % NS, p0 = PER > 1 ? group * N : 0;
+        const int x = PER > 1 ? 2 * u + group : u, slot = x % SLOTS;
+        const int key0 = (w.step + j0) * KT + p0;
+        ok = mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x1a) &&
+             mbar_wait(&c_full[cb], (u / NS) & 1, status, EPILOGUE_WAIT, 0x1b);
         ok = warp_all(ok);
         if (!ok) break;
         tc_fence_after();
-        const float2* sk = reinterpret_cast<const float2*>(smem + L::A_SCALE + cb * L::SCALES) +
-                           (part * COLS / 2 + qt) * G;
+        const float2* sk =
+            reinterpret_cast<const float2*>(smem + L::A_SCALE + cb * L::SCALES) + (p0 / 2 + qt) * G;
 #pragma unroll
-        for (int c0 = 0; c0 < COLS; c0 += CH) {
+        for (int k = 0; k < N; k += CH) {
           uint32_t raw[G][CH / 2];
 #pragma unroll
-          for (int c = 0; c < G; ++c)
-            tmem_ld_frag(tmem + 256 * sb + c * KT + part * COLS + c0 + lane_addr, raw[c]);
+          for (int c = 0; c < G; ++c) tmem_ld_frag(scores + L::SLOT * slot + c * N + k, raw[c]);
           tc_wait_ld();
-          if (c0 + CH == COLS) {
+          if (k + CH == N) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[sb]);
+            if (lane == 0) mbar_arrive(&s_free[slot]);
           }
           float2 x[2][CH / 8];
 #pragma unroll
           for (int j = 0; j < CH / 8; ++j) {
-            const float2* s = sk + (c0 / 2 + 4 * j) * G;
+            const float2* s = sk + (k / 2 + 4 * j) * G;
             float2 f[G];
             if (G == 1) {
               f[0] = s[0];
@@ -570,12 +631,12 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
                 x[r][j] = fma2(pair_at(raw[c][4 * j + 2 * r], raw[c][4 * j + 2 * r + 1]), f[c], x[r][j]);
             }
           }
-          if (all_see < key0 + c0 + CH) {
+          if (all_see < key0 + k + CH) {
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
               for (int j = 0; j < CH / 8; ++j) {
-                const int key = key0 + c0 + 8 * j + 2 * qt;
+                const int key = key0 + k + 8 * j + 2 * qt;
                 if (key >= sees[r]) x[r][j].x = -INFINITY;
                 if (key + 1 >= sees[r]) x[r][j].y = -INFINITY;
               }
@@ -587,18 +648,14 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
             return v;
           };
           float2 more[2] = {weights(0), weights(1)};
-          // The reference is the maximum of the first columns, and moves where weights are far above 1:
-          // no maximum is taken but then.  (A row that sees none of the first sees none behind them.)
-          const bool start = j0 == 0 && c0 == 0;
-          const float far = fmaxf(more[0].x + more[0].y, more[1].x + more[1].y);
-          if (__any_sync(0xffffffffu, start || far > LEAD)) {
+          // The reference is the maximum of the thread's first columns, and moves where weights are far
+          // above 1: no maximum is taken but then.  (A row that sees none of the first sees none behind.)
+          if (start || fmaxf(more[0].x + more[0].y, more[1].x + more[1].y) > LEAD) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               float top = fmaxf(x[r][0].x, x[r][0].y);
 #pragma unroll
               for (int j = 1; j < CH / 8; ++j) top = fmaxf(top, fmaxf(x[r][j].x, x[r][j].y));
-#pragma unroll
-              for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
               const float by = top == -INFINITY ? 0.f : start ? top : fmaxf(top, 0.f);
               const float f = start ? 0.f : ex2(-by);
               sum[r] = mul2(sum[r], make_float2(f, f));
@@ -607,6 +664,7 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
               for (int j = 0; j < CH / 8; ++j) x[r][j] = add2(x[r][j], make_float2(-by, -by));
               more[r] = weights(r);
             }
+            start = false;
           }
 #pragma unroll
           for (int r = 0; r < 2; ++r) sum[r] = add2(sum[r], more[r]);
@@ -615,13 +673,19 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
         if (lane == 0) mbar_arrive(&c_free[cb]);
       }
       if (!ok) break;
-      const size_t place = static_cast<size_t>(w.index + blockIdx.x) * ROW_PARTS + part;
+      i += n;
+      const size_t place = static_cast<size_t>(w.index + blockIdx.x) * ROW_PARTS + group;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float l = sum[r].x + sum[r].y;
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (qt == 0) lse[place * TILE + row0 + qg + 8 * r] = m_ref[r] + log2f(l);
+        float l = sum[r].x + sum[r].y, m = l == 0.f ? -INFINITY : m_ref[r];
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+          const float top = fmaxf(m, m2);
+          l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + (m2 == -INFINITY ? 0.f : l2 * ex2(m2 - top));
+          m = top;
+        }
+        if (qt == 0) lse[place * TILE + row0 + qg + 8 * r] = m + log2f(l);
       }
       if (tid == 0) {
         if (w.step == 0) span[2 * w.index] = blockIdx.x;
@@ -638,47 +702,58 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
 // tile's first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
-    const __grid_constant__ CUtensorMap tmap_q, const Geometry g, const int8_t* kc, const __half* ks,
-    const float* lse, const int* span, float* parts, int* span_out, int* status) {
+    const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+    const Geometry g, const __half* ks, const float* lse, const int* span, float* parts, int* span_out,
+    int* status) {
   using L = Shape<D>;
-  constexpr int G = L::G, N = L::N, PER = L::PER, BQ = L::BQ, BK = L::BK;
+  constexpr int G = L::G, N = L::N, PER = L::PER_B, BQ = L::BQ, BK = L::BK, BR = L::BR, NC = L::NC;
+  constexpr int SLOTS = L::SLOTS, HALVES = TILE / L::RK;         // copies of a tile's keys
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ Plan plan;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::B_BAR);
-  uint64_t* k_full = bars;                       // [BK] a tile's keys
+  uint64_t* r_full = bars;                       // [BR] keys as the cache has them
+  uint64_t* r_free = r_full + BR;                // [BR] they have been read
+  uint64_t* k_full = r_free + BR;                // [BK] a tile's keys as FP16 integers
   uint64_t* k_free = k_full + BK;                // [BK] its last product is through
   uint64_t* q_full = k_free + BK;                // [BQ] a unit's queries
   uint64_t* q_free = q_full + BQ;                // [BQ] its products are through
-  uint64_t* s_full = q_free + BQ;                // [2] scores of a product
-  uint64_t* s_free = s_full + 2;                 // [2] they have been read (an arrival per warp)
-  uint64_t* l_full = s_free + 2;                 // [NS] a unit's lse
+  uint64_t* s_full = q_free + BQ;                // [SLOTS] scores of a product
+  uint64_t* s_free = s_full + SLOTS;             // [SLOTS] they have been read (an arrival per warp)
+  uint64_t* l_full = s_free + SLOTS;             // [NS] a unit's lse
   uint64_t* l_free = l_full + NS;                // [NS] they have been used (an arrival per warp)
-  uint64_t* c_full = l_free + NS;                // [NS] a tile's scales
-  uint64_t* c_free = c_full + NS;                // [NS] they have been read (an arrival per warp)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_free + NS);
+  uint64_t* c_full = l_free + NS;                // [NC] a tile's scales
+  uint64_t* c_free = c_full + NC;                // [NC] they have been read (an arrival per warp)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_free + NC);
   const int tid = threadIdx.x, warp = warp_same(tid >> 5), lane = tid & 31;
   if (tid == 0) {
+    for (int b = 0; b < BR; ++b) {
+      mbar_init(&r_full[b], 1);
+      mbar_init(&r_free[b], DQ_WARPS);
+    }
     for (int b = 0; b < BK; ++b) {
-      mbar_init(&k_full[b], TEAMS * DQ_WARPS / BK);
+      mbar_init(&k_full[b], DQ_WARPS);
       mbar_init(&k_free[b], 1);
     }
     for (int b = 0; b < BQ; ++b) {
       mbar_init(&q_full[b], 1);
       mbar_init(&q_free[b], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < SLOTS; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&s_free[b], EP_WARPS);
+      mbar_init(&s_free[b], EP_GROUP);
     }
     for (int b = 0; b < NS; ++b) {
       mbar_init(&l_full[b], 1);
       mbar_init(&l_free[b], EP_WARPS);
-      mbar_init(&c_full[b], TEAMS * DQ_WARPS / BK);
+    }
+    for (int b = 0; b < NC; ++b) {
+      mbar_init(&c_full[b], DQ_WARPS);
       mbar_init(&c_free[b], EP_WARPS);
     }
     mbar_fence_init();
     prefetch_tmap(&tmap_q);
+    prefetch_tmap(&tmap_k);
   }
   if (g.per * g.rep < TILE) clear_tails(smem + L::B_Q, BQ * G, g.per * g.rep);
   grid_wait();
@@ -704,40 +779,40 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       int n = 0;
       for (; u.more(); u.next(), ++n) {
         const int b = n % BQ;
-        if (n >= BQ && !mbar_wait(&q_free[b], (n / BQ - 1) & 1, status, STATUS_TMA_WAIT, 0x20)) break;
+        if (n >= BQ && !mbar_wait(&q_free[b], (n / BQ - 1) & 1, status, TMA_WAIT, 0x20)) break;
         mbar_expect_tx(&q_full[b], static_cast<uint32_t>(G) * 64 * 2 * g.rep * g.per);
         for (int s = 0; s < G; ++s)
           tma_load_3d(smem + L::B_Q + b * L::Q_BYTES + s * L::QSUB, &tmap_q, &q_full[b], s * 64,
                       u.w.h * g.rep, u.w.ch.row_start + row_tile(u.w, u.step()) * g.per);
       }
       for (int i = max(n - BQ, 0); i < n; ++i)     // our copies have landed before exit
-        mbar_wait(&q_full[i % BQ], (i / BQ) & 1, status, STATUS_TMA_WAIT, 0x21);
+        mbar_wait(&q_full[i % BQ], (i / BQ) & 1, status, TMA_WAIT, 0x21);
     }
   } else if (warp == MMA_WARP) {
     constexpr uint32_t idesc = umma_idesc(1, 0, 0, 0, 0, TILE, N);
     const uint32_t leader = elect_one();
-    const uint64_t kd = umma_desc(smem_u32(smem), 16, 1024);
-    const uint64_t qd = umma_desc(smem_u32(smem + L::B_Q), 16, 1024);
+    const uint32_t kd = desc_low(smem);
+    const uint32_t qd = desc_low(smem + L::B_Q);
     int n = 0, i = 0, x = 0;                       // tiles, units, products
-    for (Walk<0> w(g, plan); w.left > 0 && ok; w.next_tile(), ++n) {
-      const int last = i + w.here();
-      ok = warp_all(mbar_wait(&k_full[n % BK], (n / BK) & 1, status, STATUS_MMA_WAIT, 0x22));
-      const uint64_t kb = kd + static_cast<uint64_t>(n % BK) * (L::T_BYTES / 16);
+    for (Walk<0> w(g, plan); warp_same(w.left) > 0 && ok; w.next_tile(), ++n) {
+      const int last = i + warp_same(w.here());
+      ok = warp_all(mbar_wait(&k_full[n % BK], (n / BK) & 1, status, MMA_WAIT, 0x22));
+      const uint32_t kb = kd + (n % BK) * (L::T_BYTES / 16);
       for (; i < last && ok; ++i) {
         const int b = i % BQ;
-        ok = warp_all(mbar_wait(&q_full[b], (i / BQ) & 1, status, STATUS_MMA_WAIT, 0x23));
-        for (int part = 0; part < PER && ok; ++part, ++x) {
-          const int s = x & 1;
-          if (x >= 2) ok = mbar_wait(&s_free[s], (x / 2 - 1) & 1, status, STATUS_MMA_WAIT, 0x24);
+        ok = warp_all(mbar_wait(&q_full[b], (i / BQ) & 1, status, MMA_WAIT, 0x23));
+        for (int p = 0; p < PER && ok; ++p, ++x) {
+          const int s = x % SLOTS;
+          if (x >= SLOTS) ok = mbar_wait(&s_free[s], (x / SLOTS - 1) & 1, status, MMA_WAIT, 0x24);
           ok = warp_all(ok);
           tc_fence_after();
           if (!ok) break;
-          const uint64_t qb = qd + static_cast<uint64_t>(b) * (L::Q_BYTES / 16) + part * (N * 128 / 16);
+          const uint32_t qb = qd + (b) * (L::Q_BYTES / 16) + p * (N * 128 / 16);
 #pragma unroll
           for (int c = 0; c < G; ++c)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mma_ss(leader, tmem + 256 * s + c * N, kb + (c * L::TSUB + k * 32) / 16,
+              mma_ss(leader, tmem + L::SLOT * s + c * N, kb + (c * L::TSUB + k * 32) / 16,
                      qb + (c * L::QSUB + k * 32) / 16, idesc, k != 0 ? 1u : 0u);
           tc_commit_by(leader, &s_full[s]);
         }
@@ -768,7 +843,7 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     u.skip(mine);
     ask();
     for (int n = mine; n < units; n += AUX_WARPS) {
-      const int b = n % NS, live = rows;         // (see span_of)
+      const int b = n % NS, live = rows;           // (see span_of)
       const int lo = max(0, min(first, CTAS - 1)), hi = max(lo, min(last, CTAS - 1));
       auto part = [&, at = index](int x) {
         return *reinterpret_cast<const float4*>(lse + (static_cast<size_t>(at + lo) * ROW_PARTS + x) * TILE +
@@ -804,7 +879,7 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       v.y = 4 * lane + 1 < live ? -m.y - log2f(l.y) : -INFINITY;
       v.z = 4 * lane + 2 < live ? -m.z - log2f(l.z) : -INFINITY;
       v.w = 4 * lane + 3 < live ? -m.w - log2f(l.w) : -INFINITY;
-      if (n >= NS) ok = mbar_wait(&l_free[b], (n / NS - 1) & 1, status, STATUS_DECODE_WAIT, 0x25);
+      if (n >= NS) ok = mbar_wait(&l_free[b], (n / NS - 1) & 1, status, DECODE_WAIT, 0x25);
       ok = warp_all(ok);
       if (!ok) break;
       *reinterpret_cast<float4*>(smem + L::B_LSE + b * TILE * 4 + lane * 16) = v;
@@ -812,56 +887,66 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       if (lane == 0) mbar_arrive(&l_full[b]);
     }
   } else if (warp >= EP_WARPS) {
-    // ---------------- keys: a tile, INT8 to FP16 integers, and their scales; the team's next tile in
-    // registers
-    // (a team per buffer: one that waits for a buffer two turns behind cannot tell the turns apart)
-    constexpr int DQ = TEAMS * DQ_WARPS * 32 / BK, KI = TILE * D / 16 / DQ;
-    static_assert(BK <= TEAMS, "a team per buffer");
-    const int t = (tid - EP_WARPS * 32) % DQ, team = warp_same((tid - EP_WARPS * 32) / DQ);
+    // ---------------- keys: a tile, INT8 to FP16 integers, and their scales.  The copies are this role's
+    // own, BR ahead: the first lane of its first warp asks for them.
+    constexpr int DQ = DQ_WARPS * 32, KI = L::R_BYTES / 16 / DQ;
+    const int t = tid - EP_WARPS * 32;
     const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
-    uint4 raw[KI];
     __half scale[G];
     Ahead next;
     Walk<0> w(g, plan);
+    int n = 0, y = 0, asked = 0;                   // tiles, copies used and asked for
+    int tile_row[2] = {0, 0}, tile_h[2] = {0, 0};  // the tile at work and the next one
+    int tiles = 0;                                 // known so far
     auto ask = [&] {
       if (w.left > 0) next.ask(g, w.ch, w.tile * TILE, w.h);
     };
-    auto skip = [&](int n) {
-      for (; n > 0 && w.left > 0; --n) w.next_tile();
-    };
-    bool more;
-    auto fetch = [&] {                             // what `next` names, and the page behind it
-      more = w.left > 0;
-      if (!more) return;
-      const size_t cell = next.cell(g, status);
-#pragma unroll
-      for (int j = 0; j < KI; ++j) {
-        const int x = t + j * DQ, key = x / (D / 16), c = x % (D / 16);
-        raw[j] = *reinterpret_cast<const uint4*>(kc + (cell + static_cast<size_t>(key) * g.kvh) * D + c * 16);
-      }
-#pragma unroll
-      for (int c = 0; c < G; ++c) scale[c] = ks[(cell + static_cast<size_t>(t & (TILE - 1)) * g.kvh) * G + c];
-      skip(BK);
+    auto know = [&] {                              // the tile that `next` names, and the page behind it
+      if (w.left <= 0) return;
+      tile_row[tiles & 1] = next.row(g, status);
+      tile_h[tiles & 1] = next.h;
+      ++tiles;
+      w.next_tile();
       ask();
     };
-    skip(team);
-    ask();
-    fetch();
-    for (int n = team; more; n += BK) {
-      const int b = n % BK, cb = n % NS;
-      if (n >= BK) ok = mbar_wait(&k_free[b], (n / BK - 1) & 1, status, STATUS_DECODE_WAIT, 0x26);
-      ok = warp_all(ok);
-      if (!ok) break;
-      unsigned char* buf = smem + b * L::T_BYTES;
-#pragma unroll
-      for (int j = 0; j < KI; ++j) {
-        const int x = t + j * DQ;
-        place(buf, L::TSUB, raw[j], x / (D / 16), x % (D / 16));
+    // The copies of the tiles that are known, as far as buffers are free (their last use was BR copies ago).
+    auto copy = [&] {
+      if (t == 0) for (; asked < tiles * HALVES && asked < y + BR; ++asked) {
+        const int r = asked % BR, of = asked / HALVES & 1;
+        if (asked >= BR && !mbar_wait(&r_free[r], (asked / BR - 1) & 1, status, TMA_WAIT, 0x29)) return;
+        mbar_expect_tx(&r_full[r], L::R_BYTES);
+        tma_load_3d(smem + L::B_R + r * L::R_BYTES, &tmap_k, &r_full[r], 0, tile_h[of],
+                    tile_row[of] + asked % HALVES * L::RK);
       }
+    };
+    ask();
+    know();
+    copy();
+    for (; n < tiles; ++n) {
+      const int b = n % BK, cb = n % NC;
+      const size_t cell = (static_cast<size_t>(tile_row[n & 1]) + (t & (TILE - 1))) * g.kvh + tile_h[n & 1];
+#pragma unroll
+      for (int c = 0; c < G; ++c) scale[c] = ks[cell * G + c];
+      know();
+      copy();
+      __syncwarp();
+      ok = warp_all(n < BK || mbar_wait(&k_free[b], (n / BK - 1) & 1, status, DECODE_WAIT, 0x26));
+      for (int part = 0; part < HALVES && ok; ++part) {
+        const int r = y % BR;
+        ok = warp_all(mbar_wait(&r_full[r], (y / BR) & 1, status, DECODE_WAIT, 0x2b));
+        if (!ok) break;
+        convert<D, KI, DQ>(smem + L::B_R + r * L::R_BYTES, smem + b * L::T_BYTES, L::TSUB, t, part * L::RK);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&r_free[r]);
+        ++y;
+        copy();
+        __syncwarp();
+      }
+      if (!ok) break;
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[b]);
-      if (n >= NS) ok = mbar_wait(&c_free[cb], (n / NS - 1) & 1, status, STATUS_DECODE_WAIT, 0x29);
+      if (n >= NC) ok = mbar_wait(&c_free[cb], (n / NC - 1) & 1, status, DECODE_WAIT, 0x2c);
       ok = warp_all(ok);
       if (!ok) break;
       float* sc = reinterpret_cast<float*>(smem + L::B_SCALE + cb * G * TILE * 4);
@@ -870,17 +955,21 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
         if (t < TILE) sc[c * TILE + t] = __half2float(scale[c]) * qscale;
       __syncwarp();
       if (lane == 0) mbar_arrive(&c_full[cb]);
-      fetch();
     }
+    if (t == 0)                                    // our copies have landed before exit
+      for (int i = y; i < asked; ++i)
+        mbar_wait(&r_full[i % BR], (i / BR) & 1, status, TMA_WAIT, 0x2d);
+    __syncwarp();
   } else {
-    // ---------------- sums: a key per lane, a quarter of a product's rows per warp
-    const int quad = warp & 3, part = warp >> 2, key_at = quad * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
-    constexpr int COLS = N / KEY_PARTS, CB = G > 2 ? 8 : 16;     // of a warp, and at a time
-    int i = 0, x = 0, n = 0;                       // units, products, tiles
+    // ---------------- sums: a key per lane, half of the rows of every other product per warp
+    const int quad = warp & 3, half = warp >> 2 & 1, group = warp >> 3, key_at = quad * 32 + lane;
+    constexpr int COLS = N / 2, CB = G > 2 ? 8 : 16;             // of a warp, and at a time
+    const uint32_t scores = tmem + half * COLS + (static_cast<uint32_t>(quad * 32) << 16);
+    const int col0 = group * N + half * COLS;      // of the row tile
+    int i = 0, n = 0;                              // units, tiles
     for (Walk<0> w(g, plan); w.left > 0 && ok; w.next_tile(), ++n) {
-      const int cb = n % NS, here = w.here();
-      ok = mbar_wait(&c_full[cb], (n / NS) & 1, status, STATUS_EPILOGUE_WAIT, 0x2a);
+      const int cb = n % NC, here = w.here();
+      ok = mbar_wait(&c_full[cb], (n / NC) & 1, status, EPILOGUE_WAIT, 0x2a);
       ok = warp_all(ok);
       if (!ok) break;
       float2 f[G];
@@ -891,62 +980,59 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&c_free[cb]);
-      const int key = w.tile * TILE + key_at;
+      // of the chunk's rows times heads those from `see` on see the key
+      const int see = (w.tile * TILE + key_at - w.ch.pos0) * g.rep, rows = w.ch.q_len * g.rep;
+      const int clear = w.tile * TILE + TILE - 1 - w.ch.pos0;      // positions from there on see all keys
       float2 total = make_float2(0.f, 0.f);
-      for (int j0 = 0; j0 < here && ok; ++j0, ++i) {
-        const int lb = i % NS, rt = row_tile(w, w.step + j0);
-        // columns whose rows see the key: those from `see` up to `rows`
-        const int see = (key - w.ch.pos0 - rt * g.per) * g.rep;
-        const int rows = min(g.per, w.ch.q_len - rt * g.per) * g.rep;
-        const bool edge = w.tile * TILE + TILE - 1 > w.ch.pos0 + rt * g.per || rows < g.per * g.rep;
-        const float* neg = reinterpret_cast<const float*>(smem + L::B_LSE + lb * TILE * 4);
+      for (int j0 = 0; j0 < here; ++j0) {
+        const int u = i + j0, lb = u % NS, x = PER * u + group, slot = x % SLOTS;
+        ok = mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x27) &&
+             mbar_wait(&l_full[lb], (u / NS) & 1, status, EPILOGUE_WAIT, 0x28);
+        ok = warp_all(ok);
+        if (!ok) break;
+        tc_fence_after();
+        const int pos = row_tile(w, w.step + j0) * g.per;          // of the tile's first row
+        const bool edge = pos < clear || pos + g.per > w.ch.q_len;
+        const int first = pos * g.rep + col0;
+        const float* neg = reinterpret_cast<const float*>(smem + L::B_LSE + lb * TILE * 4) + col0;
 #pragma unroll
-        for (int p0 = 0; p0 < PER; ++p0, ++x) {
-          const int sb = x & 1;
-          ok = mbar_wait(&s_full[sb], (x / 2) & 1, status, STATUS_EPILOGUE_WAIT, 0x27) &&
-               (p0 > 0 || mbar_wait(&l_full[lb], (i / NS) & 1, status, STATUS_EPILOGUE_WAIT, 0x28));
-          ok = warp_all(ok);
-          if (!ok) break;
-          tc_fence_after();
+        for (int k = 0; k < COLS; k += CB) {
+          uint32_t raw[G][CB];
 #pragma unroll
-          for (int c0 = 0; c0 < COLS; c0 += CB) {
-            const int col0 = part * COLS + c0;
-            uint32_t raw[G][CB];
-#pragma unroll
-            for (int c = 0; c < G; ++c) tmem_ld_rows(tmem + 256 * sb + c * N + col0 + lane_addr, raw[c]);
-            tc_wait_ld();
-            if (c0 + CB == COLS) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&s_free[sb]);
-            }
-            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int j = 0; j < CB; j += 4) {
-              const float4 v = *reinterpret_cast<const float4*>(neg + p0 * N + col0 + j);
-              float2 y[2] = {make_float2(v.x, v.y), make_float2(v.z, v.w)};
-#pragma unroll
-              for (int p = 0; p < 2; ++p) {
-#pragma unroll
-                for (int c = 0; c < G; ++c)
-                  y[p] = fma2(pair_at(raw[c][j + 2 * p], raw[c][j + 2 * p + 1]), f[c], y[p]);
-                y[p] = make_float2(ex2(y[p].x), ex2(y[p].y));
-                if (edge) {
-                  const int col = p0 * N + col0 + j + 2 * p;
-                  if (col < see || col >= rows) y[p].x = 0.f;
-                  if (col + 1 < see || col + 1 >= rows) y[p].y = 0.f;
-                }
-                sum = add2(sum, y[p]);
-              }
-            }
-            total = add2(total, sum);
+          for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
+          tc_wait_ld();
+          if (k + CB == COLS) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[slot]);
           }
+          float2 sum = make_float2(0.f, 0.f);      // of these columns: short chains of sums
+#pragma unroll
+          for (int j = 0; j < CB; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(neg + k + j);
+            float2 y[2] = {make_float2(v.x, v.y), make_float2(v.z, v.w)};
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+#pragma unroll
+              for (int c = 0; c < G; ++c)
+                y[p] = fma2(pair_at(raw[c][j + 2 * p], raw[c][j + 2 * p + 1]), f[c], y[p]);
+              y[p] = make_float2(ex2(y[p].x), ex2(y[p].y));
+              if (edge) {
+                const int row = first + k + j + 2 * p;
+                if (row < see || row >= rows) y[p].x = 0.f;
+                if (row + 1 < see || row + 1 >= rows) y[p].y = 0.f;
+              }
+              sum = add2(sum, y[p]);
+            }
+          }
+          total = add2(total, sum);
         }
         __syncwarp();
-        if (ok && lane == 0) mbar_arrive(&l_free[lb]);
+        if (lane == 0) mbar_arrive(&l_free[lb]);
       }
       if (!ok) break;
-      parts[(static_cast<size_t>(w.index + blockIdx.x) * KEY_PARTS + part) * TILE + key_at] =
+      i += here;
+      parts[(static_cast<size_t>(w.index + blockIdx.x) * KEY_PARTS + group * 2 + half) * TILE + key_at] =
           total.x + total.y;
       if (tid == 0) {
         if (w.step == 0) span_out[2 * w.index] = blockIdx.x;
@@ -1025,6 +1111,15 @@ static int launch(const __half* q, const Geometry& g, const int8_t* kc, const __
           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return -3;
+  CUtensorMap tk;                                  // the cache as [slots][heads][D] bytes
+  cuuint64_t k_dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(g.kvh),
+                          static_cast<cuuint64_t>(g.num_pages) * 128};
+  cuuint64_t k_strides[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(g.kvh) * D};
+  cuuint32_t k_box[3] = {static_cast<cuuint32_t>(D), 1, static_cast<cuuint32_t>(L::RK)};
+  if (enc(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(kc), k_dims, k_strides, k_box, estr,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return -3;
   static const int slot[2] = {runtime_new_slot(), runtime_new_slot()};
   if (const int e = runtime_allow_smem(slot[0], stats_kernel<D>, L::A_TOTAL)) return e;
   if (const int e = runtime_allow_smem(slot[1], sums_kernel<D>, L::B_TOTAL)) return e;
@@ -1034,9 +1129,9 @@ static int launch(const __half* q, const Geometry& g, const int8_t* kc, const __
   int* row_span = reinterpret_cast<int*>(parts + (b.key_tiles + CTAS) * KEY_PARTS * TILE);
   int* key_span = row_span + 2 * b.row_tiles;
   const int ctas = ctas_for(b.units);
-  launch_early(stats_kernel<D>, dim3(ctas), THREADS, L::A_TOTAL, stream, tq, g, kc, ks, lse, row_span,
+  launch_early(stats_kernel<D>, dim3(ctas), THREADS, L::A_TOTAL, stream, tq, tk, g, ks, lse, row_span,
                runtime_status_ptr());
-  launch_early(sums_kernel<D>, dim3(ctas), THREADS, L::B_TOTAL, stream, tq, g, kc, ks,
+  launch_early(sums_kernel<D>, dim3(ctas), THREADS, L::B_TOTAL, stream, tq, tk, g, ks,
                static_cast<const float*>(lse), static_cast<const int*>(row_span), parts, key_span,
                runtime_status_ptr());
   launch_early(add_kernel, dim3((g.limit + TILE - 1) / TILE, g.kvh, g.n_chunks), TILE, 0, stream, g,
@@ -1073,6 +1168,7 @@ extern "C" int orinfer_prefill_weights(const __half* q, const int* chunks, int n
     return -1;
   if (limit > max_pages * 128LL) return -1;
   const kw::Bounds b = kw::bounds(n_chunks, max_q_len, kvh, qh / kvh, limit);
+  if (num_pages <= 0 || num_pages > (1 << 24)) return -1;
   if (b.units > 0x3fffffffLL || b.key_tiles > 0x3fffffffLL) return -1;
   if (runtime_ensure_init() != cudaSuccess) return -2;
   kw::Geometry g;
