@@ -18,6 +18,8 @@
 // had at place (tile + CTA) of a list, which is nobody else's; the tile's first and last CTA are noted.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "api.h"
 #include "common.cuh"
 #include "tma.h"
@@ -27,15 +29,18 @@ namespace kw {
 
 constexpr int TILE = 128;                        // rows of a tile: positions x query heads; keys of a tile
 constexpr int MAX_CHUNKS = 512;
-constexpr int EP_WARPS = 16, EP_GROUP = 8;       // softmax or sums: two groups, a product each in turn
+// Softmax or sums: two groups, a product each in turn, of which a warp has 32 lanes and half of the columns.
+// Whoever waits on a barrier does so for each of its phases: one that came for every other one could not
+// tell them apart.
+constexpr int EP_WARPS = 16, EP_GROUP = 8, PARTS = 4;
+constexpr int GROUPS = EP_WARPS / EP_GROUP;
 constexpr int DQ_WARPS = 8;                      // INT8 to FP16
 constexpr int AUX_WARPS = 2;                     // scales or rows' lse, in turn
 constexpr int AUX_WARP = EP_WARPS + DQ_WARPS, MMA_WARP = AUX_WARP + AUX_WARPS;
 constexpr int TMA_WARP = MMA_WARP + 1, THREADS = (TMA_WARP + 1) * 32;
 constexpr int CTAS = 148;
 constexpr int NS = 4;                            // places of scales, or of rows' lse
-constexpr int ROW_PARTS = 2, KEY_PARTS = 4;      // warps that share a row's keys, or a key's rows
-constexpr float LEAD = 1.1529215046068470e18f;   // 2^60: weights under a reference that has to move
+constexpr float FAR = 1.1529215046068470e18f;    // 2^60: weights under a reference that has to move
 
 struct Chunk {            // of one request
   int row_start;          // first packed row
@@ -67,20 +72,20 @@ struct Geometry {
   }
 };
 
-// Tiles of a chunk and steps of a tile.  KT keys to a step of a row tile; 0: key tiles, a step is a row
-// tile, the last ones of the chunk.
-template <int KT>
+// Tiles of a chunk and steps of a tile.  KT keys to a step of NT neighbouring row tiles; 0: key tiles, a
+// step is a row tile, from the first one that sees the key tile on.
+template <int KT, int NT = 1>
 struct Order {
-  __device__ static int row_tiles(const Geometry& g, const Chunk& ch) {
-    return (ch.q_len + g.per - 1) / g.per;
-  }
   __device__ static int tiles(const Geometry& g, const Chunk& ch) {
     if (ch.q_len <= 0) return 0;
-    return KT ? row_tiles(g, ch) : (ch.pos0 + ch.q_len + TILE - 1) / TILE;
+    return KT ? (ch.q_len + NT * g.per - 1) / (NT * g.per) : (ch.pos0 + ch.q_len + TILE - 1) / TILE;
+  }
+  __device__ static int first(const Geometry& g, const Chunk& ch, int tile) {
+    return KT ? 0 : max(tile * TILE - ch.pos0, 0) / g.per;
   }
   __device__ static int steps(const Geometry& g, const Chunk& ch, int tile) {
-    if (KT) return (ch.pos0 + min((tile + 1) * g.per, ch.q_len) + (KT ? KT : 1) - 1) / (KT ? KT : 1);
-    return row_tiles(g, ch) - max(tile * TILE - ch.pos0, 0) / g.per;
+    if (KT) return (ch.pos0 + min((tile + 1) * NT * g.per, ch.q_len) + KT - 1) / (KT ? KT : 1);
+    return (ch.q_len + g.per - 1) / g.per - first(g, ch, tile);
   }
 };
 
@@ -88,16 +93,16 @@ struct Order {
 struct Plan {
   int units[MAX_CHUNKS], tiles[MAX_CHUNKS];
 };
-template <int KT>
+template <int KT, int NT = 1>
 __device__ __forceinline__ void make_plan(Plan& plan, const Geometry& g, int* status) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int c = warp; c < g.n_chunks; c += THREADS / 32) {
     const Chunk ch = g.at(c);
     if (ch.q_len == 0 && blockIdx.x == 0 && lane == 0 && g.chunks[c].q_len != 0)
       report_status(status, STATUS_BAD_INDEX, 0x70);
-    const int tiles = Order<KT>::tiles(g, ch);
+    const int tiles = Order<KT, NT>::tiles(g, ch);
     int sum = 0;
-    for (int t = lane; t < tiles; t += 32) sum += Order<KT>::steps(g, ch, t);
+    for (int t = lane; t < tiles; t += 32) sum += Order<KT, NT>::steps(g, ch, t);
     sum = __reduce_add_sync(0xffffffffu, sum);
     if (lane == 0) {
       plan.units[c] = sum;
@@ -107,12 +112,13 @@ __device__ __forceinline__ void make_plan(Plan& plan, const Geometry& g, int* st
 }
 
 // A CTA's walk over its units, tile by tile.  All warps have one, a warp together.
-template <int KT>
+template <int KT, int NT = 1>
 struct Walk {
   const Geometry& g;
   const Plan& plan;
   Chunk ch;
-  int c, h, tile, step, steps, left, index;      // index: of the tile, among all chunks' and heads'
+  int c, h, tile, step, steps, left, first;      // first: the tile's first row tile (of key tiles)
+  int index;                                     // of the tile, among all chunks' and heads'
   __device__ Walk(const Geometry& geo, const Plan& p) : g(geo), plan(p) {
     const int lane = threadIdx.x & 31;
     int total = 0;
@@ -134,7 +140,7 @@ struct Walk {
     index += h * plan.tiles[c];
     ch = g.at(c);
     for (int t0 = 0;; t0 += 32) {                // the tile in which it lies, 32 at a time
-      const int n = t0 + lane < plan.tiles[c] ? Order<KT>::steps(g, ch, t0 + lane) : 0;
+      const int n = t0 + lane < plan.tiles[c] ? Order<KT, NT>::steps(g, ch, t0 + lane) : 0;
       int before = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -152,6 +158,7 @@ struct Walk {
       at -= __shfl_sync(0xffffffffu, before, 31);
     }
     index += tile;
+    first = Order<KT, NT>::first(g, ch, tile);
   }
   __device__ int here() const { return min(steps - step, left); }        // units of this tile
   __device__ void next_tile() {
@@ -167,13 +174,14 @@ struct Walk {
         ch = g.at(c);
       }
     }
-    steps = Order<KT>::steps(g, ch, tile);
+    steps = Order<KT, NT>::steps(g, ch, tile);
+    first = Order<KT, NT>::first(g, ch, tile);
   }
 };
 // The same unit by unit, for roles that go ahead of the others.
-template <int KT>
+template <int KT, int NT = 1>
 struct Units {
-  Walk<KT> w;
+  Walk<KT, NT> w;
   int i;                                         // of the tile's
   __device__ Units(const Geometry& g, const Plan& p) : w(g, p), i(0) {}
   __device__ bool more() const { return w.left > 0; }
@@ -193,16 +201,17 @@ struct Shape {
   static constexpr int G = D / 64;               // scale groups of a key
   static constexpr int QSUB = TILE * 128;        // bytes of 64 channels of a tile of 128 rows or keys
   static constexpr int Q_BYTES = G * QSUB;
-  static constexpr int N = 64;                   // columns of a product
+  static constexpr int N = D > 128 ? 64 : 128;   // columns of a product
   static constexpr int SLOT = G * N;             // and of TMEM, a group of channels after the other
-  static constexpr int SLOTS = D > 128 ? 2 : 4;  // products that have a place
+  static constexpr int SLOTS = 512 / SLOT;       // products that have a place
   static constexpr int RK = D > 128 ? 64 : 128;  // keys that are copied at a time
   static constexpr int R_BYTES = RK * D;
   // ---- stats_kernel
   static constexpr int KT = RK;                  // keys of a step
+  static constexpr int NT = D > 128 ? 1 : 2;     // row tiles of a step: converted keys serve them all
   static constexpr int KSUB = KT * 128, K_BYTES = G * KSUB, PER_A = KT / N;
-  static constexpr int NQ = D > 128 ? 1 : 2, NK = 3, NR = 3;   // buffers of queries, keys, raw keys
-  static constexpr int A_K = NQ * Q_BYTES;
+  static constexpr int NQ = 1, NK = D > 128 ? 3 : 2, NR = 3;   // buffers of queries, keys, raw keys
+  static constexpr int A_K = NQ * NT * Q_BYTES;
   static constexpr int A_R = A_K + NK * K_BYTES;
   static constexpr int A_SCALE = A_R + NR * R_BYTES;
   static constexpr int SCALES = KT * G * 4;
@@ -221,7 +230,7 @@ struct Shape {
   static constexpr int B_TOTAL = B_BAR + 512 + 1024;
   static_assert(A_TOTAL + sizeof(Plan) <= 227 * 1024 && B_TOTAL + sizeof(Plan) <= 227 * 1024,
                 "exceeds the shared memory of one CTA");
-  static_assert(SLOT * SLOTS <= 512, "exceeds tensor memory");
+  static_assert(SLOTS % GROUPS == 0, "a slot is always the same group's");
 };
 
 constexpr int TMA_WAIT = STATUS_TMA_WAIT, MMA_WAIT = STATUS_MMA_WAIT;
@@ -271,26 +280,6 @@ __device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t tmem_d, uint32_
       "mov.b64 b, {%2, %6};\n\t"
       "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(tmem_d),
       "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(leader), "r"(DESC_HIGH)
-      : "memory");
-}
-// Sixteen TMEM lanes as fragments: per eight columns lane (g = lane / 4, t = lane % 4) holds columns 2t
-// and 2t + 1 of rows g and g + 8.
-__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {       // 32 columns
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[8]) {        // 16 columns
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7])
-      : "r"(taddr)
       : "memory");
 }
 // 32 lanes, a row each
@@ -381,14 +370,15 @@ __device__ __forceinline__ void clear_tails(unsigned char* q, int tiles, int row
   fence_proxy_async();
 }
 
-// lse: [row tiles + CTAs][2][128], log2 of a part's sum of weights; span: a row tile's first and last CTA.
+// lse: [tiles + CTAs][2 groups][2 halves][128], log2 of the sum of weights that a group has seen in half of
+// the columns, of the tile's row tile (group % NT); span: a tile's first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
     const Geometry g, const __half* ks, float* lse, int* span, int* status) {
   using L = Shape<D>;
   constexpr int G = L::G, KT = L::KT, N = L::N, PER = L::PER_A, NQ = L::NQ, NK = L::NK, NR = L::NR;
-  constexpr int SLOTS = L::SLOTS;
+  constexpr int SLOTS = L::SLOTS, NT = L::NT;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ Plan plan;
@@ -424,15 +414,15 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     }
     for (int b = 0; b < NS; ++b) {
       mbar_init(&c_full[b], 1);
-      mbar_init(&c_free[b], EP_GROUP * PER);
+      mbar_init(&c_free[b], EP_GROUP * PER * NT);
     }
     mbar_fence_init();
     prefetch_tmap(&tmap_q);
     prefetch_tmap(&tmap_k);
   }
-  if (g.per * g.rep < TILE) clear_tails(smem, NQ * G, g.per * g.rep);
+  if (g.per * g.rep < TILE) clear_tails(smem, NQ * NT * G, g.per * g.rep);
   grid_wait();
-  make_plan<KT>(plan, g, status);
+  make_plan<KT, NT>(plan, g, status);
   if (warp == MMA_WARP) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -445,7 +435,7 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
   bool ok = true;
 
   if (warp == TMA_WARP) {
-    Units<KT> u(g, plan);
+    Units<KT, NT> u(g, plan);
     if (lane == 0) {
       int n = 0, i = 0;                            // tiles, units
       Ahead next;
@@ -455,10 +445,10 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
         if (fresh) {
           const int b = n % NQ;
           if (n >= NQ && !mbar_wait(&q_free[b], (n / NQ - 1) & 1, status, TMA_WAIT, 0x10)) break;
-          mbar_expect_tx(&q_full[b], static_cast<uint32_t>(G) * 64 * 2 * g.rep * g.per);
-          for (int s = 0; s < G; ++s)
-            tma_load_3d(smem + b * L::Q_BYTES + s * L::QSUB, &tmap_q, &q_full[b], s * 64, u.w.h * g.rep,
-                        u.w.ch.row_start + u.w.tile * g.per);
+          mbar_expect_tx(&q_full[b], static_cast<uint32_t>(NT * G) * 64 * 2 * g.rep * g.per);
+          for (int s = 0; s < NT * G; ++s)         // (rows behind the last are zeros)
+            tma_load_3d(smem + (b * NT * G + s) * L::QSUB, &tmap_q, &q_full[b], s % G * 64, u.w.h * g.rep,
+                        u.w.ch.row_start + (u.w.tile * NT + s / G) * g.per);
           ++n;
         }
         const int b = i % NR, h = next.h, row = next.row(g, status), tile = u.w.index;
@@ -481,25 +471,26 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     const uint32_t qd = desc_low(smem);
     const uint32_t kd = desc_low(smem + L::A_K);
     int n = 0, i = 0, x = 0;                       // tiles, units, products
-    for (Walk<KT> w(g, plan); warp_same(w.left) > 0 && ok; w.next_tile(), ++n) {
+    for (Walk<KT, NT> w(g, plan); warp_same(w.left) > 0 && ok; w.next_tile(), ++n) {
       const int last = i + warp_same(w.here());
       ok = warp_all(mbar_wait(&q_full[n % NQ], (n / NQ) & 1, status, MMA_WAIT, 0x14));
-      const uint32_t qb = qd + (n % NQ) * (L::Q_BYTES / 16);
+      const uint32_t qb = qd + n % NQ * NT * (L::Q_BYTES / 16);
       for (; i < last && ok; ++i) {
         const int b = i % NK;
         ok = warp_all(mbar_wait(&k_full[b], (i / NK) & 1, status, MMA_WAIT, 0x15));
-        for (int p = 0; p < PER && ok; ++p, ++x) {
+        for (int p = 0; p < PER * NT && ok; ++p, ++x) {          // by turns of the row tiles
           const int s = x % SLOTS;
           if (x >= SLOTS) ok = mbar_wait(&s_free[s], (x / SLOTS - 1) & 1, status, MMA_WAIT, 0x16);
           ok = warp_all(ok);
           tc_fence_after();
           if (!ok) break;
-          const uint32_t kb = kd + (b) * (L::K_BYTES / 16) + p * (N * 128 / 16);
+          const uint32_t kb = kd + b * (L::K_BYTES / 16) + p / NT * (N * 128 / 16);
+          const uint32_t qt = qb + p % NT * (L::Q_BYTES / 16);
 #pragma unroll
           for (int c = 0; c < G; ++c)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mma_ss(leader, tmem + L::SLOT * s + c * N, qb + (c * L::QSUB + k * 32) / 16,
+              mma_ss(leader, tmem + L::SLOT * s + c * N, qt + (c * L::QSUB + k * 32) / 16,
                      kb + (c * L::KSUB + k * 32) / 16, idesc, k != 0 ? 1u : 0u);
           tc_commit_by(leader, &s_full[s]);
         }
@@ -514,7 +505,7 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
     __half raw[KS];
     Ahead next;
-    Units<KT> u(g, plan);
+    Units<KT, NT> u(g, plan);
     auto ask = [&] {
       if (u.more()) next.ask(g, u.w.ch, u.step() * KT, u.w.h);
     };
@@ -550,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
   } else if (warp >= EP_WARPS) {
     // ---------------- keys: INT8 to FP16 integers
     constexpr int DQ = DQ_WARPS * 32, KI = L::R_BYTES / 16 / DQ;
-    const int t = tid - EP_WARPS * 32, units = max(Walk<KT>(g, plan).left, 0);
+    const int t = tid - EP_WARPS * 32, units = max(Walk<KT, NT>(g, plan).left, 0);
     for (int i = 0; i < units; ++i) {
       const int b = i % NK, r = i % NR;
       ok = mbar_wait(&r_full[r], (i / NR) & 1, status, DECODE_WAIT, 0x18) &&
@@ -566,127 +557,122 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       }
     }
   } else {
-    // ---------------- sixteen rows per warp, every other product; a thread holds columns 2 qt and 2 qt + 1
-    // of every eight, of rows qg and qg + 8, and has a reference of its own for each
-    const int qg = lane >> 2, qt = lane & 3, row0 = (warp & 3) * 32 + (warp >> 2 & 1) * 16;
-    constexpr int CH = G > 2 ? 16 : 32;          // columns at a time
-    const int group = warp >> 3;
-    const uint32_t scores = tmem + (static_cast<uint32_t>(row0) << 16);
+    // ---------------- a row per lane; a group has a row tile, or every other unit
+    constexpr int CB = G > 1 ? 8 : 16, COLS = N / 2;             // columns at a time, and of a warp
+    constexpr bool EACH = PER * NT == GROUPS;
+    static_assert(EACH || PER * NT == 1, "products of a unit");
+    const int group = warp >> 3, half = warp >> 2 & 1, at = (warp & 3) * 32 + lane;
+    const uint32_t scores = tmem + half * COLS + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     int i = 0;
-    for (Walk<KT> w(g, plan); w.left > 0 && ok; w.next_tile()) {
-      int sees[2];                               // keys that its rows see
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int p = w.tile * g.per + (row0 + qg + 8 * r) / g.rep;
-        sees[r] = (row0 + qg + 8 * r) < g.per * g.rep && p < w.ch.q_len ? w.ch.pos0 + p + 1 : 0;
-      }
-      const int all_see = __reduce_min_sync(0xffffffffu, min(sees[0], sees[1]));
-      float m_ref[2] = {0.f, 0.f};
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    for (Walk<KT, NT> w(g, plan); w.left > 0 && ok; w.next_tile()) {
+      const int p = (w.tile * NT + group % NT) * g.per + at / g.rep;
+      // keys that the row sees, and those that all rows of the warp see
+      const int sees = at < g.per * g.rep && p < w.ch.q_len ? w.ch.pos0 + p + 1 : 0;
+      const int all_see = __reduce_min_sync(0xffffffffu, sees);
+      const bool any = __any_sync(0xffffffffu, sees > 0);
+      float m_ref = 0.f;
+      float2 sum = make_float2(0.f, 0.f);
       const int n = w.here();
       bool start = true;
-      // every unit where it has two products, else every other one
-      for (int j0 = PER > 1 || (i & 1) == group ? 0 : 1; j0 < n; j0 += PER > 1 ? 1 : 2) {
-        const int u = i + j0, cb = u % NS, p0 = PER > 1 ? group * N : 0;
-        const int x = PER > 1 ? 2 * u + group : u, slot = x % SLOTS;
-        const int key0 = (w.step + j0) * KT + p0;
-        ok = mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x1a) &&
-             mbar_wait(&c_full[cb], (u / NS) & 1, status, EPILOGUE_WAIT, 0x1b);
-        ok = warp_all(ok);
+      for (int j0 = EACH ? 0 : (group - i) & (GROUPS - 1); j0 < n; j0 += EACH ? 1 : GROUPS) {
+        const int u = i + j0, cb = u % NS;
+        const int x = EACH ? u * GROUPS + group : u, slot = x % SLOTS;
+        const int key0 = (w.step + j0) * KT + half * COLS;
+        ok = warp_all(mbar_wait(&c_full[cb], (u / NS) & 1, status, EPILOGUE_WAIT, 0x1b) &&
+                      mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x1a));
         if (!ok) break;
         tc_fence_after();
-        const float2* sk =
-            reinterpret_cast<const float2*>(smem + L::A_SCALE + cb * L::SCALES) + (p0 / 2 + qt) * G;
+        const float2* scales =
+            reinterpret_cast<const float2*>(smem + L::A_SCALE + cb * L::SCALES) + half * COLS / 2 * G;
+        // The columns, CB at a time, to `each` as scores less `ref`: the next ones come meanwhile.
+        auto columns = [&](float ref, auto each) {
+          uint32_t raw[G][CB];
+          auto ask = [&](int k) {
 #pragma unroll
-        for (int k = 0; k < N; k += CH) {
-          uint32_t raw[G][CH / 2];
-#pragma unroll
-          for (int c = 0; c < G; ++c) tmem_ld_frag(scores + L::SLOT * slot + c * N + k, raw[c]);
-          tc_wait_ld();
-          if (k + CH == N) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[slot]);
-          }
-          float2 x[2][CH / 8];
-#pragma unroll
-          for (int j = 0; j < CH / 8; ++j) {
-            const float2* s = sk + (k / 2 + 4 * j) * G;
-            float2 f[G];
-            if (G == 1) {
-              f[0] = s[0];
-            } else {
-#pragma unroll
-              for (int c = 0; c < G; c += 2) {
-                const float4 v = *reinterpret_cast<const float4*>(s + c);
-                f[c] = make_float2(v.x, v.y);
-                f[(c + 1) % G] = make_float2(v.z, v.w);
-              }
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              x[r][j] = make_float2(-m_ref[r], -m_ref[r]);
-#pragma unroll
-              for (int c = 0; c < G; ++c)
-                x[r][j] = fma2(pair_at(raw[c][4 * j + 2 * r], raw[c][4 * j + 2 * r + 1]), f[c], x[r][j]);
-            }
-          }
-          if (all_see < key0 + k + CH) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-              for (int j = 0; j < CH / 8; ++j) {
-                const int key = key0 + k + 8 * j + 2 * qt;
-                if (key >= sees[r]) x[r][j].x = -INFINITY;
-                if (key + 1 >= sees[r]) x[r][j].y = -INFINITY;
-              }
-          }
-          auto weights = [&](int r) {              // of these columns: short chains of sums
-            float2 v = make_float2(ex2(x[r][0].x), ex2(x[r][0].y));
-#pragma unroll
-            for (int j = 1; j < CH / 8; ++j) v = add2(v, make_float2(ex2(x[r][j].x), ex2(x[r][j].y)));
-            return v;
+            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
           };
-          float2 more[2] = {weights(0), weights(1)};
-          // The reference is the maximum of the thread's first columns, and moves where weights are far
-          // above 1: no maximum is taken but then.  (A row that sees none of the first sees none behind.)
-          if (start || fmaxf(more[0].x + more[0].y, more[1].x + more[1].y) > LEAD) {
+          ask(0);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              float top = fmaxf(x[r][0].x, x[r][0].y);
+          for (int k = 0; k < COLS; k += CB) {
+            tc_wait_ld();
+            float2 y[CB / 2];
 #pragma unroll
-              for (int j = 1; j < CH / 8; ++j) top = fmaxf(top, fmaxf(x[r][j].x, x[r][j].y));
-              const float by = top == -INFINITY ? 0.f : start ? top : fmaxf(top, 0.f);
-              const float f = start ? 0.f : ex2(-by);
-              sum[r] = mul2(sum[r], make_float2(f, f));
-              m_ref[r] += by;
+            for (int j = 0; j < CB / 2; ++j) {
+              const float2* f = scales + (k / 2 + j) * G;
+              float2 fg[G];
+              if (G == 1) {
+                fg[0] = f[0];
+              } else {
 #pragma unroll
-              for (int j = 0; j < CH / 8; ++j) x[r][j] = add2(x[r][j], make_float2(-by, -by));
-              more[r] = weights(r);
+                for (int c = 0; c < G; c += 2) {
+                  const float4 v = *reinterpret_cast<const float4*>(f + c);
+                  fg[c] = make_float2(v.x, v.y);
+                  fg[(c + 1) % G] = make_float2(v.z, v.w);
+                }
+              }
+              y[j] = make_float2(-ref, -ref);
+#pragma unroll
+              for (int c = 0; c < G; ++c) y[j] = fma2(pair_at(raw[c][2 * j], raw[c][2 * j + 1]), fg[c], y[j]);
             }
-            start = false;
+            if (k + CB < COLS) ask(k + CB);
+            each(k, y);
           }
+        };
+        auto weights = [&] {                     // chains of sums of a quarter of the columns
+          float2 v[4];
+          columns(m_ref, [&](int k, float2(&y)[CB / 2]) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r) sum[r] = add2(sum[r], more[r]);
+            for (int j = 0; j < CB / 2; ++j) {
+              const float2 e = make_float2(ex2(y[j].x), ex2(y[j].y));
+              v[j & 3] = k == 0 && j < 4 ? e : add2(v[j & 3], e);
+            }
+          });
+          return add2(add2(v[0], v[1]), add2(v[2], v[3]));
+        };
+        // The reference is the maximum of the row's first columns, and moves where weights are far above
+        // 1: no maximum is taken but then, and where some row of the warp does not see all of the columns.
+        // (A row that sees none of the first sees none behind them.)
+        bool plain = !start && all_see >= key0 + COLS;
+        float2 more = make_float2(0.f, 0.f);
+        if (plain) {
+          more = weights();
+          plain = !__any_sync(0xffffffffu, more.x + more.y > FAR);
         }
+        if (!plain && any) {
+          float top = -INFINITY;
+          columns(0.f, [&](int k, float2(&y)[CB / 2]) {
+#pragma unroll
+            for (int j = 0; j < CB / 2; ++j) {
+              if (key0 + k + 2 * j < sees) top = fmaxf(top, y[j].x);
+              if (key0 + k + 2 * j + 1 < sees) top = fmaxf(top, y[j].y);
+            }
+          });
+          const float now = start ? (top == -INFINITY ? 0.f : top) : fmaxf(m_ref, top);
+          const float f = start ? 0.f : ex2(m_ref - now);
+          sum = mul2(sum, make_float2(f, f));
+          m_ref = now;
+          start = false;
+          more = make_float2(0.f, 0.f);
+          columns(m_ref, [&](int k, float2(&y)[CB / 2]) {
+#pragma unroll
+            for (int j = 0; j < CB / 2; ++j)
+              more = add2(more, make_float2(key0 + k + 2 * j < sees ? ex2(y[j].x) : 0.f,
+                                            key0 + k + 2 * j + 1 < sees ? ex2(y[j].y) : 0.f));
+          });
+        }
+        sum = add2(sum, more);
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&c_free[cb]);
+        if (lane == 0) {
+          mbar_arrive(&s_free[slot]);
+          mbar_arrive(&c_free[cb]);
+        }
       }
       if (!ok) break;
       i += n;
-      const size_t place = static_cast<size_t>(w.index + blockIdx.x) * ROW_PARTS + group;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float l = sum[r].x + sum[r].y, m = l == 0.f ? -INFINITY : m_ref[r];
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-          const float top = fmaxf(m, m2);
-          l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + (m2 == -INFINITY ? 0.f : l2 * ex2(m2 - top));
-          m = top;
-        }
-        if (qt == 0) lse[place * TILE + row0 + qg + 8 * r] = m + log2f(l);
-      }
+      const float l = sum.x + sum.y;
+      lse[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + group * 2 + half) * TILE + at] =
+          l == 0.f ? -INFINITY : m_ref + log2f(l);
       if (tid == 0) {
         if (w.step == 0) span[2 * w.index] = blockIdx.x;
         if (w.step + n == w.steps) span[2 * w.index + 1] = blockIdx.x;
@@ -698,8 +684,8 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-// parts: [key tiles + CTAs][4][128], sums over a quarter of the rows of its units each; span_out: a key
-// tile's first and last CTA.
+// parts: [key tiles + CTAs][2 groups][2 halves][128], sums of what they have seen; span_out: a key tile's
+// first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -708,6 +694,8 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
   using L = Shape<D>;
   constexpr int G = L::G, N = L::N, PER = L::PER_B, BQ = L::BQ, BK = L::BK, BR = L::BR, NC = L::NC;
   constexpr int SLOTS = L::SLOTS, HALVES = TILE / L::RK;         // copies of a tile's keys
+  constexpr int NT = L::NT;
+  static_assert(PER == 1 || PER == GROUPS, "every other unit for a group, or its part of each");
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ Plan plan;
@@ -745,7 +733,7 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     }
     for (int b = 0; b < NS; ++b) {
       mbar_init(&l_full[b], 1);
-      mbar_init(&l_free[b], EP_WARPS);
+      mbar_init(&l_free[b], EP_GROUP * PER);
     }
     for (int b = 0; b < NC; ++b) {
       mbar_init(&c_full[b], DQ_WARPS);
@@ -768,10 +756,6 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
   const uint32_t tmem = warp_same(*tmem_slot);
   grid_release();
   bool ok = true;
-  // row tile of a unit: the tile's steps are the last ones of the chunk
-  auto row_tile = [&](const Walk<0>& w, int step) {
-    return Order<0>::row_tiles(g, w.ch) - w.steps + step;
-  };
 
   if (warp == TMA_WARP) {
     Units<0> u(g, plan);
@@ -783,7 +767,7 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
         mbar_expect_tx(&q_full[b], static_cast<uint32_t>(G) * 64 * 2 * g.rep * g.per);
         for (int s = 0; s < G; ++s)
           tma_load_3d(smem + L::B_Q + b * L::Q_BYTES + s * L::QSUB, &tmap_q, &q_full[b], s * 64,
-                      u.w.h * g.rep, u.w.ch.row_start + row_tile(u.w, u.step()) * g.per);
+                      u.w.h * g.rep, u.w.ch.row_start + (u.w.first + u.step()) * g.per);
       }
       for (int i = max(n - BQ, 0); i < n; ++i)     // our copies have landed before exit
         mbar_wait(&q_full[i % BQ], (i / BQ) & 1, status, TMA_WAIT, 0x21);
@@ -797,7 +781,7 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     for (Walk<0> w(g, plan); warp_same(w.left) > 0 && ok; w.next_tile(), ++n) {
       const int last = i + warp_same(w.here());
       ok = warp_all(mbar_wait(&k_full[n % BK], (n / BK) & 1, status, MMA_WAIT, 0x22));
-      const uint32_t kb = kd + (n % BK) * (L::T_BYTES / 16);
+      const uint32_t kb = kd + n % BK * (L::T_BYTES / 16);
       for (; i < last && ok; ++i) {
         const int b = i % BQ;
         ok = warp_all(mbar_wait(&q_full[b], (i / BQ) & 1, status, MMA_WAIT, 0x23));
@@ -807,7 +791,7 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
           ok = warp_all(ok);
           tc_fence_after();
           if (!ok) break;
-          const uint32_t qb = qd + (b) * (L::Q_BYTES / 16) + p * (N * 128 / 16);
+          const uint32_t qb = qd + b * (L::Q_BYTES / 16) + p * (N * 128 / 16);
 #pragma unroll
           for (int c = 0; c < G; ++c)
 #pragma unroll
@@ -824,17 +808,15 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
   } else if (warp >= AUX_WARP) {
     // ---------------- the rows' lse, of the parts that a tile's CTAs have left; four rows a lane.  A row
     // that is none gets one that leaves no weight.  A unit's CTAs are asked for a turn before.
-    int base_c = 0, base = 0;                      // row tiles of the chunks before
+    int base_c = 0, base = 0;                      // tiles of rows of the chunks before
     Units<0> u(g, plan);
-    int index = 0, rows = 0, first = 0, last = 0;
+    int index = 0, mate = 0, rows = 0, first = 0, last = 0;
     auto ask = [&] {
       if (!u.more()) return;
-      for (; base_c < u.w.c; ++base_c) {
-        const Chunk ch = g.at(base_c);
-        if (ch.q_len > 0) base += Order<0>::row_tiles(g, ch) * g.kvh;
-      }
-      const int rt = row_tile(u.w, u.step());
-      index = base + u.w.h * Order<0>::row_tiles(g, u.w.ch) + rt;
+      for (; base_c < u.w.c; ++base_c) base += Order<1, NT>::tiles(g, g.at(base_c)) * g.kvh;
+      const int rt = u.w.first + u.step();
+      index = base + u.w.h * Order<1, NT>::tiles(g, u.w.ch) + rt / NT;
+      mate = rt % NT;
       rows = min(g.per, u.w.ch.q_len - rt * g.per) * g.rep;
       first = span[2 * index];
       last = span[2 * index + 1];
@@ -845,24 +827,26 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     for (int n = mine; n < units; n += AUX_WARPS) {
       const int b = n % NS, live = rows;           // (see span_of)
       const int lo = max(0, min(first, CTAS - 1)), hi = max(lo, min(last, CTAS - 1));
-      auto part = [&, at = index](int x) {
-        return *reinterpret_cast<const float4*>(lse + (static_cast<size_t>(at + lo) * ROW_PARTS + x) * TILE +
-                                                4 * lane);
+      // what the CTAs' groups have left of the row tile
+      constexpr int EACH = PARTS / NT;
+      const int count = (hi - lo + 1) * EACH;
+      auto part = [&, from = (static_cast<size_t>(index + lo) * PARTS + mate * EACH) * TILE + 4 * lane](int x) {
+        const size_t at = static_cast<size_t>(x / EACH * PARTS + x % EACH) * TILE;
+        return x < count ? *reinterpret_cast<const float4*>(lse + from + at)
+                         : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       };
-      float4 m = part(0), l = make_float4(1.f, 1.f, 1.f, 1.f);
       auto join = [](float& m, float& l, float x) {
         const float top = fmaxf(m, x);
         l = (m == -INFINITY ? 0.f : l * exp2f(m - top)) + (x == -INFINITY ? 0.f : exp2f(x - top));
         m = top;
       };
-      constexpr int BATCH = 3;
-      for (int x = 1; x < (hi - lo + 1) * ROW_PARTS; x += BATCH) {
+      constexpr int BATCH = 4;
+      float4 m = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), l = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int x = 0; x < count; x += BATCH) {
         float4 p[BATCH];
 #pragma unroll
-        for (int k = 0; k < BATCH; ++k)
-          p[k] = x + k < (hi - lo + 1) * ROW_PARTS
-                     ? part(x + k) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (x == 1) {
+        for (int k = 0; k < BATCH; ++k) p[k] = part(x + k);
+        if (x == 0) {
           u.skip(AUX_WARPS);
           ask();
         }
@@ -961,16 +945,15 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
         mbar_wait(&r_full[i % BR], (i / BR) & 1, status, TMA_WAIT, 0x2d);
     __syncwarp();
   } else {
-    // ---------------- sums: a key per lane, half of the rows of every other product per warp
-    const int quad = warp & 3, half = warp >> 2 & 1, group = warp >> 3, key_at = quad * 32 + lane;
-    constexpr int COLS = N / 2, CB = G > 2 ? 8 : 16;             // of a warp, and at a time
-    const uint32_t scores = tmem + half * COLS + (static_cast<uint32_t>(quad * 32) << 16);
-    const int col0 = group * N + half * COLS;      // of the row tile
+    // ---------------- sums: a key per lane
+    const int group = warp >> 3, half = warp >> 2 & 1, key_at = (warp & 3) * 32 + lane;
+    constexpr int CB = G > 1 ? 8 : 16, COLS = N / 2;             // columns at a time, and of a warp
+    const int col0 = group % PER * N + half * COLS;              // of the unit
+    const uint32_t scores = tmem + half * COLS + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     int i = 0, n = 0;                              // units, tiles
     for (Walk<0> w(g, plan); w.left > 0 && ok; w.next_tile(), ++n) {
       const int cb = n % NC, here = w.here();
-      ok = mbar_wait(&c_full[cb], (n / NC) & 1, status, EPILOGUE_WAIT, 0x2a);
-      ok = warp_all(ok);
+      ok = warp_all(mbar_wait(&c_full[cb], (n / NC) & 1, status, EPILOGUE_WAIT, 0x2a));
       if (!ok) break;
       float2 f[G];
 #pragma unroll
@@ -984,56 +967,66 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       const int see = (w.tile * TILE + key_at - w.ch.pos0) * g.rep, rows = w.ch.q_len * g.rep;
       const int clear = w.tile * TILE + TILE - 1 - w.ch.pos0;      // positions from there on see all keys
       float2 total = make_float2(0.f, 0.f);
-      for (int j0 = 0; j0 < here; ++j0) {
-        const int u = i + j0, lb = u % NS, x = PER * u + group, slot = x % SLOTS;
-        ok = mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x27) &&
-             mbar_wait(&l_full[lb], (u / NS) & 1, status, EPILOGUE_WAIT, 0x28);
-        ok = warp_all(ok);
+      constexpr int EVERY = GROUPS / PER;
+      const int skip = PER > 1 ? 0 : (i ^ group) & 1, end = i + here;
+      int pos = (w.first + w.step + skip) * g.per;  // of a unit's first row
+      for (i += skip; i < end; i += EVERY, pos += EVERY * g.per) {
+        const int lb = i % NS, x = PER * i + group % PER, slot = x % SLOTS;
+        ok = warp_all(mbar_wait(&l_full[lb], (i / NS) & 1, status, EPILOGUE_WAIT, 0x28) &&
+                      mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x27));
         if (!ok) break;
         tc_fence_after();
-        const int pos = row_tile(w, w.step + j0) * g.per;          // of the tile's first row
         const bool edge = pos < clear || pos + g.per > w.ch.q_len;
         const int first = pos * g.rep + col0;
         const float* neg = reinterpret_cast<const float*>(smem + L::B_LSE + lb * TILE * 4) + col0;
-#pragma unroll
-        for (int k = 0; k < COLS; k += CB) {
+        auto weights = [&](auto masked) {
           uint32_t raw[G][CB];
+          auto ask = [&](int k) {
 #pragma unroll
-          for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
-          tc_wait_ld();
-          if (k + CB == COLS) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[slot]);
-          }
-          float2 sum = make_float2(0.f, 0.f);      // of these columns: short chains of sums
+            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
+          };
+          ask(0);
+          float2 v[4];                             // chains of sums of a quarter of the columns
 #pragma unroll
-          for (int j = 0; j < CB; j += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(neg + k + j);
-            float2 y[2] = {make_float2(v.x, v.y), make_float2(v.z, v.w)};
+          for (int k = 0; k < COLS; k += CB) {
+            tc_wait_ld();
+            float2 y[CB / 2];
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
+            for (int j = 0; j < CB / 2; j += 2) {
+              const float4 from = *reinterpret_cast<const float4*>(neg + k + 2 * j);
+              y[j] = make_float2(from.x, from.y);
+              y[j + 1] = make_float2(from.z, from.w);
 #pragma unroll
-              for (int c = 0; c < G; ++c)
-                y[p] = fma2(pair_at(raw[c][j + 2 * p], raw[c][j + 2 * p + 1]), f[c], y[p]);
-              y[p] = make_float2(ex2(y[p].x), ex2(y[p].y));
-              if (edge) {
-                const int row = first + k + j + 2 * p;
-                if (row < see || row >= rows) y[p].x = 0.f;
-                if (row + 1 < see || row + 1 >= rows) y[p].y = 0.f;
+              for (int c = 0; c < G; ++c) {
+                y[j] = fma2(pair_at(raw[c][2 * j], raw[c][2 * j + 1]), f[c], y[j]);
+                y[j + 1] = fma2(pair_at(raw[c][2 * j + 2], raw[c][2 * j + 3]), f[c], y[j + 1]);
               }
-              sum = add2(sum, y[p]);
+            }
+            if (k + CB < COLS) ask(k + CB);           // (they come while these are weighed)
+#pragma unroll
+            for (int j = 0; j < CB / 2; ++j) {
+              float2 e = make_float2(ex2(y[j].x), ex2(y[j].y));
+              if (masked) {
+                const int row = first + k + 2 * j;
+                if (row < see || row >= rows) e.x = 0.f;
+                if (row + 1 < see || row + 1 >= rows) e.y = 0.f;
+              }
+              v[j & 3] = k == 0 && j < 4 ? e : add2(v[j & 3], e);
             }
           }
-          total = add2(total, sum);
-        }
+          return add2(add2(v[0], v[1]), add2(v[2], v[3]));
+        };
+        total = add2(total, edge ? weights(std::true_type()) : weights(std::false_type()));
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&l_free[lb]);
+        if (lane == 0) {
+          mbar_arrive(&s_free[slot]);
+          mbar_arrive(&l_free[lb]);
+        }
       }
       if (!ok) break;
-      i += here;
-      parts[(static_cast<size_t>(w.index + blockIdx.x) * KEY_PARTS + group * 2 + half) * TILE + key_at] =
-          total.x + total.y;
+      i = end;
+      parts[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + group * 2 + half) * TILE + key_at] = total.x + total.y;
       if (tid == 0) {
         if (w.step == 0) span_out[2 * w.index] = blockIdx.x;
         if (w.step + here == w.steps) span_out[2 * w.index + 1] = blockIdx.x;
@@ -1066,8 +1059,8 @@ __global__ void __launch_bounds__(TILE) add_kernel(
         const int2 of = span_of(span, index);
         float sum = 0.f;
         for (int x = of.x; x <= of.y; ++x)
-          for (int part = 0; part < KEY_PARTS; ++part)
-            sum += parts[(static_cast<size_t>(index + x) * KEY_PARTS + part) * TILE + tid];
+          for (int part = 0; part < PARTS; ++part)
+            sum += parts[(static_cast<size_t>(index + x) * PARTS + part) * TILE + tid];
         total += sum;
         seen = max(seen, other.pos0 + other.q_len);
       }
@@ -1125,8 +1118,8 @@ static int launch(const __half* q, const Geometry& g, const int8_t* kc, const __
   if (const int e = runtime_allow_smem(slot[1], sums_kernel<D>, L::B_TOTAL)) return e;
   const Bounds b = bounds(g.n_chunks, g.longest, g.kvh, g.rep, g.limit);
   float* lse = work;
-  float* parts = lse + (b.row_tiles + CTAS) * ROW_PARTS * TILE;
-  int* row_span = reinterpret_cast<int*>(parts + (b.key_tiles + CTAS) * KEY_PARTS * TILE);
+  float* parts = lse + (b.row_tiles + CTAS) * PARTS * TILE;
+  int* row_span = reinterpret_cast<int*>(parts + (b.key_tiles + CTAS) * PARTS * TILE);
   int* key_span = row_span + 2 * b.row_tiles;
   const int ctas = ctas_for(b.units);
   launch_early(stats_kernel<D>, dim3(ctas), THREADS, L::A_TOTAL, stream, tq, tk, g, ks, lse, row_span,
@@ -1149,7 +1142,7 @@ extern "C" size_t orinfer_prefill_weights_work_bytes(int n_chunks, int max_q_len
                                                      int limit) {
   if (n_chunks <= 0 || rep <= 0) return 0;
   const kw::Bounds b = kw::bounds(n_chunks, max_q_len, kvh, rep, limit);
-  return ((b.row_tiles + kw::CTAS) * kw::ROW_PARTS + (b.key_tiles + kw::CTAS) * kw::KEY_PARTS) *
+  return ((b.row_tiles + kw::CTAS) * kw::PARTS + (b.key_tiles + kw::CTAS) * kw::PARTS) *
              kw::TILE * sizeof(float) +
          2 * (b.row_tiles + b.key_tiles) * sizeof(int);
 }
