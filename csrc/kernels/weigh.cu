@@ -29,16 +29,13 @@ namespace kw {
 
 constexpr int TILE = 128;                        // rows of a tile: positions x query heads; keys of a tile
 constexpr int MAX_CHUNKS = 512;
-// Softmax or sums: two groups, a product each in turn, of which a warp has 32 lanes and half of the columns.
-// Whoever waits on a barrier does so for each of its phases: one that came for every other one could not
-// tell them apart.
-constexpr int EP_WARPS = 16, EP_GROUP = 8, PARTS = 4;
-constexpr int GROUPS = EP_WARPS / EP_GROUP;
-constexpr int DQ_WARPS = 8;                      // INT8 to FP16
-constexpr int AUX_WARPS = 2;                     // scales or rows' lse, in turn
+constexpr int EP_WARPS = 8;                      // softmax or sums: 32 lanes and half of a product's columns
+constexpr int DQ_WARPS = 4;                      // INT8 to FP16
+constexpr int AUX_WARPS = 2;                     // scales, in turn
 constexpr int AUX_WARP = EP_WARPS + DQ_WARPS, MMA_WARP = AUX_WARP + AUX_WARPS;
 constexpr int TMA_WARP = MMA_WARP + 1, THREADS = (TMA_WARP + 1) * 32;
 constexpr int CTAS = 148;
+constexpr int PARTS = 2;                         // halves of a tile's columns
 constexpr int NS = 4;                            // places of scales, or of rows' lse
 constexpr float FAR = 1.1529215046068470e18f;    // 2^60: weights under a reference that has to move
 
@@ -230,7 +227,6 @@ struct Shape {
   static constexpr int B_TOTAL = B_BAR + 512 + 1024;
   static_assert(A_TOTAL + sizeof(Plan) <= 227 * 1024 && B_TOTAL + sizeof(Plan) <= 227 * 1024,
                 "exceeds the shared memory of one CTA");
-  static_assert(SLOTS % GROUPS == 0, "a slot is always the same group's");
 };
 
 constexpr int TMA_WAIT = STATUS_TMA_WAIT, MMA_WAIT = STATUS_MMA_WAIT;
@@ -370,8 +366,8 @@ __device__ __forceinline__ void clear_tails(unsigned char* q, int tiles, int row
   fence_proxy_async();
 }
 
-// lse: [tiles + CTAs][2 groups][2 halves][128], log2 of the sum of weights that a group has seen in half of
-// the columns, of the tile's row tile (group % NT); span: a tile's first and last CTA.
+// lse: [tiles + CTAs][NT][2][128], log2 of the sum of weights of a row tile in half of its CTA's columns; span:
+// a tile's first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -410,11 +406,11 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     }
     for (int b = 0; b < SLOTS; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&s_free[b], EP_GROUP);
+      mbar_init(&s_free[b], EP_WARPS);
     }
     for (int b = 0; b < NS; ++b) {
       mbar_init(&c_full[b], 1);
-      mbar_init(&c_free[b], EP_GROUP * PER * NT);
+      mbar_init(&c_free[b], EP_WARPS);
     }
     mbar_fence_init();
     prefetch_tmap(&tmap_q);
@@ -557,45 +553,44 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       }
     }
   } else {
-    // ---------------- a row per lane; a group has a row tile, or every other unit
+    // ---------------- a row per lane, of each row tile, and half of the columns
     constexpr int CB = G > 1 ? 8 : 16, COLS = N / 2;             // columns at a time, and of a warp
-    constexpr bool EACH = PER * NT == GROUPS;
-    static_assert(EACH || PER * NT == 1, "products of a unit");
-    const int group = warp >> 3, half = warp >> 2 & 1, at = (warp & 3) * 32 + lane;
+    const int half = warp >> 2, at = (warp & 3) * 32 + lane;
     const uint32_t scores = tmem + half * COLS + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    static_assert(PER == 1, "a product for each row tile");
     int i = 0;
     for (Walk<KT, NT> w(g, plan); w.left > 0 && ok; w.next_tile()) {
-      const int p = (w.tile * NT + group % NT) * g.per + at / g.rep;
-      // keys that the row sees, and those that all rows of the warp see
-      const int sees = at < g.per * g.rep && p < w.ch.q_len ? w.ch.pos0 + p + 1 : 0;
-      const int all_see = __reduce_min_sync(0xffffffffu, sees);
-      const bool any = __any_sync(0xffffffffu, sees > 0);
-      float m_ref = 0.f;
-      float2 sum = make_float2(0.f, 0.f);
+      int sees[NT], all_see[NT];                 // keys that the rows see, and that all rows of the warp see
+      float m_ref[NT];
+      float2 sum[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int p = (w.tile * NT + t) * g.per + at / g.rep;
+        sees[t] = at < g.per * g.rep && p < w.ch.q_len ? w.ch.pos0 + p + 1 : 0;
+        all_see[t] = __reduce_min_sync(0xffffffffu, sees[t]);
+        m_ref[t] = 0.f;
+        sum[t] = make_float2(0.f, 0.f);
+      }
       const int n = w.here();
-      bool start = true;
-      for (int j0 = EACH ? 0 : (group - i) & (GROUPS - 1); j0 < n; j0 += EACH ? 1 : GROUPS) {
-        const int u = i + j0, cb = u % NS;
-        const int x = EACH ? u * GROUPS + group : u, slot = x % SLOTS;
-        const int key0 = (w.step + j0) * KT + half * COLS;
-        ok = warp_all(mbar_wait(&c_full[cb], (u / NS) & 1, status, EPILOGUE_WAIT, 0x1b) &&
-                      mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x1a));
-        if (!ok) break;
-        tc_fence_after();
+      for (int j0 = 0; j0 < n && ok; ++j0, ++i) {
+        const int cb = i % NS, key0 = (w.step + j0) * KT + half * COLS;
+        ok = warp_all(mbar_wait(&c_full[cb], (i / NS) & 1, status, EPILOGUE_WAIT, 0x1b));
         const float2* scales =
             reinterpret_cast<const float2*>(smem + L::A_SCALE + cb * L::SCALES) + half * COLS / 2 * G;
-        // The columns, CB at a time, to `each` as scores less `ref`: the next ones come meanwhile.
-        auto columns = [&](float ref, auto each) {
-          uint32_t raw[G][CB];
-          auto ask = [&](int k) {
 #pragma unroll
-            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
-          };
-          ask(0);
+        for (int t = 0; t < NT; ++t) {
+          const int x = i * NT + t, slot = x % SLOTS;
+          ok = warp_all(ok && mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x1a));
+          if (!ok) break;
+          tc_fence_after();
+          // ---- scores less the reference
+          float2 y[COLS / 2];
+          uint32_t raw[G][CB];
 #pragma unroll
           for (int k = 0; k < COLS; k += CB) {
+#pragma unroll
+            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
             tc_wait_ld();
-            float2 y[CB / 2];
 #pragma unroll
             for (int j = 0; j < CB / 2; ++j) {
               const float2* f = scales + (k / 2 + j) * G;
@@ -610,69 +605,60 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
                   fg[(c + 1) % G] = make_float2(v.z, v.w);
                 }
               }
-              y[j] = make_float2(-ref, -ref);
+              float2 v = make_float2(-m_ref[t], -m_ref[t]);
 #pragma unroll
-              for (int c = 0; c < G; ++c) y[j] = fma2(pair_at(raw[c][2 * j], raw[c][2 * j + 1]), fg[c], y[j]);
+              for (int c = 0; c < G; ++c) v = fma2(pair_at(raw[c][2 * j], raw[c][2 * j + 1]), fg[c], v);
+              y[k / 2 + j] = v;
             }
-            if (k + CB < COLS) ask(k + CB);
-            each(k, y);
           }
-        };
-        auto weights = [&] {                     // chains of sums of a quarter of the columns
-          float2 v[4];
-          columns(m_ref, [&](int k, float2(&y)[CB / 2]) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[slot]);
+          if (all_see[t] < key0 + COLS) {
 #pragma unroll
-            for (int j = 0; j < CB / 2; ++j) {
+            for (int j = 0; j < COLS / 2; ++j) {
+              if (key0 + 2 * j >= sees[t]) y[j].x = -INFINITY;
+              if (key0 + 2 * j + 1 >= sees[t]) y[j].y = -INFINITY;
+            }
+          }
+          // ---- weights.  The reference is the maximum of the row's first columns, and moves where weights are
+          // far above 1: no maximum is taken but then.  (A row that sees none of the first sees none behind.)
+          auto weights = [&] {                     // chains of sums of a quarter of the columns
+            float2 v[4];
+#pragma unroll
+            for (int j = 0; j < COLS / 2; ++j) {
               const float2 e = make_float2(ex2(y[j].x), ex2(y[j].y));
-              v[j & 3] = k == 0 && j < 4 ? e : add2(v[j & 3], e);
+              v[j & 3] = j < 4 ? e : add2(v[j & 3], e);
             }
-          });
-          return add2(add2(v[0], v[1]), add2(v[2], v[3]));
-        };
-        // The reference is the maximum of the row's first columns, and moves where weights are far above
-        // 1: no maximum is taken but then, and where some row of the warp does not see all of the columns.
-        // (A row that sees none of the first sees none behind them.)
-        bool plain = !start && all_see >= key0 + COLS;
-        float2 more = make_float2(0.f, 0.f);
-        if (plain) {
-          more = weights();
-          plain = !__any_sync(0xffffffffu, more.x + more.y > FAR);
-        }
-        if (!plain && any) {
-          float top = -INFINITY;
-          columns(0.f, [&](int k, float2(&y)[CB / 2]) {
+            return add2(add2(v[0], v[1]), add2(v[2], v[3]));
+          };
+          const bool start = j0 == 0;
+          float2 more = weights();
+          if (__any_sync(0xffffffffu, start || more.x + more.y > FAR)) {
+            float top = fmaxf(y[0].x, y[0].y);
 #pragma unroll
-            for (int j = 0; j < CB / 2; ++j) {
-              if (key0 + k + 2 * j < sees) top = fmaxf(top, y[j].x);
-              if (key0 + k + 2 * j + 1 < sees) top = fmaxf(top, y[j].y);
-            }
-          });
-          const float now = start ? (top == -INFINITY ? 0.f : top) : fmaxf(m_ref, top);
-          const float f = start ? 0.f : ex2(m_ref - now);
-          sum = mul2(sum, make_float2(f, f));
-          m_ref = now;
-          start = false;
-          more = make_float2(0.f, 0.f);
-          columns(m_ref, [&](int k, float2(&y)[CB / 2]) {
+            for (int j = 1; j < COLS / 2; ++j) top = fmaxf(top, fmaxf(y[j].x, y[j].y));
+            const float by = top == -INFINITY ? 0.f : start ? top : fmaxf(top, 0.f);
+            const float f = start ? 0.f : ex2(-by);
+            sum[t] = mul2(sum[t], make_float2(f, f));
+            m_ref[t] += by;
 #pragma unroll
-            for (int j = 0; j < CB / 2; ++j)
-              more = add2(more, make_float2(key0 + k + 2 * j < sees ? ex2(y[j].x) : 0.f,
-                                            key0 + k + 2 * j + 1 < sees ? ex2(y[j].y) : 0.f));
-          });
+            for (int j = 0; j < COLS / 2; ++j) y[j] = add2(y[j], make_float2(-by, -by));
+            more = weights();
+          }
+          sum[t] = add2(sum[t], more);
         }
-        sum = add2(sum, more);
-        tc_fence_before();
+        if (!ok) break;
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&s_free[slot]);
-          mbar_arrive(&c_free[cb]);
-        }
+        if (lane == 0) mbar_arrive(&c_free[cb]);
       }
       if (!ok) break;
-      i += n;
-      const float l = sum.x + sum.y;
-      lse[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + group * 2 + half) * TILE + at] =
-          l == 0.f ? -INFINITY : m_ref + log2f(l);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float l = sum[t].x + sum[t].y;
+        lse[((static_cast<size_t>(w.index + blockIdx.x) * NT + t) * PARTS + half) * TILE + at] =
+            l == 0.f ? -INFINITY : m_ref[t] + log2f(l);
+      }
       if (tid == 0) {
         if (w.step == 0) span[2 * w.index] = blockIdx.x;
         if (w.step + n == w.steps) span[2 * w.index + 1] = blockIdx.x;
@@ -684,18 +670,46 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-// parts: [key tiles + CTAs][2 groups][2 halves][128], sums of what they have seen; span_out: a key tile's
+// A CTA per row tile, KV head and chunk: what the tile's CTAs have left becomes the rows' lse, negative, at
+// [row tiles][128]; a row that is none gets one that leaves no weight.
+template <int NT>
+__global__ void __launch_bounds__(TILE) join_kernel(const Geometry g, const float* lse, const int* span,
+                                                    float* rows) {
+  grid_wait();
+  grid_release();
+  const int c = blockIdx.z, h = blockIdx.y, rt = blockIdx.x, at = threadIdx.x;
+  const Chunk ch = g.at(c);
+  if (rt * g.per >= ch.q_len) return;
+  int base = 0, tiles = 0;                         // of the chunks before: tiles, row tiles
+  for (int d = 0; d < c; ++d) {
+    const Chunk other = g.at(d);
+    base += Order<1, NT>::tiles(g, other) * g.kvh;
+    tiles += Order<1, 1>::tiles(g, other) * g.kvh;
+  }
+  const int index = base + h * Order<1, NT>::tiles(g, ch) + rt / NT;
+  const int2 of = span_of(span, index);
+  float m = -INFINITY, l = 0.f;
+  for (int x = of.x; x <= of.y; ++x)
+    for (int half = 0; half < PARTS; ++half) {
+      const float v = lse[((static_cast<size_t>(index + x) * NT + rt % NT) * PARTS + half) * TILE + at];
+      const float top = fmaxf(m, v);
+      l = (m == -INFINITY ? 0.f : l * exp2f(m - top)) + (v == -INFINITY ? 0.f : exp2f(v - top));
+      m = top;
+    }
+  const bool there = at < min(g.per, ch.q_len - rt * g.per) * g.rep;
+  rows[(static_cast<size_t>(tiles) + h * Order<1, 1>::tiles(g, ch) + rt) * TILE + at] =
+      there ? -m - log2f(l) : -INFINITY;
+}
+
+// rows: join_kernel's.  parts: [key tiles + CTAs][2][128], sums of half of the columns; span_out: a key tile's
 // first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-    const Geometry g, const __half* ks, const float* lse, const int* span, float* parts, int* span_out,
-    int* status) {
+    const Geometry g, const __half* ks, const float* rows, float* parts, int* span_out, int* status) {
   using L = Shape<D>;
   constexpr int G = L::G, N = L::N, PER = L::PER_B, BQ = L::BQ, BK = L::BK, BR = L::BR, NC = L::NC;
   constexpr int SLOTS = L::SLOTS, HALVES = TILE / L::RK;         // copies of a tile's keys
-  constexpr int NT = L::NT;
-  static_assert(PER == 1 || PER == GROUPS, "every other unit for a group, or its part of each");
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ Plan plan;
@@ -729,11 +743,11 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     }
     for (int b = 0; b < SLOTS; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&s_free[b], EP_GROUP);
+      mbar_init(&s_free[b], EP_WARPS);
     }
     for (int b = 0; b < NS; ++b) {
       mbar_init(&l_full[b], 1);
-      mbar_init(&l_free[b], EP_GROUP * PER);
+      mbar_init(&l_free[b], EP_WARPS);
     }
     for (int b = 0; b < NC; ++b) {
       mbar_init(&c_full[b], DQ_WARPS);
@@ -760,17 +774,26 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
   if (warp == TMA_WARP) {
     Units<0> u(g, plan);
     if (lane == 0) {
-      int n = 0;
+      int n = 0, copied = 0, base_c = 0, base = 0;             // row tiles of the chunks before
       for (; u.more(); u.next(), ++n) {
-        const int b = n % BQ;
+        const int b = n % BQ, lb = n % NS, rt = u.w.first + u.step();
+        for (; base_c < u.w.c; ++base_c) base += Order<1>::tiles(g, g.at(base_c)) * g.kvh;
+        const int index = base + u.w.h * Order<1>::tiles(g, u.w.ch) + rt;
+        if (n >= NS && !mbar_wait(&l_free[lb], (n / NS - 1) & 1, status, TMA_WAIT, 0x25)) break;
+        mbar_expect_tx(&l_full[lb], TILE * 4);
+        bulk_load(smem + L::B_LSE + lb * TILE * 4, rows + static_cast<size_t>(index) * TILE, TILE * 4,
+                  &l_full[lb]);
+        ++copied;
         if (n >= BQ && !mbar_wait(&q_free[b], (n / BQ - 1) & 1, status, TMA_WAIT, 0x20)) break;
         mbar_expect_tx(&q_full[b], static_cast<uint32_t>(G) * 64 * 2 * g.rep * g.per);
         for (int s = 0; s < G; ++s)
           tma_load_3d(smem + L::B_Q + b * L::Q_BYTES + s * L::QSUB, &tmap_q, &q_full[b], s * 64,
-                      u.w.h * g.rep, u.w.ch.row_start + (u.w.first + u.step()) * g.per);
+                      u.w.h * g.rep, u.w.ch.row_start + rt * g.per);
       }
       for (int i = max(n - BQ, 0); i < n; ++i)     // our copies have landed before exit
         mbar_wait(&q_full[i % BQ], (i / BQ) & 1, status, TMA_WAIT, 0x21);
+      for (int i = max(copied - NS, 0); i < copied; ++i)
+        mbar_wait(&l_full[i % NS], (i / NS) & 1, status, TMA_WAIT, 0x2e);
     }
   } else if (warp == MMA_WARP) {
     constexpr uint32_t idesc = umma_idesc(1, 0, 0, 0, 0, TILE, N);
@@ -805,71 +828,7 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       if (ok) tc_commit_by(leader, &k_free[n % BK]);
     }
     __syncwarp();
-  } else if (warp >= AUX_WARP) {
-    // ---------------- the rows' lse, of the parts that a tile's CTAs have left; four rows a lane.  A row
-    // that is none gets one that leaves no weight.  A unit's CTAs are asked for a turn before.
-    int base_c = 0, base = 0;                      // tiles of rows of the chunks before
-    Units<0> u(g, plan);
-    int index = 0, mate = 0, rows = 0, first = 0, last = 0;
-    auto ask = [&] {
-      if (!u.more()) return;
-      for (; base_c < u.w.c; ++base_c) base += Order<1, NT>::tiles(g, g.at(base_c)) * g.kvh;
-      const int rt = u.w.first + u.step();
-      index = base + u.w.h * Order<1, NT>::tiles(g, u.w.ch) + rt / NT;
-      mate = rt % NT;
-      rows = min(g.per, u.w.ch.q_len - rt * g.per) * g.rep;
-      first = span[2 * index];
-      last = span[2 * index + 1];
-    };
-    const int mine = warp - AUX_WARP, units = max(u.w.left, 0);
-    u.skip(mine);
-    ask();
-    for (int n = mine; n < units; n += AUX_WARPS) {
-      const int b = n % NS, live = rows;           // (see span_of)
-      const int lo = max(0, min(first, CTAS - 1)), hi = max(lo, min(last, CTAS - 1));
-      // what the CTAs' groups have left of the row tile
-      constexpr int EACH = PARTS / NT;
-      const int count = (hi - lo + 1) * EACH;
-      auto part = [&, from = (static_cast<size_t>(index + lo) * PARTS + mate * EACH) * TILE + 4 * lane](int x) {
-        const size_t at = static_cast<size_t>(x / EACH * PARTS + x % EACH) * TILE;
-        return x < count ? *reinterpret_cast<const float4*>(lse + from + at)
-                         : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      };
-      auto join = [](float& m, float& l, float x) {
-        const float top = fmaxf(m, x);
-        l = (m == -INFINITY ? 0.f : l * exp2f(m - top)) + (x == -INFINITY ? 0.f : exp2f(x - top));
-        m = top;
-      };
-      constexpr int BATCH = 4;
-      float4 m = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), l = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int x = 0; x < count; x += BATCH) {
-        float4 p[BATCH];
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) p[k] = part(x + k);
-        if (x == 0) {
-          u.skip(AUX_WARPS);
-          ask();
-        }
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          join(m.x, l.x, p[k].x);
-          join(m.y, l.y, p[k].y);
-          join(m.z, l.z, p[k].z);
-          join(m.w, l.w, p[k].w);
-        }
-      }
-      float4 v;
-      v.x = 4 * lane < live ? -m.x - log2f(l.x) : -INFINITY;
-      v.y = 4 * lane + 1 < live ? -m.y - log2f(l.y) : -INFINITY;
-      v.z = 4 * lane + 2 < live ? -m.z - log2f(l.z) : -INFINITY;
-      v.w = 4 * lane + 3 < live ? -m.w - log2f(l.w) : -INFINITY;
-      if (n >= NS) ok = mbar_wait(&l_free[b], (n / NS - 1) & 1, status, DECODE_WAIT, 0x25);
-      ok = warp_all(ok);
-      if (!ok) break;
-      *reinterpret_cast<float4*>(smem + L::B_LSE + b * TILE * 4 + lane * 16) = v;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&l_full[b]);
-    }
+  } else if (warp >= AUX_WARP) {                   // (scales come with the keys)
   } else if (warp >= EP_WARPS) {
     // ---------------- keys: a tile, INT8 to FP16 integers, and their scales.  The copies are this role's
     // own, BR ahead: the first lane of its first warp asks for them.
@@ -945,14 +904,13 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
         mbar_wait(&r_full[i % BR], (i / BR) & 1, status, TMA_WAIT, 0x2d);
     __syncwarp();
   } else {
-    // ---------------- sums: a key per lane
-    const int group = warp >> 3, half = warp >> 2 & 1, key_at = (warp & 3) * 32 + lane;
+    // ---------------- sums: a key per lane, half of the columns
     constexpr int CB = G > 1 ? 8 : 16, COLS = N / 2;             // columns at a time, and of a warp
-    const int col0 = group % PER * N + half * COLS;              // of the unit
+    const int half = warp >> 2, key_at = (warp & 3) * 32 + lane;
     const uint32_t scores = tmem + half * COLS + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     int i = 0, n = 0;                              // units, tiles
     for (Walk<0> w(g, plan); w.left > 0 && ok; w.next_tile(), ++n) {
-      const int cb = n % NC, here = w.here();
+      const int cb = n % NC, end = i + w.here();
       ok = warp_all(mbar_wait(&c_full[cb], (n / NC) & 1, status, EPILOGUE_WAIT, 0x2a));
       if (!ok) break;
       float2 f[G];
@@ -964,72 +922,69 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       __syncwarp();
       if (lane == 0) mbar_arrive(&c_free[cb]);
       // of the chunk's rows times heads those from `see` on see the key
-      const int see = (w.tile * TILE + key_at - w.ch.pos0) * g.rep, rows = w.ch.q_len * g.rep;
+      const int see = (w.tile * TILE + key_at - w.ch.pos0) * g.rep, last = w.ch.q_len * g.rep;
       const int clear = w.tile * TILE + TILE - 1 - w.ch.pos0;      // positions from there on see all keys
       float2 total = make_float2(0.f, 0.f);
-      constexpr int EVERY = GROUPS / PER;
-      const int skip = PER > 1 ? 0 : (i ^ group) & 1, end = i + here;
-      int pos = (w.first + w.step + skip) * g.per;  // of a unit's first row
-      for (i += skip; i < end; i += EVERY, pos += EVERY * g.per) {
-        const int lb = i % NS, x = PER * i + group % PER, slot = x % SLOTS;
-        ok = warp_all(mbar_wait(&l_full[lb], (i / NS) & 1, status, EPILOGUE_WAIT, 0x28) &&
-                      mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x27));
-        if (!ok) break;
-        tc_fence_after();
+      int pos = (w.first + w.step) * g.per;        // of a unit's first row
+      for (; i < end && ok; ++i, pos += g.per) {
+        const int lb = i % NS;
         const bool edge = pos < clear || pos + g.per > w.ch.q_len;
-        const int first = pos * g.rep + col0;
-        const float* neg = reinterpret_cast<const float*>(smem + L::B_LSE + lb * TILE * 4) + col0;
-        auto weights = [&](auto masked) {
-          uint32_t raw[G][CB];
-          auto ask = [&](int k) {
+        ok = warp_all(mbar_wait(&l_full[lb], (i / NS) & 1, status, EPILOGUE_WAIT, 0x28));
 #pragma unroll
-            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
-          };
-          ask(0);
-          float2 v[4];                             // chains of sums of a quarter of the columns
+        for (int p = 0; p < PER; ++p) {
+          const int x = PER * i + p, slot = x % SLOTS, col0 = p * N + half * COLS;
+          ok = warp_all(ok && mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x27));
+          if (!ok) break;
+          tc_fence_after();
+          const float* neg = reinterpret_cast<const float*>(smem + L::B_LSE + lb * TILE * 4) + col0;
+          float2 y[COLS / 2];                      // scores less the rows' lse
+          uint32_t raw[G][CB];
 #pragma unroll
           for (int k = 0; k < COLS; k += CB) {
+#pragma unroll
+            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
             tc_wait_ld();
-            float2 y[CB / 2];
 #pragma unroll
             for (int j = 0; j < CB / 2; j += 2) {
               const float4 from = *reinterpret_cast<const float4*>(neg + k + 2 * j);
-              y[j] = make_float2(from.x, from.y);
-              y[j + 1] = make_float2(from.z, from.w);
+              float2 v[2] = {make_float2(from.x, from.y), make_float2(from.z, from.w)};
 #pragma unroll
-              for (int c = 0; c < G; ++c) {
-                y[j] = fma2(pair_at(raw[c][2 * j], raw[c][2 * j + 1]), f[c], y[j]);
-                y[j + 1] = fma2(pair_at(raw[c][2 * j + 2], raw[c][2 * j + 3]), f[c], y[j + 1]);
-              }
-            }
-            if (k + CB < COLS) ask(k + CB);           // (they come while these are weighed)
+              for (int c = 0; c < G; ++c)
 #pragma unroll
-            for (int j = 0; j < CB / 2; ++j) {
-              float2 e = make_float2(ex2(y[j].x), ex2(y[j].y));
-              if (masked) {
-                const int row = first + k + 2 * j;
-                if (row < see || row >= rows) e.x = 0.f;
-                if (row + 1 < see || row + 1 >= rows) e.y = 0.f;
-              }
-              v[j & 3] = k == 0 && j < 4 ? e : add2(v[j & 3], e);
+                for (int e = 0; e < 2; ++e)
+                  v[e] = fma2(pair_at(raw[c][2 * (j + e)], raw[c][2 * (j + e) + 1]), f[c], v[e]);
+              y[k / 2 + j] = v[0];
+              y[k / 2 + j + 1] = v[1];
             }
           }
-          return add2(add2(v[0], v[1]), add2(v[2], v[3]));
-        };
-        total = add2(total, edge ? weights(std::true_type()) : weights(std::false_type()));
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&s_free[slot]);
-          mbar_arrive(&l_free[lb]);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&s_free[slot]);
+            if (p + 1 == PER) mbar_arrive(&l_free[lb]);
+          }
+          float2 v[4];                             // chains of sums of a quarter of the columns
+#pragma unroll
+          for (int j = 0; j < COLS / 2; ++j) y[j] = make_float2(ex2(y[j].x), ex2(y[j].y));
+          if (edge) {
+            const int first = pos * g.rep + col0;
+#pragma unroll
+            for (int j = 0; j < COLS / 2; ++j) {
+              const int row = first + 2 * j;
+              if (row < see || row >= last) y[j].x = 0.f;
+              if (row + 1 < see || row + 1 >= last) y[j].y = 0.f;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < COLS / 2; ++j) v[j & 3] = j < 4 ? y[j] : add2(v[j & 3], y[j]);
+          total = add2(total, add2(add2(v[0], v[1]), add2(v[2], v[3])));
         }
       }
       if (!ok) break;
-      i = end;
-      parts[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + group * 2 + half) * TILE + key_at] = total.x + total.y;
+      parts[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + half) * TILE + key_at] = total.x + total.y;
       if (tid == 0) {
         if (w.step == 0) span_out[2 * w.index] = blockIdx.x;
-        if (w.step + here == w.steps) span_out[2 * w.index + 1] = blockIdx.x;
+        if (w.step + w.here() == w.steps) span_out[2 * w.index + 1] = blockIdx.x;
       }
     }
   }
@@ -1118,15 +1073,17 @@ static int launch(const __half* q, const Geometry& g, const int8_t* kc, const __
   if (const int e = runtime_allow_smem(slot[1], sums_kernel<D>, L::B_TOTAL)) return e;
   const Bounds b = bounds(g.n_chunks, g.longest, g.kvh, g.rep, g.limit);
   float* lse = work;
-  float* parts = lse + (b.row_tiles + CTAS) * PARTS * TILE;
+  float* rows = lse + 2 * (b.row_tiles + CTAS) * PARTS * TILE;    // (a tile has a place for two row tiles)
+  float* parts = rows + b.row_tiles * TILE;
   int* row_span = reinterpret_cast<int*>(parts + (b.key_tiles + CTAS) * PARTS * TILE);
   int* key_span = row_span + 2 * b.row_tiles;
   const int ctas = ctas_for(b.units);
   launch_early(stats_kernel<D>, dim3(ctas), THREADS, L::A_TOTAL, stream, tq, tk, g, ks, lse, row_span,
                runtime_status_ptr());
+  launch_early(join_kernel<L::NT>, dim3((g.longest + g.per - 1) / g.per, g.kvh, g.n_chunks), TILE, 0, stream,
+               g, static_cast<const float*>(lse), static_cast<const int*>(row_span), rows);
   launch_early(sums_kernel<D>, dim3(ctas), THREADS, L::B_TOTAL, stream, tq, tk, g, ks,
-               static_cast<const float*>(lse), static_cast<const int*>(row_span), parts, key_span,
-               runtime_status_ptr());
+               static_cast<const float*>(rows), parts, key_span, runtime_status_ptr());
   launch_early(add_kernel, dim3((g.limit + TILE - 1) / TILE, g.kvh, g.n_chunks), TILE, 0, stream, g,
                static_cast<const float*>(parts), static_cast<const int*>(key_span), weights, slot_stride,
                head_stride, sums, sums_slot_stride, sums_head_stride);
@@ -1142,7 +1099,7 @@ extern "C" size_t orinfer_prefill_weights_work_bytes(int n_chunks, int max_q_len
                                                      int limit) {
   if (n_chunks <= 0 || rep <= 0) return 0;
   const kw::Bounds b = kw::bounds(n_chunks, max_q_len, kvh, rep, limit);
-  return ((b.row_tiles + kw::CTAS) * kw::PARTS + (b.key_tiles + kw::CTAS) * kw::PARTS) *
+  return (2 * (b.row_tiles + kw::CTAS) * kw::PARTS + b.row_tiles + (b.key_tiles + kw::CTAS) * kw::PARTS) *
              kw::TILE * sizeof(float) +
          2 * (b.row_tiles + b.key_tiles) * sizeof(int);
 }
