@@ -29,13 +29,17 @@ namespace kw {
 
 constexpr int TILE = 128;                        // rows of a tile: positions x query heads; keys of a tile
 constexpr int MAX_CHUNKS = 512;
-constexpr int EP_WARPS = 8;                      // softmax or sums: 32 lanes and half of a product's columns
+// Softmax or sums: two groups, a product each in turn, so that one computes while the other waits and reads.
+// Whoever waits on a barrier does so for each of its phases: one that came for every other one could not
+// tell them apart.
+constexpr int EP_WARPS = 16, EP_GROUP = 8, GROUPS = 2;
 constexpr int DQ_WARPS = 4;                      // INT8 to FP16
 constexpr int AUX_WARPS = 2;                     // scales, in turn
 constexpr int AUX_WARP = EP_WARPS + DQ_WARPS, MMA_WARP = AUX_WARP + AUX_WARPS;
 constexpr int TMA_WARP = MMA_WARP + 1, THREADS = (TMA_WARP + 1) * 32;
 constexpr int CTAS = 148;
-constexpr int PARTS = 2;                         // halves of a tile's columns
+constexpr int PARTS = 4;                         // of a tile: two groups, two halves of the columns
+constexpr int COLS = 32;                         // columns that a thread has in registers
 constexpr int NS = 4;                            // places of scales, or of rows' lse
 constexpr float FAR = 1.1529215046068470e18f;    // 2^60: weights under a reference that has to move
 
@@ -225,6 +229,7 @@ struct Shape {
   static constexpr int NC = 2;
   static constexpr int B_BAR = B_SCALE + NC * G * TILE * 4;
   static constexpr int B_TOTAL = B_BAR + 512 + 1024;
+  static_assert(SLOTS % GROUPS == 0, "a slot is always the same group's");
   static_assert(A_TOTAL + sizeof(Plan) <= 227 * 1024 && B_TOTAL + sizeof(Plan) <= 227 * 1024,
                 "exceeds the shared memory of one CTA");
 };
@@ -366,8 +371,8 @@ __device__ __forceinline__ void clear_tails(unsigned char* q, int tiles, int row
   fence_proxy_async();
 }
 
-// lse: [tiles + CTAs][NT][2][128], log2 of the sum of weights of a row tile in half of its CTA's columns; span:
-// a tile's first and last CTA.
+// lse: [tiles + CTAs][2 groups][2 halves][128], log2 of the sum of weights that a group has seen in half of the
+// columns, of its row tile or of the one that there is; span: a tile's first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -406,11 +411,11 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
     }
     for (int b = 0; b < SLOTS; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&s_free[b], EP_WARPS);
+      mbar_init(&s_free[b], EP_GROUP);
     }
     for (int b = 0; b < NS; ++b) {
       mbar_init(&c_full[b], 1);
-      mbar_init(&c_free[b], EP_WARPS);
+      mbar_init(&c_free[b], EP_GROUP * NT);
     }
     mbar_fence_init();
     prefetch_tmap(&tmap_q);
@@ -553,43 +558,40 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
       }
     }
   } else {
-    // ---------------- a row per lane, of each row tile, and half of the columns
-    constexpr int CB = G > 1 ? 8 : 16, COLS = N / 2;             // columns at a time, and of a warp
-    const int half = warp >> 2, at = (warp & 3) * 32 + lane;
-    const uint32_t scores = tmem + half * COLS + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    // ---------------- a row per lane; a group has a row tile, or every other unit
+    constexpr int CB = G > 1 ? 8 : 16;           // columns that are read at a time
+    constexpr int EVERY = GROUPS / NT;
+    const int group = warp >> 3, half = warp >> 2 & 1, at = (warp & 3) * 32 + lane;
+    const uint32_t scores = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     static_assert(PER == 1, "a product for each row tile");
     int i = 0;
     for (Walk<KT, NT> w(g, plan); w.left > 0 && ok; w.next_tile()) {
-      int sees[NT], all_see[NT];                 // keys that the rows see, and that all rows of the warp see
-      float m_ref[NT];
-      float2 sum[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int p = (w.tile * NT + t) * g.per + at / g.rep;
-        sees[t] = at < g.per * g.rep && p < w.ch.q_len ? w.ch.pos0 + p + 1 : 0;
-        all_see[t] = __reduce_min_sync(0xffffffffu, sees[t]);
-        m_ref[t] = 0.f;
-        sum[t] = make_float2(0.f, 0.f);
-      }
+      const int p = (w.tile * NT + group % NT) * g.per + at / g.rep;
+      // keys that the row sees, and those that all rows of the warp see
+      const int sees = at < g.per * g.rep && p < w.ch.q_len ? w.ch.pos0 + p + 1 : 0;
+      const int all_see = __reduce_min_sync(0xffffffffu, sees);
+      float m_ref = 0.f;
+      float2 sum = make_float2(0.f, 0.f);
       const int n = w.here();
-      for (int j0 = 0; j0 < n && ok; ++j0, ++i) {
-        const int cb = i % NS, key0 = (w.step + j0) * KT + half * COLS;
-        ok = warp_all(mbar_wait(&c_full[cb], (i / NS) & 1, status, EPILOGUE_WAIT, 0x1b));
-        const float2* scales =
-            reinterpret_cast<const float2*>(smem + L::A_SCALE + cb * L::SCALES) + half * COLS / 2 * G;
+      bool start = true;
+      for (int j0 = EVERY > 1 ? (i ^ group) & 1 : 0; j0 < n; j0 += EVERY) {
+        const int u = i + j0, cb = u % NS, x = u * NT + group % NT, slot = x % SLOTS;
+        ok = warp_all(mbar_wait(&c_full[cb], (u / NS) & 1, status, EPILOGUE_WAIT, 0x1b) &&
+                      mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x1a));
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int x = i * NT + t, slot = x % SLOTS;
-          ok = warp_all(ok && mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x1a));
-          if (!ok) break;
-          tc_fence_after();
+        for (int p0 = 0; p0 < N / 2; p0 += COLS) {
+          const int k0 = half * (N / 2) + p0, key0 = (w.step + j0) * KT + k0;
+          const float2* scales =
+              reinterpret_cast<const float2*>(smem + L::A_SCALE + cb * L::SCALES) + k0 / 2 * G;
           // ---- scores less the reference
           float2 y[COLS / 2];
           uint32_t raw[G][CB];
 #pragma unroll
           for (int k = 0; k < COLS; k += CB) {
 #pragma unroll
-            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
+            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k0 + k, raw[c]);
             tc_wait_ld();
 #pragma unroll
             for (int j = 0; j < CB / 2; ++j) {
@@ -605,20 +607,25 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
                   fg[(c + 1) % G] = make_float2(v.z, v.w);
                 }
               }
-              float2 v = make_float2(-m_ref[t], -m_ref[t]);
+              float2 v = make_float2(-m_ref, -m_ref);
 #pragma unroll
               for (int c = 0; c < G; ++c) v = fma2(pair_at(raw[c][2 * j], raw[c][2 * j + 1]), fg[c], v);
               y[k / 2 + j] = v;
             }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[slot]);
-          if (all_see[t] < key0 + COLS) {
+          if (p0 + COLS == N / 2) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&s_free[slot]);
+              mbar_arrive(&c_free[cb]);
+            }
+          }
+          if (all_see < key0 + COLS) {
 #pragma unroll
             for (int j = 0; j < COLS / 2; ++j) {
-              if (key0 + 2 * j >= sees[t]) y[j].x = -INFINITY;
-              if (key0 + 2 * j + 1 >= sees[t]) y[j].y = -INFINITY;
+              if (key0 + 2 * j >= sees) y[j].x = -INFINITY;
+              if (key0 + 2 * j + 1 >= sees) y[j].y = -INFINITY;
             }
           }
           // ---- weights.  The reference is the maximum of the row's first columns, and moves where weights are
@@ -632,33 +639,29 @@ __global__ void __launch_bounds__(THREADS, 1) stats_kernel(
             }
             return add2(add2(v[0], v[1]), add2(v[2], v[3]));
           };
-          const bool start = j0 == 0;
-          float2 more = weights();
+          float2 more = make_float2(0.f, 0.f);
+          if (!start) more = weights();
           if (__any_sync(0xffffffffu, start || more.x + more.y > FAR)) {
             float top = fmaxf(y[0].x, y[0].y);
 #pragma unroll
             for (int j = 1; j < COLS / 2; ++j) top = fmaxf(top, fmaxf(y[j].x, y[j].y));
             const float by = top == -INFINITY ? 0.f : start ? top : fmaxf(top, 0.f);
             const float f = start ? 0.f : ex2(-by);
-            sum[t] = mul2(sum[t], make_float2(f, f));
-            m_ref[t] += by;
+            sum = mul2(sum, make_float2(f, f));
+            m_ref += by;
 #pragma unroll
             for (int j = 0; j < COLS / 2; ++j) y[j] = add2(y[j], make_float2(-by, -by));
             more = weights();
+            start = false;
           }
-          sum[t] = add2(sum[t], more);
+          sum = add2(sum, more);
         }
-        if (!ok) break;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&c_free[cb]);
       }
       if (!ok) break;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float l = sum[t].x + sum[t].y;
-        lse[((static_cast<size_t>(w.index + blockIdx.x) * NT + t) * PARTS + half) * TILE + at] =
-            l == 0.f ? -INFINITY : m_ref[t] + log2f(l);
-      }
+      i += n;
+      const float l = sum.x + sum.y;
+      lse[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + group * 2 + half) * TILE + at] =
+          l == 0.f ? -INFINITY : m_ref + log2f(l);
       if (tid == 0) {
         if (w.step == 0) span[2 * w.index] = blockIdx.x;
         if (w.step + n == w.steps) span[2 * w.index + 1] = blockIdx.x;
@@ -690,8 +693,8 @@ __global__ void __launch_bounds__(TILE) join_kernel(const Geometry g, const floa
   const int2 of = span_of(span, index);
   float m = -INFINITY, l = 0.f;
   for (int x = of.x; x <= of.y; ++x)
-    for (int half = 0; half < PARTS; ++half) {
-      const float v = lse[((static_cast<size_t>(index + x) * NT + rt % NT) * PARTS + half) * TILE + at];
+    for (int part = rt % NT * 2; part < (NT > 1 ? rt % NT * 2 + 2 : PARTS); ++part) {
+      const float v = lse[(static_cast<size_t>(index + x) * PARTS + part) * TILE + at];
       const float top = fmaxf(m, v);
       l = (m == -INFINITY ? 0.f : l * exp2f(m - top)) + (v == -INFINITY ? 0.f : exp2f(v - top));
       m = top;
@@ -701,7 +704,8 @@ __global__ void __launch_bounds__(TILE) join_kernel(const Geometry g, const floa
       there ? -m - log2f(l) : -INFINITY;
 }
 
-// rows: join_kernel's.  parts: [key tiles + CTAs][2][128], sums of half of the columns; span_out: a key tile's
+// rows: join_kernel's.  parts: [key tiles + CTAs][2 groups][2 halves][128], sums of
+// what they have seen; span_out: a key tile's
 // first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
@@ -743,11 +747,11 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     }
     for (int b = 0; b < SLOTS; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&s_free[b], EP_WARPS);
+      mbar_init(&s_free[b], EP_GROUP);
     }
     for (int b = 0; b < NS; ++b) {
       mbar_init(&l_full[b], 1);
-      mbar_init(&l_free[b], EP_WARPS);
+      mbar_init(&l_free[b], EP_GROUP * PER);
     }
     for (int b = 0; b < NC; ++b) {
       mbar_init(&c_full[b], DQ_WARPS);
@@ -904,13 +908,14 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
         mbar_wait(&r_full[i % BR], (i / BR) & 1, status, TMA_WAIT, 0x2d);
     __syncwarp();
   } else {
-    // ---------------- sums: a key per lane, half of the columns
-    constexpr int CB = G > 1 ? 8 : 16, COLS = N / 2;             // columns at a time, and of a warp
-    const int half = warp >> 2, key_at = (warp & 3) * 32 + lane;
-    const uint32_t scores = tmem + half * COLS + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    // ---------------- sums: a key per lane; a group has every other unit, or half of the rows of each
+    constexpr int CB = G > 1 ? 8 : 16;             // columns that are read at a time
+    constexpr int EVERY = GROUPS / PER;
+    const int group = warp >> 3, half = warp >> 2 & 1, key_at = (warp & 3) * 32 + lane, part = group % PER * N;
+    const uint32_t scores = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     int i = 0, n = 0;                              // units, tiles
     for (Walk<0> w(g, plan); w.left > 0 && ok; w.next_tile(), ++n) {
-      const int cb = n % NC, end = i + w.here();
+      const int cb = n % NC, here = w.here();
       ok = warp_all(mbar_wait(&c_full[cb], (n / NC) & 1, status, EPILOGUE_WAIT, 0x2a));
       if (!ok) break;
       float2 f[G];
@@ -923,30 +928,29 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       if (lane == 0) mbar_arrive(&c_free[cb]);
       // of the chunk's rows times heads those from `see` on see the key
       const int see = (w.tile * TILE + key_at - w.ch.pos0) * g.rep, last = w.ch.q_len * g.rep;
-      const int clear = w.tile * TILE + TILE - 1 - w.ch.pos0;      // positions from there on see all keys
+      const int see_all = (w.tile * TILE + TILE - 1 - w.ch.pos0) * g.rep;    // and all keys of the tile
       float2 total = make_float2(0.f, 0.f);
-      int pos = (w.first + w.step) * g.per;        // of a unit's first row
-      for (; i < end && ok; ++i, pos += g.per) {
-        const int lb = i % NS;
-        const bool edge = pos < clear || pos + g.per > w.ch.q_len;
-        ok = warp_all(mbar_wait(&l_full[lb], (i / NS) & 1, status, EPILOGUE_WAIT, 0x28));
+      for (int j0 = EVERY > 1 ? (i ^ group) & 1 : 0; j0 < here; j0 += EVERY) {
+        const int u = i + j0, lb = u % NS, x = PER * u + group % PER, slot = x % SLOTS;
+        const int pos = (w.first + w.step + j0) * g.per;           // of the unit's first row
+        ok = warp_all(mbar_wait(&l_full[lb], (u / NS) & 1, status, EPILOGUE_WAIT, 0x28) &&
+                      mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x27));
+        if (!ok) break;
+        tc_fence_after();
+        const float* neg = reinterpret_cast<const float*>(smem + L::B_LSE + lb * TILE * 4) + part;
 #pragma unroll
-        for (int p = 0; p < PER; ++p) {
-          const int x = PER * i + p, slot = x % SLOTS, col0 = p * N + half * COLS;
-          ok = warp_all(ok && mbar_wait(&s_full[slot], (x / SLOTS) & 1, status, EPILOGUE_WAIT, 0x27));
-          if (!ok) break;
-          tc_fence_after();
-          const float* neg = reinterpret_cast<const float*>(smem + L::B_LSE + lb * TILE * 4) + col0;
+        for (int p0 = 0; p0 < N / 2; p0 += COLS) {
+          const int k0 = half * (N / 2) + p0;
           float2 y[COLS / 2];                      // scores less the rows' lse
           uint32_t raw[G][CB];
 #pragma unroll
           for (int k = 0; k < COLS; k += CB) {
 #pragma unroll
-            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k, raw[c]);
+            for (int c = 0; c < G; ++c) tmem_ld_rows(scores + L::SLOT * slot + c * N + k0 + k, raw[c]);
             tc_wait_ld();
 #pragma unroll
             for (int j = 0; j < CB / 2; j += 2) {
-              const float4 from = *reinterpret_cast<const float4*>(neg + k + 2 * j);
+              const float4 from = *reinterpret_cast<const float4*>(neg + k0 + k + 2 * j);
               float2 v[2] = {make_float2(from.x, from.y), make_float2(from.z, from.w)};
 #pragma unroll
               for (int c = 0; c < G; ++c)
@@ -957,17 +961,18 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
               y[k / 2 + j + 1] = v[1];
             }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&s_free[slot]);
-            if (p + 1 == PER) mbar_arrive(&l_free[lb]);
+          if (p0 + COLS == N / 2) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&s_free[slot]);
+              mbar_arrive(&l_free[lb]);
+            }
           }
-          float2 v[4];                             // chains of sums of a quarter of the columns
 #pragma unroll
           for (int j = 0; j < COLS / 2; ++j) y[j] = make_float2(ex2(y[j].x), ex2(y[j].y));
-          if (edge) {
-            const int first = pos * g.rep + col0;
+          const int first = pos * g.rep + part + k0;
+          if (first < see_all || first + COLS > last) {
 #pragma unroll
             for (int j = 0; j < COLS / 2; ++j) {
               const int row = first + 2 * j;
@@ -975,16 +980,18 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
               if (row + 1 < see || row + 1 >= last) y[j].y = 0.f;
             }
           }
+          float2 v[4];                             // chains of sums of a quarter of the columns
 #pragma unroll
           for (int j = 0; j < COLS / 2; ++j) v[j & 3] = j < 4 ? y[j] : add2(v[j & 3], y[j]);
           total = add2(total, add2(add2(v[0], v[1]), add2(v[2], v[3])));
         }
       }
       if (!ok) break;
-      parts[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + half) * TILE + key_at] = total.x + total.y;
+      i += here;
+      parts[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + group * 2 + half) * TILE + key_at] = total.x + total.y;
       if (tid == 0) {
         if (w.step == 0) span_out[2 * w.index] = blockIdx.x;
-        if (w.step + w.here() == w.steps) span_out[2 * w.index + 1] = blockIdx.x;
+        if (w.step + here == w.steps) span_out[2 * w.index + 1] = blockIdx.x;
       }
     }
   }
@@ -1073,7 +1080,7 @@ static int launch(const __half* q, const Geometry& g, const int8_t* kc, const __
   if (const int e = runtime_allow_smem(slot[1], sums_kernel<D>, L::B_TOTAL)) return e;
   const Bounds b = bounds(g.n_chunks, g.longest, g.kvh, g.rep, g.limit);
   float* lse = work;
-  float* rows = lse + 2 * (b.row_tiles + CTAS) * PARTS * TILE;    // (a tile has a place for two row tiles)
+  float* rows = lse + (b.row_tiles + CTAS) * PARTS * TILE;
   float* parts = rows + b.row_tiles * TILE;
   int* row_span = reinterpret_cast<int*>(parts + (b.key_tiles + CTAS) * PARTS * TILE);
   int* key_span = row_span + 2 * b.row_tiles;
@@ -1099,7 +1106,7 @@ extern "C" size_t orinfer_prefill_weights_work_bytes(int n_chunks, int max_q_len
                                                      int limit) {
   if (n_chunks <= 0 || rep <= 0) return 0;
   const kw::Bounds b = kw::bounds(n_chunks, max_q_len, kvh, rep, limit);
-  return (2 * (b.row_tiles + kw::CTAS) * kw::PARTS + b.row_tiles + (b.key_tiles + kw::CTAS) * kw::PARTS) *
+  return ((b.row_tiles + kw::CTAS) * kw::PARTS + b.row_tiles + (b.key_tiles + kw::CTAS) * kw::PARTS) *
              kw::TILE * sizeof(float) +
          2 * (b.row_tiles + b.key_tiles) * sizeof(int);
 }
