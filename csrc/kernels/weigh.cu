@@ -34,7 +34,7 @@ constexpr int MAX_CHUNKS = 512;
 // tell them apart.
 constexpr int EP_WARPS = 16, EP_GROUP = 8, GROUPS = 2;
 constexpr int DQ_WARPS = 4;                      // INT8 to FP16
-constexpr int AUX_WARPS = 2;                     // scales, in turn
+constexpr int AUX_WARPS = 1;                     // scales
 constexpr int AUX_WARP = EP_WARPS + DQ_WARPS, MMA_WARP = AUX_WARP + AUX_WARPS;
 constexpr int TMA_WARP = MMA_WARP + 1, THREADS = (TMA_WARP + 1) * 32;
 constexpr int CTAS = 148;
