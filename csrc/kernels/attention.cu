@@ -1105,18 +1105,17 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
 // a record per step of the loop, and attn_finish computing every factor anew for each channel, one
 // row of 2000 keys and 32 / 8 heads of 128 took 10.7 us (now 8.3), 16 / 2 heads of 256 (32 records)
 // 15.1 (10.0), 64 rows of 640 keys unsplit 26.8 (22.9).
+// Channels `d0`, d0 + step, ... of a head of a row, a warp's lanes 32 neighbouring ones.
 template <int D, bool SHARED>
-__global__ void attn_merge_kernel(
-    const float* scratch, const __half* gate, __half* __restrict__ out, int qh, int splits,
-    const SharedParts parts) {
-  grid_wait();
-  grid_release();
-  const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31;
+__device__ __forceinline__ void attn_merge(const float* scratch, const __half* gate,
+                                           __half* __restrict__ out, int row, int head, int qh,
+                                           int splits, int d0, int step, const SharedParts& parts) {
+  const int lane = threadIdx.x & 31;
   const float* rec = scratch + (static_cast<size_t>(row) * qh + head) * splits * (D + 2);
   float m = -INFINITY;
   for (int s = lane; s < splits; s += 32) m = fmaxf(m, rec[s * (D + 2)]);
   m = warp_max(m);
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+  for (int d = d0; d < D; d += step) {
     float l = 0.f, o = 0.f;
     for (int s0 = 0; s0 < splits; s0 += 32) {
       const int n = min(32, splits - s0);
@@ -1174,74 +1173,145 @@ __global__ void attn_merge_kernel(
     attn_store(l > 0.f ? o / l : 0.f, gate, out, (static_cast<size_t>(row) * qh + head) * D + d);
   }
 }
+template <int D, bool SHARED>
+__global__ void attn_merge_kernel(
+    const float* scratch, const __half* gate, __half* __restrict__ out, int qh, int splits,
+    const SharedParts parts) {
+  grid_wait();
+  grid_release();
+  attn_merge<D, SHARED>(scratch, gate, out, blockIdx.x, blockIdx.y, qh, splits, threadIdx.x, blockDim.x,
+                        parts);
+}
 
 // ---------------------------------------------------------------- weights of the keys
 // sums[request][KV head][key] = weights[...] + the weights 2^(score - reference) / sum that the key got
 // from the row's query heads of that KV head, in the order of the heads; rows of one request (a
 // verification's) in the order of the rows, by the CTA of the first of them.  So no order of arrival
-// shows in the sums, and a row's output does not wait for them.
+// shows in the sums, and a row's output does not wait for them.  Where the keys are split, the CTAs of
+// the first column put the outputs together meanwhile.
 //
 // A CTA takes WEIGH_KEYS keys of a row and KV head.  Scores are written once by the row kernels and read
-// once here, 4 rep bytes a key beside the 2 D and more of its key and value, mostly within L2.
-constexpr int WEIGH_THREADS = 256, WEIGH_KEYS = 4 * WEIGH_THREADS;
+// once here, 4 rep bytes a key beside the 2 D and more of its key and value, mostly within L2.  It is a
+// chain of loads that wait for each other, so what can be asked for at once is: scores and factors of the
+// CTA's own row before it is known whether an earlier row's CTA has them, the factors of the rows behind it
+// together, their scores a row ahead.
+constexpr int WEIGH_THREADS = 256, WEIGH_KEYS = 4 * WEIGH_THREADS, WEIGH_ROWS = 32;
+template <int D, int REP>
 __global__ void __launch_bounds__(WEIGH_THREADS) attn_weigh_kernel(
     const Weighed weighed, const int* row_req, const int* row_pos, const float* weights,
     long long slot_stride, long long head_stride, float* sums, long long sums_slot_stride,
-    long long sums_head_stride, int capacity, int rows, int qh, int rep, int splits, int* status) {
-  __shared__ unsigned s_same[WEIGH_THREADS / 32];
-  __shared__ float2 s_f[8];                        // a head's reference and 1 / sum
+    long long sums_head_stride, int capacity, int rows, int qh, int splits, const float* scratch,
+    const __half* gate, __half* __restrict__ out, int* status) {
+  __shared__ int2 s_rows[WEIGH_ROWS];              // rows of the request, in their order, and their keys
+  __shared__ int s_count[WEIGH_THREADS / 32];
+  __shared__ float2 s_f[WEIGH_ROWS][REP];          // a head's reference and 1 / sum
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_wait();
   grid_release();
-  const int row = blockIdx.x, h = blockIdx.y, key = blockIdx.z * WEIGH_KEYS + 4 * tid;
-  if (row_pos[row] < 0) return;
-  const int req = row_req[row];
+  const int row = blockIdx.x, h = blockIdx.y, z = static_cast<int>(blockIdx.z) - (splits > 1);
+  const int key = z * WEIGH_KEYS + 4 * tid;
+  if (z < 0) {
+    constexpr int AT_ONCE = WEIGH_THREADS / D;     // heads
+    for (int i = tid / D; i < REP; i += AT_ONCE)
+      attn_merge<D, false>(scratch, gate, out, row, h * REP + i, qh, splits, tid % D, D, SharedParts());
+    return;
+  }
+  auto factor = [&](int r, int i) {                // by a warp
+    const float2* ml = weighed.ml + (static_cast<size_t>(r) * qh + h * REP + i) * splits;
+    const float2 own = lane < splits ? ml[lane] : make_float2(-INFINITY, 0.f);
+    const float m = warp_max(own.x);
+    const float l = warp_sum(own.x == -INFINITY ? 0.f : own.y * exp2f(own.x - m));
+    return make_float2(m, l > 0.f ? 1.f / l : l == 0.f ? 0.f : l);
+  };
+  const int pos = row_pos[row], req = row_req[row], limit = min(weighed.keys, capacity);
+  int other_pos = tid < rows ? row_pos[tid] : -1, other_req = tid < rows ? row_req[tid] : 0;
+  float2 own_f = make_float2(0.f, 0.f);
+  if (warp < REP) own_f = factor(row, warp);
+  if (pos < 0) return;
+  float4 v[2][REP];                                // scores of a row and of the next one
+  auto ask = [&](int b, int r, int n) {
+#pragma unroll
+    for (int i = 0; i < REP; ++i)
+      if (key < n)
+        v[b][i] = *reinterpret_cast<const float4*>(
+            weighed.scores + (static_cast<size_t>(r) * qh + h * REP + i) * weighed.keys + key);
+  };
+  const int own_n = min(pos + 1, limit);
+  ask(0, row, own_n);
+  const float* from = weights + req * slot_stride + h * head_stride;
+  float so_far[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) so_far[k] = key + k < own_n ? from[key + k] : 0.f;
+  // ---- the request's rows: none before this one
+  int count = 0;
+  bool mine = true;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   int seen = 0;                                    // keys that some row of the request sees
-  for (int r0 = 0; r0 < rows; r0 += WEIGH_THREADS) {
-    const int mine = r0 + tid;
-    const bool same = mine < rows && row_req[mine] == req && row_pos[mine] >= 0;
-    const unsigned votes = __ballot_sync(0xffffffffu, same);
-    if (__syncthreads_or(same && mine < row)) return;             // an earlier row's CTA has it
-    if (lane == 0) s_same[warp] = votes;
-    __syncthreads();
-    for (int w = 0; w < WEIGH_THREADS / 32; ++w) {
-      for (unsigned left = s_same[w]; left != 0; left &= left - 1) {
-        const int r = r0 + 32 * w + __ffs(left) - 1;
-        const int n = min(min(row_pos[r] + 1, weighed.keys), capacity);
-        seen = max(seen, n);
-        if (static_cast<int>(blockIdx.z) * WEIGH_KEYS >= n) continue;
-        const size_t head0 = static_cast<size_t>(r) * qh + h * rep;
-        __syncthreads();                           // (the factors of the row before are used)
-        if (warp < rep) {
-          const float2* ml = weighed.ml + (head0 + warp) * splits;
-          const float2 own = lane < splits ? ml[lane] : make_float2(-INFINITY, 0.f);
-          const float m = warp_max(own.x);
-          const float l = warp_sum(own.x == -INFINITY ? 0.f : own.y * exp2f(own.x - m));
-          if (lane == 0) s_f[warp] = make_float2(m, l > 0.f ? 1.f / l : l == 0.f ? 0.f : l);
-        }
-        __syncthreads();
-        if (key >= n) continue;
-        for (int i = 0; i < rep; ++i) {
-          const float2 f = s_f[i];
-          const float* from = weighed.scores + (head0 + i) * weighed.keys + key;
-          const float4 v = *reinterpret_cast<const float4*>(from);
-          const float s[4] = {v.x, v.y, v.z, v.w};
+  auto weigh = [&](int b, int n, const float2* f) {
+    seen = max(seen, n);
+    if (key >= n) return;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (key + k < n) acc[k] = fmaf(exp2f(s[k] - f.x), f.y, acc[k]);
-        }
-      }
+    for (int i = 0; i < REP; ++i) {
+      const float s[4] = {v[b][i].x, v[b][i].y, v[b][i].z, v[b][i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (key + k < n) acc[k] = fmaf(exp2f(s[k] - f[i].x), f[i].y, acc[k]);
+    }
+  };
+  // those that are found, in their order; the first one's scores and factors are there
+  auto take = [&](bool first) {
+    for (int x = warp; x < count * REP; x += WEIGH_THREADS / 32) {
+      const int r = x / REP, i = x % REP;
+      const float2 f = first && r == 0 ? own_f : factor(s_rows[r].x, i);
+      if (lane == 0) s_f[r][i] = f;
+    }
+    if (!first) ask(0, s_rows[0].x, s_rows[0].y);
+    __syncthreads();
+    for (int r = 0; r < count; r += 2) {
+      if (r + 1 < count) ask(1, s_rows[r + 1].x, s_rows[r + 1].y);
+      weigh(0, s_rows[r].y, s_f[r]);
+      if (r + 1 >= count) break;
+      if (r + 2 < count) ask(0, s_rows[r + 2].x, s_rows[r + 2].y);
+      weigh(1, s_rows[r + 1].y, s_f[r + 1]);
+    }
+    __syncthreads();
+    count = 0;
+  };
+  bool first = true;
+  for (int r0 = 0; r0 < rows && mine; r0 += WEIGH_THREADS) {
+    const int other = r0 + tid;
+    if (r0 > 0) {
+      other_pos = other < rows ? row_pos[other] : -1;
+      other_req = other < rows ? row_req[other] : 0;
+    }
+    const bool same = other_pos >= 0 && other_req == req;
+    const unsigned votes = __ballot_sync(0xffffffffu, same);
+    if (lane == 0) s_count[warp] = __popc(votes);
+    mine = !__syncthreads_or(same && other < row);               // (else an earlier row's CTA has it)
+    if (!mine) break;
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < WEIGH_THREADS / 32; ++w) {
+      if (w < warp) before += s_count[w];
+      all += s_count[w];
+    }
+    before += __popc(votes & ((1u << lane) - 1u));
+    for (int done = 0; done < all; done += WEIGH_ROWS) {
+      if (same && before >= done && before < done + WEIGH_ROWS)
+        s_rows[before - done] = make_int2(other, min(other_pos + 1, limit));
+      count = min(WEIGH_ROWS, all - done);
+      __syncthreads();
+      take(first);
+      first = false;
     }
     __syncthreads();
   }
-  if (tid == 0 && blockIdx.z == 0 && row_pos[row] >= min(weighed.keys, capacity))
-    report_status(status, STATUS_BAD_INDEX, 0x60);
-  const float* from = weights + req * slot_stride + h * head_stride;
+  if (!mine) return;
+  if (tid == 0 && z == 0 && pos >= limit) report_status(status, STATUS_BAD_INDEX, 0x60);
   float* to = sums + req * sums_slot_stride + h * sums_head_stride;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (key + k < seen) to[key + k] = from[key + k] + acc[k];
+    if (key + k < seen) to[key + k] = (key + k < own_n ? so_far[k] : from[key + k]) + acc[k];
 }
 
 // Whether a launch of the row kernel may start early.  Of 64 and 128 channels three and more CTAs
@@ -1342,7 +1412,7 @@ static int launch_attn(const __half* q, const __half* gate, const int* row_req, 
     start(kernel, SMEM, q, gate, row_req, row_pos, page_table, max_pages, kc, vc, ks, vs, out, qh,
           kvh, splits, scratch, rep, apart_keys, parts, weighed);
   }
-  if (splits > 1)
+  if (splits > 1 && !WEIGH)                        // (weighed calls: see attn_weigh_kernel)
     launch_early(attn_merge_kernel<D, SHARED>, dim3(rows, qh), D < 128 ? 64 : 128, 0, stream,
                  scratch, gate, out, qh, splits, parts);
   return static_cast<int>(cudaGetLastError());
@@ -1443,9 +1513,16 @@ extern "C" int orinfer_attention_weighed(
   CASE(64) CASE(128) CASE(256)
 #undef CASE
   if (e != 0) return e;
-  const dim3 grid(rows, kvh, (w.keys + WEIGH_KEYS - 1) / WEIGH_KEYS);
-  launch_early(attn_weigh_kernel, grid, WEIGH_THREADS, 0, stream, w, row_req, row_pos, weights,
-               slot_stride, head_stride, sums, sums_slot_stride, sums_head_stride, capacity, rows,
-               qh, rep, splits, runtime_status_ptr());
+  const dim3 grid(rows, kvh, (w.keys + WEIGH_KEYS - 1) / WEIGH_KEYS + (splits > 1 ? 1 : 0));
+#define CASE(DD, REP)                                                                               \
+  if (head_dim == DD && rep == REP)                                                                 \
+    launch_early(attn_weigh_kernel<DD, REP>, grid, WEIGH_THREADS, 0, stream, w, row_req, row_pos,   \
+                 weights, slot_stride, head_stride, sums, sums_slot_stride, sums_head_stride,       \
+                 capacity, rows, qh, splits, static_cast<const float*>(parts), gate, out,           \
+                 runtime_status_ptr());
+  CASE(64, 1) CASE(64, 2) CASE(64, 4) CASE(64, 8)
+  CASE(128, 1) CASE(128, 2) CASE(128, 4) CASE(128, 5) CASE(128, 8)
+  CASE(256, 1) CASE(256, 2) CASE(256, 4) CASE(256, 8)
+#undef CASE
   return static_cast<int>(cudaGetLastError());
 }

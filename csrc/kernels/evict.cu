@@ -6,10 +6,11 @@
 // (keys carry their rotary angle).  What is kept goes to fresh pages and the old ones lose a reference,
 // so pages that others share are never written, the move needs no order, and a call repeats.
 //
-// One CTA does the bookkeeping of the pages (the lowest free ones, in the order of the requests).  Then a
-// CTA per request, layer and KV head finds its threshold, the weight of the last key that stays, by
-// three histograms of the weights' bits (11, 11, 10) and walks the keys once: those above the
-// threshold, and of those equal to it the first so many, are copied as they are found.
+// The first kernel looks, the second one changes.  In the first, one CTA does the bookkeeping of the pages (the
+// lowest free ones, in the order of the requests), and beside it one per request, layer and KV head finds
+// its threshold, the weight of the last key that stays, by three histograms of the weights' bits (11, 11,
+// 10), and walks the keys once: those above the threshold, and of those equal to it the first so many, go
+// to a list with their weights.  In the second a CTA fills a fresh page of a layer and head from the list.
 #include "api.h"
 #include "common.cuh"
 
@@ -17,19 +18,21 @@ namespace orinfer {
 namespace ev {
 
 constexpr int PAGE = 128;                          // tokens
-constexpr int PLAN_THREADS = 1024;
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int BLOCK = 4 * THREADS;                 // keys of a step of the walk
 constexpr int BINS = 2048;                         // of a histogram
 constexpr int WORK_HEAD = 4;                       // status, -, -, -
 
-// What the bookkeeping leaves: the first naming of a slot [slots]; per request its tokens [n], its rank
-// among those that are cut (-1: it stays as it is) [n]; fresh pages [n][pages of `keep`]; the table
-// rows as they were [n][max_pages].
+// What the first kernel leaves: the keys that stay and their weights [items][keep]; the first naming of a
+// slot [slots]; per request its rank among those that are cut (-1: it stays as it is) [n]; fresh pages
+// [n][pages of `keep`]; the table rows as they were [n][max_pages].
 struct Work {
-  int *head, *named, *len, *rank, *fresh, *rows;
-  __host__ __device__ Work(int* w, int slots, int n, int kept)
-      : head(w), named(w + WORK_HEAD), len(named + slots), rank(len + n), fresh(rank + n),
+  int* head;
+  int2* list;
+  int *named, *len, *rank, *fresh, *rows;
+  __host__ __device__ Work(int* w, int slots, int n, int kept, size_t items, int keep)
+      : head(w), list(reinterpret_cast<int2*>(w + WORK_HEAD)),
+        named(w + WORK_HEAD + 2 * items * keep), len(named + slots), rank(len + n), fresh(rank + n),
         rows(fresh + static_cast<size_t>(n) * kept) {}
 };
 
@@ -51,20 +54,18 @@ __device__ __forceinline__ int block_rank(bool flag, int* warp_sums, int& total)
   return before + __popc(votes & ((1u << lane) - 1u));
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
-    const int* table, int* table_out, const int* lens, int* lens_out, const int* refs,
-    int* refs_out, const int* list, int n, int slots, int max_pages, int pages, int keep,
-    int* work, int* status_out) {
-  __shared__ int sums[PLAN_THREADS / 32];
+// The bookkeeping, by one CTA: which requests are cut, their fresh pages, the references of all pages.
+__device__ __forceinline__ void make_plan(const Work& w, const int* table, const int* lens, const int* refs,
+                                          int* refs_out, const int* list, int n, int slots,
+                                          int max_pages, int pages, int keep, int* status_out) {
+  __shared__ int sums[32];
   __shared__ int s_wrong;
   const int kept = (keep + PAGE - 1) / PAGE, tid = threadIdx.x;
-  const Work w(work, slots, n, kept);
-  grid_wait();
-  grid_release();
+  if (tid < 32) sums[tid] = 0;                     // (fewer warps than the scan looks at)
   if (tid == 0) s_wrong = 0;
-  for (int s = tid; s < slots; s += PLAN_THREADS) w.named[s] = n;
+  for (int s = tid; s < slots; s += THREADS) w.named[s] = n;
   __syncthreads();
-  for (int i = tid; i < n; i += PLAN_THREADS) {
+  for (int i = tid; i < n; i += THREADS) {
     const int s = list[i];
     if (s >= 0 && s < slots)
       atomicMin(&w.named[s], i);
@@ -73,7 +74,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
   }
   __syncthreads();
   // ---- requests: lengths that fit the table, pages that somebody holds
-  for (int i = tid / 16; i < n; i += PLAN_THREADS / 16) {        // sixteen lanes per request
+  for (int i = tid / 16; i < n; i += THREADS / 16) {        // sixteen lanes per request
     const int s = list[i], lane = tid & 15;
     if (s < 0 || s >= slots) {
       if (lane == 0) w.len[i] = 0;
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
   __syncthreads();
   int status = s_wrong ? 2 : 0;
   int cut = 0;
-  for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
     const int i = i0 + tid;
     const bool mine = i < n && status == 0 && w.len[i] > keep;
     int total;
@@ -103,10 +104,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
   }
   // ---- the free pages in ascending order are theirs
   const long long need = static_cast<long long>(cut) * kept;
-  int found = 0;
-  for (int p0 = 0; p0 < pages; p0 += PLAN_THREADS) {
-    const int p = p0 + tid;
-    const int held = p < pages ? refs[p] : 1;
+  int found = 0, next = tid < pages ? refs[tid] : 1;
+  for (int p0 = 0; p0 < pages; p0 += THREADS) {
+    const int p = p0 + tid, held = next;
+    next = p + THREADS < pages ? refs[p + THREADS] : 1;
     int total;
     const int rank = found + block_rank(p > 0 && held <= 0, sums, total);
     if (p < pages && refs_out != refs) refs_out[p] = held;
@@ -114,12 +115,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     found += total;
   }
   if (status == 0 && found < need) status = 1;
-  if (lens_out != lens)
-    for (int s = tid; s < slots; s += PLAN_THREADS) lens_out[s] = lens[s];
   __syncthreads();
   if (status == 0) {
-    for (int r = tid; r < need; r += PLAN_THREADS) refs_out[w.fresh[r]] = 1;
-    for (int i = tid / 32; i < n; i += PLAN_THREADS / 32) {      // a warp per request
+    for (int r = tid; r < need; r += THREADS) refs_out[w.fresh[r]] = 1;
+    for (int i = tid / 32; i < n; i += THREADS / 32) {      // a warp per request
       const int rank = w.rank[i];
       if (rank < 0) continue;
       const size_t at = static_cast<size_t>(list[i]) * max_pages;
@@ -127,10 +126,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
         const int page = table[at + j];
         w.rows[static_cast<size_t>(i) * max_pages + j] = page;
         if (page > 0) atomicSub(&refs_out[page], 1);
-        if (table_out == table)
-          table_out[at + j] = j < kept ? w.fresh[static_cast<size_t>(rank) * kept + j] : 0;
       }
-      if ((tid & 31) == 0) lens_out[list[i]] = keep;
     }
   }
   if (tid == 0) {
@@ -145,48 +141,31 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return x != x ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// D: channels of a head.  Item (request, layer, head); the CTAs behind the items write the table where
-// it is not changed in place.
-template <int D>
-__global__ void __launch_bounds__(THREADS) move_kernel(
-    const Cache cache, const int* table, int* table_out, const int* list, int n, int slots,
-    int max_pages, int keep, int first, int recent, const float* weights, float* sums,
-    int capacity, int* work, int items) {
-  constexpr int G = D / 64, UNITS = 2 * D / 16;    // 16-byte units of a key and its value
+// Tokens that a CTA moves: all of a thread's loads are in flight at once, eight at most.
+constexpr int move_tokens(int d) { return d > 128 ? PAGE / 2 : PAGE; }
+
+// Item (request, layer, head): CTA 1 + item; CTA 0 does the bookkeeping.
+__global__ void __launch_bounds__(THREADS) select_kernel(
+    const Cache cache, const int* table, const int* lens, const int* refs, int* refs_out,
+    const int* list, int n, int slots, int max_pages, int keep, int first, int recent,
+    const float* weights, int capacity, int* work, int items, int* status_out) {
   __shared__ int s_hist[BINS];
   __shared__ int s_warp[WARPS], s_pick[3];
-  __shared__ int s_from[BLOCK], s_to[BLOCK];       // places of the tokens to be copied
-  const int kept = (keep + PAGE - 1) / PAGE;
-  const Work w(work, slots, n, kept);
+  const Work w(work, slots, n, (keep + PAGE - 1) / PAGE, items, keep);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_wait();
   grid_release();
-  const int status = w.head[0];
-  if (static_cast<int>(blockIdx.x) >= items) {
-    const int total = slots * max_pages;
-    for (int i = (blockIdx.x - items) * THREADS + tid; i < total;
-         i += (gridDim.x - items) * THREADS) {
-      const int s = i / max_pages, j = i % max_pages, who = w.named[s];
-      const int rank = status == 0 && who < n ? w.rank[who] : -1;
-      table_out[i] = rank < 0 ? table[i]
-                     : j < kept ? w.fresh[static_cast<size_t>(rank) * kept + j] : 0;
-    }
+  if (blockIdx.x == 0) {
+    make_plan(w, table, lens, refs, refs_out, list, n, slots, max_pages, cache.pages, keep, status_out);
     return;
   }
-  const int h = blockIdx.x % cache.kvh, layer = blockIdx.x / cache.kvh % cache.layers;
-  const int who = blockIdx.x / cache.kvh / cache.layers;
-  const int slot = list[who];
-  if (slot < 0 || slot >= slots || w.named[slot] != who) return;
+  const int item = blockIdx.x - 1, h = item % cache.kvh, layer = item / cache.kvh % cache.layers;
+  const int slot = list[item / cache.kvh / cache.layers];
+  if (slot < 0 || slot >= slots) return;
+  const int len = lens[slot], lo = first, hi = len - recent;
+  if (len <= keep || len > capacity) return;       // (the latter is found wrong by the bookkeeping)
   const size_t line = (static_cast<size_t>(layer) * slots + slot) * cache.kvh + h;
   const float* from = weights + line * capacity;
-  float* to = sums + line * capacity;
-  const int rank = status == 0 ? w.rank[who] : -1;
-  if (rank < 0) {                                  // it stays as it is
-    if (to != from)
-      for (int i = tid; i < capacity; i += THREADS) to[i] = from[i];
-    return;
-  }
-  const int len = w.len[who], lo = first, hi = len - recent;
 
   // ---- the threshold: `want` keys of [lo, hi) stay; of those whose bits begin as `prefix` (the upper 32 -
   // shift ones), the first `want`, and all above
@@ -197,9 +176,18 @@ __global__ void __launch_bounds__(THREADS) move_kernel(
     const int next = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = 1 << (shift - next);
     for (int i = tid; i < BINS; i += THREADS) s_hist[i] = 0;
     __syncthreads();
-    for (int i = lo + tid; i < hi; i += THREADS) {
-      const uint32_t u = ordered(from[i]);
-      if (pass == 0 || u >> shift == prefix) atomicAdd(&s_hist[u >> next & (bins - 1)], 1);
+    constexpr int AHEAD = 8;                       // loads in flight
+    for (int i0 = lo + tid; i0 < hi; i0 += AHEAD * THREADS) {
+      float x[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (i0 + k * THREADS < hi) x[k] = from[i0 + k * THREADS];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (i0 + k * THREADS >= hi) break;
+        const uint32_t u = ordered(x[k]);
+        if (pass == 0 || u >> shift == prefix) atomicAdd(&s_hist[u >> next & (bins - 1)], 1);
+      }
     }
     __syncthreads();
     // the bin in which the `want`-th from the top lies
@@ -234,23 +222,28 @@ __global__ void __launch_bounds__(THREADS) move_kernel(
   }
 
   // ---- the walk
-  const int8_t* kc = reinterpret_cast<const int8_t*>(cache.bases[layer]);
-  const int8_t* vc = reinterpret_cast<const int8_t*>(cache.bases[cache.layers + layer]);
-  const __half* ks = reinterpret_cast<const __half*>(cache.bases[2 * cache.layers + layer]);
-  const __half* vs = reinterpret_cast<const __half*>(cache.bases[3 * cache.layers + layer]);
-  const int* pages = w.rows + static_cast<size_t>(who) * max_pages;
-  const int* fresh = w.fresh + static_cast<size_t>(rank) * kept;
-  const size_t token = static_cast<size_t>(cache.kvh) * D;
+  int2* stays = w.list + static_cast<size_t>(item) * keep;
   int done = 0, equal = 0;                         // keys kept so far; of them or not, equal to the threshold
+  // a warp takes 128 neighbouring keys, a lane four of them 32 apart, the next ones ahead
+  float ahead[4];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int key = k0 + warp * 128 + k * 32 + lane;
+      ahead[k] = key < len ? from[key] : 0.f;
+    }
+  };
+  load(0);
   for (int k0 = 0; k0 < len; k0 += BLOCK) {
-    // a warp takes 128 neighbouring keys, a lane four of them 32 apart
     float x[4];
     unsigned over[4], same[4];
     int n_over = 0, n_same = 0;
 #pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = ahead[k];
+    load(k0 + BLOCK);
+#pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int key = k0 + warp * 128 + k * 32 + lane;
-      x[k] = key < len ? from[key] : 0.f;
       const bool between = key >= lo && key < hi;
       const uint32_t u = shift < 32 ? ordered(x[k]) >> shift : 0u;
       over[k] = __ballot_sync(0xffffffffu, key < len && (!between || (!none && u > prefix)));
@@ -258,6 +251,7 @@ __global__ void __launch_bounds__(THREADS) move_kernel(
       n_over += __popc(over[k]);
       n_same += __popc(same[k]);
     }
+    __syncthreads();                               // (the counts of the step before are read)
     if (lane == 0) s_warp[warp] = n_over | n_same << 16;
     __syncthreads();
     int o_before = 0, s_before = equal, o_all = 0, s_all = 0;
@@ -272,66 +266,119 @@ __global__ void __launch_bounds__(THREADS) move_kernel(
       s_all += v >> 16;
     }
     // (of the equal ones before a key, at most `want` are kept)
-    const int base = min(equal, want);
+    const int base = done - min(equal, want);
     const unsigned lower = (1u << lane) - 1u;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int eq = s_before + __popc(same[k] & lower);
-      const bool stays = (over[k] >> lane & 1u) || ((same[k] >> lane & 1u) && eq < want);
-      const int at = o_before + __popc(over[k] & lower) + min(eq, want) - base;
-      if (stays) {
-        const int key = k0 + warp * 128 + k * 32 + lane, out = done + at;
-        s_from[at] = pages[key >> 7] * PAGE + (key & 127);
-        s_to[at] = fresh[out >> 7] * PAGE + (out & 127);
-        to[out] = x[k];
-      }
+      if ((over[k] >> lane & 1u) || ((same[k] >> lane & 1u) && eq < want))
+        stays[base + o_before + __popc(over[k] & lower) + min(eq, want)] =
+            make_int2(k0 + warp * 128 + k * 32 + lane, __float_as_int(x[k]));
       o_before += __popc(over[k]);
       s_before += __popc(same[k]);
     }
-    const int count = o_all + min(equal + s_all, want) - base;
+    done = base + o_all + min(equal + s_all, want);
     equal += s_all;
-    __syncthreads();
-    // ---- copies
-    constexpr int BATCH = 4;
-    for (int u0 = tid; u0 < count * UNITS; u0 += BATCH * THREADS) {
-      uint4 v[BATCH];
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        const int u = u0 + b * THREADS, t = u / UNITS, c = u % UNITS;
-        if (t < count) {
-          const int8_t* p = c < UNITS / 2 ? kc : vc;
-          v[b] = *reinterpret_cast<const uint4*>(p + s_from[t] * token + h * D + c % (UNITS / 2) * 16);
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        const int u = u0 + b * THREADS, t = u / UNITS, c = u % UNITS;
-        if (t < count) {
-          int8_t* p = const_cast<int8_t*>(c < UNITS / 2 ? kc : vc);
-          *reinterpret_cast<uint4*>(p + s_to[t] * token + h * D + c % (UNITS / 2) * 16) = v[b];
-        }
-      }
-    }
-    for (int u = tid; u < count * 2 * G; u += THREADS) {
-      const int t = u / (2 * G), c = u % (2 * G);
-      const unsigned short* p = reinterpret_cast<const unsigned short*>(c < G ? ks : vs);
-      unsigned short* o = const_cast<unsigned short*>(p);
-      o[(static_cast<size_t>(s_to[t]) * cache.kvh + h) * G + c % G] =
-          p[(static_cast<size_t>(s_from[t]) * cache.kvh + h) * G + c % G];
-    }
-    done += count;
-    __syncthreads();                               // (the lists are used)
   }
-  for (int i = keep + tid; i < capacity; i += THREADS) to[i] = 0.f;
 }
 
+// D: channels of a head.  CTA (request, layer, part of a fresh page, head): neighbours write what lies side by
+// side.  Those behind them write the table and the lengths.
 template <int D>
-static void launch_move(int blocks, int items, cudaStream_t stream, const Cache& cache, const int* table,
-                        int* table_out, const int* list, int n, int slots, int max_pages, int keep,
-                        int first, int recent, const float* weights, float* sums, int capacity,
-                        int* work) {
-  launch_early(move_kernel<D>, dim3(blocks), THREADS, 0, stream, cache, table, table_out, list, n,
-               slots, max_pages, keep, first, recent, weights, sums, capacity, work, items);
+__global__ void __launch_bounds__(THREADS) move_kernel(
+    const Cache cache, const int* table, int* table_out, const int* lens, int* lens_out,
+    const int* list, int n, int slots, int max_pages, int keep, const float* weights, float* sums,
+    int capacity, int* work, int items) {
+  constexpr int G = D / 64, UNITS = 2 * D / 16;    // 16-byte units of a key and its value
+  constexpr int TOKENS = move_tokens(D);           // of a CTA
+  constexpr int EACH = TOKENS * UNITS / THREADS, S_EACH = TOKENS * 2 * G / THREADS;
+  __shared__ int s_list[TOKENS];                   // sources: places in the cache
+  const int kept = (keep + PAGE - 1) / PAGE, parts = (keep + TOKENS - 1) / TOKENS;
+  const Work w(work, slots, n, kept, items, keep);
+  const int tid = threadIdx.x;
+  grid_wait();
+  grid_release();
+  const int status = w.head[0];
+  const long long moves = static_cast<long long>(items) * parts;
+  if (static_cast<long long>(blockIdx.x) >= moves) {
+    const long long total = static_cast<long long>(slots) * max_pages;
+    const int ctas = gridDim.x - static_cast<int>(moves);
+    for (long long i = (blockIdx.x - moves) * THREADS + tid; i < total + slots;
+         i += static_cast<long long>(ctas) * THREADS) {
+      const int s = static_cast<int>(i < total ? i / max_pages : i - total), who = w.named[s];
+      const int rank = status == 0 && who < n ? w.rank[who] : -1;
+      if (i < total) {
+        const int j = static_cast<int>(i % max_pages);
+        if (rank >= 0)
+          table_out[i] = j < kept ? w.fresh[static_cast<size_t>(rank) * kept + j] : 0;
+        else if (table_out != table)
+          table_out[i] = table[i];
+      } else if (rank >= 0) {
+        lens_out[s] = keep;
+      } else if (lens_out != lens) {
+        lens_out[s] = lens[s];
+      }
+    }
+    return;
+  }
+  const int h = blockIdx.x % cache.kvh, part = blockIdx.x / cache.kvh % parts;
+  const int layer = blockIdx.x / cache.kvh / parts % cache.layers;
+  const int who = blockIdx.x / cache.kvh / parts / cache.layers, slot = list[who];
+  const int item = (who * cache.layers + layer) * cache.kvh + h;
+  if (slot < 0 || slot >= slots || w.named[slot] != who) return;
+  const size_t line = (static_cast<size_t>(layer) * slots + slot) * cache.kvh + h;
+  const float* from = weights + line * capacity;
+  float* to = sums + line * capacity;
+  const int rank = status == 0 ? w.rank[who] : -1;
+  if (rank < 0) {                                  // it stays as it is
+    if (to != from)
+      for (int i = part * THREADS + tid; i < capacity; i += parts * THREADS) to[i] = from[i];
+    return;
+  }
+  const int t0 = part * TOKENS, count = min(TOKENS, keep - t0);
+  if (tid < count) {
+    const int2 v = w.list[static_cast<size_t>(item) * keep + t0 + tid];
+    to[t0 + tid] = __int_as_float(v.y);
+    s_list[tid] = w.rows[static_cast<size_t>(who) * max_pages + (v.x >> 7)] * PAGE + (v.x & 127);
+  }
+  const int page = w.fresh[static_cast<size_t>(rank) * kept + t0 / PAGE];
+  const size_t target = (static_cast<size_t>(page) * PAGE + t0 % PAGE) * cache.kvh + h;
+  for (int i = keep + part * THREADS + tid; i < capacity; i += parts * THREADS) to[i] = 0.f;
+  int8_t* kc = reinterpret_cast<int8_t*>(cache.bases[layer]);
+  int8_t* vc = reinterpret_cast<int8_t*>(cache.bases[cache.layers + layer]);
+  unsigned short* ks = reinterpret_cast<unsigned short*>(cache.bases[2 * cache.layers + layer]);
+  unsigned short* vs = reinterpret_cast<unsigned short*>(cache.bases[3 * cache.layers + layer]);
+  __syncthreads();
+  // all of a thread's loads ahead of its stores
+  uint4 v[EACH];
+  unsigned short sc[S_EACH];
+#pragma unroll
+  for (int b = 0; b < EACH; ++b) {
+    const int t = (b * THREADS + tid) / UNITS, c = tid % UNITS;
+    if (t < count)
+      v[b] = __ldcs(reinterpret_cast<const uint4*>(
+          (c < UNITS / 2 ? kc : vc) + (static_cast<size_t>(s_list[t]) * cache.kvh + h) * D +
+          c % (UNITS / 2) * 16));
+  }
+#pragma unroll
+  for (int b = 0; b < S_EACH; ++b) {
+    const int t = (b * THREADS + tid) / (2 * G), c = tid % (2 * G);
+    if (t < count)
+      sc[b] = (c < G ? ks : vs)[(static_cast<size_t>(s_list[t]) * cache.kvh + h) * G + c % G];
+  }
+#pragma unroll
+  for (int b = 0; b < EACH; ++b) {
+    const int t = (b * THREADS + tid) / UNITS, c = tid % UNITS;
+    if (t < count)
+      __stcs(reinterpret_cast<uint4*>((c < UNITS / 2 ? kc : vc) +
+                                      (target + static_cast<size_t>(t) * cache.kvh) * D +
+                                      c % (UNITS / 2) * 16), v[b]);
+  }
+#pragma unroll
+  for (int b = 0; b < S_EACH; ++b) {
+    const int t = (b * THREADS + tid) / (2 * G), c = tid % (2 * G);
+    if (t < count) (c < G ? ks : vs)[(target + static_cast<size_t>(t) * cache.kvh) * G + c % G] = sc[b];
+  }
 }
 
 }  // namespace ev
@@ -339,9 +386,10 @@ static void launch_move(int blocks, int items, cudaStream_t stream, const Cache&
 
 using namespace orinfer;
 
-extern "C" size_t orinfer_evict_work_words(int slots, int n, int max_pages, int keep) {
+extern "C" size_t orinfer_evict_work_words(int layers, int kvh, int slots, int n, int max_pages, int keep) {
   const size_t kept = (static_cast<size_t>(keep) + ev::PAGE - 1) / ev::PAGE;
-  return ev::WORK_HEAD + slots + 2 * static_cast<size_t>(n) + n * (kept + max_pages);
+  return ev::WORK_HEAD + 2 * static_cast<size_t>(n) * layers * kvh * keep + slots + 2 * static_cast<size_t>(n) +
+         n * (kept + max_pages);
 }
 
 extern "C" int orinfer_evict_keys(const long long* bases, int layers, int kvh, int head_dim, int pages,
@@ -356,21 +404,25 @@ extern "C" int orinfer_evict_keys(const long long* bases, int layers, int kvh, i
       capacity < max_pages * static_cast<long long>(ev::PAGE))
     return -1;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return -1;
-  if (static_cast<long long>(n) * layers * kvh > (1 << 30) ||
-      static_cast<long long>(slots) * max_pages > (1 << 30) ||
+  if ((reinterpret_cast<uintptr_t>(work) & 7) != 0) return -1;
+  const int kept = (keep + ev::PAGE - 1) / ev::PAGE;
+  const long long items = static_cast<long long>(n) * layers * kvh;
+  if (items * kept > (1 << 29) || static_cast<long long>(slots) * max_pages > (1 << 30) ||
       static_cast<long long>(pages) * ev::PAGE > 0x7fffffffLL)
     return -1;
-  launch_early(ev::plan_kernel, dim3(1), ev::PLAN_THREADS, 0, stream, table, table_out, lens,
-               lens_out, refs, refs_out, list, n, slots, max_pages, pages, keep, work, status_out);
-  if (const cudaError_t e = cudaGetLastError()) return static_cast<int>(e);
   const ev::Cache cache{bases, layers, kvh, pages};
-  const int items = n * layers * kvh;
-  const int more = table_out == table ? 0 : (slots * max_pages + 4 * ev::THREADS - 1) / (4 * ev::THREADS);
-  if (items + more == 0) return 0;
-#define CASE(D)                                                                                    \
-  if (head_dim == D)                                                                               \
-    ev::launch_move<D>(items + more, items, stream, cache, table, table_out, list, n, slots, max_pages, \
-                       keep, first, recent, weights, sums, capacity, work);
+  launch_early(ev::select_kernel, dim3(1 + static_cast<unsigned>(items)), ev::THREADS, 0, stream, cache, table,
+               lens, refs, refs_out, list, n, slots, max_pages, keep, first, recent, weights, capacity, work,
+               static_cast<int>(items), status_out);
+  if (const cudaError_t e = cudaGetLastError()) return static_cast<int>(e);
+  const int more = (slots * max_pages + slots + 4 * ev::THREADS - 1) / (4 * ev::THREADS);
+  const int tokens = ev::move_tokens(head_dim), parts = (keep + tokens - 1) / tokens;
+  const dim3 grid(static_cast<unsigned>(items * parts + more));
+#define CASE(D)                                                                                   \
+  if (head_dim == D)                                                                              \
+    launch_early(ev::move_kernel<D>, grid, ev::THREADS, 0, stream, cache, table, table_out, lens, \
+                 lens_out, list, n, slots, max_pages, keep, weights, sums, capacity, work,        \
+                 static_cast<int>(items));
   CASE(64) CASE(128) CASE(256)
 #undef CASE
   return static_cast<int>(cudaGetLastError());

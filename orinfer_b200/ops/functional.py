@@ -292,7 +292,7 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
         ptr(kcache), ptr(vcache), ptr(kscale), ptr(vscale), ptr(out), ptr(weights),
         weights.stride(0), weights.stride(1), ptr(sums), sums.stride(0), sums.stride(1), capacity,
         live, qh, kvh, d, splits, keys, ptr(scratch), max_kv_len or 0, stream()), "attention_weighed")
-    count_launches((3 if splits > 1 else 2) if live else 0)
+    count_launches(2 if live else 0)
     return out
 
 
@@ -744,14 +744,14 @@ def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: t
           f"{keep} keys of {width * 128} with {first} first and {recent} last ones")
     _current(cache.device)
     status = torch.empty(1, dtype=torch.int32, device=cache.device)
-    work = torch.empty(native.lib().orinfer_evict_work_words(total, n, width, keep),
-                       dtype=torch.int32, device=cache.device)
+    work = torch.empty(native.lib().orinfer_evict_work_words(
+        cache.layers, cache.kvh, total, n, width, keep), dtype=torch.int32, device=cache.device)
     check(native.lib().orinfer_evict_keys(
         cache.bases.data_ptr(), cache.layers, cache.kvh, cache.head_dim, cache.pages,
         table.data_ptr(), t.data_ptr(), lens.data_ptr(), l.data_ptr(), refs.data_ptr(), r.data_ptr(),
         slots.data_ptr(), n, total, width, keep, first, recent, weights.data_ptr(), sums.data_ptr(),
         weights.shape[3], work.data_ptr(), status.data_ptr(), stream()), "evict_keys")
-    count_launches(2 if n or t is not table else 1)
+    count_launches(2)
     return t, l, r, status
 
 

@@ -98,7 +98,7 @@ def _load() -> ctypes.CDLL:
         "orinfer_copy_pages": ([P, P, P, I, I, P, P, I, P], I),
         "orinfer_fork_pages": ([P, P, P, I, I, P, P, P, P, P, P, P, P, I, I, I, P, P, P], I),
         "orinfer_free_pages": ([P, P, P, P, P, P, P, I, I, I, I, P], I),
-        "orinfer_evict_work_words": ([I, I, I, I], c_size_t),
+        "orinfer_evict_work_words": ([I, I, I, I, I, I], c_size_t),
         "orinfer_evict_keys": ([P, I, I, I, I, P, P, P, P, P, P, P, I, I, I, I, I, I, P, P, I, P, P,
                                 P], I),
         "orinfer_compact_pages": ([P, P, P, I, I, P, P, P, P, P, I, I, P, P], I),
