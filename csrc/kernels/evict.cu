@@ -11,6 +11,8 @@
 // its threshold, the weight of the last key that stays, by three histograms of the weights' bits (11, 11,
 // 10), and walks the keys once: those above the threshold, and of those equal to it the first so many, go
 // to a list with their weights.  In the second a CTA fills a fresh page of a layer and head from the list.
+#include <type_traits>
+
 #include "api.h"
 #include "common.cuh"
 
@@ -18,8 +20,9 @@ namespace orinfer {
 namespace ev {
 
 constexpr int PAGE = 128;                          // tokens
-constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int BLOCK = 4 * THREADS;                 // keys of a step of the walk
+constexpr int THREADS = 256, WARPS = THREADS / 32;               // of the first kernel
+constexpr int MOVE_THREADS = 256;                  // and of the second
+constexpr int LANE_KEYS = 8, BLOCK = LANE_KEYS * THREADS;        // keys of a step of the walk
 constexpr int BINS = 2048;                         // of a histogram
 constexpr int WORK_HEAD = 4;                       // status, -, -, -
 
@@ -224,26 +227,26 @@ __global__ void __launch_bounds__(THREADS) select_kernel(
   // ---- the walk
   int2* stays = w.list + static_cast<size_t>(item) * keep;
   int done = 0, equal = 0;                         // keys kept so far; of them or not, equal to the threshold
-  // a warp takes 128 neighbouring keys, a lane four of them 32 apart, the next ones ahead
-  float ahead[4];
+  // a warp takes 256 neighbouring keys, a lane eight of them 32 apart, the next ones ahead
+  float ahead[LANE_KEYS];
   auto load = [&](int k0) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int key = k0 + warp * 128 + k * 32 + lane;
+    for (int k = 0; k < LANE_KEYS; ++k) {
+      const int key = k0 + warp * (32 * LANE_KEYS) + k * 32 + lane;
       ahead[k] = key < len ? from[key] : 0.f;
     }
   };
   load(0);
   for (int k0 = 0; k0 < len; k0 += BLOCK) {
-    float x[4];
-    unsigned over[4], same[4];
+    float x[LANE_KEYS];
+    unsigned over[LANE_KEYS], same[LANE_KEYS];
     int n_over = 0, n_same = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = ahead[k];
+    for (int k = 0; k < LANE_KEYS; ++k) x[k] = ahead[k];
     load(k0 + BLOCK);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int key = k0 + warp * 128 + k * 32 + lane;
+    for (int k = 0; k < LANE_KEYS; ++k) {
+      const int key = k0 + warp * (32 * LANE_KEYS) + k * 32 + lane;
       const bool between = key >= lo && key < hi;
       const uint32_t u = shift < 32 ? ordered(x[k]) >> shift : 0u;
       over[k] = __ballot_sync(0xffffffffu, key < len && (!between || (!none && u > prefix)));
@@ -269,11 +272,11 @@ __global__ void __launch_bounds__(THREADS) select_kernel(
     const int base = done - min(equal, want);
     const unsigned lower = (1u << lane) - 1u;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < LANE_KEYS; ++k) {
       const int eq = s_before + __popc(same[k] & lower);
       if ((over[k] >> lane & 1u) || ((same[k] >> lane & 1u) && eq < want))
         stays[base + o_before + __popc(over[k] & lower) + min(eq, want)] =
-            make_int2(k0 + warp * 128 + k * 32 + lane, __float_as_int(x[k]));
+            make_int2(k0 + warp * (32 * LANE_KEYS) + k * 32 + lane, __float_as_int(x[k]));
       o_before += __popc(over[k]);
       s_before += __popc(same[k]);
     }
@@ -285,26 +288,27 @@ __global__ void __launch_bounds__(THREADS) select_kernel(
 // D: channels of a head.  CTA (request, layer, part of a fresh page, head): neighbours write what lies side by
 // side.  Those behind them write the table and the lengths.
 template <int D>
-__global__ void __launch_bounds__(THREADS) move_kernel(
+__global__ void __launch_bounds__(MOVE_THREADS) move_kernel(
     const Cache cache, const int* table, int* table_out, const int* lens, int* lens_out,
     const int* list, int n, int slots, int max_pages, int keep, const float* weights, float* sums,
     int capacity, int* work, int items) {
   constexpr int G = D / 64, UNITS = 2 * D / 16;    // 16-byte units of a key and its value
   constexpr int TOKENS = move_tokens(D);           // of a CTA
-  constexpr int EACH = TOKENS * UNITS / THREADS, S_EACH = TOKENS * 2 * G / THREADS;
+  constexpr int EACH = TOKENS * UNITS / MOVE_THREADS;
+  static_assert(2 * TOKENS <= MOVE_THREADS, "a thread has the scales of a key or a value");
+  using Scales = std::conditional_t<G == 1, unsigned short, std::conditional_t<G == 2, uint32_t, uint2>>;
   __shared__ int s_list[TOKENS];                   // sources: places in the cache
   const int kept = (keep + PAGE - 1) / PAGE, parts = (keep + TOKENS - 1) / TOKENS;
   const Work w(work, slots, n, kept, items, keep);
   const int tid = threadIdx.x;
   grid_wait();
   grid_release();
-  const int status = w.head[0];
   const long long moves = static_cast<long long>(items) * parts;
   if (static_cast<long long>(blockIdx.x) >= moves) {
     const long long total = static_cast<long long>(slots) * max_pages;
-    const int ctas = gridDim.x - static_cast<int>(moves);
-    for (long long i = (blockIdx.x - moves) * THREADS + tid; i < total + slots;
-         i += static_cast<long long>(ctas) * THREADS) {
+    const int status = w.head[0], ctas = gridDim.x - static_cast<int>(moves);
+    for (long long i = (blockIdx.x - moves) * MOVE_THREADS + tid; i < total + slots;
+         i += static_cast<long long>(ctas) * MOVE_THREADS) {
       const int s = static_cast<int>(i < total ? i / max_pages : i - total), who = w.named[s];
       const int rank = status == 0 && who < n ? w.rank[who] : -1;
       if (i < total) {
@@ -323,62 +327,55 @@ __global__ void __launch_bounds__(THREADS) move_kernel(
   }
   const int h = blockIdx.x % cache.kvh, part = blockIdx.x / cache.kvh % parts;
   const int layer = blockIdx.x / cache.kvh / parts % cache.layers;
-  const int who = blockIdx.x / cache.kvh / parts / cache.layers, slot = list[who];
+  const int who = blockIdx.x / cache.kvh / parts / cache.layers;
   const int item = (who * cache.layers + layer) * cache.kvh + h;
-  if (slot < 0 || slot >= slots || w.named[slot] != who) return;
+  const int t0 = part * TOKENS, count = min(TOKENS, keep - t0);
+  // (what does not wait for one another is asked for together: a CTA is a chain of loads)
+  const int status = w.head[0], slot = list[who], ranked = w.rank[who];
+  int2 mine = make_int2(0, 0);
+  if (tid < count) mine = w.list[static_cast<size_t>(item) * keep + t0 + tid];
+  if (slot < 0 || slot >= slots) return;
   const size_t line = (static_cast<size_t>(layer) * slots + slot) * cache.kvh + h;
   const float* from = weights + line * capacity;
   float* to = sums + line * capacity;
-  const int rank = status == 0 ? w.rank[who] : -1;
-  if (rank < 0) {                                  // it stays as it is
-    if (to != from)
-      for (int i = part * THREADS + tid; i < capacity; i += parts * THREADS) to[i] = from[i];
+  const int rank = status == 0 ? ranked : -1;
+  if (rank < 0) {                                  // it stays as it is, or is named again
+    if (to != from && (status != 0 || w.named[slot] == who))
+      for (int i = part * MOVE_THREADS + tid; i < capacity; i += parts * MOVE_THREADS) to[i] = from[i];
     return;
   }
-  const int t0 = part * TOKENS, count = min(TOKENS, keep - t0);
   if (tid < count) {
-    const int2 v = w.list[static_cast<size_t>(item) * keep + t0 + tid];
-    to[t0 + tid] = __int_as_float(v.y);
-    s_list[tid] = w.rows[static_cast<size_t>(who) * max_pages + (v.x >> 7)] * PAGE + (v.x & 127);
+    s_list[tid] = w.rows[static_cast<size_t>(who) * max_pages + (mine.x >> 7)] * PAGE + (mine.x & 127);
+    to[t0 + tid] = __int_as_float(mine.y);
   }
   const int page = w.fresh[static_cast<size_t>(rank) * kept + t0 / PAGE];
   const size_t target = (static_cast<size_t>(page) * PAGE + t0 % PAGE) * cache.kvh + h;
-  for (int i = keep + part * THREADS + tid; i < capacity; i += parts * THREADS) to[i] = 0.f;
+  for (int i = keep + part * MOVE_THREADS + tid; i < capacity; i += parts * MOVE_THREADS) to[i] = 0.f;
   int8_t* kc = reinterpret_cast<int8_t*>(cache.bases[layer]);
   int8_t* vc = reinterpret_cast<int8_t*>(cache.bases[cache.layers + layer]);
-  unsigned short* ks = reinterpret_cast<unsigned short*>(cache.bases[2 * cache.layers + layer]);
-  unsigned short* vs = reinterpret_cast<unsigned short*>(cache.bases[3 * cache.layers + layer]);
+  Scales* scales = reinterpret_cast<Scales*>(cache.bases[(tid & 1 ? 3 : 2) * cache.layers + layer]);
   __syncthreads();
   // all of a thread's loads ahead of its stores
   uint4 v[EACH];
-  unsigned short sc[S_EACH];
+  Scales sc;
 #pragma unroll
   for (int b = 0; b < EACH; ++b) {
-    const int t = (b * THREADS + tid) / UNITS, c = tid % UNITS;
+    const int t = (b * MOVE_THREADS + tid) / UNITS, c = tid % UNITS;
     if (t < count)
-      v[b] = __ldcs(reinterpret_cast<const uint4*>(
-          (c < UNITS / 2 ? kc : vc) + (static_cast<size_t>(s_list[t]) * cache.kvh + h) * D +
-          c % (UNITS / 2) * 16));
+      v[b] = *reinterpret_cast<const uint4*>((c < UNITS / 2 ? kc : vc) +
+                                             (static_cast<size_t>(s_list[t]) * cache.kvh + h) * D +
+                                             c % (UNITS / 2) * 16);
   }
-#pragma unroll
-  for (int b = 0; b < S_EACH; ++b) {
-    const int t = (b * THREADS + tid) / (2 * G), c = tid % (2 * G);
-    if (t < count)
-      sc[b] = (c < G ? ks : vs)[(static_cast<size_t>(s_list[t]) * cache.kvh + h) * G + c % G];
-  }
+  if (tid >> 1 < count) sc = scales[static_cast<size_t>(s_list[tid >> 1]) * cache.kvh + h];
 #pragma unroll
   for (int b = 0; b < EACH; ++b) {
-    const int t = (b * THREADS + tid) / UNITS, c = tid % UNITS;
+    const int t = (b * MOVE_THREADS + tid) / UNITS, c = tid % UNITS;
     if (t < count)
-      __stcs(reinterpret_cast<uint4*>((c < UNITS / 2 ? kc : vc) +
-                                      (target + static_cast<size_t>(t) * cache.kvh) * D +
-                                      c % (UNITS / 2) * 16), v[b]);
+      *reinterpret_cast<uint4*>((c < UNITS / 2 ? kc : vc) +
+                                (target + static_cast<size_t>(t) * cache.kvh) * D +
+                                c % (UNITS / 2) * 16) = v[b];
   }
-#pragma unroll
-  for (int b = 0; b < S_EACH; ++b) {
-    const int t = (b * THREADS + tid) / (2 * G), c = tid % (2 * G);
-    if (t < count) (c < G ? ks : vs)[(target + static_cast<size_t>(t) * cache.kvh) * G + c % G] = sc[b];
-  }
+  if (tid >> 1 < count) scales[target + static_cast<size_t>(tid >> 1) * cache.kvh] = sc;
 }
 
 }  // namespace ev
@@ -415,12 +412,12 @@ extern "C" int orinfer_evict_keys(const long long* bases, int layers, int kvh, i
                lens, refs, refs_out, list, n, slots, max_pages, keep, first, recent, weights, capacity, work,
                static_cast<int>(items), status_out);
   if (const cudaError_t e = cudaGetLastError()) return static_cast<int>(e);
-  const int more = (slots * max_pages + slots + 4 * ev::THREADS - 1) / (4 * ev::THREADS);
+  const int more = (slots * max_pages + slots + 4 * ev::MOVE_THREADS - 1) / (4 * ev::MOVE_THREADS);
   const int tokens = ev::move_tokens(head_dim), parts = (keep + tokens - 1) / tokens;
   const dim3 grid(static_cast<unsigned>(items * parts + more));
 #define CASE(D)                                                                                   \
   if (head_dim == D)                                                                              \
-    launch_early(ev::move_kernel<D>, grid, ev::THREADS, 0, stream, cache, table, table_out, lens, \
+    launch_early(ev::move_kernel<D>, grid, ev::MOVE_THREADS, 0, stream, cache, table, table_out, lens, \
                  lens_out, list, n, slots, max_pages, keep, weights, sums, capacity, work,        \
                  static_cast<int>(items));
   CASE(64) CASE(128) CASE(256)

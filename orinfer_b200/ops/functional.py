@@ -705,8 +705,9 @@ class KeyCache:
         for layer in zip(k, v, ks, vs):
             got = _cached(self.device, any_table, *layer)
             _need(layer[0].dtype == layer[1].dtype == torch.int8 and got == (*k[0].shape[:1], *k[0].shape[2:])
-                  and layer[0].data_ptr() % 16 == layer[1].data_ptr() % 16 == 0,
-                  "layers alike, keys and values on 16-byte boundaries")
+                  and layer[0].data_ptr() % 16 == layer[1].data_ptr() % 16 == 0
+                  and all(t.data_ptr() % (got[2] // 32) == 0 for t in layer[2:]),
+                  "layers alike, keys and values on 16-byte boundaries, scales on those of a key's")
         self.pages, _, self.kvh, self.head_dim = k[0].shape
         self.bases = torch.tensor([t.data_ptr() for t in self.tensors], dtype=torch.int64,
                                   device=self.device)
