@@ -1190,34 +1190,34 @@ __global__ void attn_merge_kernel(
 // shows in the sums, and a row's output does not wait for them.  Where the keys are split, the CTAs of
 // the first column put the outputs together meanwhile.
 //
-// A CTA takes WEIGH_KEYS keys of a row and KV head.  Scores are written once by the row kernels and read
-// once here, 4 rep bytes a key beside the 2 D and more of its key and value, mostly within L2.  It is a
-// chain of loads that wait for each other, so what can be asked for at once is: scores and factors of the
-// CTA's own row before it is known whether an earlier row's CTA has them, the factors of the rows behind it
-// together, their scores a row ahead.
-constexpr int WEIGH_THREADS = 256, WEIGH_KEYS = 4 * WEIGH_THREADS, WEIGH_ROWS = 32;
+// A CTA takes WEIGH_KEYS keys of a row and some KV heads, as many as let the launch start early
+// (EARLY_CTAS).  Scores are written once by the row kernels and read once here, 4 rep bytes a key beside
+// the 2 D and more of its key and value, mostly within L2.  It is a chain of loads that wait for each
+// other, so what can be asked for at once is: the scores and factors of the CTA's own row before it is
+// known whether an earlier row's CTA has them.
+constexpr int WEIGH_THREADS = 256, WEIGH_KEYS = 4 * WEIGH_THREADS;
 template <int D, int REP>
-__global__ void __launch_bounds__(WEIGH_THREADS) attn_weigh_kernel(
+__global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_kernel(
     const Weighed weighed, const int* row_req, const int* row_pos, const float* weights,
     long long slot_stride, long long head_stride, float* sums, long long sums_slot_stride,
-    long long sums_head_stride, int capacity, int rows, int qh, int splits, const float* scratch,
-    const __half* gate, __half* __restrict__ out, int* status) {
-  __shared__ int2 s_rows[WEIGH_ROWS];              // rows of the request, in their order, and their keys
+    long long sums_head_stride, int capacity, int rows, int qh, int splits, int heads,
+    const float* scratch, const __half* gate, __half* __restrict__ out, int* status) {
+  __shared__ int2 s_rows[WEIGH_THREADS];           // rows of the request, in their order, and their keys
   __shared__ int s_count[WEIGH_THREADS / 32];
-  __shared__ float2 s_f[WEIGH_ROWS][REP];          // a head's reference and 1 / sum
+  __shared__ float2 s_f[WEIGH_THREADS][REP];       // a head's reference and 1 / sum
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_wait();
   grid_release();
-  const int row = blockIdx.x, h = blockIdx.y, z = static_cast<int>(blockIdx.z) - (splits > 1);
+  const int row = blockIdx.x, z = static_cast<int>(blockIdx.z) - (splits > 1);
+  const int h_lo = blockIdx.y * heads, h_hi = min(h_lo + heads, qh / REP);
   const int key = z * WEIGH_KEYS + 4 * tid;
   if (z < 0) {
-    constexpr int AT_ONCE = WEIGH_THREADS / D;     // heads
-    for (int i = tid / D; i < REP; i += AT_ONCE)
-      attn_merge<D, false>(scratch, gate, out, row, h * REP + i, qh, splits, tid % D, D, SharedParts());
+    for (int i = h_lo * REP + tid / D; i < h_hi * REP; i += WEIGH_THREADS / D)
+      attn_merge<D, false>(scratch, gate, out, row, i, qh, splits, tid % D, D, SharedParts());
     return;
   }
-  auto factor = [&](int r, int i) {                // by a warp
-    const float2* ml = weighed.ml + (static_cast<size_t>(r) * qh + h * REP + i) * splits;
+  auto factor = [&](int r, int head) {             // by a warp
+    const float2* ml = weighed.ml + (static_cast<size_t>(r) * qh + head) * splits;
     const float2 own = lane < splits ? ml[lane] : make_float2(-INFINITY, 0.f);
     const float m = warp_max(own.x);
     const float l = warp_sum(own.x == -INFINITY ? 0.f : own.y * exp2f(own.x - m));
@@ -1226,59 +1226,24 @@ __global__ void __launch_bounds__(WEIGH_THREADS) attn_weigh_kernel(
   const int pos = row_pos[row], req = row_req[row], limit = min(weighed.keys, capacity);
   int other_pos = tid < rows ? row_pos[tid] : -1, other_req = tid < rows ? row_req[tid] : 0;
   float2 own_f = make_float2(0.f, 0.f);
-  if (warp < REP) own_f = factor(row, warp);
+  if (warp < REP) own_f = factor(row, h_lo * REP + warp);
   if (pos < 0) return;
-  float4 v[2][REP];                                // scores of a row and of the next one
-  auto ask = [&](int b, int r, int n) {
+  if (tid == 0 && z == 0 && blockIdx.y == 0 && pos >= limit)
+    report_status(status, STATUS_BAD_INDEX, 0x60);
+  float4 v[REP];                                   // scores of a row
+  auto ask = [&](int r, int n, int h) {
 #pragma unroll
     for (int i = 0; i < REP; ++i)
       if (key < n)
-        v[b][i] = *reinterpret_cast<const float4*>(
+        v[i] = *reinterpret_cast<const float4*>(
             weighed.scores + (static_cast<size_t>(r) * qh + h * REP + i) * weighed.keys + key);
   };
   const int own_n = min(pos + 1, limit);
-  ask(0, row, own_n);
-  const float* from = weights + req * slot_stride + h * head_stride;
-  float so_far[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) so_far[k] = key + k < own_n ? from[key + k] : 0.f;
-  // ---- the request's rows: none before this one
-  int count = 0;
-  bool mine = true;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  int seen = 0;                                    // keys that some row of the request sees
-  auto weigh = [&](int b, int n, const float2* f) {
-    seen = max(seen, n);
-    if (key >= n) return;
-#pragma unroll
-    for (int i = 0; i < REP; ++i) {
-      const float s[4] = {v[b][i].x, v[b][i].y, v[b][i].z, v[b][i].w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (key + k < n) acc[k] = fmaf(exp2f(s[k] - f[i].x), f[i].y, acc[k]);
-    }
-  };
-  // those that are found, in their order; the first one's scores and factors are there
-  auto take = [&](bool first) {
-    for (int x = warp; x < count * REP; x += WEIGH_THREADS / 32) {
-      const int r = x / REP, i = x % REP;
-      const float2 f = first && r == 0 ? own_f : factor(s_rows[r].x, i);
-      if (lane == 0) s_f[r][i] = f;
-    }
-    if (!first) ask(0, s_rows[0].x, s_rows[0].y);
-    __syncthreads();
-    for (int r = 0; r < count; r += 2) {
-      if (r + 1 < count) ask(1, s_rows[r + 1].x, s_rows[r + 1].y);
-      weigh(0, s_rows[r].y, s_f[r]);
-      if (r + 1 >= count) break;
-      if (r + 2 < count) ask(0, s_rows[r + 2].x, s_rows[r + 2].y);
-      weigh(1, s_rows[r + 1].y, s_f[r + 1]);
-    }
-    __syncthreads();
-    count = 0;
-  };
+  ask(row, own_n, h_lo);
+  // ---- the request's rows, as many as there are among WEIGH_THREADS at a time: none before this one
   bool first = true;
-  for (int r0 = 0; r0 < rows && mine; r0 += WEIGH_THREADS) {
+  int done = 0;                                    // keys whose sums are there
+  for (int r0 = 0; r0 < rows; r0 += WEIGH_THREADS) {
     const int other = r0 + tid;
     if (r0 > 0) {
       other_pos = other < rows ? row_pos[other] : -1;
@@ -1287,31 +1252,56 @@ __global__ void __launch_bounds__(WEIGH_THREADS) attn_weigh_kernel(
     const bool same = other_pos >= 0 && other_req == req;
     const unsigned votes = __ballot_sync(0xffffffffu, same);
     if (lane == 0) s_count[warp] = __popc(votes);
-    mine = !__syncthreads_or(same && other < row);               // (else an earlier row's CTA has it)
-    if (!mine) break;
-    int before = 0, all = 0;
+    if (__syncthreads_or(same && other < row)) return;           // an earlier row's CTA has them
+    int at = __popc(votes & ((1u << lane) - 1u)), count = 0;
 #pragma unroll
     for (int w = 0; w < WEIGH_THREADS / 32; ++w) {
-      if (w < warp) before += s_count[w];
-      all += s_count[w];
+      if (w < warp) at += s_count[w];
+      count += s_count[w];
     }
-    before += __popc(votes & ((1u << lane) - 1u));
-    for (int done = 0; done < all; done += WEIGH_ROWS) {
-      if (same && before >= done && before < done + WEIGH_ROWS)
-        s_rows[before - done] = make_int2(other, min(other_pos + 1, limit));
-      count = min(WEIGH_ROWS, all - done);
-      __syncthreads();
-      take(first);
-      first = false;
-    }
+    if (same) s_rows[at] = make_int2(other, min(other_pos + 1, limit));
     __syncthreads();
-  }
-  if (!mine) return;
-  if (tid == 0 && z == 0 && pos >= limit) report_status(status, STATUS_BAD_INDEX, 0x60);
-  float* to = sums + req * sums_slot_stride + h * sums_head_stride;
+    if (count == 0) continue;
+    int seen = 0;                                  // keys that some of the rows see
+    for (int h = h_lo; h < h_hi; ++h) {
+      const float* from = weights + req * slot_stride + h * head_stride;
+      float* to = sums + req * sums_slot_stride + h * sums_head_stride;
+      float so_far[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+      const int2 one = s_rows[0];
+      if (!first) ask(one.x, one.y, h);
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (key + k < seen) to[key + k] = (key + k < own_n ? so_far[k] : from[key + k]) + acc[k];
+      for (int k = 0; k < 4; ++k)
+        so_far[k] = key + k < one.y ? (key + k < done ? to : from)[key + k] : 0.f;
+      for (int x = warp; x < count * REP; x += WEIGH_THREADS / 32) {
+        const int r = x / REP, i = x % REP;
+        const float2 f = first && r == 0 ? own_f : factor(s_rows[r].x, h * REP + i);
+        if (lane == 0) s_f[r][i] = f;
+      }
+      __syncthreads();
+      for (int r = 0; r < count; ++r) {
+        const int n = s_rows[r].y;
+        seen = max(seen, n);
+        if (r > 0) ask(s_rows[r].x, n, h);
+        if (key < n) {
+#pragma unroll
+          for (int i = 0; i < REP; ++i) {
+            const float s[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            const float2 f = s_f[r][i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (key + k < n) acc[k] = fmaf(exp2f(s[k] - f.x), f.y, acc[k]);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (key + k < seen)
+          to[key + k] = (key + k < one.y ? so_far[k] : (key + k < done ? to : from)[key + k]) + acc[k];
+      first = false;
+      __syncthreads();                             // (the factors are used)
+    }
+    done = max(done, seen);
+  }
 }
 
 // Whether a launch of the row kernel may start early.  Of 64 and 128 channels three and more CTAs
@@ -1513,12 +1503,16 @@ extern "C" int orinfer_attention_weighed(
   CASE(64) CASE(128) CASE(256)
 #undef CASE
   if (e != 0) return e;
-  const dim3 grid(rows, kvh, (w.keys + WEIGH_KEYS - 1) / WEIGH_KEYS + (splits > 1 ? 1 : 0));
+  const int columns = (w.keys + WEIGH_KEYS - 1) / WEIGH_KEYS + (splits > 1 ? 1 : 0);
+  const long long ctas = static_cast<long long>(rows) * kvh * columns;
+  const int per = static_cast<int>(ctas <= EARLY_CTAS ? 1 : (ctas + EARLY_CTAS - 1) / EARLY_CTAS);
+  const int per_cta = per < kvh ? per : kvh;
+  const dim3 grid(rows, (kvh + per_cta - 1) / per_cta, columns);
 #define CASE(DD, REP)                                                                               \
   if (head_dim == DD && rep == REP)                                                                 \
     launch_early(attn_weigh_kernel<DD, REP>, grid, WEIGH_THREADS, 0, stream, w, row_req, row_pos,   \
                  weights, slot_stride, head_stride, sums, sums_slot_stride, sums_head_stride,       \
-                 capacity, rows, qh, splits, static_cast<const float*>(parts), gate, out,           \
+                 capacity, rows, qh, splits, per_cta, static_cast<const float*>(parts), gate, out,  \
                  runtime_status_ptr());
   CASE(64, 1) CASE(64, 2) CASE(64, 4) CASE(64, 8)
   CASE(128, 1) CASE(128, 2) CASE(128, 4) CASE(128, 5) CASE(128, 8)
