@@ -13,7 +13,7 @@ python/orinfer_build/models/qwen35/build.py:802-1116.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
@@ -45,6 +45,10 @@ class KVPool:
     def cache_pages(self) -> F.CachePages:
         """The pool as ``fork_pages``, ``compact_pages`` and ``copy_pages`` address it."""
         return F.CachePages([*self.k, *self.v, *self.ks, *self.vs])
+
+    def key_cache(self, layers: Optional[int] = None) -> F.KeyCache:
+        """The first ``layers`` layers (default: all) as ``evict_keys`` addresses them."""
+        return F.KeyCache(self.k[:layers], self.v[:layers], self.ks[:layers], self.vs[:layers])
 
     @staticmethod
     def bytes_per_page(cfg: ModelConfig, extra_layers: int = 0) -> int:
@@ -148,6 +152,14 @@ class Packet:
     # Single rows whose contexts begin with the same pages (samples of one prompt): the plan of
     # their attention, for exactly the packet's rows.  None = every row reads all of its keys.
     shared: Optional[F.SharedPrefix] = None
+    # Requests whose cache is cut down: ``weights`` has fp32 [slots, KV heads, keys] of every
+    # attention layer, which the packet's rows add the attention weight of each key to; of the
+    # prefill chunks only the rows of ``weigh_chunks`` (as ``chunks``) where that is given.
+    # ``rope_pos`` int32 [rows] gives the rotary positions where ``row_pos`` counts the keys that
+    # are left.
+    weights: Optional[Sequence[torch.Tensor]] = None
+    weigh_chunks: Optional[torch.Tensor] = None
+    rope_pos: Optional[torch.Tensor] = None
 
     def ensure_segments(self) -> None:
         if self.segments is not None:
@@ -215,6 +227,13 @@ class ModelRunner:
     def _attention_core(self, lw: LayerWeights, kv_slot: int, qkv, p: Packet, rows: int):
         """q/k head norm + RoPE + INT8 KV write, then attention into ``ws.attn``."""
         cfg, ws = self.cfg, self.ws
+        weights = None
+        if p.weights is not None:
+            if p.shared is not None or p.attend_pos is not None or kv_slot >= len(p.weights) or (
+                    p.weigh_chunks is not None and p.chunks is None):
+                raise ValueError("weights of attention layers, for rows that see their own keys as far "
+                                 "as themselves; weigh_chunks of chunks")
+            weights = p.weights[kv_slot]
         F.qk_rope_kv(qkv, lw.q_norm if cfg.qk_norm else None, lw.k_norm if cfg.qk_norm else None,
                      ws.cos, ws.sin, p.row_req, p.row_pos, p.page_table, self.kv.k[kv_slot],
                      self.kv.v[kv_slot], self.kv.ks[kv_slot], self.kv.vs[kv_slot],
@@ -240,9 +259,20 @@ class ModelRunner:
                                        total_rows=rows, max_kv_len=p.max_chunk_kv or p.max_kv_len)
             if done:
                 row_rows = p.decode_rows
+                if weights is not None:
+                    F.prefill_weights(ws.q, p.chunks if p.weigh_chunks is None else p.weigh_chunks,
+                                      p.max_q_len, p.page_table, self.kv.k[kv_slot],
+                                      self.kv.ks[kv_slot], weights, total_rows=rows,
+                                      max_kv_len=p.max_chunk_kv or p.max_kv_len)
         if row_rows > 0:
             splits = min(F.attention_splits(p.max_kv_len, row_rows, cfg.kv_heads),
                          max(ws.SPLIT_ROWS // row_rows, 1))
+            if weights is not None:
+                F.attention_weighed(ws.q, gate, p.row_req, p.row_pos, p.page_table,
+                                    self.kv.k[kv_slot], self.kv.v[kv_slot], self.kv.ks[kv_slot],
+                                    self.kv.vs[kv_slot], weights, splits=splits, out=ws.attn,
+                                    rows=row_rows, max_kv_len=p.max_kv_len)
+                return
             scratch = ws.attn_scratch if splits > 1 else None
             see = p.row_pos if p.attend_pos is None else p.attend_pos
             F.attention(ws.q, gate, p.row_req, see, p.page_table, self.kv.k[kv_slot],
@@ -491,15 +521,16 @@ class ModelRunner:
         """Fill the rotary tables of the packet: the table kernel for ordinary positions,
         PyTorch for (t, h, w) positions and for partially rotated heads."""
         cfg, ws = self.cfg, self.ws
+        pos = p.row_pos if p.rope_pos is None else p.rope_pos
         if p.mrope is None and not cfg.rotary_dim:
-            F.rope_table(p.row_pos, cfg.head_dim, cfg.rope_theta, ws.cos, ws.sin, rows=rows)
+            F.rope_table(pos, cfg.head_dim, cfg.rope_theta, ws.cos, ws.sin, rows=rows)
             return
         if p.mrope is not None:
             from .vision import mrope_tables
             cos, sin = mrope_tables(p.mrope[:, :rows], cfg.head_dim, cfg.rope_theta)
         else:
             from ..ref.ops_ref import rope_tables
-            cos, sin = rope_tables(p.row_pos[:rows], cfg.head_dim, cfg.rope_theta, cfg.rotary_dim)
+            cos, sin = rope_tables(pos[:rows], cfg.head_dim, cfg.rope_theta, cfg.rotary_dim)
         ws.cos[:rows].copy_(cos)
         ws.sin[:rows].copy_(sin)
 

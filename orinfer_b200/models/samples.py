@@ -18,47 +18,18 @@ from ..config import PAGE_TOKENS
 from ..core import sampling as S
 from ..ops import functional as F
 from .runner import ModelRunner, Packet
+from .slots import SlotPages
 
 
-class PromptSamples:
+class PromptSamples(SlotPages):
     """Prompts and their samples in the cache of ``runner``, which nothing else uses meanwhile.
     ``slots`` bounds the prompts held and the samples decoded at once, ``max_tokens`` the length of
     each."""
 
     def __init__(self, runner: ModelRunner, slots: int, max_tokens: int):
-        self.runner, self.device, self.slots = runner, runner.device, slots
-        self.max_tokens = max_tokens
+        super().__init__(runner, slots, max_tokens)
         self.cache = runner.kv.cache_pages()
-        width = -(-max_tokens // PAGE_TOKENS)
-        zeros = lambda *s: torch.zeros(*s, dtype=torch.int32, device=self.device)
-        self.table, self.lens, self.refs = zeros(slots, width), zeros(slots), zeros(runner.kv.pages)
-        self._free = list(range(slots - 1, -1, -1))
         self._prompts: Dict[int, tuple] = {}            # slot -> (tokens, last logits, recurrent state)
-
-    # ---------------------------------------------------------------- pages
-    def _i32(self, v):
-        return torch.tensor(v, dtype=torch.int32, device=self.device)
-
-    def _take(self, slots: Sequence[int], columns: Sequence[int]) -> None:
-        """Gives each slot a free page at a column of its row, the lowest pages first."""
-        held = self.refs.cpu()
-        pages = [p for p in range(1, len(held)) if held[p] == 0][:len(slots)]
-        if len(pages) < len(slots):
-            raise MemoryError(f"{len(slots)} pages wanted, {len(pages)} free")
-        at = torch.tensor(pages, device=self.device)
-        self.refs[at] = 1
-        self.table[torch.tensor(slots, device=self.device),
-                   torch.tensor(columns, device=self.device)] = at.int()
-
-    def _release(self, slots: Sequence[int]) -> None:
-        F.free_pages(self.table, self.lens, self.refs, self._i32(list(slots)),
-                     out=(self.table, self.lens, self.refs))
-        self._free += list(slots)
-
-    @property
-    def held(self) -> int:
-        """Pages that a prompt or a sample holds."""
-        return int((self.refs > 0).sum())
 
     def compact(self) -> int:
         """Moves the pages that are held to the front; returns how many there are."""

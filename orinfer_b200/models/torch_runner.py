@@ -45,8 +45,14 @@ class TorchRunner:
         q, s = R.a8(z)
         return R.qgemm(q, s, self._w(lin), lin.scale, out_f32)
 
+    @staticmethod
+    def _angles(p: Packet) -> torch.Tensor:
+        return (p.row_pos if p.rope_pos is None else p.rope_pos)[:p.rows]
+
     def _attention(self, lw: LayerWeights, slot: int, y: torch.Tensor, p: Packet, cos, sin):
         cfg = self.cfg
+        if p.weights is not None:
+            raise ValueError("the plain runner does not count attention weights")
         rows, d, qh, kvh = p.rows, cfg.head_dim, cfg.q_heads, cfg.kv_heads
         proj = self._linear(lw.qkv, y)
         gated = cfg.gated_attention and lw.qkv.n == cfg.q_dim + 2 * cfg.kv_dim
@@ -170,7 +176,7 @@ class TorchRunner:
             x = x.index_copy(0, p.overlay_rows, p.overlay.to(x.dtype))
         resid = torch.zeros(rows, cfg.hidden)
         if p.mrope is None:
-            cos, sin = R.rope_tables(p.row_pos[:rows], cfg.head_dim, cfg.rope_theta, cfg.rotary_dim)
+            cos, sin = R.rope_tables(self._angles(p), cfg.head_dim, cfg.rope_theta, cfg.rotary_dim)
         else:
             from .vision import mrope_tables
             cos, sin = mrope_tables(p.mrope[:, :rows], cfg.head_dim, cfg.rope_theta)
@@ -232,7 +238,7 @@ class TorchRunner:
         ye = R.rms_norm(e, m.norm_e, cfg.eps, zc)
         yh = R.rms_norm(hidden[:rows].float(), m.norm_h, cfg.eps, zc)
         x = self._linear(m.fc, torch.cat([ye, yh], dim=1))
-        cos, sin = R.rope_tables(p.row_pos[:rows], cfg.head_dim, cfg.rope_theta, cfg.rotary_dim)
+        cos, sin = R.rope_tables(self._angles(p), cfg.head_dim, cfg.rope_theta, cfg.rotary_dim)
         resid = x
         y = R.rms_norm(resid, m.layer.in_norm, cfg.eps, zc)
         mix = self._attention(m.layer, self.mtp_kv_index, y, p, cos, sin)

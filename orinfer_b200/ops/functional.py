@@ -364,7 +364,7 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
         page_table.shape[1], ptr(kcache), ptr(kscale), pages, ptr(weights), weights.stride(0),
         weights.stride(1), ptr(sums), sums.stride(0), sums.stride(1), limit, qh, kvh, d, ptr(work),
         stream()), "prefill_weights")
-    count_launches(3)
+    count_launches(4)
 
 
 class SharedPrefix:

@@ -125,3 +125,64 @@ def test_weights_of_a_row_add_up_to_its_heads():
     got, _ = R.key_weights(q, torch.tensor([0, 1, 0]), torch.tensor([200, 5, -1]), table, k, s)
     assert torch.allclose(got.sum(2), torch.full((2, 2), 3.0, dtype=torch.float64))
     assert bool((got[0, :, 201:] == 0).all()) and bool((got[1, :, 6:] == 0).all())
+
+
+def prefill(index=0, longest=3, **changed):
+    ints = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    given = dict(q=torch.zeros(3, 4, 64, dtype=torch.float16), chunks=ints(1, 4), table=ints(2, 3),
+                 k=torch.zeros(5, 128, 2, 64, dtype=torch.int8),
+                 ks=torch.zeros(5, 128, 2, 1, dtype=torch.float16), weights=torch.zeros(2, 2, 384))
+    given.update({k: changed.pop(k) for k in list(changed) if k in given})
+    given = {k: v if isinstance(v, On) else On.gpu(index, v) for k, v in given.items()}
+    q, chunks, table, k, ks, weights = given.values()
+    return F.prefill_weights(q, chunks, longest, table, k, ks, weights, **changed)
+
+
+@pytest.mark.parametrize("changed", [
+    dict(q=torch.zeros(3, 4, 64)), dict(q=torch.zeros(3, 4, 128, dtype=torch.float16)),
+    dict(q=torch.zeros(3, 5, 64, dtype=torch.float16)),
+    dict(q=torch.zeros(3, 34, 64, dtype=torch.float16)),         # 17 query heads to a KV head
+    dict(q=torch.zeros(3 * 256 + 1, dtype=torch.float16)[1:].view(3, 4, 64)),
+    dict(chunks=torch.zeros(1, 4)), dict(chunks=torch.zeros(1, 3, dtype=torch.int32)),
+    dict(chunks=torch.zeros(4, 2, dtype=torch.int32).t()),
+    dict(chunks=torch.zeros(513, 4, dtype=torch.int32)),
+    dict(chunks=On.gpu(1, torch.zeros(1, 4, dtype=torch.int32))),
+    dict(table=torch.zeros(3, 3, dtype=torch.int32)), dict(k=torch.zeros(4, 128, 2, 64, dtype=torch.int8)),
+    dict(k=torch.zeros(5 * 128 * 128 + 1, dtype=torch.int8)[1:].view(5, 128, 2, 64)),
+    dict(ks=torch.zeros(5, 128, 2, 2, dtype=torch.float16)), dict(weights=torch.zeros(2, 1, 384)),
+    dict(weights=torch.zeros(2, 2, 384).double()), dict(weights=On.gpu(1, torch.zeros(2, 2, 384))),
+    dict(weights_out=On.gpu(0, torch.zeros(2, 2, 383))), dict(total_rows=4), dict(total_rows=-1),
+    dict(longest=-1),
+])
+def test_prefill_weights_refuses(nothing_runs, changed):  # noqa: F811
+    with pytest.raises(native.KernelError):
+        prefill(**changed)
+
+
+@pytest.mark.parametrize("changed", [dict(longest=0), dict(total_rows=0), dict(max_kv_len=0),
+                                     dict(chunks=torch.zeros(0, 4, dtype=torch.int32))])
+def test_prefill_weights_of_nothing_launches_nothing(nothing_runs, changed):  # noqa: F811
+    assert prefill(**changed) is None
+
+
+def test_prefill_weights_on_another_device_than_the_current_one(nothing_runs):  # noqa: F811
+    with pytest.raises(native.KernelError, match="current"):
+        prefill(index=1)
+
+
+def test_the_plain_runner_turns_keys_where_it_is_told_and_counts_nothing():
+    from orinfer_b200.config import PRESETS
+    from orinfer_b200.models.runner import KVPool, Packet
+    from orinfer_b200.models.torch_runner import TorchRunner
+    from orinfer_b200.models.weights import random_model
+    cfg = PRESETS["tiny"]
+    runner = TorchRunner(random_model(cfg, seed=1), KVPool.allocate(cfg, 3, "cpu"), max_rows=8)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)
+    ids, table, keys = i32([5, 9, 11]), i32([[1], [2]]), []
+    for slot, pos, rope in ((0, [7, 8, 9], None), (1, [2, 3, 4], i32([7, 8, 9]))):
+        runner.logits(Packet(ids, i32([slot] * 3), i32(pos), table, 3, 10, rope_pos=rope))
+        keys.append(runner.kv.k[0][slot + 1, pos])
+    assert torch.equal(*keys)
+    with pytest.raises(ValueError):
+        runner.logits(Packet(ids, i32([0] * 3), i32([0, 1, 2]), table, 3, 3,
+                             weights=torch.zeros(cfg.layers, 2, cfg.kv_heads, 128)))
