@@ -1200,7 +1200,7 @@ template <int D, int REP>
 __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_kernel(
     const Weighed weighed, const int* row_req, const int* row_pos, const float* weights,
     long long slot_stride, long long head_stride, float* sums, long long sums_slot_stride,
-    long long sums_head_stride, int capacity, int rows, int qh, int splits, int heads,
+    long long sums_head_stride, int capacity, int rows, int qh, int splits, int heads, int merges,
     const float* scratch, const __half* gate, __half* __restrict__ out, int* status) {
   __shared__ int2 s_rows[WEIGH_THREADS];           // rows of the request, in their order, and their keys
   __shared__ int s_count[WEIGH_THREADS / 32];
@@ -1208,25 +1208,28 @@ __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_ker
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_wait();
   grid_release();
-  const int row = blockIdx.x, z = static_cast<int>(blockIdx.z) - (splits > 1);
+  const int row = blockIdx.x, z = static_cast<int>(blockIdx.z) - merges;
   const int h_lo = blockIdx.y * heads, h_hi = min(h_lo + heads, qh / REP);
   const int key = z * WEIGH_KEYS + 4 * tid;
   if (z < 0) {
-    for (int i = h_lo * REP + tid / D; i < h_hi * REP; i += WEIGH_THREADS / D)
-      attn_merge<D, false>(scratch, gate, out, row, i, qh, splits, tid % D, D, SharedParts());
+    const int head = h_lo * REP + static_cast<int>(blockIdx.z) * (WEIGH_THREADS / D) + tid / D;
+    if (head < h_hi * REP)
+      attn_merge<D, false>(scratch, gate, out, row, head, qh, splits, tid % D, D, SharedParts());
     return;
   }
-  auto factor = [&](int r, int head) {             // by a warp
-    const float2* ml = weighed.ml + (static_cast<size_t>(r) * qh + head) * splits;
-    const float2 own = lane < splits ? ml[lane] : make_float2(-INFINITY, 0.f);
+  auto part = [&](int r, int head) {               // a split's maximum and sum, a lane each
+    return lane < splits ? weighed.ml[(static_cast<size_t>(r) * qh + head) * splits + lane]
+                         : make_float2(-INFINITY, 0.f);
+  };
+  auto joined = [&](float2 own) {                  // by a warp
     const float m = warp_max(own.x);
     const float l = warp_sum(own.x == -INFINITY ? 0.f : own.y * exp2f(own.x - m));
     return make_float2(m, l > 0.f ? 1.f / l : l == 0.f ? 0.f : l);
   };
   const int pos = row_pos[row], req = row_req[row], limit = min(weighed.keys, capacity);
   int other_pos = tid < rows ? row_pos[tid] : -1, other_req = tid < rows ? row_req[tid] : 0;
-  float2 own_f = make_float2(0.f, 0.f);
-  if (warp < REP) own_f = factor(row, h_lo * REP + warp);
+  float2 own_part = make_float2(-INFINITY, 0.f);
+  if (warp < REP) own_part = part(row, h_lo * REP + warp);
   if (pos < 0) return;
   if (tid == 0 && z == 0 && blockIdx.y == 0 && pos >= limit)
     report_status(status, STATUS_BAD_INDEX, 0x60);
@@ -1272,10 +1275,21 @@ __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_ker
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         so_far[k] = key + k < one.y ? (key + k < done ? to : from)[key + k] : 0.f;
-      for (int x = warp; x < count * REP; x += WEIGH_THREADS / 32) {
-        const int r = x / REP, i = x % REP;
-        const float2 f = first && r == 0 ? own_f : factor(s_rows[r].x, h * REP + i);
-        if (lane == 0) s_f[r][i] = f;
+      for (int x0 = warp; x0 < count * REP; x0 += 4 * (WEIGH_THREADS / 32)) {
+        float2 f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int x = x0 + k * (WEIGH_THREADS / 32), r = x / REP;
+          if (x < count * REP)
+            f[k] = first && x < REP ? own_part : part(s_rows[r].x, h * REP + x % REP);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int x = x0 + k * (WEIGH_THREADS / 32);
+          if (x >= count * REP) break;
+          f[k] = joined(f[k]);
+          if (lane == 0) s_f[x / REP][x % REP] = f[k];
+        }
       }
       __syncthreads();
       for (int r = 0; r < count; ++r) {
@@ -1503,16 +1517,23 @@ extern "C" int orinfer_attention_weighed(
   CASE(64) CASE(128) CASE(256)
 #undef CASE
   if (e != 0) return e;
-  const int columns = (w.keys + WEIGH_KEYS - 1) / WEIGH_KEYS + (splits > 1 ? 1 : 0);
-  const long long ctas = static_cast<long long>(rows) * kvh * columns;
-  const int per = static_cast<int>(ctas <= EARLY_CTAS ? 1 : (ctas + EARLY_CTAS - 1) / EARLY_CTAS);
-  const int per_cta = per < kvh ? per : kvh;
-  const dim3 grid(rows, (kvh + per_cta - 1) / per_cta, columns);
+  const int chunks = (w.keys + WEIGH_KEYS - 1) / WEIGH_KEYS;
+  int per_cta, merges, groups;
+  auto ctas = [&](int heads) {
+    per_cta = heads;
+    groups = (kvh + heads - 1) / heads;
+    merges = splits > 1 ? (heads * rep * head_dim + WEIGH_THREADS - 1) / WEIGH_THREADS : 0;
+    return static_cast<long long>(rows) * groups * (chunks + merges);
+  };
+  int most = 1;
+  while (most < kvh && ctas(most) > EARLY_CTAS) ++most;
+  if (ctas(most) > EARLY_CTAS) ctas(1);
+  const dim3 grid(rows, groups, chunks + merges);
 #define CASE(DD, REP)                                                                               \
   if (head_dim == DD && rep == REP)                                                                 \
     launch_early(attn_weigh_kernel<DD, REP>, grid, WEIGH_THREADS, 0, stream, w, row_req, row_pos,   \
                  weights, slot_stride, head_stride, sums, sums_slot_stride, sums_head_stride,       \
-                 capacity, rows, qh, splits, per_cta, static_cast<const float*>(parts), gate, out,  \
+                 capacity, rows, qh, splits, per_cta, merges, static_cast<const float*>(parts), gate, out,  \
                  runtime_status_ptr());
   CASE(64, 1) CASE(64, 2) CASE(64, 4) CASE(64, 8)
   CASE(128, 1) CASE(128, 2) CASE(128, 4) CASE(128, 5) CASE(128, 8)
