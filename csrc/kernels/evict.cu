@@ -404,7 +404,7 @@ extern "C" int orinfer_evict_keys(const long long* bases, int layers, int kvh, i
   if ((reinterpret_cast<uintptr_t>(work) & 7) != 0) return -1;
   const int kept = (keep + ev::PAGE - 1) / ev::PAGE;
   const long long items = static_cast<long long>(n) * layers * kvh;
-  if (items * kept > (1 << 29) || static_cast<long long>(slots) * max_pages > (1 << 30) ||
+  if (items * kept > (1 << 29) || static_cast<long long>(slots) * (max_pages + 1LL) > (1 << 30) ||
       static_cast<long long>(pages) * ev::PAGE > 0x7fffffffLL)
     return -1;
   const ev::Cache cache{bases, layers, kvh, pages};

@@ -216,30 +216,36 @@ def _current(where):
 
 def _weight_sums(weights, weights_out, lead, kvh, where):
     """(capacity, strides of weights, the sums that are written and their strides)."""
+    shape = weights.shape
     out = weights if weights_out is None else weights_out
-    for t in (weights, out):
-        if (t.dtype != torch.float32 or t.dim() != 3 or t.shape[1] != kvh or t.device != where
-                or t.stride(2) != 1 or t.shape != weights.shape):
-            raise native.KernelError("weights: fp32 [slots, KV heads, keys] on the cache's GPU, keys in "
-                                     "one piece, weights_out like them")
-    _need(weights.shape[0] >= lead, "weights: a slot for each row of the page table")
-    return weights.shape[2], out
+    if (weights.dtype != torch.float32 or len(shape) != 3 or shape[1] != kvh or weights.stride(2) != 1
+            or weights.device != where
+            or (out is not weights and (out.dtype != torch.float32 or out.shape != shape
+                                        or out.stride(2) != 1 or out.device != where))):
+        raise native.KernelError("weights: fp32 [slots, KV heads, keys] on the cache's GPU, keys in one "
+                                 "piece, weights_out like them")
+    if shape[0] < lead:
+        raise native.KernelError("weights: a slot for each row of the page table")
+    return shape[2], out
 
 
-def _cached(where, page_table, *tensors):
-    """Checks a cache's tensors [pages, 128, KV heads, channels or groups]; returns (pages, KV heads,
-    channels)."""
-    codes = [t for t in tensors if t.dtype == torch.int8]
-    scales = [t for t in tensors if t.dtype == torch.float16]
-    pages, tokens, kvh, d = codes[0].shape if codes and codes[0].dim() == 4 else (0, 0, 0, 0)
-    _need(tokens == 128 and d in (64, 128, 256) and len(codes) == len(scales) == len(tensors) // 2
-          and all(t.shape == (pages, 128, kvh, d) for t in codes)
-          and all(t.shape == (pages, 128, kvh, d // 64) for t in scales),
-          "a cache: int8 [pages, 128, KV heads, 64, 128 or 256] and fp16 scales, one per 64 channels")
-    for t in (page_table, *tensors):
+def _cached(where, page_table, codes, scales, *more):
+    """Checks a cache's tensors [pages, 128, KV heads, channels or groups] (codes and scales of the keys,
+    of the values); returns (pages, KV heads, channels)."""
+    shape = codes.shape
+    pages, tokens, kvh, d = shape if len(shape) == 4 else (0, 0, 0, 0)
+    groups = (pages, 128, kvh, d // 64)
+    if (tokens != 128 or d not in (64, 128, 256) or codes.dtype != torch.int8
+            or scales.dtype != torch.float16 or scales.shape != groups
+            or (more and (more[0].dtype != torch.int8 or more[0].shape != shape
+                          or more[1].dtype != torch.float16 or more[1].shape != groups))):
+        raise native.KernelError("a cache: int8 [pages, 128, KV heads, 64, 128 or 256] and fp16 scales, "
+                                 "one per 64 channels")
+    for t in (page_table, codes, scales, *more):
         if not t.is_contiguous() or t.device != where:
             raise native.KernelError("page table and cache: contiguous, on the queries' GPU")
-    _need(page_table.dtype == torch.int32 and page_table.dim() == 2, "page_table: int32 [slots, pages]")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2:
+        raise native.KernelError("page_table: int32 [slots, pages]")
     return pages, kvh, d
 
 
@@ -259,36 +265,41 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     what ``weights`` holds, get none and set the status word."""
     _cuda(q, gate, row_req, row_pos, weights)
     where = q.device
-    _need(q.dim() == 3 and q.dtype == torch.float16 and q.is_contiguous(), "q: fp16 [rows, heads, D]")
+    if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
+        raise native.KernelError("q: fp16 [rows, heads, D]")
     n, qh, d = q.shape
-    _, kvh, dim = _cached(where, page_table, kcache, vcache, kscale, vscale)
-    _need(d == dim and qh % kvh == 0, f"{qh} query heads of {d} on {kvh} KV heads of {dim} channels")
-    if gate is not None:
-        _need(gate.dtype == torch.float16 and gate.numel() == q.numel() and gate.is_contiguous()
-              and gate.device == where, "gate: fp16, as many as q has")
+    _, kvh, dim = _cached(where, page_table, kcache, kscale, vcache, vscale)
+    if d != dim or qh % kvh != 0:
+        raise native.KernelError(f"{qh} query heads of {d} on {kvh} KV heads of {dim} channels")
+    if gate is not None and (gate.dtype != torch.float16 or gate.numel() != q.numel()
+                             or not gate.is_contiguous() or gate.device != where):
+        raise native.KernelError("gate: fp16, as many as q has")
     live = n if rows is None else rows
-    _need(0 <= live <= n, f"{live} rows of {n}")
+    if not 0 <= live <= n:
+        raise native.KernelError(f"{live} rows of {n}")
     for t in (row_req, row_pos):
-        _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] >= live and t.is_contiguous()
-              and t.device == where, "row_req, row_pos: int32, one for each row, on the queries' GPU")
-    capacity, sums = _weight_sums(weights, weights_out, page_table.shape[0], kvh, where)
+        if (t.dtype != torch.int32 or t.dim() != 1 or t.numel() < live or not t.is_contiguous()
+                or t.device != where):
+            raise native.KernelError("row_req, row_pos: int32, one for each row, on the queries' GPU")
+    lead, width = page_table.shape
+    capacity, sums = _weight_sums(weights, weights_out, lead, kvh, where)
     _current(where)
-    width = page_table.shape[1] * 128
-    keys = width if max_kv_len is None else max(1, min(int(max_kv_len), width))
-    _need(1 <= splits <= 32 and keys > 0, "1 to 32 splits of some keys")
+    keys = width * 128 if max_kv_len is None else max(1, min(int(max_kv_len), width * 128))
+    if not 1 <= splits <= 32 or keys == 0:
+        raise native.KernelError("1 to 32 splits of some keys")
     if out is None:
         out = torch.empty(n, qh * d, dtype=torch.float16, device=where)
-    else:
-        _need(out.dtype == torch.float16 and out.is_contiguous() and out.numel() >= live * qh * d
-              and out.device == where, "out: fp16 [rows, heads * D]")
+    elif (out.dtype != torch.float16 or not out.is_contiguous() or out.numel() < live * qh * d
+          or out.device != where):
+        raise native.KernelError("out: fp16 [rows, heads * D]")
     need = native.lib().orinfer_attention_weighed_scratch_bytes(live, qh, d, splits, keys)
     if scratch is None:
         scratch = torch.empty(need // 4, dtype=torch.float32, device=where)
-    else:
-        _need(scratch.numel() * scratch.element_size() >= need and scratch.is_contiguous()
-              and scratch.device == where, f"scratch: {need} bytes")
+    elif (scratch.numel() * scratch.element_size() < need or not scratch.is_contiguous()
+          or scratch.device != where):
+        raise native.KernelError(f"scratch: {need} bytes")
     check(native.lib().orinfer_attention_weighed(
-        ptr(q), ptr(gate), ptr(row_req), ptr(row_pos), ptr(page_table), page_table.shape[1],
+        ptr(q), ptr(gate), ptr(row_req), ptr(row_pos), ptr(page_table), width,
         ptr(kcache), ptr(vcache), ptr(kscale), ptr(vscale), ptr(out), ptr(weights),
         weights.stride(0), weights.stride(1), ptr(sums), sums.stride(0), sums.stride(1), capacity,
         live, qh, kvh, d, splits, keys, ptr(scratch), max_kv_len or 0, stream()), "attention_weighed")
@@ -338,20 +349,26 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     ``max_q_len`` rows or of rows that are not there is left out and sets the status word."""
     _cuda(q, chunks, weights)
     where = q.device
-    _need(q.dim() == 3 and q.dtype == torch.float16 and q.is_contiguous(), "q: fp16 [rows, heads, D]")
+    if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
+        raise native.KernelError("q: fp16 [rows, heads, D]")
     n, qh, d = q.shape
     pages, kvh, dim = _cached(where, page_table, kcache, kscale)
-    _need(d == dim and qh % kvh == 0 and qh // kvh <= 16,
-          f"{qh} query heads of {d} on {kvh} KV heads of {dim} channels")
-    _need(q.data_ptr() % 16 == kcache.data_ptr() % 16 == 0, "q and kcache on 16-byte boundaries")
-    _need(chunks.dtype == torch.int32 and chunks.dim() == 2 and chunks.shape[1] == 4
-          and chunks.is_contiguous() and chunks.device == where, "chunks: int32 [C, 4], on the queries' GPU")
-    _need(chunks.shape[0] <= 512, "at most 512 chunks")
+    if d != dim or qh % kvh != 0 or qh // kvh > 16:
+        raise native.KernelError(f"{qh} query heads of {d} on {kvh} KV heads of {dim} channels")
+    if q.data_ptr() % 16 or kcache.data_ptr() % 16:
+        raise native.KernelError("q and kcache on 16-byte boundaries")
+    if (chunks.dtype != torch.int32 or chunks.dim() != 2 or chunks.shape[1] != 4
+            or not chunks.is_contiguous() or chunks.device != where):
+        raise native.KernelError("chunks: int32 [C, 4], on the queries' GPU")
+    if chunks.shape[0] > 512:
+        raise native.KernelError("at most 512 chunks")
     live = n if total_rows is None else total_rows
-    _need(0 <= live <= n and max_q_len >= 0, f"{live} rows of {n}, chunks of {max_q_len}")
-    capacity, sums = _weight_sums(weights, weights_out, page_table.shape[0], kvh, where)
+    if not 0 <= live <= n or max_q_len < 0:
+        raise native.KernelError(f"{live} rows of {n}, chunks of {max_q_len}")
+    lead, width = page_table.shape
+    capacity, sums = _weight_sums(weights, weights_out, lead, kvh, where)
     _current(where)
-    limit = min(page_table.shape[1] * 128, capacity)
+    limit = min(width * 128, capacity)
     if max_kv_len is not None:
         limit = min(limit, max_kv_len)
     max_q_len = min(max_q_len, live)
@@ -360,8 +377,8 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     work = torch.empty(native.lib().orinfer_prefill_weights_work_bytes(
         chunks.shape[0], max_q_len, kvh, qh // kvh, limit) // 4, dtype=torch.float32, device=where)
     check(native.lib().orinfer_prefill_weights(
-        ptr(q), ptr(chunks), chunks.shape[0], max_q_len, live, ptr(page_table), page_table.shape[0],
-        page_table.shape[1], ptr(kcache), ptr(kscale), pages, ptr(weights), weights.stride(0),
+        ptr(q), ptr(chunks), chunks.shape[0], max_q_len, live, ptr(page_table), lead, width,
+        ptr(kcache), ptr(kscale), pages, ptr(weights), weights.stride(0),
         weights.stride(1), ptr(sums), sums.stride(0), sums.stride(1), limit, qh, kvh, d, ptr(work),
         stream()), "prefill_weights")
     count_launches(4)
@@ -703,8 +720,8 @@ class KeyCache:
         self.device, self.layers = k[0].device, len(k)
         any_table = torch.empty(0, 0, dtype=torch.int32, device=self.device)
         for layer in zip(k, v, ks, vs):
-            got = _cached(self.device, any_table, *layer)
-            _need(layer[0].dtype == layer[1].dtype == torch.int8 and got == (*k[0].shape[:1], *k[0].shape[2:])
+            got = _cached(self.device, any_table, layer[0], layer[2], layer[1], layer[3])
+            _need(got == (*k[0].shape[:1], *k[0].shape[2:])
                   and layer[0].data_ptr() % 16 == layer[1].data_ptr() % 16 == 0
                   and all(t.data_ptr() % (got[2] // 32) == 0 for t in layer[2:]),
                   "layers alike, keys and values on 16-byte boundaries, scales on those of a key's")
@@ -734,15 +751,16 @@ def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: t
     total, width = table.shape
     if lens.dim() != 1 or lens.numel() != total or refs.dim() != 1 or refs.numel() != cache.pages:
         raise native.KernelError("lens: [slots], refs: [pages]")
-    sums = weights if weights_out is None else weights_out
-    for w in (weights, sums):
-        if (w.dtype != torch.float32 or w.shape[:3] != (cache.layers, total, cache.kvh) or w.dim() != 4
-                or not w.is_contiguous() or w.device != cache.device or w.shape != weights.shape):
-            raise native.KernelError("weights: contiguous fp32 [layers, slots, KV heads, keys] on the "
-                                     "cache's GPU, weights_out like them")
-    _need(weights.shape[3] >= width * 128, "weights: a place for each key of a table row")
-    _need(1 <= keep <= width * 128 and first >= 0 and recent >= 0 and first + recent <= keep,
-          f"{keep} keys of {width * 128} with {first} first and {recent} last ones")
+    sums, shape = weights if weights_out is None else weights_out, weights.shape
+    for w in (weights,) if sums is weights else (weights, sums):
+        if (w.dtype != torch.float32 or w.shape != shape or not w.is_contiguous()
+                or w.device != cache.device):
+            raise native.KernelError("weights: contiguous fp32 on the cache's GPU, weights_out like them")
+    if len(shape) != 4 or shape[:3] != (cache.layers, total, cache.kvh) or shape[3] < width * 128:
+        raise native.KernelError("weights: [layers, slots, KV heads, keys], a place for each key of a "
+                                 "table row")
+    if not 1 <= keep <= width * 128 or first < 0 or recent < 0 or first + recent > keep:
+        raise native.KernelError(f"{keep} keys of {width * 128} with {first} first and {recent} last ones")
     _current(cache.device)
     status = torch.empty(1, dtype=torch.int32, device=cache.device)
     work = torch.empty(native.lib().orinfer_evict_work_words(
