@@ -1000,16 +1000,18 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-// A CTA per key tile, KV head and chunk: chunks of one request are added in their order by the first's.
+// A CTA per key tile, ADD_HEADS KV heads and chunk: chunks of one request are added in their order by the
+// first's.  A chain of small loads (chunk, span, parts, sums); a thread asks for its heads' together.
+constexpr int ADD_HEADS = 4;
 __global__ void __launch_bounds__(TILE) add_kernel(
     const Geometry g, const float* parts, const int* span, const float* weights, long long slot_stride,
     long long head_stride, float* sums, long long sums_slot_stride, long long sums_head_stride) {
   grid_wait();
   grid_release();
-  const int c = blockIdx.z, h = blockIdx.y, tile = blockIdx.x, tid = threadIdx.x;
+  const int c = blockIdx.z, h0 = blockIdx.y * ADD_HEADS, tile = blockIdx.x, tid = threadIdx.x;
   const Chunk ch = g.at(c);
   if (ch.q_len <= 0) return;
-  float total = 0.f;
+  float total[ADD_HEADS] = {};
   int base = 0, seen = 0;                          // key tiles of the chunks before; keys that are seen
   for (int d = 0; d < g.n_chunks; ++d) {
     const Chunk other = g.at(d);
@@ -1017,22 +1019,45 @@ __global__ void __launch_bounds__(TILE) add_kernel(
     if (other.q_len > 0 && other.slot == ch.slot) {
       if (d < c) return;
       if (tile < tiles) {
-        const int index = base + h * tiles + tile;
-        const int2 of = span_of(span, index);
-        float sum = 0.f;
-        for (int x = of.x; x <= of.y; ++x)
+        int2 of[ADD_HEADS];
+        float v[ADD_HEADS][PARTS];
+        auto place = [&](int k, int x, int part) {
+          return (static_cast<size_t>(base + (h0 + k) * tiles + tile + x) * PARTS + part) * TILE + tid;
+        };
+#pragma unroll
+        for (int k = 0; k < ADD_HEADS; ++k)
+          if (h0 + k < g.kvh) of[k] = span_of(span, base + (h0 + k) * tiles + tile);
+#pragma unroll
+        for (int k = 0; k < ADD_HEADS; ++k)
+#pragma unroll
           for (int part = 0; part < PARTS; ++part)
-            sum += parts[(static_cast<size_t>(index + x) * PARTS + part) * TILE + tid];
-        total += sum;
+            if (h0 + k < g.kvh && of[k].x <= of[k].y) v[k][part] = parts[place(k, of[k].x, part)];
+#pragma unroll
+        for (int k = 0; k < ADD_HEADS; ++k) {
+          if (h0 + k >= g.kvh || of[k].x > of[k].y) continue;
+          float sum = 0.f;
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) sum += v[k][part];
+          for (int x = of[k].x + 1; x <= of[k].y; ++x)
+            for (int part = 0; part < PARTS; ++part) sum += parts[place(k, x, part)];
+          total[k] += sum;
+        }
         seen = max(seen, other.pos0 + other.q_len);
       }
     }
     base += tiles * g.kvh;
   }
   const int key = tile * TILE + tid;
-  if (key < seen)
-    sums[ch.slot * sums_slot_stride + h * sums_head_stride + key] =
-        weights[ch.slot * slot_stride + h * head_stride + key] + total;
+  if (key >= seen) return;
+  const float* from = weights + ch.slot * slot_stride + h0 * head_stride + key;
+  float* to = sums + ch.slot * sums_slot_stride + h0 * sums_head_stride + key;
+  float before[ADD_HEADS];
+#pragma unroll
+  for (int k = 0; k < ADD_HEADS; ++k)
+    if (h0 + k < g.kvh) before[k] = from[k * head_stride];
+#pragma unroll
+  for (int k = 0; k < ADD_HEADS; ++k)
+    if (h0 + k < g.kvh) to[k * sums_head_stride] = before[k] + total[k];
 }
 
 // Tiles that a call may have at most, of rows and of keys, and its units.
@@ -1091,7 +1116,8 @@ static int launch(const __half* q, const Geometry& g, const int8_t* kc, const __
                g, static_cast<const float*>(lse), static_cast<const int*>(row_span), rows);
   launch_early(sums_kernel<D>, dim3(ctas), THREADS, L::B_TOTAL, stream, tq, tk, g, ks,
                static_cast<const float*>(rows), parts, key_span, runtime_status_ptr());
-  launch_early(add_kernel, dim3((g.limit + TILE - 1) / TILE, g.kvh, g.n_chunks), TILE, 0, stream, g,
+  launch_early(add_kernel, dim3((g.limit + TILE - 1) / TILE, (g.kvh + ADD_HEADS - 1) / ADD_HEADS, g.n_chunks),
+               TILE, 0, stream, g,
                static_cast<const float*>(parts), static_cast<const int*>(key_span), weights, slot_stride,
                head_stride, sums, sums_slot_stride, sums_head_stride);
   return static_cast<int>(cudaGetLastError());
