@@ -236,8 +236,9 @@ int orinfer_attention_shared(const __half* q, const __half* gate, const int* row
                              float* scratch, int context, cudaStream_t stream);
 
 // Eviction from the cache (evict.cu).  bases: device int64 [4][layers], the addresses of the keys, values
-// (16-byte aligned) and their scales (aligned to a key's); weights, sums: FP32 [layers][slots][KV heads][capacity]; work: as
-// many words as the first says, on an 8-byte boundary.  Outputs may be the inputs.
+// (16-byte aligned) and their scales (aligned to a key's); weights, sums: FP32 [layers][slots][KV
+// heads][capacity]; work: as many words as the first says, on an 8-byte boundary.  Outputs may be the
+// inputs.
 size_t orinfer_evict_work_words(int layers, int kvh, int slots, int n, int max_pages, int keep);
 int orinfer_evict_keys(const long long* bases, int layers, int kvh, int head_dim, int pages,
                        const int* table, int* table_out, const int* lens, int* lens_out,

@@ -66,6 +66,15 @@ struct RowScales {
   }
 };
 
+// What a call that also weighs the keys (attention_weighed) gets out of the row kernels: every score,
+// times log2 e, and every part's reference and sum of weights.  (Nothing else of a kernel changes, so
+// that its outputs have the bits of `attention`.)
+struct Weighed {
+  float* scores = nullptr;         // [rows][query heads][keys]
+  float2* ml = nullptr;            // [rows][query heads][splits]
+  int keys = 0;                    // a multiple of 4; what a row sees beyond is not written
+};
+
 // One CTA per (row, KV head, key split); its four warps take blocks of KB keys in turn (a block
 // lies inside one page) and carry their own softmax state, merged in shared memory at the end.
 //
@@ -88,15 +97,6 @@ struct RowScales {
 // scale shuffles, a permute and a subtraction per pair of INT8 values, the head and remainder, two
 // maxima per block) with under three warps per scheduler, which wait for fixed latencies and for
 // each other; for loads they wait a third of that (0.3 to 0.6 warps per issue).
-// What a call that also weighs the keys (attention_weighed) gets out of the row kernels: every score,
-// times log2 e, and every part's reference and sum of weights.  (Nothing else of a kernel changes, so
-// that its outputs have the bits of `attention`.)
-struct Weighed {
-  float* scores = nullptr;         // [rows][query heads][keys]
-  float2* ml = nullptr;            // [rows][query heads][splits]
-  int keys = 0;                    // a multiple of 4; what a row sees beyond is not written
-};
-
 template <int D>
 struct AttnTile {
   static constexpr int G = D / 64;                 // scale groups per row
@@ -1191,10 +1191,14 @@ __global__ void attn_merge_kernel(
 // the first column put the outputs together meanwhile.
 //
 // A CTA takes WEIGH_KEYS keys of a row and some KV heads, as many as let the launch start early
-// (EARLY_CTAS).  Scores are written once by the row kernels and read once here, 4 rep bytes a key beside
-// the 2 D and more of its key and value, mostly within L2.  It is a chain of loads that wait for each
-// other, so what can be asked for at once is: the scores and factors of the CTA's own row before it is
-// known whether an earlier row's CTA has them.
+// (EARLY_CTAS), one where no number does.  Scores are written once by the row kernels and read once
+// here, 4 rep bytes a key beside the 2 D and more of its key and value, mostly within L2; making them
+// again would read the keys again.  The kernel is a chain of loads that wait for each other, so what can
+// be asked for at once is: the scores and factors of the CTA's own row before it is known whether an
+// earlier row's CTA has them, a request's factors four at a time.  32 / 8 heads of 128: 128 rows of 640
+// keys 9 us behind the row kernel's 37 (a CTA per head, too many to start early: the call 49.2 us, now
+// 45.4), 6 rows of 24000 keys 12 behind 53 (17 with one CTA for all of a row's outputs), 36 rows of 3000
+// keys, four a request, 16 / 2 heads of 256: 15 behind 35 (21 without asking for factors together).
 constexpr int WEIGH_THREADS = 256, WEIGH_KEYS = 4 * WEIGH_THREADS;
 template <int D, int REP>
 __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_kernel(
@@ -1533,8 +1537,8 @@ extern "C" int orinfer_attention_weighed(
   if (head_dim == DD && rep == REP)                                                                 \
     launch_early(attn_weigh_kernel<DD, REP>, grid, WEIGH_THREADS, 0, stream, w, row_req, row_pos,   \
                  weights, slot_stride, head_stride, sums, sums_slot_stride, sums_head_stride,       \
-                 capacity, rows, qh, splits, per_cta, merges, static_cast<const float*>(parts), gate, out,  \
-                 runtime_status_ptr());
+                 capacity, rows, qh, splits, per_cta, merges, static_cast<const float*>(parts),     \
+                 gate, out, runtime_status_ptr());
   CASE(64, 1) CASE(64, 2) CASE(64, 4) CASE(64, 8)
   CASE(128, 1) CASE(128, 2) CASE(128, 4) CASE(128, 5) CASE(128, 8)
   CASE(256, 1) CASE(256, 2) CASE(256, 4) CASE(256, 8)

@@ -11,6 +11,13 @@
 // its threshold, the weight of the last key that stays, by three histograms of the weights' bits (11, 11,
 // 10), and walks the keys once: those above the threshold, and of those equal to it the first so many, go
 // to a list with their weights.  In the second a CTA fills a fresh page of a layer and head from the list.
+//
+// The second is bound by memory: 2 (D + D / 32) bytes of a kept key's key and value read and as many
+// written, pieces of D bytes in no order of pages.  36 layers of 8 heads of 128: eleven requests of 1450 keys
+// cut to 1000 292 us, 5.6 TB/s (a CTA that walks its keys itself: 390); two of 12000 to 2000 117 (199);
+// seventeen of 2100 to 1100, 12 layers of 2 heads of 256: 62.  The first, 47, 39 and 13 us of these, is a
+// chain of passes over weights that lie in L2, half of it the walk: with weights in shared memory it took
+// 53, 49 and 13, with 512 threads 50 and 70, since fewer CTAs are at work beside each other.
 #include <type_traits>
 
 #include "api.h"
@@ -180,17 +187,26 @@ __global__ void __launch_bounds__(THREADS) select_kernel(
     for (int i = tid; i < BINS; i += THREADS) s_hist[i] = 0;
     __syncthreads();
     constexpr int AHEAD = 8;                       // loads in flight
-    for (int i0 = lo + tid; i0 < hi; i0 += AHEAD * THREADS) {
+    auto count = [&](float x) {
+      const uint32_t u = ordered(x);
+      if (pass == 0 || u >> shift == prefix) atomicAdd(&s_hist[u >> next & (bins - 1)], 1);
+    };
+    int i0 = lo + tid;
+    for (; i0 + (AHEAD - 1) * THREADS < hi; i0 += AHEAD * THREADS) {
+      float x[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) x[k] = from[i0 + k * THREADS];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) count(x[k]);
+    }
+    if (i0 < hi) {
       float x[AHEAD];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k)
         if (i0 + k * THREADS < hi) x[k] = from[i0 + k * THREADS];
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        if (i0 + k * THREADS >= hi) break;
-        const uint32_t u = ordered(x[k]);
-        if (pass == 0 || u >> shift == prefix) atomicAdd(&s_hist[u >> next & (bins - 1)], 1);
-      }
+      for (int k = 0; k < AHEAD; ++k)
+        if (i0 + k * THREADS < hi) count(x[k]);
     }
     __syncthreads();
     // the bin in which the `want`-th from the top lies
@@ -247,12 +263,12 @@ __global__ void __launch_bounds__(THREADS) select_kernel(
 #pragma unroll
     for (int k = 0; k < LANE_KEYS; ++k) {
       const int key = k0 + warp * (32 * LANE_KEYS) + k * 32 + lane;
-      const bool between = key >= lo && key < hi;
+      const bool between = static_cast<unsigned>(key - lo) < static_cast<unsigned>(hi - lo);
       const uint32_t u = shift < 32 ? ordered(x[k]) >> shift : 0u;
       over[k] = __ballot_sync(0xffffffffu, key < len && (!between || (!none && u > prefix)));
       same[k] = __ballot_sync(0xffffffffu, between && !none && u == prefix);
       n_over += __popc(over[k]);
-      n_same += __popc(same[k]);
+      if (same[k]) n_same += __popc(same[k]);      // (few have any)
     }
     __syncthreads();                               // (the counts of the step before are read)
     if (lane == 0) s_warp[warp] = n_over | n_same << 16;
@@ -271,14 +287,20 @@ __global__ void __launch_bounds__(THREADS) select_kernel(
     // (of the equal ones before a key, at most `want` are kept)
     const int base = done - min(equal, want);
     const unsigned lower = (1u << lane) - 1u;
+    int at = base + o_before + min(s_before, want);          // of the next key that stays
 #pragma unroll
     for (int k = 0; k < LANE_KEYS; ++k) {
-      const int eq = s_before + __popc(same[k] & lower);
-      if ((over[k] >> lane & 1u) || ((same[k] >> lane & 1u) && eq < want))
-        stays[base + o_before + __popc(over[k] & lower) + min(eq, want)] =
+      unsigned stay = over[k];
+      if (same[k]) {
+        // of the warp's equal ones the first that are still wanted
+        const bool mine = (same[k] >> lane & 1u) && s_before + __popc(same[k] & lower) < want;
+        stay |= __ballot_sync(0xffffffffu, mine);
+        s_before += __popc(same[k]);
+      }
+      if (stay >> lane & 1u)
+        stays[at + __popc(stay & lower)] =
             make_int2(k0 + warp * (32 * LANE_KEYS) + k * 32 + lane, __float_as_int(x[k]));
-      o_before += __popc(over[k]);
-      s_before += __popc(same[k]);
+      at += __popc(stay);
     }
     done = base + o_all + min(equal + s_all, want);
     equal += s_all;

@@ -5,7 +5,8 @@
 // made twice, by two kernels on tcgen05 tensor cores, neither of which writes any:
 //   stats_kernel  S = Q K^T, a row per TMEM lane: maxima and sums of weights, one lse for each row;
 //   sums_kernel   S^T = K Q^T, a key per lane: a thread adds the weights of its key, no lane to lane sums.
-// The third adds what the parts of a key's sum have, in their order, to the sums so far.
+// Behind the first join_kernel makes a row's lse of its parts, once for all who use it; behind the
+// second add_kernel adds the parts of a key's sum, in their order, to the sums so far.
 //
 // A query tile is 128 rows: P = 128 / rep positions of one request times the `rep` query heads that
 // share a KV head.  K is the exact FP16 integers that the cache holds; products of each group of 64
@@ -16,6 +17,22 @@
 // order (chunk, KV head, tile, step): row tiles walk their keys, key tiles the row tiles that see them.
 // Every CTA takes as many units, wherever a tile begins or ends, and leaves a part of each tile that it
 // had at place (tile + CTA) of a list, which is nobody else's; the tile's first and last CTA are noted.
+//
+// A CTA is persistent: a warp for copies (queries, and raw INT8 keys), one for products, one for scales,
+// four that make FP16 integers of keys, and sixteen for weights in two groups that take alternate
+// products, each half of the columns.  What bounds it is neither memory nor the tensor cores but the
+// weights' arithmetic and its waits: a unit of 128 x 128 is 16384 exponentials, 1024 cycles of the SM's
+// unit for them, and 512 of products; it takes about 1560 cycles in sums_kernel and 1850 in stats_kernel,
+// which has the maxima beside.  32 / 8 heads of 128, 4096 rows: 131 and 111 us, join and add 5 and 7;
+// 64 rows behind 20000 keys of six requests 98 and 126; two times 777 rows behind 3000 keys, 16 / 2 heads of
+// 256 (twice the products' columns to a weight): 66 and 53.  On the way, both kernels at 4096 rows:
+// eight warps for weights, each product by all of them 181 and 163; sixteen 169 and 156; sums by products of 128 rows
+// 160 and 151; lse joined once and scores kept in registers while they are weighed 176 and 140 (joined by
+// every CTA for each unit: 35 us of sums); two groups on alternate products 160 and 119; 32
+// columns in registers 136 and 113; one warp for scales 134 and 113.  Slower: polynomials for 2 or 4 of 8
+// pairs of exponentials (sums 122 and 139 for 116), TMEM read 16 or 32 columns at a time (116 to 130), eight warps
+// for integers (147), a maximum for every columns' group in stats (148 for 136), more registers for
+// the weights' warps taken from the others (spills).
 #include <cuda.h>
 
 #include <type_traits>

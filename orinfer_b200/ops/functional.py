@@ -742,9 +742,9 @@ def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: t
     references per page (page 0 is nobody's).
 
     Returns (table, lens, refs, status int32 [1]); ``out`` may be the inputs.  The slots' rows of
-    ``weights`` move along, with zeros behind, in place or to ``weights_out``; those of slots that are
-    not cut stay (``weights_out`` gets a copy), and a slot that is named again is cut once.  Status 1: not
-    enough free pages, 2: a slot that does not exist, a length that its row does not hold or a page
+    ``weights`` move along, with zeros behind, in place or to ``weights_out`` (which gets a copy of those
+    that are named and not cut, and nothing of the others).  A slot that is named again is cut once.
+    Status 1: not enough free pages, 2: a slot that does not exist, a length that its row does not hold or a page
     that nobody holds; nothing is changed then."""
     n = _slots(slots, where=cache.device)
     t, l, r = _tables((table, lens, refs), out, cache.device)
