@@ -6,7 +6,7 @@
 // (keys carry their rotary angle).  What is kept goes to fresh pages and the old ones lose a reference,
 // so pages that others share are never written, the move needs no order, and a call repeats.
 //
-// The first kernel looks, the second one changes.  In the first, one CTA does the bookkeeping of the pages (the
+// The first kernel looks, the second changes.  In the first, one CTA does the bookkeeping of the pages (the
 // lowest free ones, in the order of the requests), and beside it one per request, layer and KV head finds
 // its threshold, the weight of the last key that stays, by three histograms of the weights' bits (11, 11,
 // 10), and walks the keys once: those above the threshold, and of those equal to it the first so many, go

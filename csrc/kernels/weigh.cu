@@ -19,20 +19,22 @@
 // had at place (tile + CTA) of a list, which is nobody else's; the tile's first and last CTA are noted.
 //
 // A CTA is persistent: a warp for copies (queries, and raw INT8 keys), one for products, one for scales,
-// four that make FP16 integers of keys, and sixteen for weights in two groups that take alternate
-// products, each half of the columns.  What bounds it is neither memory nor the tensor cores but the
-// weights' arithmetic and its waits: a unit of 128 x 128 is 16384 exponentials, 1024 cycles of the SM's
-// unit for them, and 512 of products; it takes about 1560 cycles in sums_kernel and 1850 in stats_kernel,
-// which has the maxima beside.  32 / 8 heads of 128, 4096 rows: 131 and 111 us, join and add 5 and 7;
-// 64 rows behind 20000 keys of six requests 98 and 126; two times 777 rows behind 3000 keys, 16 / 2 heads of
-// 256 (twice the products' columns to a weight): 66 and 53.  On the way, both kernels at 4096 rows:
-// eight warps for weights, each product by all of them 181 and 163; sixteen 169 and 156; sums by products of 128 rows
-// 160 and 151; lse joined once and scores kept in registers while they are weighed 176 and 140 (joined by
-// every CTA for each unit: 35 us of sums); two groups on alternate products 160 and 119; 32
-// columns in registers 136 and 113; one warp for scales 134 and 113.  Slower: polynomials for 2 or 4 of 8
-// pairs of exponentials (sums 122 and 139 for 116), TMEM read 16 or 32 columns at a time (116 to 130), eight warps
-// for integers (147), a maximum for every columns' group in stats (148 for 136), more registers for
-// the weights' warps taken from the others (spills).
+// four that make FP16 integers of keys, and sixteen for weights, in two groups that have a product each
+// in turn, half of its columns to a warp.  What bounds it is neither memory nor the tensor cores but the
+// weights: a unit of 128 x 128 is 16384 exponentials, 1024 cycles of the SM's unit for them, and 512 of
+// products; it takes about 1560 cycles in sums_kernel (that unit 72 % busy, half of the issue slots used)
+// and 1850 in stats_kernel (60 %), which has other scales for each column and the reference beside.
+// 32 / 8 heads of 128, 4096 rows: 131 and 111 us, join and add 5 and 7; 64 rows behind 20000 keys of six
+// requests: 98 and 126; two times 777 rows behind 3000 keys, 16 / 2 heads of 256 (twice the products'
+// columns to a weight): 66 and 53.
+//
+// On the way, both kernels at 4096 rows: eight warps for weights 181 and 163; sixteen 169 and 156;
+// products of 128 rows in sums 160 and 151; lse joined once (by every CTA for each unit it cost 35 us of
+// sums) and scores kept in registers while they are weighed 176 and 140; two groups on alternate products
+// 160 and 119; 32 columns in registers 136 and 113; one warp for scales 134 and 113.  Slower: polynomials
+// for 2 or 4 of 8 pairs of exponentials (sums 122 and 139 for 116), TMEM read 16 or 32 columns at a time
+// (116 to 130), eight warps for integers (147), a maximum of every few columns in stats (148 for 136), more
+// registers for the weights' warps at the others' cost (spills).
 #include <cuda.h>
 
 #include <type_traits>
@@ -721,9 +723,8 @@ __global__ void __launch_bounds__(TILE) join_kernel(const Geometry g, const floa
       there ? -m - log2f(l) : -INFINITY;
 }
 
-// rows: join_kernel's.  parts: [key tiles + CTAs][2 groups][2 halves][128], sums of
-// what they have seen; span_out: a key tile's
-// first and last CTA.
+// rows: join_kernel's.  parts: [key tiles + CTAs][2 groups][2 halves][128], sums of what they have seen;
+// span_out: a key tile's first and last CTA.
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
     const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -1005,7 +1006,8 @@ __global__ void __launch_bounds__(THREADS, 1) sums_kernel(
       }
       if (!ok) break;
       i += here;
-      parts[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + group * 2 + half) * TILE + key_at] = total.x + total.y;
+      parts[(static_cast<size_t>(w.index + blockIdx.x) * PARTS + group * 2 + half) * TILE + key_at] =
+          total.x + total.y;
       if (tid == 0) {
         if (w.step == 0) span_out[2 * w.index] = blockIdx.x;
         if (w.step + here == w.steps) span_out[2 * w.index + 1] = blockIdx.x;
