@@ -261,8 +261,8 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     sees the softmax weights of the row's query heads of that KV head.  Rows of one request are added
     in their order; what no row sees stays.  With ``weights_out`` the sums of seen keys go there
     instead, so that a step may be taken back.  Rows see at most ``max_kv_len`` keys (by default as
-    many as the page table has), which the call's ``scratch`` is made for; keys beyond that, or beyond
-    what ``weights`` holds, get none and set the status word."""
+    many as the page table has), which the call's ``scratch`` is made for (4 bytes for each score); keys
+    beyond that, or beyond what ``weights`` holds, get none and set the status word."""
     _cuda(q, gate, row_req, row_pos, weights)
     where = q.device
     if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
@@ -346,7 +346,8 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     KV head, summed over the rows; chunks of one request are added in their order.  With
     ``weights_out`` the sums of seen keys go there instead.  A chunk that reaches beyond
     ``max_kv_len`` keys (by default as many as the page table and ``weights`` have), of more than
-    ``max_q_len`` rows or of rows that are not there is left out and sets the status word."""
+    ``max_q_len`` rows or of rows that are not there is left out and sets the status word.  The
+    workspace has 2 KB for 128 of ``max_kv_len`` keys of each chunk and KV head."""
     _cuda(q, chunks, weights)
     where = q.device
     if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
@@ -745,7 +746,8 @@ def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: t
     ``weights`` move along, with zeros behind, in place or to ``weights_out`` (which gets a copy of those
     that are named and not cut, and nothing of the others).  A slot that is named again is cut once.
     Status 1: not enough free pages, 2: a slot that does not exist, a length that its row does not hold or a page
-    that nobody holds; nothing is changed then."""
+    that nobody holds; nothing is changed then.  The workspace has 8 bytes for each kept key of a layer
+    and KV head."""
     n = _slots(slots, where=cache.device)
     t, l, r = _tables((table, lens, refs), out, cache.device)
     total, width = table.shape

@@ -190,3 +190,33 @@ def test_the_example_runs(cuda):
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
     assert [len(d) for d in module.main("tiny", 3, 20)] == [20] * 3
+
+
+def test_a_packet_of_decode_rows_and_chunks_counts_both(make):
+    """Two requests take a step while two prompts are prefilled, one of which lets its last ten rows count.
+    Every row that counts gives each head a weight of one (5e-4: see above), to its own request."""
+    from orinfer_b200.models.runner import Packet
+    pool = make("tiny", slots=4, bound=300, keep=200)
+    cfg, i32, heads = pool.runner.cfg, pool._i32, pool.runner.cfg.q_heads // pool.runner.cfg.kv_heads
+    a, b = pool.add(text(200, cfg.vocab, 1)), pool.add(text(33, cfg.vocab, 2))
+    free = [s for s in range(4) if s not in (a, b)]
+    pool._take([free[0], free[1]], [0, 0])
+    pool._grow([a, b], 1)
+    before = pool.weights.double().sum(3)
+    n = (100, 41)
+    ids = [7, 8, *text(n[0], cfg.vocab, 3), *text(n[1], cfg.vocab, 4)]
+    slots = [a, b, *[free[0]] * n[0], *[free[1]] * n[1]]
+    chunks = [[2, n[0], 0, free[0]], [2 + n[0], n[1], 0, free[1]]]
+    count = [chunks[0], [2 + n[0] + n[1] - 10, 10, n[1] - 10, free[1]]]
+    p = Packet(i32(ids), i32(slots), i32([200, 33, *range(n[0]), *range(n[1])]), pool.table, sum(n) + 2, 201,
+               torch.tensor([0, 1, sum(n) + 1], device=pool.device), chunks=i32(chunks), max_q_len=100,
+               decode_rows=2, max_chunk_kv=100, weights=list(pool.weights), weigh_chunks=i32(count))
+    logits = pool.runner.logits(p)
+    got = pool.weights.double().sum(3) - before
+    for slot, rows in ((a, 1), (b, 1), (free[0], n[0]), (free[1], 10)):
+        assert float((got[:, slot] / (rows * heads) - 1).abs().max()) <= 5e-4
+    assert bool((pool.weights[:, free[0], :, 100:] == 0).all())
+    assert bool((pool.weights[:, free[1], :, :n[1]] > 0).all()) and bool((pool.weights[:, b, :, 34:] == 0).all())
+    plain = pool.runner.logits(Packet(p.ids, p.row_req, p.row_pos, pool.table, p.rows, 201, p.logit_rows,
+                                      chunks=p.chunks, max_q_len=100, decode_rows=2, max_chunk_kv=100))
+    assert torch.equal(logits, plain)
