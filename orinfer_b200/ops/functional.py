@@ -263,7 +263,7 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     instead, so that a step may be taken back.  Rows see at most ``max_kv_len`` keys (by default as
     many as the page table has), which the call's ``scratch`` is made for (4 bytes for each score); keys
     beyond that, or beyond what ``weights`` holds, get none and set the status word."""
-    _cuda(q, gate, row_req, row_pos, weights)
+    _cuda(q)                                         # (and the others are on its GPU)
     where = q.device
     if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
         raise native.KernelError("q: fp16 [rows, heads, D]")
@@ -292,17 +292,21 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     elif (out.dtype != torch.float16 or not out.is_contiguous() or out.numel() < live * qh * d
           or out.device != where):
         raise native.KernelError("out: fp16 [rows, heads * D]")
-    need = native.lib().orinfer_attention_weighed_scratch_bytes(live, qh, d, splits, keys)
+    lib = native.lib()
+    need = lib.orinfer_attention_weighed_scratch_bytes(live, qh, d, splits, keys)
     if scratch is None:
         scratch = torch.empty(need // 4, dtype=torch.float32, device=where)
     elif (scratch.numel() * scratch.element_size() < need or not scratch.is_contiguous()
           or scratch.device != where):
         raise native.KernelError(f"scratch: {need} bytes")
-    check(native.lib().orinfer_attention_weighed(
-        ptr(q), ptr(gate), ptr(row_req), ptr(row_pos), ptr(page_table), width,
-        ptr(kcache), ptr(vcache), ptr(kscale), ptr(vscale), ptr(out), ptr(weights),
-        weights.stride(0), weights.stride(1), ptr(sums), sums.stride(0), sums.stride(1), capacity,
-        live, qh, kvh, d, splits, keys, ptr(scratch), max_kv_len or 0, stream()), "attention_weighed")
+    slot_stride, head_stride, _ = weights.stride()
+    sums_slot_stride, sums_head_stride, _ = sums.stride()
+    check(lib.orinfer_attention_weighed(
+        q.data_ptr(), ptr(gate), row_req.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(), width,
+        kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), out.data_ptr(),
+        weights.data_ptr(), slot_stride, head_stride, sums.data_ptr(), sums_slot_stride,
+        sums_head_stride, capacity, live, qh, kvh, d, splits, keys, scratch.data_ptr(), max_kv_len or 0,
+        stream()), "attention_weighed")
     count_launches(2 if live else 0)
     return out
 
@@ -348,7 +352,7 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     ``max_kv_len`` keys (by default as many as the page table and ``weights`` have), of more than
     ``max_q_len`` rows or of rows that are not there is left out and sets the status word.  The
     workspace has 2 KB for 128 of ``max_kv_len`` keys of each chunk and KV head."""
-    _cuda(q, chunks, weights)
+    _cuda(q)                                         # (and the others are on its GPU)
     where = q.device
     if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
         raise native.KernelError("q: fp16 [rows, heads, D]")
@@ -375,12 +379,15 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     max_q_len = min(max_q_len, live)
     if chunks.shape[0] == 0 or max_q_len == 0 or limit <= 0:
         return
-    work = torch.empty(native.lib().orinfer_prefill_weights_work_bytes(
+    lib = native.lib()
+    work = torch.empty(lib.orinfer_prefill_weights_work_bytes(
         chunks.shape[0], max_q_len, kvh, qh // kvh, limit) // 4, dtype=torch.float32, device=where)
-    check(native.lib().orinfer_prefill_weights(
-        ptr(q), ptr(chunks), chunks.shape[0], max_q_len, live, ptr(page_table), lead, width,
-        ptr(kcache), ptr(kscale), pages, ptr(weights), weights.stride(0),
-        weights.stride(1), ptr(sums), sums.stride(0), sums.stride(1), limit, qh, kvh, d, ptr(work),
+    slot_stride, head_stride, _ = weights.stride()
+    sums_slot_stride, sums_head_stride, _ = sums.stride()
+    check(lib.orinfer_prefill_weights(
+        q.data_ptr(), chunks.data_ptr(), chunks.shape[0], max_q_len, live, page_table.data_ptr(), lead,
+        width, kcache.data_ptr(), kscale.data_ptr(), pages, weights.data_ptr(), slot_stride, head_stride,
+        sums.data_ptr(), sums_slot_stride, sums_head_stride, limit, qh, kvh, d, work.data_ptr(),
         stream()), "prefill_weights")
     count_launches(4)
 
