@@ -116,9 +116,7 @@ class BoundedRequests(SlotPages):
     def step(self, tokens: Dict[int, int]) -> torch.Tensor:
         """Appends a token to each of the given slots; returns their logits, in that order."""
         slots = list(tokens)
-        for s in slots:
-            if s not in self.text:
-                raise ValueError(f"slot {s} holds no request")
+        self._known(slots)
         if not 0 < len(slots) <= self.runner.ws.max_rows:
             raise ValueError(f"{len(slots)} requests, at most {self.runner.ws.max_rows} at once")
         self.cut([s for s in slots if self._len[s] == self.bound])
@@ -140,6 +138,7 @@ class BoundedRequests(SlotPages):
         ``stop(tokens)`` says so, and may go on with another call."""
         if len(slots) != len(options) or len(set(slots)) != len(slots):
             raise ValueError("options for each slot, a slot once")
+        self._known(slots)
         for o in options:
             o.validate()
         got: Dict[int, List[int]] = {s: [] for s in slots}
@@ -158,8 +157,14 @@ class BoundedRequests(SlotPages):
 
     def drop(self, slot: int) -> None:
         """Gives up a request."""
+        self._known([slot])
         del self.text[slot]
         self._give_up(slot)
+
+    def _known(self, slots: Sequence[int]) -> None:
+        for s in slots:
+            if s not in self.text:
+                raise ValueError(f"slot {s} holds no request")
 
     def _give_up(self, slot: int) -> None:
         self.logits.pop(slot, None)

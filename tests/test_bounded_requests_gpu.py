@@ -220,3 +220,16 @@ def test_a_packet_of_decode_rows_and_chunks_counts_both(make):
     plain = pool.runner.logits(Packet(p.ids, p.row_req, p.row_pos, pool.table, p.rows, 201, p.logit_rows,
                                       chunks=p.chunks, max_q_len=100, decode_rows=2, max_chunk_kv=100))
     assert torch.equal(logits, plain)
+
+
+def test_a_slot_without_a_request_is_refused(make):
+    pool = make("tiny")
+    slot = pool.add([1, 2, 3])
+    option = S.SamplingOptions(temperature=0.9, top_k=5)
+    other = slot - 1 if slot else slot + 1
+    for call in (lambda: pool.generate([slot, other], [option] * 2, 2), lambda: pool.step({other: 1}),
+                 lambda: pool.drop(other), lambda: pool.generate([slot, slot], [option] * 2, 2)):
+        with pytest.raises(ValueError):
+            call()
+    assert pool.text[slot] == [1, 2, 3] and pool.held == 1
+    assert pool.generate([slot], [option], 0) == [[]] and pool.generate([], [], 3) == []
