@@ -181,7 +181,8 @@ int orinfer_qgemm_grouped_launches(int fmt, int S, int experts, int max_tiles, i
 size_t orinfer_attention_scratch_bytes(int rows, int qh, int head_dim, int splits);
 int orinfer_attention_starts_early(int rows, int kvh, int head_dim, int splits);
 int orinfer_attention_in_digits(int qh, int kvh, int head_dim, int max_pages, int splits);
-// context: keys that any row sees at most, 0 for as many as the page table has.
+// context: keys that any row sees at most, 0 for as many as the page table has.  Keys and values on
+// 16-byte boundaries.
 int orinfer_attention(const __half* q, const __half* gate, const int* row_req, const int* row_pos,
                       const int* page_table, int max_pages, const int8_t* kcache,
                       const int8_t* vcache, const __half* kscale, const __half* vscale,

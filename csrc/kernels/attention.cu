@@ -1455,6 +1455,11 @@ extern "C" int orinfer_attention_starts_early(int rows, int kvh, int head_dim, i
   return attn_starts_early(head_dim, static_cast<long long>(rows) * kvh * splits) ? 1 : 0;
 }
 
+// Both forms copy keys and values 16 bytes at a time.
+static bool attn_cache_aligned(const int8_t* kc, const int8_t* vc) {
+  return ((reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc)) & 15) == 0;
+}
+
 // Whether such a call takes the digit form (given aligned tensors).
 extern "C" int orinfer_attention_in_digits(int qh, int kvh, int head_dim, int max_pages,
                                            int splits) {
@@ -1470,6 +1475,7 @@ extern "C" int orinfer_attention(const __half* q, const __half* gate, const int*
                                  cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (splits < 1 || (splits > 1 && scratch == nullptr) || kvh <= 0 || qh % kvh) return -1;
+  if (!attn_cache_aligned(kc, vc)) return -1;
   const int rep = qh / kvh;
 #define CASE(DD)                                                                            \
   if (head_dim == DD)                                                                       \
@@ -1502,7 +1508,7 @@ extern "C" int orinfer_attention_weighed(
     int context, cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (splits < 1 || splits > 32 || keys < 1 || scratch == nullptr || kvh <= 0 || qh % kvh) return -1;
-  if (weights == nullptr || sums == nullptr || capacity < 0) return -1;
+  if (weights == nullptr || sums == nullptr || capacity < 0 || !attn_cache_aligned(kc, vc)) return -1;
   if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return -1;
   const int rep = qh / kvh;
   if (rep != 1 && rep != 2 && rep != 4 && rep != 8 && !(rep == 5 && head_dim == 128)) return -1;

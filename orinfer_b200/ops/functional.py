@@ -271,6 +271,8 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     _, kvh, dim = _cached(where, page_table, kcache, kscale, vcache, vscale)
     if d != dim or qh % kvh != 0:
         raise native.KernelError(f"{qh} query heads of {d} on {kvh} KV heads of {dim} channels")
+    if kcache.data_ptr() % 16 or vcache.data_ptr() % 16:
+        raise native.KernelError("kcache and vcache on 16-byte boundaries")
     if gate is not None and (gate.dtype != torch.float16 or gate.numel() != q.numel()
                              or not gate.is_contiguous() or gate.device != where):
         raise native.KernelError("gate: fp16, as many as q has")
