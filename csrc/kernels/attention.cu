@@ -73,6 +73,10 @@ struct Weighed {
   float* scores = nullptr;         // [rows][query heads][keys]
   float2* ml = nullptr;            // [rows][query heads][splits]
   int keys = 0;                    // a multiple of 4; what a row sees beyond is not written
+  int slots = 0;                   // rows of the page table, and of the sums
+  // A row of a request that is not there sees nothing: its index leads out of the table and, in
+  // attn_weigh_kernel, which reports it, out of the caller's sums.
+  __device__ __forceinline__ bool there(int req) const { return req >= 0 && req < slots; }
 };
 
 // One CTA per (row, KV head, key split); its four warps take blocks of KB keys in turn (a block
@@ -275,7 +279,8 @@ __global__ void __launch_bounds__(
   const int row = blockIdx.x, split = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int kv_len = row_pos[row] + 1;
+  const int req = row_req[row];
+  const int kv_len = WEIGH && !weighed.there(req) ? 0 : row_pos[row] + 1;
   const bool apart = APART && kv_len <= apart_keys;
   if (apart && (blockIdx.y & (ATTN_WARPS - 1)) != 0) return;
   const int h = apart ? min(static_cast<int>(blockIdx.y) + warp, kvh - 1) : blockIdx.y;
@@ -283,7 +288,7 @@ __global__ void __launch_bounds__(
   const int first = SHARED ? min(parts.rows[row].x, max(kv_len, 0)) : 0;
   const int per = (kv_len - first + splits - 1) / splits;
   const int k_lo = first + split * per, k_hi = min(kv_len, k_lo + per);
-  const int* pages = page_table + static_cast<size_t>(row_req[row]) * max_pages;
+  const int* pages = page_table + static_cast<size_t>(req) * max_pages;
   const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
 
   using T = AttnTile<D>;
@@ -657,7 +662,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
   const int row = blockIdx.x, split = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3, upper = lane >> 4, head = g & 3;
-  const int kv_len = row_pos[row] + 1;
+  const int req = row_req[row];
+  const int kv_len = WEIGH && !weighed.there(req) ? 0 : row_pos[row] + 1;
   const bool apart = APART && kv_len <= apart_keys;
   if (apart && (blockIdx.y & (ATTN_WARPS - 1)) != 0) return;
   const int h = apart ? min(static_cast<int>(blockIdx.y) + warp, kvh - 1) : blockIdx.y;
@@ -665,7 +671,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
   const int first = SHARED ? min(parts.rows[row].x, max(kv_len, 0)) : 0;
   const int per = (kv_len - first + splits - 1) / splits;
   const int k_lo = first + split * per, k_hi = min(kv_len, k_lo + per);
-  const int* pages = page_table + static_cast<size_t>(row_req[row]) * max_pages;
+  const int* pages = page_table + static_cast<size_t>(req) * max_pages;
 
   extern __shared__ unsigned char digits_smem[];
   unsigned char* smem = digits_smem + ((1024u - (smem_u32(digits_smem) & 1023u)) & 1023u);
@@ -1235,8 +1241,12 @@ __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_ker
   float2 own_part = make_float2(-INFINITY, 0.f);
   if (warp < REP) own_part = part(row, h_lo * REP + warp);
   if (pos < 0) return;
-  if (tid == 0 && z == 0 && blockIdx.y == 0 && pos >= limit)
-    report_status(status, STATUS_BAD_INDEX, 0x60);
+  const bool reports = tid == 0 && z == 0 && blockIdx.y == 0;
+  if (!weighed.there(req)) {
+    if (reports) report_status(status, STATUS_BAD_INDEX, 0x61);
+    return;
+  }
+  if (reports && pos >= limit) report_status(status, STATUS_BAD_INDEX, 0x60);
   float4 v[REP];                                   // scores of a row
   auto ask = [&](int r, int n, int h) {
 #pragma unroll
@@ -1501,19 +1511,20 @@ extern "C" size_t orinfer_attention_weighed_scratch_bytes(int rows, int qh, int 
 
 extern "C" int orinfer_attention_weighed(
     const __half* q, const __half* gate, const int* row_req, const int* row_pos,
-    const int* page_table, int max_pages, const int8_t* kc, const int8_t* vc, const __half* ks,
-    const __half* vs, __half* out, const float* weights, long long slot_stride,
+    const int* page_table, int slots, int max_pages, const int8_t* kc, const int8_t* vc,
+    const __half* ks, const __half* vs, __half* out, const float* weights, long long slot_stride,
     long long head_stride, float* sums, long long sums_slot_stride, long long sums_head_stride,
     int capacity, int rows, int qh, int kvh, int head_dim, int splits, int keys, float* scratch,
     int context, cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (splits < 1 || splits > 32 || keys < 1 || scratch == nullptr || kvh <= 0 || qh % kvh) return -1;
-  if (weights == nullptr || sums == nullptr || capacity < 0 || !attn_cache_aligned(kc, vc)) return -1;
+  if (weights == nullptr || sums == nullptr || capacity < 0 || slots < 0 || !attn_cache_aligned(kc, vc)) return -1;
   if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return -1;
   const int rep = qh / kvh;
   if (rep != 1 && rep != 2 && rep != 4 && rep != 8 && !(rep == 5 && head_dim == 128)) return -1;
   Weighed w;
   w.keys = (keys + 3) / 4 * 4;
+  w.slots = slots;
   const size_t heads = static_cast<size_t>(rows) * qh;
   w.scores = scratch;
   w.ml = reinterpret_cast<float2*>(scratch + heads * w.keys);

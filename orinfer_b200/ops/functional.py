@@ -262,7 +262,8 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     in their order; what no row sees stays.  With ``weights_out`` the sums of seen keys go there
     instead, so that a step may be taken back.  Rows see at most ``max_kv_len`` keys (by default as
     many as the page table has), which the call's ``scratch`` is made for (4 bytes for each score); keys
-    beyond that, or beyond what ``weights`` holds, get none and set the status word."""
+    beyond that, or beyond what ``weights`` holds, get none and set the status word.  A row whose request
+    is no row of the page table sees nothing, adds nothing and sets it too; one at position -1 is padding."""
     _cuda(q)                                         # (and the others are on its GPU)
     where = q.device
     if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
@@ -304,8 +305,8 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     slot_stride, head_stride, _ = weights.stride()
     sums_slot_stride, sums_head_stride, _ = sums.stride()
     check(lib.orinfer_attention_weighed(
-        q.data_ptr(), ptr(gate), row_req.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(), width,
-        kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), out.data_ptr(),
+        q.data_ptr(), ptr(gate), row_req.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(), lead,
+        width, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), out.data_ptr(),
         weights.data_ptr(), slot_stride, head_stride, sums.data_ptr(), sums_slot_stride,
         sums_head_stride, capacity, live, qh, kvh, d, splits, keys, scratch.data_ptr(), max_kv_len or 0,
         stream()), "attention_weighed")
