@@ -263,16 +263,18 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     instead, so that a step may be taken back.  Rows see at most ``max_kv_len`` keys (by default as
     many as the page table has), which the call's ``scratch`` is made for (4 bytes for each score); keys
     beyond that, or beyond what ``weights`` holds, get none and set the status word.  A row whose request
-    is no row of the page table sees nothing, adds nothing and sets it too; one at position -1 is padding."""
+    is no row of the page table sees nothing, adds nothing and sets it too, and so does a page that the
+    cache does not have, for which page 0 is read; a row at position -1 is padding."""
     _cuda(q)                                         # (and the others are on its GPU)
     where = q.device
     if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
         raise native.KernelError("q: fp16 [rows, heads, D]")
     n, qh, d = q.shape
-    _, kvh, dim = _cached(where, page_table, kcache, kscale, vcache, vscale)
+    pages, kvh, dim = _cached(where, page_table, kcache, kscale, vcache, vscale)
     if d != dim or qh % kvh != 0:
         raise native.KernelError(f"{qh} query heads of {d} on {kvh} KV heads of {dim} channels")
-    if kcache.data_ptr() % 16 or vcache.data_ptr() % 16:
+    k_at, v_at = kcache.data_ptr(), vcache.data_ptr()
+    if (k_at | v_at) & 15:
         raise native.KernelError("kcache and vcache on 16-byte boundaries")
     if gate is not None and (gate.dtype != torch.float16 or gate.numel() != q.numel()
                              or not gate.is_contiguous() or gate.device != where):
@@ -306,8 +308,8 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     sums_slot_stride, sums_head_stride, _ = sums.stride()
     check(lib.orinfer_attention_weighed(
         q.data_ptr(), ptr(gate), row_req.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(), lead,
-        width, kcache.data_ptr(), vcache.data_ptr(), kscale.data_ptr(), vscale.data_ptr(), out.data_ptr(),
-        weights.data_ptr(), slot_stride, head_stride, sums.data_ptr(), sums_slot_stride,
+        width, k_at, v_at, kscale.data_ptr(), vscale.data_ptr(), pages,
+        out.data_ptr(), weights.data_ptr(), slot_stride, head_stride, sums.data_ptr(), sums_slot_stride,
         sums_head_stride, capacity, live, qh, kvh, d, splits, keys, scratch.data_ptr(), max_kv_len or 0,
         stream()), "attention_weighed")
     count_launches(2 if live else 0)

@@ -28,5 +28,5 @@ def test_the_entries_refuse_a_cache_off_16_bytes(kc, vc):
     lib = native.lib()
     assert lib.orinfer_attention(at, None, at, at, at, 1, *cache, at, at, at, 1, 2, 1, 128, 1, None, 0,
                                  None) == -1
-    assert lib.orinfer_attention_weighed(at, None, at, at, at, 1, 1, *cache, at, at, at, at, 256, 128, at,
-                                         256, 128, 128, 1, 2, 1, 128, 1, 128, at, 0, None) == -1
+    assert lib.orinfer_attention_weighed(at, None, at, at, at, 1, 1, *cache, at, at, 1, at, at, 256, 128,
+                                         at, 256, 128, 128, 1, 2, 1, 128, 1, 128, at, 0, None) == -1

@@ -69,3 +69,45 @@ def test_padding_of_any_request_is_no_fault(dev):
     args[3] = torch.tensor([199, -1, -1], dtype=torch.int32, device=dev)
     out = F.attention_weighed(*args, sums(dev, args), splits=2)
     assert status() == (0, 0) and bool((out[1:] == 0).all())
+
+
+@pytest.mark.parametrize("qh,kvh,d,splits", FORMS)
+def test_positions_behind_the_row_of_the_table(dev, qh, kvh, d, splits):
+    """Such a row sees what its row of the table has; the last one's would end behind the table.  Its
+    keys are cut into parts elsewhere, so that outputs are two roundings to FP16 of sums of 384 terms
+    of at most 127 x 0.02, whose own roundings are 384 steps of 2^-24 of that each."""
+    from orinfer_b200.ops import functional as F
+    args = list(batch(dev, [3 * 128, 100, 3 * 128], qh, kvh, d, seed=6))
+    args[4] = args[4][:, :3].contiguous()
+    want = F.attention(*args, splits=splits)
+    base = sums(dev, args)
+    weights, good = base.clone(), args[3].clone()
+    args[3] = torch.tensor([10**6, 99, 3 * 128], dtype=torch.int32, device=dev)
+    out = F.attention_weighed(*args, weights, splits=splits)
+    assert status() == (BAD_INDEX, 0x60)
+    args[3] = good
+    off = (out.double() - want.double()).abs()
+    assert bool((off <= 2.0 ** -10 * want.double().abs() + 2 * 384 * 2.0 ** -24 * 2.54).all())
+    assert torch.equal(out[1], want[1])
+    near(weights, base, args)
+
+
+@pytest.mark.parametrize("qh,kvh,d,splits", FORMS)
+@pytest.mark.parametrize("bad", [-1, 10**9, "first"])
+def test_pages_that_the_cache_does_not_have(dev, qh, kvh, d, splits, bad):
+    """Page 0 is read for them; here it has the keys of the page that the table should name."""
+    from orinfer_b200.ops import functional as F
+    args = list(batch(dev, [5000, 700, 90], qh, kvh, d, seed=7))
+    for row, column in ((0, 20), (0, 39), (1, 5), (2, 0)):
+        table = args[4]
+        for cache in args[5:]:
+            cache[0] = cache[int(table[row, column])]
+        want = F.attention(*args, splits=splits)
+        base = sums(dev, args)
+        given, weights = list(args), base.clone()
+        given[4] = table.clone()
+        given[4][row, column] = args[5].shape[0] if bad == "first" else bad
+        out = F.attention_weighed(*given, weights, splits=splits)
+        assert status() == (BAD_INDEX, 0x62)
+        assert torch.equal(out, want)
+        near(weights, base, args)
