@@ -72,7 +72,8 @@ struct RowScales {
 struct Weighed {
   float* scores = nullptr;         // [rows][query heads][keys]
   float2* ml = nullptr;            // [rows][query heads][splits]
-  int keys = 0;                    // a multiple of 4; what a row sees beyond is not written
+  int keys = 0;                    // places of a row's scores, a multiple of 4; what it sees beyond is not written
+  int counted = 0;                 // of them those whose keys get their weights
   int slots = 0;                   // rows of the page table, and of the sums
   int most = 0;                    // keys that a row of the table has a place for
   int pages = 0;                   // of the cache
@@ -1253,7 +1254,7 @@ __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_ker
     const float l = warp_sum(own.x == -INFINITY ? 0.f : own.y * exp2f(own.x - m));
     return make_float2(m, l > 0.f ? 1.f / l : l == 0.f ? 0.f : l);
   };
-  const int pos = row_pos[row], req = row_req[row], limit = min(weighed.keys, capacity);
+  const int pos = row_pos[row], req = row_req[row], limit = min(weighed.counted, capacity);
   int other_pos = tid < rows ? row_pos[tid] : -1, other_req = tid < rows ? row_req[tid] : 0;
   float2 own_part = make_float2(-INFINITY, 0.f);
   if (warp < REP) own_part = part(row, h_lo * REP + warp);
@@ -1552,6 +1553,7 @@ extern "C" int orinfer_attention_weighed(
   if (rep != 1 && rep != 2 && rep != 4 && rep != 8 && !(rep == 5 && head_dim == 128)) return -1;
   Weighed w;
   w.keys = (keys + 3) / 4 * 4;
+  w.counted = keys;
   w.slots = slots;
   w.most = max_pages * 128;
   w.pages = num_pages;

@@ -111,3 +111,20 @@ def test_pages_that_the_cache_does_not_have(dev, qh, kvh, d, splits, bad):
         assert status() == (BAD_INDEX, 0x62)
         assert torch.equal(out, want)
         near(weights, base, args)
+
+
+@pytest.mark.parametrize("most", [1, 97, 98, 99, 100])
+@pytest.mark.parametrize("over", [0, 1, 2])
+def test_the_bound_of_keys_is_met_to_the_key(dev, most, over):
+    """Keys behind ``max_kv_len`` get nothing and are reported, wherever it lies among four."""
+    from orinfer_b200.ops import functional as F
+    args = batch(dev, [most + over, 1], 4, 2, 64)
+    base = sums(dev, args)
+    weights = base.clone()
+    F.attention_weighed(*args, weights, max_kv_len=most)
+    assert status() == ((BAD_INDEX, 0x60) if over else (0, 0))
+    want = base.clone()
+    F.attention_weighed(*args, want)
+    assert status() == (0, 0)
+    assert torch.equal(weights[..., :most], want[..., :most])
+    assert torch.equal(weights[..., most:], base[..., most:])
