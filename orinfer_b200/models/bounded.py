@@ -64,12 +64,11 @@ class BoundedRequests(SlotPages):
             self._len.update(dict.fromkeys(slots, self.keep))
         return int(status) == 0
 
-    def _grow(self, slots: Sequence[int], tokens: int) -> None:
-        """Pages for ``tokens`` more tokens of each slot."""
+    def _grow(self, slots: Sequence[int], tokens: int):
+        """Pages for ``tokens`` more tokens of each slot; returns what was taken, or None."""
         at = [(s, c) for s in slots for c in range(-(-self._len[s] // PAGE_TOKENS),
                                                    -(-(self._len[s] + tokens) // PAGE_TOKENS))]
-        if at:
-            self._take([s for s, _ in at], [c for _, c in at])
+        return self._take([s for s, _ in at], [c for _, c in at]) if at else None
 
     def _wrote(self, slots: Sequence[int], tokens: int) -> None:
         self.lens[torch.tensor(list(slots), device=self.device)] += tokens
@@ -114,19 +113,33 @@ class BoundedRequests(SlotPages):
         return logits
 
     def step(self, tokens: Dict[int, int]) -> torch.Tensor:
-        """Appends a token to each of the given slots; returns their logits, in that order."""
+        """Appends a token to each of the given slots; returns their logits, in that order.  Where the
+        forward raises, the requests are as they were before it, though cut down if they were at the
+        bound, and the step may be taken again; those of a model with recurrent layers, whose states have
+        moved on, are given up."""
         slots = list(tokens)
         self._known(slots)
         if not 0 < len(slots) <= self.runner.ws.max_rows:
             raise ValueError(f"{len(slots)} requests, at most {self.runner.ws.max_rows} at once")
         self.cut([s for s in slots if self._len[s] == self.bound])
-        self._grow(slots, 1)
         at = [self._len[s] for s in slots]
         p = Packet(self._i32([int(tokens[s]) for s in slots]), self._i32(slots), self._i32(at),
                    self.table, len(slots), max(at) + 1, weights=self.weights,
                    rope_pos=self._i32([len(self.text[s]) for s in slots]))
-        logits = self.runner.logits(p)
-        self._wrote(slots, 1)
+        rows = torch.tensor(slots, device=self.device)
+        before = self.weights[:, rows, :, :max(at) + 1]      # (a copy)
+        taken = self._grow(slots, 1)
+        try:
+            logits = self.runner.logits(p)
+            self._wrote(slots, 1)
+        except BaseException:
+            self.weights[:, rows, :, :max(at) + 1] = before
+            if taken is not None:
+                self._put_back(taken)
+            if self.runner.cfg.arch == "hybrid":
+                for s in slots:
+                    self.drop(s)
+            raise
         for r, s in enumerate(slots):
             self.text[s].append(int(tokens[s]))
             self.logits[s] = logits[r]

@@ -26,16 +26,24 @@ class SlotPages:
     def _i32(self, v):
         return torch.tensor(v, dtype=torch.int32, device=self.device)
 
-    def _take(self, slots: Sequence[int], columns: Sequence[int]) -> None:
-        """Gives each slot a free page at a column of its row, the lowest pages first."""
+    def _take(self, slots: Sequence[int], columns: Sequence[int]):
+        """Gives each slot a free page at a column of its row, the lowest pages first; returns what
+        ``_put_back`` needs."""
         held = self.refs.cpu()
         pages = [p for p in range(1, len(held)) if held[p] == 0][:len(slots)]
         if len(pages) < len(slots):
             raise MemoryError(f"{len(slots)} pages wanted, {len(pages)} free")
-        at = torch.tensor(pages, device=self.device)
+        at, where = torch.tensor(pages, device=self.device), (
+            torch.tensor(slots, device=self.device), torch.tensor(columns, device=self.device))
         self.refs[at] = 1
-        self.table[torch.tensor(slots, device=self.device),
-                   torch.tensor(columns, device=self.device)] = at.int()
+        self.table[where] = at.int()
+        return at, where
+
+    def _put_back(self, taken) -> None:
+        """Undoes a ``_take`` whose pages nothing has been forked from."""
+        at, where = taken
+        self.table[where] = 0
+        self.refs[at] = 0
 
     def _release(self, slots: Sequence[int]) -> None:
         F.free_pages(self.table, self.lens, self.refs, self._i32(list(slots)),
