@@ -227,13 +227,7 @@ class ModelRunner:
     def _attention_core(self, lw: LayerWeights, kv_slot: int, qkv, p: Packet, rows: int):
         """q/k head norm + RoPE + INT8 KV write, then attention into ``ws.attn``."""
         cfg, ws = self.cfg, self.ws
-        weights = None
-        if p.weights is not None:
-            if p.shared is not None or p.attend_pos is not None or kv_slot >= len(p.weights) or (
-                    p.weigh_chunks is not None and p.chunks is None):
-                raise ValueError("weights of attention layers, for rows that see their own keys as far "
-                                 "as themselves; weigh_chunks of chunks")
-            weights = p.weights[kv_slot]
+        weights = None if p.weights is None else p.weights[kv_slot]
         F.qk_rope_kv(qkv, lw.q_norm if cfg.qk_norm else None, lw.k_norm if cfg.qk_norm else None,
                      ws.cos, ws.sin, p.row_req, p.row_pos, p.page_table, self.kv.k[kv_slot],
                      self.kv.v[kv_slot], self.kv.ks[kv_slot], self.kv.vs[kv_slot],
@@ -244,8 +238,6 @@ class ModelRunner:
         gated = cfg.gated_attention and lw.qkv.n == cfg.q_dim + 2 * cfg.kv_dim
         gate = ws.gate if gated else None
         if p.shared is not None:
-            if p.chunks is not None or p.attend_pos is not None:
-                raise ValueError("a packet with shared prefixes has single rows only")
             F.attention_shared(ws.q[:rows], None if gate is None else gate[:rows], p.row_req,
                                p.row_pos, p.page_table, self.kv.k[kv_slot], self.kv.v[kv_slot],
                                self.kv.ks[kv_slot], self.kv.vs[kv_slot], p.shared,
@@ -440,12 +432,36 @@ class ModelRunner:
         return self._row_parallel("down", lw.down, q8, sc, rows)
 
     # ---------------------------------------------------------------- forward
+    def _check(self, p: Packet, kv_slots: Sequence[int]) -> None:
+        """Raises for a packet that the attention layers at these places of the pool would not
+        serve: here, since a layer that refuses comes behind others that have changed the cache, the
+        recurrent states and the packet's weights."""
+        if p.rows > self.ws.max_rows:
+            raise ValueError(f"packet of {p.rows} rows exceeds workspace ({self.ws.max_rows})")
+        if p.shared is not None and (p.chunks is not None or p.attend_pos is not None):
+            raise ValueError("a packet with shared prefixes has single rows only")
+        at = p.rope_pos
+        if at is not None and (p.mrope is not None or at.dtype != torch.int32 or at.dim() != 1
+                               or at.numel() < p.rows or not at.is_contiguous()
+                               or at.device != p.row_pos.device):
+            raise ValueError("rope_pos: int32, one for each row, beside row_pos; not with mrope")
+        if p.weights is None:
+            return
+        if p.shared is not None or p.attend_pos is not None or len(p.weights) <= max(kv_slots, default=0) or (
+                p.weigh_chunks is not None and p.chunks is None):
+            raise ValueError("weights of attention layers, for rows that see their own keys as far "
+                             "as themselves; weigh_chunks of chunks")
+        chunks = p.chunks if p.weigh_chunks is None else p.weigh_chunks
+        rows = p.rows if p.chunks is None else p.decode_rows
+        for slot in kv_slots[:1] if isinstance(p.weights, torch.Tensor) else kv_slots:
+            F.check_weighing(p.weights[slot], p.page_table, self.kv.k[slot], self.cfg.q_heads, rows=rows,
+                             chunks=chunks)
+
     def forward_hidden(self, p: Packet):
         """Runs embedding + all layers; leaves the last branch output in ws.hidden and
         the running residual in ws.resid (final residual = resid + hidden)."""
         cfg, ws, rows = self.cfg, self.ws, p.rows
-        if rows > ws.max_rows:
-            raise ValueError(f"packet of {rows} rows exceeds workspace ({ws.max_rows})")
+        self._check(p, list(self._attn_index.values()))
         x = F.embed_w8(p.ids, self.w.embed_q, self.w.embed_s, out=ws.hidden)
         if p.overlay_rows is not None:
             x.index_copy_(0, p.overlay_rows, p.overlay.to(x.dtype))
@@ -626,6 +642,7 @@ class ModelRunner:
         concat(norm_e(embed), norm_h(hidden)) -> fc -> one decoder layer -> norm -> shared head
         (kernels/cuda/model/speculation.py:31 mtp_norm_concat of the reference)."""
         cfg, ws, m, rows = self.cfg, self.ws, self.w.mtp, p.rows
+        self._check(p, [self.mtp_kv_index])
         h = cfg.hidden
         if getattr(ws, "mtp_buf", None) is None:
             e = lambda *s, dt=torch.float16: torch.empty(*s, dtype=dt, device=self.device)

@@ -46,13 +46,18 @@ class TorchRunner:
         return R.qgemm(q, s, self._w(lin), lin.scale, out_f32)
 
     @staticmethod
+    def _check(p: Packet) -> None:
+        if p.weights is not None:
+            raise ValueError("the plain runner does not count attention weights")
+        if p.rope_pos is not None and p.mrope is not None:
+            raise ValueError("rope_pos: not with mrope")
+
+    @staticmethod
     def _angles(p: Packet) -> torch.Tensor:
         return (p.row_pos if p.rope_pos is None else p.rope_pos)[:p.rows]
 
     def _attention(self, lw: LayerWeights, slot: int, y: torch.Tensor, p: Packet, cos, sin):
         cfg = self.cfg
-        if p.weights is not None:
-            raise ValueError("the plain runner does not count attention weights")
         rows, d, qh, kvh = p.rows, cfg.head_dim, cfg.q_heads, cfg.kv_heads
         proj = self._linear(lw.qkv, y)
         gated = cfg.gated_attention and lw.qkv.n == cfg.q_dim + 2 * cfg.kv_dim
@@ -169,6 +174,7 @@ class TorchRunner:
     supports_media = True
 
     def forward_hidden(self, p: Packet):
+        self._check(p)
         cfg = self.cfg
         rows = p.rows
         x = R.embed_w8(p.ids[:rows], self.w.embed_q, self.w.embed_s)
@@ -232,6 +238,7 @@ class TorchRunner:
 
     def mtp_rows(self, tokens: torch.Tensor, hidden: torch.Tensor, p: Packet):
         """Same contract as ModelRunner.mtp_rows, in plain PyTorch."""
+        self._check(p)
         cfg, m, rows = self.cfg, self.w.mtp, p.rows
         zc = cfg.zero_centered_norm
         e = R.embed_w8(tokens[:rows], self.w.embed_q, self.w.embed_s)

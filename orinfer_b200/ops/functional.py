@@ -249,6 +249,31 @@ def _cached(where, page_table, codes, scales, *more):
     return pages, kvh, d
 
 
+def _chunk_list(chunks, where):
+    if (chunks.dtype != torch.int32 or chunks.dim() != 2 or chunks.shape[1] != 4
+            or not chunks.is_contiguous() or chunks.device != where):
+        raise native.KernelError("chunks: int32 [C, 4], on the queries' GPU")
+    if chunks.shape[0] > 512:
+        raise native.KernelError("at most 512 chunks")
+
+
+def check_weighing(weights: torch.Tensor, page_table: torch.Tensor, kcache: torch.Tensor, qh: int, *,
+                   rows: int = 0, chunks: Optional[torch.Tensor] = None) -> None:
+    """Raises where :func:`attention_weighed` of ``rows`` rows, or :func:`prefill_weights` of
+    ``chunks``, would refuse a layer's ``weights``: for a program that runs layer by layer and has to know
+    before the first."""
+    _cuda(page_table, kcache)
+    kvh, d = kcache.shape[2:]
+    _weight_sums(weights, None, page_table.shape[0], kvh, page_table.device)
+    rep = qh // kvh if qh % kvh == 0 else 0
+    if (d not in (64, 128, 256) or not 0 < rep <= 16
+            or (rows and not (rep in (1, 2, 4, 8) or (rep == 5 and d == 128)))):
+        raise native.KernelError(f"{qh} query heads on {kvh} KV heads of {d} channels")
+    if chunks is not None:
+        _chunk_list(chunks, page_table.device)
+    _current(page_table.device)
+
+
 def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: torch.Tensor,
                       row_pos: torch.Tensor, page_table: torch.Tensor, kcache: torch.Tensor,
                       vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor,
@@ -367,11 +392,7 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
         raise native.KernelError(f"{qh} query heads of {d} on {kvh} KV heads of {dim} channels")
     if q.data_ptr() % 16 or kcache.data_ptr() % 16:
         raise native.KernelError("q and kcache on 16-byte boundaries")
-    if (chunks.dtype != torch.int32 or chunks.dim() != 2 or chunks.shape[1] != 4
-            or not chunks.is_contiguous() or chunks.device != where):
-        raise native.KernelError("chunks: int32 [C, 4], on the queries' GPU")
-    if chunks.shape[0] > 512:
-        raise native.KernelError("at most 512 chunks")
+    _chunk_list(chunks, where)
     live = n if total_rows is None else total_rows
     if not 0 <= live <= n or max_q_len < 0:
         raise native.KernelError(f"{live} rows of {n}, chunks of {max_q_len}")

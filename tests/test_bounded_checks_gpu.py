@@ -87,3 +87,44 @@ def test_a_prompt_that_raises_takes_nothing(make, monkeypatch):  # noqa: F811
         monkeypatch.undo()
         after = state(pool)
         assert same(after, before, cache=False) and len(pool._free) == 3
+
+
+def recurrent(runner):
+    pools = getattr(runner, "_gdn", None)
+    return [] if pools is None else [pools["state"].clone(), pools["hist"].clone()]
+
+
+@pytest.mark.parametrize("preset", ["tiny", "tiny-hybrid"])
+def test_a_packet_that_is_refused_changes_nothing(make, preset):  # noqa: F811
+    """Whatever layer would refuse it: keys, values, recurrent states and weights stay as they were."""
+    from orinfer_b200.models.runner import Packet
+    from orinfer_b200.ops import native
+    pool = make(preset)
+    runner, i32, w = pool.runner, pool._i32, pool.weights
+    slot = pool.add(text(100, runner.cfg.vocab))
+    layers = list(w)
+    last = lambda t: layers[:-1] + [t]
+    single = lambda **kw: Packet(i32([1]), i32([slot]), i32([100]), pool.table, 1, 101,
+                                 **{"weights": w, **kw})
+    chunk = lambda **kw: Packet(i32([1] * 5), i32([slot] * 5), i32(list(range(100, 105))), pool.table, 5, 105,
+                                chunks=i32([[0, 5, 100, slot]]), max_q_len=5, max_chunk_kv=105,
+                                **{"weights": w, **kw})
+    bad = [single(weights=layers[:-1]), chunk(weights=layers[:-1]), single(weights=[]),
+           single(attend_pos=i32([100])), single(weigh_chunks=i32([[0, 1, 100, slot]])),
+           chunk(weigh_chunks=i32([[0, 1, 100, slot]] * 513)),
+           chunk(weigh_chunks=i32([[0, 1, 100, slot]]).long()),
+           single(rope_pos=i32([100]).long()), single(rope_pos=i32([[100]])), single(rope_pos=i32([])),
+           chunk(rope_pos=i32([100] * 4)), single(rope_pos=i32([100]).cpu()),
+           single(rope_pos=i32([100]), mrope=i32([[100]] * 3))]
+    for make_packet in (single, chunk):
+        bad += [make_packet(weights=last(t)) for t in (
+            layers[-1].double(), layers[-1][:-1], layers[-1][:, :-1], layers[-1].transpose(1, 2),
+            layers[-1][..., ::2], layers[-1].cpu())]
+    before = state(pool), recurrent(runner)
+    for packet in bad:
+        with pytest.raises((ValueError, native.KernelError)):
+            runner.logits(packet)
+        assert same(state(pool), before[0])
+        assert all(torch.equal(a, b) for a, b in zip(recurrent(runner), before[1]))
+    runner.logits(single())
+    assert not same(state(pool), before[0])

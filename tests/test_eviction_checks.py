@@ -30,3 +30,20 @@ def test_the_entries_refuse_a_cache_off_16_bytes(kc, vc):
                                  None) == -1
     assert lib.orinfer_attention_weighed(at, None, at, at, at, 1, 1, *cache, at, at, 1, at, at, 256, 128,
                                          at, 256, 128, 128, 1, 2, 1, 128, 1, 128, at, 0, None) == -1
+
+
+def test_the_plain_runner_refuses_before_anything_changes():
+    from orinfer_b200.config import PRESETS
+    from orinfer_b200.models.runner import KVPool, Packet
+    from orinfer_b200.models.torch_runner import TorchRunner
+    from orinfer_b200.models.weights import random_model
+    cfg = PRESETS["tiny-hybrid"]
+    assert not cfg.is_full_attention(0)
+    runner = TorchRunner(random_model(cfg, seed=1), KVPool.allocate(cfg, 3, "cpu"), max_rows=8)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)
+    for kw in (dict(weights=torch.zeros(1, 2, cfg.kv_heads, 128)),
+               dict(rope_pos=i32([7]), mrope=i32([[7]] * 3))):
+        with pytest.raises(ValueError):
+            runner.logits(Packet(i32([5]), i32([0]), i32([0]), i32([[1]]), 1, 1, **kw))
+        assert not hasattr(runner, "_gdn_pool")
+        assert all(bool((t == 0).all()) for t in (*runner.kv.k, *runner.kv.v))
