@@ -7,6 +7,7 @@ The matching fp32 PyTorch statement of each op lives in ``orinfer_b200.ref.ops_r
 
 from __future__ import annotations
 
+from bisect import bisect_left
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -214,19 +215,56 @@ def _current(where):
         raise native.KernelError(f"tensors on {where}, which is not the current device")
 
 
+def _sums_apart(shape, at, a, b, from_, c, d):
+    """The sums that are written, lines of keys from address ``at`` on, ``a`` and ``b`` elements apart, share
+    no place with one another, nor with the weights that are read (``from_``, ``c``, ``d``), unless they are
+    those."""
+    n, heads, keys = shape
+    if 0 in shape:
+        return True
+    places = lambda at, a, b: sorted(at + 4 * (i * a + j * b) for i in range(n) for j in range(heads))
+    mine = None
+    if not ((heads < 2 or b >= keys) and (n < 2 or a >= (heads - 1) * b + keys)
+            or (n < 2 or a >= keys) and (heads < 2 or b >= (n - 1) * a + keys)):
+        mine = places(at, a, b)
+        if any(y - x < 4 * keys for x, y in zip(mine, mine[1:])):
+            return False
+    end = lambda at, a, b: at + 4 * ((n - 1) * a + (heads - 1) * b + keys)
+    if (at, a, b) == (from_, c, d) or at >= end(from_, c, d) or from_ >= end(at, a, b):
+        return True
+    theirs = places(from_, c, d)                     # one within the other: line by line
+    for x in mine or places(at, a, b):
+        i = bisect_left(theirs, x)
+        if (i < len(theirs) and theirs[i] - x < 4 * keys) or (i > 0 and x - theirs[i - 1] < 4 * keys):
+            return False
+    return True
+
+
 def _weight_sums(weights, weights_out, lead, kvh, where):
-    """(capacity, strides of weights, the sums that are written and their strides)."""
-    shape = weights.shape
-    out = weights if weights_out is None else weights_out
-    if (weights.dtype != torch.float32 or len(shape) != 3 or shape[1] != kvh or weights.stride(2) != 1
-            or weights.device != where
-            or (out is not weights and (out.dtype != torch.float32 or out.shape != shape
-                                        or out.stride(2) != 1 or out.device != where))):
-        raise native.KernelError("weights: fp32 [slots, KV heads, keys] on the cache's GPU, keys in one "
-                                 "piece, weights_out like them")
-    if shape[0] < lead:
+    """(keys of a line, (address and strides of the weights), (those of the sums that are written))."""
+    shape, strides = weights.shape, weights.stride()
+    if (weights.dtype != torch.float32 or len(shape) != 3 or shape[1] != kvh or strides[2] != 1
+            or weights.device != where):
+        raise native.KernelError("weights: fp32 [slots, KV heads, keys] on the cache's GPU, keys in one piece")
+    n, _, keys = shape
+    if n < lead:
         raise native.KernelError("weights: a slot for each row of the page table")
-    return shape[2], out
+    slot, head, _ = strides
+    read = (weights.data_ptr(), slot, head)
+    if weights_out is None:
+        if head >= keys and slot >= head * kvh:      # (what `_sums_apart` would see first)
+            return keys, read, read
+        written = read
+    else:
+        strides = weights_out.stride()
+        if (weights_out.dtype != torch.float32 or weights_out.shape != shape or strides[2] != 1
+                or weights_out.device != where):
+            raise native.KernelError("weights_out: like weights")
+        written = (weights_out.data_ptr(), *strides[:2])
+    if not _sums_apart(shape, *written, *read):
+        raise native.KernelError("weights: every sum in a place of its own (no expanded tensor), weights_out "
+                                 "apart from weights or the same")
+    return keys, read, written
 
 
 def _cached(where, page_table, codes, scales, *more):
@@ -285,7 +323,8 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     ``weights`` fp32 [slots, KV heads, keys], slots as in the page table, gets for every key that a row
     sees the softmax weights of the row's query heads of that KV head.  Rows of one request are added
     in their order; what no row sees stays.  With ``weights_out`` the sums of seen keys go there
-    instead, so that a step may be taken back.  Rows see at most ``max_kv_len`` keys (by default as
+    instead, so that a step may be taken back.  Every sum that is written has a place of its own, and
+    ``weights_out`` shares none with ``weights``, unless it is that.  Rows see at most ``max_kv_len`` keys (by default as
     many as the page table has), which the call's ``scratch`` is made for (4 bytes for each score); keys
     beyond that, or beyond what ``weights`` holds, get none and set the status word.  A row whose request
     is no row of the page table sees nothing, adds nothing and sets it too, and so does a page that the
@@ -312,7 +351,7 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
                 or t.device != where):
             raise native.KernelError("row_req, row_pos: int32, one for each row, on the queries' GPU")
     lead, width = page_table.shape
-    capacity, sums = _weight_sums(weights, weights_out, lead, kvh, where)
+    capacity, read, written = _weight_sums(weights, weights_out, lead, kvh, where)
     _current(where)
     keys = width * 128 if max_kv_len is None else max(1, min(int(max_kv_len), width * 128))
     if not 1 <= splits <= 32 or keys == 0:
@@ -329,14 +368,11 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     elif (scratch.numel() * scratch.element_size() < need or not scratch.is_contiguous()
           or scratch.device != where):
         raise native.KernelError(f"scratch: {need} bytes")
-    slot_stride, head_stride, _ = weights.stride()
-    sums_slot_stride, sums_head_stride, _ = sums.stride()
     check(lib.orinfer_attention_weighed(
         q.data_ptr(), ptr(gate), row_req.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(), lead,
         width, k_at, v_at, kscale.data_ptr(), vscale.data_ptr(), pages,
-        out.data_ptr(), weights.data_ptr(), slot_stride, head_stride, sums.data_ptr(), sums_slot_stride,
-        sums_head_stride, capacity, live, qh, kvh, d, splits, keys, scratch.data_ptr(), max_kv_len or 0,
-        stream()), "attention_weighed")
+        out.data_ptr(), *read, *written, capacity, live, qh, kvh, d, splits, keys, scratch.data_ptr(),
+        max_kv_len or 0, stream()), "attention_weighed")
     count_launches(2 if live else 0)
     return out
 
@@ -378,7 +414,7 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     chunk's entry names the rows that count.  ``weights`` fp32 [slots, KV heads, keys], slots as in
     the page table, gets for every key that a row sees the softmax weights of the query heads of that
     KV head, summed over the rows; chunks of one request are added in their order.  With
-    ``weights_out`` the sums of seen keys go there instead.  A chunk that reaches beyond
+    ``weights_out`` the sums of seen keys go there instead (places as for :func:`attention_weighed`).  A chunk that reaches beyond
     ``max_kv_len`` keys (by default as many as the page table and ``weights`` have), of more than
     ``max_q_len`` rows or of rows that are not there is left out and sets the status word.  The
     workspace has 2 KB for 128 of ``max_kv_len`` keys of each chunk and KV head."""
@@ -397,7 +433,7 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     if not 0 <= live <= n or max_q_len < 0:
         raise native.KernelError(f"{live} rows of {n}, chunks of {max_q_len}")
     lead, width = page_table.shape
-    capacity, sums = _weight_sums(weights, weights_out, lead, kvh, where)
+    capacity, read, written = _weight_sums(weights, weights_out, lead, kvh, where)
     _current(where)
     limit = min(width * 128, capacity)
     if max_kv_len is not None:
@@ -408,13 +444,10 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     lib = native.lib()
     work = torch.empty(lib.orinfer_prefill_weights_work_bytes(
         chunks.shape[0], max_q_len, kvh, qh // kvh, limit) // 4, dtype=torch.float32, device=where)
-    slot_stride, head_stride, _ = weights.stride()
-    sums_slot_stride, sums_head_stride, _ = sums.stride()
     check(lib.orinfer_prefill_weights(
         q.data_ptr(), chunks.data_ptr(), chunks.shape[0], max_q_len, live, page_table.data_ptr(), lead,
-        width, kcache.data_ptr(), kscale.data_ptr(), pages, weights.data_ptr(), slot_stride, head_stride,
-        sums.data_ptr(), sums_slot_stride, sums_head_stride, limit, qh, kvh, d, work.data_ptr(),
-        stream()), "prefill_weights")
+        width, kcache.data_ptr(), kscale.data_ptr(), pages, *read, *written, limit, qh, kvh, d,
+        work.data_ptr(), stream()), "prefill_weights")
     count_launches(4)
 
 
@@ -777,7 +810,7 @@ def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: t
 
     Returns (table, lens, refs, status int32 [1]); ``out`` may be the inputs.  The slots' rows of
     ``weights`` move along, with zeros behind, in place or to ``weights_out`` (which gets a copy of those
-    that are named and not cut, and nothing of the others).  A slot that is named again is cut once.
+    that are named and not cut, and nothing of the others, and overlaps ``weights`` not in part).  A slot that is named again is cut once.
     Status 1: not enough free pages, 2: a slot that does not exist, a length that its row does not hold or a page
     that nobody holds; nothing is changed then.  The workspace has 8 bytes for each kept key of a layer
     and KV head."""
@@ -791,6 +824,8 @@ def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: t
         if (w.dtype != torch.float32 or w.shape != shape or not w.is_contiguous()
                 or w.device != cache.device):
             raise native.KernelError("weights: contiguous fp32 on the cache's GPU, weights_out like them")
+    if sums is not weights and 0 < abs(sums.data_ptr() - weights.data_ptr()) < 4 * weights.numel():
+        raise native.KernelError("weights_out: apart from weights or the same")
     if len(shape) != 4 or shape[:3] != (cache.layers, total, cache.kvh) or shape[3] < width * 128:
         raise native.KernelError("weights: [layers, slots, KV heads, keys], a place for each key of a "
                                  "table row")

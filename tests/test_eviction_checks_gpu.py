@@ -128,3 +128,28 @@ def test_the_bound_of_keys_is_met_to_the_key(dev, most, over):
     assert status() == (0, 0)
     assert torch.equal(weights[..., :most], want[..., :most])
     assert torch.equal(weights[..., most:], base[..., most:])
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (1, 0, 2)])
+def test_weights_and_sums_in_turns_in_one_buffer(dev, order):
+    """Two buffers line by line in one, and weights that are read from one line for all slots."""
+    from orinfer_b200.ops import functional as F
+    args = batch(dev, [200, 700, 90], 4, 2, 128)
+    keys = args[4].shape[1] * 128
+    shape = [3, 2, keys]
+    inv = [order.index(i) for i in range(3)]
+    base = torch.zeros(*[shape[i] for i in order[:2]], 2, keys, device=dev)
+    one, two = (base[:, :, i].permute(*inv) for i in (0, 1))
+    one.copy_(sums(dev, args))
+    before = one.clone()
+    want = before.clone()
+    F.attention_weighed(*args, want, splits=2)
+    F.attention_weighed(*args, one, splits=2, weights_out=two)
+    seen = torch.arange(keys, device=dev)[None, :] <= args[3][:, None]
+    seen = seen[:, None].expand(shape)
+    assert torch.equal(one, before) and torch.equal(two[seen], want[seen])
+    line = sums(dev, args)[:1, :1].expand(shape)
+    want = line.clone()
+    F.attention_weighed(*args, want, splits=2)
+    F.attention_weighed(*args, line, splits=2, weights_out=two)
+    assert torch.equal(two[seen], want[seen])
