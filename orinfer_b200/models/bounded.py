@@ -47,6 +47,7 @@ class BoundedRequests(SlotPages):
     # ---------------------------------------------------------------- cache
     def cut(self, slots: Sequence[int]) -> None:
         """Cuts those of the slots down that have more than ``keep`` tokens."""
+        self._known(slots)
         slots = [s for s in slots if self._len[s] > self.keep]
         # all at once, or one after the other where free pages are too few for that
         if not self._cut(slots) and not all(self._cut([s]) for s in slots):
@@ -176,7 +177,7 @@ class BoundedRequests(SlotPages):
 
     def _known(self, slots: Sequence[int]) -> None:
         for s in slots:
-            if s not in self.text:
+            if s not in self._len:
                 raise ValueError(f"slot {s} holds no request")
 
     def _give_up(self, slot: int) -> None:

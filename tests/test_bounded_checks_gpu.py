@@ -128,3 +128,15 @@ def test_a_packet_that_is_refused_changes_nothing(make, preset):  # noqa: F811
         assert all(torch.equal(a, b) for a, b in zip(recurrent(runner), before[1]))
     runner.logits(single())
     assert not same(state(pool), before[0])
+
+
+def test_a_cut_of_slots_without_a_request_is_refused(make):  # noqa: F811
+    pool = make("tiny")
+    slot = pool.add(text(300, pool.runner.cfg.vocab))
+    before = state(pool)
+    for slots in ([slot, pool._free[0]], [9], [-1]):
+        with pytest.raises(ValueError, match="holds no request"):
+            pool.cut(slots)
+        assert same(state(pool), before)
+    pool.cut([slot, slot])
+    assert pool._len == {slot: 150} and pool.lens[slot] == 150 and pool.held == 2
