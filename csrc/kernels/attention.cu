@@ -79,8 +79,8 @@ struct Weighed {
   int pages = 0;                   // of the cache
   // A row of a request that is not there sees nothing: its index leads out of the table and, in
   // attn_weigh_kernel, which reports it, out of the caller's sums.  Nor does a row see keys behind its row of
-  // the table, and for a page that does not exist page 0 is read, both reported there too.  (125 rows of up
-  // to 640 keys: 45.6 us without these checks, 46.5 with them, 47.4 where the limit is of the row's keys, not
+  // the table, and for a page that does not exist page 0 is read, both reported there too.  (125 rows of
+  // 323 to 640 keys: 45.6 us without these checks, 46.5 with them, 47.4 where the limit is of the row's keys, not
   // of a part's last one, and the two indices are not asked for together.)
   __device__ __forceinline__ bool there(int req) const { return req >= 0 && req < slots; }
   __device__ __forceinline__ int limit(int req) const { return there(req) ? most : 0; }
@@ -1218,10 +1218,10 @@ __global__ void attn_merge_kernel(
 // here, 4 rep bytes a key beside the 2 D and more of its key and value, mostly within L2; making them
 // again would read the keys again.  The kernel is a chain of loads that wait for each other, so what can
 // be asked for at once is: the scores and factors of the CTA's own row before it is known whether an
-// earlier row's CTA has them, a request's factors four at a time.  32 / 8 heads of 128: 128 rows of 640
-// keys 9 us behind the row kernel's 37 (a CTA per head, too many to start early: the call 49.2 us, now
-// 45.4), 6 rows of 24000 keys 12 behind 53 (17 with one CTA for all of a row's outputs), 36 rows of 3000
-// keys, four a request, 16 / 2 heads of 256: 15 behind 35 (21 without asking for factors together).
+// earlier row's CTA has them, a request's factors four at a time.  32 / 8 heads of 128: 125 rows of 323 to
+// 640 keys 9.6 us behind the row kernel's 37 (a CTA per head, too many to start early, cost the call 3.8 us
+// more), 6 rows of 13751 to 24000 keys 12 behind 53 (17 with one CTA for all of a row's outputs), 36 rows of
+// 1584 to 3000 keys, four a request, 16 / 2 heads of 256: 15 behind 35 (21 without asking for factors together).
 constexpr int WEIGH_THREADS = 256, WEIGH_KEYS = 4 * WEIGH_THREADS;
 template <int D, int REP>
 __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_kernel(

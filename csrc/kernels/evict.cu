@@ -13,12 +13,17 @@
 // to a list with their weights.  In the second a CTA fills a fresh page of a layer and head from the list.
 //
 // The second is bound by memory: 2 (D + D / 32) bytes of a kept key's key and value read and as many
-// written, pieces of D bytes in no order of pages.  36 layers of 8 heads of 128: eleven requests of 1450 keys
-// cut to 1000 292 us, 5.6 TB/s (a CTA that walks its keys itself: 390); two of 12000 to 2000 117 (199);
-// seventeen of 2100 to 1100, 12 layers of 2 heads of 256: 62.  The first, 46, 35 and 13 us of these, is a
+// written, pieces of D bytes in no order of pages.  36 layers of 8 heads of 128: eleven requests of 1006 to
+// 1450 keys cut to 1000 292 us, 5.6 TB/s (a CTA that walks its keys itself: 390); two of 8292 and 12000 to
+// 2000 117 (199); seventeen of 1137 to 2100 to 1100, 12 layers of 2 heads of 256: 62.  The first, 46, 35 and
+// 13 us of these, is a
 // chain of passes over weights that lie in L2.  It took 47, 40 and 13 before its walk was shortened; then
 // with weights in shared memory 53, 49 and 13, since fewer CTAs are at work beside each other, and with 512
 // threads 70 and 50 of the first two.
+//
+// The pool is gone through by the one CTA that does the bookkeeping, 256 pages at a time, all of it: a small call
+// (one request of 700 keys, 2 heads of 64) takes 34 us cold in a pool of 64 or 1500 pages, 50 in one of 15000
+// and 103 in one of 60000.
 #include <type_traits>
 
 #include "api.h"

@@ -24,9 +24,9 @@
 // weights: a unit of 128 x 128 is 16384 exponentials, 1024 cycles of the SM's unit for them, and 512 of
 // products; it takes about 1560 cycles in sums_kernel (that unit 72 % busy, half of the issue slots used)
 // and 1850 in stats_kernel (60 %), which has other scales for each column and the reference beside.
-// 32 / 8 heads of 128, 4096 rows: 131 and 111 us, join and add 5 and 7; 64 rows behind 20000 keys of six
-// requests: 98 and 126; two times 777 rows behind 3000 keys, 16 / 2 heads of 256 (twice the products'
-// columns to a weight): 66 and 53.
+// 32 / 8 heads of 128, 4096 rows: 131 and 111 us, join and add 5 and 7; six requests of 37 to 64 rows behind
+// 11459 to 20000 keys: 98 and 126; two of 777 and 537 rows behind 3000 and 2073 keys, 16 / 2 heads of 256
+// (twice the products' columns to a weight): 66 and 53.
 //
 // On the way, both kernels at 4096 rows: eight warps for weights 181 and 163; sixteen 169 and 156;
 // products of 128 rows in sums 160 and 151; lse joined once (by every CTA for each unit it cost 35 us of
@@ -1170,7 +1170,9 @@ static int launch(const __half* q, const Geometry& g, const int8_t* kc, const __
   const int ctas = ctas_for(b.units);
   launch_early(stats_kernel<D>, dim3(ctas), THREADS, L::A_TOTAL, stream, tq, tk, g, ks, lse, row_span,
                runtime_status_ptr());
-  // slices by the parts that a tile has where all of the CTAs are at work on as many tiles as there can be
+  // Slices by the parts that a tile has where all of the CTAs are at work on as many tiles as there can be.
+  // us of the join in 1, 4 and 8 of them: 296 parts 30, 11.7, 9.5; 148 18.5, 9.2, 7.9; 74 8.1, 6.5, 6.1; 37
+  // 7.9, 6.4, 5.9; 18 6.1, 5.1, 5.9; 6 6.2, 6.9, 7.9; 4 4.5, 5.1, 5.8; less than one (4096 rows) 5, 12.5, 21.7.
   const long long most = PARTS * static_cast<long long>(ctas) / b.row_tiles;
   const dim3 join(TILE, most >= 64 ? JOIN_SLICES : most >= 16 ? 4 : 1);
   launch_early(join_kernel<L::NT>, dim3((g.longest + g.per - 1) / g.per, g.kvh, g.n_chunks), join, 0, stream,

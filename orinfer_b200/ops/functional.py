@@ -414,10 +414,11 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     chunk's entry names the rows that count.  ``weights`` fp32 [slots, KV heads, keys], slots as in
     the page table, gets for every key that a row sees the softmax weights of the query heads of that
     KV head, summed over the rows; chunks of one request are added in their order.  With
-    ``weights_out`` the sums of seen keys go there instead (places as for :func:`attention_weighed`).  A chunk that reaches beyond
-    ``max_kv_len`` keys (by default as many as the page table and ``weights`` have), of more than
-    ``max_q_len`` rows or of rows that are not there is left out and sets the status word.  The
-    workspace has 2 KB for 128 of ``max_kv_len`` keys of each chunk and KV head."""
+    ``weights_out`` the sums of seen keys go there instead (places as for :func:`attention_weighed`).
+    A chunk that reaches beyond ``max_kv_len`` keys (by default as many as the page table and ``weights``
+    have), of more than ``max_q_len`` rows, of rows or of a slot that are not there is left out and sets the
+    status word, and so does a page that the cache does not have, for which page 0 is read.  The workspace has, of each chunk and KV head as if all were the largest, 2 KB for 128 of ``max_kv_len``
+    keys and 2.5 KB for 128 pairs of a row, of ``max_q_len``, and a query head of the KV head's."""
     _cuda(q)                                         # (and the others are on its GPU)
     where = q.device
     if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
