@@ -38,6 +38,7 @@ from ..config import PAGE_TOKENS, GraphMode, LoadOptions, ModelConfig, Phase as 
 from ..core import sampling as S
 from ..core.prefix import RadixPrefixCache
 from ..utils import trace
+from ..utils.capture import recording
 from ..models.runner import KVPool, Packet
 from ..models.weights import ModelWeights
 from .pages import OutOfPages, PagePool
@@ -1343,7 +1344,7 @@ class Engine:
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
         before = native.launches()
-        with torch.cuda.graph(graph):                        # records only: nothing runs here
+        with recording(graph):                               # records only: nothing runs here
             tok, lg = self.runner.greedy(st, need_logits=need)
         entry = dict(graph=graph, packet=st, tok=tok, lg=lg, launches=native.launches() - before)
         native.count_launches(-entry["launches"])            # recorded, not launched
@@ -1379,7 +1380,7 @@ class Engine:
                 graph = torch.cuda.CUDAGraph()
                 from ..ops import native
                 before = native.launches()
-                with torch.cuda.graph(graph):            # records only: nothing runs here
+                with recording(graph):                   # records only: nothing runs here
                     body()
                 g.graph = graph
                 g.local = getattr(self.runner, "_last_local", None)

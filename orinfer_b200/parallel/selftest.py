@@ -19,6 +19,8 @@ import torch
 import torch.distributed as dist
 import torch.multiprocessing as mp
 
+from ..utils.capture import recording
+
 PREFLIGHT_S = 30.0
 MIN_FREE = 512 << 20
 
@@ -75,7 +77,7 @@ def run_checks(rank: int, world: int, dev) -> List[str]:
         dist.all_reduce(buf)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        with recording(g):
             dist.all_reduce(buf)
         for v in (2.0, 5.0):
             buf.fill_(v)
