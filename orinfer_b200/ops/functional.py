@@ -241,7 +241,7 @@ def _sums_apart(shape, at, a, b, from_, c, d):
 
 
 def _weight_sums(weights, weights_out, lead, kvh, where):
-    """(keys of a line, (address and strides of the weights), (those of the sums that are written))."""
+    """(keys of a line, address and strides of the weights, those of the sums that are written)."""
     shape, strides = weights.shape, weights.stride()
     if (weights.dtype != torch.float32 or len(shape) != 3 or shape[1] != kvh or strides[2] != 1
             or weights.device != where):
@@ -250,21 +250,25 @@ def _weight_sums(weights, weights_out, lead, kvh, where):
     if n < lead:
         raise native.KernelError("weights: a slot for each row of the page table")
     slot, head, _ = strides
-    read = (weights.data_ptr(), slot, head)
+    at = weights.data_ptr()
+    plain = head >= keys and slot >= head * kvh      # (what `_sums_apart` finds, seen at once)
     if weights_out is None:
-        if head >= keys and slot >= head * kvh:      # (what `_sums_apart` would see first)
-            return keys, read, read
-        written = read
+        sums = at
+        if plain:
+            return keys, at, slot, head, at, slot, head
     else:
-        strides = weights_out.stride()
+        sums, strides = weights_out.data_ptr(), weights_out.stride()
         if (weights_out.dtype != torch.float32 or weights_out.shape != shape or strides[2] != 1
                 or weights_out.device != where):
             raise native.KernelError("weights_out: like weights")
-        written = (weights_out.data_ptr(), *strides[:2])
-    if not _sums_apart(shape, *written, *read):
+        if plain and strides[0] == slot and strides[1] == head and (
+                sums == at or not -4 * n * slot < sums - at < 4 * n * slot):
+            return keys, at, slot, head, sums, slot, head
+    sums_slot, sums_head, _ = strides
+    if not _sums_apart(shape, sums, sums_slot, sums_head, at, slot, head):
         raise native.KernelError("weights: every sum in a place of its own (no expanded tensor), weights_out "
                                  "apart from weights or the same")
-    return keys, read, written
+    return keys, at, slot, head, sums, sums_slot, sums_head
 
 
 def _cached(where, page_table, codes, scales, *more):
@@ -351,7 +355,8 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
                 or t.device != where):
             raise native.KernelError("row_req, row_pos: int32, one for each row, on the queries' GPU")
     lead, width = page_table.shape
-    capacity, read, written = _weight_sums(weights, weights_out, lead, kvh, where)
+    capacity, at, slot, head, sums, sums_slot, sums_head = _weight_sums(weights, weights_out, lead, kvh,
+                                                                        where)
     _current(where)
     keys = width * 128 if max_kv_len is None else max(1, min(int(max_kv_len), width * 128))
     if not 1 <= splits <= 32 or keys == 0:
@@ -371,8 +376,8 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     check(lib.orinfer_attention_weighed(
         q.data_ptr(), ptr(gate), row_req.data_ptr(), row_pos.data_ptr(), page_table.data_ptr(), lead,
         width, k_at, v_at, kscale.data_ptr(), vscale.data_ptr(), pages,
-        out.data_ptr(), *read, *written, capacity, live, qh, kvh, d, splits, keys, scratch.data_ptr(),
-        max_kv_len or 0, stream()), "attention_weighed")
+        out.data_ptr(), at, slot, head, sums, sums_slot, sums_head, capacity, live, qh, kvh, d, splits,
+        keys, scratch.data_ptr(), max_kv_len or 0, stream()), "attention_weighed")
     count_launches(2 if live else 0)
     return out
 
@@ -434,7 +439,8 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
     if not 0 <= live <= n or max_q_len < 0:
         raise native.KernelError(f"{live} rows of {n}, chunks of {max_q_len}")
     lead, width = page_table.shape
-    capacity, read, written = _weight_sums(weights, weights_out, lead, kvh, where)
+    capacity, at, slot, head, sums, sums_slot, sums_head = _weight_sums(weights, weights_out, lead, kvh,
+                                                                        where)
     _current(where)
     limit = min(width * 128, capacity)
     if max_kv_len is not None:
@@ -447,8 +453,8 @@ def prefill_weights(q: torch.Tensor, chunks: torch.Tensor, max_q_len: int,
         chunks.shape[0], max_q_len, kvh, qh // kvh, limit) // 4, dtype=torch.float32, device=where)
     check(lib.orinfer_prefill_weights(
         q.data_ptr(), chunks.data_ptr(), chunks.shape[0], max_q_len, live, page_table.data_ptr(), lead,
-        width, kcache.data_ptr(), kscale.data_ptr(), pages, *read, *written, limit, qh, kvh, d,
-        work.data_ptr(), stream()), "prefill_weights")
+        width, kcache.data_ptr(), kscale.data_ptr(), pages, at, slot, head, sums, sums_slot, sums_head,
+        limit, qh, kvh, d, work.data_ptr(), stream()), "prefill_weights")
     count_launches(4)
 
 
@@ -825,7 +831,8 @@ def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: t
         if (w.dtype != torch.float32 or w.shape != shape or not w.is_contiguous()
                 or w.device != cache.device):
             raise native.KernelError("weights: contiguous fp32 on the cache's GPU, weights_out like them")
-    if sums is not weights and 0 < abs(sums.data_ptr() - weights.data_ptr()) < 4 * weights.numel():
+    at, to = weights.data_ptr(), sums.data_ptr()
+    if at != to and abs(to - at) < 4 * weights.numel():
         raise native.KernelError("weights_out: apart from weights or the same")
     if len(shape) != 4 or shape[:3] != (cache.layers, total, cache.kvh) or shape[3] < width * 128:
         raise native.KernelError("weights: [layers, slots, KV heads, keys], a place for each key of a "
@@ -839,7 +846,7 @@ def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: t
     check(native.lib().orinfer_evict_keys(
         cache.bases.data_ptr(), cache.layers, cache.kvh, cache.head_dim, cache.pages,
         table.data_ptr(), t.data_ptr(), lens.data_ptr(), l.data_ptr(), refs.data_ptr(), r.data_ptr(),
-        slots.data_ptr(), n, total, width, keep, first, recent, weights.data_ptr(), sums.data_ptr(),
+        slots.data_ptr(), n, total, width, keep, first, recent, at, to,
         weights.shape[3], work.data_ptr(), status.data_ptr(), stream()), "evict_keys")
     count_launches(2)
     return t, l, r, status
