@@ -192,8 +192,8 @@ int orinfer_attention(const __half* q, const __half* gate, const int* row_req, c
 // The same, and sums[request][KV head][key] = weights[...] + the weight that every key got from the
 // call's rows (FP32, strides in elements, `capacity` keys of a request; sums may be weights).  keys: what
 // any row sees at most, which the scores' place is made for; scratch: 16-byte aligned.  slots: rows of
-// the page table; a row of a request that is none of them gives zeros, adds nothing and is reported, as are
-// keys behind a table row, which nobody sees, and pages from num_pages on, for which page 0 is read.
+// the page table; a row of a request that is none of them, or of a position behind its table row, gives zeros,
+// adds nothing and is reported, and so are pages from num_pages on, for which page 0 is read.
 size_t orinfer_attention_weighed_scratch_bytes(int rows, int qh, int head_dim, int splits, int keys);
 int orinfer_attention_weighed(const __half* q, const __half* gate, const int* row_req,
                               const int* row_pos, const int* page_table, int slots, int max_pages,

@@ -6,6 +6,8 @@
 // partial (max, sum, out) records that a second kernel merges.  Replaces the decode
 // configurations of causal_attention_int8 and merge_attention_int8
 // (kernels/cuda/model/attention_rows.py:61-276,280-400).
+#include <climits>
+
 #include "api.h"
 #include "attention_shared.h"
 #include "common.cuh"
@@ -75,15 +77,16 @@ struct Weighed {
   int keys = 0;                    // places of a row's scores, a multiple of 4; what it sees beyond is not written
   int counted = 0;                 // of them those whose keys get their weights
   int slots = 0;                   // rows of the page table, and of the sums
-  int most = 0;                    // keys that a row of the table has a place for
+  int most = 0;                    // keys that such a row has a place for
   int pages = 0;                   // of the cache
-  // A row of a request that is not there sees nothing: its index leads out of the table and, in
-  // attn_weigh_kernel, which reports it, out of the caller's sums.  Nor does a row see keys behind its row of
-  // the table, and for a page that does not exist page 0 is read, both reported there too.  (125 rows of
-  // 323 to 640 keys: 45.6 us without these checks, 46.5 with them, 47.4 where the limit is of the row's keys, not
-  // of a part's last one, and the two indices are not asked for together.)
-  __device__ __forceinline__ bool there(int req) const { return req >= 0 && req < slots; }
-  __device__ __forceinline__ int limit(int req) const { return there(req) ? most : 0; }
+  // A row whose request or position the page table has no place for sees nothing: its index leads out of the
+  // table and, in attn_weigh_kernel, which reports it, out of the caller's sums.  For a page that does not
+  // exist page 0 is read (reported there too).  125 rows of 323 to 640 keys: 45.6 us without these checks,
+  // 46.5 with them, 47.4 where a row's keys, not a part's, are cut short and its two indices are not asked
+  // for together.
+  __device__ __forceinline__ bool there(int req, int pos) const {
+    return req >= 0 && req < slots && pos < most;
+  }
   __device__ __forceinline__ bool has(int page) const { return page >= 0 && page < pages; }
   __device__ __forceinline__ int page(int id) const { return has(id) ? id : 0; }
 };
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(
   const int per = (kv_len - first + splits - 1) / splits;
   const int k_lo = first + split * per;
   int k_hi = min(kv_len, k_lo + per);
-  if (WEIGH) k_hi = min(k_hi, weighed.limit(req));
+  if (WEIGH && !weighed.there(req, pos)) k_hi = INT_MIN;
   const int* pages = page_table + static_cast<size_t>(req) * max_pages;
   const float qscale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
 
@@ -686,7 +689,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, DigitTile<D>::MIN_CTAS) attn_
   const int per = (kv_len - first + splits - 1) / splits;
   const int k_lo = first + split * per;
   int k_hi = min(kv_len, k_lo + per);
-  if (WEIGH) k_hi = min(k_hi, weighed.limit(req));
+  if (WEIGH && !weighed.there(req, pos)) k_hi = INT_MIN;
   const int* pages = page_table + static_cast<size_t>(req) * max_pages;
 
   extern __shared__ unsigned char digits_smem[];
@@ -1226,9 +1229,8 @@ constexpr int WEIGH_THREADS = 256, WEIGH_KEYS = 4 * WEIGH_THREADS;
 template <int D, int REP>
 __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_kernel(
     const Weighed weighed, const int* row_req, const int* row_pos, const int* page_table, int max_pages,
-    const float* weights,
-    long long slot_stride, long long head_stride, float* sums, long long sums_slot_stride,
-    long long sums_head_stride, int capacity, int rows, int qh, int splits, int heads, int merges,
+    const float* weights, long long slot_stride, long long head_stride, float* sums,
+    long long sums_slot_stride, long long sums_head_stride, int capacity, int rows, int qh, int splits, int heads, int merges,
     const float* scratch, const __half* gate, __half* __restrict__ out, int* status) {
   __shared__ int2 s_rows[WEIGH_THREADS];           // rows of the request, in their order, and their keys
   __shared__ int s_count[WEIGH_THREADS / 32];
@@ -1259,7 +1261,7 @@ __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_ker
   float2 own_part = make_float2(-INFINITY, 0.f);
   if (warp < REP) own_part = part(row, h_lo * REP + warp);
   if (pos < 0) return;
-  const bool there = weighed.there(req);
+  const bool there = weighed.there(req, pos);
   if (tid == 0 && z == 0 && blockIdx.y == 0 && (!there || pos >= limit))
     report_status(status, STATUS_BAD_INDEX, there ? 0x60 : 0x61);
   float4 v[REP];                                   // scores of a row
@@ -1289,7 +1291,7 @@ __global__ void __launch_bounds__(WEIGH_THREADS, REP > 4 ? 3 : 4) attn_weigh_ker
       other_pos = other < rows ? row_pos[other] : -1;
       other_req = other < rows ? row_req[other] : 0;
     }
-    const bool same = other_pos >= 0 && other_req == req;
+    const bool same = other_req == req && other_pos >= 0 && other_pos < weighed.most;
     const unsigned votes = __ballot_sync(0xffffffffu, same);
     if (lane == 0) s_count[warp] = __popc(votes);
     if (__syncthreads_or(same && other < row)) {   // an earlier row's CTA has them
@@ -1540,7 +1542,8 @@ extern "C" int orinfer_attention_weighed(
     const __half* q, const __half* gate, const int* row_req, const int* row_pos,
     const int* page_table, int slots, int max_pages, const int8_t* kc, const int8_t* vc,
     const __half* ks, const __half* vs, int num_pages, __half* out, const float* weights,
-    long long slot_stride, long long head_stride, float* sums, long long sums_slot_stride, long long sums_head_stride,
+    long long slot_stride, long long head_stride, float* sums, long long sums_slot_stride,
+    long long sums_head_stride,
     int capacity, int rows, int qh, int kvh, int head_dim, int splits, int keys, float* scratch,
     int context, cudaStream_t stream) {
   if (rows <= 0) return 0;
@@ -1585,7 +1588,8 @@ extern "C" int orinfer_attention_weighed(
 #define CASE(DD, REP)                                                                               \
   if (head_dim == DD && rep == REP)                                                                 \
     launch_early(attn_weigh_kernel<DD, REP>, grid, WEIGH_THREADS, 0, stream, w, row_req, row_pos,   \
-                 page_table, max_pages, weights, slot_stride, head_stride, sums, sums_slot_stride, sums_head_stride,       \
+                 page_table, max_pages, weights, slot_stride, head_stride, sums, sums_slot_stride,  \
+                 sums_head_stride,                                                                  \
                  capacity, rows, qh, splits, per_cta, merges, static_cast<const float*>(parts),     \
                  gate, out, runtime_status_ptr());
   CASE(64, 1) CASE(64, 2) CASE(64, 4) CASE(64, 8)

@@ -328,11 +328,12 @@ def attention_weighed(q: torch.Tensor, gate: Optional[torch.Tensor], row_req: to
     sees the softmax weights of the row's query heads of that KV head.  Rows of one request are added
     in their order; what no row sees stays.  With ``weights_out`` the sums of seen keys go there
     instead, so that a step may be taken back.  Every sum that is written has a place of its own, and
-    ``weights_out`` shares none with ``weights``, unless it is that.  Rows see at most ``max_kv_len`` keys (by default as
-    many as the page table has), which the call's ``scratch`` is made for (4 bytes for each score); keys
+    ``weights_out`` shares none with ``weights``, unless it is that.  Rows see at most ``max_kv_len`` keys
+    (by default as many as the page table has), which the call's ``scratch`` is made for (4 bytes for each score); keys
     beyond that, or beyond what ``weights`` holds, get none and set the status word.  A row whose request
-    is no row of the page table sees nothing, adds nothing and sets it too, and so does a page that the
-    cache does not have, for which page 0 is read; a row at position -1 is padding."""
+    is no row of the page table, or whose position lies behind that row, sees nothing, adds nothing and sets it
+    too, and so does a page that the cache does not have, for which page 0 is read; a row at position -1 is
+    padding."""
     _cuda(q)                                         # (and the others are on its GPU)
     where = q.device
     if q.dim() != 3 or q.dtype != torch.float16 or not q.is_contiguous():
@@ -817,7 +818,8 @@ def evict_keys(cache: KeyCache, table: torch.Tensor, lens: torch.Tensor, refs: t
 
     Returns (table, lens, refs, status int32 [1]); ``out`` may be the inputs.  The slots' rows of
     ``weights`` move along, with zeros behind, in place or to ``weights_out`` (which gets a copy of those
-    that are named and not cut, and nothing of the others, and overlaps ``weights`` not in part).  A slot that is named again is cut once.
+    that are named and not cut, and nothing of the others, and overlaps ``weights`` not in part).  A slot
+    that is named again is cut once.
     Status 1: not enough free pages, 2: a slot that does not exist, a length that its row does not hold or a page
     that nobody holds; nothing is changed then.  The workspace has 8 bytes for each kept key of a layer
     and KV head."""
